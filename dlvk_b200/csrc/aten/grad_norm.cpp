@@ -1,0 +1,171 @@
+// ATen-level wrapper of the gradient-list kernels (grad_norm.cu): the norm of
+// a list of tensors and clipping by it.
+#include <ATen/ATen.h>
+#include <ATen/cuda/CUDAContext.h>
+#include <c10/cuda/CUDAGuard.h>
+
+#include <algorithm>
+#include <cmath>
+
+#include "dlvk/aten_ops.h"
+#include "dlvk/kernels.h"
+
+namespace dlvk {
+namespace aten {
+namespace {
+
+// Byte range of one tensor.  Column slices of one matrix have ranges that
+// interleave without sharing an element: `row` bytes of every `pitch` bytes.
+struct Extent {
+  uintptr_t lo, hi;
+  int64_t row, pitch;  // pitch 0: one dense run
+  int64_t index;
+};
+
+Extent extent_of(const at::Tensor& t, int64_t index) {
+  const int64_t es = t.element_size();
+  Extent e{reinterpret_cast<uintptr_t>(t.data_ptr()), 0, 0, 0, index};
+  int64_t span = 1, run = 1;
+  bool rows = false, regular = true;
+  // dimensions from the innermost stride outwards
+  std::vector<std::pair<int64_t, int64_t>> dims;  // stride, size
+  for (int64_t d = 0; d < t.dim(); ++d)
+    if (t.size(d) > 1) dims.emplace_back(t.stride(d), t.size(d));
+  std::sort(dims.begin(), dims.end());
+  for (const auto& [st, sz] : dims) {
+    span += st * (sz - 1);
+    if (!rows && st == run) {
+      run *= sz;
+    } else if (!rows) {
+      rows = true;
+      e.row = run * es;
+      e.pitch = st * es;
+      run = st * sz;  // the next dimension continues the rows when its stride is this
+    } else {
+      regular = regular && st == run;
+      run = st * sz;
+    }
+  }
+  e.hi = e.lo + (uintptr_t)(span * es);
+  if (!rows || !regular) e.row = e.pitch = 0;
+  return e;
+}
+
+bool share_bytes(const Extent& a, const Extent& b) {
+  if (a.hi <= b.lo || b.hi <= a.lo) return false;
+  if (a.pitch == 0 || a.pitch != b.pitch) return true;
+  const int64_t p = a.pitch, d = (int64_t)((b.lo - a.lo) % (uintptr_t)p);  // a.lo <= b.lo (sorted)
+  return d < a.row || d + b.row > p;
+}
+
+// Each written tensor must share no byte with another tensor of the call
+// (its own input apart).
+void check_disjoint(std::vector<Extent>& ex, const char* what) {
+  std::sort(ex.begin(), ex.end(), [](const Extent& a, const Extent& b) { return a.lo < b.lo; });
+  std::vector<Extent> open;
+  for (const Extent& e : ex) {
+    open.erase(std::remove_if(open.begin(), open.end(), [&](const Extent& o) { return o.hi <= e.lo; }), open.end());
+    for (const Extent& o : open)
+      TORCH_CHECK(!share_bytes(o, e), "dlvk.", what, ": tensors ", std::min(o.index, e.index), " and ",
+                  std::max(o.index, e.index), " of the call share memory, which is written");
+    open.push_back(e);
+  }
+}
+
+bool dense_alike(const at::Tensor& a, const at::Tensor& b) {
+  if (a.is_contiguous() && b.is_contiguous()) return true;
+  return a.is_non_overlapping_and_dense() && a.strides() == b.strides();
+}
+
+StridedItem strided_item(const at::Tensor& in, const at::Tensor& out, uint8_t kind, const char* what) {
+  StridedItem s{};
+  s.in = in.data_ptr();
+  s.out = out.data_ptr();
+  s.n = in.numel();
+  s.kind = kind;
+  int64_t size[4], si[4], so[4];
+  int nd = 0;
+  for (int64_t d = 0; d < in.dim(); ++d) {
+    if (in.size(d) == 1) continue;
+    if (nd > 0 && si[nd - 1] == in.stride(d) * in.size(d) && so[nd - 1] == out.stride(d) * out.size(d)) {
+      size[nd - 1] *= in.size(d);  // continues the dimension before it
+      si[nd - 1] = in.stride(d);
+      so[nd - 1] = out.stride(d);
+      continue;
+    }
+    TORCH_CHECK(nd < 4, "dlvk.", what, ": a tensor with more than four separate strides; pass a contiguous one");
+    size[nd] = in.size(d);
+    si[nd] = in.stride(d);
+    so[nd] = out.stride(d);
+    ++nd;
+  }
+  for (int d = 0; d < 4; ++d) s.size[d] = 1;
+  for (int d = 0; d < nd; ++d) {
+    s.size[4 - nd + d] = size[d];
+    s.in_stride[4 - nd + d] = si[d];
+    s.out_stride[4 - nd + d] = so[d];
+  }
+  return s;
+}
+
+at::Tensor run(const std::vector<at::Tensor>& grads, const std::vector<at::Tensor>* outs, bool scale, double max_norm,
+               const char* what) {
+  TORCH_CHECK(!grads.empty(), "dlvk.", what, ": an empty list has no device; the norm of no tensors is 0");
+  TORCH_CHECK(outs == nullptr || outs->size() == grads.size(), "dlvk.", what, ": ", grads.size(), " gradients and ",
+              outs ? outs->size() : 0, " outputs");
+  check_cuda(grads[0], "gradients");
+  const at::Device dev = grads[0].device();
+  std::vector<DenseItem> dense;
+  std::vector<StridedItem> strided;
+  std::vector<Extent> ex;
+  dense.reserve(grads.size());
+  if (scale) ex.reserve(grads.size() * (outs ? 2 : 1));
+  for (size_t i = 0; i < grads.size(); ++i) {
+    const at::Tensor& t = grads[i];
+    const at::Tensor& o = outs ? (*outs)[i] : t;
+    TORCH_CHECK(t.device() == dev && o.device() == dev, "dlvk.", what, ": tensor ", i, " is on another device than ",
+                dev);
+    const auto ti = t.scalar_type(), to = o.scalar_type();
+    TORCH_CHECK((ti == at::kFloat || ti == at::kBFloat16) && (to == at::kFloat || to == at::kBFloat16), "dlvk.", what,
+                ": tensor ", i, " is neither fp32 nor bf16");
+    TORCH_CHECK(t.layout() == at::kStrided && o.layout() == at::kStrided, "dlvk.", what, ": tensor ", i, " is not strided");
+    if (outs) TORCH_CHECK(t.sizes() == o.sizes(), "dlvk.", what, ": gradient ", i, " is ", t.sizes(), ", its output ", o.sizes());
+    if (t.numel() == 0) continue;
+    const bool same = t.data_ptr() == o.data_ptr();
+    if (outs && same)
+      TORCH_CHECK(ti == to && t.strides() == o.strides(), "dlvk.", what, ": output ", i,
+                  " starts where its gradient does but is laid out otherwise");
+    const uint8_t kind = (uint8_t)((ti == at::kBFloat16 ? 1 : 0) | (to == at::kBFloat16 ? 2 : 0));
+    if (dense_alike(t, o)) dense.push_back({t.data_ptr(), o.data_ptr(), t.numel(), kind});
+    else strided.push_back(strided_item(t, o, kind, what));
+    if (scale) {
+      for (int64_t d = 0; d < o.dim(); ++d)
+        TORCH_CHECK(o.size(d) == 1 || o.stride(d) != 0, "dlvk.", what, ": output ", i,
+                    " repeats its elements (an expanded tensor)");
+      ex.push_back(extent_of(o, (int64_t)i));
+      if (!same) ex.push_back(extent_of(t, (int64_t)i));
+    }
+  }
+  if (scale) check_disjoint(ex, what);
+  c10::cuda::CUDAGuard g(dev);
+  auto opt = grads[0].options();
+  at::Tensor norm = at::empty({}, opt.dtype(at::kFloat));
+  const int parts = grad_norm_parts(dense.data(), (int)dense.size(), strided.data(), (int)strided.size());
+  at::Tensor partial = at::empty({std::max(parts, 1)}, opt.dtype(at::kDouble));
+  grad_norm(dense.data(), (int)dense.size(), strided.data(), (int)strided.size(), scale, (float)max_norm,
+            norm.data_ptr<float>(), partial.data_ptr<double>(), stream());
+  return norm;
+}
+
+}  // namespace
+
+at::Tensor global_norm_op(const std::vector<at::Tensor>& grads) { return run(grads, nullptr, false, 0.0, "global_norm"); }
+
+at::Tensor clip_global_norm_op(const std::vector<at::Tensor>& grads, double max_norm,
+                               const c10::optional<std::vector<at::Tensor>>& out) {
+  TORCH_CHECK(max_norm > 0.0, "dlvk.clip_global_norm: max_norm must be above 0, got ", max_norm);
+  return run(grads, out.has_value() ? &*out : nullptr, true, max_norm, "clip_global_norm");
+}
+
+}  // namespace aten
+}  // namespace dlvk

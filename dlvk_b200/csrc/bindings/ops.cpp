@@ -108,6 +108,8 @@ void register_ops(py::module& m) {
   }, py::arg("w"), py::arg("g"), py::arg("l1"), py::arg("l2"), py::arg("ll1"), py::arg("ll2"),
      py::arg("loss_out") = py::none(),
      py::arg("gscale") = py::none());
+  m.def("global_norm", &global_norm_op, py::arg("grads"));
+  m.def("clip_global_norm", &clip_global_norm_op, py::arg("grads"), py::arg("max_norm"), py::arg("out") = py::none());
   m.def("grad_stats_scratch_floats", &grad_stats_scratch_floats);
   m.def("scaler_update", &scaler_update_op);
   m.def("optim_hyper_bytes", &optim_hyper_bytes);

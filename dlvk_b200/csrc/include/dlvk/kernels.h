@@ -187,6 +187,32 @@ void regularize(const float* w, void* g, DType g_dt, int64_t n, float l1, float 
 void scaler_update(float* scale, int* good_steps, const int* found_inf, float growth, float backoff, int interval,
                    float smin, float smax, float* inv_scale, cudaStream_t s);
 
+// ---- global gradient norm over a list of tensors (grad_norm.cu) -------------
+constexpr int NORM_LIST_MAX = 1024;  // dense tensors per launch
+// kind: bit 0 = bf16 input, bit 1 = bf16 output (else fp32).
+struct DenseItem {
+  const void* in;
+  void* out;
+  int64_t n;
+  uint8_t kind;
+};
+// A tensor with gaps or of another element order than its output: sizes and
+// strides (elements) over at most four dimensions, leading ones of size 1.
+struct StridedItem {
+  const void* in;
+  void* out;
+  int64_t n;
+  int64_t size[4], in_stride[4], out_stride[4];
+  uint8_t kind;
+};
+// Number of fp64 partial sums that grad_norm() writes for these items.
+int grad_norm_parts(const DenseItem* dense, int n_dense, const StridedItem* strided, int n_strided);
+// *norm = sqrt(sum of squares of all inputs); with `scale` also
+// out = in * min(1, max_norm / (norm + 1e-6)), or 1 for a norm that is not
+// finite.  `in == out` scales in place; otherwise inputs and outputs are disjoint.
+void grad_norm(const DenseItem* dense, int n_dense, const StridedItem* strided, int n_strided, bool scale,
+               float max_norm, float* norm, double* partial, cudaStream_t s);
+
 // ---- convolution / pooling ---------------------------------------------------
 struct ConvDesc {
   int N, Cin, H, W, Cout, KH, KW, stride, pad, Ho, Wo;

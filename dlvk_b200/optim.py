@@ -331,6 +331,21 @@ class RMSprop(Optimizer):
         super().__init__(learning_rate, epsilon=epsilon, alpha=alpha, weight_decay=weight_decay)
 
 
+def _tensor_list(tensors: Iterable) -> List[torch.Tensor]:
+    from .tensor import Tensor as FacadeTensor
+
+    return [t.data if isinstance(t, FacadeTensor) else t for t in tensors]
+
+
+def _cpu_norm(grads: List[torch.Tensor]) -> torch.Tensor:
+    total = torch.zeros((), dtype=torch.float64)
+    for g in grads:
+        if g.device.type != "cpu" or g.dtype not in (torch.float32, torch.bfloat16):
+            raise ValueError(f"gradient list: {g.dtype} on {g.device} among fp32 / bf16 tensors on the CPU")
+        total = total + g.detach().double().square().sum()
+    return total.sqrt()
+
+
 class GradientClipping:
     """Global-norm utilities (src/optimizers/optimizers.cpp:9-55)."""
 
@@ -352,6 +367,42 @@ class GradientClipping:
                 else:
                     g.mul_(s)
         return norm
+
+    @staticmethod
+    def global_norm(grads: Iterable[torch.Tensor]) -> torch.Tensor:
+        """sqrt(sum of squares over all tensors) as an fp32 scalar on their
+        device, without a host read (csrc/kernels/grad_norm.cu).  fp32 and
+        bf16 tensors of any strides may be mixed; a tensor given twice counts
+        twice, no tensors at all have norm 0."""
+        grads = _tensor_list(grads)
+        if grads and grads[0].is_cuda:
+            return K.N().global_norm(grads)
+        return _cpu_norm(grads).float()
+
+    @staticmethod
+    def clip_global_norm(grads: Iterable[torch.Tensor], max_norm: float,
+                         out: Optional[Iterable[torch.Tensor]] = None) -> torch.Tensor:
+        """Scale all tensors by min(1, max_norm / (norm + 1e-6)) and return
+        their norm before that, as global_norm does.  In place, or into the
+        tensors `out` (same shapes, fp32 or bf16 whatever the gradients are:
+        for instance the views of a flat optimizer buffer).  A norm that is
+        not finite scales by 1, so that the caller, who gets that norm, can
+        skip the step.  Tensors that are written must not share memory."""
+        grads = _tensor_list(grads)
+        outs = None if out is None else _tensor_list(out)
+        if not float(max_norm) > 0.0:
+            raise ValueError(f"clip_global_norm: max_norm must be above 0, got {max_norm}")
+        if outs is not None and len(outs) != len(grads):
+            raise ValueError(f"clip_global_norm: {len(grads)} gradients and {len(outs)} outputs")
+        if grads and grads[0].is_cuda:
+            return K.N().clip_global_norm(grads, float(max_norm), outs)
+        norm = _cpu_norm(grads)
+        coef = min(1.0, float(max_norm) / (float(norm) + 1e-6)) if math.isfinite(norm) else 1.0
+        for g, o in zip(grads, grads if outs is None else outs):
+            if g.shape != o.shape:
+                raise ValueError(f"clip_global_norm: a gradient is {tuple(g.shape)}, its output {tuple(o.shape)}")
+            o.copy_(g.float() * coef)
+        return norm.float()
 
     @staticmethod
     def clip_grad_value(grads: List[torch.Tensor], clip_value: float) -> None:
