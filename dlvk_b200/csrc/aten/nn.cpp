@@ -405,6 +405,74 @@ void embedding_bwd_op(const at::Tensor& ids, const at::Tensor& dy, const at::Ten
                 dtable.size(0), (int)dtable.size(1), stream());
 }
 
+namespace {
+void check_ids(const at::Tensor& ids, const at::Tensor& other, const char* what) {
+  TORCH_CHECK(ids.scalar_type() == at::kInt || ids.scalar_type() == at::kLong, "dlvk.", what,
+              ": ids are int32 or int64, got ", ids.scalar_type());
+  TORCH_CHECK(ids.device() == other.device(), "dlvk.", what, ": ids on ", ids.device(), ", the values on ",
+              other.device());
+}
+void check_f32_bf16(const at::Tensor& t, const char* what, const char* name) {
+  TORCH_CHECK(t.scalar_type() == at::kFloat || t.scalar_type() == at::kBFloat16, "dlvk.", what, ": ", name,
+              " is fp32 or bf16, got ", t.scalar_type());
+}
+}  // namespace
+
+at::Tensor embedding_lookup_op(const at::Tensor& ids, const at::Tensor& table, double scale) {
+  check_cuda(table, "table");
+  check_ids(ids, table, "embedding_lookup");
+  check_f32_bf16(table, "embedding_lookup", "table");
+  TORCH_CHECK(table.dim() == 2, "dlvk.embedding_lookup: table [V, D], got ", table.sizes());
+  c10::cuda::CUDAGuard g(table.device());
+  const int64_t V = table.size(0), D = table.size(1);
+  TORCH_CHECK(D < (1LL << 31) - 4096, "dlvk.embedding_lookup: rows of ", D, " elements");
+  auto idc = ids.contiguous();
+  auto tc = (D <= 1 || table.stride(1) == 1) ? table : table.contiguous();
+  std::vector<int64_t> shp(ids.sizes().begin(), ids.sizes().end());
+  shp.push_back(D);
+  auto out = at::empty(shp, table.options());
+  embedding_lookup(to_dtype(tc), idc.scalar_type() == at::kLong, idc.data_ptr(), tc.data_ptr(), out.data_ptr(),
+                   idc.numel(), V, (int)D, tc.stride(0), (float)scale, stream());
+  return out;
+}
+
+at::Tensor embedding_grad_op(const at::Tensor& ids, const at::Tensor& dy, int64_t num_embeddings, double scale,
+                             int64_t padding_idx, c10::optional<at::Tensor> out, bool accumulate) {
+  check_cuda(dy, "dy");
+  check_ids(ids, dy, "embedding_grad");
+  check_f32_bf16(dy, "embedding_grad", "dy");
+  const int64_t n = ids.numel(), V = num_embeddings;
+  TORCH_CHECK(dy.dim() == ids.dim() + 1 && dy.sizes().slice(0, ids.dim()) == ids.sizes(),
+              "dlvk.embedding_grad: ids ", ids.sizes(), " need dy of those sizes and a last one, got ", dy.sizes());
+  const int64_t D = dy.size(-1);
+  TORCH_CHECK(V >= 0, "dlvk.embedding_grad: num_embeddings ", V);
+  TORCH_CHECK(D < (1LL << 31) - 4096, "dlvk.embedding_grad: rows of ", D, " elements");
+  TORCH_CHECK(n < (1LL << 31) - 1024 && V < (1LL << 31) - 1024, "dlvk.embedding_grad: more than 2^31 tokens or words");
+  c10::cuda::CUDAGuard g(dy.device());
+  at::Tensor dt;
+  if (out.has_value()) {
+    dt = *out;
+    TORCH_CHECK(dt.scalar_type() == at::kFloat && dt.is_contiguous() && dt.dim() == 2 && dt.size(0) == V &&
+                    dt.size(1) == D && dt.device() == dy.device(),
+                "dlvk.embedding_grad: out must be a contiguous fp32 [", V, ", ", D, "] tensor on dy's device");
+  } else {
+    TORCH_CHECK(!accumulate, "dlvk.embedding_grad: accumulate needs out");
+    dt = at::empty({V, D}, dy.options().dtype(at::kFloat));
+  }
+  auto idc = ids.contiguous();
+  auto dyc = dy.dim() == 2 && (D <= 1 || dy.stride(1) == 1) ? dy : dy.contiguous();
+  auto io = dy.options().dtype(at::kInt);
+  const int64_t pf = embedding_grad_part_floats(n, (int)D);
+  // one allocation: part first (16-byte aligned), then the three integer arrays
+  auto ws = at::empty({pf + V + 1 + 2 * n}, io);
+  int* base = ws.data_ptr<int>();
+  int* start = base + pf;
+  embedding_grad(to_dtype(dyc), idc.scalar_type() == at::kLong, idc.data_ptr(), dyc.data_ptr(),
+                 dyc.dim() == 2 ? dyc.stride(0) : D, dt.data_ptr<float>(), n, V, (int)D, (float)scale, padding_idx,
+                 accumulate, start, start + V + 1, start + V + 1 + n, reinterpret_cast<float*>(base), stream());
+  return dt;
+}
+
 std::vector<at::Tensor> quantize_rows_op(const at::Tensor& x) {
   check_cuda(x, "x");
   c10::cuda::CUDAGuard g(x.device());

@@ -253,6 +253,10 @@ void register_nn(py::module& m) {
         py::arg("step") = 0, py::arg("step_t") = py::none());
   m.def("embedding_fwd", &embedding_fwd_op);
   m.def("embedding_bwd", &embedding_bwd_op);
+  m.def("embedding_lookup", &embedding_lookup_op, py::arg("ids"), py::arg("table"), py::arg("scale") = 1.0);
+  m.def("embedding_grad", &embedding_grad_op, py::arg("ids"), py::arg("dy"), py::arg("num_embeddings"),
+        py::arg("scale") = 1.0, py::arg("padding_idx") = -1, py::arg("out") = py::none(),
+        py::arg("accumulate") = false);
 }
 
 }  // namespace bind

@@ -68,6 +68,8 @@ std::vector<at::Tensor> layernorm_fwd_op(const at::Tensor& x, c10::optional<at::
 at::Tensor layernorm_bwd_op(const at::Tensor& x, c10::optional<at::Tensor> gamma, const at::Tensor& mean, const at::Tensor& rstd, const at::Tensor& dy, c10::optional<at::Tensor> dgamma, c10::optional<at::Tensor> dbeta, bool accumulate, c10::optional<at::Tensor> dres, c10::optional<at::Tensor> dres_colsum = c10::nullopt, bool dres_colsum_accumulate = false);
 at::Tensor dropout_op(const at::Tensor& x, double p, int64_t stream_id, int64_t seed, int64_t step, c10::optional<at::Tensor> step_t);
 at::Tensor embedding_fwd_op(const at::Tensor& ids, const at::Tensor& table);
+at::Tensor embedding_lookup_op(const at::Tensor& ids, const at::Tensor& table, double scale);
+at::Tensor embedding_grad_op(const at::Tensor& ids, const at::Tensor& dy, int64_t num_embeddings, double scale, int64_t padding_idx, c10::optional<at::Tensor> out, bool accumulate);
 void embedding_bwd_op(const at::Tensor& ids, const at::Tensor& dy, const at::Tensor& dtable);
 std::vector<at::Tensor> quantize_rows_op(const at::Tensor& x);
 at::Tensor gemm_i8_op(const at::Tensor& qa, const at::Tensor& qbt, const at::Tensor& sa, const at::Tensor& sb, c10::optional<at::Tensor> bias, int64_t act, c10::optional<at::ScalarType> out_dtype, int64_t force_path);

@@ -290,6 +290,20 @@ void embedding_fwd(DType dt, const int32_t* ids, const void* table, void* out, i
 void embedding_bwd(DType dt, const int32_t* ids, const void* dy, float* dtable, int64_t n, int64_t V, int D,
                    cudaStream_t s);
 
+// ---- embedding lookup with scale, gradient by sorted tokens (embedding.cu) ---
+// ids: int32 or int64 (ids64).  Rows of table / dy are ld elements apart.
+// out[i, :] = scale * table[ids[i], :], zeros for ids outside [0, V).
+void embedding_lookup(DType dt, bool ids64, const void* ids, const void* table, void* out, int64_t n, int64_t V, int D,
+                      int64_t ld, float scale, cudaStream_t s);
+// dtable[v, :] (fp32 [V, D]) = (or, accumulate, +=) scale * sum of dy[i, :] over
+// ids[i] == v, in a fixed order; ids outside [0, V) and `padding` (-1: none)
+// have no gradient.  Scratch: start V + 1 ints, order and word n ints each,
+// part embedding_grad_part_floats(n, D) floats.
+int64_t embedding_grad_part_floats(int64_t n, int D);
+void embedding_grad(DType dt, bool ids64, const void* ids, const void* dy, int64_t ld, float* dtable, int64_t n,
+                    int64_t V, int D, float scale, int64_t padding, bool accumulate, int* start, int* order, int* word,
+                    float* part, cudaStream_t s);
+
 // ---- device error word -------------------------------------------------------
 uint32_t* device_error_word();     // per current device, zero-initialised
 uint32_t read_device_error(bool clear);

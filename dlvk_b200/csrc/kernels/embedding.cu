@@ -1,0 +1,421 @@
+// Embedding lookup with scaling, and its gradient by sorted tokens.
+//
+//   y[i, :]  = scale * table[id_i, :]              (zeros for ids outside [0, V))
+//   dT[v, :] = scale * sum over i with id_i = v, in ascending i, of dy[i, :]
+//
+// The reference's lookup (shaders/embedding_lookup.comp:24-55) has no scale
+// and returns no gradient.  Here the gradient has no floating-point atomics:
+// the tokens are sorted by word, stably, and every row of dT is written once
+// by a sum whose order depends on nothing but the ids, so two runs agree bit
+// for bit, and rows without a token get their zeros in the same pass.
+//
+// What bounds them: the lookup moves n D elements in and out; the gradient
+// reads dy once and writes V D fp32 once (8192 x 1024 bf16 tokens over 32000
+// words: 17 MB in, 131 MB out, 22.6 us at the measured copy rate), so the
+// sort has to be short.
+#include <algorithm>
+
+#include "dlvk/common.h"
+#include "dlvk/kernels.h"
+
+namespace dlvk {
+namespace {
+
+constexpr int SORT_THREADS = 1024;
+constexpr int SORT_WARPS = SORT_THREADS / 32;
+constexpr int SORT_WORDS = 1024;  // most words of one block: a count per warp and word in shared memory
+constexpr int RED_THREADS = 256;
+
+template <typename T> struct Vec { static constexpr int N = 16 / (int)sizeof(T); };
+
+template <typename T, int VEC>
+__device__ __forceinline__ void load_vec(const T* p, float* v) {
+  if constexpr (VEC == 1) {
+    v[0] = to_f32(*p);
+  } else {
+    const uint4 u = *reinterpret_cast<const uint4*>(p);
+    const T* e = reinterpret_cast<const T*>(&u);
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) v[k] = to_f32(e[k]);
+  }
+}
+
+// ---------------------------------------------------------------- lookup
+// A warp copies a row; a lane has up to four 16-byte loads in flight.
+template <typename T, typename ID, int VEC>
+__global__ void __launch_bounds__(256) lookup_kernel(const ID* __restrict__ ids, const T* __restrict__ table,
+                                                     T* __restrict__ out, int64_t n, int64_t V, int D, int64_t ld,
+                                                     float scale) {
+  const int64_t i = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  if (i >= n) return;
+  const int lane = threadIdx.x & 31;
+  const int64_t id = (int64_t)ids[i];
+  const bool ok = id >= 0 && id < V;
+  const T* src = table + (ok ? id : 0) * ld;
+  T* dst = out + i * D;
+  for (int c = lane * VEC; c < D; c += 4 * 32 * VEC) {
+    float v[4][VEC];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) v[k][j] = 0.f;
+      if (ok && c + k * 32 * VEC < D) load_vec<T, VEC>(src + c + k * 32 * VEC, v[k]);
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int at = c + k * 32 * VEC;
+      if (at >= D) break;
+      if constexpr (VEC == 1) {
+        dst[at] = from_f32<T>(v[k][0] * scale);
+      } else {
+        uint4 u;
+        T* e = reinterpret_cast<T*>(&u);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) e[j] = from_f32<T>(v[k][j] * scale);
+        *reinterpret_cast<uint4*>(dst + at) = u;
+      }
+    }
+  }
+}
+
+// ---------------------------------------------------------------- sort
+// Stable sort of the tokens by word in one launch, without a word between
+// blocks.  Block b owns the words [b R, (b + 1) R) and reads all ids twice:
+// once to count its own words (per warp: warp w has the w-th part of the ids)
+// and the tokens of smaller words, which is where its part of the order
+// begins; once more to place its tokens.  A token's place is its word's
+// start + the counts of earlier warps + its rank among the warp's tokens so
+// far, so equal words stay in ascending position.  Every block reading all
+// ids costs 148 x 4 n bytes from L2 (8192 tokens: 5 MB), far less than the
+// passes over memory of a radix sort of so few keys.
+//   start[v], v in [0, V]: first place of word v; order[place]: the token.
+template <typename ID>
+__global__ void __launch_bounds__(SORT_THREADS) sort_tokens_kernel(const ID* __restrict__ ids, int n, int V, int R,
+                                                                   int padding, int* __restrict__ start,
+                                                                   int* __restrict__ order, int* __restrict__ word) {
+  extern __shared__ int cnt[];  // [SORT_WARPS][R]
+  __shared__ int warp_part[SORT_WARPS];
+  __shared__ int before_sm;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int v0 = blockIdx.x * R, v1 = min(V, v0 + R);
+  for (int i = tid; i < SORT_WARPS * R; i += SORT_THREADS) cnt[i] = 0;
+  if (tid == 0) before_sm = 0;
+  __syncthreads();
+
+  const int per = ((n + SORT_THREADS - 1) / SORT_THREADS) * 32;  // ids of a warp, whole groups of 32
+  const int lo = min((int64_t)n, (int64_t)warp * per), hi = min((int64_t)n, (int64_t)(warp + 1) * per);
+  int* mine = cnt + warp * R;
+  int before = 0;
+  for (int base = lo; base < hi; base += 256) {
+    int id[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const int i = base + k * 32 + lane;
+      const int64_t raw = i < hi ? (int64_t)ids[i] : -1;
+      id[k] = (raw >= 0 && raw < V && raw != padding) ? (int)raw : -1;
+    }
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      before += id[k] >= 0 && id[k] < v0;
+      if (id[k] >= v0 && id[k] < v1) atomicAdd(&mine[id[k] - v0], 1);
+    }
+  }
+  before = __reduce_add_sync(0xffffffffu, before);
+  if (lane == 0 && before) atomicAdd(&before_sm, before);
+  __syncthreads();
+
+  // thread r: word v0 + r.  Its total over the warps, then the block's scan.
+  int total = 0;
+  if (tid < R)
+    for (int w = 0; w < SORT_WARPS; ++w) total += cnt[w * R + tid];
+  int incl = total;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int t = __shfl_up_sync(0xffffffffu, incl, o);
+    if (lane >= o) incl += t;
+  }
+  if (lane == 31) warp_part[warp] = incl;
+  __syncthreads();
+  if (warp == 0) {
+    int p = warp_part[lane];
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int t = __shfl_up_sync(0xffffffffu, p, o);
+      if (lane >= o) p += t;
+    }
+    warp_part[lane] = p;
+  }
+  __syncthreads();
+  int at = before_sm + incl - total + (warp > 0 ? warp_part[warp - 1] : 0);
+  if (tid < R && v0 + tid < V) {
+    start[v0 + tid] = at;
+    if (v0 + tid == V - 1) start[V] = at + total;
+  }
+  if (tid < R)
+    for (int w = 0; w < SORT_WARPS; ++w) {
+      const int c = cnt[w * R + tid];
+      cnt[w * R + tid] = at;
+      at += c;
+    }
+  __syncthreads();
+
+  for (int base = lo; base < hi; base += 256) {
+    int id[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const int i = base + k * 32 + lane;
+      const int64_t raw = i < hi ? (int64_t)ids[i] : -1;
+      id[k] = (raw >= v0 && raw < v1 && raw != padding) ? (int)raw : -1;
+    }
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const bool hit = id[k] >= 0;
+      if (!__any_sync(0xffffffffu, hit)) continue;
+      const unsigned peers = __match_any_sync(0xffffffffu, id[k]);
+      if (hit) {
+        const int place = mine[id[k] - v0] + __popc(peers & ((1u << lane) - 1u));
+        order[place] = base + k * 32 + lane;
+        word[place] = id[k];
+      }
+      __syncwarp();
+      if (hit && lane == __ffs(peers) - 1) mine[id[k] - v0] += __popc(peers);
+      __syncwarp();
+    }
+  }
+}
+
+// ---------------------------------------------------------------- sums
+template <int VEC>
+__device__ __forceinline__ void put_row(float* dst, const float* acc, float scale, bool accumulate) {
+  if constexpr (VEC == 1) {
+    *dst = accumulate ? fmaf(acc[0], scale, *dst) : acc[0] * scale;
+  } else {
+#pragma unroll
+    for (int k = 0; k < VEC; k += 4) {
+      float4 o = accumulate ? *reinterpret_cast<const float4*>(dst + k) : make_float4(0.f, 0.f, 0.f, 0.f);
+      o.x = fmaf(acc[k], scale, o.x);
+      o.y = fmaf(acc[k + 1], scale, o.y);
+      o.z = fmaf(acc[k + 2], scale, o.z);
+      o.w = fmaf(acc[k + 3], scale, o.w);
+      *reinterpret_cast<float4*>(dst + k) = o;
+    }
+  }
+}
+
+// The first blocks sum chunks of C consecutive places of the order; the rest
+// write the zero rows.  TX threads go across a row, 256 / TX chunks to a
+// block.  A word whose tokens lie in one chunk is finished here; what a chunk
+// has of a word that continues from the chunk before goes to part[2 chunk],
+// of one that begins here and continues to part[2 chunk + 1] (join_kernel).
+template <typename T, int VEC>
+__global__ void __launch_bounds__(RED_THREADS) sum_chunks_kernel(
+    const T* __restrict__ dy, int64_t ld, const int* __restrict__ start, const int* __restrict__ order,
+    const int* __restrict__ word, float* __restrict__ dtable, float* __restrict__ part, int V, int D, int C, int TX,
+    int chunk_blocks, float scale, int accumulate) {
+  if ((int)blockIdx.x >= chunk_blocks) {
+    // zero rows: a warp takes every warps-th word
+    const int warps = (gridDim.x - chunk_blocks) * (RED_THREADS / 32), lane = threadIdx.x & 31;
+    for (int v = (blockIdx.x - chunk_blocks) * (RED_THREADS / 32) + (threadIdx.x >> 5); v < V; v += warps) {
+      if (start[v] != start[v + 1]) continue;
+      float* row = dtable + (int64_t)v * D;
+      if constexpr (VEC > 1) {
+        for (int c = lane * 4; c < D; c += 128) *reinterpret_cast<float4*>(row + c) = make_float4(0.f, 0.f, 0.f, 0.f);
+      } else {
+        for (int c = lane; c < D; c += 32) row[c] = 0.f;
+      }
+    }
+    return;
+  }
+  const int tx = threadIdx.x % TX;
+  const int chunk = blockIdx.x * (RED_THREADS / TX) + threadIdx.x / TX;
+  const int total = start[V];
+  const int c0 = chunk * C, c1 = min(total, c0 + C);
+  for (int col = tx * VEC; col < D && c0 < c1; col += TX * VEC) {
+    float acc[VEC];
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) acc[k] = 0.f;
+    for (int j = c0; j < c1; j += 8) {
+      float v[8][VEC];
+      int w[9];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        const int i = min(j + u, c1 - 1);
+        w[u] = word[i];
+        load_vec<T, VEC>(dy + (int64_t)order[i] * ld + col, v[u]);
+      }
+      w[8] = j + 8 < c1 ? word[j + 8] : -1;
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        if (j + u < c1) {
+#pragma unroll
+          for (int k = 0; k < VEC; ++k) acc[k] += v[u][k];
+          if (j + u + 1 == c1 || w[u + 1] != w[u]) {  // the last of its word in this chunk
+            const int first = start[w[u]], end = start[w[u] + 1];
+            if (first >= c0 && end <= c1) {
+              put_row<VEC>(dtable + (int64_t)w[u] * D + col, acc, scale, accumulate);
+            } else {
+              put_row<VEC>(part + ((int64_t)chunk * 2 + (first >= c0)) * D + col, acc, 1.f, false);
+            }
+#pragma unroll
+            for (int k = 0; k < VEC; ++k) acc[k] = 0.f;
+          }
+        }
+      }
+    }
+  }
+}
+
+// Joins the parts of a word that spans chunks, in their order: the block row
+// of the chunk where it begins.
+template <int VEC>
+__global__ void __launch_bounds__(RED_THREADS) join_kernel(const int* __restrict__ start, const int* __restrict__ word,
+                                                           const float* __restrict__ part, float* __restrict__ dtable,
+                                                           int V, int D, int C, int TX, int chunks, float scale,
+                                                           int accumulate) {
+  const int chunk = blockIdx.x * (RED_THREADS / TX) + threadIdx.x / TX;
+  const int total = start[V];
+  const int64_t c1 = (int64_t)(chunk + 1) * C;
+  if (chunk >= chunks || c1 >= total) return;
+  const int w = word[c1 - 1];
+  const int end = start[w + 1];
+  if (end <= c1 || start[w] < c1 - C) return;
+  const int last = (end - 1) / C;  // the chunk that holds its last token
+  for (int col = (threadIdx.x % TX) * VEC; col < D; col += TX * VEC) {
+    float acc[VEC];
+    load_vec<float, VEC>(part + ((int64_t)chunk * 2 + 1) * D + col, acc);
+    int c = chunk + 1;
+    for (; c + 7 <= last; c += 8) {
+      float v[8][VEC];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) load_vec<float, VEC>(part + (int64_t)(c + u) * 2 * D + col, v[u]);
+#pragma unroll
+      for (int u = 0; u < 8; ++u)
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) acc[k] += v[u][k];
+    }
+    for (; c <= last; ++c) {
+      float v[VEC];
+      load_vec<float, VEC>(part + (int64_t)c * 2 * D + col, v);
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) acc[k] += v[k];
+    }
+    put_row<VEC>(dtable + (int64_t)w * D + col, acc, scale, accumulate);
+  }
+}
+
+// Places of one chunk: more for long inputs, where there are chunks enough.
+int chunk_of(int64_t n) { return n <= 16384 ? 16 : (n <= 65536 ? 32 : 64); }
+
+// Threads across a row of D elements, VEC each: a power of two up to a block.
+int across(int D, int vec) {
+  int tx = 1;
+  while (tx < RED_THREADS && tx * vec < D) tx *= 2;
+  return tx;
+}
+
+bool al16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
+template <typename T, typename ID>
+void lookup_t(const ID* ids, const T* table, T* out, int64_t n, int64_t V, int D, int64_t ld, float scale,
+              cudaStream_t s) {
+  constexpr int VEC = Vec<T>::N;
+  const unsigned grid = (unsigned)((n + 7) / 8);
+  if (D % VEC == 0 && ld % VEC == 0 && al16(table) && al16(out))
+    lookup_kernel<T, ID, VEC><<<grid, 256, 0, s>>>(ids, table, out, n, V, D, ld, scale);
+  else
+    lookup_kernel<T, ID, 1><<<grid, 256, 0, s>>>(ids, table, out, n, V, D, ld, scale);
+  DLVK_POST_LAUNCH();
+}
+
+template <typename T, int VEC>
+void sums(const T* dy, int64_t ld, const int* start, const int* order, const int* word, float* dtable, float* part,
+          int64_t n, int V, int D, float scale, bool accumulate, cudaStream_t s) {
+  const int C = chunk_of(n);
+  const int chunks = (int)((n + C - 1) / C);
+  const int tx = across(D, VEC), per = RED_THREADS / tx;
+  const int chunk_blocks = (chunks + per - 1) / per;
+  const int zero_blocks = accumulate ? 0 : (int)std::min<int64_t>((V + 7) / 8, 148 * 8);
+  if (chunk_blocks + zero_blocks > 0) {
+    sum_chunks_kernel<T, VEC><<<chunk_blocks + zero_blocks, RED_THREADS, 0, s>>>(
+        dy, ld, start, order, word, dtable, part, V, D, C, tx, chunk_blocks, scale, accumulate ? 1 : 0);
+    DLVK_POST_LAUNCH();
+  }
+  if (chunks > 1) {
+    constexpr int JV = VEC > 1 ? 4 : 1;
+    const int jx = across(D, JV), jper = RED_THREADS / jx;
+    join_kernel<JV><<<(chunks + jper - 1) / jper, RED_THREADS, 0, s>>>(start, word, part, dtable, V, D, C, jx, chunks,
+                                                                       scale, accumulate ? 1 : 0);
+    DLVK_POST_LAUNCH();
+  }
+}
+
+}  // namespace
+
+void embedding_lookup(DType dt, bool ids64, const void* ids, const void* table, void* out, int64_t n, int64_t V, int D,
+                      int64_t ld, float scale, cudaStream_t s) {
+  if (n == 0 || D == 0) return;
+  DLVK_CHECK(n < (1LL << 34), "embedding_lookup: too many tokens for one launch");
+  const int32_t* i32 = reinterpret_cast<const int32_t*>(ids);
+  const int64_t* i64 = reinterpret_cast<const int64_t*>(ids);
+  if (dt == DType::F32) {
+    const float* t = reinterpret_cast<const float*>(table);
+    float* o = reinterpret_cast<float*>(out);
+    if (ids64) lookup_t(i64, t, o, n, V, D, ld, scale, s);
+    else lookup_t(i32, t, o, n, V, D, ld, scale, s);
+  } else {
+    DLVK_CHECK(dt == DType::BF16, "embedding_lookup: the table is fp32 or bf16");
+    const __nv_bfloat16* t = reinterpret_cast<const __nv_bfloat16*>(table);
+    __nv_bfloat16* o = reinterpret_cast<__nv_bfloat16*>(out);
+    if (ids64) lookup_t(i64, t, o, n, V, D, ld, scale, s);
+    else lookup_t(i32, t, o, n, V, D, ld, scale, s);
+  }
+}
+
+int64_t embedding_grad_part_floats(int64_t n, int D) {
+  const int C = chunk_of(n);
+  return (n + C - 1) / C * 2 * D;
+}
+
+void embedding_grad(DType dt, bool ids64, const void* ids, const void* dy, int64_t ld, float* dtable, int64_t n,
+                    int64_t V, int D, float scale, int64_t padding, bool accumulate, int* start, int* order, int* word,
+                    float* part, cudaStream_t s) {
+  if (V == 0 || D == 0) return;
+  DLVK_CHECK(n < (1LL << 31) - 1024 && V < (1LL << 31) - SORT_WORDS, "embedding_grad: more than 2^31 tokens or words");
+  // words of a block: all 148 SMs, at least 8 each, at most what its counts have room for
+  const int R = (int)std::min<int64_t>(SORT_WORDS, std::max<int64_t>(8, (V + 147) / 148));
+  const int blocks = (int)((V + R - 1) / R);
+  const size_t smem = (size_t)SORT_WARPS * R * sizeof(int);
+  static bool attr_set[kMaxDevices] = {false};
+  const int dev = current_device_slot();
+  if (!attr_set[dev]) {
+    const int most = SORT_WARPS * SORT_WORDS * (int)sizeof(int);
+    DLVK_CUDA_CHECK(cudaFuncSetAttribute(sort_tokens_kernel<int32_t>, cudaFuncAttributeMaxDynamicSharedMemorySize, most));
+    DLVK_CUDA_CHECK(cudaFuncSetAttribute(sort_tokens_kernel<int64_t>, cudaFuncAttributeMaxDynamicSharedMemorySize, most));
+    attr_set[dev] = true;
+  }
+  const int pad = padding >= 0 && padding < V ? (int)padding : -1;
+  if (ids64)
+    sort_tokens_kernel<<<blocks, SORT_THREADS, smem, s>>>(reinterpret_cast<const int64_t*>(ids), (int)n, (int)V, R, pad,
+                                                          start, order, word);
+  else
+    sort_tokens_kernel<<<blocks, SORT_THREADS, smem, s>>>(reinterpret_cast<const int32_t*>(ids), (int)n, (int)V, R, pad,
+                                                          start, order, word);
+  DLVK_POST_LAUNCH();
+  const bool out_ok = al16(dtable) && al16(part);
+  if (dt == DType::F32) {
+    const float* g = reinterpret_cast<const float*>(dy);
+    if (D % 4 == 0 && ld % 4 == 0 && al16(g) && out_ok)
+      sums<float, 4>(g, ld, start, order, word, dtable, part, n, (int)V, D, scale, accumulate, s);
+    else
+      sums<float, 1>(g, ld, start, order, word, dtable, part, n, (int)V, D, scale, accumulate, s);
+  } else {
+    DLVK_CHECK(dt == DType::BF16, "embedding_grad: dy is fp32 or bf16");
+    const __nv_bfloat16* g = reinterpret_cast<const __nv_bfloat16*>(dy);
+    if (D % 8 == 0 && ld % 8 == 0 && al16(g) && out_ok)
+      sums<__nv_bfloat16, 8>(g, ld, start, order, word, dtable, part, n, (int)V, D, scale, accumulate, s);
+    else
+      sums<__nv_bfloat16, 1>(g, ld, start, order, word, dtable, part, n, (int)V, D, scale, accumulate, s);
+  }
+}
+
+}  // namespace dlvk

@@ -396,6 +396,8 @@ def build_graph(model, input_shape: Sequence[int]) -> Tuple[List[bytes], List[by
                 x = g.op({"relu": "Relu", "sigmoid": "Sigmoid", "tanh": "Tanh"}[a], [x])
         elif isinstance(layer, L.EmbeddingLayer):
             x = g.op("Gather", [g.param(layer.weight), x], axis=0)
+            if layer.embed_scale != 1.0:
+                x = g.op("Mul", [x, g.init("embed_scale", torch.tensor(layer.embed_scale))])
         elif isinstance(layer, L.LayerNormLayer):
             x = _layernorm(g, x, layer)
         elif isinstance(layer, L.PositionalEncodingLayer):

@@ -33,7 +33,8 @@ def layer_from_config(d: dict) -> L.ModernLayer:
     if t == "Flatten":
         return L.FlattenLayer()
     if t == "Embedding":
-        return L.EmbeddingLayer(d["num_embeddings"], d["embedding_dim"])
+        return L.EmbeddingLayer(d["num_embeddings"], d["embedding_dim"], embed_scale=g("embed_scale", 1.0),
+                                padding_idx=g("padding_idx", None))
     if t == "LayerNorm":
         return L.LayerNormLayer(d["normalized_shape"], g("eps", 1e-5))
     if t == "MultiHeadAttention":

@@ -556,14 +556,21 @@ class FlattenLayer(ModernLayer):
 
 
 class EmbeddingLayer(ModernLayer):
-    """Token embedding; ids outside [0, V) produce zeros
-    (shaders/embedding_lookup.comp:36-44)."""
+    """Token embedding, times `embed_scale` (for instance the root of the
+    width); ids outside [0, V) produce zeros
+    (shaders/embedding_lookup.comp:36-44).  Positions that hold `padding_idx`
+    are looked up like any other and contribute no gradient."""
 
     type_name = "Embedding"
 
-    def __init__(self, num_embeddings: int, embedding_dim: int, init_std: float = 1.0):
+    def __init__(self, num_embeddings: int, embedding_dim: int, init_std: float = 1.0, embed_scale: float = 1.0,
+                 padding_idx: Optional[int] = None):
         super().__init__()
         self.num_embeddings, self.embedding_dim = int(num_embeddings), int(embedding_dim)
+        self.embed_scale = float(embed_scale)
+        if padding_idx is not None and not 0 <= int(padding_idx) < self.num_embeddings:
+            raise ValueError(f"padding_idx {padding_idx} is outside [0, {self.num_embeddings})")
+        self.padding_idx = None if padding_idx is None else int(padding_idx)
         self.weight = self._param("weight", _normal((self.num_embeddings, self.embedding_dim), init_std))
         self._anchor = None
 
@@ -574,7 +581,9 @@ class EmbeddingLayer(ModernLayer):
         ids = x.data if facade else x
         if self.device_ctx is None:
             self.to(ids.device, torch.float32)
-        y = Fn.EmbeddingFn.apply(ids.to(torch.int32), self.weight, Fn._ANCHOR)
+        if ids.dtype not in (torch.int32, torch.int64):
+            ids = ids.to(torch.int32)
+        y = Fn.EmbeddingFn.apply(ids, self.weight, Fn._ANCHOR, self.embed_scale, self.padding_idx)
         if self.track:
             self._last_in, self._last_out = None, y
         self.output_shape = tuple(y.shape)

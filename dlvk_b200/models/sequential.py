@@ -46,6 +46,11 @@ def layer_config(layer) -> dict:
         v = getattr(layer, k, None)
         if isinstance(v, (int, float, bool, str)):
             d[k] = v
+    if isinstance(layer, L.EmbeddingLayer):  # only what differs from a plain lookup
+        if layer.embed_scale != 1.0:
+            d["embed_scale"] = layer.embed_scale
+        if layer.padding_idx is not None:
+            d["padding_idx"] = layer.padding_idx
     if isinstance(layer, L.ActivationLayer):
         d["type"] = "Activation"
         d["activation"] = layer.activation.value
@@ -150,8 +155,9 @@ class Sequential(Model):
     def add_flatten(self):
         return self.add(L.FlattenLayer())
 
-    def add_embedding(self, num_embeddings: int, embedding_dim: int, init_std: float = 1.0):
-        return self.add(L.EmbeddingLayer(num_embeddings, embedding_dim, init_std))
+    def add_embedding(self, num_embeddings: int, embedding_dim: int, init_std: float = 1.0, embed_scale: float = 1.0,
+                      padding_idx: Optional[int] = None):
+        return self.add(L.EmbeddingLayer(num_embeddings, embedding_dim, init_std, embed_scale, padding_idx))
 
     def add_layernorm(self, normalized_shape: int, eps: float = 1e-5):
         return self.add(L.LayerNormLayer(normalized_shape, eps))

@@ -83,9 +83,9 @@ def wide_mlp(device=None, dtype="bf16", seed=0, width=4096, depth=4, d_in=1024, 
 
 
 def transformer(device=None, dtype="bf16", seed=0, vocab=32000, d_model=1024, layers=12, heads=16, d_ff=4096,
-                std=0.02) -> Sequential:
+                std=0.02, embed_scale=1.0, padding_idx=None) -> Sequential:
     m = Sequential(device, dtype, seed=seed)
-    m.add_embedding(vocab, d_model, init_std=std)
+    m.add_embedding(vocab, d_model, init_std=std, embed_scale=embed_scale, padding_idx=padding_idx)
     for _ in range(layers):
         m.add_transformer_encoder(d_model, heads, d_ff, init_std=std)
     m.add_layernorm(d_model)

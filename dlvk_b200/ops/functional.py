@@ -254,21 +254,23 @@ class DropoutFn(torch.autograd.Function):
 
 
 class EmbeddingFn(torch.autograd.Function):
+    """scale * table[ids]; the table's gradient is summed in token order
+    (NN.embedding_grad), without the positions that hold `padding_idx`."""
+
     @staticmethod
-    def forward(ctx, ids, table, anchor):
-        ctx.table = table
+    def forward(ctx, ids, table, anchor, scale=1.0, padding_idx=None):
+        ctx.table, ctx.scale, ctx.padding_idx = table, scale, padding_idx
         ctx.save_for_backward(ids)
-        return NN.embedding_fwd(ids, table.value)
+        return NN.embedding_lookup(ids, table.value, scale)
 
     @staticmethod
     def backward(ctx, gy):
         (ids,) = ctx.saved_tensors
         T = ctx.table
-        if not T.take_accumulate_flag():
-            zero_(T.grad)
-        NN.embedding_bwd(ids, gy.contiguous(), T.grad)
+        NN.embedding_grad(ids, gy, T.shape[0], ctx.scale, ctx.padding_idx, out=T.grad,
+                          accumulate=T.take_accumulate_flag())
         T.grad_ready()
-        return None, None, None
+        return None, None, None, None, None
 
 
 class AttentionFn(torch.autograd.Function):

@@ -219,6 +219,57 @@ def embedding_bwd(ids, dy, dtable):
     dtable.index_add_(0, idl[ok], dy.reshape(-1, dtable.shape[1]).float()[ok])
 
 
+def _check_embedding(ids, padding_idx, num_embeddings):
+    if ids.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"embedding ids are int32 or int64, got {ids.dtype}")
+    if padding_idx is not None and not 0 <= padding_idx < num_embeddings:
+        raise ValueError(f"padding_idx {padding_idx} is outside [0, {num_embeddings})")
+
+
+def embedding_lookup(ids, table, scale: float = 1.0):
+    """scale * table[ids] ([V, D] fp32 or bf16, rows any distance apart), one
+    rounding; ids outside [0, V) give zeros."""
+    if native(table):
+        return N().embedding_lookup(ids, table, scale)
+    _check_embedding(ids, None, table.shape[0])
+    idl = ids.long()
+    ok = (idl >= 0) & (idl < table.shape[0])
+    if table.shape[0] == 0:
+        return torch.zeros(*ids.shape, table.shape[1], dtype=table.dtype)
+    out = table[idl.clamp(0, table.shape[0] - 1)].float() * scale
+    return torch.where(ok[..., None], out, torch.zeros_like(out)).to(table.dtype)
+
+
+def embedding_grad(ids, dy, num_embeddings: int, scale: float = 1.0, padding_idx=None, out=None,
+                   accumulate: bool = False):
+    """Gradient of embedding_lookup w.r.t. its table, fp32 [num_embeddings, D]:
+    row v is scale * the sum of dy over the positions with id v, in ascending
+    position, the same bits every time (csrc/kernels/embedding.cu).  Ids
+    outside [0, V) and `padding_idx` have none.  `out` is overwritten whole,
+    or with `accumulate` added to."""
+    if native(dy):
+        if padding_idx is None:
+            padding_idx = -1
+        elif not 0 <= padding_idx < num_embeddings:
+            raise ValueError(f"padding_idx {padding_idx} is outside [0, {num_embeddings})")
+        return N().embedding_grad(ids, dy, num_embeddings, scale, padding_idx, out, accumulate)
+    _check_embedding(ids, padding_idx, num_embeddings)
+    if tuple(dy.shape[:-1]) != tuple(ids.shape):
+        raise ValueError(f"embedding_grad: ids {tuple(ids.shape)}, dy {tuple(dy.shape)}")
+    if out is None:
+        if accumulate:
+            raise ValueError("embedding_grad: accumulate needs out")
+        out = torch.empty(num_embeddings, dy.shape[-1], dtype=torch.float32)
+    elif tuple(out.shape) != (num_embeddings, dy.shape[-1]) or out.dtype != torch.float32:
+        raise ValueError(f"embedding_grad: out must be fp32 [{num_embeddings}, {dy.shape[-1]}]")
+    idl = ids.reshape(-1).long()
+    ok = (idl >= 0) & (idl < num_embeddings)
+    if padding_idx is not None:
+        ok &= idl != padding_idx
+    total = torch.zeros_like(out).index_add_(0, idl[ok], dy.reshape(-1, dy.shape[-1]).float()[ok])
+    return out.add_(total, alpha=scale) if accumulate else out.copy_(total * scale)
+
+
 # ---------------------------------------------------------------- attention
 def flash_ok(qkv, B: int, S: int, H: int, D: int) -> bool:
     """The fused tcgen05 attention kernels apply: bf16, head dim 64, S a
