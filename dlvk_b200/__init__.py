@@ -21,7 +21,7 @@ from .models.params import Parameter, ParamStore
 from .optim import (Optimizer, SGD, Adam, RMSprop, GradientClipping, LRScheduler, StepLRScheduler,
                     ExponentialLRScheduler, CosineAnnealingLRScheduler, LinearLRScheduler)
 from .losses import (LossFunction, CrossEntropyLoss, MeanSquaredError, BinaryCrossEntropyLoss, MSELoss, BCELoss,
-                     LossOpsGPU)
+                     LossOpsGPU, LinearCrossEntropyLoss)
 
 # The reference spells the device class VulkanDevice; this framework's device
 # runtime is CUDA.

@@ -92,6 +92,9 @@ struct GemmArgs {
   uint32_t* relu_bits_out = nullptr;
   const uint32_t* relu_bits = nullptr;
   int64_t ldbits = 0;
+  // Sum split-K partials in a fixed order (through the workspace) instead of
+  // adding them into an fp32 C as they come.
+  bool ordered = false;
 };
 // SIMT GEMM.  With a workspace of gemm_simt_workspace_floats(a) floats, a
 // small 2-D GEMM with a plain epilogue splits K across blocks (fp32 partials,
@@ -289,6 +292,61 @@ void embedding_fwd(DType dt, const int32_t* ids, const void* table, void* out, i
 // dtable must be zeroed (or hold the gradient to accumulate into).
 void embedding_bwd(DType dt, const int32_t* ids, const void* dy, float* dtable, int64_t n, int64_t V, int D,
                    cudaStream_t s);
+
+// ---- softmax cross entropy of a projection, without keeping its logits --------
+// z = x W + bias, x [rows, width], W [width, classes]; loss_i = log sum exp(z_i)
+// - z_i[label_i].  A label outside [0, classes) or equal to `ignore` does not
+// count.  Tensor-core passes (gemm_tc.cu): bf16 operands, the logits stay in
+// the accumulators.
+struct CeProjection {
+  const __nv_bfloat16* x = nullptr;  // row stride ldx
+  const __nv_bfloat16* w = nullptr;  // w_k: W^T, row (class) stride ldw; else W, row (width) stride ldw
+  int64_t rows = 0, width = 0, classes = 0, ldx = 0, ldw = 0;
+  bool w_k = false;
+  const float* bias = nullptr;       // fp32 [classes]
+  const void* labels = nullptr;
+  bool labels64 = false;
+  int64_t ignore = -1;
+  float2* stats = nullptr;           // [ce_tc_stat_cols][rows] (maximum, sum of exp(z - maximum))
+  float* zlabel = nullptr;           // [rows], written for rows that count
+  const float2* norm = nullptr;      // [rows] maximum and 1 / sum, for the gradient
+  const float* gscale = nullptr;     // device scalar: gradient w.r.t. a counted row's loss
+  unsigned* done = nullptr;          // set to 0 by ce_stats_tc, for ce_finish
+};
+bool ce_tc_supported(const CeProjection& c);
+int ce_tc_stat_cols(int64_t rows, int64_t classes);
+void ce_stats_tc(const CeProjection& c, cudaStream_t s, uint32_t* err);
+// dl[:, 0 : n] = (softmax - onehot) * gscale of the classes [col0, col0 + n),
+// bf16, row stride ldd; colsum (or null): its fp32 column sums per 32 rows
+// [ceil(rows / 32)][n], for colsum_partials.
+void ce_grad_tc(const CeProjection& c, int col0, int n, __nv_bfloat16* dl, int64_t ldd, float* colsum, cudaStream_t s,
+                uint32_t* err);
+// The passes around them, and the same statistics / gradient from logits in
+// memory (vocab_loss.cu).
+struct CeRows {
+  int64_t rows = 0, classes = 0, ignore = -1;
+  const void* labels = nullptr;
+  bool labels64 = false;
+};
+// Joins the statistics: rows_loss (0 where a row does not count), norm; the
+// last block to finish sums them: *loss = sum (mean: / counted rows),
+// *gscale = (mean: 1 / counted) * (*grad_scale or 1), *correct += rows whose
+// class has the largest logit.  partial: 3 doubles per 32 rows.  `done` was
+// set to 0 by the statistics' launch.  With x_clean: a copy of x whose uncounted rows are 0.
+void ce_finish(const CeRows& r, const float2* stats, int stat_cols, const float* zlabel, float* rows_loss, float2* norm,
+               bool mean, const float* grad_scale, float* loss, float* gscale, unsigned long long* correct,
+               double* partial, unsigned* done, DType dt, const void* x, int64_t ldx, int64_t width, void* x_clean,
+               int64_t ldc, cudaStream_t s);
+// One (maximum, sum) per row from logits z [rows, n] fp32 of the classes from col0 on.
+void ce_piece_stats(const CeRows& r, const float* z, int64_t ldz, int64_t col0, int64_t n, float2* stats,
+                    float* zlabel, unsigned* done, cudaStream_t s);
+// z becomes the gradient in place; dl (or null) its bf16 copy, row stride ldz.
+void ce_piece_grad(const CeRows& r, float* z, int64_t ldz, int64_t col0, int64_t n, const float2* norm,
+                   const float* gscale, __nv_bfloat16* dl, cudaStream_t s);
+// dst [rows, cols] (row stride ldd) = src (strides rs, cs), or += (accumulate);
+// columns [cols, pad_to) become 0.  fp32 or bf16 each.
+void copy_matrix(DType dst_dt, DType src_dt, const void* src, int64_t rs, int64_t cs, void* dst, int64_t ldd,
+                 int64_t rows, int64_t cols, int64_t pad_to, bool accumulate, cudaStream_t s);
 
 // ---- embedding lookup with scale, gradient by sorted tokens (embedding.cu) ---
 // ids: int32 or int64 (ids64).  Rows of table / dy are ld elements apart.

@@ -28,6 +28,7 @@
 #include "dlvk/common.h"
 #include "dlvk/kernels.h"
 #include "dlvk/sm100.h"
+#include "dlvk/tmap.h"
 
 namespace dlvk {
 namespace {
@@ -36,6 +37,21 @@ using namespace sm100;
 
 constexpr int BM = 128;
 constexpr int BK = 64;  // bf16 elements per 128-byte swizzle row
+constexpr int CE_ROW_OUT = -(1 << 30);  // place of the class in a chunk, for a row that does not count
+
+// Operands of the softmax cross entropy epilogues.
+struct CeEpilogue {
+  const void* labels;  // int32 or int64 class of each row
+  int labels64;
+  int64_t ignore;      // a class that does not count (-1: none)
+  int64_t classes;     // classes of the whole vocabulary; others do not count
+  int col0;            // class of this launch's first column
+  float2* stats;       // EPI 3: [column half tiles][M] (maximum, sum)
+  float* zlabel;       // EPI 3: the logit of each row's class
+  const float2* norm;  // EPI 4: each row's maximum and 1 / sum of exp(z - maximum)
+  const float* gscale; // EPI 4: gradient of the loss w.r.t. each counted row's loss
+  unsigned* done;      // EPI 3: set to 0
+};
 
 struct TcParams {
   int M, N, K, batch;  // batch = number of (outer, inner) pairs
@@ -72,6 +88,7 @@ struct TcParams {
   uint32_t* bits_out;      // ReLU bitmask written (plain / TMA-store epilogues), or null
   const uint32_t* bits_in; // ReLU bitmask applied (staged epilogue), or null
   int64_t ldbits;          // 32-bit words per bitmask row
+  CeEpilogue ce;           // softmax cross entropy epilogues (EPI 3 and 4)
 };
 
 // PAIR: a 2-CTA cluster shares one 256 x BN tile (tcgen05 cta_group::2);
@@ -244,7 +261,8 @@ __device__ __forceinline__ void colsum_chunk(const TcParams& p, int row0, int la
       v[j] = keep + __shfl_xor_sync(0xffffffffu, send, h);
     }
   }
-  if (n0 + lane < p.N) p.colsum[(int64_t)(row0 >> 5) * p.N + n0 + lane] = v[0];
+  // a tile's last rows may be whole blocks past M, which have no partial
+  if (n0 + lane < p.N && row0 < p.M) p.colsum[(int64_t)(row0 >> 5) * p.N + n0 + lane] = v[0];
 }
 
 // v[j] += R[row, n0 + j] (bf16, C's dtype) for a row-per-lane epilogue: the
@@ -468,11 +486,84 @@ __device__ __forceinline__ void epi_store(const TcParams& p, const float* stg, i
   }
 }
 
+// ---- softmax cross entropy over the accumulators (logits in fp32) ----
+// The products of a vocabulary projection are consumed where they are made:
+// EPI 3 reduces each row's logits to a running maximum and sum, EPI 4 turns
+// them into the gradient (softmax - onehot) * scale, rounded once to bf16.
+// A thread owns one row of the tile, so neither needs a shuffle.
+constexpr float LOG2E = 1.4426950408889634f;
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// The row's class: -1 for rows that do not count and rows past the end.
+__device__ __forceinline__ int ce_label(const TcParams& p, int row) {
+  if (row >= p.M) return -1;
+  const int64_t lab = p.ce.labels64 ? reinterpret_cast<const int64_t*>(p.ce.labels)[row]
+                                    : (int64_t) reinterpret_cast<const int32_t*>(p.ce.labels)[row];
+  return (lab >= 0 && lab < p.ce.classes && lab != p.ce.ignore) ? (int)lab : -1;
+}
+
+// Accumulator chunk + bias; columns past N become -inf (softmax 0).
+__device__ __forceinline__ void ce_logits(const TcParams& p, const uint32_t* r, int n0, float* v) {
+#pragma unroll
+  for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]);
+  const int valid = p.N - n0;
+  if (p.bias) add_bias<32>(p.bias, true, n0, min(32, valid), v);
+  if (valid < 32) {
+#pragma unroll
+    for (int j = 0; j < 32; ++j) v[j] = j < valid ? v[j] : -INFINITY;
+  }
+}
+
+// Folds 32 logits into the running (maximum, sum of exp(z - maximum)).  A
+// maximum of -inf (every logit so far masked) is replaced by 0 in the
+// exponents, which then are exp(-inf) = 0; a NaN logit makes the sum NaN.
+// The maximum is taken off before the scaling to powers of 2, in a step of
+// its own: -3.4e38 (a mask of fp32's lowest value) times log2 e would be -inf.
+__device__ __forceinline__ void ce_online(const float* v, float& m, float& s) {
+  float t[16];
+#pragma unroll
+  for (int j = 0; j < 16; ++j) t[j] = fmaxf(v[j], v[j + 16]);
+#pragma unroll
+  for (int h = 8; h >= 1; h >>= 1)
+#pragma unroll
+    for (int j = 0; j < h; ++j) t[j] = fmaxf(t[j], t[j + h]);
+  const float mn = fmaxf(m, t[0]);
+  const float c = mn == -INFINITY ? 0.f : mn;
+  s *= ex2((m - c) * LOG2E);
+  float a[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int j = 0; j < 32; ++j) a[j & 3] += ex2((v[j] - c) * LOG2E);
+  s += (a[0] + a[1]) + (a[2] + a[3]);
+  m = mn;
+}
+
+// v[j] = (softmax - onehot) * g, for a row that does not count 0 whatever its
+// logits are; f = g / sum.
+__device__ __forceinline__ void ce_gradient(float m, float f, float g, int at, float* v) {
+#pragma unroll
+  for (int j = 0; j < 32; ++j) v[j] = ex2((v[j] - m) * LOG2E) * f;
+  if ((unsigned)at < 32u) {  // one chunk of the whole row
+#pragma unroll
+    for (int j = 0; j < 32; ++j) v[j] -= j == at ? g : 0.f;
+  }
+  if (at == CE_ROW_OUT) {
+#pragma unroll
+    for (int j = 0; j < 32; ++j) v[j] = 0.f;
+  }
+}
+
 // EPI = 1 compiles only the TMA-store epilogue (plain, bias, activation,
 // bf16 residual or mask, bitmask, column sums, reduce-add): a kernel with a
 // smaller instruction footprint for the common launches, whose epilogue
 // otherwise misses in the instruction cache.  EPI = 2 is that path with
-// alpha, bias and activation only.  EPI = 0 has every path.
+// alpha, bias and activation only.  EPI = 0 has every path.  EPI = 3 stores
+// nothing but each row's softmax statistics, EPI = 4 the cross entropy's
+// gradient as bf16 boxes.
 template <int BN, bool PAIR = false, int EPI = 0>
 __global__ void __launch_bounds__(320, 1)
     gemm_tc_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
@@ -536,6 +627,9 @@ __global__ void __launch_bounds__(320, 1)
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
   pdl_wait();  // the previous kernel's outputs (our operands) are complete from here on
+  if constexpr (EPI == 3) {
+    if (blockIdx.x == 0 && threadIdx.x == 0) *p.ce.done = 0u;
+  }
   GEMM_STAMP(threadIdx.x == 0, 5);
 
   if (warp == 0) {
@@ -795,6 +889,17 @@ __global__ void __launch_bounds__(320, 1)
       tmem_ld32(tbase, r[0]);
       tmem_ld_wait();
       GEMM_STAMP(threadIdx.x == 64 && last_tile, 13);
+      [[maybe_unused]] float ce_m = -INFINITY, ce_s = 0.f, ce_g = 0.f;
+      [[maybe_unused]] int ce_lab = -1;
+      if constexpr (EPI >= 3) {
+        ce_lab = ce_label(p, row0 + lane);
+        if (EPI == 4 && ce_lab >= 0) {
+          const float2 norm = p.ce.norm[row0 + lane];
+          ce_g = *p.ce.gscale;
+          ce_m = norm.x;
+          ce_s = norm.y * ce_g;
+        }
+      }
       // Unrolled by two (the register double buffer needs the chunk parity at
       // compile time), not fully: eight full copies of the chunk body for the
       // 512-column tile make the epilogue's code large.
@@ -803,7 +908,20 @@ __global__ void __launch_bounds__(320, 1)
         if (i == 1) GEMM_STAMP(threadIdx.x == 64 && last_tile, 15);
         if (i + 1 < NCH) tmem_ld32(tbase + (uint32_t)((i + 1) * 32), r[(i + 1) & 1]);
         const int n0 = tn * BN + (half * NCH + i) * 32;
-        if (EPI == 0 && staged) {
+        if constexpr (EPI == 3) {
+          if (n0 < p.N) {
+            float v[32];
+            ce_logits(p, r[i & 1], n0, v);
+            ce_online(v, ce_m, ce_s);
+            const int at = ce_lab - n0;
+            if ((unsigned)at < 32u) {  // ce_lab = -1 gives a negative place
+              float z = v[0];
+#pragma unroll
+              for (int j = 1; j < 32; ++j) z = j == at ? v[j] : z;
+              p.ce.zlabel[row0 + lane] = z;
+            }
+          }
+        } else if (EPI == 0 && staged) {
 #pragma unroll
           for (int j = 0; j < 32; ++j) stg[lane * 33 + j] = __uint_as_float(r[i & 1][j]) * p.alpha;
           __syncwarp();
@@ -812,7 +930,7 @@ __global__ void __launch_bounds__(320, 1)
             else epi_store<__nv_bfloat16, 8>(p, stg, row0, n0, lane, cb, rb, mb);
           }
           __syncwarp();
-        } else if (EPI == 1 || p.tma_c) {
+        } else if (EPI == 1 || EPI == 4 || p.tma_c) {
           // Row `lane` of this warp's box goes to smem and one lane stores the
           // box with TMA (rows >= M / columns >= N are clipped).  fp32: one
           // 32 x 32 box (128-byte rows) per chunk.  bf16: chunks i, i+1 fill
@@ -825,15 +943,20 @@ __global__ void __launch_bounds__(320, 1)
           if (nbox < p.N) {
             float v[32];
 #pragma unroll
-            const float rbv = (EPI != 2 && p.row_bias && row0 + lane < p.M) ? p.row_bias[row0 + lane] : 0.f;
+            const float rbv = (EPI < 2 && p.row_bias && row0 + lane < p.M) ? p.row_bias[row0 + lane] : 0.f;
+            if constexpr (EPI == 4) {
+              ce_logits(p, r[i & 1], n0, v);
+              ce_gradient(ce_m, ce_s, ce_g, ce_lab < 0 ? CE_ROW_OUT : ce_lab - p.ce.col0 - n0, v);
+            } else {
 #pragma unroll
-            for (int j = 0; j < 32; ++j) v[j] = fmaf(__uint_as_float(r[i & 1][j]), p.alpha, rbv);
-            if (p.bias && n0 < p.N) add_bias<32>(p.bias, p.bias_f32, n0, min(32, p.N - n0), v);
-            if (EPI != 2 && p.R) add_row_residual(p, rb, row0 + lane, n0, v);
-            apply_act<32>(p.act, v);
-            if (EPI != 2 && p.Mk) mask_row_bf16(p, mb, row0 + lane, n0, v);
-            if (EPI != 2 && p.bits_in) mask_row_bits(p, row0 + lane, n0, v);
-            if (EPI != 2 && p.bits_out && n0 < p.N && row0 + lane < p.M) store_bits(p, row0 + lane, n0, v);
+              for (int j = 0; j < 32; ++j) v[j] = fmaf(__uint_as_float(r[i & 1][j]), p.alpha, rbv);
+              if (p.bias && n0 < p.N) add_bias<32>(p.bias, p.bias_f32, n0, min(32, p.N - n0), v);
+            }
+            if (EPI < 2 && p.R) add_row_residual(p, rb, row0 + lane, n0, v);
+            if (EPI < 3) apply_act<32>(p.act, v);
+            if (EPI < 2 && p.Mk) mask_row_bf16(p, mb, row0 + lane, n0, v);
+            if (EPI < 2 && p.bits_in) mask_row_bits(p, row0 + lane, n0, v);
+            if (EPI < 2 && p.bits_out && n0 < p.N && row0 + lane < p.M) store_bits(p, row0 + lane, n0, v);
             // Boxes start on 1024-byte boundaries (the swizzled box layout is
             // defined on aligned addresses).
             if (opens) {
@@ -872,7 +995,7 @@ __global__ void __launch_bounds__(320, 1)
                 st_shared_v4(a ^ (((a >> 7) & 7u) << 4), w[0], w[1], w[2], w[3]);
               }
             }
-            if (BN != 512 && EPI != 2 && p.colsum) {  // after the box write: consumes v (512-wide tiles: never, see host)
+            if (BN != 512 && EPI != 2 && EPI != 3 && p.colsum) {  // after the box write: consumes v (512-wide tiles: never, see host)
               if (row0 + lane >= p.M) {
 #pragma unroll
                 for (int j = 0; j < 32; ++j) v[j] = 0.f;
@@ -948,6 +1071,10 @@ __global__ void __launch_bounds__(320, 1)
           }
         }
         if (i + 1 < NCH) tmem_ld_wait();
+      }
+      if constexpr (EPI == 3) {
+        if (row0 + lane < p.M)
+          p.ce.stats[(int64_t)(2 * tn + half) * p.M + row0 + lane] = make_float2(ce_m, ce_s);
       }
       GEMM_STAMP(threadIdx.x == 64 && last_tile, 14);
       tc_fence_before();
@@ -1283,7 +1410,7 @@ bool split_red_enabled() {
 // an epilogue that is linear in the accumulator (alpha only; beta 0 or 1),
 // and the alignment the fp32 C map needs.
 bool split_red_ok(DType out_dt, const GemmArgs& a) {
-  return split_red_enabled() && tma_c_enabled() && out_dt == DType::F32 && a.batch == 1 && a.batch2 == 1 &&
+  return !a.ordered && split_red_enabled() && tma_c_enabled() && out_dt == DType::F32 && a.batch == 1 && a.batch2 == 1 &&
          (a.beta == 0.f || a.beta == 1.f) && a.bias == nullptr && a.residual == nullptr &&
          a.relu_mask == nullptr && a.relu_bits == nullptr && a.relu_bits_out == nullptr && a.act == ACT_NONE &&
          al16(a.C) && (a.ldc * 4) % 16 == 0 &&
@@ -1641,6 +1768,90 @@ int& pair_flag() {
 }  // namespace
 
 bool gemm_tc_pair_enabled() { return pair_flag() != 0; }
+
+// ---- softmax cross entropy of a projection -------------------------------------
+// Logits tile width: CTA pairs on 256 x 256 tiles from 256 rows on, single
+// CTAs below, on 128 columns where 256-wide tiles would leave SMs without one.
+namespace {
+struct CeTiling {
+  bool pair;
+  int bn;
+};
+CeTiling ce_tiling(int64_t M, int64_t N) {
+  if (gemm_tc_pair_enabled() && M >= 256) return {true, 256};
+  return {false, (N + 255) / 256 * ((M + BM - 1) / BM) >= sm_count() ? 256 : 128};
+}
+
+void ce_launch(const CeProjection& c, bool grad, int n, int col0, __nv_bfloat16* dl, int64_t ldd, float* colsum,
+               cudaStream_t s, uint32_t* err) {
+  tmap::bind_context();
+  // the statistics run over all classes at once, so both passes tile alike
+  const CeTiling t = ce_tiling(c.rows, c.classes);
+  const __nv_bfloat16* w = c.w + (c.w_k ? (int64_t)col0 * c.ldw : col0);
+  const uint64_t da = (uint64_t)c.ldx * (uint64_t)c.rows;
+  const CUtensorMap ta = make_tmap(c.x, c.width, c.rows, 1, 1, c.ldx, da, da, BM, Elem::BF16);
+  CUtensorMap tb;
+  if (c.w_k) {
+    const uint64_t d = (uint64_t)c.ldw * (uint64_t)n;
+    tb = make_tmap(w, c.width, n, 1, 1, c.ldw, d, d, t.pair ? 128 : t.bn, Elem::BF16);
+  } else {
+    const uint64_t d = (uint64_t)c.ldw * (uint64_t)c.width;
+    tb = make_tmap(w, n, c.width, 1, 1, c.ldw, d, d, BK, Elem::BF16, true);
+  }
+  TcParams p{};
+  p.M = (int)c.rows;
+  p.N = n;
+  p.K = (int)c.width;
+  p.batch = p.batch2 = 1;
+  p.tiles_m = (int)((c.rows + (t.pair ? 2 * BM : BM) - 1) / (t.pair ? 2 * BM : BM));
+  p.tiles_n = (n + t.bn - 1) / t.bn;
+  p.b_mn = c.w_k ? 0 : 1;
+  p.alpha = 1.f;
+  p.bias = c.bias ? c.bias + col0 : nullptr;
+  p.bias_f32 = 1;
+  p.err = err;
+  p.splits = 1;
+  p.kb_per_split = (int)((c.width + BK - 1) / BK);
+  p.ce = {c.labels, c.labels64 ? 1 : 0, c.ignore, c.classes, col0, c.stats, c.zlabel, c.norm, c.gscale, c.done};
+  if (!grad) {
+    if (t.pair) launch_tc_pair_k<256, 3>(ta, tb, ta, p, 0, s);
+    else if (t.bn == 256) launch_tc_k<256, 3>(ta, tb, ta, p, 0, s);
+    else launch_tc_k<128, 3>(ta, tb, ta, p, 0, s);
+    return;
+  }
+  p.C = dl;
+  p.ldc = ldd;
+  p.vec_ok = 1;
+  p.colsum = colsum;
+  const CUtensorMap tc = make_c_map(p, c.rows, n);
+  DLVK_CHECK(p.tma_c == 1, "cross entropy gradient: its tile map was refused");
+  if (t.pair) launch_tc_pair_k<256, 4>(ta, tb, tc, p, 0, s);
+  else if (t.bn == 256) launch_tc_k<256, 4>(ta, tb, tc, p, 0, s);
+  else launch_tc_k<128, 4>(ta, tb, tc, p, 0, s);
+}
+}  // namespace
+
+bool ce_tc_supported(const CeProjection& c) {
+  return al16(c.x) && al16(c.w) && c.ldx % 8 == 0 && c.ldw % 8 == 0 && c.rows >= 1 && c.width >= 1 &&
+         c.classes >= 64 && c.rows < (1LL << 31) - 256 && c.classes < (1LL << 30) && c.width < (1LL << 31) - 64 &&
+         ((c.rows + 127) / 128) * ((c.classes + 127) / 128) < (1LL << 31) && tma_c_enabled();
+}
+
+int ce_tc_stat_cols(int64_t rows, int64_t classes) {
+  const int bn = ce_tiling(rows, classes).bn;
+  return (int)(2 * ((classes + bn - 1) / bn));
+}
+
+void ce_stats_tc(const CeProjection& c, cudaStream_t s, uint32_t* err) {
+  DLVK_CHECK(ce_tc_supported(c), "ce_stats_tc: unsupported layout");
+  ce_launch(c, false, (int)c.classes, 0, nullptr, 0, nullptr, s, err);
+}
+
+void ce_grad_tc(const CeProjection& c, int col0, int n, __nv_bfloat16* dl, int64_t ldd, float* colsum, cudaStream_t s,
+                uint32_t* err) {
+  DLVK_CHECK(ce_tc_supported(c) && col0 % 8 == 0 && ldd % 8 == 0 && al16(dl), "ce_grad_tc: unsupported layout");
+  ce_launch(c, true, n, col0, dl, ldd, colsum, s, err);
+}
 
 void gemm_tc_set_pair(bool on) { pair_flag() = on ? 1 : 0; }
 

@@ -167,6 +167,11 @@ class MultiGPUTrainer:
         loss_sum = correct = n = rows = 0.0
         with torch.no_grad():
             for x, y in loader:
+                if getattr(self.loss_fn, "fuses_head", False):
+                    loss, hits, seen = self.model.head_loss(x, y, self.loss_fn)
+                    loss_sum, n = loss_sum + float(loss) * x.shape[0], n + x.shape[0]
+                    correct, rows = correct + hits, rows + seen
+                    continue
                 out = self.model.forward_logits(x) if fused else self.model.forward(x)
                 yd = y.to(out.device)
                 loss, _ = self.loss_fn.value_and_grad(out, yd, from_logits=fused)

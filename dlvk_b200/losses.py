@@ -80,6 +80,74 @@ class CrossEntropyLoss(LossFunction):
         return self.forward(out, target), self.backward(out, target)
 
 
+class LinearCrossEntropyLoss(LossFunction):
+    """Cross entropy of a model's last Dense layer and softmax taken together:
+    the loss and the gradients of hidden @ weight + bias without an array of
+    logits, which for a large vocabulary is the largest of the step.
+
+    hidden [..., E], weight [E, V] (also the transpose of a [V, E] embedding
+    table), bias [V] or None, target int32 / int64 [...].  Targets outside
+    [0, V) and `ignore_index` do not count; the mean is over those that do
+    (CrossEntropyLoss divides by all rows), and 0 when there are none.
+
+    `Sequential.train_step`, `TrainStep` and the trainers take it in the place
+    of CrossEntropyLoss for a model that ends in a Dense layer without
+    activation (and a Softmax or none)."""
+
+    fuses_head = True
+
+    def __init__(self, reduction: str = "mean", ignore_index=None):
+        if reduction not in ("mean", "sum", "none"):
+            raise ValueError(f"reduction is mean, sum or none, got {reduction!r}")
+        self.reduction, self.ignore_index = reduction, ignore_index
+
+    @staticmethod
+    def _rows(hidden, target):
+        hidden, target = _unwrap(hidden), _unwrap(target)
+        if target.shape != hidden.shape[:-1]:
+            raise ValueError(f"hidden {tuple(hidden.shape)} needs a target of {tuple(hidden.shape[:-1])}, "
+                             f"got {tuple(target.shape)}")
+        if hidden.dim() != 2:
+            hidden, target = hidden.reshape(-1, hidden.shape[-1]), target.reshape(-1)
+        return hidden.detach(), target
+
+    def forward(self, hidden, weight, target, bias=None, correct=None):
+        """The loss alone: a scalar, or with reduction "none" each row's (0 where it does not count)."""
+        x, t = self._rows(hidden, target)
+        loss, rows, _, _, _ = K.linear_ce(x, _unwrap(weight).detach(), t, bias, self.ignore_index,
+                                          self.reduction != "sum", False, correct=correct)
+        return rows.reshape(_unwrap(target).shape) if self.reduction == "none" else loss
+
+    def __call__(self, hidden, weight, target, bias=None):
+        return self.forward(hidden, weight, target, bias)
+
+    def value_and_grad(self, hidden, weight, target, bias=None, grad_scale=None):
+        """(loss, dhidden, dweight, dbias): gradients of the loss (times the
+        device scalar grad_scale) in the operands' layouts and types, dbias fp32."""
+        if self.reduction == "none":
+            raise ValueError("value_and_grad needs reduction mean or sum")
+        x, t = self._rows(hidden, target)
+        loss, _, dx, dw, db = K.linear_ce(x, _unwrap(weight).detach(), t, bias, self.ignore_index,
+                                          self.reduction == "mean", True, grad_scale)
+        return loss, dx.reshape(_unwrap(hidden).shape), dw, db
+
+    def head_backward(self, head, hidden, target, grad_scale=None, correct=None):
+        """(loss, dhidden) for a Dense layer `head`, whose parameters receive
+        their gradients (and whose grad-ready hooks fire)."""
+        if self.reduction == "none":
+            raise ValueError("training needs reduction mean or sum")
+        x, t = self._rows(hidden, target)
+        W, b = head.weight, head.bias
+        loss, _, dx, _, _ = K.linear_ce(
+            x, W.value, t, b.master if b is not None else None, self.ignore_index, self.reduction == "mean", True,
+            grad_scale, dw_out=W.grad, dw_accumulate=W.take_accumulate_flag(), db_out=b.grad if b is not None else None,
+            db_accumulate=b.take_accumulate_flag() if b is not None else False, correct=correct)
+        W.grad_ready()
+        if b is not None:
+            b.grad_ready()
+        return loss, dx.reshape(hidden.shape)
+
+
 class MeanSquaredError(LossFunction):
     def forward(self, predictions, targets):
         p = _unwrap(predictions)

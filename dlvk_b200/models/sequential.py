@@ -301,6 +301,57 @@ class Sequential(Model):
         self._last_out = y
         return y
 
+    # ----------------------------------------------------------- losses that take the head
+    def _head(self):
+        """(number of layers before it, the Dense layer at the end): what a
+        loss with `fuses_head` computes together with itself."""
+        n = len(self.m_layers) - (1 if self.has_trailing_softmax() else 0) - 1
+        head = self.m_layers[n] if n >= 0 else None
+        if not isinstance(head, L.DenseLayer) or head._act != K.ACT_NONE:
+            raise ValueError("this loss needs a model that ends in a Dense layer without activation "
+                             "(and a Softmax or none)")
+        return n, head
+
+    def _forward_hidden(self, x):
+        """(the head, its input, whether that input's ReLU backward was left to the head)."""
+        self.build()
+        n, head = self._head()
+        x = self._prepare_input(x)
+        with torch.set_grad_enabled(self.is_training):
+            h = self._run(x, upto=n)
+        seen, deferred = 0, False
+        for fn, k in self._plan:
+            if seen + k > n:
+                break
+            seen, deferred = seen + k, getattr(fn, "relu_feeds_dense", False)
+        if h.dim() > 2 and h.shape[-1] != head.input_size:
+            h = h.reshape(h.shape[0], -1)
+        if h.dtype != head.compute_dtype:
+            h = h.to(head.compute_dtype)
+        return head, h, deferred
+
+    def head_loss_backward(self, x, y, loss_fn, grad_scale=None, correct=None):
+        """Forward, loss and backward with a loss that takes the head
+        (LinearCrossEntropyLoss); returns the loss as a device scalar."""
+        head, h, deferred = self._forward_hidden(x)
+        self._last_out = None  # there are no logits for a later backward()
+        y = y.to(h.device)
+        loss, dh = loss_fn.head_backward(head, h, y, grad_scale, correct)
+        if h.requires_grad:
+            if deferred:
+                dh = K.binary(dh, h.detach(), K.BIN_RELU_BWD)
+            torch.autograd.backward(h, dh)
+        self.store.finish_backward()
+        return loss
+
+    def head_loss(self, x, y, loss_fn):
+        """(loss, correct rows, rows) of a batch without a gradient."""
+        head, h, _ = self._forward_hidden(x)
+        correct = torch.zeros(1, dtype=torch.int64, device=h.device)
+        loss = loss_fn.forward(h, head.weight.value, y.to(h.device), head.bias.master if head.bias is not None else None,
+                               correct=correct)
+        return loss, int(correct), y.numel()
+
     def backward(self, grad_output):
         """Backpropagate `grad_output` (gradient w.r.t. the last forward output)."""
         from ..tensor import Tensor as FacadeTensor
@@ -384,6 +435,12 @@ class Sequential(Model):
         self.build()
         self.store.zero_grad()
         self.dev.advance_step()
+        if getattr(loss_fn, "fuses_head", False):
+            loss = self.head_loss_backward(x, y, loss_fn)
+            if grad_hook is not None:
+                grad_hook(self)
+            optimizer.step(self)
+            return loss
         fused = getattr(loss_fn, "fuses_softmax", False) and self.has_trailing_softmax()
         out = self.forward_logits(x) if fused else self.forward(x)
         loss, dout = loss_fn.value_and_grad(out, y, from_logits=fused)

@@ -279,6 +279,67 @@ def softmax_ce(logits: torch.Tensor, target: torch.Tensor, grad_scale: float = 1
     return loss, dl
 
 
+def linear_ce(hidden: torch.Tensor, weight: torch.Tensor, target: torch.Tensor, bias=None, ignore_index=None,
+              mean: bool = True, want_grad: bool = True, grad_scale=None, dw_out=None, dw_accumulate: bool = False,
+              db_out=None, db_accumulate: bool = False, correct=None):
+    """Softmax cross entropy of hidden [N, E] @ weight [E, V] + bias without
+    an [N, V] array of logits.  Returns (loss, rows, dhidden, dweight, dbias):
+    the mean (or sum) over the rows that count and each row's own loss in
+    fp32, and the gradients of grad_scale (a device scalar, default 1) times
+    the loss, None where not wanted.  Rows whose target is outside [0, V) or
+    equals ignore_index count nothing; when no row counts, all is 0.
+
+    weight may be the transpose of a [V, E] table; dweight has its layout and
+    type, or goes to dw_out (fp32, `dw_accumulate` adds).  dbias is fp32.
+    `correct` (int64) is increased by the rows whose target has the largest
+    logit.  On the GPU: csrc/aten/linear_ce.cpp, bf16 and fp32."""
+    ignore = -1 if ignore_index is None else int(ignore_index)
+    if native(hidden):
+        return N().linear_ce(hidden, weight, target, bias, ignore, mean, want_grad, grad_scale, dw_out, dw_accumulate,
+                             db_out, db_accumulate, correct)
+    n, classes = hidden.shape[0], weight.shape[1]
+    if hidden.dim() != 2 or weight.dim() != 2 or weight.shape[0] != hidden.shape[1] or classes < 1:
+        raise ValueError(f"linear_ce: hidden {tuple(hidden.shape)}, weight {tuple(weight.shape)}")
+    if target.dtype not in (torch.int32, torch.int64) or tuple(target.shape) != (n,):
+        raise ValueError(f"linear_ce: target must be int32 or int64 [{n}], got {target.dtype} {tuple(target.shape)}")
+    if weight.dtype != hidden.dtype or hidden.dtype not in (torch.float32, torch.bfloat16):
+        raise ValueError(f"linear_ce: hidden is {hidden.dtype}, the weight {weight.dtype}")
+    if bias is not None and tuple(bias.shape) != (classes,):
+        raise ValueError(f"linear_ce: bias must be [{classes}], got {tuple(bias.shape)}")
+    lab = target.long()
+    counted = (lab >= 0) & (lab < classes) & (lab != ignore)
+    x, w, at = hidden.float()[counted], weight.float(), lab[counted]
+    z = x @ w
+    if bias is not None:
+        z = z + bias.float()
+    top = z.amax(-1, keepdim=True)
+    e = torch.exp(z - top)
+    total = e.sum(-1, keepdim=True)
+    zl = z.gather(1, at[:, None])[:, 0]
+    rows = torch.zeros(n)
+    rows[counted] = top[:, 0] - zl + torch.log(total[:, 0])
+    share = (1.0 / max(int(counted.sum()), 1)) if mean else 1.0
+    loss = rows.sum() * share
+    if correct is not None:
+        correct += (zl >= z.amax(-1)).sum() if zl.numel() else 0
+    if not want_grad:
+        return loss, rows, None, None, None
+    dz = e / total
+    dz[torch.arange(at.numel()), at] -= 1.0
+    dz *= share * (1.0 if grad_scale is None else float(grad_scale))
+    dx = torch.zeros_like(hidden)
+    dx[counted] = (dz @ w.t()).to(hidden.dtype)
+
+    def put(value, out, accumulate, like):
+        if out is None:
+            return value.to(like)
+        return out.add_(value) if accumulate else out.copy_(value)
+
+    dw = put(x.t() @ dz, dw_out, dw_accumulate, weight.dtype)
+    db = put(dz.sum(0), db_out, db_accumulate, torch.float32) if bias is not None else None
+    return loss, rows, dx, dw, db
+
+
 def sum_scalar(v: torch.Tensor, scale: float = 1.0) -> torch.Tensor:
     if native(v):
         return N().sum_scalar(v, scale)

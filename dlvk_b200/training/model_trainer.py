@@ -154,6 +154,12 @@ class ModelTrainer:
         fused = getattr(self.loss_function, "fuses_softmax", False) and self.model.has_trailing_softmax()
         with torch.no_grad():
             for xb, yb in self.create_batches(x_test, y_test, batch_size):
+                if getattr(self.loss_function, "fuses_head", False):
+                    loss, hits, rows = self.model.head_loss(xb, yb, self.loss_function)
+                    tot_loss += float(loss) * xb.shape[0]
+                    correct += hits * xb.shape[0] / max(rows, 1)  # per sample: its rows' mean
+                    total += xb.shape[0]
+                    continue
                 out = self.model.forward_logits(xb) if fused else self.model.forward(xb)
                 yb_d = yb.to(out.device)
                 loss, _ = self.loss_function.value_and_grad(out, yb_d, from_logits=fused)

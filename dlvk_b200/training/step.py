@@ -81,15 +81,21 @@ class TrainStep:
         m.dev.advance_step()
         if self.dp is not None:
             self.dp.begin_step()
-        fused = getattr(self.loss_fn, "fuses_softmax", False) and m.has_trailing_softmax()
-        out = m.forward_logits(self.x) if fused else m.forward(self.x)
-        loss, dout = self.loss_fn.value_and_grad(out, self.y, from_logits=fused)
-        if self.metrics:
-            self._record_metrics(out, loss)
-        if self.scaler is not None:
-            self.scaler.scale_grad_output(dout)
-        torch.autograd.backward(out, dout)
-        m.store.finish_backward()
+        if getattr(self.loss_fn, "fuses_head", False):
+            loss = m.head_loss_backward(self.x, self.y, self.loss_fn,
+                                        self.scaler.scale if self.scaler is not None else None, self.correct)
+            if self.metrics:
+                self.loss_sum.add_(loss.reshape(1), alpha=float(self.x.shape[0]))
+        else:
+            fused = getattr(self.loss_fn, "fuses_softmax", False) and m.has_trailing_softmax()
+            out = m.forward_logits(self.x) if fused else m.forward(self.x)
+            loss, dout = self.loss_fn.value_and_grad(out, self.y, from_logits=fused)
+            if self.metrics:
+                self._record_metrics(out, loss)
+            if self.scaler is not None:
+                self.scaler.scale_grad_output(dout)
+            torch.autograd.backward(out, dout)
+            m.store.finish_backward()
         if self.regularizer is not None:
             self.regularizer.apply_to_store(m.store, self.scaler.scale if self.scaler is not None else None)
         if self.dp is not None:

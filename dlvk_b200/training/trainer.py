@@ -131,6 +131,11 @@ class Trainer:
         tot, correct, n, rows = 0.0, 0, 0, 0
         with torch.no_grad():
             for x, y in batches:
+                if getattr(self.loss_fn, "fuses_head", False):
+                    loss, hits, seen = self.model.head_loss(x, y, self.loss_fn)
+                    tot, n = tot + float(loss) * x.shape[0], n + x.shape[0]
+                    correct, rows = correct + hits, rows + seen
+                    continue
                 out = self.model.forward_logits(x) if fused else self.model.forward(x)
                 yd = y.to(out.device)
                 loss, _ = self.loss_fn.value_and_grad(out, yd, from_logits=fused)
@@ -169,11 +174,13 @@ def make_loss(name: str):
     name = name.lower()
     if name in ("crossentropy", "cross_entropy", "ce"):
         return Lo.CrossEntropyLoss()
+    if name in ("linear_crossentropy", "linear_cross_entropy"):
+        return Lo.LinearCrossEntropyLoss()
     if name == "mse":
         return Lo.MeanSquaredError()
     if name in ("bce", "binary_crossentropy"):
         return Lo.BinaryCrossEntropyLoss()
-    raise ValueError(f"unknown loss '{name}' (mse, crossentropy, bce)")
+    raise ValueError(f"unknown loss '{name}' (mse, crossentropy, linear_crossentropy, bce)")
 
 
 def create_trainer(model, optimizer_name: str = "adam", learning_rate: float = 0.001,
