@@ -104,12 +104,13 @@ void product_into(const Operand& A, const Operand& B, const at::Tensor& dst, boo
               accumulate, stream());
 }
 
-// Classes of one piece of the gradient: `room` elements of [rows, piece], at
-// least 4096, in equal pieces of whole tiles.  A larger piece costs memory, a
-// smaller one another pass over the fp32 sums of dx.
-int64_t piece_of(int64_t rows, int64_t classes, int64_t room) {
-  const int64_t most = std::max<int64_t>(4096, room / std::max<int64_t>(rows, 1));
-  return std::min(round_up(ceil_div(classes, ceil_div(classes, most)), 256), round_up(classes, 256));
+// Rows of one block: `room` elements of [rows, classes], at least 2048 (every
+// block reads and writes the fp32 sums of dW once: 8 bytes per element of W
+// for 6 flops per row and element, 14% of the products' time at 2048), in
+// equal blocks of whole tiles.
+int64_t block_of(int64_t rows, int64_t classes, int64_t room) {
+  const int64_t most = std::max<int64_t>(2048, room / classes);
+  return std::min(rows, round_up(ceil_div(rows, ceil_div(rows, most)), 256));
 }
 
 }  // namespace
@@ -193,99 +194,134 @@ LinearCeResult linear_ce_op(const at::Tensor& x, const at::Tensor& w, const at::
   c.ldw = w_k ? wq.stride(1) : wq.stride(0);
   c.w_k = w_k;
   c.bias = bc.defined() ? bc.data_ptr<float>() : nullptr;
-  c.labels = tc.data_ptr();
   c.labels64 = tc.scalar_type() == at::kLong;
   c.ignore = ignore_index;
-  CeRows r{N, V, ignore_index, c.labels, c.labels64};
-  const bool tensor = bf && ce_tc_supported(c);  // else the logits of one piece at a time in memory
+  const bool tensor = bf && ce_tc_supported(c);  // else a block's logits go through memory in fp32
+  const bool keep = tensor && want_grad && !bias.has_value();  // exponentials kept, not made again
 
-  const int64_t piece = piece_of(N, V, tensor ? (128 << 20) : (64 << 20));
-  const int64_t pieces = ceil_div(V, piece);
-  const int stat_cols = tensor ? ce_tc_stat_cols(N, V) : (int)pieces;
-  const int64_t blocks = ceil_div(N, 32);
-  // scratch: 8-byte items first (sums, statistics), then floats, then the counter
-  const at::Tensor ws = at::empty({6 * blocks + 2 * N * stat_cols + 3 * N + 2}, f32);
+  // 256 MB of a block's exponentials, gradients or logits; the loss alone
+  // keeps a 32nd of that on the tensor cores, the statistics
+  const int64_t rows = block_of(N, V, !tensor ? (64LL << 20) : want_grad ? (128LL << 20) : (1LL << 30));
+  const int64_t blocks = ceil_div(N, rows);
+  const int stat_cols = tensor ? ce_tc_stat_cols(rows, V) : 1;
+  const int groups = (int)ceil_div(N, 32), lab_size = c.labels64 ? 8 : 4;
+  // scratch: 8-byte items first (sums, statistics, norms), then floats, then the counter
+  const at::Tensor ws = at::empty({6LL * groups + 2 * rows * stat_cols + 3 * rows + 2}, f32);
   double* partial = reinterpret_cast<double*>(ws.data_ptr<float>());
-  float2* stats = reinterpret_cast<float2*>(ws.data_ptr<float>() + 6 * blocks);
-  float2* norm = stats + N * stat_cols;
-  float* zlabel = reinterpret_cast<float*>(norm + N);
-  float* gscale = zlabel + N;
+  float2* stats = reinterpret_cast<float2*>(ws.data_ptr<float>() + 6LL * groups);
+  float2* norm = stats + rows * stat_cols;
+  float* zlabel = reinterpret_cast<float*>(norm + rows);
+  float* gscale = zlabel + rows;
   unsigned* done = reinterpret_cast<unsigned*>(gscale + 1);
+  const float* gsp = grad_scale.has_value() ? grad_scale->data_ptr<float>() : nullptr;
   c.stats = stats;
   c.zlabel = zlabel;
   c.norm = norm;
   c.gscale = gscale;
-  c.done = done;
 
+  const int64_t ldv = round_up(V, 8);
   const bool parts = !bf && fp32_gemm_mode() == 3 && (double)N * E * V >= kTf32Macs;
-  const Operand xo = parts ? split(xq) : Operand{xq, {}, {}}, wo = parts ? split(wq) : Operand{wq, {}, {}};
-  at::Tensor z;  // fp32 logits of a piece, where they do go through memory
-  auto logits = [&](int64_t col0, int64_t n) {
-    const at::Tensor zn = z.narrow(1, 0, n);
-    product(xo, wo.columns(col0, n), zn, false,
-            bc.defined() ? c10::optional<at::Tensor>(bc.narrow(0, col0, n)) : c10::nullopt);
-  };
-  if (tensor) {
-    ce_stats_tc(c, stream(), device_error_word());
-  } else {
-    z = at::empty({N, piece}, f32);
-    for (int64_t k = 0; k < pieces; ++k) {
-      const int64_t col0 = k * piece, n = std::min(piece, V - col0);
-      logits(col0, n);
-      ce_piece_stats(r, z.data_ptr<float>(), piece, col0, n, stats + k * N, zlabel, done, stream());
-    }
-  }
-  // dW = x^T dz reads x once more, with zeros in the rows that do not count:
-  // their dz is 0, but 0 times an infinity or NaN left there would not be.
-  at::Tensor xc;
+  const auto whole = [&](const at::Tensor& t) { return parts ? split(t) : Operand{t, {}, {}}; };
+  const Operand wo = tensor && !want_grad ? Operand{wq, {}, {}} : whole(wq);
+  at::Tensor z, dl, xc, part, dw32;
+  if (!tensor) z = at::empty({rows, ldv}, f32);
+  bool dw_k = false;
   if (want_grad) {
-    const int64_t ld = round_up(E, 16 / x.element_size());
-    xc = at::empty({N, ld}, x.options()).narrow(1, 0, E);
+    dl = bf ? at::empty({rows, ldv}, x.options()) : z;
+    // dW = x^T dz reads x once more, with zeros in the rows that do not count:
+    // their dz is 0, but 0 times an infinity or NaN left there would not be.
+    xc = at::empty({rows, round_up(E, 16 / x.element_size())}, x.options()).narrow(1, 0, E);
+    dw_k = out.dw.stride(1) != 1 && V > 1;  // the gradient's rows are classes too
+    // sums over several blocks are fp32 until the last
+    if (blocks > 1 && out.dw.scalar_type() != at::kFloat)
+      dw32 = dw_k ? at::empty({V, round_up(E, 4)}, f32).narrow(1, 0, E).t()
+                  : at::empty({E, round_up(V, 4)}, f32).narrow(1, 0, V);
+    if (out.dbias.defined()) part = at::empty({tensor ? ceil_div(rows, 32) * V : ldv}, f32);
   }
-  ce_finish(r, stats, stat_cols, zlabel, out.rows.data_ptr<float>(), norm, mean,
-            grad_scale.has_value() ? grad_scale->data_ptr<float>() : nullptr, out.loss.data_ptr<float>(), gscale,
-            correct.has_value() ? reinterpret_cast<unsigned long long*>(correct->data_ptr<int64_t>()) : nullptr, partial,
-            done, to_dtype(x), xq.data_ptr(), xq.stride(0), E, xc.defined() ? xc.data_ptr() : nullptr,
-            xc.defined() ? xc.stride(0) : 0, stream());
-  if (!want_grad) return out;
+  const at::Tensor dw = dw32.defined() ? dw32 : out.dw;
+  CeRows all{N, V, ignore_index, tc.data_ptr(), c.labels64};
+  if (blocks > 1) ce_count(all, mean, gsp, gscale, done, stream());
 
-  const Operand xco = parts ? split(xc) : Operand{xc, {}, {}};
-  const bool dw_k = out.dw.stride(1) != 1 && V > 1;  // the gradient's rows are classes too
-  at::Tensor dl = bf ? at::empty({N, piece}, x.options()) : z;
-  at::Tensor sum;  // dx of several pieces, fp32
-  if (pieces > 1) sum = at::empty({N, E}, f32);
-  at::Tensor part;
-  if (out.dbias.defined()) part = at::empty({tensor ? blocks * piece : piece}, f32);
-  for (int64_t k = 0; k < pieces; ++k) {
-    const int64_t col0 = k * piece, n = std::min(piece, V - col0);
-    if (tensor) {
-      ce_grad_tc(c, (int)col0, (int)n, reinterpret_cast<__nv_bfloat16*>(dl.data_ptr()), piece,
+  for (int64_t k = 0; k < blocks; ++k) {
+    const int64_t r0 = k * rows, n = std::min(rows, N - r0);
+    CeRows r = all;
+    r.rows = n;
+    r.labels = static_cast<const char*>(tc.data_ptr()) + r0 * lab_size;
+    const at::Tensor xk = xq.narrow(0, r0, n);
+    c.rows = n;
+    TORCH_INTERNAL_ASSERT(!tensor || n * ce_tc_stat_cols(n, V) <= rows * stat_cols);
+    c.x = bf ? reinterpret_cast<const __nv_bfloat16*>(xk.data_ptr()) : nullptr;
+    c.labels = r.labels;
+    c.done = blocks == 1 ? done : nullptr;
+    if (keep) {
+      ce_exp_tc(c, dl.data_ptr(), ldv, stream(), device_error_word());
+    } else if (tensor) {
+      ce_stats_tc(c, stream(), device_error_word());
+    } else {
+      product(whole(xk), wo, z.narrow(0, 0, n).narrow(1, 0, V), false,
+              bc.defined() ? c10::optional<at::Tensor>(bc) : c10::nullopt);
+      ce_memory_stats(r, z.data_ptr<float>(), ldv, stats, zlabel, c.done, stream());
+    }
+    CeFinish f{};
+    f.stats = stats;
+    f.stat_cols = tensor ? ce_tc_stat_cols(n, V) : 1;
+    f.zlabel = zlabel;
+    f.rows_loss = out.rows.data_ptr<float>() + r0;
+    f.norm = norm;
+    f.mean = mean;
+    f.set_gscale = blocks == 1;
+    f.grad_scale = gsp;
+    f.loss = out.loss.data_ptr<float>();
+    f.gscale = gscale;
+    f.correct = correct.has_value() ? reinterpret_cast<unsigned long long*>(correct->data_ptr<int64_t>()) : nullptr;
+    f.partial = partial;
+    f.done = done;
+    f.first_group = (int)(r0 / 32);  // blocks are whole tiles, the last apart
+    f.total_groups = groups;
+    if (want_grad) {
+      f.x = xk.data_ptr();
+      f.ldx = xk.stride(0);
+      f.width = E;
+      f.x_clean = xc.data_ptr();
+      f.ldc = xc.stride(0);
+    }
+    ce_finish(r, f, to_dtype(x), stream());
+    if (!want_grad) continue;
+
+    if (keep) {
+      ce_rescale(r, stats, ce_tc_stat_width(n, V), norm, gscale, dl.data_ptr(), ldv, stream());
+    } else if (tensor) {
+      ce_grad_tc(c, reinterpret_cast<__nv_bfloat16*>(dl.data_ptr()), ldv,
                  part.defined() ? part.data_ptr<float>() : nullptr, stream(), device_error_word());
       if (part.defined())
-        colsum_partials(part.data_ptr<float>(), blocks, n, 1.f, out.dbias.data_ptr<float>() + col0, db_accumulate,
-                        stream());
+        colsum_partials(part.data_ptr<float>(), ceil_div(n, 32), V, 1.f, out.dbias.data_ptr<float>(),
+                        db_accumulate || k > 0, stream());
     } else {
-      if (pieces > 1) logits(col0, n);
-      ce_piece_grad(r, z.data_ptr<float>(), piece, col0, n, norm, gscale,
-                    bf ? reinterpret_cast<__nv_bfloat16*>(dl.data_ptr()) : nullptr, stream());
-      if (part.defined()) {  // the columns past n are left over from nothing: only n of the sums are kept
-        const int64_t ns = colsum_scratch_floats(N, piece);
+      ce_memory_grad(r, z.data_ptr<float>(), ldv, norm, gscale,
+                     bf ? reinterpret_cast<__nv_bfloat16*>(dl.data_ptr()) : nullptr, stream());
+      if (part.defined()) {  // the padding's columns are summed too and left out of the copy
+        const int64_t ns = colsum_scratch_floats(n, ldv);
         const at::Tensor scr = ns > 0 ? at::empty({ns}, f32) : at::Tensor();
-        colsum(DType::F32, DType::F32, z.data_ptr(), N, piece, 1.f, part.data_ptr<float>(), false,
+        colsum(DType::F32, DType::F32, z.data_ptr(), n, ldv, 1.f, part.data_ptr<float>(), false,
                ns > 0 ? scr.data_ptr<float>() : nullptr, stream());
-        copy_matrix(DType::F32, DType::F32, part.data_ptr(), 0, 1, out.dbias.data_ptr<float>() + col0, n, 1, n, n,
-                    db_accumulate, stream());
+        copy_matrix(DType::F32, DType::F32, part.data_ptr(), 0, 1, out.dbias.data_ptr<float>(), V, 1, V, V,
+                    db_accumulate || k > 0, stream());
       }
     }
-    const Operand d = parts ? split(dl.narrow(1, 0, n)) : Operand{dl.narrow(1, 0, n), {}, {}};
-    const Operand wp = wo.columns(col0, n);
-    if (pieces == 1) product_into(d, wp.t(), out.dx, false);
-    else product_into(d, wp.t(), sum, k > 0);
-    const at::Tensor dwp = out.dw.narrow(1, col0, n);
-    if (dw_k) product_into(d.t(), xco, dwp.t(), dw_accumulate);
-    else product_into(xco.t(), d, dwp, dw_accumulate);
+    const Operand d = whole(dl.narrow(0, 0, n).narrow(1, 0, V)), xo = whole(xc.narrow(0, 0, n));
+    product_into(d, wo.t(), out.dx.narrow(0, r0, n), false);
+    const bool add = dw32.defined() ? k > 0 : (dw_accumulate || k > 0);
+    if (dw_k) product_into(d.t(), xo, dw.t(), add);
+    else product_into(xo.t(), d, dw, add);
   }
-  if (pieces > 1) unary(DType::F32, to_dtype(x), sum.data_ptr(), out.dx.data_ptr(), N * E, UN_COPY, 0.f, 0.f, stream());
+  if (dw32.defined()) {
+    const at::Tensor src = dw_k ? dw32.t() : dw32, dst = dw_k ? out.dw.t() : out.dw;
+    if (src.is_contiguous() && dst.is_contiguous())
+      unary(DType::F32, to_dtype(dst), src.data_ptr(), dst.data_ptr(), src.numel(), UN_COPY, 0.f, 0.f, stream());
+    else
+      copy_matrix(to_dtype(dst), DType::F32, src.data_ptr(), src.stride(0), 1, dst.data_ptr(), dst.stride(0),
+                  dst.size(0), dst.size(1), dst.size(1), false, stream());
+  }
   return out;
 }
 

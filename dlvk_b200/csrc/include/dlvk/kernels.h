@@ -311,16 +311,20 @@ struct CeProjection {
   float* zlabel = nullptr;           // [rows], written for rows that count
   const float2* norm = nullptr;      // [rows] maximum and 1 / sum, for the gradient
   const float* gscale = nullptr;     // device scalar: gradient w.r.t. a counted row's loss
-  unsigned* done = nullptr;          // set to 0 by ce_stats_tc, for ce_finish
+  unsigned* done = nullptr;          // set to 0 with the statistics (or null)
 };
 bool ce_tc_supported(const CeProjection& c);
+// The statistics have one column per ce_tc_stat_width() classes.
+int ce_tc_stat_width(int64_t rows, int64_t classes);
 int ce_tc_stat_cols(int64_t rows, int64_t classes);
 void ce_stats_tc(const CeProjection& c, cudaStream_t s, uint32_t* err);
-// dl[:, 0 : n] = (softmax - onehot) * gscale of the classes [col0, col0 + n),
-// bf16, row stride ldd; colsum (or null): its fp32 column sums per 32 rows
-// [ceil(rows / 32)][n], for colsum_partials.
-void ce_grad_tc(const CeProjection& c, int col0, int n, __nv_bfloat16* dl, int64_t ldd, float* colsum, cudaStream_t s,
-                uint32_t* err);
+// The statistics, and e = 2^15 exp(z - the maximum of its statistics column),
+// fp16 [rows, classes], row stride lde.
+void ce_exp_tc(const CeProjection& c, void* e, int64_t lde, cudaStream_t s, uint32_t* err);
+// dl [rows, classes] = (softmax - onehot) * gscale, bf16, row stride ldd;
+// colsum (or null): its fp32 column sums per 32 rows [ceil(rows / 32)][classes],
+// for colsum_partials.
+void ce_grad_tc(const CeProjection& c, __nv_bfloat16* dl, int64_t ldd, float* colsum, cudaStream_t s, uint32_t* err);
 // The passes around them, and the same statistics / gradient from logits in
 // memory (vocab_loss.cu).
 struct CeRows {
@@ -328,21 +332,44 @@ struct CeRows {
   const void* labels = nullptr;
   bool labels64 = false;
 };
-// Joins the statistics: rows_loss (0 where a row does not count), norm; the
-// last block to finish sums them: *loss = sum (mean: / counted rows),
-// *gscale = (mean: 1 / counted) * (*grad_scale or 1), *correct += rows whose
-// class has the largest logit.  partial: 3 doubles per 32 rows.  `done` was
-// set to 0 by the statistics' launch.  With x_clean: a copy of x whose uncounted rows are 0.
-void ce_finish(const CeRows& r, const float2* stats, int stat_cols, const float* zlabel, float* rows_loss, float2* norm,
-               bool mean, const float* grad_scale, float* loss, float* gscale, unsigned long long* correct,
-               double* partial, unsigned* done, DType dt, const void* x, int64_t ldx, int64_t width, void* x_clean,
-               int64_t ldc, cudaStream_t s);
-// One (maximum, sum) per row from logits z [rows, n] fp32 of the classes from col0 on.
-void ce_piece_stats(const CeRows& r, const float* z, int64_t ldz, int64_t col0, int64_t n, float2* stats,
-                    float* zlabel, unsigned* done, cudaStream_t s);
-// z becomes the gradient in place; dl (or null) its bf16 copy, row stride ldz.
-void ce_piece_grad(const CeRows& r, float* z, int64_t ldz, int64_t col0, int64_t n, const float2* norm,
-                   const float* gscale, __nv_bfloat16* dl, cudaStream_t s);
+// *gscale = (mean: 1 / counted rows, else 1) * (*grad_scale or 1); *done = 0.
+void ce_count(const CeRows& r, bool mean, const float* grad_scale, float* gscale, unsigned* done, cudaStream_t s);
+// Joins the statistics of one block of rows: rows_loss (0 where a row does
+// not count) and norm; x_clean, when given, becomes a copy of x whose
+// uncounted rows are 0.  The last of all `total_groups` groups of 32 rows (of
+// every block of rows; this one's are first_group onwards) adds up the
+// losses: *loss = sum (mean: / counted rows), *correct += rows whose class has
+// the largest logit, and, when set_gscale, *gscale as ce_count's.
+// partial: 3 doubles per group.  `done` was set to 0 before the first block.
+struct CeFinish {
+  const float2* stats;
+  int stat_cols;
+  const float* zlabel;
+  float* rows_loss;
+  float2* norm;
+  bool mean, set_gscale;
+  const float* grad_scale;
+  float *loss, *gscale;
+  unsigned long long* correct;
+  double* partial;
+  unsigned* done;
+  int first_group, total_groups;
+  const void* x;
+  int64_t ldx, width;
+  void* x_clean;
+  int64_t ldc;
+};
+void ce_finish(const CeRows& r, const CeFinish& f, DType dt, cudaStream_t s);
+// e (ce_exp_tc's, fp16) becomes the gradient (softmax - onehot) * gscale in
+// place, bf16; stat_width classes to a statistics column.
+void ce_rescale(const CeRows& r, const float2* stats, int stat_width, const float2* norm, const float* gscale, void* e,
+                int64_t lde, cudaStream_t s);
+// Statistics (one column) and gradient (in place; dl, or null, its bf16 copy)
+// of logits z [rows, classes] fp32; row strides ldz.
+void ce_memory_stats(const CeRows& r, const float* z, int64_t ldz, float2* stats, float* zlabel, unsigned* done,
+                     cudaStream_t s);
+void ce_memory_grad(const CeRows& r, float* z, int64_t ldz, const float2* norm, const float* gscale, __nv_bfloat16* dl,
+                    cudaStream_t s);
 // dst [rows, cols] (row stride ldd) = src (strides rs, cs), or += (accumulate);
 // columns [cols, pad_to) become 0.  fp32 or bf16 each.
 void copy_matrix(DType dst_dt, DType src_dt, const void* src, int64_t rs, int64_t cs, void* dst, int64_t ldd,

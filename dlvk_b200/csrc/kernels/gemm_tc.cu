@@ -20,6 +20,7 @@
 //  * every mbarrier wait is bounded (2 s) and reports through `err`.
 #include <cuda.h>
 #include <cudaTypedefs.h>
+#include <cuda_fp16.h>
 #include <cstdlib>
 #include <cstring>
 #include <mutex>
@@ -45,12 +46,11 @@ struct CeEpilogue {
   int labels64;
   int64_t ignore;      // a class that does not count (-1: none)
   int64_t classes;     // classes of the whole vocabulary; others do not count
-  int col0;            // class of this launch's first column
-  float2* stats;       // EPI 3: [column half tiles][M] (maximum, sum)
-  float* zlabel;       // EPI 3: the logit of each row's class
+  float2* stats;       // EPI 3, 5: [column half tiles][M] (maximum, sum)
+  float* zlabel;       // EPI 3, 5: the logit of each row's class
   const float2* norm;  // EPI 4: each row's maximum and 1 / sum of exp(z - maximum)
   const float* gscale; // EPI 4: gradient of the loss w.r.t. each counted row's loss
-  unsigned* done;      // EPI 3: set to 0
+  unsigned* done;      // EPI 3, 5: set to 0 (or null)
 };
 
 struct TcParams {
@@ -490,7 +490,14 @@ __device__ __forceinline__ void epi_store(const TcParams& p, const float* stg, i
 // The products of a vocabulary projection are consumed where they are made:
 // EPI 3 reduces each row's logits to a running maximum and sum, EPI 4 turns
 // them into the gradient (softmax - onehot) * scale, rounded once to bf16.
-// A thread owns one row of the tile, so neither needs a shuffle.
+// EPI 5 does what EPI 3 does and stores exp(z - maximum), the maximum being
+// that of the thread's half of the tile's columns, from which the gradient
+// needs no second product.  A thread owns one row of the tile, so none of
+// them needs a shuffle.
+// EPI 5 rounds to fp16 after a factor of 2^15: the values lie in (0, 1], so
+// they keep 11 bits down to 2e-9 of the largest and some down to 1e-12, where
+// bf16 would round every one of them as coarsely as the gradient itself.
+constexpr float CE_EXP_SCALE = 32768.f;
 constexpr float LOG2E = 1.4426950408889634f;
 
 __device__ __forceinline__ float ex2(float x) {
@@ -519,12 +526,8 @@ __device__ __forceinline__ void ce_logits(const TcParams& p, const uint32_t* r, 
   }
 }
 
-// Folds 32 logits into the running (maximum, sum of exp(z - maximum)).  A
-// maximum of -inf (every logit so far masked) is replaced by 0 in the
-// exponents, which then are exp(-inf) = 0; a NaN logit makes the sum NaN.
-// The maximum is taken off before the scaling to powers of 2, in a step of
-// its own: -3.4e38 (a mask of fp32's lowest value) times log2 e would be -inf.
-__device__ __forceinline__ void ce_online(const float* v, float& m, float& s) {
+// Maximum of 32 logits and m.
+__device__ __forceinline__ float ce_max(const float* v, float m) {
   float t[16];
 #pragma unroll
   for (int j = 0; j < 16; ++j) t[j] = fmaxf(v[j], v[j + 16]);
@@ -532,7 +535,16 @@ __device__ __forceinline__ void ce_online(const float* v, float& m, float& s) {
   for (int h = 8; h >= 1; h >>= 1)
 #pragma unroll
     for (int j = 0; j < h; ++j) t[j] = fmaxf(t[j], t[j + h]);
-  const float mn = fmaxf(m, t[0]);
+  return fmaxf(m, t[0]);
+}
+
+// Folds 32 logits into the running (maximum, sum of exp(z - maximum)).  A
+// maximum of -inf (every logit so far masked) is replaced by 0 in the
+// exponents, which then are exp(-inf) = 0; a NaN logit makes the sum NaN.
+// The maximum is taken off before the scaling to powers of 2, in a step of
+// its own: -3.4e38 (a mask of fp32's lowest value) times log2 e would be -inf.
+__device__ __forceinline__ void ce_online(const float* v, float& m, float& s) {
+  const float mn = ce_max(v, m);
   const float c = mn == -INFINITY ? 0.f : mn;
   s *= ex2((m - c) * LOG2E);
   float a[4] = {0.f, 0.f, 0.f, 0.f};
@@ -540,6 +552,29 @@ __device__ __forceinline__ void ce_online(const float* v, float& m, float& s) {
   for (int j = 0; j < 32; ++j) a[j & 3] += ex2((v[j] - c) * LOG2E);
   s += (a[0] + a[1]) + (a[2] + a[3]);
   m = mn;
+}
+
+// v = 2^15 exp(v - m); s += the sum of exp(v - m).
+__device__ __forceinline__ void ce_exponentials(float m, float& s, float* v) {
+  float a[4] = {0.f, 0.f, 0.f, 0.f};
+  const float c = m == -INFINITY ? 0.f : m;
+#pragma unroll
+  for (int j = 0; j < 32; ++j) {
+    v[j] = ex2((v[j] - c) * LOG2E);
+    a[j & 3] += v[j];
+    v[j] *= CE_EXP_SCALE;
+  }
+  s += (a[0] + a[1]) + (a[2] + a[3]);
+}
+
+// The logit of the row's class, when it is one of these 32.
+__device__ __forceinline__ void ce_pick(const TcParams& p, int row, int at, const float* v) {
+  if ((unsigned)at < 32u) {  // a class of -1 gives a negative place
+    float z = v[0];
+#pragma unroll
+    for (int j = 1; j < 32; ++j) z = j == at ? v[j] : z;
+    p.ce.zlabel[row] = z;
+  }
 }
 
 // v[j] = (softmax - onehot) * g, for a row that does not count 0 whatever its
@@ -563,7 +598,7 @@ __device__ __forceinline__ void ce_gradient(float m, float f, float g, int at, f
 // otherwise misses in the instruction cache.  EPI = 2 is that path with
 // alpha, bias and activation only.  EPI = 0 has every path.  EPI = 3 stores
 // nothing but each row's softmax statistics, EPI = 4 the cross entropy's
-// gradient as bf16 boxes.
+// gradient as bf16 boxes, EPI = 5 statistics and exponentials as fp16 boxes.
 template <int BN, bool PAIR = false, int EPI = 0>
 __global__ void __launch_bounds__(320, 1)
     gemm_tc_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
@@ -627,8 +662,8 @@ __global__ void __launch_bounds__(320, 1)
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
   pdl_wait();  // the previous kernel's outputs (our operands) are complete from here on
-  if constexpr (EPI == 3) {
-    if (blockIdx.x == 0 && threadIdx.x == 0) *p.ce.done = 0u;
+  if constexpr (EPI == 3 || EPI == 5) {
+    if (blockIdx.x == 0 && threadIdx.x == 0 && p.ce.done != nullptr) *p.ce.done = 0u;
   }
   GEMM_STAMP(threadIdx.x == 0, 5);
 
@@ -900,6 +935,21 @@ __global__ void __launch_bounds__(320, 1)
           ce_s = norm.y * ce_g;
         }
       }
+      if constexpr (EPI == 5) {  // the maximum first: the accumulators are read twice
+#pragma unroll 2
+        for (int i = 0; i < NCH; ++i) {
+          if (i + 1 < NCH) tmem_ld32(tbase + (uint32_t)((i + 1) * 32), r[(i + 1) & 1]);
+          const int n0 = tn * BN + (half * NCH + i) * 32;
+          if (n0 < p.N) {
+            float v[32];
+            ce_logits(p, r[i & 1], n0, v);
+            ce_m = ce_max(v, ce_m);
+          }
+          if (i + 1 < NCH) tmem_ld_wait();
+        }
+        tmem_ld32(tbase, r[0]);
+        tmem_ld_wait();
+      }
       // Unrolled by two (the register double buffer needs the chunk parity at
       // compile time), not fully: eight full copies of the chunk body for the
       // 512-column tile make the epilogue's code large.
@@ -913,13 +963,7 @@ __global__ void __launch_bounds__(320, 1)
             float v[32];
             ce_logits(p, r[i & 1], n0, v);
             ce_online(v, ce_m, ce_s);
-            const int at = ce_lab - n0;
-            if ((unsigned)at < 32u) {  // ce_lab = -1 gives a negative place
-              float z = v[0];
-#pragma unroll
-              for (int j = 1; j < 32; ++j) z = j == at ? v[j] : z;
-              p.ce.zlabel[row0 + lane] = z;
-            }
+            ce_pick(p, row0 + lane, ce_lab - n0, v);
           }
         } else if (EPI == 0 && staged) {
 #pragma unroll
@@ -930,7 +974,7 @@ __global__ void __launch_bounds__(320, 1)
             else epi_store<__nv_bfloat16, 8>(p, stg, row0, n0, lane, cb, rb, mb);
           }
           __syncwarp();
-        } else if (EPI == 1 || EPI == 4 || p.tma_c) {
+        } else if (EPI == 1 || EPI >= 4 || p.tma_c) {
           // Row `lane` of this warp's box goes to smem and one lane stores the
           // box with TMA (rows >= M / columns >= N are clipped).  fp32: one
           // 32 x 32 box (128-byte rows) per chunk.  bf16: chunks i, i+1 fill
@@ -946,7 +990,11 @@ __global__ void __launch_bounds__(320, 1)
             const float rbv = (EPI < 2 && p.row_bias && row0 + lane < p.M) ? p.row_bias[row0 + lane] : 0.f;
             if constexpr (EPI == 4) {
               ce_logits(p, r[i & 1], n0, v);
-              ce_gradient(ce_m, ce_s, ce_g, ce_lab < 0 ? CE_ROW_OUT : ce_lab - p.ce.col0 - n0, v);
+              ce_gradient(ce_m, ce_s, ce_g, ce_lab < 0 ? CE_ROW_OUT : ce_lab - n0, v);
+            } else if constexpr (EPI == 5) {
+              ce_logits(p, r[i & 1], n0, v);
+              ce_pick(p, row0 + lane, ce_lab - n0, v);
+              ce_exponentials(ce_m, ce_s, v);
             } else {
 #pragma unroll
               for (int j = 0; j < 32; ++j) v[j] = fmaf(__uint_as_float(r[i & 1][j]), p.alpha, rbv);
@@ -988,14 +1036,19 @@ __global__ void __launch_bounds__(320, 1)
                 uint32_t w[4];
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
-                  const __nv_bfloat162 h = __floats2bfloat162_rn(v[8 * j + 2 * k], v[8 * j + 2 * k + 1]);
-                  w[k] = *reinterpret_cast<const uint32_t*>(&h);
+                  if constexpr (EPI == 5) {
+                    const __half2 h = __floats2half2_rn(v[8 * j + 2 * k], v[8 * j + 2 * k + 1]);
+                    w[k] = *reinterpret_cast<const uint32_t*>(&h);
+                  } else {
+                    const __nv_bfloat162 h = __floats2bfloat162_rn(v[8 * j + 2 * k], v[8 * j + 2 * k + 1]);
+                    w[k] = *reinterpret_cast<const uint32_t*>(&h);
+                  }
                 }
                 const uint32_t a = bb + (uint32_t)((i & 1) * 4 + j) * 16u;
                 st_shared_v4(a ^ (((a >> 7) & 7u) << 4), w[0], w[1], w[2], w[3]);
               }
             }
-            if (BN != 512 && EPI != 2 && EPI != 3 && p.colsum) {  // after the box write: consumes v (512-wide tiles: never, see host)
+            if (BN != 512 && (EPI < 2 || EPI == 4) && p.colsum) {  // after the box write: consumes v (512-wide tiles: never, see host)
               if (row0 + lane >= p.M) {
 #pragma unroll
                 for (int j = 0; j < 32; ++j) v[j] = 0.f;
@@ -1072,7 +1125,7 @@ __global__ void __launch_bounds__(320, 1)
         }
         if (i + 1 < NCH) tmem_ld_wait();
       }
-      if constexpr (EPI == 3) {
+      if constexpr (EPI == 3 || EPI == 5) {
         if (row0 + lane < p.M)
           p.ce.stats[(int64_t)(2 * tn + half) * p.M + row0 + lane] = make_float2(ce_m, ce_s);
       }
@@ -1782,52 +1835,48 @@ CeTiling ce_tiling(int64_t M, int64_t N) {
   return {false, (N + 255) / 256 * ((M + BM - 1) / BM) >= sm_count() ? 256 : 128};
 }
 
-void ce_launch(const CeProjection& c, bool grad, int n, int col0, __nv_bfloat16* dl, int64_t ldd, float* colsum,
-               cudaStream_t s, uint32_t* err) {
+template <int EPI>
+void ce_launch(const CeProjection& c, void* out, int64_t ldo, float* colsum, cudaStream_t s, uint32_t* err) {
+  DLVK_CHECK(ce_tc_supported(c) && (EPI == 3 || (ldo % 8 == 0 && al16(out))), "cross entropy: unsupported layout");
   tmap::bind_context();
-  // the statistics run over all classes at once, so both passes tile alike
   const CeTiling t = ce_tiling(c.rows, c.classes);
-  const __nv_bfloat16* w = c.w + (c.w_k ? (int64_t)col0 * c.ldw : col0);
   const uint64_t da = (uint64_t)c.ldx * (uint64_t)c.rows;
   const CUtensorMap ta = make_tmap(c.x, c.width, c.rows, 1, 1, c.ldx, da, da, BM, Elem::BF16);
   CUtensorMap tb;
   if (c.w_k) {
-    const uint64_t d = (uint64_t)c.ldw * (uint64_t)n;
-    tb = make_tmap(w, c.width, n, 1, 1, c.ldw, d, d, t.pair ? 128 : t.bn, Elem::BF16);
+    const uint64_t d = (uint64_t)c.ldw * (uint64_t)c.classes;
+    tb = make_tmap(c.w, c.width, c.classes, 1, 1, c.ldw, d, d, t.pair ? 128 : t.bn, Elem::BF16);
   } else {
     const uint64_t d = (uint64_t)c.ldw * (uint64_t)c.width;
-    tb = make_tmap(w, n, c.width, 1, 1, c.ldw, d, d, BK, Elem::BF16, true);
+    tb = make_tmap(c.w, c.classes, c.width, 1, 1, c.ldw, d, d, BK, Elem::BF16, true);
   }
   TcParams p{};
   p.M = (int)c.rows;
-  p.N = n;
+  p.N = (int)c.classes;
   p.K = (int)c.width;
   p.batch = p.batch2 = 1;
   p.tiles_m = (int)((c.rows + (t.pair ? 2 * BM : BM) - 1) / (t.pair ? 2 * BM : BM));
-  p.tiles_n = (n + t.bn - 1) / t.bn;
+  p.tiles_n = (int)((c.classes + t.bn - 1) / t.bn);
   p.b_mn = c.w_k ? 0 : 1;
   p.alpha = 1.f;
-  p.bias = c.bias ? c.bias + col0 : nullptr;
+  p.bias = c.bias;
   p.bias_f32 = 1;
   p.err = err;
   p.splits = 1;
   p.kb_per_split = (int)((c.width + BK - 1) / BK);
-  p.ce = {c.labels, c.labels64 ? 1 : 0, c.ignore, c.classes, col0, c.stats, c.zlabel, c.norm, c.gscale, c.done};
-  if (!grad) {
-    if (t.pair) launch_tc_pair_k<256, 3>(ta, tb, ta, p, 0, s);
-    else if (t.bn == 256) launch_tc_k<256, 3>(ta, tb, ta, p, 0, s);
-    else launch_tc_k<128, 3>(ta, tb, ta, p, 0, s);
-    return;
+  p.ce = {c.labels, c.labels64 ? 1 : 0, c.ignore, c.classes, c.stats, c.zlabel, c.norm, c.gscale, c.done};
+  CUtensorMap tc = ta;
+  if (EPI >= 4) {  // 16-bit boxes (fp16 bits are stored as they are)
+    p.C = out;
+    p.ldc = ldo;
+    p.vec_ok = 1;
+    p.colsum = colsum;
+    tc = make_c_map(p, c.rows, c.classes);
+    DLVK_CHECK(p.tma_c == 1, "cross entropy: the output's tile map was refused");
   }
-  p.C = dl;
-  p.ldc = ldd;
-  p.vec_ok = 1;
-  p.colsum = colsum;
-  const CUtensorMap tc = make_c_map(p, c.rows, n);
-  DLVK_CHECK(p.tma_c == 1, "cross entropy gradient: its tile map was refused");
-  if (t.pair) launch_tc_pair_k<256, 4>(ta, tb, tc, p, 0, s);
-  else if (t.bn == 256) launch_tc_k<256, 4>(ta, tb, tc, p, 0, s);
-  else launch_tc_k<128, 4>(ta, tb, tc, p, 0, s);
+  if (t.pair) launch_tc_pair_k<256, EPI>(ta, tb, tc, p, 0, s);
+  else if (t.bn == 256) launch_tc_k<256, EPI>(ta, tb, tc, p, 0, s);
+  else launch_tc_k<128, EPI>(ta, tb, tc, p, 0, s);
 }
 }  // namespace
 
@@ -1837,20 +1886,18 @@ bool ce_tc_supported(const CeProjection& c) {
          ((c.rows + 127) / 128) * ((c.classes + 127) / 128) < (1LL << 31) && tma_c_enabled();
 }
 
+int ce_tc_stat_width(int64_t rows, int64_t classes) { return ce_tiling(rows, classes).bn / 2; }
 int ce_tc_stat_cols(int64_t rows, int64_t classes) {
   const int bn = ce_tiling(rows, classes).bn;
   return (int)(2 * ((classes + bn - 1) / bn));
 }
 
-void ce_stats_tc(const CeProjection& c, cudaStream_t s, uint32_t* err) {
-  DLVK_CHECK(ce_tc_supported(c), "ce_stats_tc: unsupported layout");
-  ce_launch(c, false, (int)c.classes, 0, nullptr, 0, nullptr, s, err);
+void ce_stats_tc(const CeProjection& c, cudaStream_t s, uint32_t* err) { ce_launch<3>(c, nullptr, 0, nullptr, s, err); }
+void ce_exp_tc(const CeProjection& c, void* e, int64_t lde, cudaStream_t s, uint32_t* err) {
+  ce_launch<5>(c, e, lde, nullptr, s, err);
 }
-
-void ce_grad_tc(const CeProjection& c, int col0, int n, __nv_bfloat16* dl, int64_t ldd, float* colsum, cudaStream_t s,
-                uint32_t* err) {
-  DLVK_CHECK(ce_tc_supported(c) && col0 % 8 == 0 && ldd % 8 == 0 && al16(dl), "ce_grad_tc: unsupported layout");
-  ce_launch(c, true, n, col0, dl, ldd, colsum, s, err);
+void ce_grad_tc(const CeProjection& c, __nv_bfloat16* dl, int64_t ldd, float* colsum, cudaStream_t s, uint32_t* err) {
+  ce_launch<4>(c, dl, ldd, colsum, s, err);
 }
 
 void gemm_tc_set_pair(bool on) { pair_flag() = on ? 1 : 0; }

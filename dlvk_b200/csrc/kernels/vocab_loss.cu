@@ -6,14 +6,19 @@
 //   dz_iv = (exp(z_iv) / sum - [v = label]) * g      dx = dz W^T   dW = x^T dz   db = sum_i dz
 //
 // The reference computes the loss from stored probabilities
-// (src/loss/loss_functions.cpp:127-160).  Here the logits of the whole
-// vocabulary never reach memory: a first product keeps a maximum and a sum
-// per row and 128 (64) classes, ce_finish joins them, and a second product
-// makes the logits again, a piece of the vocabulary at a time, and leaves only
-// their gradient, which the two gradient products then read.  That is four
-// products for the three that the gradient cannot do without; what it saves
-// is two [rows, classes] arrays and a pass over each.
+// (src/loss/loss_functions.cpp:127-160).  Here the logits of the vocabulary
+// are taken a tile of 256 words at a time: the first product's epilogue keeps
+// a maximum and a sum per row and 128 words, ce_finish joins them.  For the
+// gradients a block of rows at a time leaves exp(z - local maximum) behind
+// (16 bits, at most 256 MB whatever the batch), ce_rescale turns those into
+// dz, and the two gradient products read dz: three products, one pass over
+// the block.  Making the logits a second time instead costs a fourth product
+// (8192 x 1024 x 32000: 434 us against 2 x 85 us for the pass); it is
+// what a bias gradient takes, whose fp32 sums 16-bit exponentials are too
+// coarse for.
 #include <algorithm>
+
+#include <cuda_fp16.h>
 
 #include "dlvk/common.h"
 #include "dlvk/kernels.h"
@@ -40,97 +45,110 @@ __device__ __forceinline__ void join(float& m, float& s, float m2, float s2) {
   m = mn;
 }
 
-constexpr int FIN_ROWS = 32;
+// 1 / counted rows (mean) or 1; no row counts: the loss and every gradient are 0.
+__device__ __forceinline__ double share_of(int mean, double counted) {
+  return mean ? (counted > 0.0 ? 1.0 / counted : 0.0) : 1.0;
+}
 
-// A block joins 32 rows (lane = row, warps share the columns), copies their x
-// rows when asked, and adds up their losses; the block that comes last adds
-// the blocks' sums in their order.
+__global__ void __launch_bounds__(1024) count_kernel(CeRows r, int mean, const float* __restrict__ grad_scale,
+                                                     float* __restrict__ gscale, unsigned* __restrict__ done) {
+  __shared__ int sm[32];
+  int n = 0;
+  for (int64_t i = threadIdx.x; i < r.rows; i += 1024) n += row_label(r, i) >= 0;
+  n = __reduce_add_sync(0xffffffffu, n);
+  if ((threadIdx.x & 31) == 0) sm[threadIdx.x >> 5] = n;
+  __syncthreads();
+  if (threadIdx.x < 32) {
+    n = __reduce_add_sync(0xffffffffu, sm[threadIdx.x]);
+    if (threadIdx.x == 0) {
+      *gscale = (float)(share_of(mean, n) * (grad_scale ? (double)*grad_scale : 1.0));
+      *done = 0u;
+    }
+  }
+}
+
+constexpr int FIN_ROWS = 32, FIN_WARPS = 16;
+
+// A block joins 32 rows (lane = row, the warps share the columns), copies
+// their x rows when asked, and adds up their losses; the block that comes
+// last of all adds the blocks' sums in their order.
 template <typename T>
-__global__ void __launch_bounds__(256) finish_kernel(CeRows r, const float2* __restrict__ stats, int cols,
-                                                     const float* __restrict__ zlabel, float* __restrict__ rows_loss,
-                                                     float2* __restrict__ norm, int mean,
-                                                     const float* __restrict__ grad_scale, float* __restrict__ loss,
-                                                     float* __restrict__ gscale,
-                                                     unsigned long long* __restrict__ correct,
-                                                     double* __restrict__ partial, unsigned* __restrict__ done,
-                                                     const T* __restrict__ x, int64_t ldx, int64_t width,
-                                                     T* __restrict__ x_clean, int64_t ldc, int vec) {
-  __shared__ float sm_m[8][FIN_ROWS], sm_s[8][FIN_ROWS];
+__global__ void __launch_bounds__(FIN_WARPS * 32) finish_kernel(CeRows r, CeFinish f, int vec) {
+  __shared__ float sm_m[FIN_WARPS][FIN_ROWS], sm_s[FIN_WARPS][FIN_ROWS];
   __shared__ int counted[FIN_ROWS];
   __shared__ int last;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t row0 = (int64_t)blockIdx.x * FIN_ROWS, row = row0 + lane;
   float m = -INFINITY, s = 0.f;
   if (row < r.rows) {
-    int c = warp;
-    for (; c + 24 < cols; c += 32) {
-      float2 v[4];
+    for (int c = warp; c < f.stat_cols; c += 8 * FIN_WARPS) {
+      float2 v[8];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) v[k] = stats[(int64_t)(c + 8 * k) * r.rows + row];
+      for (int k = 0; k < 8; ++k)
+        v[k] = c + k * FIN_WARPS < f.stat_cols ? f.stats[(int64_t)(c + k * FIN_WARPS) * r.rows + row]
+                                               : make_float2(-INFINITY, 0.f);
 #pragma unroll
-      for (int k = 0; k < 4; ++k) join(m, s, v[k].x, v[k].y);
-    }
-    for (; c < cols; c += 8) {
-      const float2 v = stats[(int64_t)c * r.rows + row];
-      join(m, s, v.x, v.y);
+      for (int k = 0; k < 8; ++k) join(m, s, v[k].x, v[k].y);
     }
   }
   sm_m[warp][lane] = m;
   sm_s[warp][lane] = s;
+  if (warp == 1) counted[lane] = row < r.rows && row_label(r, row) >= 0;
   __syncthreads();
   if (warp == 0) {
-    for (int w = 1; w < 8; ++w) join(m, s, sm_m[w][lane], sm_s[w][lane]);
-    int lab = -1, hit = 0;
+    for (int w = 1; w < FIN_WARPS; ++w) join(m, s, sm_m[w][lane], sm_s[w][lane]);
+    int hit = 0;
     float l = 0.f;
     if (row < r.rows) {
-      lab = row_label(r, row);
-      norm[row] = make_float2(m, 1.f / s);
-      if (lab >= 0) {
-        const float z = zlabel[row];
+      f.norm[row] = make_float2(m, 1.f / s);
+      if (counted[lane]) {
+        const float z = f.zlabel[row];
         l = (m - z) + logf(s);
         hit = z >= m;
       }
-      rows_loss[row] = l;
+      f.rows_loss[row] = l;
     }
-    counted[lane] = lab >= 0;
     double d = l;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) d += __shfl_xor_sync(0xffffffffu, d, o);
-    const int n = __popc(__ballot_sync(0xffffffffu, lab >= 0));
+    const int n = __popc(__ballot_sync(0xffffffffu, counted[lane]));
     const int h = __popc(__ballot_sync(0xffffffffu, hit));
     if (lane == 0) {
-      partial[3 * blockIdx.x] = d;
-      partial[3 * blockIdx.x + 1] = n;
-      partial[3 * blockIdx.x + 2] = h;
+      double* p = f.partial + 3 * ((int64_t)f.first_group + blockIdx.x);
+      p[0] = d;
+      p[1] = n;
+      p[2] = h;
       __threadfence();
-      last = atomicAdd(done, 1u) == gridDim.x - 1;
+      last = atomicAdd(f.done, 1u) == (unsigned)f.total_groups - 1u;
     }
   }
-  __syncthreads();
-  if (x_clean != nullptr) {
-    for (int k = warp; k < FIN_ROWS && row0 + k < r.rows; k += 8) {
-      const T* src = x + (row0 + k) * ldx;
-      T* dst = x_clean + (row0 + k) * ldc;
+  if (f.x_clean != nullptr) {
+    const T* x = reinterpret_cast<const T*>(f.x);
+    T* y = reinterpret_cast<T*>(f.x_clean);
+    for (int k = warp; k < FIN_ROWS && row0 + k < r.rows; k += FIN_WARPS) {
+      const T* src = x + (row0 + k) * f.ldx;
+      T* dst = y + (row0 + k) * f.ldc;
       if (vec) {  // rows of whole 16-byte steps
         constexpr int V = 16 / (int)sizeof(T);
-        for (int64_t c = lane * V; c < width; c += 32 * V)
+        for (int64_t c = lane * V; c < f.width; c += 32 * V)
           *reinterpret_cast<uint4*>(dst + c) =
               counted[k] ? *reinterpret_cast<const uint4*>(src + c) : make_uint4(0u, 0u, 0u, 0u);
       } else {
-        for (int64_t c = lane; c < width; c += 32) dst[c] = counted[k] ? src[c] : from_f32<T>(0.f);
+        for (int64_t c = lane; c < f.width; c += 32) dst[c] = counted[k] ? src[c] : from_f32<T>(0.f);
       }
     }
   }
+  __syncthreads();
   if (!last) return;
   // every block's sums are visible: their writers fenced before they counted
   __threadfence();
   double d = 0.0, n = 0.0, h = 0.0;
-  for (unsigned b = threadIdx.x; b < gridDim.x; b += 256) {
-    d += __ldcg(partial + 3 * b);
-    n += __ldcg(partial + 3 * b + 1);
-    h += __ldcg(partial + 3 * b + 2);
+  for (int b = threadIdx.x; b < f.total_groups; b += FIN_WARPS * 32) {
+    d += __ldcg(f.partial + 3 * (int64_t)b);
+    n += __ldcg(f.partial + 3 * (int64_t)b + 1);
+    h += __ldcg(f.partial + 3 * (int64_t)b + 2);
   }
-  __shared__ double sm_d[3][8];
+  __shared__ double sm_d[3][FIN_WARPS];
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
     d += __shfl_xor_sync(0xffffffffu, d, o);
@@ -145,33 +163,96 @@ __global__ void __launch_bounds__(256) finish_kernel(CeRows r, const float2* __r
   __syncthreads();
   if (threadIdx.x == 0) {
     d = n = h = 0.0;
-    for (int w = 0; w < 8; ++w) {
+    for (int w = 0; w < FIN_WARPS; ++w) {
       d += sm_d[0][w];
       n += sm_d[1][w];
       h += sm_d[2][w];
     }
-    // no row counts: the loss and every gradient are 0
-    const double share = mean ? (n > 0.0 ? 1.0 / n : 0.0) : 1.0;
-    *loss = (float)(d * share);
-    *gscale = (float)(share * (grad_scale ? (double)*grad_scale : 1.0));
-    if (correct) *correct += (unsigned long long)h;
+    const double share = share_of(f.mean, n);
+    *f.loss = (float)(d * share);
+    if (f.set_gscale) *f.gscale = (float)(share * (f.grad_scale ? (double)*f.grad_scale : 1.0));
+    if (f.correct) *f.correct += (unsigned long long)h;
+  }
+}
+
+// e -> dz in place.  A block has 32 rows of 2048 classes, a thread 8 classes
+// of each; what a row's 2^-15 e is multiplied by, exp(local maximum - maximum)
+// / sum * g, is made once per row and statistics column.  Bound by HBM: 2
+// bytes in, 2 out per logit.
+constexpr int RS_COLS = 2048, RS_ROWS = 32;
+__global__ void __launch_bounds__(256) rescale_kernel(CeRows r, const float2* __restrict__ stats, int width_shift,
+                                                      const float2* __restrict__ norm,
+                                                      const float* __restrict__ gscale, uint16_t* __restrict__ e,
+                                                      int64_t lde) {
+  __shared__ float factor[RS_COLS / 64][RS_ROWS];
+  __shared__ int label[RS_ROWS];
+  const int64_t row0 = (int64_t)blockIdx.y * RS_ROWS, col0 = (int64_t)blockIdx.x * RS_COLS;
+  const int rows = (int)min((int64_t)RS_ROWS, r.rows - row0);
+  const float g = *gscale;
+  const int64_t stat0 = col0 >> width_shift, stats_all = (r.classes + (1 << width_shift) - 1) >> width_shift;
+  for (int i = threadIdx.x; i < (RS_COLS >> width_shift) * RS_ROWS; i += 256) {
+    const int k = i % RS_ROWS, t = i / RS_ROWS;
+    float v = 0.f;
+    if (k < rows && stat0 + t < stats_all) {
+      const float2 n = norm[row0 + k];
+      v = exp2f((stats[(stat0 + t) * r.rows + row0 + k].x - n.x) * LOG2E) * n.y * g * (1.f / 32768.f);
+    }
+    factor[t][k] = v;
+  }
+  if (threadIdx.x < RS_ROWS) label[threadIdx.x] = (int)threadIdx.x < rows ? row_label(r, row0 + threadIdx.x) : -1;
+  __syncthreads();
+  const int64_t col = col0 + threadIdx.x * 8;
+  if (col >= r.classes) return;
+  const float* mine = factor[(threadIdx.x * 8) >> width_shift];
+  uint16_t* p = e + row0 * lde + col;
+  for (int k0 = 0; k0 < rows; k0 += 8) {
+    uint4 u[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      if (k0 + k < rows) u[k] = *reinterpret_cast<const uint4*>(p + (k0 + k) * lde);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      if (k0 + k >= rows) break;
+      const int lab = label[k0 + k];
+      const float f = mine[k0 + k];
+      const __half2* h = reinterpret_cast<const __half2*>(&u[k]);
+      float v[8];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float2 t = __half22float2(h[j]);
+        v[2 * j] = t.x * f;
+        v[2 * j + 1] = t.y * f;
+      }
+      const int64_t at = lab - col;
+      if (lab < 0) {  // 0 whatever the row's logits were
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = 0.f;
+      } else if (at >= 0 && at < 8) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] -= j == at ? g : 0.f;
+      }
+      uint4 o;
+      __nv_bfloat162* w = reinterpret_cast<__nv_bfloat162*>(&o);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) w[j] = __floats2bfloat162_rn(v[2 * j], v[2 * j + 1]);
+      *reinterpret_cast<uint4*>(p + (k0 + k) * lde) = o;
+    }
   }
 }
 
 // One row of logits per block.
-__global__ void __launch_bounds__(256) piece_stats_kernel(CeRows r, const float* __restrict__ z, int64_t ldz,
-                                                          int64_t col0, int64_t n, float2* __restrict__ stats,
-                                                          float* __restrict__ zlabel, unsigned* __restrict__ done) {
+__global__ void __launch_bounds__(256) memory_stats_kernel(CeRows r, const float* __restrict__ z, int64_t ldz,
+                                                           float2* __restrict__ stats, float* __restrict__ zlabel,
+                                                           unsigned* __restrict__ done) {
   __shared__ float sm_m[8], sm_s[8];
-  if (blockIdx.x == 0 && threadIdx.x == 0) *done = 0u;
+  if (blockIdx.x == 0 && threadIdx.x == 0 && done != nullptr) *done = 0u;
   const int64_t row = blockIdx.x;
   const float* p = z + row * ldz;
-  const int64_t at = row_label(r, row) - col0;
   float m = -INFINITY, s = 0.f;
-  for (int64_t c = threadIdx.x; c < n; c += 4 * 256) {
+  for (int64_t c = threadIdx.x; c < r.classes; c += 4 * 256) {
     float v[4];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) v[k] = c + k * 256 < n ? p[c + k * 256] : -INFINITY;
+    for (int k = 0; k < 4; ++k) v[k] = c + k * 256 < r.classes ? p[c + k * 256] : -INFINITY;
     const float mn = fmaxf(fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])), m);
     const float b = mn == -INFINITY ? 0.f : mn;
     s *= exp2f((m - b) * LOG2E);
@@ -192,26 +273,26 @@ __global__ void __launch_bounds__(256) piece_stats_kernel(CeRows r, const float*
   if (threadIdx.x == 0) {
     for (int w = 1; w < 8; ++w) join(m, s, sm_m[w], sm_s[w]);
     stats[row] = make_float2(m, s);
-    if (at >= 0 && at < n && row_label(r, row) >= 0) zlabel[row] = p[at];
+    const int lab = row_label(r, row);
+    if (lab >= 0) zlabel[row] = p[lab];
   }
 }
 
-__global__ void __launch_bounds__(256) piece_grad_kernel(CeRows r, float* __restrict__ z, int64_t ldz, int64_t col0,
-                                                         int64_t n, const float2* __restrict__ norm,
-                                                         const float* __restrict__ gscale,
-                                                         __nv_bfloat16* __restrict__ dl) {
+__global__ void __launch_bounds__(256) memory_grad_kernel(CeRows r, float* __restrict__ z, int64_t ldz,
+                                                          const float2* __restrict__ norm,
+                                                          const float* __restrict__ gscale,
+                                                          __nv_bfloat16* __restrict__ dl) {
   const int64_t row = blockIdx.x;
   float* p = z + row * ldz;
   const int lab = row_label(r, row);
-  const int64_t at = lab - col0;
   const float g = *gscale;
-  const float2 nr = norm[row];
-  const float f = nr.y * g;
-  for (int64_t c = threadIdx.x; c < n; c += 256) {
+  const float2 n = norm[row];
+  const float f = n.y * g;
+  for (int64_t c = threadIdx.x; c < r.classes; c += 256) {
     float v = 0.f;
     if (lab >= 0) {
-      v = exp2f((p[c] - nr.x) * LOG2E) * f;
-      if (c == at) v -= g;
+      v = exp2f((p[c] - n.x) * LOG2E) * f;
+      if (c == lab) v -= g;
     }
     p[c] = v;
     if (dl) dl[row * ldz + c] = __float2bfloat16_rn(v);
@@ -248,41 +329,44 @@ void copy_matrix_t(const void* src, int64_t rs, int64_t cs, void* dst, int64_t l
 bool al16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 template <typename T>
-void finish_t(const CeRows& r, const float2* stats, int stat_cols, const float* zlabel, float* rows_loss, float2* norm,
-              bool mean, const float* grad_scale, float* loss, float* gscale, unsigned long long* correct,
-              double* partial, unsigned* done, const void* x, int64_t ldx, int64_t width, void* x_clean, int64_t ldc,
-              cudaStream_t s) {
+void finish_t(const CeRows& r, const CeFinish& f, cudaStream_t s) {
   constexpr int V = 16 / (int)sizeof(T);
-  const int vec = al16(x) && al16(x_clean) && ldx % V == 0 && ldc % V == 0 && width % V == 0;
-  finish_kernel<T><<<(unsigned)((r.rows + FIN_ROWS - 1) / FIN_ROWS), 256, 0, s>>>(
-      r, stats, stat_cols, zlabel, rows_loss, norm, mean ? 1 : 0, grad_scale, loss, gscale, correct, partial, done,
-      reinterpret_cast<const T*>(x), ldx, width, reinterpret_cast<T*>(x_clean), ldc, vec);
+  const int vec = al16(f.x) && al16(f.x_clean) && f.ldx % V == 0 && f.ldc % V == 0 && f.width % V == 0;
+  finish_kernel<T><<<(unsigned)((r.rows + FIN_ROWS - 1) / FIN_ROWS), FIN_WARPS * 32, 0, s>>>(r, f, vec);
   DLVK_POST_LAUNCH();
 }
 
 }  // namespace
 
-void ce_finish(const CeRows& r, const float2* stats, int stat_cols, const float* zlabel, float* rows_loss, float2* norm,
-               bool mean, const float* grad_scale, float* loss, float* gscale, unsigned long long* correct,
-               double* partial, unsigned* done, DType dt, const void* x, int64_t ldx, int64_t width, void* x_clean,
-               int64_t ldc, cudaStream_t s) {
-  if (dt == DType::F32)
-    finish_t<float>(r, stats, stat_cols, zlabel, rows_loss, norm, mean, grad_scale, loss, gscale, correct, partial,
-                    done, x, ldx, width, x_clean, ldc, s);
-  else
-    finish_t<__nv_bfloat16>(r, stats, stat_cols, zlabel, rows_loss, norm, mean, grad_scale, loss, gscale, correct,
-                            partial, done, x, ldx, width, x_clean, ldc, s);
-}
-
-void ce_piece_stats(const CeRows& r, const float* z, int64_t ldz, int64_t col0, int64_t n, float2* stats,
-                    float* zlabel, unsigned* done, cudaStream_t s) {
-  piece_stats_kernel<<<(unsigned)r.rows, 256, 0, s>>>(r, z, ldz, col0, n, stats, zlabel, done);
+void ce_count(const CeRows& r, bool mean, const float* grad_scale, float* gscale, unsigned* done, cudaStream_t s) {
+  count_kernel<<<1, 1024, 0, s>>>(r, mean ? 1 : 0, grad_scale, gscale, done);
   DLVK_POST_LAUNCH();
 }
 
-void ce_piece_grad(const CeRows& r, float* z, int64_t ldz, int64_t col0, int64_t n, const float2* norm,
-                   const float* gscale, __nv_bfloat16* dl, cudaStream_t s) {
-  piece_grad_kernel<<<(unsigned)r.rows, 256, 0, s>>>(r, z, ldz, col0, n, norm, gscale, dl);
+void ce_finish(const CeRows& r, const CeFinish& f, DType dt, cudaStream_t s) {
+  if (dt == DType::F32) finish_t<float>(r, f, s);
+  else finish_t<__nv_bfloat16>(r, f, s);
+}
+
+void ce_rescale(const CeRows& r, const float2* stats, int stat_width, const float2* norm, const float* gscale, void* e,
+                int64_t lde, cudaStream_t s) {
+  DLVK_CHECK((stat_width == 64 || stat_width == 128) && lde % 8 == 0 && al16(e), "ce_rescale: layout");
+  const dim3 grid((unsigned)((r.classes + RS_COLS - 1) / RS_COLS), (unsigned)((r.rows + RS_ROWS - 1) / RS_ROWS));
+  DLVK_CHECK(grid.y <= 65535u, "ce_rescale: more than 2^21 rows in one block of rows");
+  rescale_kernel<<<grid, 256, 0, s>>>(r, stats, stat_width == 64 ? 6 : 7, norm, gscale,
+                                      reinterpret_cast<uint16_t*>(e), lde);
+  DLVK_POST_LAUNCH();
+}
+
+void ce_memory_stats(const CeRows& r, const float* z, int64_t ldz, float2* stats, float* zlabel, unsigned* done,
+                     cudaStream_t s) {
+  memory_stats_kernel<<<(unsigned)r.rows, 256, 0, s>>>(r, z, ldz, stats, zlabel, done);
+  DLVK_POST_LAUNCH();
+}
+
+void ce_memory_grad(const CeRows& r, float* z, int64_t ldz, const float2* norm, const float* gscale, __nv_bfloat16* dl,
+                    cudaStream_t s) {
+  memory_grad_kernel<<<(unsigned)r.rows, 256, 0, s>>>(r, z, ldz, norm, gscale, dl);
   DLVK_POST_LAUNCH();
 }
 

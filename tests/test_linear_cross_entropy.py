@@ -10,6 +10,8 @@ from the same inputs:
 * a probability is exp of (z - lse): off by the errors of both, 2^-22 (|z| +
   |lse| + 2) for the roundings of the exponent, the table-free exp2 and the
   sum's, relative;
+* without a bias, bf16 operands keep exp(z - local maximum) as fp16 times 2^15: 2^-11 of it,
+  and 2^-40 of the largest where it is that small;
 * dz = (p - onehot) g is rounded to bf16 (2^-8) where the operands are bf16;
 * dx, dW are fp32 sums of those (2^-23 per addition of their magnitude) and one
   rounding to their type; db is an fp32 sum of unrounded dz.
@@ -66,6 +68,8 @@ def exact(x, w, t, b, mean=True, ignore=None, scale=1.0):
     perr = p * (dz_ + top[:, None] + 2.0 ** -22 * (zf + lse.abs()[:, None] + 2))
     d = p.clone()
     d[i, lab] -= 1.0
+    if bf and b is None and m:
+        perr = perr + 2.0 ** -11 * p + 2.0 ** -40 * p.amax(-1, keepdim=True)
     # 2^-22: the subtraction and the product by g
     derr = (perr + 2.0 ** -22 * (p + d.abs())) * g
     d *= g
@@ -134,10 +138,28 @@ def test_values(device, dtype, tied, bias, shape):
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("tied", [False, True])
-def test_several_pieces(dtype, tied):
-    # the gradient of 33000 / 20000 rows of 5003 classes does not fit one piece
-    x, w, t, b = operands(33000 if dtype == torch.bfloat16 else 20000, 16, 5003, dtype, "cuda", tied, True)
+@pytest.mark.parametrize("bias", [False, True])
+def test_several_blocks(dtype, tied, bias):
+    # 33000 / 20000 rows of 5003 classes are two blocks
+    x, w, t, b = operands(33000 if dtype == torch.bfloat16 else 20000, 16, 5003, dtype, "cuda", tied, bias)
+    t[::7] = -1
     check(x, w, t, b)
+    W = torch.ones_like(w, dtype=torch.float32)
+    K.linear_ce(x, w, t, b, dw_out=W, dw_accumulate=True)
+    ref, lim = exact(x, w, t, b)["dw"]
+    near(W, (1.0 + ref, lim + 2.0 ** -22 * (1 + ref.abs())), "accumulated")
+
+
+@pytest.mark.gpu
+def test_loss_alone_in_several_blocks():
+    # 2^30 / 60000 rows: three blocks, and a last one of 40 rows
+    n = 2 * 8960 + 40
+    x, w, t, _ = operands(n, 8, 120000, torch.bfloat16, "cuda", True)
+    rows = dl.LinearCrossEntropyLoss("none").forward(x, w, t)
+    for part in (slice(0, 300), slice(8900, 9000), slice(n - 50, n)):
+        near(rows[part], exact(x[part], w, t[part], None, mean=False)["rows"], "rows")
+    mean = dl.LinearCrossEntropyLoss().forward(x, w, t)
+    assert abs(float(mean) - float(rows.double().mean())) <= 2.0 ** -23 * float(mean)
 
 
 @pytest.mark.gpu
