@@ -35,71 +35,72 @@ at::Tensor rows_of_16(const at::Tensor& t) {
   return turn ? n.t() : n;
 }
 
-// An operand of the products: an fp32 one with its two TF32 parts where the
-// products run on the tensor cores (three of them: 3xTF32), made once.
+// An operand of the products: a matrix with one unit stride, as it is or
+// (fp32 on the tensor cores) in three bf16 parts `pitch` apart.
 struct Operand {
-  at::Tensor v, hi, lo;
-  Operand t() const { return hi.defined() ? Operand{v.t(), hi.t(), lo.t()} : Operand{v.t(), {}, {}}; }
-  Operand columns(int64_t at, int64_t n) const {
-    return hi.defined() ? Operand{v.narrow(1, at, n), hi.narrow(1, at, n), lo.narrow(1, at, n)}
-                        : Operand{v.narrow(1, at, n), {}, {}};
-  }
+  const char* p;
+  int64_t rows, cols, rs, cs;
+  int64_t pitch = 0;
+  at::ScalarType type;
+  Operand t() const { return {p, cols, rows, cs, rs, pitch, type}; }
 };
-
-// `t` (one unit stride, rows of whole 16-byte steps) and its parts.
-Operand split(const at::Tensor& t) {
-  const bool turn = t.stride(1) != 1;
-  at::Tensor v = turn ? t.t() : t;
-  const int64_t rows = v.size(0), cols = v.size(1), ld = round_up(cols, 4);
-  if (v.stride(0) != ld) {  // gaps between the rows: the parts are made of a dense copy
-    const at::Tensor c = at::empty({rows, ld}, t.options());
-    copy_matrix(DType::F32, DType::F32, v.data_ptr(), v.stride(0), 1, c.data_ptr(), ld, rows, cols, ld, false, stream());
-    v = c.narrow(1, 0, cols);
-  }
-  // the last row's padding may lie past the end of t's memory: split up to its last element
-  const int64_t n = (rows - 1) * ld + cols;
-  const at::Tensor hi = at::empty({rows, ld}, t.options()), lo = at::empty({rows, ld}, t.options());
-  tf32_split(v.data_ptr<float>(), hi.data_ptr<float>(), lo.data_ptr<float>(), n, stream());
-  const Operand o{t, hi.narrow(1, 0, cols), lo.narrow(1, 0, cols)};
-  return turn ? Operand{t, o.hi.t(), o.lo.t()} : o;
+Operand operand(const at::Tensor& t) {
+  return {static_cast<const char*>(t.data_ptr()), t.size(0), t.size(1), t.stride(0), t.stride(1), 0, t.scalar_type()};
+}
+// `parts` [rows, 3 pitch] of a matrix [rows, cols] (or, turned, its transpose).
+Operand parts_operand(const at::Tensor& parts, int64_t rows, int64_t cols, bool turn = false) {
+  const int64_t pitch = parts.size(1) / 3;
+  const Operand o{static_cast<const char*>(parts.data_ptr()), rows, cols, 3 * pitch, 1, pitch, at::kBFloat16};
+  return turn ? o.t() : o;
 }
 
-constexpr double kTf32Macs = 67108864.0;  // as gemm_op: smaller products stay on the SIMT kernel
-
-// out (+)= A B (+ bias per column), sums in a fixed order.
-void product(const Operand& A, const Operand& B, const at::Tensor& out, bool accumulate,
-             const c10::optional<at::Tensor>& bias = c10::nullopt) {
-  const double macs = (double)out.size(0) * out.size(1) * A.v.size(1);
-  if (A.hi.defined() && B.hi.defined() && macs >= kTf32Macs) {
-    GemmArgs ll = fill_args(A.lo, B.hi, out), lh = fill_args(A.hi, B.lo, out), hh = fill_args(A.hi, B.hi, out);
-    if (gemm_tf32_tc_supported(ll) && gemm_tf32_tc_supported(lh) && gemm_tf32_tc_supported(hh)) {
-      if (bias.has_value()) hh.bias = bias->data_ptr();
-      int pass = 0;
-      for (GemmArgs* a : {&ll, &lh, &hh}) {  // the small terms first
-        a->ordered = true;
-        a->beta = (pass++ > 0 || accumulate) ? 1.f : 0.f;
-        const int64_t n = gemm_tc_workspace_floats(*a, 0, DType::F32, true);
-        const at::Tensor ws = n > 0 ? at::empty({n}, out.options()) : at::Tensor();
-        gemm_tf32_tc(DType::F32, *a, stream(), device_error_word(), 0, n > 0 ? ws.data_ptr<float>() : nullptr, n);
-      }
-      return;
-    }
+// out (+)= scale * A B (+ bias per column), the sums in a fixed order.
+void product(const Operand& A, const Operand& B, const at::Tensor& out, const float* scale, bool accumulate,
+             const float* bias = nullptr) {
+  GemmArgs a;
+  a.A = A.p;
+  a.B = B.p;
+  a.C = out.data_ptr();
+  a.M = A.rows;
+  a.K = A.cols;
+  a.N = B.cols;
+  a.sam = A.rs;
+  a.sak = A.cs;
+  a.sbk = B.rs;
+  a.sbn = B.cs;
+  a.ldc = out.stride(0);
+  a.beta = accumulate ? 1.f : 0.f;
+  a.bias = bias;
+  a.bias_dtype = (int)DType::F32;
+  a.ordered = true;
+  a.parts = A.pitch > 0;
+  a.pitch_a = A.pitch;
+  a.pitch_b = B.pitch;
+  const DType odt = to_dtype(out);
+  if (A.type == at::kBFloat16 && gemm_tc_supported(a)) {
+    a.alpha_ptr = scale;
+    const int64_t n = gemm_tc_workspace_floats(a, 0, odt);
+    const at::Tensor ws = n > 0 ? at::empty({n}, out.options().dtype(at::kFloat)) : at::Tensor();
+    gemm_tc(odt, a, stream(), device_error_word(), 0, n > 0 ? ws.data_ptr<float>() : nullptr, n);
+    return;
   }
-  const bool simt = A.v.scalar_type() == at::kFloat && fp32_gemm_mode() != 1;
-  gemm_op(A.v, B.v, bias, ACT_NONE, 1.0, accumulate ? 1.0 : 0.0, out, c10::nullopt, simt ? 2 : 0, 0, c10::nullopt,
-          c10::nullopt, c10::nullopt, 1.0, false, c10::nullopt, c10::nullopt, true);
+  TORCH_INTERNAL_ASSERT(scale == nullptr && !a.parts);
+  const int64_t n = gemm_simt_workspace_floats(a);
+  const at::Tensor ws = n > 0 ? at::empty({n}, out.options().dtype(at::kFloat)) : at::Tensor();
+  gemm_simt(A.type == at::kFloat ? DType::F32 : DType::BF16, odt, a, stream(), n > 0 ? ws.data_ptr<float>() : nullptr,
+            n);
 }
 
-// dst (+)= A B.  Output rows that are no whole 16-byte steps go through a
-// padded copy: the products store whole boxes.
-void product_into(const Operand& A, const Operand& B, const at::Tensor& dst, bool accumulate) {
+// dst (+)= scale * A B.  Output rows that are no whole 16-byte steps go
+// through a padded copy: the products store whole boxes.
+void product_into(const Operand& A, const Operand& B, const at::Tensor& dst, const float* scale, bool accumulate) {
   const int64_t n = dst.size(1), step = 16 / dst.element_size();
   if (dst.stride(0) % step == 0 && reinterpret_cast<uintptr_t>(dst.data_ptr()) % 16 == 0) {
-    product(A, B, dst, accumulate);
+    product(A, B, dst, scale, accumulate);
     return;
   }
   const at::Tensor c = at::empty({dst.size(0), round_up(n, step)}, dst.options());
-  product(A, B, c.narrow(1, 0, n), false);
+  product(A, B, c.narrow(1, 0, n), scale, false);
   copy_matrix(to_dtype(dst), to_dtype(c), c.data_ptr(), c.size(1), 1, dst.data_ptr(), dst.stride(0), dst.size(0), n, n,
               accumulate, stream());
 }
@@ -177,33 +178,62 @@ LinearCeResult linear_ce_op(const at::Tensor& x, const at::Tensor& w, const at::
 
   const at::Tensor tc = target.contiguous();
   const at::Tensor bc = bias.has_value() ? bias->to(at::kFloat).contiguous() : at::Tensor();
-  at::Tensor xq = rows_of_16(x);
-  if (xq.stride(1) != 1) xq = rows_of_16(x.contiguous());  // the products read x by rows
-  at::Tensor wq = rows_of_16((w.stride(0) == 1 || w.stride(1) == 1) ? w : w.contiguous());
-  const bool w_k = wq.stride(1) != 1;  // classes are rows: W^T is what memory holds
-
+  const float* biasp = bc.defined() ? bc.data_ptr<float>() : nullptr;
+  const CeRows all{N, V, ignore_index, tc.data_ptr(), tc.scalar_type() == at::kLong};
+  at::Tensor xq, wq;
+  bool w_k;  // classes are rows: W^T is what memory holds
   CeProjection c;
-  if (bf) {
-    c.x = reinterpret_cast<const __nv_bfloat16*>(xq.data_ptr());
-    c.w = reinterpret_cast<const __nv_bfloat16*>(wq.data_ptr());
+  // fp32 operands of some size run as six products of bf16 parts; a small or
+  // narrow one keeps the SIMT product (it would be mostly padding)
+  const bool parts = !bf && fp32_gemm_mode() != 0 && E >= 16 && V >= 64 && (double)N * E * V >= 4194304.0;
+  if (parts) {
+    const at::Tensor xs = x.stride(1) == 1 ? x : x.contiguous();
+    const at::Tensor wr = (w.stride(0) == 1 || w.stride(1) == 1) ? w : w.contiguous();
+    w_k = wr.stride(1) != 1;
+    const at::Tensor wm = w_k ? wr.t() : wr;  // rows of unit stride
+    const auto b16 = x.options().dtype(at::kBFloat16);
+    const int64_t ep = round_up(E, 64), wp = round_up(wm.size(1), 64);
+    xq = at::empty({N, 3 * ep}, b16);
+    wq = at::empty({wm.size(0), 3 * wp}, b16);
+    // rows that do not count are zeros, whatever they hold (see x_clean below)
+    split_parts(xs.data_ptr<float>(), xs.stride(0), N, E, reinterpret_cast<__nv_bfloat16*>(xq.data_ptr()), ep, &all,
+                stream());
+    split_parts(wm.data_ptr<float>(), wm.stride(0), wm.size(0), wm.size(1),
+                reinterpret_cast<__nv_bfloat16*>(wq.data_ptr()), wp, nullptr, stream());
+    c.parts = true;
+    c.pitch_x = ep;
+    c.pitch_w = wp;
+    c.ldx = 3 * ep;
+    c.ldw = 3 * wp;
+  } else {
+    xq = rows_of_16(x);
+    if (xq.stride(1) != 1) xq = rows_of_16(x.contiguous());  // the products read x by rows
+    wq = rows_of_16((w.stride(0) == 1 || w.stride(1) == 1) ? w : w.contiguous());
+    w_k = wq.stride(1) != 1;
+    c.ldx = xq.stride(0);
+    c.ldw = w_k ? wq.stride(1) : wq.stride(0);
   }
+  const Operand wo = parts ? parts_operand(wq, w_k ? V : E, w_k ? E : V, w_k) : operand(wq);  // [E, V]
+  c.x = reinterpret_cast<const __nv_bfloat16*>(xq.data_ptr());
+  c.w = reinterpret_cast<const __nv_bfloat16*>(wq.data_ptr());
   c.rows = N;
   c.width = E;
   c.classes = V;
-  c.ldx = xq.stride(0);
-  c.ldw = w_k ? wq.stride(1) : wq.stride(0);
   c.w_k = w_k;
-  c.bias = bc.defined() ? bc.data_ptr<float>() : nullptr;
-  c.labels64 = tc.scalar_type() == at::kLong;
+  c.bias = biasp;
+  c.labels64 = all.labels64;
   c.ignore = ignore_index;
-  const bool tensor = bf && ce_tc_supported(c);  // else a block's logits go through memory in fp32
-  const bool keep = tensor && want_grad && !bias.has_value();  // exponentials kept, not made again
+  // Where the logits are: in the accumulators (bf16, and the loss alone of
+  // fp32 parts), else a block of them in memory as fp32.
+  const bool tc_ok = (bf || parts) && E >= 16 && ce_tc_supported(c);
+  const bool fused = tc_ok && (bf || !want_grad);
+  const bool keep = fused && want_grad && !bias.has_value();  // exponentials kept, not made again
 
   // 256 MB of a block's exponentials, gradients or logits; the loss alone
   // keeps a 32nd of that on the tensor cores, the statistics
-  const int64_t rows = block_of(N, V, !tensor ? (64LL << 20) : want_grad ? (128LL << 20) : (1LL << 30));
+  const int64_t rows = block_of(N, V, !fused ? (64LL << 20) : want_grad ? (128LL << 20) : (1LL << 30));
   const int64_t blocks = ceil_div(N, rows);
-  const int stat_cols = tensor ? ce_tc_stat_cols(rows, V) : 1;
+  const int stat_cols = fused ? ce_tc_stat_cols(rows, V) : 1;
   const int groups = (int)ceil_div(N, 32), lab_size = c.labels64 ? 8 : 4;
   // scratch: 8-byte items first (sums, statistics, norms), then floats, then the counter
   const at::Tensor ws = at::empty({6LL * groups + 2 * rows * stat_cols + 3 * rows + 2}, f32);
@@ -219,27 +249,23 @@ LinearCeResult linear_ce_op(const at::Tensor& x, const at::Tensor& w, const at::
   c.norm = norm;
   c.gscale = gscale;
 
-  const int64_t ldv = round_up(V, 8);
-  const bool parts = !bf && fp32_gemm_mode() == 3 && (double)N * E * V >= kTf32Macs;
-  const auto whole = [&](const at::Tensor& t) { return parts ? split(t) : Operand{t, {}, {}}; };
-  const Operand wo = tensor && !want_grad ? Operand{wq, {}, {}} : whole(wq);
+  const int64_t ldv = round_up(V, 8), vp = round_up(V, 64);
   at::Tensor z, dl, xc, part, dw32;
-  if (!tensor) z = at::empty({rows, ldv}, f32);
+  if (!fused) z = at::empty({rows, ldv}, f32);
   bool dw_k = false;
   if (want_grad) {
-    dl = bf ? at::empty({rows, ldv}, x.options()) : z;
+    dl = parts ? at::empty({rows, 3 * vp}, xq.options()) : bf ? at::empty({rows, ldv}, x.options()) : z;
     // dW = x^T dz reads x once more, with zeros in the rows that do not count:
     // their dz is 0, but 0 times an infinity or NaN left there would not be.
-    xc = at::empty({rows, round_up(E, 16 / x.element_size())}, x.options()).narrow(1, 0, E);
+    if (!parts) xc = at::empty({rows, round_up(E, 16 / x.element_size())}, x.options()).narrow(1, 0, E);
     dw_k = out.dw.stride(1) != 1 && V > 1;  // the gradient's rows are classes too
     // sums over several blocks are fp32 until the last
     if (blocks > 1 && out.dw.scalar_type() != at::kFloat)
       dw32 = dw_k ? at::empty({V, round_up(E, 4)}, f32).narrow(1, 0, E).t()
                   : at::empty({E, round_up(V, 4)}, f32).narrow(1, 0, V);
-    if (out.dbias.defined()) part = at::empty({tensor ? ceil_div(rows, 32) * V : ldv}, f32);
+    if (out.dbias.defined()) part = at::empty({fused ? ceil_div(rows, 32) * V : ldv}, f32);
   }
   const at::Tensor dw = dw32.defined() ? dw32 : out.dw;
-  CeRows all{N, V, ignore_index, tc.data_ptr(), c.labels64};
   if (blocks > 1) ce_count(all, mean, gsp, gscale, done, stream());
 
   for (int64_t k = 0; k < blocks; ++k) {
@@ -248,23 +274,23 @@ LinearCeResult linear_ce_op(const at::Tensor& x, const at::Tensor& w, const at::
     r.rows = n;
     r.labels = static_cast<const char*>(tc.data_ptr()) + r0 * lab_size;
     const at::Tensor xk = xq.narrow(0, r0, n);
+    Operand xo = parts ? parts_operand(xk, n, E) : operand(xk);
     c.rows = n;
-    TORCH_INTERNAL_ASSERT(!tensor || n * ce_tc_stat_cols(n, V) <= rows * stat_cols);
-    c.x = bf ? reinterpret_cast<const __nv_bfloat16*>(xk.data_ptr()) : nullptr;
+    TORCH_INTERNAL_ASSERT(!fused || n * ce_tc_stat_cols(n, V) <= rows * stat_cols);
+    c.x = reinterpret_cast<const __nv_bfloat16*>(xk.data_ptr());
     c.labels = r.labels;
     c.done = blocks == 1 ? done : nullptr;
     if (keep) {
       ce_exp_tc(c, dl.data_ptr(), ldv, stream(), device_error_word());
-    } else if (tensor) {
+    } else if (fused) {
       ce_stats_tc(c, stream(), device_error_word());
     } else {
-      product(whole(xk), wo, z.narrow(0, 0, n).narrow(1, 0, V), false,
-              bc.defined() ? c10::optional<at::Tensor>(bc) : c10::nullopt);
+      product(xo, wo, z.narrow(0, 0, n).narrow(1, 0, V), nullptr, false, biasp);
       ce_memory_stats(r, z.data_ptr<float>(), ldv, stats, zlabel, c.done, stream());
     }
     CeFinish f{};
     f.stats = stats;
-    f.stat_cols = tensor ? ce_tc_stat_cols(n, V) : 1;
+    f.stat_cols = fused ? ce_tc_stat_cols(n, V) : 1;
     f.zlabel = zlabel;
     f.rows_loss = out.rows.data_ptr<float>() + r0;
     f.norm = norm;
@@ -278,19 +304,22 @@ LinearCeResult linear_ce_op(const at::Tensor& x, const at::Tensor& w, const at::
     f.done = done;
     f.first_group = (int)(r0 / 32);  // blocks are whole tiles, the last apart
     f.total_groups = groups;
-    if (want_grad) {
+    if (xc.defined()) {
       f.x = xk.data_ptr();
       f.ldx = xk.stride(0);
       f.width = E;
       f.x_clean = xc.data_ptr();
       f.ldc = xc.stride(0);
+      xo = operand(xc.narrow(0, 0, n));
     }
     ce_finish(r, f, to_dtype(x), stream());
     if (!want_grad) continue;
 
+    Operand d = parts ? parts_operand(dl, n, V) : operand(dl.narrow(0, 0, n).narrow(1, 0, V));
+    const float* scale = gscale;  // dz holds softmax - onehot, the products its factor
     if (keep) {
-      ce_rescale(r, stats, ce_tc_stat_width(n, V), norm, gscale, dl.data_ptr(), ldv, stream());
-    } else if (tensor) {
+      ce_rescale(r, stats, ce_tc_stat_width(n, V), norm, dl.data_ptr(), ldv, stream());
+    } else if (fused) {
       ce_grad_tc(c, reinterpret_cast<__nv_bfloat16*>(dl.data_ptr()), ldv,
                  part.defined() ? part.data_ptr<float>() : nullptr, stream(), device_error_word());
       if (part.defined())
@@ -298,7 +327,9 @@ LinearCeResult linear_ce_op(const at::Tensor& x, const at::Tensor& w, const at::
                         db_accumulate || k > 0, stream());
     } else {
       ce_memory_grad(r, z.data_ptr<float>(), ldv, norm, gscale,
-                     bf ? reinterpret_cast<__nv_bfloat16*>(dl.data_ptr()) : nullptr, stream());
+                     dl.is_same(z) ? nullptr : reinterpret_cast<__nv_bfloat16*>(dl.data_ptr()), parts ? vp : 0,
+                     stream());
+      if (!parts) scale = nullptr;  // these carry it
       if (part.defined()) {  // the padding's columns are summed too and left out of the copy
         const int64_t ns = colsum_scratch_floats(n, ldv);
         const at::Tensor scr = ns > 0 ? at::empty({ns}, f32) : at::Tensor();
@@ -308,19 +339,15 @@ LinearCeResult linear_ce_op(const at::Tensor& x, const at::Tensor& w, const at::
                     db_accumulate || k > 0, stream());
       }
     }
-    const Operand d = whole(dl.narrow(0, 0, n).narrow(1, 0, V)), xo = whole(xc.narrow(0, 0, n));
-    product_into(d, wo.t(), out.dx.narrow(0, r0, n), false);
+    product_into(d, wo.t(), out.dx.narrow(0, r0, n), scale, false);
     const bool add = dw32.defined() ? k > 0 : (dw_accumulate || k > 0);
-    if (dw_k) product_into(d.t(), xo, dw.t(), add);
-    else product_into(xo.t(), d, dw, add);
+    if (dw_k) product_into(d.t(), xo, dw.t(), scale, add);
+    else product_into(xo.t(), d, dw, scale, add);
   }
   if (dw32.defined()) {
     const at::Tensor src = dw_k ? dw32.t() : dw32, dst = dw_k ? out.dw.t() : out.dw;
-    if (src.is_contiguous() && dst.is_contiguous())
-      unary(DType::F32, to_dtype(dst), src.data_ptr(), dst.data_ptr(), src.numel(), UN_COPY, 0.f, 0.f, stream());
-    else
-      copy_matrix(to_dtype(dst), DType::F32, src.data_ptr(), src.stride(0), 1, dst.data_ptr(), dst.stride(0),
-                  dst.size(0), dst.size(1), dst.size(1), false, stream());
+    copy_matrix(to_dtype(dst), DType::F32, src.data_ptr(), src.stride(0), 1, dst.data_ptr(), dst.stride(0),
+                dst.size(0), dst.size(1), dst.size(1), false, stream());
   }
   return out;
 }

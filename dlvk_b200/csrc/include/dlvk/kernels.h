@@ -95,6 +95,14 @@ struct GemmArgs {
   // Sum split-K partials in a fixed order (through the workspace) instead of
   // adding them into an fp32 C as they come.
   bool ordered = false;
+  const float* alpha_ptr = nullptr;  // optional device factor of alpha (tensor-core path)
+  // bf16 operands that hold an fp32 matrix in three parts side by side along
+  // their contiguous dimension, pitch_a / pitch_b (multiples of 64) elements
+  // apart (split_parts): C = the fp32 product, as six bf16 ones.  The padding
+  // of K is zero.  Tensor-core path; gemm_tc_workspace_floats() says what room
+  // its split-K takes, without which the sums are unsplit.
+  bool parts = false;
+  int64_t pitch_a = 0, pitch_b = 0;
 };
 // SIMT GEMM.  With a workspace of gemm_simt_workspace_floats(a) floats, a
 // small 2-D GEMM with a plain epilogue splits K across blocks (fp32 partials,
@@ -310,7 +318,11 @@ struct CeProjection {
   float2* stats = nullptr;           // [ce_tc_stat_cols][rows] (maximum, sum of exp(z - maximum))
   float* zlabel = nullptr;           // [rows], written for rows that count
   const float2* norm = nullptr;      // [rows] maximum and 1 / sum, for the gradient
-  const float* gscale = nullptr;     // device scalar: gradient w.r.t. a counted row's loss
+  const float* gscale = nullptr;     // device scalar: factor of ce_grad_tc's column sums
+  // fp32 operands in three parts (GemmArgs::parts); ldx and ldw are then the
+  // distances of whole rows of parts
+  bool parts = false;
+  int64_t pitch_x = 0, pitch_w = 0;
   unsigned* done = nullptr;          // set to 0 with the statistics (or null)
 };
 bool ce_tc_supported(const CeProjection& c);
@@ -321,8 +333,8 @@ void ce_stats_tc(const CeProjection& c, cudaStream_t s, uint32_t* err);
 // The statistics, and e = 2^15 exp(z - the maximum of its statistics column),
 // fp16 [rows, classes], row stride lde.
 void ce_exp_tc(const CeProjection& c, void* e, int64_t lde, cudaStream_t s, uint32_t* err);
-// dl [rows, classes] = (softmax - onehot) * gscale, bf16, row stride ldd;
-// colsum (or null): its fp32 column sums per 32 rows [ceil(rows / 32)][classes],
+// dl [rows, classes] = softmax - onehot, bf16, row stride ldd; colsum (or
+// null): gscale times its fp32 column sums per 32 rows [ceil(rows / 32)][classes],
 // for colsum_partials.
 void ce_grad_tc(const CeProjection& c, __nv_bfloat16* dl, int64_t ldd, float* colsum, cudaStream_t s, uint32_t* err);
 // The passes around them, and the same statistics / gradient from logits in
@@ -360,16 +372,23 @@ struct CeFinish {
   int64_t ldc;
 };
 void ce_finish(const CeRows& r, const CeFinish& f, DType dt, cudaStream_t s);
-// e (ce_exp_tc's, fp16) becomes the gradient (softmax - onehot) * gscale in
-// place, bf16; stat_width classes to a statistics column.
-void ce_rescale(const CeRows& r, const float2* stats, int stat_width, const float2* norm, const float* gscale, void* e,
-                int64_t lde, cudaStream_t s);
-// Statistics (one column) and gradient (in place; dl, or null, its bf16 copy)
-// of logits z [rows, classes] fp32; row strides ldz.
+// e (ce_exp_tc's, fp16) becomes softmax - onehot in place, bf16; stat_width
+// classes to a statistics column.
+void ce_rescale(const CeRows& r, const float2* stats, int stat_width, const float2* norm, void* e, int64_t lde,
+                cudaStream_t s);
+// Statistics (one column) and gradient of logits z [rows, classes] fp32, row
+// stride ldz: z becomes (softmax - onehot) * gscale; dl, when given, that
+// rounded to bf16 (pitch 0, row stride ldz), or softmax - onehot in three
+// parts (pitch of a part, row stride 3 pitch, zeros in the padding).
 void ce_memory_stats(const CeRows& r, const float* z, int64_t ldz, float2* stats, float* zlabel, unsigned* done,
                      cudaStream_t s);
 void ce_memory_grad(const CeRows& r, float* z, int64_t ldz, const float2* norm, const float* gscale, __nv_bfloat16* dl,
-                    cudaStream_t s);
+                    int64_t pitch, cudaStream_t s);
+// dst [rows, 3 pitch] bf16: src (fp32 [rows, cols], row stride ld) = the sum of
+// its three parts to 2^-24; zeros in the padding, and with `mask` in the rows
+// that do not count.
+void split_parts(const float* src, int64_t ld, int64_t rows, int64_t cols, __nv_bfloat16* dst, int64_t pitch,
+                 const CeRows* mask, cudaStream_t s);
 // dst [rows, cols] (row stride ldd) = src (strides rs, cs), or += (accumulate);
 // columns [cols, pad_to) become 0.  fp32 or bf16 each.
 void copy_matrix(DType dst_dt, DType src_dt, const void* src, int64_t rs, int64_t cs, void* dst, int64_t ldd,

@@ -49,7 +49,7 @@ struct CeEpilogue {
   float2* stats;       // EPI 3, 5: [column half tiles][M] (maximum, sum)
   float* zlabel;       // EPI 3, 5: the logit of each row's class
   const float2* norm;  // EPI 4: each row's maximum and 1 / sum of exp(z - maximum)
-  const float* gscale; // EPI 4: gradient of the loss w.r.t. each counted row's loss
+  const float* gscale; // EPI 4: factor of the column sums
   unsigned* done;      // EPI 3, 5: set to 0 (or null)
 };
 
@@ -88,8 +88,17 @@ struct TcParams {
   uint32_t* bits_out;      // ReLU bitmask written (plain / TMA-store epilogues), or null
   const uint32_t* bits_in; // ReLU bitmask applied (staged epilogue), or null
   int64_t ldbits;          // 32-bit words per bitmask row
-  CeEpilogue ce;           // softmax cross entropy epilogues (EPI 3 and 4)
+  CeEpilogue ce;           // softmax cross entropy epilogues (EPI 3 to 5)
+  const float* alpha_ptr;  // device factor of alpha, or null
+  int products;            // 1; 6: fp32 operands in three bf16 parts each
+  int a_pitch, b_pitch;    // distance of an operand's parts along its contiguous dimension
 };
+
+// The six products of operands in three parts (x = x0 + x1 + x2, 8 bits
+// each) that reach above 2^-24 of the whole, small ones first: x2 w0, x0 w2,
+// x1 w1, x1 w0, x0 w1, x0 w0.  Four bits per product.
+__device__ __forceinline__ int part_a(int i) { return (0x001102 >> (4 * i)) & 15; }
+__device__ __forceinline__ int part_b(int i) { return (0x010120 >> (4 * i)) & 15; }
 
 // PAIR: a 2-CTA cluster shares one 256 x BN tile (tcgen05 cta_group::2);
 // each CTA stages its 128 rows of A and its BN/2 columns of B.
@@ -489,7 +498,11 @@ __device__ __forceinline__ void epi_store(const TcParams& p, const float* stg, i
 // ---- softmax cross entropy over the accumulators (logits in fp32) ----
 // The products of a vocabulary projection are consumed where they are made:
 // EPI 3 reduces each row's logits to a running maximum and sum, EPI 4 turns
-// them into the gradient (softmax - onehot) * scale, rounded once to bf16.
+// them into their gradient softmax - onehot, rounded once to bf16.  The
+// factor 1 / (counted rows) of a mean is left to the epilogues of the products
+// that read it: rounded into every -1 of the one-hot part it would be wrong by
+// the same 2^-9 everywhere, and so would the sums (error of dW at 8192 rows,
+// 32000 words against 64 bits: 0.0033 with it, 0.0018 without).
 // EPI 5 does what EPI 3 does and stores exp(z - maximum), the maximum being
 // that of the thread's half of the tile's columns, from which the gradient
 // needs no second product.  A thread owns one row of the tile, so none of
@@ -577,14 +590,14 @@ __device__ __forceinline__ void ce_pick(const TcParams& p, int row, int at, cons
   }
 }
 
-// v[j] = (softmax - onehot) * g, for a row that does not count 0 whatever its
-// logits are; f = g / sum.
-__device__ __forceinline__ void ce_gradient(float m, float f, float g, int at, float* v) {
+// v[j] = softmax - onehot, for a row that does not count 0 whatever its
+// logits are; f = 1 / sum.
+__device__ __forceinline__ void ce_gradient(float m, float f, int at, float* v) {
 #pragma unroll
   for (int j = 0; j < 32; ++j) v[j] = ex2((v[j] - m) * LOG2E) * f;
   if ((unsigned)at < 32u) {  // one chunk of the whole row
 #pragma unroll
-    for (int j = 0; j < 32; ++j) v[j] -= j == at ? g : 0.f;
+    for (int j = 0; j < 32; ++j) v[j] -= j == at ? 1.f : 0.f;
   }
   if (at == CE_ROW_OUT) {
 #pragma unroll
@@ -681,7 +694,10 @@ __global__ void __launch_bounds__(320, 1)
         const int arow = tm * TILE_M + (int)rank * BM;
         // sub-block j of this CTA: columns tn*BN + j*MMA_N + rank*MMA_N/2 + [0, MMA_N/2)
         const int bcol = tn * BN + (int)rank * (C::MMA_N / 2);
-        for (int kb = kb0; kb < kb1; ++kb) {
+        const int run = kb1 - kb0;
+        for (int it = 0; it < run * p.products; ++it) {
+          const int pr = p.products == 1 ? 0 : it / run, kb = kb0 + it - pr * run;
+          const int ao = p.products == 1 ? 0 : part_a(pr) * p.a_pitch, bo6 = p.products == 1 ? 0 : part_b(pr) * p.b_pitch;
           {
             GEMM_T0();
             if (!mbar_wait(&empty[stage], phase ^ 1u, p.err)) goto producer_done_pair;
@@ -692,22 +708,22 @@ __global__ void __launch_bounds__(320, 1)
           const uint32_t fb = mapa_shared(smem_u32(&full[stage]), 0);  // the leader's full barrier
           if (rank == 0) mbar_arrive_expect_tx(&full[stage], 2 * C::STAGE_BYTES);
           if (!p.a_mn) {
-            tma_load_4d_pair(sA, &tmA, fb, kb * BK, arow, abi, abo);
+            tma_load_4d_pair(sA, &tmA, fb, kb * BK + ao, arow, abi, abo);
           } else {
 #pragma unroll
             for (int j = 0; j < BM / 64; ++j)
-              tma_load_4d_pair(sA + j * 8192, &tmA, fb, arow + j * 64, kb * BK, abi, abo);
+              tma_load_4d_pair(sA + j * 8192, &tmA, fb, arow + j * 64 + ao, kb * BK, abi, abo);
           }
 #pragma unroll
           for (int sub = 0; sub < C::NSUB; ++sub) {
             uint8_t* sBs = sB + sub * C::SUB_B_BYTES;
             const int col = bcol + sub * C::MMA_N;
             if (!p.b_mn) {
-              tma_load_4d_pair(sBs, &tmB, fb, kb * BK, col, bi, bo);
+              tma_load_4d_pair(sBs, &tmB, fb, kb * BK + bo6, col, bi, bo);
             } else {
 #pragma unroll
               for (int j = 0; j < C::MMA_N / 128; ++j)
-                tma_load_4d_pair(sBs + j * 8192, &tmB, fb, col + j * 64, kb * BK, bi, bo);
+                tma_load_4d_pair(sBs + j * 8192, &tmB, fb, col + j * 64 + bo6, kb * BK, bi, bo);
             }
           }
           if (++stage == C::STAGES) {
@@ -727,7 +743,10 @@ __global__ void __launch_bounds__(320, 1)
       while (work_next(p, gridDim.x, num_kb, tiles_per_split, num_tiles, w, tm, tn, b, sp, kb0, kb1, last)) {
         const int bo = b / p.batch2, bi = b - bo * p.batch2;
         const int abo = p.a_bcast ? 0 : bo, abi = p.a_bcast ? 0 : bi;
-        for (int kb = kb0; kb < kb1; ++kb) {
+        const int run = kb1 - kb0;
+        for (int it = 0; it < run * p.products; ++it) {
+          const int pr = p.products == 1 ? 0 : it / run, kb = kb0 + it - pr * run;
+          const int ao = p.products == 1 ? 0 : part_a(pr) * p.a_pitch, bo6 = p.products == 1 ? 0 : part_b(pr) * p.b_pitch;
           {
             GEMM_T0();
             if (!mbar_wait(&empty[stage], phase ^ 1u, p.err)) goto producer_done;
@@ -737,16 +756,16 @@ __global__ void __launch_bounds__(320, 1)
           uint8_t* sB = sA + C::A_BYTES;
           mbar_arrive_expect_tx(&full[stage], C::STAGE_BYTES);
           if (!p.a_mn) {
-            tma_load_4d(sA, &tmA, &full[stage], kb * bke, tm * BM, abi, abo);
+            tma_load_4d(sA, &tmA, &full[stage], kb * bke + ao, tm * BM, abi, abo);
           } else {
             for (int j = 0; j < BM / mn_box; ++j)
-              tma_load_4d(sA + j * mn_box_bytes, &tmA, &full[stage], tm * BM + j * mn_box, kb * bke, abi, abo);
+              tma_load_4d(sA + j * mn_box_bytes, &tmA, &full[stage], tm * BM + j * mn_box + ao, kb * bke, abi, abo);
           }
           if (!p.b_mn) {
-            tma_load_4d(sB, &tmB, &full[stage], kb * bke, tn * BN, bi, bo);
+            tma_load_4d(sB, &tmB, &full[stage], kb * bke + bo6, tn * BN, bi, bo);
           } else {
             for (int j = 0; j < BN / mn_box; ++j)
-              tma_load_4d(sB + j * mn_box_bytes, &tmB, &full[stage], tn * BN + j * mn_box, kb * bke, bi, bo);
+              tma_load_4d(sB + j * mn_box_bytes, &tmB, &full[stage], tn * BN + j * mn_box + bo6, kb * bke, bi, bo);
           }
           if (++stage == C::STAGES) {
             stage = 0;
@@ -779,7 +798,7 @@ __global__ void __launch_bounds__(320, 1)
           tc_fence_after();
           const uint32_t d = tmem_base + (uint32_t)(acc * BN);
           bool ok = true;
-          for (int kb = kb0; kb < kb1; ++kb) {
+          for (int it = 0; it < (kb1 - kb0) * p.products; ++it) {
             GEMM_T0();
             if (!mbar_wait(&full[stage], phase, p.err)) { ok = false; break; }
             GEMM_ACC(2);
@@ -795,7 +814,7 @@ __global__ void __launch_bounds__(320, 1)
                 const uint32_t bs = bBase + sub * C::SUB_B_BYTES;
                 const uint64_t bd = p.b_mn ? make_sw128_desc(bs + k * 2048, 8192, 1024)
                                            : make_sw128_desc(bs + k * 32, 16, 1024);
-                mma_f16_pair(d + (uint32_t)(sub * C::MMA_N), ad, bd, idesc, (kb != kb0 || k != 0) ? 1u : 0u);
+                mma_f16_pair(d + (uint32_t)(sub * C::MMA_N), ad, bd, idesc, (it != 0 || k != 0) ? 1u : 0u);
               }
             }
             const uint32_t eb = smem_u32(&empty[stage]);
@@ -840,7 +859,7 @@ __global__ void __launch_bounds__(320, 1)
         tc_fence_after();
         const uint32_t d = tmem_base + (uint32_t)(acc * BN);
         bool ok = true;
-        for (int kb = kb0; kb < kb1; ++kb) {
+        for (int it = 0; it < (kb1 - kb0) * p.products; ++it) {
           GEMM_T0();
           if (!mbar_wait(&full[stage], phase, p.err)) { ok = false; break; }
           GEMM_ACC(2);
@@ -856,9 +875,9 @@ __global__ void __launch_bounds__(320, 1)
             const uint64_t bd = p.b_mn ? (p.tf32 ? make_sw128b32_desc(bBase + k * mn_step, (uint32_t)mn_box_bytes, 512)
                                                  : make_sw128_desc(bBase + k * mn_step, (uint32_t)mn_box_bytes, 1024))
                                        : make_sw128_desc(bBase + k * 32, 16, 1024);
-            if (p.i8) mma_i8(d, ad, bd, idesc, (kb != kb0 || k != 0) ? 1u : 0u);
-            else if (p.tf32) mma_tf32(d, ad, bd, idesc, (kb != kb0 || k != 0) ? 1u : 0u);
-            else mma_f16(d, ad, bd, idesc, (kb != kb0 || k != 0) ? 1u : 0u);
+            if (p.i8) mma_i8(d, ad, bd, idesc, (it != 0 || k != 0) ? 1u : 0u);
+            else if (p.tf32) mma_tf32(d, ad, bd, idesc, (it != 0 || k != 0) ? 1u : 0u);
+            else mma_f16(d, ad, bd, idesc, (it != 0 || k != 0) ? 1u : 0u);
           }
           mma_commit(&empty[stage]);
           if (++stage == C::STAGES) {
@@ -890,6 +909,7 @@ __global__ void __launch_bounds__(320, 1)
     // path, which handles all three.
     const bool staged = (p.beta != 0.f) || (p.out_f32 && (p.R != nullptr || p.Mk != nullptr));
     constexpr int NCH = BN / 64;  // 32-column chunks per warp
+    const float alpha = p.alpha_ptr != nullptr ? p.alpha * *p.alpha_ptr : p.alpha;
     int acc = 0, ecount = 0;
     uint32_t acc_phase = 0;
     // TMA-store boxes (4 KB): one slot per warp in the epilogue area, so each
@@ -932,7 +952,7 @@ __global__ void __launch_bounds__(320, 1)
           const float2 norm = p.ce.norm[row0 + lane];
           ce_g = *p.ce.gscale;
           ce_m = norm.x;
-          ce_s = norm.y * ce_g;
+          ce_s = norm.y;
         }
       }
       if constexpr (EPI == 5) {  // the maximum first: the accumulators are read twice
@@ -967,7 +987,7 @@ __global__ void __launch_bounds__(320, 1)
           }
         } else if (EPI == 0 && staged) {
 #pragma unroll
-          for (int j = 0; j < 32; ++j) stg[lane * 33 + j] = __uint_as_float(r[i & 1][j]) * p.alpha;
+          for (int j = 0; j < 32; ++j) stg[lane * 33 + j] = __uint_as_float(r[i & 1][j]) * alpha;
           __syncwarp();
           if (n0 < p.N && row0 < p.M) {
             if (p.out_f32) epi_store<float, 4>(p, stg, row0, n0, lane, cb, rb, mb);
@@ -990,14 +1010,14 @@ __global__ void __launch_bounds__(320, 1)
             const float rbv = (EPI < 2 && p.row_bias && row0 + lane < p.M) ? p.row_bias[row0 + lane] : 0.f;
             if constexpr (EPI == 4) {
               ce_logits(p, r[i & 1], n0, v);
-              ce_gradient(ce_m, ce_s, ce_g, ce_lab < 0 ? CE_ROW_OUT : ce_lab - n0, v);
+              ce_gradient(ce_m, ce_s, ce_lab < 0 ? CE_ROW_OUT : ce_lab - n0, v);
             } else if constexpr (EPI == 5) {
               ce_logits(p, r[i & 1], n0, v);
               ce_pick(p, row0 + lane, ce_lab - n0, v);
               ce_exponentials(ce_m, ce_s, v);
             } else {
 #pragma unroll
-              for (int j = 0; j < 32; ++j) v[j] = fmaf(__uint_as_float(r[i & 1][j]), p.alpha, rbv);
+              for (int j = 0; j < 32; ++j) v[j] = fmaf(__uint_as_float(r[i & 1][j]), alpha, rbv);
               if (p.bias && n0 < p.N) add_bias<32>(p.bias, p.bias_f32, n0, min(32, p.N - n0), v);
             }
             if (EPI < 2 && p.R) add_row_residual(p, rb, row0 + lane, n0, v);
@@ -1053,6 +1073,10 @@ __global__ void __launch_bounds__(320, 1)
 #pragma unroll
                 for (int j = 0; j < 32; ++j) v[j] = 0.f;
               }
+              if constexpr (EPI == 4) {
+#pragma unroll
+                for (int j = 0; j < 32; ++j) v[j] *= ce_g;
+              }
               colsum_chunk(p, row0, lane, n0, v);
             }
             if (!bf || (i & 1)) {
@@ -1073,10 +1097,10 @@ __global__ void __launch_bounds__(320, 1)
             float v[32];
             const float rbv = p.row_bias ? p.row_bias[row] : 0.f;
 #pragma unroll
-            for (int j = 0; j < 32; ++j) v[j] = fmaf(__uint_as_float(r[i & 1][j]), p.alpha, rbv);
+            for (int j = 0; j < 32; ++j) v[j] = fmaf(__uint_as_float(r[i & 1][j]), alpha, rbv);
             if (p.i8) {
               // int32 accumulators -> real values: alpha * acc * row_scale * col_scale
-              const float rs = p.alpha * p.row_scale[row];
+              const float rs = alpha * p.row_scale[row];
 #pragma unroll
               for (int j = 0; j < 32; ++j) v[j] = (float)(int)r[i & 1][j] * rs;
               float cs[32];
@@ -1308,7 +1332,7 @@ __global__ void splitk_reduce_kernel(const float* __restrict__ ws, int splits, i
     const int64_t m = r / a.N, n = r - m * a.N;
     const int64_t bo = b / a.batch2, bi = b - bo * a.batch2;
     T* c = reinterpret_cast<T*>(a.C) + bo * a.batch_stride_c + bi * a.batch2_stride_c + m * a.ldc + n;
-    float v = a.alpha * acc;
+    float v = (a.alpha_ptr ? a.alpha * *a.alpha_ptr : a.alpha) * acc;
     if (a.beta != 0.f) v += a.beta * to_f32(*c);
     if (a.bias)
       v += a.bias_dtype == (int)DType::F32 ? reinterpret_cast<const float*>(a.bias)[n]
@@ -1325,6 +1349,51 @@ __global__ void splitk_reduce_kernel(const float* __restrict__ ws, int splits, i
     if (a.relu_bits && !((a.relu_bits[m * a.ldbits + (n >> 5)] >> (n & 31)) & 1u)) v = 0.f;
 
     *c = from_f32<T>(v);
+  }
+}
+
+// The same for a plain 2-D GEMM (alpha, beta, bias) whose rows are whole
+// 16-byte steps of the output: four columns a thread, all splits' loads at
+// once (2 splits of 4096 x 1024: 35.5 us one element a thread).
+template <typename T>
+__global__ void __launch_bounds__(256) splitk_reduce4_kernel(const float* __restrict__ ws, int splits,
+                                                             int64_t per_split, GemmArgs a) {
+  const float alpha = a.alpha_ptr ? a.alpha * *a.alpha_ptr : a.alpha;
+  for (int64_t i = 4 * (blockIdx.x * (int64_t)blockDim.x + threadIdx.x); i < per_split;
+       i += 4 * (int64_t)gridDim.x * blockDim.x) {
+    float acc[4] = {0.f, 0.f, 0.f, 0.f};
+    int s = 0;
+    for (; s + 4 <= splits; s += 4) {
+      float4 u[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) u[k] = *reinterpret_cast<const float4*>(ws + (s + k) * per_split + i);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        acc[0] += u[k].x; acc[1] += u[k].y; acc[2] += u[k].z; acc[3] += u[k].w;
+      }
+    }
+    for (; s < splits; ++s) {
+      const float4 u = *reinterpret_cast<const float4*>(ws + s * per_split + i);
+      acc[0] += u.x; acc[1] += u.y; acc[2] += u.z; acc[3] += u.w;
+    }
+    const int64_t m = i / a.N, n = i - m * a.N;
+    T* c = reinterpret_cast<T*>(a.C) + m * a.ldc + n;
+    float v[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      v[k] = alpha * acc[k];
+      if (a.beta != 0.f) v[k] += a.beta * to_f32(c[k]);
+      if (a.bias)
+        v[k] += a.bias_dtype == (int)DType::F32 ? reinterpret_cast<const float*>(a.bias)[n + k]
+                                                : __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(a.bias)[n + k]);
+    }
+    if constexpr (sizeof(T) == 4) {
+      *reinterpret_cast<float4*>(c) = make_float4(v[0], v[1], v[2], v[3]);
+    } else {
+      const __nv_bfloat162 lo = __floats2bfloat162_rn(v[0], v[1]), hi = __floats2bfloat162_rn(v[2], v[3]);
+      *reinterpret_cast<uint2*>(c) = make_uint2(*reinterpret_cast<const uint32_t*>(&lo),
+                                                *reinterpret_cast<const uint32_t*>(&hi));
+    }
   }
 }
 
@@ -1363,7 +1432,7 @@ int streamk_mode() {
 void choose_tiling(const GemmArgs& a, int sms, int& BN, int& splits, bool& pair, bool red = false,
                    bool out_f32 = false, bool single_cta = false, bool* sk = nullptr) {
   if (sk) *sk = false;
-  const int64_t kbs = (a.K + BK - 1) / BK;
+  const int64_t kbs = (a.K + BK - 1) / BK, products = a.parts ? 6 : 1;
   const double sm_flops = 8.1e12;
   double best = 1e300;
   BN = 256;
@@ -1392,11 +1461,16 @@ void choose_tiling(const GemmArgs& a, int sms, int& BN, int& splits, bool& pair,
     const int64_t tile_m = c.pair ? 2 * BM : BM;
     const int64_t tiles = ((a.M + tile_m - 1) / tile_m) * ((a.N + c.bn - 1) / c.bn) * a.batch * a.batch2;
     const int64_t slots = c.pair ? sms / 2 : sms;
-    for (int sp : {1, 2, 3, 4, 6, 8}) {
-      if (sp > 1 && kbs / sp < 8) break;
+    for (int sp : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32}) {
+      if (sp > 8 && !a.parts) break;
+      if (sp > 1 && kbs * products / sp < 8) break;
+      // The accumulators lose a little with every addition (2^-24, always
+      // towards zero): at most 2048 elements of K for products that are to be
+      // as good as fp32, the rest is summed in the reduction.
+      if (a.parts && sp < 32 && (kbs + sp - 1) / sp > 32) continue;
       const int64_t units = tiles * sp;
       const int64_t waves = (units + slots - 1) / slots;
-      const double unit_s = (double)tile_m * c.bn * BK * 2.0 * ((kbs + sp - 1) / sp) /
+      const double unit_s = (double)tile_m * c.bn * BK * 2.0 * products * ((kbs + sp - 1) / sp) /
                             (sm_flops * (c.pair ? 2 : 1) * c.eff);
       // Epilogue of one CTA's 128 x BN block (measured: ~17 GB/s per CTA for
       // 128 x 256, ~18 GB/s for 128 x 512), exposed once at the end, or
@@ -1628,20 +1702,20 @@ void gemm_tc_impl(DType out_dt, const GemmArgs& a, cudaStream_t s, uint32_t* err
   const uint64_t ab2 = a_bcast ? 1 : (uint64_t)a.batch2, ab = a_bcast ? 1 : (uint64_t)a.batch;
   if (a_k) {
     const uint64_t d = (uint64_t)a.sam * (uint64_t)a.M;
-    ta = make_tmap(a.A, a.K, a.M, ab2, ab, a.sam, pick((int64_t)ab2, a.batch2_stride_a, d),
+    ta = make_tmap(a.A, a.parts ? 3 * a.pitch_a : a.K, a.M, ab2, ab, a.sam, pick((int64_t)ab2, a.batch2_stride_a, d),
                    pick((int64_t)ab, a.batch_stride_a, d), BM, el);
   } else {
     const uint64_t d = (uint64_t)a.sak * (uint64_t)a.K;
-    ta = make_tmap(a.A, a.M, a.K, ab2, ab, a.sak, pick((int64_t)ab2, a.batch2_stride_a, d),
+    ta = make_tmap(a.A, a.parts ? 3 * a.pitch_a : a.M, a.K, ab2, ab, a.sak, pick((int64_t)ab2, a.batch2_stride_a, d),
                    pick((int64_t)ab, a.batch_stride_a, d), (uint32_t)bke, el, true);
   }
   if (b_k) {
     const uint64_t d = (uint64_t)a.sbn * (uint64_t)a.N;
-    tb = make_tmap(a.B, a.K, a.N, a.batch2, a.batch, a.sbn, pick(a.batch2, a.batch2_stride_b, d),
+    tb = make_tmap(a.B, a.parts ? 3 * a.pitch_b : a.K, a.N, a.batch2, a.batch, a.sbn, pick(a.batch2, a.batch2_stride_b, d),
                         pick(a.batch, a.batch_stride_b, d), pair ? 128 : BN, el);
   } else {
     const uint64_t d = (uint64_t)a.sbk * (uint64_t)a.K;
-    tb = make_tmap(a.B, a.N, a.K, a.batch2, a.batch, a.sbk, pick(a.batch2, a.batch2_stride_b, d),
+    tb = make_tmap(a.B, a.parts ? 3 * a.pitch_b : a.N, a.K, a.batch2, a.batch, a.sbk, pick(a.batch2, a.batch2_stride_b, d),
                         pick(a.batch, a.batch_stride_b, d), (uint32_t)bke, el, true);
   }
   TcParams p{};
@@ -1675,6 +1749,10 @@ void gemm_tc_impl(DType out_dt, const GemmArgs& a, cudaStream_t s, uint32_t* err
   p.m_vec = a.relu_mask && al16(a.relu_mask) && ((a.ldm * esz) % 16 == 0) && ((a.batch_stride_m * esz) % 16 == 0) &&
             ((a.batch2_stride_m * esz) % 16 == 0);
   p.alpha = a.alpha;
+  p.alpha_ptr = a.alpha_ptr;
+  p.products = a.parts ? 6 : 1;
+  p.a_pitch = (int)a.pitch_a;
+  p.b_pitch = (int)a.pitch_b;
   p.beta = a.beta;
   p.bias = a.bias;
   p.bias_f32 = (a.bias_dtype == (int)DType::F32);
@@ -1689,6 +1767,9 @@ void gemm_tc_impl(DType out_dt, const GemmArgs& a, cudaStream_t s, uint32_t* err
   p.tf32 = tf32 ? 1 : 0;
   p.splits = splits;
   p.kb_per_split = (int)(((a.K + bke - 1) / bke + splits - 1) / splits);
+  // rounding up may leave nothing for the last splits
+  splits = std::min(splits, (int)(((a.K + bke - 1) / bke + p.kb_per_split - 1) / p.kb_per_split));
+  p.splits = splits;
   p.split_stride = 0;
   p.sk = sk ? 1 : 0;
   if ((splits > 1 || sk) && red) {
@@ -1725,6 +1806,7 @@ void gemm_tc_impl(DType out_dt, const GemmArgs& a, cudaStream_t s, uint32_t* err
     p.split_stride = per;
     p.vec_ok = al16(workspace) && (a.N % 4 == 0);
     p.alpha = 1.f;
+    p.alpha_ptr = nullptr;
     p.beta = 0.f;
     p.bias = nullptr;
     p.row_bias = nullptr;
@@ -1737,8 +1819,14 @@ void gemm_tc_impl(DType out_dt, const GemmArgs& a, cudaStream_t s, uint32_t* err
     else if (pair) launch_tc_pair<256>(ta, tb, tc, p, max_ctas, s);
     else if (BN == 256) launch_tc<256>(ta, tb, tc, p, max_ctas, s);
     else launch_tc<128>(ta, tb, tc, p, max_ctas, s);
+    const bool plain = a.batch == 1 && a.batch2 == 1 && !a.row_bias && !a.residual && a.act == ACT_NONE &&
+                       !a.relu_mask && !a.relu_bits && a.N % 4 == 0 && a.ldc % 4 == 0 && al16(a.C) && al16(workspace);
     const int g = (int)std::min<int64_t>((per + 255) / 256, 148 * 16);
-    if (out_dt == DType::F32) splitk_reduce_kernel<float><<<g, 256, 0, s>>>(workspace, splits, per, a);
+    if (plain) {
+      const int g4 = (int)std::min<int64_t>((per / 4 + 255) / 256, 148 * 8);
+      if (out_dt == DType::F32) splitk_reduce4_kernel<float><<<g4, 256, 0, s>>>(workspace, splits, per, a);
+      else splitk_reduce4_kernel<__nv_bfloat16><<<g4, 256, 0, s>>>(workspace, splits, per, a);
+    } else if (out_dt == DType::F32) splitk_reduce_kernel<float><<<g, 256, 0, s>>>(workspace, splits, per, a);
     else splitk_reduce_kernel<__nv_bfloat16><<<g, 256, 0, s>>>(workspace, splits, per, a);
     DLVK_POST_LAUNCH();
     return;
@@ -1841,14 +1929,14 @@ void ce_launch(const CeProjection& c, void* out, int64_t ldo, float* colsum, cud
   tmap::bind_context();
   const CeTiling t = ce_tiling(c.rows, c.classes);
   const uint64_t da = (uint64_t)c.ldx * (uint64_t)c.rows;
-  const CUtensorMap ta = make_tmap(c.x, c.width, c.rows, 1, 1, c.ldx, da, da, BM, Elem::BF16);
+  const CUtensorMap ta = make_tmap(c.x, c.parts ? 3 * c.pitch_x : c.width, c.rows, 1, 1, c.ldx, da, da, BM, Elem::BF16);
   CUtensorMap tb;
   if (c.w_k) {
     const uint64_t d = (uint64_t)c.ldw * (uint64_t)c.classes;
-    tb = make_tmap(c.w, c.width, c.classes, 1, 1, c.ldw, d, d, t.pair ? 128 : t.bn, Elem::BF16);
+    tb = make_tmap(c.w, c.parts ? 3 * c.pitch_w : c.width, c.classes, 1, 1, c.ldw, d, d, t.pair ? 128 : t.bn, Elem::BF16);
   } else {
     const uint64_t d = (uint64_t)c.ldw * (uint64_t)c.width;
-    tb = make_tmap(c.w, c.classes, c.width, 1, 1, c.ldw, d, d, BK, Elem::BF16, true);
+    tb = make_tmap(c.w, c.parts ? 3 * c.pitch_w : c.classes, c.width, 1, 1, c.ldw, d, d, BK, Elem::BF16, true);
   }
   TcParams p{};
   p.M = (int)c.rows;
@@ -1859,6 +1947,9 @@ void ce_launch(const CeProjection& c, void* out, int64_t ldo, float* colsum, cud
   p.tiles_n = (int)((c.classes + t.bn - 1) / t.bn);
   p.b_mn = c.w_k ? 0 : 1;
   p.alpha = 1.f;
+  p.products = c.parts ? 6 : 1;
+  p.a_pitch = (int)c.pitch_x;
+  p.b_pitch = (int)c.pitch_w;
   p.bias = c.bias;
   p.bias_f32 = 1;
   p.err = err;
@@ -1973,6 +2064,7 @@ void gemm_i8_tc(const int8_t* A, const int8_t* Bt, const float* row_scale, const
   p.splits = 1;
   p.kb_per_split = (int)((K + 2 * BK - 1) / (2 * BK));
   p.i8 = 1;
+  p.products = 1;
   p.row_scale = row_scale;
   p.col_scale = col_scale;
   if (BN == 256) launch_tc<256>(ta, tb, ta, p, 0, s);

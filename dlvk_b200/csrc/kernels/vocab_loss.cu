@@ -34,6 +34,19 @@ __device__ __forceinline__ int row_label(const CeRows& r, int64_t i) {
   return (lab >= 0 && lab < r.classes && lab != r.ignore) ? (int)lab : -1;
 }
 
+// x = q0 + q1 + q2 to 2^-24 of x, bf16 each: what rounding leaves is exact in
+// fp32 and goes to the next part.  An infinity or NaN is in q0 alone, and a
+// finite x above bf16's range is held at its end.
+__device__ __forceinline__ void three_parts(float x, __nv_bfloat16* q) {
+  q[0] = __float2bfloat16_rn(x);
+  q[1] = q[2] = __float2bfloat16_rn(0.f);
+  if (!isfinite(x)) return;
+  if (fabsf(x) > 3.38953139e38f) q[0] = __float2bfloat16_rn(copysignf(3.38953139e38f, x));
+  const float a = x - __bfloat162float(q[0]);
+  q[1] = __float2bfloat16_rn(a);
+  q[2] = __float2bfloat16_rn(a - __bfloat162float(q[1]));
+}
+
 // (m, s) joined with (m2, s2), s = sum of exp(z - m); a maximum of -inf stands
 // for "every logit masked" (its s is 0, or NaN when a NaN was among them).
 // The scaling to powers of 2 comes after the difference, which a mask of
@@ -181,21 +194,19 @@ __global__ void __launch_bounds__(FIN_WARPS * 32) finish_kernel(CeRows r, CeFini
 // bytes in, 2 out per logit.
 constexpr int RS_COLS = 2048, RS_ROWS = 32;
 __global__ void __launch_bounds__(256) rescale_kernel(CeRows r, const float2* __restrict__ stats, int width_shift,
-                                                      const float2* __restrict__ norm,
-                                                      const float* __restrict__ gscale, uint16_t* __restrict__ e,
+                                                      const float2* __restrict__ norm, uint16_t* __restrict__ e,
                                                       int64_t lde) {
   __shared__ float factor[RS_COLS / 64][RS_ROWS];
   __shared__ int label[RS_ROWS];
   const int64_t row0 = (int64_t)blockIdx.y * RS_ROWS, col0 = (int64_t)blockIdx.x * RS_COLS;
   const int rows = (int)min((int64_t)RS_ROWS, r.rows - row0);
-  const float g = *gscale;
   const int64_t stat0 = col0 >> width_shift, stats_all = (r.classes + (1 << width_shift) - 1) >> width_shift;
   for (int i = threadIdx.x; i < (RS_COLS >> width_shift) * RS_ROWS; i += 256) {
     const int k = i % RS_ROWS, t = i / RS_ROWS;
     float v = 0.f;
     if (k < rows && stat0 + t < stats_all) {
       const float2 n = norm[row0 + k];
-      v = exp2f((stats[(stat0 + t) * r.rows + row0 + k].x - n.x) * LOG2E) * n.y * g * (1.f / 32768.f);
+      v = exp2f((stats[(stat0 + t) * r.rows + row0 + k].x - n.x) * LOG2E) * n.y * (1.f / 32768.f);
     }
     factor[t][k] = v;
   }
@@ -229,7 +240,7 @@ __global__ void __launch_bounds__(256) rescale_kernel(CeRows r, const float2* __
         for (int j = 0; j < 8; ++j) v[j] = 0.f;
       } else if (at >= 0 && at < 8) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] -= j == at ? g : 0.f;
+        for (int j = 0; j < 8; ++j) v[j] -= j == at ? 1.f : 0.f;
       }
       uint4 o;
       __nv_bfloat162* w = reinterpret_cast<__nv_bfloat162*>(&o);
@@ -281,21 +292,64 @@ __global__ void __launch_bounds__(256) memory_stats_kernel(CeRows r, const float
 __global__ void __launch_bounds__(256) memory_grad_kernel(CeRows r, float* __restrict__ z, int64_t ldz,
                                                           const float2* __restrict__ norm,
                                                           const float* __restrict__ gscale,
-                                                          __nv_bfloat16* __restrict__ dl) {
+                                                          __nv_bfloat16* __restrict__ dl, int64_t pitch) {
   const int64_t row = blockIdx.x;
   float* p = z + row * ldz;
   const int lab = row_label(r, row);
   const float g = *gscale;
   const float2 n = norm[row];
-  const float f = n.y * g;
   for (int64_t c = threadIdx.x; c < r.classes; c += 256) {
     float v = 0.f;
     if (lab >= 0) {
-      v = exp2f((p[c] - n.x) * LOG2E) * f;
-      if (c == lab) v -= g;
+      v = exp2f((p[c] - n.x) * LOG2E) * n.y;
+      if (c == lab) v -= 1.f;
     }
-    p[c] = v;
-    if (dl) dl[row * ldz + c] = __float2bfloat16_rn(v);
+    p[c] = v * g;
+    if (dl == nullptr) continue;
+    if (pitch == 0) {
+      dl[row * ldz + c] = __float2bfloat16_rn(v * g);
+    } else {
+      __nv_bfloat16 q[3];
+      three_parts(v, q);
+#pragma unroll
+      for (int k = 0; k < 3; ++k) dl[row * 3 * pitch + k * pitch + c] = q[k];
+    }
+  }
+  if (pitch != 0)
+    for (int64_t c = r.classes + threadIdx.x; c < pitch; c += 256)
+#pragma unroll
+      for (int k = 0; k < 3; ++k) dl[row * 3 * pitch + k * pitch + c] = __float2bfloat16_rn(0.f);
+}
+
+// A block splits rows blockIdx.y, ...; a thread four columns.
+__global__ void __launch_bounds__(256) split_parts_kernel(const float* __restrict__ src, int64_t ld, int64_t rows,
+                                                          int64_t cols, __nv_bfloat16* __restrict__ dst, int64_t pitch,
+                                                          CeRows mask, int masked, int vec) {
+  const int64_t c = 4 * ((int64_t)blockIdx.x * 256 + threadIdx.x);
+  if (c >= pitch) return;
+  for (int64_t i = blockIdx.y; i < rows; i += gridDim.y) {
+    float v[4] = {0.f, 0.f, 0.f, 0.f};
+    if (!masked || row_label(mask, i) >= 0) {
+      const float* p = src + i * ld + c;
+      if (vec && c + 4 <= cols) {
+        const float4 u = *reinterpret_cast<const float4*>(p);
+        v[0] = u.x; v[1] = u.y; v[2] = u.z; v[3] = u.w;
+      } else {
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          if (c + k < cols) v[k] = p[k];
+      }
+    }
+    __nv_bfloat16 q[4][3];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) three_parts(v[k], q[k]);
+#pragma unroll
+    for (int t = 0; t < 3; ++t) {
+      __nv_bfloat162 a, b;
+      a.x = q[0][t]; a.y = q[1][t]; b.x = q[2][t]; b.y = q[3][t];
+      *reinterpret_cast<uint2*>(dst + i * 3 * pitch + t * pitch + c) =
+          make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+    }
   }
 }
 
@@ -313,6 +367,35 @@ __global__ void __launch_bounds__(256) copy_matrix_kernel(const TS* __restrict__
         if (accumulate) v += to_f32(dst[i * ldd + j]);
         dst[i * ldd + j] = from_f32<TD>(v);
       }
+    }
+  }
+}
+
+// fp32 -> bf16 of rows of whole 16-byte steps, eight elements a thread.
+__global__ void __launch_bounds__(256) round_matrix_kernel(const float* __restrict__ src, int64_t rs,
+                                                           __nv_bfloat16* __restrict__ dst, int64_t ldd, int64_t rows,
+                                                           int64_t cols) {
+  const int64_t c = 8 * ((int64_t)blockIdx.x * 256 + threadIdx.x);
+  if (c >= cols) return;
+  for (int64_t i = blockIdx.y; i < rows; i += 2 * (int64_t)gridDim.y) {
+    float4 u[2][2];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      if (i + k * (int64_t)gridDim.y >= rows) break;
+      const float4* p = reinterpret_cast<const float4*>(src + (i + k * (int64_t)gridDim.y) * rs + c);
+      u[k][0] = p[0];
+      u[k][1] = p[1];
+    }
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      if (i + k * (int64_t)gridDim.y >= rows) break;
+      uint4 o;
+      __nv_bfloat162* w = reinterpret_cast<__nv_bfloat162*>(&o);
+      w[0] = __floats2bfloat162_rn(u[k][0].x, u[k][0].y);
+      w[1] = __floats2bfloat162_rn(u[k][0].z, u[k][0].w);
+      w[2] = __floats2bfloat162_rn(u[k][1].x, u[k][1].y);
+      w[3] = __floats2bfloat162_rn(u[k][1].z, u[k][1].w);
+      *reinterpret_cast<uint4*>(dst + (i + k * (int64_t)gridDim.y) * ldd + c) = o;
     }
   }
 }
@@ -348,12 +431,12 @@ void ce_finish(const CeRows& r, const CeFinish& f, DType dt, cudaStream_t s) {
   else finish_t<__nv_bfloat16>(r, f, s);
 }
 
-void ce_rescale(const CeRows& r, const float2* stats, int stat_width, const float2* norm, const float* gscale, void* e,
-                int64_t lde, cudaStream_t s) {
+void ce_rescale(const CeRows& r, const float2* stats, int stat_width, const float2* norm, void* e, int64_t lde,
+                cudaStream_t s) {
   DLVK_CHECK((stat_width == 64 || stat_width == 128) && lde % 8 == 0 && al16(e), "ce_rescale: layout");
   const dim3 grid((unsigned)((r.classes + RS_COLS - 1) / RS_COLS), (unsigned)((r.rows + RS_ROWS - 1) / RS_ROWS));
   DLVK_CHECK(grid.y <= 65535u, "ce_rescale: more than 2^21 rows in one block of rows");
-  rescale_kernel<<<grid, 256, 0, s>>>(r, stats, stat_width == 64 ? 6 : 7, norm, gscale,
+  rescale_kernel<<<grid, 256, 0, s>>>(r, stats, stat_width == 64 ? 6 : 7, norm,
                                       reinterpret_cast<uint16_t*>(e), lde);
   DLVK_POST_LAUNCH();
 }
@@ -365,14 +448,32 @@ void ce_memory_stats(const CeRows& r, const float* z, int64_t ldz, float2* stats
 }
 
 void ce_memory_grad(const CeRows& r, float* z, int64_t ldz, const float2* norm, const float* gscale, __nv_bfloat16* dl,
-                    cudaStream_t s) {
-  memory_grad_kernel<<<(unsigned)r.rows, 256, 0, s>>>(r, z, ldz, norm, gscale, dl);
+                    int64_t pitch, cudaStream_t s) {
+  memory_grad_kernel<<<(unsigned)r.rows, 256, 0, s>>>(r, z, ldz, norm, gscale, dl, pitch);
+  DLVK_POST_LAUNCH();
+}
+
+void split_parts(const float* src, int64_t ld, int64_t rows, int64_t cols, __nv_bfloat16* dst, int64_t pitch,
+                 const CeRows* mask, cudaStream_t s) {
+  DLVK_CHECK(pitch % 64 == 0 && pitch >= cols && al16(dst), "split_parts: layout");
+  if (rows == 0) return;
+  const dim3 grid((unsigned)((pitch + 1023) / 1024), (unsigned)std::min<int64_t>(rows, 16384));
+  split_parts_kernel<<<grid, 256, 0, s>>>(src, ld, rows, cols, dst, pitch, mask ? *mask : CeRows{}, mask != nullptr,
+                                          al16(src) && ld % 4 == 0);
   DLVK_POST_LAUNCH();
 }
 
 void copy_matrix(DType dst_dt, DType src_dt, const void* src, int64_t rs, int64_t cs, void* dst, int64_t ldd,
                  int64_t rows, int64_t cols, int64_t pad_to, bool accumulate, cudaStream_t s) {
   if (rows == 0 || pad_to == 0) return;
+  if (dst_dt == DType::BF16 && src_dt == DType::F32 && cs == 1 && !accumulate && cols == pad_to && cols % 8 == 0 &&
+      rs % 4 == 0 && ldd % 8 == 0 && al16(src) && al16(dst)) {
+    const dim3 grid((unsigned)((cols / 8 + 255) / 256), (unsigned)std::min<int64_t>((rows + 1) / 2, 4096));
+    round_matrix_kernel<<<grid, 256, 0, s>>>(reinterpret_cast<const float*>(src), rs,
+                                             reinterpret_cast<__nv_bfloat16*>(dst), ldd, rows, cols);
+    DLVK_POST_LAUNCH();
+    return;
+  }
   if (dst_dt == DType::F32 && src_dt == DType::F32)
     copy_matrix_t<float, float>(src, rs, cs, dst, ldd, rows, cols, pad_to, accumulate, s);
   else if (dst_dt == DType::F32)
