@@ -102,7 +102,9 @@ __device__ __forceinline__ int part_b(int i) { return (0x010120 >> (4 * i)) & 15
 
 // PAIR: a 2-CTA cluster shares one 256 x BN tile (tcgen05 cta_group::2);
 // each CTA stages its 128 rows of A and its BN/2 columns of B.
-template <int BN, bool PAIR = false>
+// EXTRA: one stage fewer, whose room is a second TMA-store box per epilogue
+// warp (EPI 5 fills two boxes a tile between its other work).
+template <int BN, bool PAIR = false, bool EXTRA = false>
 // BN = 512 (PAIR only): the tile is two N = 256 MMAs per k-step; each CTA
 // stages two 128-column B sub-blocks, and the 512 accumulator columns fill
 // TMEM, so there is one accumulator buffer instead of two.
@@ -110,7 +112,7 @@ struct Cfg {
   static constexpr int A_BYTES = BM * BK * 2;
   static constexpr int B_BYTES = (PAIR ? BN / 2 : BN) * BK * 2;
   static constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
-  static constexpr int STAGES = PAIR ? (BN == 512 ? 4 : 6) : ((BN == 256) ? 4 : 6);
+  static constexpr int STAGES = (PAIR ? (BN == 512 ? 4 : 6) : ((BN == 256) ? 4 : 6)) - (EXTRA ? 1 : 0);
   static constexpr int ACCS = 2 * BN <= 512 ? 2 : 1;      // TMEM accumulator buffers
   static constexpr int TMEM_COLS = ACCS * BN;
   static constexpr int MMA_N = BN > 256 ? 256 : BN;        // N of one tcgen05.mma
@@ -119,8 +121,9 @@ struct Cfg {
   static_assert(!(BN == 512) || PAIR, "the 512-column tile is a CTA-pair tile");
   // per-warp 32x33 fp32 staging; also holds the TMA-store boxes (8 x 4 KB
   // from the next 1024-byte boundary)
-  static constexpr int EPI_BYTES = 8 * 32 * 33 * 4;
-  static_assert(EPI_BYTES >= 768 + 8 * 4096, "epilogue smem too small for the TMA-store boxes");
+  static constexpr int BOXES = EXTRA ? 2 : 1;  // boxes of a warp
+  static constexpr int EPI_BYTES = EXTRA ? 768 + 16 * 4096 : 8 * 32 * 33 * 4;
+  static_assert(EPI_BYTES >= 768 + 8 * BOXES * 4096, "epilogue smem too small for the TMA-store boxes");
   static constexpr int SMEM = STAGES * STAGE_BYTES + 1024 /*align*/ + 256 /*barriers*/ + EPI_BYTES;
   static_assert(SMEM <= 232448, "shared memory above the per-block limit");
   static_assert(STAGES * STAGE_BYTES / 8 >= 4096, "last-tile epilogue needs a 4 KB box per warp");
@@ -334,6 +337,12 @@ __device__ __forceinline__ void store_bits(const TcParams& p, int row, int n0, c
   for (int j = 0; j < 32; ++j) w |= (v[j] > 0.f ? 1u : 0u) << j;
   if (p.N - n0 < 32) w &= (1u << (p.N - n0)) - 1u;
   p.bits_out[(int64_t)row * p.ldbits + (n0 >> 5)] = w;
+}
+
+// The factor of the accumulators, read where it is used: a register held over
+// the whole epilogue made the largest instantiations spill.
+__device__ __forceinline__ float alpha_of(const TcParams& p) {
+  return p.alpha_ptr != nullptr ? p.alpha * *p.alpha_ptr : p.alpha;
 }
 
 template <typename T> __device__ __forceinline__ float ld_elem(const void* p, int64_t i) {
@@ -551,33 +560,50 @@ __device__ __forceinline__ float ce_max(const float* v, float m) {
   return fmaxf(m, t[0]);
 }
 
-// Folds 32 logits into the running (maximum, sum of exp(z - maximum)).  A
-// maximum of -inf (every logit so far masked) is replaced by 0 in the
-// exponents, which then are exp(-inf) = 0; a NaN logit makes the sum NaN.
-// The maximum is taken off before the scaling to powers of 2, in a step of
-// its own: -3.4e38 (a mask of fp32's lowest value) times log2 e would be -inf.
-__device__ __forceinline__ void ce_online(const float* v, float& m, float& s) {
-  const float mn = ce_max(v, m);
-  const float c = mn == -INFINITY ? 0.f : mn;
-  s *= ex2((m - c) * LOG2E);
-  float a[4] = {0.f, 0.f, 0.f, 0.f};
+// v = 2^((v - m) log2 e + up), in pairs: one fma each.  A maximum of -inf
+// (every logit masked) is replaced by 0: the results are exp(-inf) = 0.  One
+// near fp32's lowest value (masks of -3.4e38) times log2 e would be -inf, so
+// there the difference is taken first.
+__device__ __forceinline__ void ce_exp32(float m, float up, float* v) {
+  if (m < -2e38f && m != -INFINITY) {
 #pragma unroll
-  for (int j = 0; j < 32; ++j) a[j & 3] += ex2((v[j] - c) * LOG2E);
-  s += (a[0] + a[1]) + (a[2] + a[3]);
+    for (int j = 0; j < 32; ++j) v[j] = ex2((v[j] - m) * LOG2E + up);
+    return;
+  }
+  const float c = m == -INFINITY ? up : fmaf(m, -LOG2E, up);
+  const float2 l2 = make_float2(LOG2E, LOG2E), c2 = make_float2(c, c);
+#pragma unroll
+  for (int j = 0; j < 32; j += 2) {
+    const float2 x = __ffma2_rn(make_float2(v[j], v[j + 1]), l2, c2);
+    v[j] = ex2(x.x);
+    v[j + 1] = ex2(x.y);
+  }
+}
+
+__device__ __forceinline__ float sum32(const float* v) {
+  float2 a[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) a[j] = make_float2(v[2 * j], v[2 * j + 1]);
+#pragma unroll
+  for (int j = 4; j < 16; ++j) a[j & 3] = __fadd2_rn(a[j & 3], make_float2(v[2 * j], v[2 * j + 1]));
+  const float2 t = __fadd2_rn(__fadd2_rn(a[0], a[1]), __fadd2_rn(a[2], a[3]));
+  return t.x + t.y;
+}
+
+// Folds 32 logits into the running (maximum, sum of exp(z - maximum)); a NaN
+// logit makes the sum NaN.  v is consumed.
+__device__ __forceinline__ void ce_online(float* v, float& m, float& s) {
+  const float mn = ce_max(v, m);
+  s *= ex2((m - (mn == -INFINITY ? 0.f : mn)) * LOG2E);
+  ce_exp32(mn, 0.f, v);
+  s += sum32(v);
   m = mn;
 }
 
-// v = 2^15 exp(v - m); s += the sum of exp(v - m).
+// v = 2^15 exp(v - m); s += its sum.
 __device__ __forceinline__ void ce_exponentials(float m, float& s, float* v) {
-  float a[4] = {0.f, 0.f, 0.f, 0.f};
-  const float c = m == -INFINITY ? 0.f : m;
-#pragma unroll
-  for (int j = 0; j < 32; ++j) {
-    v[j] = ex2((v[j] - c) * LOG2E);
-    a[j & 3] += v[j];
-    v[j] *= CE_EXP_SCALE;
-  }
-  s += (a[0] + a[1]) + (a[2] + a[3]);
+  ce_exp32(m, 15.f, v);
+  s += sum32(v);
 }
 
 // The logit of the row's class, when it is one of these 32.
@@ -593,8 +619,9 @@ __device__ __forceinline__ void ce_pick(const TcParams& p, int row, int at, cons
 // v[j] = softmax - onehot, for a row that does not count 0 whatever its
 // logits are; f = 1 / sum.
 __device__ __forceinline__ void ce_gradient(float m, float f, int at, float* v) {
+  ce_exp32(m, 0.f, v);
 #pragma unroll
-  for (int j = 0; j < 32; ++j) v[j] = ex2((v[j] - m) * LOG2E) * f;
+  for (int j = 0; j < 32; ++j) v[j] *= f;
   if ((unsigned)at < 32u) {  // one chunk of the whole row
 #pragma unroll
     for (int j = 0; j < 32; ++j) v[j] -= j == at ? 1.f : 0.f;
@@ -616,7 +643,7 @@ template <int BN, bool PAIR = false, int EPI = 0>
 __global__ void __launch_bounds__(320, 1)
     gemm_tc_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                    const __grid_constant__ CUtensorMap tmC, TcParams p) {
-  using C = Cfg<BN, PAIR>;
+  using C = Cfg<BN, PAIR, (EPI >= 4)>;
   GEMM_STAMP(threadIdx.x == 0, 4);
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -909,7 +936,6 @@ __global__ void __launch_bounds__(320, 1)
     // path, which handles all three.
     const bool staged = (p.beta != 0.f) || (p.out_f32 && (p.R != nullptr || p.Mk != nullptr));
     constexpr int NCH = BN / 64;  // 32-column chunks per warp
-    const float alpha = p.alpha_ptr != nullptr ? p.alpha * *p.alpha_ptr : p.alpha;
     int acc = 0, ecount = 0;
     uint32_t acc_phase = 0;
     // TMA-store boxes (4 KB): one slot per warp in the epilogue area, so each
@@ -982,10 +1008,11 @@ __global__ void __launch_bounds__(320, 1)
           if (n0 < p.N) {
             float v[32];
             ce_logits(p, r[i & 1], n0, v);
-            ce_online(v, ce_m, ce_s);
             ce_pick(p, row0 + lane, ce_lab - n0, v);
+            ce_online(v, ce_m, ce_s);
           }
         } else if (EPI == 0 && staged) {
+          const float alpha = alpha_of(p);
 #pragma unroll
           for (int j = 0; j < 32; ++j) stg[lane * 33 + j] = __uint_as_float(r[i & 1][j]) * alpha;
           __syncwarp();
@@ -1016,6 +1043,7 @@ __global__ void __launch_bounds__(320, 1)
               ce_pick(p, row0 + lane, ce_lab - n0, v);
               ce_exponentials(ce_m, ce_s, v);
             } else {
+              const float alpha = alpha_of(p);
 #pragma unroll
               for (int j = 0; j < 32; ++j) v[j] = fmaf(__uint_as_float(r[i & 1][j]), alpha, rbv);
               if (p.bias && n0 < p.N) add_bias<32>(p.bias, p.bias_f32, n0, min(32, p.N - n0), v);
@@ -1034,8 +1062,8 @@ __global__ void __launch_bounds__(320, 1)
                 if (tcount > 0 && tcount % nslot == 0 && lane == 0) bulk_wait_group_read<0>();
               } else {
                 box = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(epi) + 1023) & ~uintptr_t(1023)) +
-                      ew * 4096;
-                if (lane == 0) bulk_wait_group_read<0>();
+                      (ew * C::BOXES + ecount % C::BOXES) * 4096;
+                if (lane == 0) bulk_wait_group_read<C::BOXES - 1>();
               }
               __syncwarp();
             }
@@ -1096,6 +1124,7 @@ __global__ void __launch_bounds__(320, 1)
           if (row < p.M && n0 < p.N) {
             float v[32];
             const float rbv = p.row_bias ? p.row_bias[row] : 0.f;
+            const float alpha = alpha_of(p);
 #pragma unroll
             for (int j = 0; j < 32; ++j) v[j] = fmaf(__uint_as_float(r[i & 1][j]), alpha, rbv);
             if (p.i8) {
@@ -1151,7 +1180,8 @@ __global__ void __launch_bounds__(320, 1)
       }
       if constexpr (EPI == 3 || EPI == 5) {
         if (row0 + lane < p.M)
-          p.ce.stats[(int64_t)(2 * tn + half) * p.M + row0 + lane] = make_float2(ce_m, ce_s);
+          p.ce.stats[(int64_t)(2 * tn + half) * p.M + row0 + lane] =
+              make_float2(ce_m, EPI == 5 ? ce_s * (1.f / CE_EXP_SCALE) : ce_s);
       }
       GEMM_STAMP(threadIdx.x == 64 && last_tile, 14);
       tc_fence_before();
@@ -1247,7 +1277,7 @@ int epi_kind(const TcParams& p) {
 template <int BN, int EPI>
 void launch_tc_k(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& tc, const TcParams& p, int max_ctas,
                  cudaStream_t s) {
-  using C = Cfg<BN>;
+  using C = Cfg<BN, false, (EPI >= 4)>;
   static bool attr_set[kMaxDevices] = {false};
   const int dev = current_device_slot();
   if (!attr_set[dev]) {
@@ -1275,7 +1305,7 @@ void launch_tc(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& 
 template <int BN, int EPI>
 void launch_tc_pair_k(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& tc, const TcParams& p,
                       int max_ctas, cudaStream_t s) {
-  using C = Cfg<BN, true>;
+  using C = Cfg<BN, true, (EPI >= 4)>;
   static int max_pairs[kMaxDevices] = {0};
   const int dev = current_device_slot();
   cudaLaunchConfig_t cfg = {};
