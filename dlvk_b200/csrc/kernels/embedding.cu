@@ -79,6 +79,26 @@ __global__ void __launch_bounds__(256) lookup_kernel(const ID* __restrict__ ids,
 }
 
 // ---------------------------------------------------------------- sort
+// Writing the zero rows is most of the gradient's traffic (32000 words of
+// 1024: 131 MB, of which 8192 tokens touch a tenth), and the sort and the last
+// joining pass are bound by latency.  So the rows are shared out over the
+// three launches: [0, Z1) are cleared beside the sort, before it is known
+// which have tokens, [Z1, Z2) and [Z2, V) where they have none, beside the
+// sums and the joins.
+__device__ __forceinline__ void clear_row(float* row, int D, int vec, int lane) {
+  if (vec) {
+    for (int c = lane * 4; c < D; c += 128) *reinterpret_cast<float4*>(row + c) = make_float4(0.f, 0.f, 0.f, 0.f);
+  } else {
+    for (int c = lane; c < D; c += 32) row[c] = 0.f;
+  }
+}
+// A warp of `warps` takes every warps-th word of [v0, v1) that has no token.
+__device__ __forceinline__ void clear_empty_rows(const int* start, float* dtable, int v0, int v1, int D, int vec,
+                                                 int warp, int warps) {
+  for (int v = v0 + warp; v < v1; v += warps)
+    if (start[v] == start[v + 1]) clear_row(dtable + (int64_t)v * D, D, vec, threadIdx.x & 31);
+}
+
 // Stable sort of the tokens by word in one launch, without a word between
 // blocks.  Block b owns the words [b R, (b + 1) R) and reads all ids twice:
 // once to count its own words (per warp: warp w has the w-th part of the ids)
@@ -92,7 +112,15 @@ __global__ void __launch_bounds__(256) lookup_kernel(const ID* __restrict__ ids,
 template <typename ID>
 __global__ void __launch_bounds__(SORT_THREADS) sort_tokens_kernel(const ID* __restrict__ ids, int n, int V, int R,
                                                                    int padding, int* __restrict__ start,
-                                                                   int* __restrict__ order, int* __restrict__ word) {
+                                                                   int* __restrict__ order, int* __restrict__ word,
+                                                                   int sort_blocks, float* __restrict__ dtable,
+                                                                   int clear_to, int D, int vec) {
+  if ((int)blockIdx.x >= sort_blocks) {
+    const int warps = (gridDim.x - sort_blocks) * SORT_WARPS;
+    for (int v = (blockIdx.x - sort_blocks) * SORT_WARPS + (threadIdx.x >> 5); v < clear_to; v += warps)
+      clear_row(dtable + (int64_t)v * D, D, vec, threadIdx.x & 31);
+    return;
+  }
   extern __shared__ int cnt[];  // [SORT_WARPS][R]
   __shared__ int warp_part[SORT_WARPS];
   __shared__ int before_sm;
@@ -203,7 +231,7 @@ __device__ __forceinline__ void put_row(float* dst, const float* acc, float scal
 }
 
 // The first blocks sum chunks of C consecutive places of the order; the rest
-// write the zero rows.  TX threads go across a row, 256 / TX chunks to a
+// write zero rows.  TX threads go across a row, 256 / TX chunks to a
 // block.  A word whose tokens lie in one chunk is finished here; what a chunk
 // has of a word that continues from the chunk before goes to part[2 chunk],
 // of one that begins here and continues to part[2 chunk + 1] (join_kernel).
@@ -211,19 +239,11 @@ template <typename T, int VEC>
 __global__ void __launch_bounds__(RED_THREADS) sum_chunks_kernel(
     const T* __restrict__ dy, int64_t ld, const int* __restrict__ start, const int* __restrict__ order,
     const int* __restrict__ word, float* __restrict__ dtable, float* __restrict__ part, int V, int D, int C, int TX,
-    int chunk_blocks, float scale, int accumulate) {
+    int chunk_blocks, float scale, int accumulate, int clear_from, int clear_to) {
   if ((int)blockIdx.x >= chunk_blocks) {
-    // zero rows: a warp takes every warps-th word
-    const int warps = (gridDim.x - chunk_blocks) * (RED_THREADS / 32), lane = threadIdx.x & 31;
-    for (int v = (blockIdx.x - chunk_blocks) * (RED_THREADS / 32) + (threadIdx.x >> 5); v < V; v += warps) {
-      if (start[v] != start[v + 1]) continue;
-      float* row = dtable + (int64_t)v * D;
-      if constexpr (VEC > 1) {
-        for (int c = lane * 4; c < D; c += 128) *reinterpret_cast<float4*>(row + c) = make_float4(0.f, 0.f, 0.f, 0.f);
-      } else {
-        for (int c = lane; c < D; c += 32) row[c] = 0.f;
-      }
-    }
+    clear_empty_rows(start, dtable, clear_from, clear_to, D, VEC > 1,
+                     (blockIdx.x - chunk_blocks) * (RED_THREADS / 32) + (threadIdx.x >> 5),
+                     (gridDim.x - chunk_blocks) * (RED_THREADS / 32));
     return;
   }
   const int tx = threadIdx.x % TX;
@@ -271,7 +291,13 @@ template <int VEC>
 __global__ void __launch_bounds__(RED_THREADS) join_kernel(const int* __restrict__ start, const int* __restrict__ word,
                                                            const float* __restrict__ part, float* __restrict__ dtable,
                                                            int V, int D, int C, int TX, int chunks, float scale,
-                                                           int accumulate) {
+                                                           int accumulate, int join_blocks, int clear_from) {
+  if ((int)blockIdx.x >= join_blocks) {
+    clear_empty_rows(start, dtable, clear_from, V, D, VEC > 1,
+                     (blockIdx.x - join_blocks) * (RED_THREADS / 32) + (threadIdx.x >> 5),
+                     (gridDim.x - join_blocks) * (RED_THREADS / 32));
+    return;
+  }
   const int chunk = blockIdx.x * (RED_THREADS / TX) + threadIdx.x / TX;
   const int total = start[V];
   const int64_t c1 = (int64_t)(chunk + 1) * C;
@@ -313,6 +339,11 @@ int across(int D, int vec) {
   return tx;
 }
 
+// Blocks that clear `rows` rows, `warps` at a time.
+int clear_blocks(int64_t rows, int warps) {
+  return (int)std::min<int64_t>((rows + warps - 1) / warps, 148 * 8);
+}
+
 bool al16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 template <typename T, typename ID>
@@ -329,22 +360,24 @@ void lookup_t(const ID* ids, const T* table, T* out, int64_t n, int64_t V, int D
 
 template <typename T, int VEC>
 void sums(const T* dy, int64_t ld, const int* start, const int* order, const int* word, float* dtable, float* part,
-          int64_t n, int V, int D, float scale, bool accumulate, cudaStream_t s) {
+          int64_t n, int V, int D, float scale, bool accumulate, int z1, int z2, cudaStream_t s) {
   const int C = chunk_of(n);
   const int chunks = (int)((n + C - 1) / C);
   const int tx = across(D, VEC), per = RED_THREADS / tx;
   const int chunk_blocks = (chunks + per - 1) / per;
-  const int zero_blocks = accumulate ? 0 : (int)std::min<int64_t>((V + 7) / 8, 148 * 8);
+  const int zero_blocks = clear_blocks(z2 - z1, RED_THREADS / 32);
   if (chunk_blocks + zero_blocks > 0) {
     sum_chunks_kernel<T, VEC><<<chunk_blocks + zero_blocks, RED_THREADS, 0, s>>>(
-        dy, ld, start, order, word, dtable, part, V, D, C, tx, chunk_blocks, scale, accumulate ? 1 : 0);
+        dy, ld, start, order, word, dtable, part, V, D, C, tx, chunk_blocks, scale, accumulate ? 1 : 0, z1, z2);
     DLVK_POST_LAUNCH();
   }
-  if (chunks > 1) {
+  const int last_blocks = clear_blocks(V - z2, RED_THREADS / 32);
+  if (chunks > 1 || last_blocks > 0) {
     constexpr int JV = VEC > 1 ? 4 : 1;
     const int jx = across(D, JV), jper = RED_THREADS / jx;
-    join_kernel<JV><<<(chunks + jper - 1) / jper, RED_THREADS, 0, s>>>(start, word, part, dtable, V, D, C, jx, chunks,
-                                                                       scale, accumulate ? 1 : 0);
+    const int join_blocks = chunks > 1 ? (chunks + jper - 1) / jper : 0;
+    join_kernel<JV><<<join_blocks + last_blocks, RED_THREADS, 0, s>>>(start, word, part, dtable, V, D, C, jx, chunks,
+                                                                      scale, accumulate ? 1 : 0, join_blocks, z2);
     DLVK_POST_LAUNCH();
   }
 }
@@ -394,28 +427,30 @@ void embedding_grad(DType dt, bool ids64, const void* ids, const void* dy, int64
     attr_set[dev] = true;
   }
   const int pad = padding >= 0 && padding < V ? (int)padding : -1;
-  if (ids64)
-    sort_tokens_kernel<<<blocks, SORT_THREADS, smem, s>>>(reinterpret_cast<const int64_t*>(ids), (int)n, (int)V, R, pad,
-                                                          start, order, word);
-  else
-    sort_tokens_kernel<<<blocks, SORT_THREADS, smem, s>>>(reinterpret_cast<const int32_t*>(ids), (int)n, (int)V, R, pad,
-                                                          start, order, word);
+  const bool f32 = dt == DType::F32;
+  DLVK_CHECK(f32 || dt == DType::BF16, "embedding_grad: dy is fp32 or bf16");
+  const int step = f32 ? 4 : 8;
+  const bool vec = D % step == 0 && ld % step == 0 && al16(dy) && al16(dtable) && al16(part);
+  // The shares of the zero rows (see clear_row), none when adding; nothing is
+  // gained by clearing rows twice where most words have tokens.
+  const int64_t half = n < V ? V : 0;
+  const int z1 = accumulate ? (int)V : (int)(half * 35 / 100);
+  const int z2 = accumulate ? (int)V : (int)(V - (n < V ? V * 25 / 100 : 0));
+  const int sort_clear = accumulate ? 0 : (int)std::min<int64_t>((z1 + SORT_WARPS - 1) / SORT_WARPS, 148);
+  const auto sort = [&](auto* p) {
+    sort_tokens_kernel<<<blocks + sort_clear, SORT_THREADS, smem, s>>>(p, (int)n, (int)V, R, pad, start, order, word, blocks,
+                                                                       dtable, z1, D, vec ? 1 : 0);
+  };
+  if (ids64) sort(reinterpret_cast<const int64_t*>(ids));
+  else sort(reinterpret_cast<const int32_t*>(ids));
   DLVK_POST_LAUNCH();
-  const bool out_ok = al16(dtable) && al16(part);
-  if (dt == DType::F32) {
-    const float* g = reinterpret_cast<const float*>(dy);
-    if (D % 4 == 0 && ld % 4 == 0 && al16(g) && out_ok)
-      sums<float, 4>(g, ld, start, order, word, dtable, part, n, (int)V, D, scale, accumulate, s);
-    else
-      sums<float, 1>(g, ld, start, order, word, dtable, part, n, (int)V, D, scale, accumulate, s);
-  } else {
-    DLVK_CHECK(dt == DType::BF16, "embedding_grad: dy is fp32 or bf16");
-    const __nv_bfloat16* g = reinterpret_cast<const __nv_bfloat16*>(dy);
-    if (D % 8 == 0 && ld % 8 == 0 && al16(g) && out_ok)
-      sums<__nv_bfloat16, 8>(g, ld, start, order, word, dtable, part, n, (int)V, D, scale, accumulate, s);
-    else
-      sums<__nv_bfloat16, 1>(g, ld, start, order, word, dtable, part, n, (int)V, D, scale, accumulate, s);
-  }
+  const float* gf = reinterpret_cast<const float*>(dy);
+  const __nv_bfloat16* gb = reinterpret_cast<const __nv_bfloat16*>(dy);
+  if (f32 && vec) sums<float, 4>(gf, ld, start, order, word, dtable, part, n, (int)V, D, scale, accumulate, z1, z2, s);
+  else if (f32) sums<float, 1>(gf, ld, start, order, word, dtable, part, n, (int)V, D, scale, accumulate, z1, z2, s);
+  else if (vec)
+    sums<__nv_bfloat16, 8>(gb, ld, start, order, word, dtable, part, n, (int)V, D, scale, accumulate, z1, z2, s);
+  else sums<__nv_bfloat16, 1>(gb, ld, start, order, word, dtable, part, n, (int)V, D, scale, accumulate, z1, z2, s);
 }
 
 }  // namespace dlvk

@@ -66,15 +66,16 @@ __device__ __forceinline__ void load4(const __nv_bfloat16* p, float* v) {
   v[2] = __uint_as_float(u.y << 16);
   v[3] = __uint_as_float(u.y & 0xffff0000u);
 }
+// Written once and not read here: evicted first, so that inputs stay in L2.
 __device__ __forceinline__ void store4(float* p, const float* v) {
-  *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+  __stcs(reinterpret_cast<float4*>(p), make_float4(v[0], v[1], v[2], v[3]));
 }
 __device__ __forceinline__ void store4(__nv_bfloat16* p, const float* v) {
   const __nv_bfloat162 a = __floats2bfloat162_rn(v[0], v[1]), b = __floats2bfloat162_rn(v[2], v[3]);
   uint2 u;
   u.x = *reinterpret_cast<const uint32_t*>(&a);
   u.y = *reinterpret_cast<const uint32_t*>(&b);
-  *reinterpret_cast<uint2*>(p) = u;
+  __stcs(reinterpret_cast<uint2*>(p), u);
 }
 
 // Sum of four squares; see the note on range at the top.  Below 1e-30 a
