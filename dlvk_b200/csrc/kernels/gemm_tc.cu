@@ -166,6 +166,15 @@ __device__ __forceinline__ void tile_coords(int t, const TcParams& p, int& tm, i
   tn = rr / gsz;
 }
 
+// The descriptor `d` moved on by `units` of 16 bytes.  Only the address field
+// (its low 14 bits, never overflowing: shared memory ends below 256 KB)
+// changes from one MMA to the next; building both descriptors anew for each of
+// a k-block's MMAs kept the one issuing thread busy for ~1500 cycles per
+// k-block of a single-CTA tile, whose MMAs take 256 to 512.
+__device__ __forceinline__ uint64_t desc_at(uint64_t d, uint32_t units) {
+  return (d & 0xffffffff00000000ull) | (uint64_t)((uint32_t)d + units);
+}
+
 // The units of work of one CTA (or CTA pair) c of n.
 //  - Tiles / split-K: unit t = (split, tile) for t = c, c + n, ...
 //  - Stream-K (p.sk): the tiles x k-blocks iteration space is cut into n
@@ -721,10 +730,11 @@ __global__ void __launch_bounds__(320, 1)
         const int arow = tm * TILE_M + (int)rank * BM;
         // sub-block j of this CTA: columns tn*BN + j*MMA_N + rank*MMA_N/2 + [0, MMA_N/2)
         const int bcol = tn * BN + (int)rank * (C::MMA_N / 2);
-        const int run = kb1 - kb0;
-        for (int it = 0; it < run * p.products; ++it) {
-          const int pr = p.products == 1 ? 0 : it / run, kb = kb0 + it - pr * run;
-          const int ao = p.products == 1 ? 0 : part_a(pr) * p.a_pitch, bo6 = p.products == 1 ? 0 : part_b(pr) * p.b_pitch;
+        const int run = kb1 - kb0, steps = run * p.products;
+        const bool a_mn = p.a_mn != 0, b_mn = p.b_mn != 0, parts = p.products != 1;
+        for (int it = 0; it < steps; ++it) {
+          const int pr = parts ? it / run : 0, kb = kb0 + it - pr * run;
+          const int ao = parts ? part_a(pr) * p.a_pitch : 0, bo6 = parts ? part_b(pr) * p.b_pitch : 0;
           {
             GEMM_T0();
             if (!mbar_wait(&empty[stage], phase ^ 1u, p.err)) goto producer_done_pair;
@@ -734,7 +744,7 @@ __global__ void __launch_bounds__(320, 1)
           uint8_t* sB = sA + C::A_BYTES;
           const uint32_t fb = mapa_shared(smem_u32(&full[stage]), 0);  // the leader's full barrier
           if (rank == 0) mbar_arrive_expect_tx(&full[stage], 2 * C::STAGE_BYTES);
-          if (!p.a_mn) {
+          if (!a_mn) {
             tma_load_4d_pair(sA, &tmA, fb, kb * BK + ao, arow, abi, abo);
           } else {
 #pragma unroll
@@ -745,7 +755,7 @@ __global__ void __launch_bounds__(320, 1)
           for (int sub = 0; sub < C::NSUB; ++sub) {
             uint8_t* sBs = sB + sub * C::SUB_B_BYTES;
             const int col = bcol + sub * C::MMA_N;
-            if (!p.b_mn) {
+            if (!b_mn) {
               tma_load_4d_pair(sBs, &tmB, fb, kb * BK + bo6, col, bi, bo);
             } else {
 #pragma unroll
@@ -770,10 +780,11 @@ __global__ void __launch_bounds__(320, 1)
       while (work_next(p, gridDim.x, num_kb, tiles_per_split, num_tiles, w, tm, tn, b, sp, kb0, kb1, last)) {
         const int bo = b / p.batch2, bi = b - bo * p.batch2;
         const int abo = p.a_bcast ? 0 : bo, abi = p.a_bcast ? 0 : bi;
-        const int run = kb1 - kb0;
-        for (int it = 0; it < run * p.products; ++it) {
-          const int pr = p.products == 1 ? 0 : it / run, kb = kb0 + it - pr * run;
-          const int ao = p.products == 1 ? 0 : part_a(pr) * p.a_pitch, bo6 = p.products == 1 ? 0 : part_b(pr) * p.b_pitch;
+        const int run = kb1 - kb0, steps = run * p.products;
+        const bool a_mn = p.a_mn != 0, b_mn = p.b_mn != 0, parts = p.products != 1;
+        for (int it = 0; it < steps; ++it) {
+          const int pr = parts ? it / run : 0, kb = kb0 + it - pr * run;
+          const int ao = parts ? part_a(pr) * p.a_pitch : 0, bo6 = parts ? part_b(pr) * p.b_pitch : 0;
           {
             GEMM_T0();
             if (!mbar_wait(&empty[stage], phase ^ 1u, p.err)) goto producer_done;
@@ -782,13 +793,13 @@ __global__ void __launch_bounds__(320, 1)
           uint8_t* sA = smem + stage * C::STAGE_BYTES;
           uint8_t* sB = sA + C::A_BYTES;
           mbar_arrive_expect_tx(&full[stage], C::STAGE_BYTES);
-          if (!p.a_mn) {
+          if (!a_mn) {
             tma_load_4d(sA, &tmA, &full[stage], kb * bke + ao, tm * BM, abi, abo);
           } else {
             for (int j = 0; j < BM / mn_box; ++j)
               tma_load_4d(sA + j * mn_box_bytes, &tmA, &full[stage], tm * BM + j * mn_box + ao, kb * bke, abi, abo);
           }
-          if (!p.b_mn) {
+          if (!b_mn) {
             tma_load_4d(sB, &tmB, &full[stage], kb * bke + bo6, tn * BN, bi, bo);
           } else {
             for (int j = 0; j < BN / mn_box; ++j)
@@ -808,6 +819,10 @@ __global__ void __launch_bounds__(320, 1)
         // M = 256 across the pair; B descriptors describe this CTA's BN/2
         // columns (the peer's half sits at the same offsets in its smem).
         const uint32_t idesc = make_idesc(1, 1, 1, p.a_mn != 0, p.b_mn != 0, 2 * BM, C::MMA_N);
+        const uint32_t smem0 = smem_u32(smem);
+        const uint64_t a0 = make_sw128_desc(smem0, p.a_mn ? 8192 : 16, 1024);
+        const uint64_t b0 = make_sw128_desc(smem0 + C::A_BYTES, p.b_mn ? 8192 : 16, 1024);
+        const uint32_t a_step = (p.a_mn ? 2048 : 32) >> 4, b_step = (p.b_mn ? 2048 : 32) >> 4;
         int stage = 0;
         uint32_t phase = 0;
         int acc = 0;
@@ -830,17 +845,13 @@ __global__ void __launch_bounds__(320, 1)
             if (!mbar_wait(&full[stage], phase, p.err)) { ok = false; break; }
             GEMM_ACC(2);
             tc_fence_after();
-            const uint32_t aBase = smem_u32(smem + stage * C::STAGE_BYTES);
-            const uint32_t bBase = aBase + C::A_BYTES;
+            const uint32_t at = (uint32_t)stage * (C::STAGE_BYTES >> 4);
 #pragma unroll
             for (int k = 0; k < BK / 16; ++k) {
-              const uint64_t ad = p.a_mn ? make_sw128_desc(aBase + k * 2048, 8192, 1024)
-                                         : make_sw128_desc(aBase + k * 32, 16, 1024);
+              const uint64_t ad = desc_at(a0, at + k * a_step);
 #pragma unroll
               for (int sub = 0; sub < C::NSUB; ++sub) {
-                const uint32_t bs = bBase + sub * C::SUB_B_BYTES;
-                const uint64_t bd = p.b_mn ? make_sw128_desc(bs + k * 2048, 8192, 1024)
-                                           : make_sw128_desc(bs + k * 32, 16, 1024);
+                const uint64_t bd = desc_at(b0, at + sub * (C::SUB_B_BYTES >> 4) + k * b_step);
                 mma_f16_pair(d + (uint32_t)(sub * C::MMA_N), ad, bd, idesc, (it != 0 || k != 0) ? 1u : 0u);
               }
             }
@@ -869,6 +880,17 @@ __global__ void __launch_bounds__(320, 1)
       // One MMA takes 32 bytes of K: a K-major operand advances 32 bytes per
       // MMA, an M/N-major one K rows of 128 bytes (16 bf16 / 8 tf32 rows).
       const uint32_t mn_step = p.tf32 ? 1024u : 2048u;
+      // M/N-major tf32 operands use the 32-byte-atom swizzle (4-row atoms 512 bytes apart).
+      const uint32_t smem0 = smem_u32(smem);
+      const auto first = [&](uint32_t addr, bool mn) {
+        return !mn ? make_sw128_desc(addr, 16, 1024)
+                   : (p.tf32 ? make_sw128b32_desc(addr, (uint32_t)mn_box_bytes, 512)
+                             : make_sw128_desc(addr, (uint32_t)mn_box_bytes, 1024));
+      };
+      const uint64_t a0 = first(smem0, p.a_mn != 0), b0 = first(smem0 + C::A_BYTES, p.b_mn != 0);
+      const uint32_t a_step = (p.a_mn ? mn_step : 32u) >> 4, b_step = (p.b_mn ? mn_step : 32u) >> 4;
+      const int kind = p.i8 ? 2 : (p.tf32 ? 1 : 0), products = p.products;
+      uint32_t* const err = p.err;
       int stage = 0;
       uint32_t phase = 0;
       int acc = 0;
@@ -885,33 +907,30 @@ __global__ void __launch_bounds__(320, 1)
         }
         tc_fence_after();
         const uint32_t d = tmem_base + (uint32_t)(acc * BN);
-        bool ok = true;
-        for (int it = 0; it < (kb1 - kb0) * p.products; ++it) {
-          GEMM_T0();
-          if (!mbar_wait(&full[stage], phase, p.err)) { ok = false; break; }
-          GEMM_ACC(2);
-          tc_fence_after();
-          const uint32_t aBase = smem_u32(smem + stage * C::STAGE_BYTES);
-          const uint32_t bBase = aBase + C::A_BYTES;
+        // One loop for each kind of operand: testing for it at every MMA
+        // costs the issuing thread more than the MMA takes.
+        const int steps = (kb1 - kb0) * products;
+        const auto run = [&](auto issue) {
+          for (int it = 0; it < steps; ++it) {
+            GEMM_T0();
+            if (!mbar_wait(&full[stage], phase, err)) return false;
+            GEMM_ACC(2);
+            tc_fence_after();
+            const uint32_t at = (uint32_t)stage * (C::STAGE_BYTES >> 4);
 #pragma unroll
-          for (int k = 0; k < BK / 16; ++k) {
-            // M/N-major tf32 operands use the 32-byte-atom swizzle (4-row atoms 512 bytes apart).
-            const uint64_t ad = p.a_mn ? (p.tf32 ? make_sw128b32_desc(aBase + k * mn_step, (uint32_t)mn_box_bytes, 512)
-                                                 : make_sw128_desc(aBase + k * mn_step, (uint32_t)mn_box_bytes, 1024))
-                                       : make_sw128_desc(aBase + k * 32, 16, 1024);
-            const uint64_t bd = p.b_mn ? (p.tf32 ? make_sw128b32_desc(bBase + k * mn_step, (uint32_t)mn_box_bytes, 512)
-                                                 : make_sw128_desc(bBase + k * mn_step, (uint32_t)mn_box_bytes, 1024))
-                                       : make_sw128_desc(bBase + k * 32, 16, 1024);
-            if (p.i8) mma_i8(d, ad, bd, idesc, (it != 0 || k != 0) ? 1u : 0u);
-            else if (p.tf32) mma_tf32(d, ad, bd, idesc, (it != 0 || k != 0) ? 1u : 0u);
-            else mma_f16(d, ad, bd, idesc, (it != 0 || k != 0) ? 1u : 0u);
+            for (int k = 0; k < BK / 16; ++k)
+              issue(desc_at(a0, at + k * a_step), desc_at(b0, at + k * b_step), (it != 0 || k != 0) ? 1u : 0u);
+            mma_commit(&empty[stage]);
+            if (++stage == C::STAGES) {
+              stage = 0;
+              phase ^= 1u;
+            }
           }
-          mma_commit(&empty[stage]);
-          if (++stage == C::STAGES) {
-            stage = 0;
-            phase ^= 1u;
-          }
-        }
+          return true;
+        };
+        const bool ok = kind == 0   ? run([&](uint64_t x, uint64_t y, uint32_t c) { mma_f16(d, x, y, idesc, c); })
+                        : kind == 1 ? run([&](uint64_t x, uint64_t y, uint32_t c) { mma_tf32(d, x, y, idesc, c); })
+                                    : run([&](uint64_t x, uint64_t y, uint32_t c) { mma_i8(d, x, y, idesc, c); });
         if (!ok) break;
         mma_commit(&tfull[acc]);
         if (++acc == C::ACCS) {
