@@ -25,6 +25,10 @@ struct Extent {
 Extent extent_of(const at::Tensor& t, int64_t index) {
   const int64_t es = t.element_size();
   Extent e{reinterpret_cast<uintptr_t>(t.data_ptr()), 0, 0, 0, index};
+  if (t.is_contiguous()) {
+    e.hi = e.lo + (uintptr_t)(t.numel() * es);
+    return e;
+  }
   int64_t span = 1, run = 1;
   bool rows = false, regular = true;
   // dimensions from the innermost stride outwards
@@ -61,7 +65,16 @@ bool share_bytes(const Extent& a, const Extent& b) {
 // Each written tensor must share no byte with another tensor of the call
 // (its own input apart).
 void check_disjoint(std::vector<Extent>& ex, const char* what) {
-  std::sort(ex.begin(), ex.end(), [](const Extent& a, const Extent& b) { return a.lo < b.lo; });
+  const auto before = [](const Extent& a, const Extent& b) { return a.lo < b.lo; };
+  if (!std::is_sorted(ex.begin(), ex.end(), before)) std::sort(ex.begin(), ex.end(), before);
+  // usually nothing overlaps even as ranges
+  uintptr_t end = 0;
+  bool apart = true;
+  for (const Extent& e : ex) {
+    apart = apart && e.lo >= end;
+    end = std::max(end, e.hi);
+  }
+  if (apart) return;
   std::vector<Extent> open;
   for (const Extent& e : ex) {
     open.erase(std::remove_if(open.begin(), open.end(), [&](const Extent& o) { return o.hi <= e.lo; }), open.end());
@@ -108,21 +121,20 @@ StridedItem strided_item(const at::Tensor& in, const at::Tensor& out, uint8_t ki
   return s;
 }
 
-at::Tensor run(const std::vector<at::Tensor>& grads, const std::vector<at::Tensor>* outs, bool scale, double max_norm,
-               const char* what) {
+at::Tensor run(const TensorRefs& grads, const TensorRefs* outs, bool scale, double max_norm, const char* what) {
   TORCH_CHECK(!grads.empty(), "dlvk.", what, ": an empty list has no device; the norm of no tensors is 0");
   TORCH_CHECK(outs == nullptr || outs->size() == grads.size(), "dlvk.", what, ": ", grads.size(), " gradients and ",
               outs ? outs->size() : 0, " outputs");
-  check_cuda(grads[0], "gradients");
-  const at::Device dev = grads[0].device();
+  check_cuda(*grads[0], "gradients");
+  const at::Device dev = grads[0]->device();
   std::vector<DenseItem> dense;
   std::vector<StridedItem> strided;
   std::vector<Extent> ex;
   dense.reserve(grads.size());
   if (scale) ex.reserve(grads.size() * (outs ? 2 : 1));
   for (size_t i = 0; i < grads.size(); ++i) {
-    const at::Tensor& t = grads[i];
-    const at::Tensor& o = outs ? (*outs)[i] : t;
+    const at::Tensor& t = *grads[i];
+    const at::Tensor& o = outs ? *(*outs)[i] : t;
     TORCH_CHECK(t.device() == dev && o.device() == dev, "dlvk.", what, ": tensor ", i, " is on another device than ",
                 dev);
     const auto ti = t.scalar_type(), to = o.scalar_type();
@@ -139,7 +151,7 @@ at::Tensor run(const std::vector<at::Tensor>& grads, const std::vector<at::Tenso
     if (dense_alike(t, o)) dense.push_back({t.data_ptr(), o.data_ptr(), t.numel(), kind});
     else strided.push_back(strided_item(t, o, kind, what));
     if (scale) {
-      for (int64_t d = 0; d < o.dim(); ++d)
+      for (int64_t d = 0; !o.is_contiguous() && d < o.dim(); ++d)
         TORCH_CHECK(o.size(d) == 1 || o.stride(d) != 0, "dlvk.", what, ": output ", i,
                     " repeats its elements (an expanded tensor)");
       ex.push_back(extent_of(o, (int64_t)i));
@@ -148,7 +160,8 @@ at::Tensor run(const std::vector<at::Tensor>& grads, const std::vector<at::Tenso
   }
   if (scale) check_disjoint(ex, what);
   c10::cuda::CUDAGuard g(dev);
-  auto opt = grads[0].options();
+  at::AutoDispatchBelowADInplaceOrView below;
+  auto opt = grads[0]->options();
   at::Tensor norm = at::empty({}, opt.dtype(at::kFloat));
   const int parts = grad_norm_parts(dense.data(), (int)dense.size(), strided.data(), (int)strided.size());
   at::Tensor partial = at::empty({std::max(parts, 1)}, opt.dtype(at::kDouble));
@@ -159,12 +172,11 @@ at::Tensor run(const std::vector<at::Tensor>& grads, const std::vector<at::Tenso
 
 }  // namespace
 
-at::Tensor global_norm_op(const std::vector<at::Tensor>& grads) { return run(grads, nullptr, false, 0.0, "global_norm"); }
+at::Tensor global_norm_op(const TensorRefs& grads) { return run(grads, nullptr, false, 0.0, "global_norm"); }
 
-at::Tensor clip_global_norm_op(const std::vector<at::Tensor>& grads, double max_norm,
-                               const c10::optional<std::vector<at::Tensor>>& out) {
+at::Tensor clip_global_norm_op(const TensorRefs& grads, double max_norm, const TensorRefs* out) {
   TORCH_CHECK(max_norm > 0.0, "dlvk.clip_global_norm: max_norm must be above 0, got ", max_norm);
-  return run(grads, out.has_value() ? &*out : nullptr, true, max_norm, "clip_global_norm");
+  return run(grads, out, true, max_norm, "clip_global_norm");
 }
 
 }  // namespace aten

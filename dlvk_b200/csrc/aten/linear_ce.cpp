@@ -44,23 +44,36 @@ struct Operand {
   at::ScalarType type;
   Operand t() const { return {p, cols, rows, cs, rs, pitch, type}; }
 };
+// Rows [r0, r0 + n) of a row-major matrix with rows ld apart.
+Operand rows_operand(const at::Tensor& t, int64_t r0, int64_t n, int64_t cols, int64_t ld) {
+  return {static_cast<const char*>(t.data_ptr()) + r0 * ld * t.element_size(), n, cols, ld, 1, 0, t.scalar_type()};
+}
 Operand operand(const at::Tensor& t) {
   return {static_cast<const char*>(t.data_ptr()), t.size(0), t.size(1), t.stride(0), t.stride(1), 0, t.scalar_type()};
 }
-// `parts` [rows, 3 pitch] of a matrix [rows, cols] (or, turned, its transpose).
-Operand parts_operand(const at::Tensor& parts, int64_t rows, int64_t cols, bool turn = false) {
+// Rows [r0, r0 + n) of the parts [.., 3 pitch] of a matrix.
+Operand parts_operand(const at::Tensor& parts, int64_t r0, int64_t n, int64_t cols) {
   const int64_t pitch = parts.size(1) / 3;
-  const Operand o{static_cast<const char*>(parts.data_ptr()), rows, cols, 3 * pitch, 1, pitch, at::kBFloat16};
-  return turn ? o.t() : o;
+  return {static_cast<const char*>(parts.data_ptr()) + r0 * 6 * pitch, n, cols, 3 * pitch, 1, pitch, at::kBFloat16};
 }
+// A row-major output, rows ld apart.
+struct Out {
+  char* p;
+  int64_t rows, cols, ld;
+  at::ScalarType type;
+};
+Out rows_out(const at::Tensor& t, int64_t r0, int64_t n, int64_t cols, int64_t ld) {
+  return {static_cast<char*>(t.data_ptr()) + r0 * ld * t.element_size(), n, cols, ld, t.scalar_type()};
+}
+DType dtype_of(at::ScalarType t) { return t == at::kFloat ? DType::F32 : DType::BF16; }
 
 // out (+)= scale * A B (+ bias per column), the sums in a fixed order.
-void product(const Operand& A, const Operand& B, const at::Tensor& out, const float* scale, bool accumulate,
-             const float* bias = nullptr) {
+void product(const Operand& A, const Operand& B, const Out& out, const float* scale, bool accumulate,
+             const at::TensorOptions& f32, const float* bias = nullptr) {
   GemmArgs a;
   a.A = A.p;
   a.B = B.p;
-  a.C = out.data_ptr();
+  a.C = out.p;
   a.M = A.rows;
   a.K = A.cols;
   a.N = B.cols;
@@ -68,7 +81,7 @@ void product(const Operand& A, const Operand& B, const at::Tensor& out, const fl
   a.sak = A.cs;
   a.sbk = B.rs;
   a.sbn = B.cs;
-  a.ldc = out.stride(0);
+  a.ldc = out.ld;
   a.beta = accumulate ? 1.f : 0.f;
   a.bias = bias;
   a.bias_dtype = (int)DType::F32;
@@ -76,32 +89,33 @@ void product(const Operand& A, const Operand& B, const at::Tensor& out, const fl
   a.parts = A.pitch > 0;
   a.pitch_a = A.pitch;
   a.pitch_b = B.pitch;
-  const DType odt = to_dtype(out);
+  const DType odt = dtype_of(out.type);
   if (A.type == at::kBFloat16 && gemm_tc_supported(a)) {
     a.alpha_ptr = scale;
     const int64_t n = gemm_tc_workspace_floats(a, 0, odt);
-    const at::Tensor ws = n > 0 ? at::empty({n}, out.options().dtype(at::kFloat)) : at::Tensor();
+    const at::Tensor ws = n > 0 ? at::empty({n}, f32) : at::Tensor();
     gemm_tc(odt, a, stream(), device_error_word(), 0, n > 0 ? ws.data_ptr<float>() : nullptr, n);
     return;
   }
   TORCH_INTERNAL_ASSERT(scale == nullptr && !a.parts);
   const int64_t n = gemm_simt_workspace_floats(a);
-  const at::Tensor ws = n > 0 ? at::empty({n}, out.options().dtype(at::kFloat)) : at::Tensor();
-  gemm_simt(A.type == at::kFloat ? DType::F32 : DType::BF16, odt, a, stream(), n > 0 ? ws.data_ptr<float>() : nullptr,
-            n);
+  const at::Tensor ws = n > 0 ? at::empty({n}, f32) : at::Tensor();
+  gemm_simt(dtype_of(A.type), odt, a, stream(), n > 0 ? ws.data_ptr<float>() : nullptr, n);
 }
 
 // dst (+)= scale * A B.  Output rows that are no whole 16-byte steps go
 // through a padded copy: the products store whole boxes.
-void product_into(const Operand& A, const Operand& B, const at::Tensor& dst, const float* scale, bool accumulate) {
-  const int64_t n = dst.size(1), step = 16 / dst.element_size();
-  if (dst.stride(0) % step == 0 && reinterpret_cast<uintptr_t>(dst.data_ptr()) % 16 == 0) {
-    product(A, B, dst, scale, accumulate);
+void product_into(const Operand& A, const Operand& B, const Out& dst, const float* scale, bool accumulate,
+                  const at::TensorOptions& f32) {
+  const int64_t step = 16 / (int64_t)c10::elementSize(dst.type);
+  if (dst.ld % step == 0 && reinterpret_cast<uintptr_t>(dst.p) % 16 == 0) {
+    product(A, B, dst, scale, accumulate, f32);
     return;
   }
-  const at::Tensor c = at::empty({dst.size(0), round_up(n, step)}, dst.options());
-  product(A, B, c.narrow(1, 0, n), scale, false);
-  copy_matrix(to_dtype(dst), to_dtype(c), c.data_ptr(), c.size(1), 1, dst.data_ptr(), dst.stride(0), dst.size(0), n, n,
+  const int64_t ld = round_up(dst.cols, step);
+  const at::Tensor c = at::empty({dst.rows, ld}, f32.dtype(dst.type));
+  product(A, B, rows_out(c, 0, dst.rows, dst.cols, ld), scale, false, f32);
+  copy_matrix(dtype_of(dst.type), dtype_of(dst.type), c.data_ptr(), ld, 1, dst.p, dst.ld, dst.rows, dst.cols, dst.cols,
               accumulate, stream());
 }
 
@@ -156,6 +170,7 @@ LinearCeResult linear_ce_op(const at::Tensor& x, const at::Tensor& w, const at::
                     db_out->numel() == V && db_out->device() == dev,
                 "dlvk.linear_ce: the bias gradient must be contiguous fp32 [", V, "] on ", dev);
   c10::cuda::CUDAGuard g(dev);
+  at::AutoDispatchBelowADInplaceOrView below;  // no autograd bookkeeping for what follows
   const auto f32 = x.options().dtype(at::kFloat);
   const bool bf = dt == at::kBFloat16;
 
@@ -213,7 +228,11 @@ LinearCeResult linear_ce_op(const at::Tensor& x, const at::Tensor& w, const at::
     c.ldx = xq.stride(0);
     c.ldw = w_k ? wq.stride(1) : wq.stride(0);
   }
-  const Operand wo = parts ? parts_operand(wq, w_k ? V : E, w_k ? E : V, w_k) : operand(wq);  // [E, V]
+  Operand wo = operand(wq);  // [E, V]
+  if (parts) {
+    wo = parts_operand(wq, 0, wq.size(0), w_k ? E : V);
+    if (w_k) wo = wo.t();
+  }
   c.x = reinterpret_cast<const __nv_bfloat16*>(xq.data_ptr());
   c.w = reinterpret_cast<const __nv_bfloat16*>(wq.data_ptr());
   c.rows = N;
@@ -250,6 +269,7 @@ LinearCeResult linear_ce_op(const at::Tensor& x, const at::Tensor& w, const at::
   c.gscale = gscale;
 
   const int64_t ldv = round_up(V, 8), vp = round_up(V, 64);
+  const int64_t ldx = round_up(E, 16 / x.element_size());
   at::Tensor z, dl, xc, part, dw32;
   if (!fused) z = at::empty({rows, ldv}, f32);
   bool dw_k = false;
@@ -257,7 +277,7 @@ LinearCeResult linear_ce_op(const at::Tensor& x, const at::Tensor& w, const at::
     dl = parts ? at::empty({rows, 3 * vp}, xq.options()) : bf ? at::empty({rows, ldv}, x.options()) : z;
     // dW = x^T dz reads x once more, with zeros in the rows that do not count:
     // their dz is 0, but 0 times an infinity or NaN left there would not be.
-    if (!parts) xc = at::empty({rows, round_up(E, 16 / x.element_size())}, x.options()).narrow(1, 0, E);
+    if (!parts) xc = at::empty({rows, ldx}, x.options());
     dw_k = out.dw.stride(1) != 1 && V > 1;  // the gradient's rows are classes too
     // sums over several blocks are fp32 until the last
     if (blocks > 1 && out.dw.scalar_type() != at::kFloat)
@@ -265,7 +285,12 @@ LinearCeResult linear_ce_op(const at::Tensor& x, const at::Tensor& w, const at::
                   : at::empty({E, round_up(V, 4)}, f32).narrow(1, 0, V);
     if (out.dbias.defined()) part = at::empty({fused ? ceil_div(rows, 32) * V : ldv}, f32);
   }
-  const at::Tensor dw = dw32.defined() ? dw32 : out.dw;
+  Out dw{};  // [E, V], or of classes by width (dw_k)
+  if (want_grad) {
+    const at::Tensor& t = dw32.defined() ? dw32 : out.dw;
+    dw = {static_cast<char*>(t.data_ptr()), dw_k ? V : E, dw_k ? E : V, dw_k ? t.stride(1) : t.stride(0),
+          t.scalar_type()};
+  }
   if (blocks > 1) ce_count(all, mean, gsp, gscale, done, stream());
 
   for (int64_t k = 0; k < blocks; ++k) {
@@ -273,11 +298,10 @@ LinearCeResult linear_ce_op(const at::Tensor& x, const at::Tensor& w, const at::
     CeRows r = all;
     r.rows = n;
     r.labels = static_cast<const char*>(tc.data_ptr()) + r0 * lab_size;
-    const at::Tensor xk = xq.narrow(0, r0, n);
-    Operand xo = parts ? parts_operand(xk, n, E) : operand(xk);
+    Operand xo = parts ? parts_operand(xq, r0, n, E) : rows_operand(xq, r0, n, E, xq.stride(0));
     c.rows = n;
     TORCH_INTERNAL_ASSERT(!fused || n * ce_tc_stat_cols(n, V) <= rows * stat_cols);
-    c.x = reinterpret_cast<const __nv_bfloat16*>(xk.data_ptr());
+    c.x = reinterpret_cast<const __nv_bfloat16*>(xo.p);
     c.labels = r.labels;
     c.done = blocks == 1 ? done : nullptr;
     if (keep) {
@@ -285,7 +309,7 @@ LinearCeResult linear_ce_op(const at::Tensor& x, const at::Tensor& w, const at::
     } else if (fused) {
       ce_stats_tc(c, stream(), device_error_word());
     } else {
-      product(xo, wo, z.narrow(0, 0, n).narrow(1, 0, V), nullptr, false, biasp);
+      product(xo, wo, rows_out(z, 0, n, V, ldv), nullptr, false, f32, biasp);
       ce_memory_stats(r, z.data_ptr<float>(), ldv, stats, zlabel, c.done, stream());
     }
     CeFinish f{};
@@ -305,17 +329,17 @@ LinearCeResult linear_ce_op(const at::Tensor& x, const at::Tensor& w, const at::
     f.first_group = (int)(r0 / 32);  // blocks are whole tiles, the last apart
     f.total_groups = groups;
     if (xc.defined()) {
-      f.x = xk.data_ptr();
-      f.ldx = xk.stride(0);
+      f.x = xo.p;
+      f.ldx = xo.rs;
       f.width = E;
       f.x_clean = xc.data_ptr();
-      f.ldc = xc.stride(0);
-      xo = operand(xc.narrow(0, 0, n));
+      f.ldc = ldx;
+      xo = rows_operand(xc, 0, n, E, ldx);
     }
     ce_finish(r, f, to_dtype(x), stream());
     if (!want_grad) continue;
 
-    Operand d = parts ? parts_operand(dl, n, V) : operand(dl.narrow(0, 0, n).narrow(1, 0, V));
+    const Operand d = parts ? parts_operand(dl, 0, n, V) : rows_operand(dl, 0, n, V, ldv);
     const float* scale = gscale;  // dz holds softmax - onehot, the products its factor
     if (keep) {
       ce_rescale(r, stats, ce_tc_stat_width(n, V), norm, dl.data_ptr(), ldv, stream());
@@ -339,10 +363,10 @@ LinearCeResult linear_ce_op(const at::Tensor& x, const at::Tensor& w, const at::
                     db_accumulate || k > 0, stream());
       }
     }
-    product_into(d, wo.t(), out.dx.narrow(0, r0, n), scale, false);
+    product_into(d, wo.t(), rows_out(out.dx, r0, n, E, E), scale, false, f32);
     const bool add = dw32.defined() ? k > 0 : (dw_accumulate || k > 0);
-    if (dw_k) product_into(d.t(), xo, dw.t(), scale, add);
-    else product_into(xo.t(), d, dw, scale, add);
+    if (dw_k) product_into(d.t(), xo, dw, scale, add, f32);
+    else product_into(xo.t(), d, dw, scale, add, f32);
   }
   if (dw32.defined()) {
     const at::Tensor src = dw_k ? dw32.t() : dw32, dst = dw_k ? out.dw.t() : out.dw;

@@ -424,6 +424,7 @@ at::Tensor embedding_lookup_op(const at::Tensor& ids, const at::Tensor& table, d
   check_f32_bf16(table, "embedding_lookup", "table");
   TORCH_CHECK(table.dim() == 2, "dlvk.embedding_lookup: table [V, D], got ", table.sizes());
   c10::cuda::CUDAGuard g(table.device());
+  at::AutoDispatchBelowADInplaceOrView below;
   const int64_t V = table.size(0), D = table.size(1);
   TORCH_CHECK(D < (1LL << 31) - 4096, "dlvk.embedding_lookup: rows of ", D, " elements");
   auto idc = ids.contiguous();
@@ -449,6 +450,7 @@ at::Tensor embedding_grad_op(const at::Tensor& ids, const at::Tensor& dy, int64_
   TORCH_CHECK(D < (1LL << 31) - 4096, "dlvk.embedding_grad: rows of ", D, " elements");
   TORCH_CHECK(n < (1LL << 31) - 1024 && V < (1LL << 31) - 1024, "dlvk.embedding_grad: more than 2^31 tokens or words");
   c10::cuda::CUDAGuard g(dy.device());
+  at::AutoDispatchBelowADInplaceOrView below;
   at::Tensor dt;
   if (out.has_value()) {
     dt = *out;

@@ -14,6 +14,18 @@ namespace dlvk {
 namespace bind {
 using namespace ::dlvk::aten;
 
+// The tensors of a Python list, which the caller keeps alive: converting a
+// list of hundreds to a vector of tensors costs a reference count each.
+TensorRefs tensor_refs(const py::list& l) {
+  TensorRefs r;
+  r.reserve(l.size());
+  for (const py::handle& h : l) {
+    TORCH_CHECK(THPVariable_Check(h.ptr()), "dlvk: a list of tensors holds something else");
+    r.push_back(&THPVariable_Unpack(h.ptr()));
+  }
+  return r;
+}
+
 void register_ops(py::module& m) {
   m.def("unary", &unary_op, py::arg("x"), py::arg("op"), py::arg("a") = 0.0, py::arg("b") = 0.0,
         py::arg("out") = py::none(), py::arg("out_dtype") = py::none());
@@ -120,8 +132,13 @@ void register_ops(py::module& m) {
   }, py::arg("w"), py::arg("g"), py::arg("l1"), py::arg("l2"), py::arg("ll1"), py::arg("ll2"),
      py::arg("loss_out") = py::none(),
      py::arg("gscale") = py::none());
-  m.def("global_norm", &global_norm_op, py::arg("grads"));
-  m.def("clip_global_norm", &clip_global_norm_op, py::arg("grads"), py::arg("max_norm"), py::arg("out") = py::none());
+  m.def("global_norm", [](const py::list& grads) { return global_norm_op(tensor_refs(grads)); }, py::arg("grads"));
+  m.def("clip_global_norm", [](const py::list& grads, double max_norm, const c10::optional<py::list>& out) {
+    const TensorRefs g = tensor_refs(grads);
+    if (!out.has_value()) return clip_global_norm_op(g, max_norm, nullptr);
+    const TensorRefs o = tensor_refs(*out);
+    return clip_global_norm_op(g, max_norm, &o);
+  }, py::arg("grads"), py::arg("max_norm"), py::arg("out") = py::none());
   m.def("grad_stats_scratch_floats", &grad_stats_scratch_floats);
   m.def("scaler_update", &scaler_update_op);
   m.def("optim_hyper_bytes", &optim_hyper_bytes);

@@ -50,8 +50,9 @@ void optim_update_op(int64_t kind, const at::Tensor& hyper, const at::Tensor& p,
 void grad_stats_op(const at::Tensor& g, double scale, double max_norm, const at::Tensor& sumsq, c10::optional<at::Tensor> flag, c10::optional<at::Tensor> clip, bool accumulate, const at::Tensor& scratch, c10::optional<at::Tensor> scale_dev);
 void scaler_update_op(const at::Tensor& scale, const at::Tensor& good_steps, const at::Tensor& found_inf, double growth, double backoff, int64_t interval, double smin, double smax, c10::optional<at::Tensor> inv_scale);
 int64_t optim_hyper_bytes();
-at::Tensor global_norm_op(const std::vector<at::Tensor>& grads);
-at::Tensor clip_global_norm_op(const std::vector<at::Tensor>& grads, double max_norm, const c10::optional<std::vector<at::Tensor>>& out);
+using TensorRefs = std::vector<const at::Tensor*>;  // a list that is read, not held
+at::Tensor global_norm_op(const TensorRefs& grads);
+at::Tensor clip_global_norm_op(const TensorRefs& grads, double max_norm, const TensorRefs* out);
 const float* optf(const c10::optional<at::Tensor>& t);
 float* optfm(const c10::optional<at::Tensor>& t);
 ConvDesc conv_desc(const at::Tensor& x, const at::Tensor& w, int64_t stride, int64_t pad);

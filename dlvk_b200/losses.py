@@ -30,6 +30,8 @@ def _to_probs(target: torch.Tensor, cols: int) -> torch.Tensor:
 
 
 def _unwrap(x):
+    if isinstance(x, torch.Tensor):
+        return x
     from .tensor import Tensor as FacadeTensor
 
     return x.data if isinstance(x, FacadeTensor) else x
@@ -109,12 +111,12 @@ class LinearCrossEntropyLoss(LossFunction):
                              f"got {tuple(target.shape)}")
         if hidden.dim() != 2:
             hidden, target = hidden.reshape(-1, hidden.shape[-1]), target.reshape(-1)
-        return hidden.detach(), target
+        return hidden, target
 
     def forward(self, hidden, weight, target, bias=None, correct=None):
         """The loss alone: a scalar, or with reduction "none" each row's (0 where it does not count)."""
         x, t = self._rows(hidden, target)
-        loss, rows, _, _, _ = K.linear_ce(x, _unwrap(weight).detach(), t, bias, self.ignore_index,
+        loss, rows, _, _, _ = K.linear_ce(x, _unwrap(weight), t, bias, self.ignore_index,
                                           self.reduction != "sum", False, correct=correct)
         return rows.reshape(_unwrap(target).shape) if self.reduction == "none" else loss
 
@@ -127,7 +129,7 @@ class LinearCrossEntropyLoss(LossFunction):
         if self.reduction == "none":
             raise ValueError("value_and_grad needs reduction mean or sum")
         x, t = self._rows(hidden, target)
-        loss, _, dx, dw, db = K.linear_ce(x, _unwrap(weight).detach(), t, bias, self.ignore_index,
+        loss, _, dx, dw, db = K.linear_ce(x, _unwrap(weight), t, bias, self.ignore_index,
                                           self.reduction == "mean", True, grad_scale)
         return loss, dx.reshape(_unwrap(hidden).shape), dw, db
 

@@ -297,6 +297,7 @@ def linear_ce(hidden: torch.Tensor, weight: torch.Tensor, target: torch.Tensor, 
     if native(hidden):
         return N().linear_ce(hidden, weight, target, bias, ignore, mean, want_grad, grad_scale, dw_out, dw_accumulate,
                              db_out, db_accumulate, correct)
+    hidden, weight = hidden.detach(), weight.detach()
     n, classes = hidden.shape[0], weight.shape[1]
     if hidden.dim() != 2 or weight.dim() != 2 or weight.shape[0] != hidden.shape[1] or classes < 1:
         raise ValueError(f"linear_ce: hidden {tuple(hidden.shape)}, weight {tuple(weight.shape)}")

@@ -332,6 +332,9 @@ class RMSprop(Optimizer):
 
 
 def _tensor_list(tensors: Iterable) -> List[torch.Tensor]:
+    tensors = list(tensors)
+    if all(map(torch.is_tensor, tensors)):
+        return tensors
     from .tensor import Tensor as FacadeTensor
 
     return [t.data if isinstance(t, FacadeTensor) else t for t in tensors]
