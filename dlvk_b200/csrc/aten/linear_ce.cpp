@@ -67,9 +67,10 @@ Out rows_out(const at::Tensor& t, int64_t r0, int64_t n, int64_t cols, int64_t l
 }
 DType dtype_of(at::ScalarType t) { return t == at::kFloat ? DType::F32 : DType::BF16; }
 
-// out (+)= scale * A B (+ bias per column), the sums in a fixed order.
+// out (+)= scale * A B (+ bias per column), the sums in a fixed order.  With
+// `before`, a bf16 out = the fp32 sum of that and the product, rounded once.
 void product(const Operand& A, const Operand& B, const Out& out, const float* scale, bool accumulate,
-             const at::TensorOptions& f32, const float* bias = nullptr) {
+             const at::TensorOptions& f32, const float* bias = nullptr, const Out* before = nullptr) {
   GemmArgs a;
   a.A = A.p;
   a.B = B.p;
@@ -90,6 +91,11 @@ void product(const Operand& A, const Operand& B, const Out& out, const float* sc
   a.pitch_a = A.pitch;
   a.pitch_b = B.pitch;
   const DType odt = dtype_of(out.type);
+  if (before != nullptr) {
+    a.residual = before->p;
+    a.ldr = before->ld;
+    a.residual_f32 = true;
+  }
   if (A.type == at::kBFloat16 && gemm_tc_supported(a)) {
     a.alpha_ptr = scale;
     const int64_t n = gemm_tc_workspace_floats(a, 0, odt);
@@ -97,7 +103,7 @@ void product(const Operand& A, const Operand& B, const Out& out, const float* sc
     gemm_tc(odt, a, stream(), device_error_word(), 0, n > 0 ? ws.data_ptr<float>() : nullptr, n);
     return;
   }
-  TORCH_INTERNAL_ASSERT(scale == nullptr && !a.parts);
+  TORCH_INTERNAL_ASSERT(scale == nullptr && !a.parts && before == nullptr);
   const int64_t n = gemm_simt_workspace_floats(a);
   const at::Tensor ws = n > 0 ? at::empty({n}, f32) : at::Tensor();
   gemm_simt(dtype_of(A.type), odt, a, stream(), n > 0 ? ws.data_ptr<float>() : nullptr, n);
@@ -268,7 +274,8 @@ LinearCeResult linear_ce_op(const at::Tensor& x, const at::Tensor& w, const at::
   c.norm = norm;
   c.gscale = gscale;
 
-  const int64_t ldv = round_up(V, 8), vp = round_up(V, 64);
+  // rows of whole 128-byte lines: a box of the tiles' stores is one line a row
+  const int64_t ldv = round_up(V, 64), vp = ldv;
   const int64_t ldx = round_up(E, 16 / x.element_size());
   at::Tensor z, dl, xc, part, dw32;
   if (!fused) z = at::empty({rows, ldv}, f32);
@@ -285,11 +292,18 @@ LinearCeResult linear_ce_op(const at::Tensor& x, const at::Tensor& w, const at::
                   : at::empty({E, round_up(V, 4)}, f32).narrow(1, 0, V);
     if (out.dbias.defined()) part = at::empty({fused ? ceil_div(rows, 32) * V : ldv}, f32);
   }
-  Out dw{};  // [E, V], or of classes by width (dw_k)
-  if (want_grad) {
-    const at::Tensor& t = dw32.defined() ? dw32 : out.dw;
-    dw = {static_cast<char*>(t.data_ptr()), dw_k ? V : E, dw_k ? E : V, dw_k ? t.stride(1) : t.stride(0),
-          t.scalar_type()};
+  const auto dw_rows = [&](const at::Tensor& t) {  // [E, V], or of classes by width (dw_k)
+    return Out{static_cast<char*>(t.data_ptr()), dw_k ? V : E, dw_k ? E : V, dw_k ? t.stride(1) : t.stride(0),
+               t.scalar_type()};
+  };
+  Out dw{}, dw_last{};
+  if (want_grad) dw = dw_last = dw_rows(dw32.defined() ? dw32 : out.dw);
+  // the last of several blocks adds to the others' sums and rounds, where its output has whole 16-byte rows
+  bool round_last = false;
+  if (dw32.defined()) {
+    const Out o = dw_rows(out.dw);
+    round_last = fused && o.ld % 8 == 0 && reinterpret_cast<uintptr_t>(o.p) % 16 == 0 && dw.cols >= 16;
+    if (round_last) dw_last = o;
   }
   if (blocks > 1) ce_count(all, mean, gsp, gscale, done, stream());
 
@@ -352,7 +366,7 @@ LinearCeResult linear_ce_op(const at::Tensor& x, const at::Tensor& w, const at::
     } else {
       ce_memory_grad(r, z.data_ptr<float>(), ldv, norm, gscale,
                      dl.is_same(z) ? nullptr : reinterpret_cast<__nv_bfloat16*>(dl.data_ptr()), parts ? vp : 0,
-                     stream());
+                     !parts || part.defined(), stream());
       if (!parts) scale = nullptr;  // these carry it
       if (part.defined()) {  // the padding's columns are summed too and left out of the copy
         const int64_t ns = colsum_scratch_floats(n, ldv);
@@ -364,11 +378,11 @@ LinearCeResult linear_ce_op(const at::Tensor& x, const at::Tensor& w, const at::
       }
     }
     product_into(d, wo.t(), rows_out(out.dx, r0, n, E, E), scale, false, f32);
-    const bool add = dw32.defined() ? k > 0 : (dw_accumulate || k > 0);
-    if (dw_k) product_into(d.t(), xo, dw, scale, add, f32);
-    else product_into(xo.t(), d, dw, scale, add, f32);
+    const Operand left = dw_k ? d.t() : xo.t(), right = dw_k ? xo : d;
+    if (round_last && k == blocks - 1) product(left, right, dw_last, scale, false, f32, nullptr, &dw);
+    else product_into(left, right, dw, scale, dw32.defined() ? k > 0 : (dw_accumulate || k > 0), f32);
   }
-  if (dw32.defined()) {
+  if (dw32.defined() && !round_last) {
     const at::Tensor src = dw_k ? dw32.t() : dw32, dst = dw_k ? out.dw.t() : out.dw;
     copy_matrix(to_dtype(dst), DType::F32, src.data_ptr(), src.stride(0), 1, dst.data_ptr(), dst.stride(0),
                 dst.size(0), dst.size(1), dst.size(1), false, stream());

@@ -70,6 +70,7 @@ struct GemmArgs {
   int act = ACT_NONE;
   const void* residual = nullptr;  // same dtype as C, added before act
   int64_t ldr = 0, batch_stride_r = 0, batch2_stride_r = 0;
+  bool residual_f32 = false;  // the residual is fp32 beside a bf16 C (tensor-core path, 2-D, beta 0)
   // Optional mask source (same dtype and shape as C): the output is zeroed
   // where mask <= 0.  Fuses the backward of a preceding ReLU into dX = dY W^T.
   const void* relu_mask = nullptr;
@@ -377,13 +378,14 @@ void ce_finish(const CeRows& r, const CeFinish& f, DType dt, cudaStream_t s);
 void ce_rescale(const CeRows& r, const float2* stats, int stat_width, const float2* norm, void* e, int64_t lde,
                 cudaStream_t s);
 // Statistics (one column) and gradient of logits z [rows, classes] fp32, row
-// stride ldz: z becomes (softmax - onehot) * gscale; dl, when given, that
+// stride ldz: z becomes (softmax - onehot) * gscale (not when keep_z is off);
+// dl, when given, that
 // rounded to bf16 (pitch 0, row stride ldz), or softmax - onehot in three
 // parts (pitch of a part, row stride 3 pitch, zeros in the padding).
 void ce_memory_stats(const CeRows& r, const float* z, int64_t ldz, float2* stats, float* zlabel, unsigned* done,
                      cudaStream_t s);
 void ce_memory_grad(const CeRows& r, float* z, int64_t ldz, const float2* norm, const float* gscale, __nv_bfloat16* dl,
-                    int64_t pitch, cudaStream_t s);
+                    int64_t pitch, bool keep_z, cudaStream_t s);
 // dst [rows, 3 pitch] bf16: src (fp32 [rows, cols], row stride ld) = the sum of
 // its three parts to 2^-24; zeros in the padding, and with `mask` in the rows
 // that do not count.

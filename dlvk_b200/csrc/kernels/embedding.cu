@@ -121,18 +121,20 @@ __global__ void __launch_bounds__(SORT_THREADS) sort_tokens_kernel(const ID* __r
       clear_row(dtable + (int64_t)v * D, D, vec, threadIdx.x & 31);
     return;
   }
-  extern __shared__ int cnt[];  // [SORT_WARPS][R]
+  extern __shared__ int cnt[];  // [SORT_WARPS][RP], then [R]: a word's first place
   __shared__ int warp_part[SORT_WARPS];
   __shared__ int before_sm;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int v0 = blockIdx.x * R, v1 = min(V, v0 + R);
-  for (int i = tid; i < SORT_WARPS * R; i += SORT_THREADS) cnt[i] = 0;
+  const int RP = R | 1;  // odd: the lanes of a warp read one word's counts from as many banks
+  int* first = cnt + SORT_WARPS * RP;
+  for (int i = tid; i < SORT_WARPS * RP; i += SORT_THREADS) cnt[i] = 0;
   if (tid == 0) before_sm = 0;
   __syncthreads();
 
   const int per = ((n + SORT_THREADS - 1) / SORT_THREADS) * 32;  // ids of a warp, whole groups of 32
   const int lo = min((int64_t)n, (int64_t)warp * per), hi = min((int64_t)n, (int64_t)(warp + 1) * per);
-  int* mine = cnt + warp * R;
+  int* mine = cnt + warp * RP;
   int before = 0;
   for (int base = lo; base < hi; base += 256) {
     int id[8];
@@ -152,10 +154,22 @@ __global__ void __launch_bounds__(SORT_THREADS) sort_tokens_kernel(const ID* __r
   if (lane == 0 && before) atomicAdd(&before_sm, before);
   __syncthreads();
 
-  // thread r: word v0 + r.  Its total over the warps, then the block's scan.
-  int total = 0;
-  if (tid < R)
-    for (int w = 0; w < SORT_WARPS; ++w) total += cnt[w * R + tid];
+  // A warp scans a word's counts over the warps (lane = warp), ...
+  static_assert(SORT_WARPS == 32, "lane = warp");
+  for (int r = warp; r < R; r += SORT_WARPS) {
+    const int c = cnt[lane * RP + r];
+    int incl = c;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int t = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += t;
+    }
+    cnt[lane * RP + r] = incl - c;
+    if (lane == 31) first[r] = incl;
+  }
+  __syncthreads();
+  // ... the block the words' totals (thread r: word v0 + r).
+  const int total = tid < R ? first[tid] : 0;
   int incl = total;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -174,17 +188,12 @@ __global__ void __launch_bounds__(SORT_THREADS) sort_tokens_kernel(const ID* __r
     warp_part[lane] = p;
   }
   __syncthreads();
-  int at = before_sm + incl - total + (warp > 0 ? warp_part[warp - 1] : 0);
+  const int at = before_sm + incl - total + (warp > 0 ? warp_part[warp - 1] : 0);
   if (tid < R && v0 + tid < V) {
     start[v0 + tid] = at;
     if (v0 + tid == V - 1) start[V] = at + total;
   }
-  if (tid < R)
-    for (int w = 0; w < SORT_WARPS; ++w) {
-      const int c = cnt[w * R + tid];
-      cnt[w * R + tid] = at;
-      at += c;
-    }
+  if (tid < R) first[tid] = at;
   __syncthreads();
 
   for (int base = lo; base < hi; base += 256) {
@@ -201,7 +210,7 @@ __global__ void __launch_bounds__(SORT_THREADS) sort_tokens_kernel(const ID* __r
       if (!__any_sync(0xffffffffu, hit)) continue;
       const unsigned peers = __match_any_sync(0xffffffffu, id[k]);
       if (hit) {
-        const int place = mine[id[k] - v0] + __popc(peers & ((1u << lane) - 1u));
+        const int place = first[id[k] - v0] + mine[id[k] - v0] + __popc(peers & ((1u << lane) - 1u));
         order[place] = base + k * 32 + lane;
         word[place] = id[k];
       }
@@ -417,11 +426,12 @@ void embedding_grad(DType dt, bool ids64, const void* ids, const void* dy, int64
   // words of a block: all 148 SMs, at least 8 each, at most what its counts have room for
   const int R = (int)std::min<int64_t>(SORT_WORDS, std::max<int64_t>(8, (V + 147) / 148));
   const int blocks = (int)((V + R - 1) / R);
-  const size_t smem = (size_t)SORT_WARPS * R * sizeof(int);
+  const auto room = [](int words) { return (SORT_WARPS * (words | 1) + words) * (int)sizeof(int); };
+  const size_t smem = (size_t)room(R);
   static bool attr_set[kMaxDevices] = {false};
   const int dev = current_device_slot();
   if (!attr_set[dev]) {
-    const int most = SORT_WARPS * SORT_WORDS * (int)sizeof(int);
+    const int most = room(SORT_WORDS);
     DLVK_CUDA_CHECK(cudaFuncSetAttribute(sort_tokens_kernel<int32_t>, cudaFuncAttributeMaxDynamicSharedMemorySize, most));
     DLVK_CUDA_CHECK(cudaFuncSetAttribute(sort_tokens_kernel<int64_t>, cudaFuncAttributeMaxDynamicSharedMemorySize, most));
     attr_set[dev] = true;
@@ -434,7 +444,7 @@ void embedding_grad(DType dt, bool ids64, const void* ids, const void* dy, int64
   // The shares of the zero rows (see clear_row), none when adding; nothing is
   // gained by clearing rows twice where most words have tokens.
   const int64_t half = n < V ? V : 0;
-  const int z1 = accumulate ? (int)V : (int)(half * 35 / 100);
+  const int z1 = accumulate ? (int)V : (int)(half * 25 / 100);
   const int z2 = accumulate ? (int)V : (int)(V - (n < V ? V * 25 / 100 : 0));
   const int sort_clear = accumulate ? 0 : (int)std::min<int64_t>((z1 + SORT_WARPS - 1) / SORT_WARPS, 148);
   const auto sort = [&](auto* p) {

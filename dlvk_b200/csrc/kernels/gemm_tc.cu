@@ -65,6 +65,7 @@ struct TcParams {
   const void* Mk;      // ReLU mask source (same dtype as C) or null: out = 0 where Mk <= 0
   int64_t ldm, bsm, bsm2;
   int r_vec, m_vec;
+  int r_f32;           // the residual is fp32 beside a bf16 C (added before the rounding)
   int out_f32;
   int vec_ok;
   float alpha, beta;
@@ -291,6 +292,22 @@ __device__ __forceinline__ void colsum_chunk(const TcParams& p, int row0, int la
 __device__ __forceinline__ void add_row_residual(const TcParams& p, int64_t rb, int row, int n0, float* v) {
   if (row >= p.M || n0 >= p.N) return;
   const int64_t off = rb + (int64_t)row * p.ldr + n0;
+  if (p.r_f32) {
+    const float* src = reinterpret_cast<const float*>(p.R) + off;
+    if (n0 + 32 <= p.N && p.r_vec) {
+#pragma unroll
+      for (int q = 0; q < 8; ++q) {
+        const float4 u = reinterpret_cast<const float4*>(src)[q];
+        v[4 * q] += u.x;
+        v[4 * q + 1] += u.y;
+        v[4 * q + 2] += u.z;
+        v[4 * q + 3] += u.w;
+      }
+    } else {
+      for (int j = 0; j < 32 && n0 + j < p.N; ++j) v[j] += src[j];
+    }
+    return;
+  }
   if (n0 + 32 <= p.N && p.r_vec) {
     const uint4* src = reinterpret_cast<const uint4*>(reinterpret_cast<const __nv_bfloat16*>(p.R) + off);
     uint4 u[4];
@@ -1507,6 +1524,9 @@ void choose_tiling(const GemmArgs& a, int sms, int& BN, int& splits, bool& pair,
     if (c.bn == 512 && (!gemm_tc_wide_enabled() || a.N < 512)) continue;
     if (c.bn != 512 && wide_flag() == 2 && pair_ok && a.N >= 512 && best < 1e300) continue;
     if (c.bn == 256 && a.N < 256) continue;
+    // reading fp32 sums in an epilogue that nothing overlaps costs more than
+    // the wide tile gains (1024 x 32000 x 4096: 249 us, 256 wide 210)
+    if (c.bn == 512 && a.residual_f32) continue;
     const int64_t tile_m = c.pair ? 2 * BM : BM;
     const int64_t tiles = ((a.M + tile_m - 1) / tile_m) * ((a.N + c.bn - 1) / c.bn) * a.batch * a.batch2;
     const int64_t slots = c.pair ? sms / 2 : sms;
@@ -1514,9 +1534,9 @@ void choose_tiling(const GemmArgs& a, int sms, int& BN, int& splits, bool& pair,
       if (sp > 8 && !a.parts) break;
       if (sp > 1 && kbs * products / sp < 8) break;
       // The accumulators lose a little with every addition (2^-24, always
-      // towards zero): at most 2048 elements of K for products that are to be
+      // towards zero): at most 1024 elements of K for products that are to be
       // as good as fp32, the rest is summed in the reduction.
-      if (a.parts && sp < 32 && (kbs + sp - 1) / sp > 32) continue;
+      if (a.parts && sp < 32 && (kbs + sp - 1) / sp > 16) continue;
       const int64_t units = tiles * sp;
       const int64_t waves = (units + slots - 1) / slots;
       const double unit_s = (double)tile_m * c.bn * BK * 2.0 * products * ((kbs + sp - 1) / sp) /
@@ -1737,6 +1757,7 @@ void gemm_tc_impl(DType out_dt, const GemmArgs& a, cudaStream_t s, uint32_t* err
                "gemm_tc: the ReLU bitmask is written by plain epilogues only");
     splits = 1;  // the bits are taken from final outputs
   }
+  if (a.residual_f32) splits = 1;  // the reductions read a residual of C's type
   if (!red && (workspace == nullptr || workspace_floats < (int64_t)splits * a.M * a.N * a.batch * a.batch2))
     splits = 1;
   if (a.colsum != nullptr || a.relu_bits_out != nullptr || !red) sk = false;
@@ -1795,6 +1816,9 @@ void gemm_tc_impl(DType out_dt, const GemmArgs& a, cudaStream_t s, uint32_t* err
              ((a.batch2_stride_c * esz) % 16 == 0);
   p.r_vec = a.residual && al16(a.residual) && ((a.ldr * esz) % 16 == 0) && ((a.batch_stride_r * esz) % 16 == 0) &&
             ((a.batch2_stride_r * esz) % 16 == 0);
+  p.r_f32 = a.residual != nullptr && a.residual_f32 && !p.out_f32;
+  DLVK_CHECK(!p.r_f32 || (a.batch == 1 && a.batch2 == 1 && a.beta == 0.f), "gemm_tc: an fp32 residual needs a 2-D GEMM without beta");
+  if (p.r_f32) p.r_vec = al16(a.residual) && a.ldr % 4 == 0;
   p.m_vec = a.relu_mask && al16(a.relu_mask) && ((a.ldm * esz) % 16 == 0) && ((a.batch_stride_m * esz) % 16 == 0) &&
             ((a.batch2_stride_m * esz) % 16 == 0);
   p.alpha = a.alpha;
@@ -2056,7 +2080,7 @@ void gemm_tc_plan(DType out_dt, const GemmArgs& a, int max_ctas, int* bn, int* s
 }
 
 int64_t gemm_tc_workspace_floats(const GemmArgs& a, int max_ctas, DType out_dt, bool tf32) {
-  if (split_red_ok(out_dt, a) || a.colsum != nullptr) return 0;
+  if (split_red_ok(out_dt, a) || a.colsum != nullptr || a.residual_f32) return 0;
   int BN = 256, splits = 1;
   bool pair = false;
   choose_tiling(a, max_ctas > 0 ? max_ctas : sm_count(), BN, splits, pair, false, out_dt == DType::F32, tf32);

@@ -80,7 +80,7 @@ __global__ void __launch_bounds__(1024) count_kernel(CeRows r, int mean, const f
   }
 }
 
-constexpr int FIN_ROWS = 32, FIN_WARPS = 16;
+constexpr int FIN_ROWS = 32, FIN_WARPS = 32;
 
 // A block joins 32 rows (lane = row, the warps share the columns), copies
 // their x rows when asked, and adds up their losses; the block that comes
@@ -198,7 +198,9 @@ __global__ void __launch_bounds__(256) rescale_kernel(CeRows r, const float2* __
                                                       int64_t lde) {
   __shared__ float factor[RS_COLS / 64][RS_ROWS];
   __shared__ int label[RS_ROWS];
-  const int64_t row0 = (int64_t)blockIdx.y * RS_ROWS, col0 = (int64_t)blockIdx.x * RS_COLS;
+  // backwards: the exponentials that were written last are still in L2
+  const int64_t row0 = (int64_t)(gridDim.y - 1 - blockIdx.y) * RS_ROWS;
+  const int64_t col0 = (int64_t)(gridDim.x - 1 - blockIdx.x) * RS_COLS;
   const int rows = (int)min((int64_t)RS_ROWS, r.rows - row0);
   const int64_t stat0 = col0 >> width_shift, stats_all = (r.classes + (1 << width_shift) - 1) >> width_shift;
   for (int i = threadIdx.x; i < (RS_COLS >> width_shift) * RS_ROWS; i += 256) {
@@ -289,36 +291,49 @@ __global__ void __launch_bounds__(256) memory_stats_kernel(CeRows r, const float
   }
 }
 
+// One row per block, four columns a thread (rows of z and of the parts are
+// whole 128-byte lines).
 __global__ void __launch_bounds__(256) memory_grad_kernel(CeRows r, float* __restrict__ z, int64_t ldz,
                                                           const float2* __restrict__ norm,
                                                           const float* __restrict__ gscale,
-                                                          __nv_bfloat16* __restrict__ dl, int64_t pitch) {
+                                                          __nv_bfloat16* __restrict__ dl, int64_t pitch, int keep_z) {
   const int64_t row = blockIdx.x;
   float* p = z + row * ldz;
   const int lab = row_label(r, row);
   const float g = *gscale;
   const float2 n = norm[row];
-  for (int64_t c = threadIdx.x; c < r.classes; c += 256) {
-    float v = 0.f;
-    if (lab >= 0) {
-      v = exp2f((p[c] - n.x) * LOG2E) * n.y;
-      if (c == lab) v -= 1.f;
+  const int64_t end = pitch != 0 ? pitch : (r.classes + 3) / 4 * 4;  // the padding becomes 0
+  for (int64_t c = 4 * threadIdx.x; c < end; c += 4 * 256) {
+    float4 u = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (lab >= 0 && c < r.classes) u = *reinterpret_cast<const float4*>(p + c);
+    float v[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      if (lab < 0 || c + k >= r.classes) {
+        v[k] = 0.f;
+      } else {
+        v[k] = exp2f((v[k] - n.x) * LOG2E) * n.y;
+        if (c + k == lab) v[k] -= 1.f;
+      }
     }
-    p[c] = v * g;
+    if (keep_z && c < ldz) *reinterpret_cast<float4*>(p + c) = make_float4(v[0] * g, v[1] * g, v[2] * g, v[3] * g);
     if (dl == nullptr) continue;
     if (pitch == 0) {
-      dl[row * ldz + c] = __float2bfloat16_rn(v * g);
-    } else {
-      __nv_bfloat16 q[3];
-      three_parts(v, q);
 #pragma unroll
-      for (int k = 0; k < 3; ++k) dl[row * 3 * pitch + k * pitch + c] = q[k];
+      for (int k = 0; k < 4; ++k) dl[row * ldz + c + k] = __float2bfloat16_rn(v[k] * g);
+    } else {
+      __nv_bfloat16 q[4][3];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) three_parts(v[k], q[k]);
+#pragma unroll
+      for (int t = 0; t < 3; ++t) {
+        __nv_bfloat162 a, b;
+        a.x = q[0][t]; a.y = q[1][t]; b.x = q[2][t]; b.y = q[3][t];
+        *reinterpret_cast<uint2*>(dl + (row * 3 + t) * pitch + c) =
+            make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+      }
     }
   }
-  if (pitch != 0)
-    for (int64_t c = r.classes + threadIdx.x; c < pitch; c += 256)
-#pragma unroll
-      for (int k = 0; k < 3; ++k) dl[row * 3 * pitch + k * pitch + c] = __float2bfloat16_rn(0.f);
 }
 
 // A block splits rows blockIdx.y, ...; a thread four columns.
@@ -448,8 +463,9 @@ void ce_memory_stats(const CeRows& r, const float* z, int64_t ldz, float2* stats
 }
 
 void ce_memory_grad(const CeRows& r, float* z, int64_t ldz, const float2* norm, const float* gscale, __nv_bfloat16* dl,
-                    int64_t pitch, cudaStream_t s) {
-  memory_grad_kernel<<<(unsigned)r.rows, 256, 0, s>>>(r, z, ldz, norm, gscale, dl, pitch);
+                    int64_t pitch, bool keep_z, cudaStream_t s) {
+  DLVK_CHECK(ldz % 4 == 0 && al16(z) && pitch % 4 == 0 && al16(dl), "ce_memory_grad: layout");
+  memory_grad_kernel<<<(unsigned)r.rows, 256, 0, s>>>(r, z, ldz, norm, gscale, dl, pitch, keep_z ? 1 : 0);
   DLVK_POST_LAUNCH();
 }
 
