@@ -140,8 +140,11 @@ at::Tensor run(const TensorRefs& grads, const TensorRefs* outs, bool scale, doub
     const auto ti = t.scalar_type(), to = o.scalar_type();
     TORCH_CHECK((ti == at::kFloat || ti == at::kBFloat16) && (to == at::kFloat || to == at::kBFloat16), "dlvk.", what,
                 ": tensor ", i, " is neither fp32 nor bf16");
-    TORCH_CHECK(t.layout() == at::kStrided && o.layout() == at::kStrided, "dlvk.", what, ": tensor ", i, " is not strided");
-    if (outs) TORCH_CHECK(t.sizes() == o.sizes(), "dlvk.", what, ": gradient ", i, " is ", t.sizes(), ", its output ", o.sizes());
+    TORCH_CHECK(t.layout() == at::kStrided && o.layout() == at::kStrided, "dlvk.", what, ": tensor ", i,
+                " is not strided");
+    if (outs)
+      TORCH_CHECK(t.sizes() == o.sizes(), "dlvk.", what, ": gradient ", i, " is ", t.sizes(), ", its output ",
+                  o.sizes());
     if (t.numel() == 0) continue;
     const bool same = t.data_ptr() == o.data_ptr();
     if (outs && same)
@@ -160,6 +163,7 @@ at::Tensor run(const TensorRefs& grads, const TensorRefs* outs, bool scale, doub
   }
   if (scale) check_disjoint(ex, what);
   c10::cuda::CUDAGuard g(dev);
+  const PdlScope pdl;
   at::AutoDispatchBelowADInplaceOrView below;
   auto opt = grads[0]->options();
   at::Tensor norm = at::empty({}, opt.dtype(at::kFloat));

@@ -176,6 +176,7 @@ LinearCeResult linear_ce_op(const at::Tensor& x, const at::Tensor& w, const at::
                     db_out->numel() == V && db_out->device() == dev,
                 "dlvk.linear_ce: the bias gradient must be contiguous fp32 [", V, "] on ", dev);
   c10::cuda::CUDAGuard g(dev);
+  const PdlScope pdl;  // each launch starts up while the one before it ends
   at::AutoDispatchBelowADInplaceOrView below;  // no autograd bookkeeping for what follows
   const auto f32 = x.options().dtype(at::kFloat);
   const bool bf = dt == at::kBFloat16;

@@ -463,6 +463,7 @@ at::Tensor embedding_grad_op(const at::Tensor& ids, const at::Tensor& dy, int64_
   }
   auto idc = ids.contiguous();
   auto dyc = dy.dim() == 2 && (D <= 1 || dy.stride(1) == 1) ? dy : dy.contiguous();
+  const PdlScope pdl;
   auto io = dy.options().dtype(at::kInt);
   const int64_t pf = embedding_grad_part_floats(n, (int)D);
   // one allocation: part first (16-byte aligned), then the three integer arrays

@@ -79,9 +79,17 @@ namespace dlvk {
 // returns once the previous grid has completed and its writes are visible.
 // The persistent tensor-core kernels call pdl_trigger() when a CTA has
 // finished its work, so their successor's prologue overlaps the tail.
-// Opt-in with DLVK_PDL=1; otherwise the launches are ordinary
-// stream-serialised ones and the waits return at once.
+// DLVK_PDL=1 turns it on everywhere, DLVK_PDL=0 off; by default it is on where
+// a launcher opens a PdlScope (operators of several short launches, every one
+// of which waits) and the other launches are ordinary stream-serialised ones,
+// whose waits return at once.
 bool pdl_enabled();
+struct PdlScope {
+  PdlScope();
+  ~PdlScope();
+  PdlScope(const PdlScope&) = delete;
+  PdlScope& operator=(const PdlScope&) = delete;
+};
 
 template <typename... KArgs, typename... Args>
 inline void launch_pdl(void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t s, Args&&... args) {

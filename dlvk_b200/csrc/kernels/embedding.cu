@@ -14,6 +14,7 @@
 // words: 17 MB in, 131 MB out, 22.6 us at the measured copy rate), so the
 // sort has to be short.
 #include <algorithm>
+#include <type_traits>
 
 #include "dlvk/common.h"
 #include "dlvk/kernels.h"
@@ -115,6 +116,7 @@ __global__ void __launch_bounds__(SORT_THREADS) sort_tokens_kernel(const ID* __r
                                                                    int* __restrict__ order, int* __restrict__ word,
                                                                    int sort_blocks, float* __restrict__ dtable,
                                                                    int clear_to, int D, int vec) {
+  pdl_wait();
   if ((int)blockIdx.x >= sort_blocks) {
     const int warps = (gridDim.x - sort_blocks) * SORT_WARPS;
     for (int v = (blockIdx.x - sort_blocks) * SORT_WARPS + (threadIdx.x >> 5); v < clear_to; v += warps)
@@ -249,6 +251,7 @@ __global__ void __launch_bounds__(RED_THREADS) sum_chunks_kernel(
     const T* __restrict__ dy, int64_t ld, const int* __restrict__ start, const int* __restrict__ order,
     const int* __restrict__ word, float* __restrict__ dtable, float* __restrict__ part, int V, int D, int C, int TX,
     int chunk_blocks, float scale, int accumulate, int clear_from, int clear_to) {
+  pdl_wait();
   if ((int)blockIdx.x >= chunk_blocks) {
     clear_empty_rows(start, dtable, clear_from, clear_to, D, VEC > 1,
                      (blockIdx.x - chunk_blocks) * (RED_THREADS / 32) + (threadIdx.x >> 5),
@@ -301,6 +304,7 @@ __global__ void __launch_bounds__(RED_THREADS) join_kernel(const int* __restrict
                                                            const float* __restrict__ part, float* __restrict__ dtable,
                                                            int V, int D, int C, int TX, int chunks, float scale,
                                                            int accumulate, int join_blocks, int clear_from) {
+  pdl_wait();
   if ((int)blockIdx.x >= join_blocks) {
     clear_empty_rows(start, dtable, clear_from, V, D, VEC > 1,
                      (blockIdx.x - join_blocks) * (RED_THREADS / 32) + (threadIdx.x >> 5),
@@ -376,8 +380,8 @@ void sums(const T* dy, int64_t ld, const int* start, const int* order, const int
   const int chunk_blocks = (chunks + per - 1) / per;
   const int zero_blocks = clear_blocks(z2 - z1, RED_THREADS / 32);
   if (chunk_blocks + zero_blocks > 0) {
-    sum_chunks_kernel<T, VEC><<<chunk_blocks + zero_blocks, RED_THREADS, 0, s>>>(
-        dy, ld, start, order, word, dtable, part, V, D, C, tx, chunk_blocks, scale, accumulate ? 1 : 0, z1, z2);
+    launch_pdl(sum_chunks_kernel<T, VEC>, dim3(chunk_blocks + zero_blocks), dim3(RED_THREADS), 0, s, dy, ld, start,
+               order, word, dtable, part, V, D, C, tx, chunk_blocks, scale, accumulate ? 1 : 0, z1, z2);
     DLVK_POST_LAUNCH();
   }
   const int last_blocks = clear_blocks(V - z2, RED_THREADS / 32);
@@ -385,8 +389,8 @@ void sums(const T* dy, int64_t ld, const int* start, const int* order, const int
     constexpr int JV = VEC > 1 ? 4 : 1;
     const int jx = across(D, JV), jper = RED_THREADS / jx;
     const int join_blocks = chunks > 1 ? (chunks + jper - 1) / jper : 0;
-    join_kernel<JV><<<join_blocks + last_blocks, RED_THREADS, 0, s>>>(start, word, part, dtable, V, D, C, jx, chunks,
-                                                                      scale, accumulate ? 1 : 0, join_blocks, z2);
+    launch_pdl(join_kernel<JV>, dim3(join_blocks + last_blocks), dim3(RED_THREADS), 0, s, start, word, part, dtable, V,
+               D, C, jx, chunks, scale, accumulate ? 1 : 0, join_blocks, z2);
     DLVK_POST_LAUNCH();
   }
 }
@@ -432,8 +436,9 @@ void embedding_grad(DType dt, bool ids64, const void* ids, const void* dy, int64
   const int dev = current_device_slot();
   if (!attr_set[dev]) {
     const int most = room(SORT_WORDS);
-    DLVK_CUDA_CHECK(cudaFuncSetAttribute(sort_tokens_kernel<int32_t>, cudaFuncAttributeMaxDynamicSharedMemorySize, most));
-    DLVK_CUDA_CHECK(cudaFuncSetAttribute(sort_tokens_kernel<int64_t>, cudaFuncAttributeMaxDynamicSharedMemorySize, most));
+    const auto attr = cudaFuncAttributeMaxDynamicSharedMemorySize;
+    DLVK_CUDA_CHECK(cudaFuncSetAttribute(sort_tokens_kernel<int32_t>, attr, most));
+    DLVK_CUDA_CHECK(cudaFuncSetAttribute(sort_tokens_kernel<int64_t>, attr, most));
     attr_set[dev] = true;
   }
   const int pad = padding >= 0 && padding < V ? (int)padding : -1;
@@ -447,9 +452,10 @@ void embedding_grad(DType dt, bool ids64, const void* ids, const void* dy, int64
   const int z1 = accumulate ? (int)V : (int)(half * 25 / 100);
   const int z2 = accumulate ? (int)V : (int)(V - (n < V ? V * 25 / 100 : 0));
   const int sort_clear = accumulate ? 0 : (int)std::min<int64_t>((z1 + SORT_WARPS - 1) / SORT_WARPS, 148);
-  const auto sort = [&](auto* p) {
-    sort_tokens_kernel<<<blocks + sort_clear, SORT_THREADS, smem, s>>>(p, (int)n, (int)V, R, pad, start, order, word, blocks,
-                                                                       dtable, z1, D, vec ? 1 : 0);
+  const auto sort = [&](const auto* p) {
+    using ID = std::remove_cv_t<std::remove_reference_t<decltype(*p)>>;
+    launch_pdl(sort_tokens_kernel<ID>, dim3(blocks + sort_clear), dim3(SORT_THREADS), smem, s, p, (int)n, (int)V, R,
+               pad, start, order, word, blocks, dtable, z1, D, vec ? 1 : 0);
   };
   if (ids64) sort(reinterpret_cast<const int64_t*>(ids));
   else sort(reinterpret_cast<const int32_t*>(ids));

@@ -1424,6 +1424,7 @@ __global__ void splitk_reduce_kernel(const float* __restrict__ ws, int splits, i
 template <typename T>
 __global__ void __launch_bounds__(256) splitk_reduce4_kernel(const float* __restrict__ ws, int splits,
                                                              int64_t per_split, GemmArgs a) {
+  pdl_wait();
   const float alpha = a.alpha_ptr ? a.alpha * *a.alpha_ptr : a.alpha;
   for (int64_t i = 4 * (blockIdx.x * (int64_t)blockDim.x + threadIdx.x); i < per_split;
        i += 4 * (int64_t)gridDim.x * blockDim.x) {
@@ -1897,8 +1898,10 @@ void gemm_tc_impl(DType out_dt, const GemmArgs& a, cudaStream_t s, uint32_t* err
     const int g = (int)std::min<int64_t>((per + 255) / 256, 148 * 16);
     if (plain) {
       const int g4 = (int)std::min<int64_t>((per / 4 + 255) / 256, 148 * 8);
-      if (out_dt == DType::F32) splitk_reduce4_kernel<float><<<g4, 256, 0, s>>>(workspace, splits, per, a);
-      else splitk_reduce4_kernel<__nv_bfloat16><<<g4, 256, 0, s>>>(workspace, splits, per, a);
+      if (out_dt == DType::F32)
+        launch_pdl(splitk_reduce4_kernel<float>, dim3(g4), dim3(256), 0, s, workspace, splits, per, a);
+      else
+        launch_pdl(splitk_reduce4_kernel<__nv_bfloat16>, dim3(g4), dim3(256), 0, s, workspace, splits, per, a);
     } else if (out_dt == DType::F32) splitk_reduce_kernel<float><<<g, 256, 0, s>>>(workspace, splits, per, a);
     else splitk_reduce_kernel<__nv_bfloat16><<<g, 256, 0, s>>>(workspace, splits, per, a);
     DLVK_POST_LAUNCH();

@@ -30,7 +30,8 @@ namespace {
 
 constexpr int THREADS = 256;
 constexpr int CHUNK = 8192;      // elements of one tensor that a block takes at a time
-constexpr int MAX_BLOCKS = 148 * 8;
+constexpr int MAX_BLOCKS = 148 * 8;         // of the sums: a partial each
+constexpr int MAX_SCALE_BLOCKS = 148 * 64;  // short blocks keep reads and writes mixed (216 M fp32: 279 -> 256 us)
 
 template <int CAP>
 struct ListTable {
@@ -66,16 +67,15 @@ __device__ __forceinline__ void load4(const __nv_bfloat16* p, float* v) {
   v[2] = __uint_as_float(u.y << 16);
   v[3] = __uint_as_float(u.y & 0xffff0000u);
 }
-// Written once and not read here: evicted first, so that inputs stay in L2.
 __device__ __forceinline__ void store4(float* p, const float* v) {
-  __stcs(reinterpret_cast<float4*>(p), make_float4(v[0], v[1], v[2], v[3]));
+  *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
 }
 __device__ __forceinline__ void store4(__nv_bfloat16* p, const float* v) {
   const __nv_bfloat162 a = __floats2bfloat162_rn(v[0], v[1]), b = __floats2bfloat162_rn(v[2], v[3]);
   uint2 u;
   u.x = *reinterpret_cast<const uint32_t*>(&a);
   u.y = *reinterpret_cast<const uint32_t*>(&b);
-  __stcs(reinterpret_cast<uint2*>(p), u);
+  *reinterpret_cast<uint2*>(p) = u;
 }
 
 // Sum of four squares; see the note on range at the top.  Below 1e-30 a
@@ -135,6 +135,7 @@ __device__ __forceinline__ double block_sum_f64(double v) {
 template <int CAP>
 __global__ void __launch_bounds__(THREADS) list_squares_kernel(const __grid_constant__ ListTable<CAP> t,
                                                                double* __restrict__ partial) {
+  pdl_wait();
   double acc = 0.0;
   for (int c = blockIdx.x; c < t.chunks; c += gridDim.x) {
     const int i = find_tensor(t, c);
@@ -168,6 +169,7 @@ __device__ __forceinline__ void store1(void* p, int64_t i, bool bf, float v) {
 
 __global__ void __launch_bounds__(THREADS) strided_squares_kernel(const __grid_constant__ StridedItem s,
                                                                   double* __restrict__ partial) {
+  pdl_wait();
   double acc = 0.0;
   const bool bf = s.kind & 1;
   for (int64_t e = blockIdx.x * (int64_t)THREADS + threadIdx.x; e < s.n; e += (int64_t)gridDim.x * THREADS)
@@ -190,13 +192,15 @@ __device__ __forceinline__ float clip_coefficient(double norm, float max_norm) {
 
 __global__ void __launch_bounds__(THREADS) list_norm_kernel(const double* __restrict__ partial, int parts,
                                                             float* __restrict__ norm) {
+  pdl_wait();
   const double r = list_norm(partial, parts);
   if (threadIdx.x == 0) *norm = (float)r;
 }
 
 template <typename TI, typename TO>
 __device__ __forceinline__ void chunk_scale(const TI* p, TO* o, int n, float c) {
-  const int head = min(n, (int)(((4 * sizeof(TI) - reinterpret_cast<uintptr_t>(p) % (4 * sizeof(TI))) / sizeof(TI)) & 3));
+  constexpr int STEP = 4 * (int)sizeof(TI);
+  const int head = min(n, (int)((STEP - reinterpret_cast<uintptr_t>(p) % STEP) / sizeof(TI)) & 3);
   if (reinterpret_cast<uintptr_t>(o + head) % (4 * sizeof(TO)) != 0) {
     // input and output are never aligned together: element by element
     int i = threadIdx.x;
@@ -242,6 +246,7 @@ template <int CAP>
 __global__ void __launch_bounds__(THREADS) list_scale_kernel(const __grid_constant__ ListTable<CAP> t,
                                                              const double* __restrict__ partial, int parts,
                                                              float max_norm, float* __restrict__ norm, int in_place) {
+  pdl_wait();
   const double r = list_norm(partial, parts);
   if (blockIdx.x == 0 && threadIdx.x == 0) *norm = (float)r;
   const float coef = clip_coefficient(r, max_norm);
@@ -266,6 +271,7 @@ __global__ void __launch_bounds__(THREADS) list_scale_kernel(const __grid_consta
 __global__ void __launch_bounds__(THREADS) strided_scale_kernel(const __grid_constant__ StridedItem s,
                                                                 const double* __restrict__ partial, int parts,
                                                                 float max_norm, float* __restrict__ norm) {
+  pdl_wait();
   const double r = list_norm(partial, parts);
   if (blockIdx.x == 0 && threadIdx.x == 0) *norm = (float)r;
   const float coef = clip_coefficient(r, max_norm);
@@ -314,12 +320,13 @@ void for_each_table(const DenseItem* dense, int n_dense, F&& launch) {
 
 template <int CAP>
 void squares_launch(const ListTable<CAP>& t, int blocks, double* partial, cudaStream_t s) {
-  list_squares_kernel<CAP><<<blocks, THREADS, 0, s>>>(t, partial);
+  launch_pdl(list_squares_kernel<CAP>, dim3(blocks), dim3(THREADS), 0, s, t, partial);
 }
 template <int CAP>
-void scale_launch(const ListTable<CAP>& t, int blocks, const double* partial, int parts, float max_norm, float* norm,
+void scale_launch(const ListTable<CAP>& t, const double* partial, int parts, float max_norm, float* norm,
                   int in_place, cudaStream_t s) {
-  list_scale_kernel<CAP><<<blocks, THREADS, 0, s>>>(t, partial, parts, max_norm, norm, in_place);
+  launch_pdl(list_scale_kernel<CAP>, dim3(std::min(t.chunks, MAX_SCALE_BLOCKS)), dim3(THREADS), 0, s, t, partial, parts,
+             max_norm, norm, in_place);
 }
 
 }  // namespace
@@ -345,23 +352,24 @@ void grad_norm(const DenseItem* dense, int n_dense, const StridedItem* strided, 
   });
   for (int i = 0; i < n_strided; ++i) {
     const int blocks = strided_blocks(strided[i].n);
-    strided_squares_kernel<<<blocks, THREADS, 0, s>>>(strided[i], partial + parts);
+    launch_pdl(strided_squares_kernel, dim3(blocks), dim3(THREADS), 0, s, strided[i], partial + parts);
     DLVK_POST_LAUNCH();
     parts += blocks;
   }
   if (!scale || n_dense + n_strided == 0) {
-    list_norm_kernel<<<1, THREADS, 0, s>>>(partial, parts, norm);
+    launch_pdl(list_norm_kernel, dim3(1), dim3(THREADS), 0, s, partial, parts, norm);
     DLVK_POST_LAUNCH();
     return;
   }
   bool in_place = true;
   for (int i = 0; i < n_dense; ++i) in_place = in_place && dense[i].in == dense[i].out;
-  for_each_table(dense, n_dense, [&](const auto& t, int blocks) {
-    scale_launch(t, blocks, partial, parts, max_norm, norm, in_place ? 1 : 0, s);
+  for_each_table(dense, n_dense, [&](const auto& t, int) {
+    scale_launch(t, partial, parts, max_norm, norm, in_place ? 1 : 0, s);
     DLVK_POST_LAUNCH();
   });
   for (int i = 0; i < n_strided; ++i) {
-    strided_scale_kernel<<<strided_blocks(strided[i].n), THREADS, 0, s>>>(strided[i], partial, parts, max_norm, norm);
+    launch_pdl(strided_scale_kernel, dim3(strided_blocks(strided[i].n)), dim3(THREADS), 0, s, strided[i], partial,
+               parts, max_norm, norm);
     DLVK_POST_LAUNCH();
   }
 }

@@ -65,6 +65,7 @@ __device__ __forceinline__ double share_of(int mean, double counted) {
 
 __global__ void __launch_bounds__(1024) count_kernel(CeRows r, int mean, const float* __restrict__ grad_scale,
                                                      float* __restrict__ gscale, unsigned* __restrict__ done) {
+  pdl_wait();
   __shared__ int sm[32];
   int n = 0;
   for (int64_t i = threadIdx.x; i < r.rows; i += 1024) n += row_label(r, i) >= 0;
@@ -87,6 +88,7 @@ constexpr int FIN_ROWS = 32, FIN_WARPS = 32;
 // last of all adds the blocks' sums in their order.
 template <typename T>
 __global__ void __launch_bounds__(FIN_WARPS * 32) finish_kernel(CeRows r, CeFinish f, int vec) {
+  pdl_wait();
   __shared__ float sm_m[FIN_WARPS][FIN_ROWS], sm_s[FIN_WARPS][FIN_ROWS];
   __shared__ int counted[FIN_ROWS];
   __shared__ int last;
@@ -196,6 +198,7 @@ constexpr int RS_COLS = 2048, RS_ROWS = 32;
 __global__ void __launch_bounds__(256) rescale_kernel(CeRows r, const float2* __restrict__ stats, int width_shift,
                                                       const float2* __restrict__ norm, uint16_t* __restrict__ e,
                                                       int64_t lde) {
+  pdl_wait();
   __shared__ float factor[RS_COLS / 64][RS_ROWS];
   __shared__ int label[RS_ROWS];
   // backwards: the exponentials that were written last are still in L2
@@ -257,6 +260,7 @@ __global__ void __launch_bounds__(256) rescale_kernel(CeRows r, const float2* __
 __global__ void __launch_bounds__(256) memory_stats_kernel(CeRows r, const float* __restrict__ z, int64_t ldz,
                                                            float2* __restrict__ stats, float* __restrict__ zlabel,
                                                            unsigned* __restrict__ done) {
+  pdl_wait();
   __shared__ float sm_m[8], sm_s[8];
   if (blockIdx.x == 0 && threadIdx.x == 0 && done != nullptr) *done = 0u;
   const int64_t row = blockIdx.x;
@@ -297,6 +301,7 @@ __global__ void __launch_bounds__(256) memory_grad_kernel(CeRows r, float* __res
                                                           const float2* __restrict__ norm,
                                                           const float* __restrict__ gscale,
                                                           __nv_bfloat16* __restrict__ dl, int64_t pitch, int keep_z) {
+  pdl_wait();
   const int64_t row = blockIdx.x;
   float* p = z + row * ldz;
   const int lab = row_label(r, row);
@@ -340,6 +345,7 @@ __global__ void __launch_bounds__(256) memory_grad_kernel(CeRows r, float* __res
 __global__ void __launch_bounds__(256) split_parts_kernel(const float* __restrict__ src, int64_t ld, int64_t rows,
                                                           int64_t cols, __nv_bfloat16* __restrict__ dst, int64_t pitch,
                                                           CeRows mask, int masked, int vec) {
+  pdl_wait();
   const int64_t c = 4 * ((int64_t)blockIdx.x * 256 + threadIdx.x);
   if (c >= pitch) return;
   for (int64_t i = blockIdx.y; i < rows; i += gridDim.y) {
@@ -372,6 +378,7 @@ template <typename TD, typename TS>
 __global__ void __launch_bounds__(256) copy_matrix_kernel(const TS* __restrict__ src, int64_t rs, int64_t cs,
                                                           TD* __restrict__ dst, int64_t ldd, int64_t rows, int64_t cols,
                                                           int64_t pad_to, int accumulate) {
+  pdl_wait();
   for (int64_t i = blockIdx.y; i < rows; i += gridDim.y) {
     for (int64_t c = blockIdx.x * 1024 + threadIdx.x; c < pad_to; c += (int64_t)gridDim.x * 1024) {
 #pragma unroll
@@ -390,6 +397,7 @@ __global__ void __launch_bounds__(256) copy_matrix_kernel(const TS* __restrict__
 __global__ void __launch_bounds__(256) round_matrix_kernel(const float* __restrict__ src, int64_t rs,
                                                            __nv_bfloat16* __restrict__ dst, int64_t ldd, int64_t rows,
                                                            int64_t cols) {
+  pdl_wait();
   const int64_t c = 8 * ((int64_t)blockIdx.x * 256 + threadIdx.x);
   if (c >= cols) return;
   for (int64_t i = blockIdx.y; i < rows; i += 2 * (int64_t)gridDim.y) {
@@ -419,8 +427,8 @@ template <typename TD, typename TS>
 void copy_matrix_t(const void* src, int64_t rs, int64_t cs, void* dst, int64_t ldd, int64_t rows, int64_t cols,
                    int64_t pad_to, bool accumulate, cudaStream_t s) {
   const dim3 grid((unsigned)std::min<int64_t>((pad_to + 1023) / 1024, 64), (unsigned)std::min<int64_t>(rows, 65535));
-  copy_matrix_kernel<TD, TS><<<grid, 256, 0, s>>>(reinterpret_cast<const TS*>(src), rs, cs, reinterpret_cast<TD*>(dst),
-                                                  ldd, rows, cols, pad_to, accumulate ? 1 : 0);
+  launch_pdl(copy_matrix_kernel<TD, TS>, grid, dim3(256), 0, s, reinterpret_cast<const TS*>(src), rs, cs,
+             reinterpret_cast<TD*>(dst), ldd, rows, cols, pad_to, accumulate ? 1 : 0);
   DLVK_POST_LAUNCH();
 }
 
@@ -430,14 +438,15 @@ template <typename T>
 void finish_t(const CeRows& r, const CeFinish& f, cudaStream_t s) {
   constexpr int V = 16 / (int)sizeof(T);
   const int vec = al16(f.x) && al16(f.x_clean) && f.ldx % V == 0 && f.ldc % V == 0 && f.width % V == 0;
-  finish_kernel<T><<<(unsigned)((r.rows + FIN_ROWS - 1) / FIN_ROWS), FIN_WARPS * 32, 0, s>>>(r, f, vec);
+  launch_pdl(finish_kernel<T>, dim3((unsigned)((r.rows + FIN_ROWS - 1) / FIN_ROWS)), dim3(FIN_WARPS * 32), 0, s, r, f,
+             vec);
   DLVK_POST_LAUNCH();
 }
 
 }  // namespace
 
 void ce_count(const CeRows& r, bool mean, const float* grad_scale, float* gscale, unsigned* done, cudaStream_t s) {
-  count_kernel<<<1, 1024, 0, s>>>(r, mean ? 1 : 0, grad_scale, gscale, done);
+  launch_pdl(count_kernel, dim3(1), dim3(1024), 0, s, r, mean ? 1 : 0, grad_scale, gscale, done);
   DLVK_POST_LAUNCH();
 }
 
@@ -451,21 +460,22 @@ void ce_rescale(const CeRows& r, const float2* stats, int stat_width, const floa
   DLVK_CHECK((stat_width == 64 || stat_width == 128) && lde % 8 == 0 && al16(e), "ce_rescale: layout");
   const dim3 grid((unsigned)((r.classes + RS_COLS - 1) / RS_COLS), (unsigned)((r.rows + RS_ROWS - 1) / RS_ROWS));
   DLVK_CHECK(grid.y <= 65535u, "ce_rescale: more than 2^21 rows in one block of rows");
-  rescale_kernel<<<grid, 256, 0, s>>>(r, stats, stat_width == 64 ? 6 : 7, norm,
-                                      reinterpret_cast<uint16_t*>(e), lde);
+  launch_pdl(rescale_kernel, grid, dim3(256), 0, s, r, stats, stat_width == 64 ? 6 : 7, norm,
+             reinterpret_cast<uint16_t*>(e), lde);
   DLVK_POST_LAUNCH();
 }
 
 void ce_memory_stats(const CeRows& r, const float* z, int64_t ldz, float2* stats, float* zlabel, unsigned* done,
                      cudaStream_t s) {
-  memory_stats_kernel<<<(unsigned)r.rows, 256, 0, s>>>(r, z, ldz, stats, zlabel, done);
+  launch_pdl(memory_stats_kernel, dim3((unsigned)r.rows), dim3(256), 0, s, r, z, ldz, stats, zlabel, done);
   DLVK_POST_LAUNCH();
 }
 
 void ce_memory_grad(const CeRows& r, float* z, int64_t ldz, const float2* norm, const float* gscale, __nv_bfloat16* dl,
                     int64_t pitch, bool keep_z, cudaStream_t s) {
   DLVK_CHECK(ldz % 4 == 0 && al16(z) && pitch % 4 == 0 && al16(dl), "ce_memory_grad: layout");
-  memory_grad_kernel<<<(unsigned)r.rows, 256, 0, s>>>(r, z, ldz, norm, gscale, dl, pitch, keep_z ? 1 : 0);
+  launch_pdl(memory_grad_kernel, dim3((unsigned)r.rows), dim3(256), 0, s, r, z, ldz, norm, gscale, dl, pitch,
+             keep_z ? 1 : 0);
   DLVK_POST_LAUNCH();
 }
 
@@ -474,8 +484,8 @@ void split_parts(const float* src, int64_t ld, int64_t rows, int64_t cols, __nv_
   DLVK_CHECK(pitch % 64 == 0 && pitch >= cols && al16(dst), "split_parts: layout");
   if (rows == 0) return;
   const dim3 grid((unsigned)((pitch + 1023) / 1024), (unsigned)std::min<int64_t>(rows, 16384));
-  split_parts_kernel<<<grid, 256, 0, s>>>(src, ld, rows, cols, dst, pitch, mask ? *mask : CeRows{}, mask != nullptr,
-                                          al16(src) && ld % 4 == 0);
+  launch_pdl(split_parts_kernel, grid, dim3(256), 0, s, src, ld, rows, cols, dst, pitch, mask ? *mask : CeRows{},
+             mask != nullptr ? 1 : 0, al16(src) && ld % 4 == 0 ? 1 : 0);
   DLVK_POST_LAUNCH();
 }
 
@@ -485,8 +495,8 @@ void copy_matrix(DType dst_dt, DType src_dt, const void* src, int64_t rs, int64_
   if (dst_dt == DType::BF16 && src_dt == DType::F32 && cs == 1 && !accumulate && cols == pad_to && cols % 8 == 0 &&
       rs % 4 == 0 && ldd % 8 == 0 && al16(src) && al16(dst)) {
     const dim3 grid((unsigned)((cols / 8 + 255) / 256), (unsigned)std::min<int64_t>((rows + 1) / 2, 4096));
-    round_matrix_kernel<<<grid, 256, 0, s>>>(reinterpret_cast<const float*>(src), rs,
-                                             reinterpret_cast<__nv_bfloat16*>(dst), ldd, rows, cols);
+    launch_pdl(round_matrix_kernel, grid, dim3(256), 0, s, reinterpret_cast<const float*>(src), rs,
+               reinterpret_cast<__nv_bfloat16*>(dst), ldd, rows, cols);
     DLVK_POST_LAUNCH();
     return;
   }
