@@ -351,13 +351,14 @@ LinearCeResult linear_ce_op(const at::Tensor& x, const at::Tensor& w, const at::
       f.ldc = ldx;
       xo = rows_operand(xc, 0, n, E, ldx);
     }
-    ce_finish(r, f, to_dtype(x), stream());
+    const bool join = keep && ce_rescale_joins(f.stat_cols);
+    if (!join) ce_finish(r, f, to_dtype(x), stream());
     if (!want_grad) continue;
 
     const Operand d = parts ? parts_operand(dl, 0, n, V) : rows_operand(dl, 0, n, V, ldv);
     const float* scale = gscale;  // dz holds softmax - onehot, the products its factor
     if (keep) {
-      ce_rescale(r, stats, ce_tc_stat_width(n, V), norm, dl.data_ptr(), ldv, stream());
+      ce_rescale(r, f, ce_tc_stat_width(n, V), join, dl.data_ptr(), ldv, stream());
     } else if (fused) {
       ce_grad_tc(c, reinterpret_cast<__nv_bfloat16*>(dl.data_ptr()), ldv,
                  part.defined() ? part.data_ptr<float>() : nullptr, stream(), device_error_word());

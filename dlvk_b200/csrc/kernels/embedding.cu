@@ -86,18 +86,28 @@ __global__ void __launch_bounds__(256) lookup_kernel(const ID* __restrict__ ids,
 // three launches: [0, Z1) are cleared beside the sort, before it is known
 // which have tokens, [Z1, Z2) and [Z2, V) where they have none, beside the
 // sums and the joins.
-__device__ __forceinline__ void clear_row(float* row, int D, int vec, int lane) {
-  if (vec) {
-    for (int c = lane * 4; c < D; c += 128) *reinterpret_cast<float4*>(row + c) = make_float4(0.f, 0.f, 0.f, 0.f);
-  } else {
-    for (int c = lane; c < D; c += 32) row[c] = 0.f;
-  }
+// A warp clears 32 / tx rows at a time, tx lanes to a row (a power of two: as
+// many as a row has 16-byte steps or elements, at most 32).  `start` null: all
+// rows of [v0, v1), else those without a token.
+__device__ __forceinline__ int lanes_of_row(int D, int vec) {
+  const int steps = vec ? D / 4 : D;
+  int tx = 1;
+  while (tx < 32 && tx < steps) tx *= 2;
+  return tx;
 }
-// A warp of `warps` takes every warps-th word of [v0, v1) that has no token.
-__device__ __forceinline__ void clear_empty_rows(const int* start, float* dtable, int v0, int v1, int D, int vec,
-                                                 int warp, int warps) {
-  for (int v = v0 + warp; v < v1; v += warps)
-    if (start[v] == start[v + 1]) clear_row(dtable + (int64_t)v * D, D, vec, threadIdx.x & 31);
+__device__ __forceinline__ void clear_rows(const int* start, float* dtable, int v0, int v1, int D, int vec, int warp,
+                                           int warps) {
+  const int lane = threadIdx.x & 31, tx = lanes_of_row(D, vec), per = 32 / tx;
+  for (int64_t v = v0 + (int64_t)warp * per + lane / tx; v < v1; v += (int64_t)warps * per) {
+    if (start != nullptr && start[v] != start[v + 1]) continue;
+    float* row = dtable + v * D;
+    if (vec) {
+      for (int c = (lane % tx) * 4; c < D; c += tx * 4)
+        *reinterpret_cast<float4*>(row + c) = make_float4(0.f, 0.f, 0.f, 0.f);
+    } else {
+      for (int c = lane % tx; c < D; c += tx) row[c] = 0.f;
+    }
+  }
 }
 
 // Stable sort of the tokens by word in one launch, without a word between
@@ -118,9 +128,8 @@ __global__ void __launch_bounds__(SORT_THREADS) sort_tokens_kernel(const ID* __r
                                                                    int clear_to, int D, int vec) {
   pdl_wait();
   if ((int)blockIdx.x >= sort_blocks) {
-    const int warps = (gridDim.x - sort_blocks) * SORT_WARPS;
-    for (int v = (blockIdx.x - sort_blocks) * SORT_WARPS + (threadIdx.x >> 5); v < clear_to; v += warps)
-      clear_row(dtable + (int64_t)v * D, D, vec, threadIdx.x & 31);
+    clear_rows(nullptr, dtable, 0, clear_to, D, vec, (blockIdx.x - sort_blocks) * SORT_WARPS + (threadIdx.x >> 5),
+               (gridDim.x - sort_blocks) * SORT_WARPS);
     return;
   }
   extern __shared__ int cnt[];  // [SORT_WARPS][RP], then [R]: a word's first place
@@ -253,9 +262,9 @@ __global__ void __launch_bounds__(RED_THREADS) sum_chunks_kernel(
     int chunk_blocks, float scale, int accumulate, int clear_from, int clear_to) {
   pdl_wait();
   if ((int)blockIdx.x >= chunk_blocks) {
-    clear_empty_rows(start, dtable, clear_from, clear_to, D, VEC > 1,
-                     (blockIdx.x - chunk_blocks) * (RED_THREADS / 32) + (threadIdx.x >> 5),
-                     (gridDim.x - chunk_blocks) * (RED_THREADS / 32));
+    clear_rows(start, dtable, clear_from, clear_to, D, VEC > 1,
+               (blockIdx.x - chunk_blocks) * (RED_THREADS / 32) + (threadIdx.x >> 5),
+               (gridDim.x - chunk_blocks) * (RED_THREADS / 32));
     return;
   }
   const int tx = threadIdx.x % TX;
@@ -306,9 +315,9 @@ __global__ void __launch_bounds__(RED_THREADS) join_kernel(const int* __restrict
                                                            int accumulate, int join_blocks, int clear_from) {
   pdl_wait();
   if ((int)blockIdx.x >= join_blocks) {
-    clear_empty_rows(start, dtable, clear_from, V, D, VEC > 1,
-                     (blockIdx.x - join_blocks) * (RED_THREADS / 32) + (threadIdx.x >> 5),
-                     (gridDim.x - join_blocks) * (RED_THREADS / 32));
+    clear_rows(start, dtable, clear_from, V, D, VEC > 1,
+               (blockIdx.x - join_blocks) * (RED_THREADS / 32) + (threadIdx.x >> 5),
+               (gridDim.x - join_blocks) * (RED_THREADS / 32));
     return;
   }
   const int chunk = blockIdx.x * (RED_THREADS / TX) + threadIdx.x / TX;
@@ -446,7 +455,7 @@ void embedding_grad(DType dt, bool ids64, const void* ids, const void* dy, int64
   DLVK_CHECK(f32 || dt == DType::BF16, "embedding_grad: dy is fp32 or bf16");
   const int step = f32 ? 4 : 8;
   const bool vec = D % step == 0 && ld % step == 0 && al16(dy) && al16(dtable) && al16(part);
-  // The shares of the zero rows (see clear_row), none when adding.  Sharing
+  // The shares of the zero rows (see clear_rows), none when adding.  Sharing
   // pays where both the sums and the zeros are long (8192 tokens x 1024 over
   // 32000 words: 40.7 -> 36.3 us, 4096 x 768 over 50257: 40.4 -> 37.6) and
   // costs where either is short (2048 x 1024 over 32000: 33.3 -> 35.8, 512 x

@@ -562,12 +562,17 @@ __device__ __forceinline__ int ce_label(const TcParams& p, int row) {
   return (lab >= 0 && lab < p.ce.classes && lab != p.ce.ignore) ? (int)lab : -1;
 }
 
-// Accumulator chunk + bias; columns past N become -inf (softmax 0).
-__device__ __forceinline__ void ce_logits(const TcParams& p, const uint32_t* r, int n0, float* v) {
+// Accumulator chunk + bias (lane l holds column n0 + l's, loaded before the
+// tile was waited for: every lane reading all 32 from memory in every chunk
+// exposed that latency); columns past N become -inf (softmax 0).
+__device__ __forceinline__ void ce_logits(const TcParams& p, const uint32_t* r, int n0, float bias, float* v) {
 #pragma unroll
   for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]);
   const int valid = p.N - n0;
-  if (p.bias) add_bias<32>(p.bias, true, n0, min(32, valid), v);
+  if (p.bias) {
+#pragma unroll
+    for (int j = 0; j < 32; ++j) v[j] += __shfl_sync(0xffffffffu, bias, j);
+  }
   if (valid < 32) {
 #pragma unroll
     for (int j = 0; j < 32; ++j) v[j] = j < valid ? v[j] : -INFINITY;
@@ -986,6 +991,21 @@ __global__ void __launch_bounds__(320, 1)
     bool last_tile;
     while (work_next(p, tstep, num_kb, tiles_per_split, num_tiles, w, tm, tn, b, sp, kb0, kb1, last_tile)) {
       int tcount = 0;  // boxes of this tile issued by this warp
+      [[maybe_unused]] float ce_bias[NCH];
+      if constexpr (EPI >= 3) {
+#pragma unroll
+        for (int i = 0; i < NCH; ++i) {
+          const int n = tn * BN + (half * NCH + i) * 32 + lane;
+          ce_bias[i] = (p.bias && n < p.N) ? reinterpret_cast<const float*>(p.bias)[n] : 0.f;
+        }
+      }
+      // the chunk's, without an index that the loops below know only at run time
+      [[maybe_unused]] const auto bias_of = [&](int i) {
+        float b = ce_bias[0];
+#pragma unroll
+        for (int j = 1; j < NCH; ++j) b = i == j ? ce_bias[j] : b;
+        return b;
+      };
 
       {
         GEMM_T0();
@@ -1024,7 +1044,7 @@ __global__ void __launch_bounds__(320, 1)
           const int n0 = tn * BN + (half * NCH + i) * 32;
           if (n0 < p.N) {
             float v[32];
-            ce_logits(p, r[i & 1], n0, v);
+            ce_logits(p, r[i & 1], n0, bias_of(i), v);
             ce_m = ce_max(v, ce_m);
           }
           if (i + 1 < NCH) tmem_ld_wait();
@@ -1043,7 +1063,7 @@ __global__ void __launch_bounds__(320, 1)
         if constexpr (EPI == 3) {
           if (n0 < p.N) {
             float v[32];
-            ce_logits(p, r[i & 1], n0, v);
+            ce_logits(p, r[i & 1], n0, bias_of(i), v);
             ce_pick(p, row0 + lane, ce_lab - n0, v);
             ce_online(v, ce_m, ce_s);
           }
@@ -1072,10 +1092,10 @@ __global__ void __launch_bounds__(320, 1)
 #pragma unroll
             const float rbv = (EPI < 2 && p.row_bias && row0 + lane < p.M) ? p.row_bias[row0 + lane] : 0.f;
             if constexpr (EPI == 4) {
-              ce_logits(p, r[i & 1], n0, v);
+              ce_logits(p, r[i & 1], n0, bias_of(i), v);
               ce_gradient(ce_m, ce_s, ce_lab < 0 ? CE_ROW_OUT : ce_lab - n0, v);
             } else if constexpr (EPI == 5) {
-              ce_logits(p, r[i & 1], n0, v);
+              ce_logits(p, r[i & 1], n0, bias_of(i), v);
               ce_pick(p, row0 + lane, ce_lab - n0, v);
               ce_exponentials(ce_m, ce_s, v);
             } else {

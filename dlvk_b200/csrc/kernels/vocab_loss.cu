@@ -81,141 +81,186 @@ __global__ void __launch_bounds__(1024) count_kernel(CeRows r, int mean, const f
   }
 }
 
-constexpr int FIN_ROWS = 32, FIN_WARPS = 32;
+constexpr int GROUP = 32;  // rows of one group of the final sums
 
-// A block joins 32 rows (lane = row, the warps share the columns), copies
-// their x rows when asked, and adds up their losses; the block that comes
-// last of all adds the blocks' sums in their order.
-template <typename T>
-__global__ void __launch_bounds__(FIN_WARPS * 32) finish_kernel(CeRows r, CeFinish f, int vec) {
-  pdl_wait();
-  __shared__ float sm_m[FIN_WARPS][FIN_ROWS], sm_s[FIN_WARPS][FIN_ROWS];
-  __shared__ int counted[FIN_ROWS];
-  __shared__ int last;
+// The joined statistics of the rows row0 + lane, in every warp's lanes after
+// a block's barrier: the warps share the columns.
+template <int WARPS>
+__device__ __forceinline__ void join_rows(const CeRows& r, const CeFinish& f, int64_t row, float (*sm_m)[GROUP],
+                                          float (*sm_s)[GROUP], float& m, float& s) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int64_t row0 = (int64_t)blockIdx.x * FIN_ROWS, row = row0 + lane;
-  float m = -INFINITY, s = 0.f;
+  m = -INFINITY;
+  s = 0.f;
   if (row < r.rows) {
-    for (int c = warp; c < f.stat_cols; c += 8 * FIN_WARPS) {
+    for (int c = warp; c < f.stat_cols; c += 8 * WARPS) {
       float2 v[8];
 #pragma unroll
       for (int k = 0; k < 8; ++k)
-        v[k] = c + k * FIN_WARPS < f.stat_cols ? f.stats[(int64_t)(c + k * FIN_WARPS) * r.rows + row]
-                                               : make_float2(-INFINITY, 0.f);
+        v[k] = c + k * WARPS < f.stat_cols ? f.stats[(int64_t)(c + k * WARPS) * r.rows + row]
+                                           : make_float2(-INFINITY, 0.f);
 #pragma unroll
       for (int k = 0; k < 8; ++k) join(m, s, v[k].x, v[k].y);
     }
   }
   sm_m[warp][lane] = m;
   sm_s[warp][lane] = s;
-  if (warp == 1) counted[lane] = row < r.rows && row_label(r, row) >= 0;
   __syncthreads();
-  if (warp == 0) {
-    for (int w = 1; w < FIN_WARPS; ++w) join(m, s, sm_m[w][lane], sm_s[w][lane]);
-    int hit = 0;
-    float l = 0.f;
-    if (row < r.rows) {
-      f.norm[row] = make_float2(m, 1.f / s);
-      if (counted[lane]) {
-        const float z = f.zlabel[row];
-        l = (m - z) + logf(s);
-        hit = z >= m;
-      }
-      f.rows_loss[row] = l;
+  m = sm_m[0][lane];
+  s = sm_s[0][lane];
+  for (int w = 1; w < WARPS; ++w) join(m, s, sm_m[w][lane], sm_s[w][lane]);
+}
+
+// Warp 0 of a group's block: the rows' losses and norms, and the group's sums.
+// True in lane 0 of the block that comes last of all.
+__device__ __forceinline__ bool group_sums(const CeRows& r, const CeFinish& f, int64_t group, int64_t row, bool counted,
+                                           float m, float s) {
+  const int lane = threadIdx.x & 31;
+  int hit = 0;
+  float l = 0.f;
+  if (row < r.rows) {
+    f.norm[row] = make_float2(m, 1.f / s);
+    if (counted) {
+      const float z = f.zlabel[row];
+      l = (m - z) + logf(s);
+      hit = z >= m;
     }
-    double d = l;
+    f.rows_loss[row] = l;
+  }
+  double d = l;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) d += __shfl_xor_sync(0xffffffffu, d, o);
-    const int n = __popc(__ballot_sync(0xffffffffu, counted[lane]));
-    const int h = __popc(__ballot_sync(0xffffffffu, hit));
-    if (lane == 0) {
-      double* p = f.partial + 3 * ((int64_t)f.first_group + blockIdx.x);
-      p[0] = d;
-      p[1] = n;
-      p[2] = h;
-      __threadfence();
-      last = atomicAdd(f.done, 1u) == (unsigned)f.total_groups - 1u;
-    }
-  }
-  if (f.x_clean != nullptr) {
-    const T* x = reinterpret_cast<const T*>(f.x);
-    T* y = reinterpret_cast<T*>(f.x_clean);
-    for (int k = warp; k < FIN_ROWS && row0 + k < r.rows; k += FIN_WARPS) {
-      const T* src = x + (row0 + k) * f.ldx;
-      T* dst = y + (row0 + k) * f.ldc;
-      if (vec) {  // rows of whole 16-byte steps
-        constexpr int V = 16 / (int)sizeof(T);
-        for (int64_t c = lane * V; c < f.width; c += 32 * V)
-          *reinterpret_cast<uint4*>(dst + c) =
-              counted[k] ? *reinterpret_cast<const uint4*>(src + c) : make_uint4(0u, 0u, 0u, 0u);
-      } else {
-        for (int64_t c = lane; c < f.width; c += 32) dst[c] = counted[k] ? src[c] : from_f32<T>(0.f);
-      }
-    }
-  }
-  __syncthreads();
-  if (!last) return;
-  // every block's sums are visible: their writers fenced before they counted
+  for (int o = 16; o > 0; o >>= 1) d += __shfl_xor_sync(0xffffffffu, d, o);
+  const int n = __popc(__ballot_sync(0xffffffffu, counted));
+  const int h = __popc(__ballot_sync(0xffffffffu, hit));
+  if (lane != 0) return false;
+  double* p = f.partial + 3 * ((int64_t)f.first_group + group);
+  p[0] = d;
+  p[1] = n;
+  p[2] = h;
   __threadfence();
-  double d = 0.0, n = 0.0, h = 0.0;
-  for (int b = threadIdx.x; b < f.total_groups; b += FIN_WARPS * 32) {
-    d += __ldcg(f.partial + 3 * (int64_t)b);
-    n += __ldcg(f.partial + 3 * (int64_t)b + 1);
-    h += __ldcg(f.partial + 3 * (int64_t)b + 2);
-  }
-  __shared__ double sm_d[3][FIN_WARPS];
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    d += __shfl_xor_sync(0xffffffffu, d, o);
-    n += __shfl_xor_sync(0xffffffffu, n, o);
-    h += __shfl_xor_sync(0xffffffffu, h, o);
-  }
-  if (lane == 0) {
-    sm_d[0][warp] = d;
-    sm_d[1][warp] = n;
-    sm_d[2][warp] = h;
-  }
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    d = n = h = 0.0;
-    for (int w = 0; w < FIN_WARPS; ++w) {
-      d += sm_d[0][w];
-      n += sm_d[1][w];
-      h += sm_d[2][w];
+  return atomicAdd(f.done, 1u) == (unsigned)f.total_groups - 1u;
+}
+
+// A group's x rows, zeros in those that do not count.
+template <typename T, int WARPS>
+__device__ __forceinline__ void copy_rows(const CeRows& r, const CeFinish& f, int64_t row0, const int* counted,
+                                          int vec) {
+  const int lane = threadIdx.x & 31;
+  const T* x = reinterpret_cast<const T*>(f.x);
+  T* y = reinterpret_cast<T*>(f.x_clean);
+  for (int k = threadIdx.x >> 5; k < GROUP && row0 + k < r.rows; k += WARPS) {
+    const T* src = x + (row0 + k) * f.ldx;
+    T* dst = y + (row0 + k) * f.ldc;
+    if (vec) {  // rows of whole 16-byte steps
+      constexpr int V = 16 / (int)sizeof(T);
+      for (int64_t c = lane * V; c < f.width; c += 32 * V)
+        *reinterpret_cast<uint4*>(dst + c) =
+            counted[k] ? *reinterpret_cast<const uint4*>(src + c) : make_uint4(0u, 0u, 0u, 0u);
+    } else {
+      for (int64_t c = lane; c < f.width; c += 32) dst[c] = counted[k] ? src[c] : from_f32<T>(0.f);
     }
-    const double share = share_of(f.mean, n);
-    *f.loss = (float)(d * share);
-    if (f.set_gscale) *f.gscale = (float)(share * (f.grad_scale ? (double)*f.grad_scale : 1.0));
-    if (f.correct) *f.correct += (unsigned long long)h;
   }
 }
 
-// e -> dz in place.  A block has 32 rows of 2048 classes, a thread 8 classes
-// of each; what a row's 2^-15 e is multiplied by, exp(local maximum - maximum)
-// / sum * g, is made once per row and statistics column.  Bound by HBM: 2
-// bytes in, 2 out per logit.
-constexpr int RS_COLS = 2048, RS_ROWS = 32;
-__global__ void __launch_bounds__(256) rescale_kernel(CeRows r, const float2* __restrict__ stats, int width_shift,
-                                                      const float2* __restrict__ norm, uint16_t* __restrict__ e,
-                                                      int64_t lde) {
+// The last block: adds the groups' sums in their order.
+template <int WARPS>
+__device__ __forceinline__ void total_sums(const CeFinish& f) {
+  __shared__ double sm_d[3][WARPS];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  // every group's sums are visible: their writers fenced before they counted
+  __threadfence();
+  double v[3] = {0.0, 0.0, 0.0};
+  for (int b = threadIdx.x; b < f.total_groups; b += WARPS * 32)
+#pragma unroll
+    for (int k = 0; k < 3; ++k) v[k] += __ldcg(f.partial + 3 * (int64_t)b + k);
+#pragma unroll
+  for (int k = 0; k < 3; ++k) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v[k] += __shfl_xor_sync(0xffffffffu, v[k], o);
+    if (lane == 0) sm_d[k][warp] = v[k];
+  }
+  __syncthreads();
+  if (threadIdx.x != 0) return;
+  for (int k = 0; k < 3; ++k) {
+    v[k] = 0.0;
+    for (int w = 0; w < WARPS; ++w) v[k] += sm_d[k][w];
+  }
+  const double share = share_of(f.mean, v[1]);
+  *f.loss = (float)(v[0] * share);
+  if (f.set_gscale) *f.gscale = (float)(share * (f.grad_scale ? (double)*f.grad_scale : 1.0));
+  if (f.correct) *f.correct += (unsigned long long)v[2];
+}
+
+// A block finishes one group of rows.
+constexpr int FIN_WARPS = 32;
+template <typename T>
+__global__ void __launch_bounds__(FIN_WARPS * 32) finish_kernel(CeRows r, CeFinish f, int vec) {
   pdl_wait();
-  __shared__ float factor[RS_COLS / 64][RS_ROWS];
-  __shared__ int label[RS_ROWS];
+  __shared__ float sm_m[FIN_WARPS][GROUP], sm_s[FIN_WARPS][GROUP];
+  __shared__ int counted[GROUP];
+  __shared__ int last;
+  const int lane = threadIdx.x & 31;
+  const int64_t row0 = (int64_t)blockIdx.x * GROUP, row = row0 + lane;
+  if (threadIdx.x < GROUP) counted[lane] = row < r.rows && row_label(r, row) >= 0;
+  float m, s;
+  join_rows<FIN_WARPS>(r, f, row, sm_m, sm_s, m, s);
+  if (threadIdx.x < 32) {
+    const bool end = group_sums(r, f, blockIdx.x, row, counted[lane] != 0, m, s);
+    if (lane == 0) last = end;
+  }
+  if (f.x_clean != nullptr) copy_rows<T, FIN_WARPS>(r, f, row0, counted, vec);
+  __syncthreads();
+  if (last) total_sums<FIN_WARPS>(f);
+}
+
+// e -> dz in place.  A block has a group of 32 rows and 2048 of their classes,
+// a thread 8 classes of each; what a row's 2^-15 e is multiplied by, exp(local
+// maximum - maximum) / sum, is made once per row and statistics column.  Bound
+// by HBM: 2 bytes in, 2 out per logit.  With JOIN the blocks also join the
+// statistics, each for itself, and the first of a group does the rest of
+// finish_kernel's work: a launch less where the statistics are few.
+constexpr int RS_COLS = 2048, RS_WARPS = 8;
+template <bool JOIN>
+__global__ void __launch_bounds__(RS_WARPS * 32) rescale_kernel(CeRows r, CeFinish f, int vec, int width_shift,
+                                                                uint16_t* __restrict__ e, int64_t lde) {
+  pdl_wait();
+  __shared__ float factor[RS_COLS / 64][GROUP];
+  __shared__ int label[GROUP], counted[GROUP];
+  __shared__ float2 norm[GROUP];
   // backwards: the exponentials that were written last are still in L2
-  const int64_t row0 = (int64_t)(gridDim.y - 1 - blockIdx.y) * RS_ROWS;
+  const int64_t group = gridDim.y - 1 - blockIdx.y, row0 = group * GROUP;
   const int64_t col0 = (int64_t)(gridDim.x - 1 - blockIdx.x) * RS_COLS;
-  const int rows = (int)min((int64_t)RS_ROWS, r.rows - row0);
-  const int64_t stat0 = col0 >> width_shift, stats_all = (r.classes + (1 << width_shift) - 1) >> width_shift;
-  for (int i = threadIdx.x; i < (RS_COLS >> width_shift) * RS_ROWS; i += 256) {
-    const int k = i % RS_ROWS, t = i / RS_ROWS;
-    float v = 0.f;
-    if (k < rows && stat0 + t < stats_all) {
-      const float2 n = norm[row0 + k];
-      v = exp2f((stats[(stat0 + t) * r.rows + row0 + k].x - n.x) * LOG2E) * n.y * (1.f / 32768.f);
+  const int rows = (int)min((int64_t)GROUP, r.rows - row0);
+  const int lane = threadIdx.x & 31;
+  if (threadIdx.x < GROUP) {
+    label[lane] = lane < rows ? row_label(r, row0 + lane) : -1;
+    counted[lane] = label[lane] >= 0;
+    if (!JOIN && lane < rows) norm[lane] = f.norm[row0 + lane];
+  }
+  if constexpr (JOIN) {
+    __shared__ float sm_m[RS_WARPS][GROUP], sm_s[RS_WARPS][GROUP];
+    __shared__ int last;
+    float m, s;
+    join_rows<RS_WARPS>(r, f, row0 + lane, sm_m, sm_s, m, s);
+    if (threadIdx.x < 32) norm[lane] = make_float2(m, 1.f / s);
+    if (col0 == 0) {  // one block of the group, which is uniform in it
+      if (threadIdx.x < 32) {
+        const bool end = group_sums(r, f, group, row0 + lane, counted[lane] != 0, m, s);
+        if (lane == 0) last = end;
+      }
+      copy_rows<__nv_bfloat16, RS_WARPS>(r, f, row0, counted, vec);
+      __syncthreads();
+      if (last) total_sums<RS_WARPS>(f);
     }
+  }
+  __syncthreads();
+  const int64_t stat0 = col0 >> width_shift, stats_all = (r.classes + (1 << width_shift) - 1) >> width_shift;
+  for (int i = threadIdx.x; i < (RS_COLS >> width_shift) * GROUP; i += RS_WARPS * 32) {
+    const int k = i % GROUP, t = i / GROUP;
+    float v = 0.f;
+    if (k < rows && stat0 + t < stats_all)
+      v = exp2f((f.stats[(stat0 + t) * r.rows + row0 + k].x - norm[k].x) * LOG2E) * norm[k].y * (1.f / 32768.f);
     factor[t][k] = v;
   }
-  if (threadIdx.x < RS_ROWS) label[threadIdx.x] = (int)threadIdx.x < rows ? row_label(r, row0 + threadIdx.x) : -1;
   __syncthreads();
   const int64_t col = col0 + threadIdx.x * 8;
   if (col >= r.classes) return;
@@ -230,14 +275,14 @@ __global__ void __launch_bounds__(256) rescale_kernel(CeRows r, const float2* __
     for (int k = 0; k < 8; ++k) {
       if (k0 + k >= rows) break;
       const int lab = label[k0 + k];
-      const float f = mine[k0 + k];
+      const float fac = mine[k0 + k];
       const __half2* h = reinterpret_cast<const __half2*>(&u[k]);
       float v[8];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const float2 t = __half22float2(h[j]);
-        v[2 * j] = t.x * f;
-        v[2 * j + 1] = t.y * f;
+        v[2 * j] = t.x * fac;
+        v[2 * j + 1] = t.y * fac;
       }
       const int64_t at = lab - col;
       if (lab < 0) {  // 0 whatever the row's logits were
@@ -434,13 +479,9 @@ void copy_matrix_t(const void* src, int64_t rs, int64_t cs, void* dst, int64_t l
 
 bool al16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
-template <typename T>
-void finish_t(const CeRows& r, const CeFinish& f, cudaStream_t s) {
-  constexpr int V = 16 / (int)sizeof(T);
-  const int vec = al16(f.x) && al16(f.x_clean) && f.ldx % V == 0 && f.ldc % V == 0 && f.width % V == 0;
-  launch_pdl(finish_kernel<T>, dim3((unsigned)((r.rows + FIN_ROWS - 1) / FIN_ROWS)), dim3(FIN_WARPS * 32), 0, s, r, f,
-             vec);
-  DLVK_POST_LAUNCH();
+// Whether the x rows and their copies are whole 16-byte steps.
+int whole_rows(const CeFinish& f, int step) {
+  return al16(f.x) && al16(f.x_clean) && f.ldx % step == 0 && f.ldc % step == 0 && f.width % step == 0;
 }
 
 }  // namespace
@@ -451,17 +492,22 @@ void ce_count(const CeRows& r, bool mean, const float* grad_scale, float* gscale
 }
 
 void ce_finish(const CeRows& r, const CeFinish& f, DType dt, cudaStream_t s) {
-  if (dt == DType::F32) finish_t<float>(r, f, s);
-  else finish_t<__nv_bfloat16>(r, f, s);
+  const dim3 grid((unsigned)((r.rows + GROUP - 1) / GROUP));
+  if (dt == DType::F32) launch_pdl(finish_kernel<float>, grid, dim3(FIN_WARPS * 32), 0, s, r, f, whole_rows(f, 4));
+  else launch_pdl(finish_kernel<__nv_bfloat16>, grid, dim3(FIN_WARPS * 32), 0, s, r, f, whole_rows(f, 8));
+  DLVK_POST_LAUNCH();
 }
 
-void ce_rescale(const CeRows& r, const float2* stats, int stat_width, const float2* norm, void* e, int64_t lde,
-                cudaStream_t s) {
+bool ce_rescale_joins(int stat_cols) { return stat_cols <= 64; }
+
+void ce_rescale(const CeRows& r, const CeFinish& f, int stat_width, bool join, void* e, int64_t lde, cudaStream_t s) {
   DLVK_CHECK((stat_width == 64 || stat_width == 128) && lde % 8 == 0 && al16(e), "ce_rescale: layout");
-  const dim3 grid((unsigned)((r.classes + RS_COLS - 1) / RS_COLS), (unsigned)((r.rows + RS_ROWS - 1) / RS_ROWS));
+  const dim3 grid((unsigned)((r.classes + RS_COLS - 1) / RS_COLS), (unsigned)((r.rows + GROUP - 1) / GROUP));
   DLVK_CHECK(grid.y <= 65535u, "ce_rescale: more than 2^21 rows in one block of rows");
-  launch_pdl(rescale_kernel, grid, dim3(256), 0, s, r, stats, stat_width == 64 ? 6 : 7, norm,
-             reinterpret_cast<uint16_t*>(e), lde);
+  const int shift = stat_width == 64 ? 6 : 7, vec = whole_rows(f, 8);
+  uint16_t* p = reinterpret_cast<uint16_t*>(e);
+  if (join) launch_pdl(rescale_kernel<true>, grid, dim3(RS_WARPS * 32), 0, s, r, f, vec, shift, p, lde);
+  else launch_pdl(rescale_kernel<false>, grid, dim3(RS_WARPS * 32), 0, s, r, f, vec, shift, p, lde);
   DLVK_POST_LAUNCH();
 }
 
