@@ -351,7 +351,7 @@ LinearCeResult linear_ce_op(const at::Tensor& x, const at::Tensor& w, const at::
       f.ldc = ldx;
       xo = rows_operand(xc, 0, n, E, ldx);
     }
-    const bool join = keep && ce_rescale_joins(f.stat_cols);
+    const bool join = keep && ce_rescale_joins(n, V, f.stat_cols);
     if (!join) ce_finish(r, f, to_dtype(x), stream());
     if (!want_grad) continue;
 

@@ -376,8 +376,8 @@ void ce_finish(const CeRows& r, const CeFinish& f, DType dt, cudaStream_t s);
 // e (ce_exp_tc's, fp16) becomes softmax - onehot in place, bf16; stat_width
 // classes to a statistics column.  After ce_finish, or with `join` instead of
 // it (bf16 x with x_clean), for as few statistics as ce_rescale_joins() says:
-// every 2048 classes of a group read them all again.
-bool ce_rescale_joins(int stat_cols);
+// every 2048 classes of a group read them all again (up to 8 MB, from L2).
+bool ce_rescale_joins(int64_t rows, int64_t classes, int stat_cols);
 void ce_rescale(const CeRows& r, const CeFinish& f, int stat_width, bool join, void* e, int64_t lde, cudaStream_t s);
 // Statistics (one column) and gradient of logits z [rows, classes] fp32, row
 // stride ldz: z becomes (softmax - onehot) * gscale (not when keep_z is off);

@@ -110,6 +110,18 @@ __device__ __forceinline__ void clear_rows(const int* start, float* dtable, int 
   }
 }
 
+// The word of token i < hi, -1 for none: past the end, padding, or an id that
+// no int holds (any other id outside [0, V) falls out of every block's range;
+// negative ones are kept negative).
+template <typename ID>
+__device__ __forceinline__ int word_at(const ID* ids, int i, int hi, int padding) {
+  if (i >= hi) return -1;
+  const ID raw = ids[i];
+  int w = (int)raw;
+  if (sizeof(ID) == 8 && (ID)w != raw) w = -1;
+  return w == padding ? -1 : w;
+}
+
 // Stable sort of the tokens by word in one launch, without a word between
 // blocks.  Block b owns the words [b R, (b + 1) R) and reads all ids twice:
 // once to count its own words (per warp: warp w has the w-th part of the ids)
@@ -146,19 +158,18 @@ __global__ void __launch_bounds__(SORT_THREADS) sort_tokens_kernel(const ID* __r
   const int per = ((n + SORT_THREADS - 1) / SORT_THREADS) * 32;  // ids of a warp, whole groups of 32
   const int lo = min((int64_t)n, (int64_t)warp * per), hi = min((int64_t)n, (int64_t)(warp + 1) * per);
   int* mine = cnt + warp * RP;
+  const unsigned range = (unsigned)(v1 - v0);
   int before = 0;
+  unsigned key[8];  // id - v0 of the warp's last 256 ids: below `range` for this block's words
   for (int base = lo; base < hi; base += 256) {
     int id[8];
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      const int i = base + k * 32 + lane;
-      const int64_t raw = i < hi ? (int64_t)ids[i] : -1;
-      id[k] = (raw >= 0 && raw < V && raw != padding) ? (int)raw : -1;
-    }
+    for (int k = 0; k < 8; ++k) id[k] = word_at(ids, base + k * 32 + lane, hi, padding);
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
-      before += id[k] >= 0 && id[k] < v0;
-      if (id[k] >= v0 && id[k] < v1) atomicAdd(&mine[id[k] - v0], 1);
+      before += (unsigned)id[k] < (unsigned)v0;  // -1 is never below
+      key[k] = (unsigned)id[k] - (unsigned)v0;
+      if (key[k] < range) atomicAdd(&mine[key[k]], 1);
     }
   }
   before = __reduce_add_sync(0xffffffffu, before);
@@ -167,6 +178,7 @@ __global__ void __launch_bounds__(SORT_THREADS) sort_tokens_kernel(const ID* __r
 
   // A warp scans a word's counts over the warps (lane = warp), ...
   static_assert(SORT_WARPS == 32, "lane = warp");
+#pragma unroll 4
   for (int r = warp; r < R; r += SORT_WARPS) {
     const int c = cnt[lane * RP + r];
     int incl = c;
@@ -207,26 +219,24 @@ __global__ void __launch_bounds__(SORT_THREADS) sort_tokens_kernel(const ID* __r
   if (tid < R) first[tid] = at;
   __syncthreads();
 
+  const bool held = hi - lo <= 256;  // one batch: still in registers
   for (int base = lo; base < hi; base += 256) {
-    int id[8];
+    if (!held) {
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      const int i = base + k * 32 + lane;
-      const int64_t raw = i < hi ? (int64_t)ids[i] : -1;
-      id[k] = (raw >= v0 && raw < v1 && raw != padding) ? (int)raw : -1;
+      for (int k = 0; k < 8; ++k) key[k] = (unsigned)word_at(ids, base + k * 32 + lane, hi, padding) - (unsigned)v0;
     }
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
-      const bool hit = id[k] >= 0;
+      const bool hit = key[k] < range;
       if (!__any_sync(0xffffffffu, hit)) continue;
-      const unsigned peers = __match_any_sync(0xffffffffu, id[k]);
+      const unsigned peers = __match_any_sync(0xffffffffu, hit ? key[k] : range);
       if (hit) {
-        const int place = first[id[k] - v0] + mine[id[k] - v0] + __popc(peers & ((1u << lane) - 1u));
+        const int place = first[key[k]] + mine[key[k]] + __popc(peers & ((1u << lane) - 1u));
         order[place] = base + k * 32 + lane;
-        word[place] = id[k];
+        word[place] = v0 + (int)key[k];
       }
       __syncwarp();
-      if (hit && lane == __ffs(peers) - 1) mine[id[k] - v0] += __popc(peers);
+      if (hit && lane == __ffs(peers) - 1) mine[key[k]] += __popc(peers);
       __syncwarp();
     }
   }

@@ -2007,16 +2007,19 @@ int& pair_flag() {
 bool gemm_tc_pair_enabled() { return pair_flag() != 0; }
 
 // ---- softmax cross entropy of a projection -------------------------------------
-// Logits tile width: CTA pairs on 256 x 256 tiles from 256 rows on, single
-// CTAs below, on 128 columns where 256-wide tiles would leave SMs without one.
+// Logits tiles: CTA pairs on 256 x 256 where those fill most of the GPU, else
+// single CTAs on 128 x 128, whose epilogues are a quarter as long, while these
+// are at most two to an SM (256 x 1024 logits of width 256: 10.8 us in pairs,
+// 7.8 so), else 128 x 256.
 namespace {
 struct CeTiling {
   bool pair;
   int bn;
 };
 CeTiling ce_tiling(int64_t M, int64_t N) {
-  if (gemm_tc_pair_enabled() && M >= 256) return {true, 256};
-  return {false, (N + 255) / 256 * ((M + BM - 1) / BM) >= sm_count() ? 256 : 128};
+  const int sms = sm_count();
+  if (gemm_tc_pair_enabled() && M >= 256 && (M + 255) / 256 * ((N + 255) / 256) >= sms * 2 / 5) return {true, 256};
+  return {false, (M + 127) / 128 * ((N + 127) / 128) <= 2 * sms ? 128 : 256};
 }
 
 template <int EPI>

@@ -216,8 +216,8 @@ __global__ void __launch_bounds__(FIN_WARPS * 32) finish_kernel(CeRows r, CeFini
 // a thread 8 classes of each; what a row's 2^-15 e is multiplied by, exp(local
 // maximum - maximum) / sum, is made once per row and statistics column.  Bound
 // by HBM: 2 bytes in, 2 out per logit.  With JOIN the blocks also join the
-// statistics, each for itself, and the first of a group does the rest of
-// finish_kernel's work: a launch less where the statistics are few.
+// statistics, each for itself, and one more block per group does the rest of
+// finish_kernel's work beside them: a launch less where the statistics are few.
 constexpr int RS_COLS = 2048, RS_WARPS = 8;
 template <bool JOIN>
 __global__ void __launch_bounds__(RS_WARPS * 32) rescale_kernel(CeRows r, CeFinish f, int vec, int width_shift,
@@ -228,6 +228,7 @@ __global__ void __launch_bounds__(RS_WARPS * 32) rescale_kernel(CeRows r, CeFini
   __shared__ float2 norm[GROUP];
   // backwards: the exponentials that were written last are still in L2
   const int64_t group = gridDim.y - 1 - blockIdx.y, row0 = group * GROUP;
+  const bool sums = JOIN && blockIdx.x == 0;
   const int64_t col0 = (int64_t)(gridDim.x - 1 - blockIdx.x) * RS_COLS;
   const int rows = (int)min((int64_t)GROUP, r.rows - row0);
   const int lane = threadIdx.x & 31;
@@ -242,7 +243,7 @@ __global__ void __launch_bounds__(RS_WARPS * 32) rescale_kernel(CeRows r, CeFini
     float m, s;
     join_rows<RS_WARPS>(r, f, row0 + lane, sm_m, sm_s, m, s);
     if (threadIdx.x < 32) norm[lane] = make_float2(m, 1.f / s);
-    if (col0 == 0) {  // one block of the group, which is uniform in it
+    if (sums) {
       if (threadIdx.x < 32) {
         const bool end = group_sums(r, f, group, row0 + lane, counted[lane] != 0, m, s);
         if (lane == 0) last = end;
@@ -250,6 +251,7 @@ __global__ void __launch_bounds__(RS_WARPS * 32) rescale_kernel(CeRows r, CeFini
       copy_rows<__nv_bfloat16, RS_WARPS>(r, f, row0, counted, vec);
       __syncthreads();
       if (last) total_sums<RS_WARPS>(f);
+      return;
     }
   }
   __syncthreads();
@@ -498,11 +500,14 @@ void ce_finish(const CeRows& r, const CeFinish& f, DType dt, cudaStream_t s) {
   DLVK_POST_LAUNCH();
 }
 
-bool ce_rescale_joins(int stat_cols) { return stat_cols <= 64; }
+bool ce_rescale_joins(int64_t rows, int64_t classes, int stat_cols) {
+  return stat_cols <= 512 && (classes + RS_COLS - 1) / RS_COLS * rows * stat_cols * 8 <= (8 << 20);
+}
 
 void ce_rescale(const CeRows& r, const CeFinish& f, int stat_width, bool join, void* e, int64_t lde, cudaStream_t s) {
   DLVK_CHECK((stat_width == 64 || stat_width == 128) && lde % 8 == 0 && al16(e), "ce_rescale: layout");
-  const dim3 grid((unsigned)((r.classes + RS_COLS - 1) / RS_COLS), (unsigned)((r.rows + GROUP - 1) / GROUP));
+  const dim3 grid((unsigned)((r.classes + RS_COLS - 1) / RS_COLS + (join ? 1 : 0)),
+                  (unsigned)((r.rows + GROUP - 1) / GROUP));
   DLVK_CHECK(grid.y <= 65535u, "ce_rescale: more than 2^21 rows in one block of rows");
   const int shift = stat_width == 64 ? 6 : 7, vec = whole_rows(f, 8);
   uint16_t* p = reinterpret_cast<uint16_t*>(e);
