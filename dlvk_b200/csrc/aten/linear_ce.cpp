@@ -104,17 +104,33 @@ void product(const Operand& A, const Operand& B, const Out& out, const float* sc
     return;
   }
   TORCH_INTERNAL_ASSERT(scale == nullptr && !a.parts && before == nullptr);
+  if (A.type == at::kFloat && out.type == at::kFloat) {
+    const float *pa = reinterpret_cast<const float*>(A.p), *pb = reinterpret_cast<const float*>(B.p);
+    float* po = reinterpret_cast<float*>(out.p);
+    if (A.rows <= FEW_ROWS && A.cs == 1 && (B.cs == 1 || B.rs == 1) && !accumulate) {
+      const bool turned = B.cs != 1;
+      const int64_t n = few_rows_scratch_floats(A.rows, A.cols, B.cols, turned);
+      const at::Tensor ws = n > 0 ? at::empty({n}, f32) : at::Tensor();
+      few_rows_product(pa, A.rs, pb, turned ? B.cs : B.rs, turned, bias, po, out.ld, A.rows, A.cols, B.cols,
+                       n > 0 ? ws.data_ptr<float>() : nullptr, stream());
+      return;
+    }
+    if (A.cols <= FEW_ROWS && A.rs == 1 && B.cs == 1 && bias == nullptr) {
+      few_rows_outer(pa, A.cs, pb, B.rs, po, out.ld, A.cols, A.rows, B.cols, accumulate, stream());
+      return;
+    }
+  }
   const int64_t n = gemm_simt_workspace_floats(a);
   const at::Tensor ws = n > 0 ? at::empty({n}, f32) : at::Tensor();
   gemm_simt(dtype_of(A.type), odt, a, stream(), n > 0 ? ws.data_ptr<float>() : nullptr, n);
 }
 
-// dst (+)= scale * A B.  Output rows that are no whole 16-byte steps go
-// through a padded copy: the products store whole boxes.
+// dst (+)= scale * A B.  On the tensor cores output rows that are no whole
+// 16-byte steps go through a padded copy: the products store whole boxes.
 void product_into(const Operand& A, const Operand& B, const Out& dst, const float* scale, bool accumulate,
                   const at::TensorOptions& f32) {
   const int64_t step = 16 / (int64_t)c10::elementSize(dst.type);
-  if (dst.ld % step == 0 && reinterpret_cast<uintptr_t>(dst.p) % 16 == 0) {
+  if (A.type == at::kFloat || (dst.ld % step == 0 && reinterpret_cast<uintptr_t>(dst.p) % 16 == 0)) {
     product(A, B, dst, scale, accumulate, f32);
     return;
   }
@@ -205,9 +221,11 @@ LinearCeResult linear_ce_op(const at::Tensor& x, const at::Tensor& w, const at::
   at::Tensor xq, wq;
   bool w_k;  // classes are rows: W^T is what memory holds
   CeProjection c;
-  // fp32 operands of some size run as six products of bf16 parts; a small or
-  // narrow one keeps the SIMT product (it would be mostly padding)
-  const bool parts = !bf && fp32_gemm_mode() != 0 && E >= 16 && V >= 64 && (double)N * E * V >= 4194304.0;
+  // fp32 operands of some size run as six products of bf16 parts; few rows read
+  // the weight as it is, and a small or narrow product, which would be mostly
+  // padding, stays on the SIMT kernel
+  const bool parts = !bf && fp32_gemm_mode() != 0 && N > FEW_ROWS && E >= 16 && V >= 64 &&
+                     (double)N * E * V >= 4194304.0;
   if (parts) {
     const at::Tensor xs = x.stride(1) == 1 ? x : x.contiguous();
     const at::Tensor wr = (w.stride(0) == 1 || w.stride(1) == 1) ? w : w.contiguous();
@@ -228,9 +246,13 @@ LinearCeResult linear_ce_op(const at::Tensor& x, const at::Tensor& w, const at::
     c.ldx = 3 * ep;
     c.ldw = 3 * wp;
   } else {
-    xq = rows_of_16(x);
-    if (xq.stride(1) != 1) xq = rows_of_16(x.contiguous());  // the products read x by rows
-    wq = rows_of_16((w.stride(0) == 1 || w.stride(1) == 1) ? w : w.contiguous());
+    wq = (w.stride(0) == 1 || w.stride(1) == 1) ? w : w.contiguous();
+    xq = x.stride(1) == 1 ? x : x.contiguous();  // the products read x by rows
+    if (bf) {
+      wq = rows_of_16(wq);
+      xq = rows_of_16(xq);
+      if (xq.stride(1) != 1) xq = rows_of_16(xq.contiguous());
+    }
     w_k = wq.stride(1) != 1;
     c.ldx = xq.stride(0);
     c.ldw = w_k ? wq.stride(1) : wq.stride(0);
@@ -259,13 +281,16 @@ LinearCeResult linear_ce_op(const at::Tensor& x, const at::Tensor& w, const at::
   // keeps a 32nd of that on the tensor cores, the statistics
   const int64_t rows = block_of(N, V, !fused ? (64LL << 20) : want_grad ? (128LL << 20) : (1LL << 30));
   const int64_t blocks = ceil_div(N, rows);
-  const int stat_cols = fused ? ce_tc_stat_cols(rows, V) : 1;
+  const auto stat_cols_of = [&](int64_t n) { return fused ? ce_tc_stat_cols(n, V) : ce_memory_stat_cols(n, V); };
+  // a last, smaller block may be cut into more statistics for each of fewer rows
+  int64_t stat_room = rows * stat_cols_of(rows);
+  if (N % rows != 0) stat_room = std::max<int64_t>(stat_room, N % rows * stat_cols_of(N % rows));
   const int groups = (int)ceil_div(N, 32), lab_size = c.labels64 ? 8 : 4;
   // scratch: 8-byte items first (sums, statistics, norms), then floats, then the counter
-  const at::Tensor ws = at::empty({6LL * groups + 2 * rows * stat_cols + 3 * rows + 2}, f32);
+  const at::Tensor ws = at::empty({6LL * groups + 2 * stat_room + 3 * rows + 2}, f32);
   double* partial = reinterpret_cast<double*>(ws.data_ptr<float>());
   float2* stats = reinterpret_cast<float2*>(ws.data_ptr<float>() + 6LL * groups);
-  float2* norm = stats + rows * stat_cols;
+  float2* norm = stats + stat_room;
   float* zlabel = reinterpret_cast<float*>(norm + rows);
   float* gscale = zlabel + rows;
   unsigned* done = reinterpret_cast<unsigned*>(gscale + 1);
@@ -315,7 +340,6 @@ LinearCeResult linear_ce_op(const at::Tensor& x, const at::Tensor& w, const at::
     r.labels = static_cast<const char*>(tc.data_ptr()) + r0 * lab_size;
     Operand xo = parts ? parts_operand(xq, r0, n, E) : rows_operand(xq, r0, n, E, xq.stride(0));
     c.rows = n;
-    TORCH_INTERNAL_ASSERT(!fused || n * ce_tc_stat_cols(n, V) <= rows * stat_cols);
     c.x = reinterpret_cast<const __nv_bfloat16*>(xo.p);
     c.labels = r.labels;
     c.done = blocks == 1 ? done : nullptr;
@@ -329,7 +353,7 @@ LinearCeResult linear_ce_op(const at::Tensor& x, const at::Tensor& w, const at::
     }
     CeFinish f{};
     f.stats = stats;
-    f.stat_cols = fused ? ce_tc_stat_cols(n, V) : 1;
+    f.stat_cols = stat_cols_of(n);
     f.zlabel = zlabel;
     f.rows_loss = out.rows.data_ptr<float>() + r0;
     f.norm = norm;

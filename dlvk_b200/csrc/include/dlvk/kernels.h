@@ -379,11 +379,12 @@ void ce_finish(const CeRows& r, const CeFinish& f, DType dt, cudaStream_t s);
 // every 2048 classes of a group read them all again (up to 8 MB, from L2).
 bool ce_rescale_joins(int64_t rows, int64_t classes, int stat_cols);
 void ce_rescale(const CeRows& r, const CeFinish& f, int stat_width, bool join, void* e, int64_t lde, cudaStream_t s);
-// Statistics (one column) and gradient of logits z [rows, classes] fp32, row
+// Statistics (ce_memory_stat_cols columns) and gradient of logits z [rows, classes] fp32, row
 // stride ldz: z becomes (softmax - onehot) * gscale (not when keep_z is off);
 // dl, when given, that
 // rounded to bf16 (pitch 0, row stride ldz), or softmax - onehot in three
 // parts (pitch of a part, row stride 3 pitch, zeros in the padding).
+int ce_memory_stat_cols(int64_t rows, int64_t classes);
 void ce_memory_stats(const CeRows& r, const float* z, int64_t ldz, float2* stats, float* zlabel, unsigned* done,
                      cudaStream_t s);
 void ce_memory_grad(const CeRows& r, float* z, int64_t ldz, const float2* norm, const float* gscale, __nv_bfloat16* dl,
@@ -397,6 +398,18 @@ void split_parts(const float* src, int64_t ld, int64_t rows, int64_t cols, __nv_
 // columns [cols, pad_to) become 0.  fp32 or bf16 each.
 void copy_matrix(DType dst_dt, DType src_dt, const void* src, int64_t rs, int64_t cs, void* dst, int64_t ldd,
                  int64_t rows, int64_t cols, int64_t pad_to, bool accumulate, cudaStream_t s);
+
+// ---- fp32 products with few rows (few_rows.cu) ---------------------------------
+constexpr int FEW_ROWS = 16;
+// out [rows, cols] = A [rows, K] B (+ bias per column), rows <= FEW_ROWS; B is
+// [K, cols] with contiguous rows ldb apart, or (turned) its transpose is.
+// scratch: few_rows_scratch_floats() floats.
+int64_t few_rows_scratch_floats(int64_t rows, int64_t K, int64_t cols, bool turned);
+void few_rows_product(const float* A, int64_t lda, const float* B, int64_t ldb, bool turned, const float* bias,
+                      float* out, int64_t ldo, int64_t rows, int64_t K, int64_t cols, float* scratch, cudaStream_t s);
+// out [A, cols] (or +=) = P^T Q, P [rows, A], Q [rows, cols], rows <= FEW_ROWS.
+void few_rows_outer(const float* P, int64_t ldp, const float* Q, int64_t ldq, float* out, int64_t ldo, int64_t rows,
+                    int64_t A, int64_t cols, bool accumulate, cudaStream_t s);
 
 // ---- embedding lookup with scale, gradient by sorted tokens (embedding.cu) ---
 // ids: int32 or int64 (ids64).  Rows of table / dy are ld elements apart.

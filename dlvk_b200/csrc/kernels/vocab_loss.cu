@@ -303,20 +303,21 @@ __global__ void __launch_bounds__(RS_WARPS * 32) rescale_kernel(CeRows r, CeFini
   }
 }
 
-// One row of logits per block.
+// A row of logits and a part of its classes per block: enough parts to fill
+// the GPU when rows are few, each a statistics column of its own.
 __global__ void __launch_bounds__(256) memory_stats_kernel(CeRows r, const float* __restrict__ z, int64_t ldz,
-                                                           float2* __restrict__ stats, float* __restrict__ zlabel,
-                                                           unsigned* __restrict__ done) {
+                                                           int64_t per, float2* __restrict__ stats,
+                                                           float* __restrict__ zlabel, unsigned* __restrict__ done) {
   pdl_wait();
   __shared__ float sm_m[8], sm_s[8];
-  if (blockIdx.x == 0 && threadIdx.x == 0 && done != nullptr) *done = 0u;
-  const int64_t row = blockIdx.x;
+  if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0 && done != nullptr) *done = 0u;
+  const int64_t row = blockIdx.x, lo = blockIdx.y * per, hi = min(r.classes, lo + per);
   const float* p = z + row * ldz;
   float m = -INFINITY, s = 0.f;
-  for (int64_t c = threadIdx.x; c < r.classes; c += 4 * 256) {
+  for (int64_t c = lo + threadIdx.x; c < hi; c += 4 * 256) {
     float v[4];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) v[k] = c + k * 256 < r.classes ? p[c + k * 256] : -INFINITY;
+    for (int k = 0; k < 4; ++k) v[k] = c + k * 256 < hi ? p[c + k * 256] : -INFINITY;
     const float mn = fmaxf(fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])), m);
     const float b = mn == -INFINITY ? 0.f : mn;
     s *= exp2f((m - b) * LOG2E);
@@ -336,14 +337,14 @@ __global__ void __launch_bounds__(256) memory_stats_kernel(CeRows r, const float
   __syncthreads();
   if (threadIdx.x == 0) {
     for (int w = 1; w < 8; ++w) join(m, s, sm_m[w], sm_s[w]);
-    stats[row] = make_float2(m, s);
+    stats[blockIdx.y * r.rows + row] = make_float2(m, s);
     const int lab = row_label(r, row);
-    if (lab >= 0) zlabel[row] = p[lab];
+    if (lab >= lo && lab < hi) zlabel[row] = p[lab];
   }
 }
 
-// One row per block, four columns a thread (rows of z and of the parts are
-// whole 128-byte lines).
+// A row and a part of its classes per block, four columns a thread (rows of z
+// and of the parts are whole 128-byte lines).
 __global__ void __launch_bounds__(256) memory_grad_kernel(CeRows r, float* __restrict__ z, int64_t ldz,
                                                           const float2* __restrict__ norm,
                                                           const float* __restrict__ gscale,
@@ -355,7 +356,7 @@ __global__ void __launch_bounds__(256) memory_grad_kernel(CeRows r, float* __res
   const float g = *gscale;
   const float2 n = norm[row];
   const int64_t end = pitch != 0 ? pitch : (r.classes + 3) / 4 * 4;  // the padding becomes 0
-  for (int64_t c = 4 * threadIdx.x; c < end; c += 4 * 256) {
+  for (int64_t c = 4 * ((int64_t)blockIdx.y * 256 + threadIdx.x); c < end; c += 4 * 256 * (int64_t)gridDim.y) {
     float4 u = make_float4(0.f, 0.f, 0.f, 0.f);
     if (lab >= 0 && c < r.classes) u = *reinterpret_cast<const float4*>(p + c);
     float v[4] = {u.x, u.y, u.z, u.w};
@@ -516,16 +517,25 @@ void ce_rescale(const CeRows& r, const CeFinish& f, int stat_width, bool join, v
   DLVK_POST_LAUNCH();
 }
 
+int ce_memory_stat_cols(int64_t rows, int64_t classes) {
+  // about eight blocks to an SM, of at least 2048 classes
+  return (int)std::max<int64_t>(1, std::min<int64_t>((8 * 148 + rows - 1) / rows, classes / 2048));
+}
+
 void ce_memory_stats(const CeRows& r, const float* z, int64_t ldz, float2* stats, float* zlabel, unsigned* done,
                      cudaStream_t s) {
-  launch_pdl(memory_stats_kernel, dim3((unsigned)r.rows), dim3(256), 0, s, r, z, ldz, stats, zlabel, done);
+  const int cols = ce_memory_stat_cols(r.rows, r.classes);
+  const int64_t per = (r.classes + cols - 1) / cols;
+  launch_pdl(memory_stats_kernel, dim3((unsigned)r.rows, (unsigned)cols), dim3(256), 0, s, r, z, ldz, per, stats,
+             zlabel, done);
   DLVK_POST_LAUNCH();
 }
 
 void ce_memory_grad(const CeRows& r, float* z, int64_t ldz, const float2* norm, const float* gscale, __nv_bfloat16* dl,
                     int64_t pitch, bool keep_z, cudaStream_t s) {
   DLVK_CHECK(ldz % 4 == 0 && al16(z) && pitch % 4 == 0 && al16(dl), "ce_memory_grad: layout");
-  launch_pdl(memory_grad_kernel, dim3((unsigned)r.rows), dim3(256), 0, s, r, z, ldz, norm, gscale, dl, pitch,
+  const unsigned parts = (unsigned)ce_memory_stat_cols(r.rows, r.classes);
+  launch_pdl(memory_grad_kernel, dim3((unsigned)r.rows, parts), dim3(256), 0, s, r, z, ldz, norm, gscale, dl, pitch,
              keep_z ? 1 : 0);
   DLVK_POST_LAUNCH();
 }

@@ -163,6 +163,20 @@ def test_loss_alone_in_several_blocks():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("tied", [False, True])
+@pytest.mark.parametrize("n,e,v", [(1, 520, 9001), (3, 1031, 2000), (4, 64, 70001), (8, 96, 11361), (16, 515, 5000),
+                                   (17, 40, 3001), (31, 700, 12000), (32, 1500, 800), (33, 128, 4000),
+                                   (2, 512, 60000), (20, 33, 60001)])
+def test_few_rows_of_fp32(tied, n, e, v):
+    x, w, t, b = operands(n, e, v, torch.float32, "cuda", tied, n % 2 == 0)
+    check(x, w, t, b)
+    W = torch.ones_like(w)
+    K.linear_ce(x, w, t, b, dw_out=W, dw_accumulate=True)
+    ref, lim = exact(x, w, t, b)["dw"]
+    near(W, (1.0 + ref, lim + 2.0 ** -22 * (1 + ref.abs())), "accumulated")
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("rows", [100, 700])
 def test_long_rows_and_wide(rows):
     x, w, t, b = operands(rows, 1032, 20001, torch.bfloat16, "cuda", True, False)
