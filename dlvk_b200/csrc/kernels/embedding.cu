@@ -87,17 +87,16 @@ __global__ void __launch_bounds__(256) lookup_kernel(const ID* __restrict__ ids,
 // which have tokens, [Z1, Z2) and [Z2, V) where they have none, beside the
 // sums and the joins.
 // A warp clears 32 / tx rows at a time, tx lanes to a row (a power of two: as
-// many as a row has 16-byte steps or elements, at most 32).  `start` null: all
+// many as a row has 16-byte steps, at least 4 and at most 32).  `start` null: all
 // rows of [v0, v1), else those without a token.
-__device__ __forceinline__ int lanes_of_row(int D, int vec) {
-  const int steps = vec ? D / 4 : D;
-  int tx = 1;
-  while (tx < 32 && tx < steps) tx *= 2;
+__device__ __forceinline__ int lanes_of_row(int D) {
+  int tx = 4;
+  while (tx < 32 && tx < D / 4) tx *= 2;
   return tx;
 }
 __device__ __forceinline__ void clear_rows(const int* start, float* dtable, int v0, int v1, int D, int vec, int warp,
                                            int warps) {
-  const int lane = threadIdx.x & 31, tx = lanes_of_row(D, vec), per = 32 / tx;
+  const int lane = threadIdx.x & 31, tx = lanes_of_row(D), per = 32 / tx;
   for (int64_t v = v0 + (int64_t)warp * per + lane / tx; v < v1; v += (int64_t)warps * per) {
     if (start != nullptr && start[v] != start[v + 1]) continue;
     float* row = dtable + v * D;
@@ -105,7 +104,12 @@ __device__ __forceinline__ void clear_rows(const int* start, float* dtable, int 
       for (int c = (lane % tx) * 4; c < D; c += tx * 4)
         *reinterpret_cast<float4*>(row + c) = make_float4(0.f, 0.f, 0.f, 0.f);
     } else {
-      for (int c = lane % tx; c < D; c += tx) row[c] = 0.f;
+      // a row that starts anywhere: up to its first 16-byte boundary, 16 bytes at a time, the rest
+      const int head = min(D, (int)((16 - reinterpret_cast<uintptr_t>(row) % 16) / 4) & 3), body = (D - head) / 4 * 4;
+      if (lane % tx < head) row[lane % tx] = 0.f;
+      for (int c = (lane % tx) * 4; c < body; c += tx * 4)
+        *reinterpret_cast<float4*>(row + head + c) = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int c = head + body + lane % tx; c < D; c += tx) row[c] = 0.f;
     }
   }
 }
