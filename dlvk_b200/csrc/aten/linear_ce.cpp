@@ -127,7 +127,8 @@ void product(const Operand& A, const Operand& B, const Out& out, const float* sc
 
 // dst (+)= scale * A B.  On the tensor cores output rows that are no whole
 // 16-byte steps go through a padded copy: the products store whole boxes.
-void product_into(const Operand& A, const Operand& B, const Out& dst, const float* scale, bool accumulate,
+// `room`: B's memory is this function's own and may be read up to its row pitch.
+void product_into(const Operand& A, const Operand& B, const Out& dst, const float* scale, bool accumulate, bool room,
                   const at::TensorOptions& f32) {
   const int64_t step = 16 / (int64_t)c10::elementSize(dst.type);
   if (A.type == at::kFloat || (dst.ld % step == 0 && reinterpret_cast<uintptr_t>(dst.p) % 16 == 0)) {
@@ -136,7 +137,10 @@ void product_into(const Operand& A, const Operand& B, const Out& dst, const floa
   }
   const int64_t ld = round_up(dst.cols, step);
   const at::Tensor c = at::empty({dst.rows, ld}, f32.dtype(dst.type));
-  product(A, B, rows_out(c, 0, dst.rows, dst.cols, ld), scale, false, f32);
+  // where B's rows have room for the padding, its columns too: whole steps all the way
+  Operand b = B;
+  if (room && B.cs == 1 && (B.pitch > 0 ? B.pitch : B.rs) >= ld) b.cols = ld;
+  product(A, b, rows_out(c, 0, dst.rows, b.cols, ld), scale, false, f32);
   copy_matrix(dtype_of(dst.type), dtype_of(dst.type), c.data_ptr(), ld, 1, dst.p, dst.ld, dst.rows, dst.cols, dst.cols,
               accumulate, stream());
 }
@@ -215,7 +219,13 @@ LinearCeResult linear_ce_op(const at::Tensor& x, const at::Tensor& w, const at::
   }
 
   const at::Tensor tc = target.contiguous();
-  const at::Tensor bc = bias.has_value() ? bias->to(at::kFloat).contiguous() : at::Tensor();
+  at::Tensor bc = bias.has_value() ? bias->to(at::kFloat).contiguous() : at::Tensor();
+  if (bc.defined() && !bf && V % 4 != 0) {  // room for whole 16-byte steps
+    const at::Tensor padded = at::empty({round_up(V, 4)}, f32);
+    copy_matrix(DType::F32, DType::F32, bc.data_ptr(), V, 1, padded.data_ptr(), padded.size(0), 1, V, padded.size(0),
+                false, stream());
+    bc = padded;
+  }
   const float* biasp = bc.defined() ? bc.data_ptr<float>() : nullptr;
   const CeRows all{N, V, ignore_index, tc.data_ptr(), tc.scalar_type() == at::kLong};
   at::Tensor xq, wq;
@@ -234,7 +244,7 @@ LinearCeResult linear_ce_op(const at::Tensor& x, const at::Tensor& w, const at::
     const auto b16 = x.options().dtype(at::kBFloat16);
     const int64_t ep = round_up(E, 64), wp = round_up(wm.size(1), 64);
     xq = at::empty({N, 3 * ep}, b16);
-    wq = at::empty({wm.size(0), 3 * wp}, b16);
+    wq = at::empty({w_k ? round_up(V, 4) : E, 3 * wp}, b16);
     // rows that do not count are zeros, whatever they hold (see x_clean below)
     split_parts(xs.data_ptr<float>(), xs.stride(0), N, E, reinterpret_cast<__nv_bfloat16*>(xq.data_ptr()), ep, &all,
                 stream());
@@ -259,7 +269,7 @@ LinearCeResult linear_ce_op(const at::Tensor& x, const at::Tensor& w, const at::
   }
   Operand wo = operand(wq);  // [E, V]
   if (parts) {
-    wo = parts_operand(wq, 0, wq.size(0), w_k ? E : V);
+    wo = parts_operand(wq, 0, w_k ? V : E, w_k ? E : V);
     if (w_k) wo = wo.t();
   }
   c.x = reinterpret_cast<const __nv_bfloat16*>(xq.data_ptr());
@@ -348,7 +358,10 @@ LinearCeResult linear_ce_op(const at::Tensor& x, const at::Tensor& w, const at::
     } else if (fused) {
       ce_stats_tc(c, stream(), device_error_word());
     } else {
-      product(xo, wo, rows_out(z, 0, n, V, ldv), nullptr, false, f32, biasp);
+      // parts: columns up to whole 16-byte steps, which wq and the bias have room for
+      Operand wl = wo;
+      if (parts) wl.cols = round_up(V, 4);
+      product(xo, wl, rows_out(z, 0, n, wl.cols, ldv), nullptr, false, f32, biasp);
       ce_memory_stats(r, z.data_ptr<float>(), ldv, stats, zlabel, c.done, stream());
     }
     CeFinish f{};
@@ -403,10 +416,10 @@ LinearCeResult linear_ce_op(const at::Tensor& x, const at::Tensor& w, const at::
                     db_accumulate || k > 0, stream());
       }
     }
-    product_into(d, wo.t(), rows_out(out.dx, r0, n, E, E), scale, false, f32);
+    product_into(d, wo.t(), rows_out(out.dx, r0, n, E, E), scale, false, !wq.is_same(w), f32);
     const Operand left = dw_k ? d.t() : xo.t(), right = dw_k ? xo : d;
     if (round_last && k == blocks - 1) product(left, right, dw_last, scale, false, f32, nullptr, &dw);
-    else product_into(left, right, dw, scale, dw32.defined() ? k > 0 : (dw_accumulate || k > 0), f32);
+    else product_into(left, right, dw, scale, dw32.defined() ? k > 0 : (dw_accumulate || k > 0), true, f32);
   }
   if (dw32.defined() && !round_last) {
     const at::Tensor src = dw_k ? dw32.t() : dw32, dst = dw_k ? out.dw.t() : out.dw;

@@ -86,30 +86,33 @@ __global__ void __launch_bounds__(256) lookup_kernel(const ID* __restrict__ ids,
 // three launches: [0, Z1) are cleared beside the sort, before it is known
 // which have tokens, [Z1, Z2) and [Z2, V) where they have none, beside the
 // sums and the joins.
-// A warp clears 32 / tx rows at a time, tx lanes to a row (a power of two: as
-// many as a row has 16-byte steps, at least 4 and at most 32).  `start` null: all
-// rows of [v0, v1), else those without a token.
-__device__ __forceinline__ int lanes_of_row(int D) {
-  int tx = 4;
-  while (tx < 32 && tx < D / 4) tx *= 2;
-  return tx;
+// A warp clears `floats` consecutive floats from p on: up to the first line of
+// 128 bytes, 16 bytes a lane (whole lines: at any other offset each store of a
+// warp touches five), the rest.
+__device__ __forceinline__ void clear_span(float* p, int64_t floats) {
+  const int lane = threadIdx.x & 31;
+  const int head = (int)min(floats, (int64_t)((128 - reinterpret_cast<uintptr_t>(p) % 128) / 4 % 32));
+  const int64_t body = (floats - head) / 4 * 4;
+  if (lane < head) p[lane] = 0.f;
+  for (int64_t c = lane * 4; c < body; c += 128)
+    *reinterpret_cast<float4*>(p + head + c) = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (head + body + lane < floats) p[head + body + lane] = 0.f;
 }
-__device__ __forceinline__ void clear_rows(const int* start, float* dtable, int v0, int v1, int D, int vec, int warp,
+// A warp of `warps` takes every warps-th group of consecutive rows (about 4 KB,
+// at most 32) of [v0, v1) and clears the runs of rows without a token in it
+// (`start` null: all).
+__device__ __forceinline__ void clear_rows(const int* start, float* dtable, int v0, int v1, int D, int warp,
                                            int warps) {
-  const int lane = threadIdx.x & 31, tx = lanes_of_row(D), per = 32 / tx;
-  for (int64_t v = v0 + (int64_t)warp * per + lane / tx; v < v1; v += (int64_t)warps * per) {
-    if (start != nullptr && start[v] != start[v + 1]) continue;
-    float* row = dtable + v * D;
-    if (vec) {
-      for (int c = (lane % tx) * 4; c < D; c += tx * 4)
-        *reinterpret_cast<float4*>(row + c) = make_float4(0.f, 0.f, 0.f, 0.f);
-    } else {
-      // a row that starts anywhere: up to its first 16-byte boundary, 16 bytes at a time, the rest
-      const int head = min(D, (int)((16 - reinterpret_cast<uintptr_t>(row) % 16) / 4) & 3), body = (D - head) / 4 * 4;
-      if (lane % tx < head) row[lane % tx] = 0.f;
-      for (int c = (lane % tx) * 4; c < body; c += tx * 4)
-        *reinterpret_cast<float4*>(row + head + c) = make_float4(0.f, 0.f, 0.f, 0.f);
-      for (int c = head + body + lane % tx; c < D; c += tx) row[c] = 0.f;
+  const int lane = threadIdx.x & 31, per = max(1, min(32, 1024 / D));
+  for (int64_t v = v0 + (int64_t)warp * per; v < v1; v += (int64_t)warps * per) {
+    const int rows = (int)min((int64_t)per, v1 - v);
+    const bool empty = lane < rows && (start == nullptr || start[v + lane] == start[v + lane + 1]);
+    unsigned left = __ballot_sync(0xffffffffu, empty);
+    while (left) {
+      const int first = __ffs(left) - 1, run = __ffs(~(left >> first)) - 1;  // run 32: ~0 has no bit, __ffs gives 0
+      const int count = run < 0 ? 32 : run;
+      clear_span(dtable + (v + first) * D, (int64_t)count * D);
+      left = first + count >= 32 ? 0u : left & ~((2u << (first + count - 1)) - 1u);
     }
   }
 }
@@ -141,10 +144,10 @@ __global__ void __launch_bounds__(SORT_THREADS) sort_tokens_kernel(const ID* __r
                                                                    int padding, int* __restrict__ start,
                                                                    int* __restrict__ order, int* __restrict__ word,
                                                                    int sort_blocks, float* __restrict__ dtable,
-                                                                   int clear_to, int D, int vec) {
+                                                                   int clear_to, int D) {
   pdl_wait();
   if ((int)blockIdx.x >= sort_blocks) {
-    clear_rows(nullptr, dtable, 0, clear_to, D, vec, (blockIdx.x - sort_blocks) * SORT_WARPS + (threadIdx.x >> 5),
+    clear_rows(nullptr, dtable, 0, clear_to, D, (blockIdx.x - sort_blocks) * SORT_WARPS + (threadIdx.x >> 5),
                (gridDim.x - sort_blocks) * SORT_WARPS);
     return;
   }
@@ -276,7 +279,7 @@ __global__ void __launch_bounds__(RED_THREADS) sum_chunks_kernel(
     int chunk_blocks, float scale, int accumulate, int clear_from, int clear_to) {
   pdl_wait();
   if ((int)blockIdx.x >= chunk_blocks) {
-    clear_rows(start, dtable, clear_from, clear_to, D, VEC > 1,
+    clear_rows(start, dtable, clear_from, clear_to, D,
                (blockIdx.x - chunk_blocks) * (RED_THREADS / 32) + (threadIdx.x >> 5),
                (gridDim.x - chunk_blocks) * (RED_THREADS / 32));
     return;
@@ -285,6 +288,8 @@ __global__ void __launch_bounds__(RED_THREADS) sum_chunks_kernel(
   const int chunk = blockIdx.x * (RED_THREADS / TX) + threadIdx.x / TX;
   const int total = start[V];
   const int c0 = chunk * C, c1 = min(total, c0 + C);
+  // the words beside the chunk (-1: none): one that goes on there is not finished here
+  const int before = c0 > 0 && c0 < c1 ? word[c0 - 1] : -1, after = c0 < c1 && c1 < total ? word[c1] : -1;
   for (int col = tx * VEC; col < D && c0 < c1; col += TX * VEC) {
     float acc[VEC];
 #pragma unroll
@@ -305,11 +310,10 @@ __global__ void __launch_bounds__(RED_THREADS) sum_chunks_kernel(
 #pragma unroll
           for (int k = 0; k < VEC; ++k) acc[k] += v[u][k];
           if (j + u + 1 == c1 || w[u + 1] != w[u]) {  // the last of its word in this chunk
-            const int first = start[w[u]], end = start[w[u] + 1];
-            if (first >= c0 && end <= c1) {
+            if (w[u] != before && w[u] != after) {
               put_row<VEC>(dtable + (int64_t)w[u] * D + col, acc, scale, accumulate);
             } else {
-              put_row<VEC>(part + ((int64_t)chunk * 2 + (first >= c0)) * D + col, acc, 1.f, false);
+              put_row<VEC>(part + ((int64_t)chunk * 2 + (w[u] != before)) * D + col, acc, 1.f, false);
             }
 #pragma unroll
             for (int k = 0; k < VEC; ++k) acc[k] = 0.f;
@@ -329,7 +333,7 @@ __global__ void __launch_bounds__(RED_THREADS) join_kernel(const int* __restrict
                                                            int accumulate, int join_blocks, int clear_from) {
   pdl_wait();
   if ((int)blockIdx.x >= join_blocks) {
-    clear_rows(start, dtable, clear_from, V, D, VEC > 1,
+    clear_rows(start, dtable, clear_from, V, D,
                (blockIdx.x - join_blocks) * (RED_THREADS / 32) + (threadIdx.x >> 5),
                (gridDim.x - join_blocks) * (RED_THREADS / 32));
     return;
@@ -375,9 +379,10 @@ int across(int D, int vec) {
   return tx;
 }
 
-// Blocks that clear `rows` rows, `warps` at a time.
-int clear_blocks(int64_t rows, int warps) {
-  return (int)std::min<int64_t>((rows + warps - 1) / warps, 148 * 8);
+// Blocks of `warps` warps that clear `rows` rows of D (clear_rows' groups).
+int clear_blocks(int64_t rows, int D, int warps) {
+  const int64_t groups = (rows + std::max(1, std::min(32, 1024 / D)) - 1) / std::max(1, std::min(32, 1024 / D));
+  return (int)std::min<int64_t>((groups + warps - 1) / warps, 148 * 8);
 }
 
 bool al16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
@@ -401,13 +406,13 @@ void sums(const T* dy, int64_t ld, const int* start, const int* order, const int
   const int chunks = (int)((n + C - 1) / C);
   const int tx = across(D, VEC), per = RED_THREADS / tx;
   const int chunk_blocks = (chunks + per - 1) / per;
-  const int zero_blocks = clear_blocks(z2 - z1, RED_THREADS / 32);
+  const int zero_blocks = clear_blocks(z2 - z1, D, RED_THREADS / 32);
   if (chunk_blocks + zero_blocks > 0) {
     launch_pdl(sum_chunks_kernel<T, VEC>, dim3(chunk_blocks + zero_blocks), dim3(RED_THREADS), 0, s, dy, ld, start,
                order, word, dtable, part, V, D, C, tx, chunk_blocks, scale, accumulate ? 1 : 0, z1, z2);
     DLVK_POST_LAUNCH();
   }
-  const int last_blocks = clear_blocks(V - z2, RED_THREADS / 32);
+  const int last_blocks = clear_blocks(V - z2, D, RED_THREADS / 32);
   if (chunks > 1 || last_blocks > 0) {
     constexpr int JV = VEC > 1 ? 4 : 1;
     const int jx = across(D, JV), jper = RED_THREADS / jx;
@@ -478,11 +483,11 @@ void embedding_grad(DType dt, bool ids64, const void* ids, const void* dy, int64
   const bool shared = n >= 4096 && n < V && V * D >= (1 << 23);
   const int z1 = accumulate ? (int)V : (shared ? (int)(V * 35 / 100) : 0);
   const int z2 = accumulate ? (int)V : (shared ? (int)(V - V * 35 / 100) : (int)V);
-  const int sort_clear = accumulate ? 0 : (int)std::min<int64_t>((z1 + SORT_WARPS - 1) / SORT_WARPS, 148);
+  const int sort_clear = accumulate ? 0 : std::min(clear_blocks(z1, D, SORT_WARPS), 148);
   const auto sort = [&](const auto* p) {
     using ID = std::remove_cv_t<std::remove_reference_t<decltype(*p)>>;
     launch_pdl(sort_tokens_kernel<ID>, dim3(blocks + sort_clear), dim3(SORT_THREADS), smem, s, p, (int)n, (int)V, R,
-               pad, start, order, word, blocks, dtable, z1, D, vec ? 1 : 0);
+               pad, start, order, word, blocks, dtable, z1, D);
   };
   if (ids64) sort(reinterpret_cast<const int64_t*>(ids));
   else sort(reinterpret_cast<const int32_t*>(ids));

@@ -5,8 +5,10 @@
 // projections and the batched attention products.
 //
 // Design:
-//  * persistent kernel, one CTA per SM, 320 threads = 10 warps:
-//      warp 0      TMA producer (one lane) over a STAGES-deep smem ring
+//  * persistent kernel, one CTA per SM, 352 threads = 11 warps:
+//      warps 0, 10 TMA producers of A and of B (one lane each) over a STAGES-
+//                  deep smem ring; one thread issuing all of a k-block's loads
+//                  (four for M- and N-major operands) took longer than its MMAs
 //      warp 1      TMEM allocator + MMA issuer (one lane)
 //      warps 2..9  epilogue: tcgen05.ld 32x32b -> alpha/beta/bias/act -> global
 //  * tile 128 x BN x 64 (BN = 256 or 128), UMMA 128 x BN x 16 (kind::f16, bf16
@@ -38,6 +40,7 @@ using namespace sm100;
 
 constexpr int BM = 128;
 constexpr int BK = 64;  // bf16 elements per 128-byte swizzle row
+constexpr int GEMM_THREADS = 352;  // 11 warps
 constexpr int CE_ROW_OUT = -(1 << 30);  // place of the class in a chunk, for a row that does not count
 
 // Operands of the softmax cross entropy epilogues.
@@ -671,7 +674,7 @@ __device__ __forceinline__ void ce_gradient(float m, float f, int at, float* v) 
 // nothing but each row's softmax statistics, EPI = 4 the cross entropy's
 // gradient as bf16 boxes, EPI = 5 statistics and exponentials as fp16 boxes.
 template <int BN, bool PAIR = false, int EPI = 0>
-__global__ void __launch_bounds__(320, 1)
+__global__ void __launch_bounds__(GEMM_THREADS, 1)
     gemm_tc_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                    const __grid_constant__ CUtensorMap tmC, TcParams p) {
   using C = Cfg<BN, PAIR, (EPI >= 4)>;
@@ -738,7 +741,11 @@ __global__ void __launch_bounds__(320, 1)
   }
   GEMM_STAMP(threadIdx.x == 0, 5);
 
-  if (warp == 0) {
+  if (warp == 0 || warp == 10) {
+    // Both wait for a free stage; A's producer announces the bytes of both (a
+    // load of B's that completes before that leaves the count negative, and
+    // the phase open, until it does).
+    const bool do_a = warp == 0;
     if (lane == 0 && PAIR) {
       int stage = 0;
       uint32_t phase = 0;
@@ -765,24 +772,27 @@ __global__ void __launch_bounds__(320, 1)
           uint8_t* sA = smem + stage * C::STAGE_BYTES;
           uint8_t* sB = sA + C::A_BYTES;
           const uint32_t fb = mapa_shared(smem_u32(&full[stage]), 0);  // the leader's full barrier
-          if (rank == 0) mbar_arrive_expect_tx(&full[stage], 2 * C::STAGE_BYTES);
-          if (!a_mn) {
-            tma_load_4d_pair(sA, &tmA, fb, kb * BK + ao, arow, abi, abo);
-          } else {
-#pragma unroll
-            for (int j = 0; j < BM / 64; ++j)
-              tma_load_4d_pair(sA + j * 8192, &tmA, fb, arow + j * 64 + ao, kb * BK, abi, abo);
-          }
-#pragma unroll
-          for (int sub = 0; sub < C::NSUB; ++sub) {
-            uint8_t* sBs = sB + sub * C::SUB_B_BYTES;
-            const int col = bcol + sub * C::MMA_N;
-            if (!b_mn) {
-              tma_load_4d_pair(sBs, &tmB, fb, kb * BK + bo6, col, bi, bo);
+          if (do_a) {
+            if (rank == 0) mbar_arrive_expect_tx(&full[stage], 2 * C::STAGE_BYTES);
+            if (!a_mn) {
+              tma_load_4d_pair(sA, &tmA, fb, kb * BK + ao, arow, abi, abo);
             } else {
 #pragma unroll
-              for (int j = 0; j < C::MMA_N / 128; ++j)
-                tma_load_4d_pair(sBs + j * 8192, &tmB, fb, col + j * 64 + bo6, kb * BK, bi, bo);
+              for (int j = 0; j < BM / 64; ++j)
+                tma_load_4d_pair(sA + j * 8192, &tmA, fb, arow + j * 64 + ao, kb * BK, abi, abo);
+            }
+          } else {
+#pragma unroll
+            for (int sub = 0; sub < C::NSUB; ++sub) {
+              uint8_t* sBs = sB + sub * C::SUB_B_BYTES;
+              const int col = bcol + sub * C::MMA_N;
+              if (!b_mn) {
+                tma_load_4d_pair(sBs, &tmB, fb, kb * BK + bo6, col, bi, bo);
+              } else {
+#pragma unroll
+                for (int j = 0; j < C::MMA_N / 128; ++j)
+                  tma_load_4d_pair(sBs + j * 8192, &tmB, fb, col + j * 64 + bo6, kb * BK, bi, bo);
+              }
             }
           }
           if (++stage == C::STAGES) {
@@ -793,6 +803,7 @@ __global__ void __launch_bounds__(320, 1)
       }
     producer_done_pair:;
     } else if (lane == 0) {
+      const int a_boxes = BM / mn_box, b_boxes = BN / mn_box;
       int stage = 0;
       uint32_t phase = 0;
       WorkIter w;
@@ -814,17 +825,18 @@ __global__ void __launch_bounds__(320, 1)
           }
           uint8_t* sA = smem + stage * C::STAGE_BYTES;
           uint8_t* sB = sA + C::A_BYTES;
-          mbar_arrive_expect_tx(&full[stage], C::STAGE_BYTES);
-          if (!a_mn) {
-            tma_load_4d(sA, &tmA, &full[stage], kb * bke + ao, tm * BM, abi, abo);
-          } else {
-            for (int j = 0; j < BM / mn_box; ++j)
-              tma_load_4d(sA + j * mn_box_bytes, &tmA, &full[stage], tm * BM + j * mn_box + ao, kb * bke, abi, abo);
-          }
-          if (!b_mn) {
+          if (do_a) {
+            mbar_arrive_expect_tx(&full[stage], C::STAGE_BYTES);
+            if (!a_mn) {
+              tma_load_4d(sA, &tmA, &full[stage], kb * bke + ao, tm * BM, abi, abo);
+            } else {
+              for (int j = 0; j < a_boxes; ++j)
+                tma_load_4d(sA + j * mn_box_bytes, &tmA, &full[stage], tm * BM + j * mn_box + ao, kb * bke, abi, abo);
+            }
+          } else if (!b_mn) {
             tma_load_4d(sB, &tmB, &full[stage], kb * bke + bo6, tn * BN, bi, bo);
           } else {
-            for (int j = 0; j < BN / mn_box; ++j)
+            for (int j = 0; j < b_boxes; ++j)
               tma_load_4d(sB + j * mn_box_bytes, &tmB, &full[stage], tn * BN + j * mn_box + bo6, kb * bke, bi, bo);
           }
           if (++stage == C::STAGES) {
@@ -1344,7 +1356,7 @@ void launch_tc_k(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap
   const int tiles = p.tiles_m * p.tiles_n * p.batch * p.splits;
   const int slots = max_ctas > 0 ? max_ctas : sm_count();
   int grid = p.sk ? slots : std::min(tiles, slots);  // stream-K: every CTA takes a share
-  launch_pdl(gemm_tc_kernel<BN, false, EPI>, dim3(grid), dim3(320), C::SMEM, s, ta, tb, tc, p);
+  launch_pdl(gemm_tc_kernel<BN, false, EPI>, dim3(grid), dim3(GEMM_THREADS), C::SMEM, s, ta, tb, tc, p);
   DLVK_POST_LAUNCH();
 }
 template <int BN>
@@ -1372,7 +1384,7 @@ void launch_tc_pair_k(const CUtensorMap& ta, const CUtensorMap& tb, const CUtens
   attr[0].val.clusterDim.z = 1;
   attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[1].val.programmaticStreamSerializationAllowed = pdl_enabled() ? 1 : 0;
-  cfg.blockDim = dim3(320, 1, 1);
+  cfg.blockDim = dim3(GEMM_THREADS, 1, 1);
   cfg.dynamicSmemBytes = C::SMEM;
   cfg.stream = s;
   cfg.attrs = attr;

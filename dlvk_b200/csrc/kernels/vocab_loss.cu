@@ -105,9 +105,23 @@ __device__ __forceinline__ void join_rows(const CeRows& r, const CeFinish& f, in
   sm_m[warp][lane] = m;
   sm_s[warp][lane] = s;
   __syncthreads();
+  // WARPS neighbouring threads join one row's parts
+  const int part = threadIdx.x % WARPS, of = threadIdx.x / WARPS;
+  m = sm_m[part][of];
+  s = sm_s[part][of];
+#pragma unroll
+  for (int o = WARPS / 2; o > 0; o >>= 1) {
+    const float m2 = __shfl_xor_sync(0xffffffffu, m, o), s2 = __shfl_xor_sync(0xffffffffu, s, o);
+    join(m, s, m2, s2);
+  }
+  __syncthreads();
+  if (part == 0) {
+    sm_m[0][of] = m;
+    sm_s[0][of] = s;
+  }
+  __syncthreads();
   m = sm_m[0][lane];
   s = sm_s[0][lane];
-  for (int w = 1; w < WARPS; ++w) join(m, s, sm_m[w][lane], sm_s[w][lane]);
 }
 
 // Warp 0 of a group's block: the rows' losses and norms, and the group's sums.
