@@ -81,11 +81,9 @@ __global__ void __launch_bounds__(256) lookup_kernel(const ID* __restrict__ ids,
 
 // ---------------------------------------------------------------- sort
 // Writing the zero rows is most of the gradient's traffic (32000 words of
-// 1024: 131 MB, of which 8192 tokens touch a tenth), and the sort and the last
-// joining pass are bound by latency.  So the rows are shared out over the
-// three launches: [0, Z1) are cleared beside the sort, before it is known
-// which have tokens, [Z1, Z2) and [Z2, V) where they have none, beside the
-// sums and the joins.
+// 1024: 131 MB, of which 8192 tokens touch a quarter), and the last joining
+// pass is bound by latency.  So [0, Z) are cleared beside the sums and [Z, V)
+// beside the joins.
 // A warp clears `floats` consecutive floats from p on: up to the first line of
 // 128 bytes, 16 bytes a lane (whole lines: at any other offset each store of a
 // warp touches five), the rest.
@@ -99,14 +97,13 @@ __device__ __forceinline__ void clear_span(float* p, int64_t floats) {
   if (head + body + lane < floats) p[head + body + lane] = 0.f;
 }
 // A warp of `warps` takes every warps-th group of consecutive rows (about 4 KB,
-// at most 32) of [v0, v1) and clears the runs of rows without a token in it
-// (`start` null: all).
+// at most 32) of [v0, v1) and clears the runs of rows without a token in it.
 __device__ __forceinline__ void clear_rows(const int* start, float* dtable, int v0, int v1, int D, int warp,
                                            int warps) {
   const int lane = threadIdx.x & 31, per = max(1, min(32, 1024 / D));
   for (int64_t v = v0 + (int64_t)warp * per; v < v1; v += (int64_t)warps * per) {
     const int rows = (int)min((int64_t)per, v1 - v);
-    const bool empty = lane < rows && (start == nullptr || start[v + lane] == start[v + lane + 1]);
+    const bool empty = lane < rows && start[v + lane] == start[v + lane + 1];
     unsigned left = __ballot_sync(0xffffffffu, empty);
     while (left) {
       const int first = __ffs(left) - 1, run = __ffs(~(left >> first)) - 1;  // run 32: ~0 has no bit, __ffs gives 0
@@ -142,29 +139,22 @@ __device__ __forceinline__ int word_at(const ID* ids, int i, int hi, int padding
 template <typename ID>
 __global__ void __launch_bounds__(SORT_THREADS) sort_tokens_kernel(const ID* __restrict__ ids, int n, int V, int R,
                                                                    int padding, int* __restrict__ start,
-                                                                   int* __restrict__ order, int* __restrict__ word,
-                                                                   int sort_blocks, float* __restrict__ dtable,
-                                                                   int clear_to, int D) {
+                                                                   int* __restrict__ order, int* __restrict__ word) {
   pdl_wait();
-  if ((int)blockIdx.x >= sort_blocks) {
-    clear_rows(nullptr, dtable, 0, clear_to, D, (blockIdx.x - sort_blocks) * SORT_WARPS + (threadIdx.x >> 5),
-               (gridDim.x - sort_blocks) * SORT_WARPS);
-    return;
-  }
-  extern __shared__ int cnt[];  // [SORT_WARPS][RP], then [R]: a word's first place
+  extern __shared__ int cnt[];  // [SORT_WARPS][R], then [R]: a word's first place
   __shared__ int warp_part[SORT_WARPS];
   __shared__ int before_sm;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int v0 = blockIdx.x * R, v1 = min(V, v0 + R);
-  const int RP = R | 1;  // odd: the lanes of a warp read one word's counts from as many banks
-  int* first = cnt + SORT_WARPS * RP;
-  for (int i = tid; i < SORT_WARPS * RP; i += SORT_THREADS) cnt[i] = 0;
+  int* first = cnt + SORT_WARPS * R;
+  const int per = (max(n, 1) + SORT_THREADS - 1) / SORT_THREADS * 32;  // ids of a warp, whole groups of 32
+  const int used = (int)(((unsigned)n + per - 1) / per);               // warps that have any
+  for (int i = tid; i < used * R; i += SORT_THREADS) cnt[i] = 0;
   if (tid == 0) before_sm = 0;
   __syncthreads();
 
-  const int per = ((n + SORT_THREADS - 1) / SORT_THREADS) * 32;  // ids of a warp, whole groups of 32
   const int lo = min((int64_t)n, (int64_t)warp * per), hi = min((int64_t)n, (int64_t)(warp + 1) * per);
-  int* mine = cnt + warp * RP;
+  int* mine = cnt + warp * R;
   const unsigned range = (unsigned)(v1 - v0);
   int before = 0;
   unsigned key[8];  // id - v0 of the warp's last 256 ids: below `range` for this block's words
@@ -183,23 +173,23 @@ __global__ void __launch_bounds__(SORT_THREADS) sort_tokens_kernel(const ID* __r
   if (lane == 0 && before) atomicAdd(&before_sm, before);
   __syncthreads();
 
-  // A warp scans a word's counts over the warps (lane = warp), ...
-  static_assert(SORT_WARPS == 32, "lane = warp");
-#pragma unroll 4
-  for (int r = warp; r < R; r += SORT_WARPS) {
-    const int c = cnt[lane * RP + r];
-    int incl = c;
+  // Thread r scans word v0 + r's counts over the warps that have tokens, eight
+  // loads at a time (a warp to a word, with shuffles, took 16.6 us instead of
+  // 6.4 for 200000 words, 6.0 instead of 5.2 for 2048 tokens over 32000), ...
+  int total = 0;
+  if (tid < R) {
+    for (int w0 = 0; w0 < used; w0 += 8) {
+      int c[8];
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int t = __shfl_up_sync(0xffffffffu, incl, o);
-      if (lane >= o) incl += t;
+      for (int u = 0; u < 8; ++u) c[u] = w0 + u < used ? cnt[(w0 + u) * R + tid] : 0;
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        if (w0 + u < used) cnt[(w0 + u) * R + tid] = total;
+        total += c[u];
+      }
     }
-    cnt[lane * RP + r] = incl - c;
-    if (lane == 31) first[r] = incl;
   }
-  __syncthreads();
-  // ... the block the words' totals (thread r: word v0 + r).
-  const int total = tid < R ? first[tid] : 0;
+  // ... the block the words' totals.
   int incl = total;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -276,10 +266,10 @@ template <typename T, int VEC>
 __global__ void __launch_bounds__(RED_THREADS) sum_chunks_kernel(
     const T* __restrict__ dy, int64_t ld, const int* __restrict__ start, const int* __restrict__ order,
     const int* __restrict__ word, float* __restrict__ dtable, float* __restrict__ part, int V, int D, int C, int TX,
-    int chunk_blocks, float scale, int accumulate, int clear_from, int clear_to) {
+    int chunk_blocks, float scale, int accumulate, int clear_to) {
   pdl_wait();
   if ((int)blockIdx.x >= chunk_blocks) {
-    clear_rows(start, dtable, clear_from, clear_to, D,
+    clear_rows(start, dtable, 0, clear_to, D,
                (blockIdx.x - chunk_blocks) * (RED_THREADS / 32) + (threadIdx.x >> 5),
                (gridDim.x - chunk_blocks) * (RED_THREADS / 32));
     return;
@@ -401,24 +391,33 @@ void lookup_t(const ID* ids, const T* table, T* out, int64_t n, int64_t V, int D
 
 template <typename T, int VEC>
 void sums(const T* dy, int64_t ld, const int* start, const int* order, const int* word, float* dtable, float* part,
-          int64_t n, int V, int D, float scale, bool accumulate, int z1, int z2, cudaStream_t s) {
+          int64_t n, int V, int D, float scale, bool accumulate, cudaStream_t s) {
   const int C = chunk_of(n);
   const int chunks = (int)((n + C - 1) / C);
   const int tx = across(D, VEC), per = RED_THREADS / tx;
   const int chunk_blocks = (chunks + per - 1) / per;
-  const int zero_blocks = clear_blocks(z2 - z1, D, RED_THREADS / 32);
+  // The share of the zero rows beside the joins (see clear_rows), none when
+  // adding: 3 in 10 where both are long (8192 tokens x 1024 over 32000 words:
+  // 40.0 -> 37.9 us, 2048 x 1024: 35.9 -> 33.8); for few tokens or a small
+  // table it gains nothing (103 x 624 over 52597: 31.8 and 31.8), and where
+  // most words have tokens there is little to clear.  Clearing a share beside
+  // the sort as well, before it is known which rows have tokens, gained
+  // nothing either (37.9) and cost 2 to 60 us for few tokens.
+  const bool shared = n >= 1024 && n < V && (int64_t)V * D >= (1 << 23);
+  const int z = accumulate ? 0 : (shared ? V - (int)((int64_t)V * 3 / 10) : V);
+  const int zero_blocks = clear_blocks(z, D, RED_THREADS / 32);
   if (chunk_blocks + zero_blocks > 0) {
     launch_pdl(sum_chunks_kernel<T, VEC>, dim3(chunk_blocks + zero_blocks), dim3(RED_THREADS), 0, s, dy, ld, start,
-               order, word, dtable, part, V, D, C, tx, chunk_blocks, scale, accumulate ? 1 : 0, z1, z2);
+               order, word, dtable, part, V, D, C, tx, chunk_blocks, scale, accumulate ? 1 : 0, z);
     DLVK_POST_LAUNCH();
   }
-  const int last_blocks = clear_blocks(V - z2, D, RED_THREADS / 32);
+  const int last_blocks = accumulate ? 0 : clear_blocks(V - z, D, RED_THREADS / 32);
   if (chunks > 1 || last_blocks > 0) {
     constexpr int JV = VEC > 1 ? 4 : 1;
     const int jx = across(D, JV), jper = RED_THREADS / jx;
     const int join_blocks = chunks > 1 ? (chunks + jper - 1) / jper : 0;
     launch_pdl(join_kernel<JV>, dim3(join_blocks + last_blocks), dim3(RED_THREADS), 0, s, start, word, part, dtable, V,
-               D, C, jx, chunks, scale, accumulate ? 1 : 0, join_blocks, z2);
+               D, C, jx, chunks, scale, accumulate ? 1 : 0, join_blocks, z);
     DLVK_POST_LAUNCH();
   }
 }
@@ -458,7 +457,7 @@ void embedding_grad(DType dt, bool ids64, const void* ids, const void* dy, int64
   // words of a block: all 148 SMs, at least 8 each, at most what its counts have room for
   const int R = (int)std::min<int64_t>(SORT_WORDS, std::max<int64_t>(8, (V + 147) / 148));
   const int blocks = (int)((V + R - 1) / R);
-  const auto room = [](int words) { return (SORT_WARPS * (words | 1) + words) * (int)sizeof(int); };
+  const auto room = [](int words) { return (SORT_WARPS + 1) * words * (int)sizeof(int); };
   const size_t smem = (size_t)room(R);
   static bool attr_set[kMaxDevices] = {false};
   const int dev = current_device_slot();
@@ -474,31 +473,21 @@ void embedding_grad(DType dt, bool ids64, const void* ids, const void* dy, int64
   DLVK_CHECK(f32 || dt == DType::BF16, "embedding_grad: dy is fp32 or bf16");
   const int step = f32 ? 4 : 8;
   const bool vec = D % step == 0 && ld % step == 0 && al16(dy) && al16(dtable) && al16(part);
-  // The shares of the zero rows (see clear_rows), none when adding.  Sharing
-  // pays where both the sums and the zeros are long (8192 tokens x 1024 over
-  // 32000 words: 40.7 -> 36.3 us, 4096 x 768 over 50257: 40.4 -> 37.6) and
-  // costs where either is short (2048 x 1024 over 32000: 33.3 -> 35.8, 512 x
-  // 256 over 8000: 14.3 -> 15.8), and nothing is gained by clearing rows
-  // twice where most words have tokens.
-  const bool shared = n >= 4096 && n < V && V * D >= (1 << 23);
-  const int z1 = accumulate ? (int)V : (shared ? (int)(V * 35 / 100) : 0);
-  const int z2 = accumulate ? (int)V : (shared ? (int)(V - V * 35 / 100) : (int)V);
-  const int sort_clear = accumulate ? 0 : std::min(clear_blocks(z1, D, SORT_WARPS), 148);
   const auto sort = [&](const auto* p) {
     using ID = std::remove_cv_t<std::remove_reference_t<decltype(*p)>>;
-    launch_pdl(sort_tokens_kernel<ID>, dim3(blocks + sort_clear), dim3(SORT_THREADS), smem, s, p, (int)n, (int)V, R,
-               pad, start, order, word, blocks, dtable, z1, D);
+    launch_pdl(sort_tokens_kernel<ID>, dim3(blocks), dim3(SORT_THREADS), smem, s, p, (int)n, (int)V, R, pad, start,
+               order, word);
   };
   if (ids64) sort(reinterpret_cast<const int64_t*>(ids));
   else sort(reinterpret_cast<const int32_t*>(ids));
   DLVK_POST_LAUNCH();
   const float* gf = reinterpret_cast<const float*>(dy);
   const __nv_bfloat16* gb = reinterpret_cast<const __nv_bfloat16*>(dy);
-  if (f32 && vec) sums<float, 4>(gf, ld, start, order, word, dtable, part, n, (int)V, D, scale, accumulate, z1, z2, s);
-  else if (f32) sums<float, 1>(gf, ld, start, order, word, dtable, part, n, (int)V, D, scale, accumulate, z1, z2, s);
+  if (f32 && vec) sums<float, 4>(gf, ld, start, order, word, dtable, part, n, (int)V, D, scale, accumulate, s);
+  else if (f32) sums<float, 1>(gf, ld, start, order, word, dtable, part, n, (int)V, D, scale, accumulate, s);
   else if (vec)
-    sums<__nv_bfloat16, 8>(gb, ld, start, order, word, dtable, part, n, (int)V, D, scale, accumulate, z1, z2, s);
-  else sums<__nv_bfloat16, 1>(gb, ld, start, order, word, dtable, part, n, (int)V, D, scale, accumulate, z1, z2, s);
+    sums<__nv_bfloat16, 8>(gb, ld, start, order, word, dtable, part, n, (int)V, D, scale, accumulate, s);
+  else sums<__nv_bfloat16, 1>(gb, ld, start, order, word, dtable, part, n, (int)V, D, scale, accumulate, s);
 }
 
 }  // namespace dlvk
