@@ -85,6 +85,21 @@ void check_disjoint(std::vector<Extent>& ex, const char* what) {
   }
 }
 
+// Whether two indexes may name one element: each stride has to pass all that
+// the smaller ones span.
+bool may_repeat(const at::Tensor& t) {
+  std::vector<std::pair<int64_t, int64_t>> dims;  // stride, size
+  for (int64_t d = 0; d < t.dim(); ++d)
+    if (t.size(d) > 1) dims.emplace_back(t.stride(d), t.size(d));
+  std::sort(dims.begin(), dims.end());
+  int64_t span = 1;
+  for (const auto& [st, sz] : dims) {
+    if (st < span) return true;
+    span += st * (sz - 1);
+  }
+  return false;
+}
+
 bool dense_alike(const at::Tensor& a, const at::Tensor& b) {
   if (a.is_contiguous() && b.is_contiguous()) return true;
   return a.is_non_overlapping_and_dense() && a.strides() == b.strides();
@@ -154,9 +169,8 @@ at::Tensor run(const TensorRefs& grads, const TensorRefs* outs, bool scale, doub
     if (dense_alike(t, o)) dense.push_back({t.data_ptr(), o.data_ptr(), t.numel(), kind});
     else strided.push_back(strided_item(t, o, kind, what));
     if (scale) {
-      for (int64_t d = 0; !o.is_contiguous() && d < o.dim(); ++d)
-        TORCH_CHECK(o.size(d) == 1 || o.stride(d) != 0, "dlvk.", what, ": output ", i,
-                    " repeats its elements (an expanded tensor)");
+      TORCH_CHECK(o.is_contiguous() || !may_repeat(o), "dlvk.", what, ": output ", i,
+                  " repeats its elements, or may (an expanded or unfolded tensor)");
       ex.push_back(extent_of(o, (int64_t)i));
       if (!same) ex.push_back(extent_of(t, (int64_t)i));
     }

@@ -2,6 +2,7 @@
 // gradients from x [rows, width] and W [width, classes] without an array of
 // logits (gemm_tc.cu EPI 3 / 4, vocab_loss.cu).
 #include <ATen/ATen.h>
+#include <ATen/MemoryOverlap.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 
@@ -191,6 +192,12 @@ LinearCeResult linear_ce_op(const at::Tensor& x, const at::Tensor& w, const at::
                     (dw_out->scalar_type() == at::kFloat || (dw_out->scalar_type() == dt && !dw_accumulate)),
                 "dlvk.linear_ce: the weight gradient must be fp32 (or, overwritten, of the weight's type) ", w.sizes(),
                 " with one unit stride on ", dev);
+  if (dw_out.has_value()) {
+    TORCH_CHECK(V == 1 || E == 1 || dw_out->stride(1) + dw_out->stride(0) > (dw_out->stride(1) == 1 ? V : E),
+                "dlvk.linear_ce: the weight gradient repeats its elements, strides ", dw_out->strides());
+    at::assert_no_overlap(*dw_out, w);
+    at::assert_no_overlap(*dw_out, x);
+  }
   if (db_out.has_value())
     TORCH_CHECK(bias.has_value() && db_out->scalar_type() == at::kFloat && db_out->is_contiguous() &&
                     db_out->numel() == V && db_out->device() == dev,

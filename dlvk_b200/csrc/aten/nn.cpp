@@ -2,6 +2,7 @@
 // layer norm, dropout, embedding and the int8 quantised GEMM (declared in
 // dlvk/aten_ops.h).
 #include <ATen/ATen.h>
+#include <ATen/MemoryOverlap.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 
@@ -457,6 +458,7 @@ at::Tensor embedding_grad_op(const at::Tensor& ids, const at::Tensor& dy, int64_
     TORCH_CHECK(dt.scalar_type() == at::kFloat && dt.is_contiguous() && dt.dim() == 2 && dt.size(0) == V &&
                     dt.size(1) == D && dt.device() == dy.device(),
                 "dlvk.embedding_grad: out must be a contiguous fp32 [", V, ", ", D, "] tensor on dy's device");
+    at::assert_no_overlap(dt, dy);
   } else {
     TORCH_CHECK(!accumulate, "dlvk.embedding_grad: accumulate needs out");
     dt = at::empty({V, D}, dy.options().dtype(at::kFloat));

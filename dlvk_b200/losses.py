@@ -116,7 +116,7 @@ class LinearCrossEntropyLoss(LossFunction):
     def forward(self, hidden, weight, target, bias=None, correct=None):
         """The loss alone: a scalar, or with reduction "none" each row's (0 where it does not count)."""
         x, t = self._rows(hidden, target)
-        loss, rows, _, _, _ = K.linear_ce(x, _unwrap(weight), t, bias, self.ignore_index,
+        loss, rows, _, _, _ = K.linear_ce(x, _unwrap(weight), t, _unwrap(bias), self.ignore_index,
                                           self.reduction != "sum", False, correct=correct)
         return rows.reshape(_unwrap(target).shape) if self.reduction == "none" else loss
 
@@ -129,7 +129,7 @@ class LinearCrossEntropyLoss(LossFunction):
         if self.reduction == "none":
             raise ValueError("value_and_grad needs reduction mean or sum")
         x, t = self._rows(hidden, target)
-        loss, _, dx, dw, db = K.linear_ce(x, _unwrap(weight), t, bias, self.ignore_index,
+        loss, _, dx, dw, db = K.linear_ce(x, _unwrap(weight), t, _unwrap(bias), self.ignore_index,
                                           self.reduction == "mean", True, grad_scale)
         return loss, dx.reshape(_unwrap(hidden).shape), dw, db
 

@@ -178,6 +178,13 @@ def test_refusals_on_the_gpu():
 
 
 @pytest.mark.gpu
+def test_refusal_of_an_output_on_the_input():
+    ids, dy = torch.zeros(3, dtype=torch.int32, device="cuda"), torch.zeros(3, 8, device="cuda")
+    with pytest.raises(RuntimeError, match="memory"):
+        nn.embedding_grad(ids, dy, 3, out=dy)
+
+
+@pytest.mark.gpu
 def test_same_bits_every_time():
     ids = zipf(8192, 3000, "cuda")
     dy = torch.randn(8192, 512, device="cuda").bfloat16()

@@ -166,6 +166,22 @@ def test_refusals_of_shared_memory():
 
 
 @pytest.mark.gpu
+def test_refusal_of_an_output_that_repeats_its_elements():
+    t = make("cuda", [(64,)])[0]
+    before = t.clone()
+    clip = dl.GradientClipping.clip_global_norm
+    for bad in (t.unfold(0, 8, 4), t.as_strided((4, 4), (1, 1)), t.as_strided((3, 5), (2, 1))):
+        with pytest.raises(RuntimeError, match="repeats"):
+            clip([bad], 0.1)
+        with pytest.raises(RuntimeError, match="repeats"):
+            clip([torch.ones(bad.shape, device="cuda")], 0.1, out=[bad])
+    assert torch.equal(t, before)
+    # read, they count what they show
+    norm = float(dl.GradientClipping.global_norm([t.unfold(0, 8, 4)]))
+    assert norm == pytest.approx(float(before.unfold(0, 8, 4).double().square().sum().sqrt()), rel=1e-6)
+
+
+@pytest.mark.gpu
 def test_captured_and_repeated_bits():
     ts = make("cuda", [(70001,), (333, 77), (5,)])
     out = [torch.zeros_like(t) for t in ts]

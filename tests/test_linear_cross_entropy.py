@@ -277,6 +277,36 @@ def test_views(device, dtype):
 
 
 @pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("n,e,v", [(4, 16, 40), (24, 64, 3001), (300, 64, 1024)])
+@pytest.mark.parametrize("bias", [False, True])
+def test_logits_near_the_largest_value(device, dtype, n, e, v, bias):
+    """One word's logit is 1.875 * 2^127 = 3.19e38, whose product with log2 e
+    is above fp32: losses 0 and 3.19e38, probabilities 1 and 0."""
+    x, w = torch.zeros(n, e, dtype=dtype, device=device), torch.zeros(e, v, dtype=dtype, device=device)
+    x[:, 0], w[0, 5] = 1.5 * 2.0 ** 64, 1.25 * 2.0 ** 63
+    t = torch.full((n,), 5, dtype=torch.int32, device=device)
+    t[1::2] = 1
+    b = torch.zeros(v, device=device) if bias else None
+    rows = dl.LinearCrossEntropyLoss("none").forward(x, w, t, b)
+    assert bool((rows[0::2] == 0).all()) and bool((rows[1::2] == 1.875 * 2.0 ** 127).all())
+    _, dx, dw, db = dl.LinearCrossEntropyLoss().value_and_grad(x, w, t, b)
+    odd = n // 2
+    want_x, want_w = torch.zeros(n, e, dtype=torch.float64), torch.zeros(e, v, dtype=torch.float64)
+    want_x[1::2, 0] = 1.25 * 2.0 ** 63 / n
+    want_w[0, 5], want_w[0, 1] = odd / n * 1.5 * 2.0 ** 64, -odd / n * 1.5 * 2.0 ** 64
+    # 1 / n and the products: a handful of fp32 roundings, and for dW one for each
+    # of the `odd` equal terms of a sum; one to the type of the output
+    half = 2.0 ** -8 if dtype == torch.bfloat16 else 0.0
+    for got, want, terms in ((dx, want_x, 1), (dw, want_w, odd)):
+        assert bool(((got.double().cpu() - want).abs() <= (half + (terms + 8) * 2.0 ** -24) * want.abs()).all())
+    if bias:
+        want_b = torch.zeros(v, dtype=torch.float64)
+        want_b[5], want_b[1] = odd / n, -odd / n
+        assert bool(((db.double().cpu() - want_b).abs() <= (odd + 8) * 2.0 ** -24 * want_b.abs()).all())
+
+
+@pytest.mark.parametrize("device", DEVICES)
 def test_no_rows(device):
     x, w, t, b = operands(3, 16, 70, torch.bfloat16, device, bias=True)
     loss, dx, dw, db = dl.LinearCrossEntropyLoss().value_and_grad(x[:0], w, t[:0], b)
@@ -364,6 +394,39 @@ def test_refusals_on_the_gpu():
         K.linear_ce(x, w, t, db_out=torch.zeros(70, device="cuda"))
     with pytest.raises(RuntimeError, match="grad_scale"):
         K.linear_ce(x, w, t, grad_scale=torch.ones(2, device="cuda"))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M,N,K_", [(160, 512, 256), (33, 256, 64), (1056, 1024, 512), (8224, 1024, 256)])
+def test_column_sums_of_a_product_with_part_tiles(M, N, K_):
+    """The products' column sums where the last tile has whole 32-row chunks
+    past M: those write nowhere, and the sums are those of the rows there are."""
+    C = K.N()
+    g = torch.Generator(device="cuda").manual_seed(3)
+    a = torch.randn(M, K_, device="cuda", generator=g).bfloat16()
+    b = (torch.randn(K_, N, device="cuda", generator=g) * 0.1).bfloat16()
+    cs = torch.full((N,), 7.0, device="cuda")
+    out = C.gemm(a, b, out_dtype=torch.float32, colsum_out=cs)
+    want = out.double().sum(0)
+    # fp32 sums of M terms in whatever order: at most M 2^-24 of the sum of magnitudes
+    lim = M * 2.0 ** -24 * out.double().abs().sum(0)
+    assert bool(((cs.double() - want).abs() <= lim).all())
+    assert int(C.read_device_error(True)) == 0
+
+
+@pytest.mark.gpu
+def test_refusals_of_a_weight_gradient_on_other_memory():
+    x, w, t, _ = operands(6, 16, 70, torch.float32, "cuda")
+    wide = torch.zeros(16, 70, device="cuda")
+    for bad in (wide[:1].expand(16, 70), wide.as_strided((16, 70), (69, 1)), wide.as_strided((16, 70), (1, 15))):
+        with pytest.raises(RuntimeError, match="repeats"):
+            K.linear_ce(x, w, t, dw_out=bad)
+    with pytest.raises(RuntimeError, match="memory"):
+        K.linear_ce(x, w, t, dw_out=w)
+    both = torch.zeros(6 * 16 + 16 * 70, device="cuda")
+    h = both[:96].view(6, 16)
+    with pytest.raises(RuntimeError, match="memory"):
+        K.linear_ce(h, w, t, dw_out=both[80:80 + 1120].view(16, 70))
 
 
 def _token_model(device, dtype, vocab=300, hidden_relu=False, bias=False):
