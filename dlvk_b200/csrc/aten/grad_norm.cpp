@@ -58,30 +58,34 @@ Extent extent_of(const at::Tensor& t, int64_t index) {
 bool share_bytes(const Extent& a, const Extent& b) {
   if (a.hi <= b.lo || b.hi <= a.lo) return false;
   if (a.pitch == 0 || a.pitch != b.pitch) return true;
-  const int64_t p = a.pitch, d = (int64_t)((b.lo - a.lo) % (uintptr_t)p);  // a.lo <= b.lo (sorted)
-  return d < a.row || d + b.row > p;
+  const Extent &f = a.lo <= b.lo ? a : b, &l = a.lo <= b.lo ? b : a;
+  const int64_t p = a.pitch, d = (int64_t)((l.lo - f.lo) % (uintptr_t)p);
+  return d < f.row || d + l.row > p;
 }
 
-// Each written tensor must share no byte with another tensor of the call
-// (its own input apart).
-void check_disjoint(std::vector<Extent>& ex, const char* what) {
+// Each written tensor must share no byte with another one of the call, written
+// or (`read`: the inputs that are not their own outputs) read.
+void check_disjoint(std::vector<Extent>& written, const std::vector<Extent>& read, const char* what) {
+  if (written.empty()) return;
+  const auto apart = [&](const Extent& a, const Extent& b) {
+    TORCH_CHECK(!share_bytes(a, b), "dlvk.", what, ": tensors ", std::min(a.index, b.index), " and ",
+                std::max(a.index, b.index), " of the call share memory, which is written");
+  };
   const auto before = [](const Extent& a, const Extent& b) { return a.lo < b.lo; };
-  if (!std::is_sorted(ex.begin(), ex.end(), before)) std::sort(ex.begin(), ex.end(), before);
-  // usually nothing overlaps even as ranges
+  if (!std::is_sorted(written.begin(), written.end(), before)) std::sort(written.begin(), written.end(), before);
+  std::vector<uintptr_t> reach(written.size());  // the highest end so far
   uintptr_t end = 0;
-  bool apart = true;
-  for (const Extent& e : ex) {
-    apart = apart && e.lo >= end;
-    end = std::max(end, e.hi);
+  for (size_t i = 0; i < written.size(); ++i) {
+    // usually nothing overlaps even as ranges
+    for (size_t k = i; k > 0 && reach[k - 1] > written[i].lo; --k) apart(written[k - 1], written[i]);
+    end = std::max(end, written[i].hi);
+    reach[i] = end;
   }
-  if (apart) return;
-  std::vector<Extent> open;
-  for (const Extent& e : ex) {
-    open.erase(std::remove_if(open.begin(), open.end(), [&](const Extent& o) { return o.hi <= e.lo; }), open.end());
-    for (const Extent& o : open)
-      TORCH_CHECK(!share_bytes(o, e), "dlvk.", what, ": tensors ", std::min(o.index, e.index), " and ",
-                  std::max(o.index, e.index), " of the call share memory, which is written");
-    open.push_back(e);
+  for (const Extent& r : read) {
+    if (r.hi <= written[0].lo || r.lo >= end) continue;
+    size_t k = std::lower_bound(written.begin(), written.end(), r.hi,
+                                [](const Extent& w, uintptr_t v) { return w.lo < v; }) - written.begin();
+    for (; k > 0 && reach[k - 1] > r.lo; --k) apart(written[k - 1], r);
   }
 }
 
@@ -144,9 +148,10 @@ at::Tensor run(const TensorRefs& grads, const TensorRefs* outs, bool scale, doub
   const at::Device dev = grads[0]->device();
   std::vector<DenseItem> dense;
   std::vector<StridedItem> strided;
-  std::vector<Extent> ex;
+  std::vector<Extent> written, read;
   dense.reserve(grads.size());
-  if (scale) ex.reserve(grads.size() * (outs ? 2 : 1));
+  if (scale) written.reserve(grads.size());
+  if (scale && outs) read.reserve(grads.size());
   for (size_t i = 0; i < grads.size(); ++i) {
     const at::Tensor& t = *grads[i];
     const at::Tensor& o = outs ? *(*outs)[i] : t;
@@ -171,11 +176,11 @@ at::Tensor run(const TensorRefs& grads, const TensorRefs* outs, bool scale, doub
     if (scale) {
       TORCH_CHECK(o.is_contiguous() || !may_repeat(o), "dlvk.", what, ": output ", i,
                   " repeats its elements, or may (an expanded or unfolded tensor)");
-      ex.push_back(extent_of(o, (int64_t)i));
-      if (!same) ex.push_back(extent_of(t, (int64_t)i));
+      written.push_back(extent_of(o, (int64_t)i));
+      if (!same) read.push_back(extent_of(t, (int64_t)i));
     }
   }
-  if (scale) check_disjoint(ex, what);
+  if (scale) check_disjoint(written, read, what);
   c10::cuda::CUDAGuard g(dev);
   const PdlScope pdl;
   at::AutoDispatchBelowADInplaceOrView below;

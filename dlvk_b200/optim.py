@@ -333,7 +333,7 @@ class RMSprop(Optimizer):
 
 def _tensor_list(tensors: Iterable) -> List[torch.Tensor]:
     tensors = list(tensors)
-    if all(map(torch.is_tensor, tensors)):
+    if set(map(type, tensors)) <= {torch.Tensor, torch.nn.Parameter}:  # one pass of few instructions
         return tensors
     from .tensor import Tensor as FacadeTensor
 

@@ -165,6 +165,37 @@ def test_refusals_of_shared_memory():
     assert torch.equal(t, before)
 
 
+@pytest.mark.parametrize("device", DEVICES)
+def test_inputs_that_share_memory_are_only_read(device):
+    g = make(device, [(12, 40)])[0]
+    grads = [g, g[:, 8:24], g, g[3:5]]
+    out = [torch.empty(t.shape, device=device) for t in grads]
+    want = torch.cat([t.double().reshape(-1) for t in grads]).norm()
+    norm = dl.GradientClipping.clip_global_norm(grads, 0.5, out=out)
+    assert float(norm) == pytest.approx(float(want), rel=1e-6)
+    for t, o in zip(grads, out):  # two fp32 roundings: the factor's and the product's
+        assert bool(((o.double() - t.double() * 0.5 / (want + 1e-6)).abs() <= 3 * 2.0 ** -24 * t.double().abs()).all())
+
+
+@pytest.mark.gpu
+def test_refusal_of_an_output_on_another_input():
+    flat = torch.zeros(4096, device="cuda")
+    clip = dl.GradientClipping.clip_global_norm
+    outs = [flat[i * 512:(i + 1) * 512] for i in range(8)]
+    grads = [torch.ones(512, device="cuda") for _ in range(8)]
+    clip(grads, 1.0, out=outs)
+    clip(grads, 1.0, out=outs[::-1])
+    for k, bad in ((0, flat[512:1024]), (3, flat[100:612]), (7, flat[3583:4095]), (5, flat[2600:3112])):
+        with pytest.raises(RuntimeError, match="share memory"):
+            clip(grads[:k] + [bad] + grads[k + 1:], 1.0, out=outs)
+    m = torch.zeros(6, 40, device="cuda")
+    cols = [m[:, 8 * i:8 * i + 8] for i in range(4)]
+    clip([torch.ones(6, 8, device="cuda") for _ in cols], 1.0, out=cols)
+    clip(cols + [m[:, 32:].clone()], 1.0, out=[torch.zeros(6, 8, device="cuda") for _ in cols] + [m[:, 32:]])
+    with pytest.raises(RuntimeError, match="share memory"):
+        clip(cols + [m[:, 30:38]], 1.0, out=[torch.zeros(6, 8, device="cuda") for _ in cols] + [m[:, 32:]])
+
+
 @pytest.mark.gpu
 def test_refusal_of_an_output_that_repeats_its_elements():
     t = make("cuda", [(64,)])[0]
