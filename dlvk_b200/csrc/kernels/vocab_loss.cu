@@ -166,9 +166,17 @@ __device__ __forceinline__ void copy_rows(const CeRows& r, const CeFinish& f, in
     T* dst = y + (row0 + k) * f.ldc;
     if (vec) {  // rows of whole 16-byte steps
       constexpr int V = 16 / (int)sizeof(T);
-      for (int64_t c = lane * V; c < f.width; c += 32 * V)
-        *reinterpret_cast<uint4*>(dst + c) =
-            counted[k] ? *reinterpret_cast<const uint4*>(src + c) : make_uint4(0u, 0u, 0u, 0u);
+      const bool keep = counted[k] != 0;
+      for (int64_t c = lane * V; c < f.width; c += 4 * 32 * V) {
+        uint4 u[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          u[q] = keep && c + q * 32 * V < f.width ? *reinterpret_cast<const uint4*>(src + c + q * 32 * V)
+                                                  : make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          if (c + q * 32 * V < f.width) *reinterpret_cast<uint4*>(dst + c + q * 32 * V) = u[q];
+      }
     } else {
       for (int64_t c = lane; c < f.width; c += 32) dst[c] = counted[k] ? src[c] : from_f32<T>(0.f);
     }
@@ -204,8 +212,8 @@ __device__ __forceinline__ void total_sums(const CeFinish& f) {
   if (f.correct) *f.correct += (unsigned long long)v[2];
 }
 
-// A block finishes one group of rows.
-constexpr int FIN_WARPS = 32;
+// A block finishes one group of rows; another copies the group's x beside it.
+constexpr int FIN_WARPS = 16;
 template <typename T>
 __global__ void __launch_bounds__(FIN_WARPS * 32) finish_kernel(CeRows r, CeFinish f, int vec) {
   pdl_wait();
@@ -215,13 +223,17 @@ __global__ void __launch_bounds__(FIN_WARPS * 32) finish_kernel(CeRows r, CeFini
   const int lane = threadIdx.x & 31;
   const int64_t row0 = (int64_t)blockIdx.x * GROUP, row = row0 + lane;
   if (threadIdx.x < GROUP) counted[lane] = row < r.rows && row_label(r, row) >= 0;
+  if (blockIdx.y != 0) {
+    __syncthreads();
+    copy_rows<T, FIN_WARPS>(r, f, row0, counted, vec);
+    return;
+  }
   float m, s;
   join_rows<FIN_WARPS>(r, f, row, sm_m, sm_s, m, s);
   if (threadIdx.x < 32) {
     const bool end = group_sums(r, f, blockIdx.x, row, counted[lane] != 0, m, s);
     if (lane == 0) last = end;
   }
-  if (f.x_clean != nullptr) copy_rows<T, FIN_WARPS>(r, f, row0, counted, vec);
   __syncthreads();
   if (last) total_sums<FIN_WARPS>(f);
 }
@@ -509,7 +521,7 @@ void ce_count(const CeRows& r, bool mean, const float* grad_scale, float* gscale
 }
 
 void ce_finish(const CeRows& r, const CeFinish& f, DType dt, cudaStream_t s) {
-  const dim3 grid((unsigned)((r.rows + GROUP - 1) / GROUP));
+  const dim3 grid((unsigned)((r.rows + GROUP - 1) / GROUP), f.x_clean != nullptr ? 2 : 1);
   if (dt == DType::F32) launch_pdl(finish_kernel<float>, grid, dim3(FIN_WARPS * 32), 0, s, r, f, whole_rows(f, 4));
   else launch_pdl(finish_kernel<__nv_bfloat16>, grid, dim3(FIN_WARPS * 32), 0, s, r, f, whole_rows(f, 8));
   DLVK_POST_LAUNCH();
