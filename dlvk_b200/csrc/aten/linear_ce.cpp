@@ -298,7 +298,7 @@ LinearCeResult linear_ce_op(const at::Tensor& x, const at::Tensor& w, const at::
   // keeps a 32nd of that on the tensor cores, the statistics
   const int64_t rows = block_of(N, V, !fused ? (64LL << 20) : want_grad ? (128LL << 20) : (1LL << 30));
   const int64_t blocks = ceil_div(N, rows);
-  const auto stat_cols_of = [&](int64_t n) { return fused ? ce_tc_stat_cols(n, V) : ce_memory_stat_cols(n, V); };
+  const auto stat_cols_of = [&](int64_t n) { return fused ? ce_tc_stat_cols(n, V, parts) : ce_memory_stat_cols(n, V); };
   // a last, smaller block may be cut into more statistics for each of fewer rows
   int64_t stat_room = rows * stat_cols_of(rows);
   if (N % rows != 0) stat_room = std::max<int64_t>(stat_room, N % rows * stat_cols_of(N % rows));

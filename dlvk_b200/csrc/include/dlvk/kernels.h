@@ -329,7 +329,7 @@ struct CeProjection {
 bool ce_tc_supported(const CeProjection& c);
 // The statistics have one column per ce_tc_stat_width() classes.
 int ce_tc_stat_width(int64_t rows, int64_t classes);
-int ce_tc_stat_cols(int64_t rows, int64_t classes);
+int ce_tc_stat_cols(int64_t rows, int64_t classes, bool parts);
 void ce_stats_tc(const CeProjection& c, cudaStream_t s, uint32_t* err);
 // The statistics, and e = 2^15 exp(z - the maximum of its statistics column),
 // fp16 [rows, classes], row stride lde.

@@ -95,35 +95,39 @@ struct TcParams {
   int64_t ldbits;          // 32-bit words per bitmask row
   CeEpilogue ce;           // softmax cross entropy epilogues (EPI 3 to 5)
   const float* alpha_ptr;  // device factor of alpha, or null
-  int products;            // 1; 6: fp32 operands in three bf16 parts each
+  int parts;               // fp32 operands in three bf16 parts each (PARTS)
   int a_pitch, b_pitch;    // distance of an operand's parts along its contiguous dimension
 };
-
-// The six products of operands in three parts (x = x0 + x1 + x2, 8 bits
-// each) that reach above 2^-24 of the whole, small ones first: x2 w0, x0 w2,
-// x1 w1, x1 w0, x0 w1, x0 w0.  Four bits per product.
-__device__ __forceinline__ int part_a(int i) { return (0x001102 >> (4 * i)) & 15; }
-__device__ __forceinline__ int part_b(int i) { return (0x010120 >> (4 * i)) & 15; }
 
 // PAIR: a 2-CTA cluster shares one 256 x BN tile (tcgen05 cta_group::2);
 // each CTA stages its 128 rows of A and its BN/2 columns of B.
 // EXTRA: one stage fewer, whose room is a second TMA-store box per epilogue
 // warp (EPI 5 fills two boxes a tile between its other work).
-template <int BN, bool PAIR = false, bool EXTRA = false>
+// PARTS: fp32 operands in three bf16 parts each, x = x0 + x1 + x2.  The six
+// products that reach above 2^-24 of the whole are made of one k-block's parts,
+// three stages of the ring: half the loads of a stage per product, which L2
+// could not keep up with (128 x 128 tiles of 913 x 1982 x 1040: 42.9 -> 22.6
+// us).  Parts 2 and 1 are given back before x0 w0, the last product, which has an
+// accumulator of its own: each addition to it loses up to 2^-24 of it, and with
+// the other five there would be six times as many.  The epilogue adds the two.
+template <int BN, bool PAIR = false, bool EXTRA = false, bool PARTS = false>
 // BN = 512 (PAIR only): the tile is two N = 256 MMAs per k-step; each CTA
 // stages two 128-column B sub-blocks, and the 512 accumulator columns fill
 // TMEM, so there is one accumulator buffer instead of two.
 struct Cfg {
   static constexpr int A_BYTES = BM * BK * 2;
   static constexpr int B_BYTES = (PAIR ? BN / 2 : BN) * BK * 2;
+  static constexpr int NP = PARTS ? 3 : 1;                 // stages of a k-block
   static constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
   static constexpr int STAGES = (PAIR ? (BN == 512 ? 4 : 6) : ((BN == 256) ? 4 : 6)) - (EXTRA ? 1 : 0);
-  static constexpr int ACCS = 2 * BN <= 512 ? 2 : 1;      // TMEM accumulator buffers
-  static constexpr int TMEM_COLS = ACCS * BN;
+  static constexpr int ACC_COLS = PARTS ? 2 * BN : BN;     // columns of one accumulator buffer
+  static constexpr int ACCS = 2 * ACC_COLS <= 512 ? 2 : 1; // TMEM accumulator buffers
+  static constexpr int TMEM_COLS = ACCS * ACC_COLS;
   static constexpr int MMA_N = BN > 256 ? 256 : BN;        // N of one tcgen05.mma
   static constexpr int NSUB = BN / MMA_N;                  // MMAs per k-step
   static constexpr int SUB_B_BYTES = B_BYTES / NSUB;       // B bytes per sub-block
   static_assert(!(BN == 512) || PAIR, "the 512-column tile is a CTA-pair tile");
+  static_assert(!PARTS || STAGES == 6, "tiles of operands in parts: 256 wide in pairs, 128 alone");
   // per-warp 32x33 fp32 staging; also holds the TMA-store boxes (8 x 4 KB
   // from the next 1024-byte boundary)
   static constexpr int BOXES = EXTRA ? 2 : 1;  // boxes of a warp
@@ -674,11 +678,42 @@ __device__ __forceinline__ void ce_gradient(float m, float f, int at, float* v) 
 // alpha, bias and activation only.  EPI = 0 has every path.  EPI = 3 stores
 // nothing but each row's softmax statistics, EPI = 4 the cross entropy's
 // gradient as bf16 boxes, EPI = 5 statistics and exponentials as fp16 boxes.
-template <int BN, bool PAIR = false, int EPI = 0>
+// PARTS: waits for a k-block's three stages (parts 2, 1, 0) from `stage` on and
+// issues its products, five into column `cols` of the accumulators from d on and
+// x0 w0 into d; every stage is committed as soon as nothing more reads it.
+// False when a wait ran out.
+template <int STEPS, typename Mma, typename Commit>
+__device__ __forceinline__ bool six_products(uint64_t* full, uint32_t phase, uint32_t* err, int stage,
+                                             uint32_t stage_units, uint64_t a0, uint64_t b0, uint32_t a_step,
+                                             uint32_t b_step, uint32_t d, uint32_t cols, bool more, Mma mma,
+                                             Commit commit) {
+  const auto product = [&](int x, int w, uint32_t to, bool add) {
+#pragma unroll
+    for (int k = 0; k < STEPS; ++k)
+      mma(to, desc_at(a0, (stage + 2 - x) * stage_units + k * a_step),
+          desc_at(b0, (stage + 2 - w) * stage_units + k * b_step), (add || k != 0) ? 1u : 0u);
+  };
+  if (!mbar_wait(&full[stage], phase, err) || !mbar_wait(&full[stage + 1], phase, err)) return false;
+  tc_fence_after();
+  product(1, 1, d + cols, more);
+  if (!mbar_wait(&full[stage + 2], phase, err)) return false;
+  tc_fence_after();
+  product(2, 0, d + cols, true);
+  product(0, 2, d + cols, true);
+  commit(stage);
+  product(1, 0, d + cols, true);
+  product(0, 1, d + cols, true);
+  commit(stage + 1);
+  product(0, 0, d, more);
+  commit(stage + 2);
+  return true;
+}
+
+template <int BN, bool PAIR = false, int EPI = 0, bool PARTS = false>
 __global__ void __launch_bounds__(GEMM_THREADS, 1)
     gemm_tc_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                    const __grid_constant__ CUtensorMap tmC, TcParams p) {
-  using C = Cfg<BN, PAIR, (EPI >= 4)>;
+  using C = Cfg<BN, PAIR, (EPI >= 4), PARTS>;
   GEMM_STAMP(threadIdx.x == 0, 4);
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -760,11 +795,9 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1)
         const int arow = tm * TILE_M + (int)rank * BM;
         // sub-block j of this CTA: columns tn*BN + j*MMA_N + rank*MMA_N/2 + [0, MMA_N/2)
         const int bcol = tn * BN + (int)rank * (C::MMA_N / 2);
-        const int run = kb1 - kb0, steps = run * p.products;
-        const bool a_mn = p.a_mn != 0, b_mn = p.b_mn != 0, parts = p.products != 1;
-        for (int it = 0; it < steps; ++it) {
-          const int pr = parts ? it / run : 0, kb = kb0 + it - pr * run;
-          const int ao = parts ? part_a(pr) * p.a_pitch : 0, bo6 = parts ? part_b(pr) * p.b_pitch : 0;
+        const bool a_mn = p.a_mn != 0, b_mn = p.b_mn != 0;
+        int part = C::NP - 1;  // parts 2, 1, 0 of each k-block
+        for (int kb = kb0; kb < kb1;) {
           {
             GEMM_T0();
             if (!mbar_wait(&empty[stage], phase ^ 1u, p.err)) goto producer_done_pair;
@@ -772,6 +805,7 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1)
           }
           uint8_t* sA = smem + stage * C::STAGE_BYTES;
           uint8_t* sB = sA + C::A_BYTES;
+          const int ao = PARTS ? part * p.a_pitch : 0, bo6 = PARTS ? part * p.b_pitch : 0;
           const uint32_t fb = mapa_shared(smem_u32(&full[stage]), 0);  // the leader's full barrier
           if (do_a) {
             if (rank == 0) mbar_arrive_expect_tx(&full[stage], 2 * C::STAGE_BYTES);
@@ -800,6 +834,10 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1)
             stage = 0;
             phase ^= 1u;
           }
+          if (part-- == 0) {
+            part = C::NP - 1;
+            ++kb;
+          }
         }
       }
     producer_done_pair:;
@@ -814,11 +852,9 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1)
       while (work_next(p, gridDim.x, num_kb, tiles_per_split, num_tiles, w, tm, tn, b, sp, kb0, kb1, last)) {
         const int bo = b / p.batch2, bi = b - bo * p.batch2;
         const int abo = p.a_bcast ? 0 : bo, abi = p.a_bcast ? 0 : bi;
-        const int run = kb1 - kb0, steps = run * p.products;
-        const bool a_mn = p.a_mn != 0, b_mn = p.b_mn != 0, parts = p.products != 1;
-        for (int it = 0; it < steps; ++it) {
-          const int pr = parts ? it / run : 0, kb = kb0 + it - pr * run;
-          const int ao = parts ? part_a(pr) * p.a_pitch : 0, bo6 = parts ? part_b(pr) * p.b_pitch : 0;
+        const bool a_mn = p.a_mn != 0, b_mn = p.b_mn != 0;
+        int part = C::NP - 1;
+        for (int kb = kb0; kb < kb1;) {
           {
             GEMM_T0();
             if (!mbar_wait(&empty[stage], phase ^ 1u, p.err)) goto producer_done;
@@ -826,6 +862,7 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1)
           }
           uint8_t* sA = smem + stage * C::STAGE_BYTES;
           uint8_t* sB = sA + C::A_BYTES;
+          const int ao = PARTS ? part * p.a_pitch : 0, bo6 = PARTS ? part * p.b_pitch : 0;
           if (do_a) {
             mbar_arrive_expect_tx(&full[stage], C::STAGE_BYTES);
             if (!a_mn) {
@@ -843,6 +880,10 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1)
           if (++stage == C::STAGES) {
             stage = 0;
             phase ^= 1u;
+          }
+          if (part-- == 0) {
+            part = C::NP - 1;
+            ++kb;
           }
         }
       }
@@ -873,26 +914,40 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1)
             GEMM_ACC(1);
           }
           tc_fence_after();
-          const uint32_t d = tmem_base + (uint32_t)(acc * BN);
+          const uint32_t d = tmem_base + (uint32_t)(acc * C::ACC_COLS);
           bool ok = true;
-          for (int it = 0; it < (kb1 - kb0) * p.products; ++it) {
-            GEMM_T0();
-            if (!mbar_wait(&full[stage], phase, p.err)) { ok = false; break; }
-            GEMM_ACC(2);
-            tc_fence_after();
-            const uint32_t at = (uint32_t)stage * (C::STAGE_BYTES >> 4);
-#pragma unroll
-            for (int k = 0; k < BK / 16; ++k) {
-              const uint64_t ad = desc_at(a0, at + k * a_step);
-#pragma unroll
-              for (int sub = 0; sub < C::NSUB; ++sub) {
-                const uint64_t bd = desc_at(b0, at + sub * (C::SUB_B_BYTES >> 4) + k * b_step);
-                mma_f16_pair(d + (uint32_t)(sub * C::MMA_N), ad, bd, idesc, (it != 0 || k != 0) ? 1u : 0u);
-              }
-            }
-            const uint32_t eb = smem_u32(&empty[stage]);
+          const auto release = [&](int st) {
+            const uint32_t eb = smem_u32(&empty[st]);
             mma_commit_pair(eb);
             mma_commit_pair(mapa_shared(eb, 1));
+          };
+          for (int it = 0; it < kb1 - kb0; ++it) {
+            GEMM_T0();
+            if constexpr (PARTS) {
+              ok = six_products<BK / 16>(full, phase, p.err, stage, C::STAGE_BYTES >> 4, a0, b0, a_step, b_step, d, BN,
+                                         it != 0,
+                                         [&](uint32_t to, uint64_t x, uint64_t y, uint32_t c) {
+                                           mma_f16_pair(to, x, y, idesc, c);
+                                         },
+                                         release);
+              if (!ok) break;
+              stage += 2;
+            } else {
+              if (!mbar_wait(&full[stage], phase, p.err)) { ok = false; break; }
+              GEMM_ACC(2);
+              tc_fence_after();
+              const uint32_t at = (uint32_t)stage * (C::STAGE_BYTES >> 4);
+#pragma unroll
+              for (int k = 0; k < BK / 16; ++k) {
+                const uint64_t ad = desc_at(a0, at + k * a_step);
+#pragma unroll
+                for (int sub = 0; sub < C::NSUB; ++sub) {
+                  const uint64_t bd = desc_at(b0, at + sub * (C::SUB_B_BYTES >> 4) + k * b_step);
+                  mma_f16_pair(d + (uint32_t)(sub * C::MMA_N), ad, bd, idesc, (it != 0 || k != 0) ? 1u : 0u);
+                }
+              }
+              release(stage);
+            }
             if (++stage == C::STAGES) {
               stage = 0;
               phase ^= 1u;
@@ -924,7 +979,7 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1)
       };
       const uint64_t a0 = first(smem0, p.a_mn != 0), b0 = first(smem0 + C::A_BYTES, p.b_mn != 0);
       const uint32_t a_step = (p.a_mn ? mn_step : 32u) >> 4, b_step = (p.b_mn ? mn_step : 32u) >> 4;
-      const int kind = p.i8 ? 2 : (p.tf32 ? 1 : 0), products = p.products;
+      const int kind = p.i8 ? 2 : (p.tf32 ? 1 : 0);
       uint32_t* const err = p.err;
       int stage = 0;
       uint32_t phase = 0;
@@ -941,21 +996,32 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1)
           GEMM_ACC(1);
         }
         tc_fence_after();
-        const uint32_t d = tmem_base + (uint32_t)(acc * BN);
+        const uint32_t d = tmem_base + (uint32_t)(acc * C::ACC_COLS);
         // One loop for each kind of operand: testing for it at every MMA
         // costs the issuing thread more than the MMA takes.
-        const int steps = (kb1 - kb0) * products;
+        const int steps = kb1 - kb0;
         const auto run = [&](auto issue) {
           for (int it = 0; it < steps; ++it) {
             GEMM_T0();
-            if (!mbar_wait(&full[stage], phase, err)) return false;
-            GEMM_ACC(2);
-            tc_fence_after();
-            const uint32_t at = (uint32_t)stage * (C::STAGE_BYTES >> 4);
+            if constexpr (PARTS) {
+              if (!six_products<BK / 16>(full, phase, err, stage, C::STAGE_BYTES >> 4, a0, b0, a_step, b_step, d, BN,
+                                         it != 0,
+                                         [&](uint32_t to, uint64_t x, uint64_t y, uint32_t c) {
+                                           mma_f16(to, x, y, idesc, c);
+                                         },
+                                         [&](int st) { mma_commit(&empty[st]); }))
+                return false;
+              stage += 2;
+            } else {
+              if (!mbar_wait(&full[stage], phase, err)) return false;
+              GEMM_ACC(2);
+              tc_fence_after();
+              const uint32_t at = (uint32_t)stage * (C::STAGE_BYTES >> 4);
 #pragma unroll
-            for (int k = 0; k < BK / 16; ++k)
-              issue(desc_at(a0, at + k * a_step), desc_at(b0, at + k * b_step), (it != 0 || k != 0) ? 1u : 0u);
-            mma_commit(&empty[stage]);
+              for (int k = 0; k < BK / 16; ++k)
+                issue(desc_at(a0, at + k * a_step), desc_at(b0, at + k * b_step), (it != 0 || k != 0) ? 1u : 0u);
+              mma_commit(&empty[stage]);
+            }
             if (++stage == C::STAGES) {
               stage = 0;
               phase ^= 1u;
@@ -963,7 +1029,8 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1)
           }
           return true;
         };
-        const bool ok = kind == 0   ? run([&](uint64_t x, uint64_t y, uint32_t c) { mma_f16(d, x, y, idesc, c); })
+        const bool ok = (PARTS || kind == 0)
+                            ? run([&](uint64_t x, uint64_t y, uint32_t c) { mma_f16(d, x, y, idesc, c); })
                         : kind == 1 ? run([&](uint64_t x, uint64_t y, uint32_t c) { mma_tf32(d, x, y, idesc, c); })
                                     : run([&](uint64_t x, uint64_t y, uint32_t c) { mma_i8(d, x, y, idesc, c); });
         if (!ok) break;
@@ -1033,11 +1100,26 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1)
       const int64_t rb = (int64_t)bo * p.bsr + (int64_t)bi * p.bsr2;
       const int64_t mb = (int64_t)bo * p.bsm + (int64_t)bi * p.bsm2;
       const int row0 = tm * TILE_M + (int)rank * BM + q * 32;
-      const uint32_t tbase = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(acc * BN + half * NCH * 32);
+      const uint32_t tbase = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(acc * C::ACC_COLS + half * NCH * 32);
       uint32_t r[2][32];
       uint8_t* box = nullptr;  // the TMA-store box being filled
-      tmem_ld32(tbase, r[0]);
-      tmem_ld_wait();
+      [[maybe_unused]] uint32_t small[PARTS ? 32 : 1];  // the other five products' chunk
+      const auto chunk_load = [&](int i) {
+        tmem_ld32(tbase + (uint32_t)(i * 32), r[i & 1]);
+        if constexpr (PARTS) tmem_ld32(tbase + (uint32_t)(BN + i * 32), small);
+      };
+      const auto chunk_wait = [&](int i) {
+        tmem_ld_wait();
+        if constexpr (PARTS) {
+#pragma unroll
+          for (int j = 0; j < 32; ++j) {
+            asm volatile("" : "+r"(r[i & 1][j]), "+r"(small[j]));  // not before the wait
+            r[i & 1][j] = __float_as_uint(__uint_as_float(r[i & 1][j]) + __uint_as_float(small[j]));
+          }
+        }
+      };
+      chunk_load(0);
+      chunk_wait(0);
       GEMM_STAMP(threadIdx.x == 64 && last_tile, 13);
       [[maybe_unused]] float ce_m = -INFINITY, ce_s = 0.f, ce_g = 0.f;
       [[maybe_unused]] int ce_lab = -1;
@@ -1071,7 +1153,7 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1)
 #pragma unroll 2
       for (int i = 0; i < NCH; ++i) {
         if (i == 1) GEMM_STAMP(threadIdx.x == 64 && last_tile, 15);
-        if (i + 1 < NCH) tmem_ld32(tbase + (uint32_t)((i + 1) * 32), r[(i + 1) & 1]);
+        if (i + 1 < NCH) chunk_load(i + 1);
         const int n0 = tn * BN + (half * NCH + i) * 32;
         if constexpr (EPI == 3) {
           if (n0 < p.N) {
@@ -1245,7 +1327,7 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1)
             }
           }
         }
-        if (i + 1 < NCH) tmem_ld_wait();
+        if (i + 1 < NCH) chunk_wait(i + 1);
       }
       if constexpr (EPI == 3 || EPI == 5) {
         if (row0 + lane < p.M)
@@ -1343,21 +1425,21 @@ int epi_kind(const TcParams& p) {
   return (extras || !plain_on) ? 1 : 2;
 }
 
-template <int BN, int EPI>
+template <int BN, int EPI, bool PARTS = false>
 void launch_tc_k(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& tc, const TcParams& p, int max_ctas,
                  cudaStream_t s) {
-  using C = Cfg<BN, false, (EPI >= 4)>;
+  using C = Cfg<BN, false, (EPI >= 4), PARTS>;
   static bool attr_set[kMaxDevices] = {false};
   const int dev = current_device_slot();
   if (!attr_set[dev]) {
-    DLVK_CUDA_CHECK(
-        cudaFuncSetAttribute(gemm_tc_kernel<BN, false, EPI>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
+    DLVK_CUDA_CHECK(cudaFuncSetAttribute(gemm_tc_kernel<BN, false, EPI, PARTS>,
+                                         cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
     attr_set[dev] = true;
   }
   const int tiles = p.tiles_m * p.tiles_n * p.batch * p.splits;
   const int slots = max_ctas > 0 ? max_ctas : sm_count();
   int grid = p.sk ? slots : std::min(tiles, slots);  // stream-K: every CTA takes a share
-  launch_pdl(gemm_tc_kernel<BN, false, EPI>, dim3(grid), dim3(GEMM_THREADS), C::SMEM, s, ta, tb, tc, p);
+  launch_pdl(gemm_tc_kernel<BN, false, EPI, PARTS>, dim3(grid), dim3(GEMM_THREADS), C::SMEM, s, ta, tb, tc, p);
   DLVK_POST_LAUNCH();
 }
 template <int BN>
@@ -1371,10 +1453,10 @@ void launch_tc(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& 
 
 // 2-CTA clusters sharing 256 x BN tiles (cta_group::2).  The persistent
 // grid is as many pairs as can be resident at once.
-template <int BN, int EPI>
+template <int BN, int EPI, bool PARTS = false>
 void launch_tc_pair_k(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& tc, const TcParams& p,
                       int max_ctas, cudaStream_t s) {
-  using C = Cfg<BN, true, (EPI >= 4)>;
+  using C = Cfg<BN, true, (EPI >= 4), PARTS>;
   static int max_pairs[kMaxDevices] = {0};
   const int dev = current_device_slot();
   cudaLaunchConfig_t cfg = {};
@@ -1391,11 +1473,11 @@ void launch_tc_pair_k(const CUtensorMap& ta, const CUtensorMap& tb, const CUtens
   cfg.attrs = attr;
   cfg.numAttrs = 1;  // occupancy query: cluster shape only
   if (max_pairs[dev] == 0) {
-    DLVK_CUDA_CHECK(
-        cudaFuncSetAttribute(gemm_tc_kernel<BN, true, EPI>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
+    DLVK_CUDA_CHECK(cudaFuncSetAttribute(gemm_tc_kernel<BN, true, EPI, PARTS>,
+                                         cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
     cfg.gridDim = dim3(2 * 74, 1, 1);
     int n = 0;
-    DLVK_CUDA_CHECK(cudaOccupancyMaxActiveClusters(&n, gemm_tc_kernel<BN, true, EPI>, &cfg));
+    DLVK_CUDA_CHECK(cudaOccupancyMaxActiveClusters(&n, gemm_tc_kernel<BN, true, EPI, PARTS>, &cfg));
     max_pairs[dev] = std::max(1, n);
   }
   const int tiles = p.tiles_m * p.tiles_n * p.batch * p.splits;
@@ -1403,7 +1485,7 @@ void launch_tc_pair_k(const CUtensorMap& ta, const CUtensorMap& tb, const CUtens
   if (max_ctas > 0) pairs = std::max(1, std::min(pairs, max_ctas / 2));
   cfg.gridDim = dim3(2 * pairs, 1, 1);
   cfg.numAttrs = 2;
-  DLVK_CUDA_CHECK(cudaLaunchKernelEx(&cfg, gemm_tc_kernel<BN, true, EPI>, ta, tb, tc, p));
+  DLVK_CUDA_CHECK(cudaLaunchKernelEx(&cfg, gemm_tc_kernel<BN, true, EPI, PARTS>, ta, tb, tc, p));
   DLVK_POST_LAUNCH();
 }
 template <int BN>
@@ -1413,6 +1495,26 @@ void launch_tc_pair(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensor
   if (k == 2) launch_tc_pair_k<BN, 2>(ta, tb, tc, p, max_ctas, s);
   else if (k == 1) launch_tc_pair_k<BN, 1>(ta, tb, tc, p, max_ctas, s);
   else launch_tc_pair_k<BN, 0>(ta, tb, tc, p, max_ctas, s);
+}
+
+// The tile that was chosen (operands in parts: 256 wide in pairs, 128 alone).
+void launch_tile(int BN, bool pair, const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& tc,
+                 const TcParams& p, int max_ctas, cudaStream_t s) {
+  if (p.parts) {
+    const bool plain = epi_kind(p) == 2;
+    if (pair && plain) launch_tc_pair_k<256, 2, true>(ta, tb, tc, p, max_ctas, s);
+    else if (pair) launch_tc_pair_k<256, 0, true>(ta, tb, tc, p, max_ctas, s);
+    else if (plain) launch_tc_k<128, 2, true>(ta, tb, tc, p, max_ctas, s);
+    else launch_tc_k<128, 0, true>(ta, tb, tc, p, max_ctas, s);
+  } else if (pair && BN == 512) {
+    launch_tc_pair<512>(ta, tb, tc, p, max_ctas, s);
+  } else if (pair) {
+    launch_tc_pair<256>(ta, tb, tc, p, max_ctas, s);
+  } else if (BN == 256) {
+    launch_tc<256>(ta, tb, tc, p, max_ctas, s);
+  } else {
+    launch_tc<128>(ta, tb, tc, p, max_ctas, s);
+  }
 }
 
 inline bool al16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
@@ -1552,8 +1654,15 @@ void choose_tiling(const GemmArgs& a, int sms, int& BN, int& splits, bool& pair,
   // (back-to-back timings of 8192 x 1024 x {1024, 3072, 4096} against the
   // 256-wide pair tile), and 1.55x is kept from K = 8192 on.
   const double wide_eff = kbs >= 128 ? 1.55 : 1.75;
-  const Cand cands[] = {{true, 512, wide_eff}, {true, 256, 1.2}, {false, 256, 1.0}, {false, 128, 0.85}};
-  for (const Cand& c : cands) {
+  const Cand all[] = {{true, 512, wide_eff}, {true, 256, 1.2}, {false, 256, 1.0}, {false, 128, 0.85}};
+  // Operands in parts: a k-block of the pair tile takes 1.5 us, of the single
+  // one 1.28, and the pair's one accumulator buffer leaves every tile's
+  // epilogue exposed, 9.6 us or with a bias 14 (768 x 10007 x 512 with bias: 55
+  // us in pairs, 46 alone; 512 x 16000 x 2048: 129 in pairs, 148 alone).
+  const Cand of_parts[] = {{true, 256, 2.07}, {false, 128, 1.215}};
+  const Cand* cands = a.parts ? of_parts : all;
+  for (int ci = 0; ci < (a.parts ? 2 : 4); ++ci) {
+    const Cand& c = cands[ci];
     if (c.pair && !pair_ok) continue;
     if (c.bn == 512 && (!gemm_tc_wide_enabled() || a.N < 512)) continue;
     if (c.bn != 512 && wide_flag() == 2 && pair_ok && a.N >= 512 && best < 1e300) continue;
@@ -1568,9 +1677,9 @@ void choose_tiling(const GemmArgs& a, int sms, int& BN, int& splits, bool& pair,
       if (sp > 8 && !a.parts) break;
       if (sp > 1 && kbs * products / sp < 8) break;
       // The accumulators lose a little with every addition (2^-24, always
-      // towards zero): at most 1024 elements of K for products that are to be
+      // towards zero): at most 1280 elements of K for products that are to be
       // as good as fp32, the rest is summed in the reduction.
-      if (a.parts && sp < 32 && (kbs + sp - 1) / sp > 16) continue;
+      if (a.parts && sp < 32 && (kbs + sp - 1) / sp > 20) continue;
       const int64_t units = tiles * sp;
       const int64_t waves = (units + slots - 1) / slots;
       const double unit_s = (double)tile_m * c.bn * BK * 2.0 * products * ((kbs + sp - 1) / sp) /
@@ -1579,7 +1688,7 @@ void choose_tiling(const GemmArgs& a, int sms, int& BN, int& splits, bool& pair,
       // 128 x 256, ~18 GB/s for 128 x 512), exposed once at the end, or
       // after every wave without a second accumulator buffer.
       const double epi_s = 128.0 * c.bn * ((out_f32 || sp > 1) ? 4.0 : 2.0) / (c.bn == 512 ? 18e9 : 17e9);
-      double t = waves * unit_s + (c.bn == 512 ? waves : 1) * epi_s;
+      double t = waves * unit_s + (a.parts && c.pair ? (a.bias ? 1.85 : 1.25) * waves : c.bn == 512 ? waves : 1) * epi_s;
       if (sp > 1) {
         const double mn = (double)a.M * a.N * a.batch * a.batch2;
         t += red ? sp * mn * 4.0 / 8e12 + (a.beta == 0.f ? mn * 4.0 / 5e12 + 2e-6 : 0.0)
@@ -1767,6 +1876,7 @@ void gemm_tc_impl(DType out_dt, const GemmArgs& a, cudaStream_t s, uint32_t* err
     const TilingOverride& ov = tiling_override();
     if (ov.pair >= 0) pair = ov.pair != 0 && !tf32 && a.M >= 256;
     if (ov.bn > 0) BN = (ov.bn == 512 && !pair) ? 256 : ov.bn;
+    if (a.parts) BN = pair ? 256 : 128;
     if (ov.splits > 0) {
       splits = ov.splits;
       sk = false;
@@ -1857,7 +1967,7 @@ void gemm_tc_impl(DType out_dt, const GemmArgs& a, cudaStream_t s, uint32_t* err
             ((a.batch2_stride_m * esz) % 16 == 0);
   p.alpha = a.alpha;
   p.alpha_ptr = a.alpha_ptr;
-  p.products = a.parts ? 6 : 1;
+  p.parts = a.parts ? 1 : 0;
   p.a_pitch = (int)a.pitch_a;
   p.b_pitch = (int)a.pitch_b;
   p.beta = a.beta;
@@ -1888,10 +1998,7 @@ void gemm_tc_impl(DType out_dt, const GemmArgs& a, cudaStream_t s, uint32_t* err
     if (p.tma_c == 2) {
       if (a.beta == 0.f)
         DLVK_CUDA_CHECK(cudaMemset2DAsync(a.C, (size_t)a.ldc * 4, 0, (size_t)a.N * 4, (size_t)a.M, s));
-      if (pair && BN == 512) launch_tc_pair<512>(ta, tb, tc, p, max_ctas, s);
-    else if (pair) launch_tc_pair<256>(ta, tb, tc, p, max_ctas, s);
-      else if (BN == 256) launch_tc<256>(ta, tb, tc, p, max_ctas, s);
-      else launch_tc<128>(ta, tb, tc, p, max_ctas, s);
+      launch_tile(BN, pair, ta, tb, tc, p, max_ctas, s);
       return;
     }
     // The map was refused: run unsplit.
@@ -1922,10 +2029,7 @@ void gemm_tc_impl(DType out_dt, const GemmArgs& a, cudaStream_t s, uint32_t* err
     p.Mk = nullptr;
     p.act = ACT_NONE;
     const CUtensorMap tc = make_c_map(p, a.M, a.N);
-    if (pair && BN == 512) launch_tc_pair<512>(ta, tb, tc, p, max_ctas, s);
-    else if (pair) launch_tc_pair<256>(ta, tb, tc, p, max_ctas, s);
-    else if (BN == 256) launch_tc<256>(ta, tb, tc, p, max_ctas, s);
-    else launch_tc<128>(ta, tb, tc, p, max_ctas, s);
+    launch_tile(BN, pair, ta, tb, tc, p, max_ctas, s);
     const bool plain = a.batch == 1 && a.batch2 == 1 && !a.row_bias && !a.residual && a.act == ACT_NONE &&
                        !a.relu_mask && !a.relu_bits && a.N % 4 == 0 && a.ldc % 4 == 0 && al16(a.C) && al16(workspace);
     const int g = (int)std::min<int64_t>((per + 255) / 256, 148 * 16);
@@ -1943,10 +2047,7 @@ void gemm_tc_impl(DType out_dt, const GemmArgs& a, cudaStream_t s, uint32_t* err
   const CUtensorMap tc = make_c_map(p, a.M, a.N);
   DLVK_CHECK(!(p.colsum && p.beta == 0.f && !(p.out_f32 && (p.R || p.Mk)) && p.tma_c == 0),
              "gemm_tc: column sums without a staged input need the TMA-store epilogue");
-  if (pair && BN == 512) launch_tc_pair<512>(ta, tb, tc, p, max_ctas, s);
-  else if (pair) launch_tc_pair<256>(ta, tb, tc, p, max_ctas, s);
-  else if (BN == 256) launch_tc<256>(ta, tb, tc, p, max_ctas, s);
-  else launch_tc<128>(ta, tb, tc, p, max_ctas, s);
+  launch_tile(BN, pair, ta, tb, tc, p, max_ctas, s);
 }
 }  // namespace
 
@@ -2029,17 +2130,18 @@ struct CeTiling {
   bool pair;
   int bn;
 };
-CeTiling ce_tiling(int64_t M, int64_t N) {
+CeTiling ce_tiling(int64_t M, int64_t N, bool parts) {
   const int sms = sm_count();
   if (gemm_tc_pair_enabled() && M >= 256 && (M + 255) / 256 * ((N + 255) / 256) >= sms * 2 / 5) return {true, 256};
-  return {false, (M + 127) / 128 * ((N + 127) / 128) <= 2 * sms ? 128 : 256};
+  return {false, parts || (M + 127) / 128 * ((N + 127) / 128) <= 2 * sms ? 128 : 256};
 }
 
 template <int EPI>
 void ce_launch(const CeProjection& c, void* out, int64_t ldo, float* colsum, cudaStream_t s, uint32_t* err) {
-  DLVK_CHECK(ce_tc_supported(c) && (EPI == 3 || (ldo % 8 == 0 && al16(out))), "cross entropy: unsupported layout");
+  DLVK_CHECK(ce_tc_supported(c) && (EPI == 3 || (ldo % 8 == 0 && al16(out) && !c.parts)),
+             "cross entropy: unsupported layout");
   tmap::bind_context();
-  const CeTiling t = ce_tiling(c.rows, c.classes);
+  const CeTiling t = ce_tiling(c.rows, c.classes, c.parts);
   const uint64_t da = (uint64_t)c.ldx * (uint64_t)c.rows;
   const CUtensorMap ta = make_tmap(c.x, c.parts ? 3 * c.pitch_x : c.width, c.rows, 1, 1, c.ldx, da, da, BM, Elem::BF16);
   CUtensorMap tb;
@@ -2059,7 +2161,7 @@ void ce_launch(const CeProjection& c, void* out, int64_t ldo, float* colsum, cud
   p.tiles_n = (int)((c.classes + t.bn - 1) / t.bn);
   p.b_mn = c.w_k ? 0 : 1;
   p.alpha = 1.f;
-  p.products = c.parts ? 6 : 1;
+  p.parts = c.parts ? 1 : 0;
   p.a_pitch = (int)c.pitch_x;
   p.b_pitch = (int)c.pitch_w;
   p.bias = c.bias;
@@ -2077,6 +2179,13 @@ void ce_launch(const CeProjection& c, void* out, int64_t ldo, float* colsum, cud
     tc = make_c_map(p, c.rows, c.classes);
     DLVK_CHECK(p.tma_c == 1, "cross entropy: the output's tile map was refused");
   }
+  if constexpr (EPI == 3) {  // the loss alone of fp32 operands
+    if (c.parts) {
+      if (t.pair) launch_tc_pair_k<256, 3, true>(ta, tb, tc, p, 0, s);
+      else launch_tc_k<128, 3, true>(ta, tb, tc, p, 0, s);
+      return;
+    }
+  }
   if (t.pair) launch_tc_pair_k<256, EPI>(ta, tb, tc, p, 0, s);
   else if (t.bn == 256) launch_tc_k<256, EPI>(ta, tb, tc, p, 0, s);
   else launch_tc_k<128, EPI>(ta, tb, tc, p, 0, s);
@@ -2089,9 +2198,9 @@ bool ce_tc_supported(const CeProjection& c) {
          ((c.rows + 127) / 128) * ((c.classes + 127) / 128) < (1LL << 31) && tma_c_enabled();
 }
 
-int ce_tc_stat_width(int64_t rows, int64_t classes) { return ce_tiling(rows, classes).bn / 2; }
-int ce_tc_stat_cols(int64_t rows, int64_t classes) {
-  const int bn = ce_tiling(rows, classes).bn;
+int ce_tc_stat_width(int64_t rows, int64_t classes) { return ce_tiling(rows, classes, false).bn / 2; }
+int ce_tc_stat_cols(int64_t rows, int64_t classes, bool parts) {
+  const int bn = ce_tiling(rows, classes, parts).bn;
   return (int)(2 * ((classes + bn - 1) / bn));
 }
 
@@ -2176,7 +2285,6 @@ void gemm_i8_tc(const int8_t* A, const int8_t* Bt, const float* row_scale, const
   p.splits = 1;
   p.kb_per_split = (int)((K + 2 * BK - 1) / (2 * BK));
   p.i8 = 1;
-  p.products = 1;
   p.row_scale = row_scale;
   p.col_scale = col_scale;
   if (BN == 256) launch_tc<256>(ta, tb, ta, p, 0, s);
