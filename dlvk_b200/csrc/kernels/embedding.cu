@@ -12,7 +12,8 @@
 // What bounds them: the lookup moves n D elements in and out; the gradient
 // reads dy once and writes V D fp32 once (8192 x 1024 bf16 tokens over 32000
 // words: 17 MB in, 131 MB out, 22.6 us at the measured copy rate), so the
-// sort has to be short.
+// sort has to be short.  Measured: that lookup 6.1 us, that gradient 36.7 (sort
+// 6.6, sums 21.8, joins 9.8, each starting up while the one before it ends).
 #include <algorithm>
 #include <type_traits>
 

@@ -19,6 +19,9 @@
 // all of them tiny) are taken in 64 bits instead, so the norm is right over
 // the whole range of fp32.  Each block's total goes to its own place and the
 // totals are added in a fixed order: the result does not vary.
+//
+// 216 M fp32 gradients (0.86 GB): norm 128 us (6.7 TB/s), clipping into another
+// buffer 407 us (two reads and a write are 395 at the measured copy rate).
 #include <algorithm>
 #include <cmath>
 

@@ -13,7 +13,7 @@
 // (16 bits, at most 256 MB whatever the batch), ce_rescale turns those into
 // dz, and the two gradient products read dz: three products, one pass over
 // the block.  Making the logits a second time instead costs a fourth product
-// (8192 x 1024 x 32000: 434 us against 2 x 85 us for the pass); it is
+// (8192 x 1024 x 32000: 434 us against 2 x 95 us for the pass); it is
 // what a bias gradient takes, whose fp32 sums 16-bit exponentials are too
 // coarse for.
 #include <algorithm>

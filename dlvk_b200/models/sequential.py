@@ -346,6 +346,8 @@ class Sequential(Model):
 
     def head_loss(self, x, y, loss_fn):
         """(loss, correct rows, rows) of a batch without a gradient."""
+        if loss_fn.reduction == "none":
+            raise ValueError("evaluation needs reduction mean or sum")
         head, h, _ = self._forward_hidden(x)
         correct = torch.zeros(1, dtype=torch.int64, device=h.device)
         loss = loss_fn.forward(h, head.weight.value, y.to(h.device), head.bias.master if head.bias is not None else None,

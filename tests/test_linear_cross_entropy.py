@@ -379,6 +379,16 @@ def test_refusals(device):
         m.train_step(torch.randn(2, 8), torch.zeros(2, dtype=torch.int32), fn, dl.SGD(0.1))
 
 
+def test_evaluation_needs_one_loss():
+    m = Sequential("cpu", "fp32", seed=0)
+    m.add_dense(8, 70)
+    x, y = torch.randn(2, 8), torch.zeros(2, dtype=torch.int32)
+    with pytest.raises(ValueError, match="reduction"):
+        m.head_loss(x, y, dl.LinearCrossEntropyLoss("none"))
+    loss, hits, rows = m.head_loss(x, y, dl.LinearCrossEntropyLoss("sum"))
+    assert rows == 2 and 0 <= hits <= 2 and float(loss) > 0
+
+
 @pytest.mark.gpu
 def test_refusals_on_the_gpu():
     x, w, t, b = operands(6, 16, 70, torch.bfloat16, "cuda", bias=True)
