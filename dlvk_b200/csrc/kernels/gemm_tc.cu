@@ -602,21 +602,18 @@ __device__ __forceinline__ float ce_max(const float* v, float m) {
   return fmaxf(m, t[0]);
 }
 
-// v = 2^((v - m) log2 e + up), in pairs: one fma each.  A maximum of -inf
-// (every logit masked) is replaced by 0: the results are exp(-inf) = 0.  One
-// near either end of fp32 (masks of -3.4e38) times log2 e would be infinite,
-// so there the difference is taken first.
+// v = 2^((v - m) log2 e + up), in pairs.  The difference is taken before the
+// scaling: it is exact where v is near m, so that v = m gives 2^up itself.  One
+// fma (v log2 e - the rounded m log2 e) would be off there by that rounding, 3e-8
+// |m|, in every row's loss, and by whole powers of 2 for masks of -1e20.  A
+// maximum of -inf (every logit masked) is replaced by 0: the results are
+// exp(-inf) = 0.
 __device__ __forceinline__ void ce_exp32(float m, float up, float* v) {
-  if (fabsf(m) > 2e38f && m != -INFINITY) {
-#pragma unroll
-    for (int j = 0; j < 32; ++j) v[j] = ex2((v[j] - m) * LOG2E + up);
-    return;
-  }
-  const float c = m == -INFINITY ? up : fmaf(m, -LOG2E, up);
-  const float2 l2 = make_float2(LOG2E, LOG2E), c2 = make_float2(c, c);
+  const float c = m == -INFINITY ? 0.f : -m;
+  const float2 c2 = make_float2(c, c), l2 = make_float2(LOG2E, LOG2E), u2 = make_float2(up, up);
 #pragma unroll
   for (int j = 0; j < 32; j += 2) {
-    const float2 x = __ffma2_rn(make_float2(v[j], v[j + 1]), l2, c2);
+    const float2 x = __ffma2_rn(__fadd2_rn(make_float2(v[j], v[j + 1]), c2), l2, u2);
     v[j] = ex2(x.x);
     v[j + 1] = ex2(x.y);
   }

@@ -1,0 +1,70 @@
+"""Softmax cross entropy of a vocabulary projection at the ends of its range:
+masks between the ordinary logits and fp32's lowest value, rows whose word is
+certain, numbers of rows that a launch's grid has to hold.
+
+The limits are those of `exact` in test_linear_cross_entropy.py unless a test
+derives its own.
+"""
+
+import pytest
+import torch
+
+import dlvk_b200 as dl
+from test_linear_cross_entropy import exact, near, operands
+
+DEVICES = [pytest.param("cpu"), pytest.param("cuda", marks=pytest.mark.gpu)]
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("low", [-1e4, -1e9, -1e20, -1e30, -1e37, -1.9e38])
+def test_words_masked_by_a_low_bias(device, dtype, low):
+    """A bias of -1e4 and below leaves a word a probability of 0 (exp of less than -9000), whatever
+    the number: a whole tile of such words adds nothing and spoils nothing."""
+    x, w, t, b = operands(300, 64, 520, dtype, device, bias=True)
+    b[500:] = low
+    b[100:300] = low
+    t = torch.where(t % 500 < 300, t % 100, t % 500)
+    loss, dx, dw, db = dl.LinearCrossEntropyLoss().value_and_grad(x, w, t, b)
+    keep = torch.ones(520, dtype=torch.bool, device=device)
+    keep[500:] = keep[100:300] = False
+    where = torch.cumsum(keep, 0) - 1
+    want = exact(x, w[:, keep], where[t], b[keep])
+    near(loss, want["loss"], "loss")
+    near(dl.LinearCrossEntropyLoss().forward(x, w, t, b), want["loss"], "loss alone")
+    near(dx, want["dx"], "dx")
+    near(dw[:, keep], want["dw"], "dw")
+    near(db[keep], want["db"], "db")
+    assert not dw[:, ~keep].any() and not db[~keep].any()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("n,v", [(12, 1040), (300, 1040), (2500, 9001)])
+@pytest.mark.parametrize("bias", [False, True])
+@pytest.mark.parametrize("high", [12.0, 120.0, 1000.0, 2.0 ** 20, 2.0 ** 100])
+def test_rows_whose_word_is_certain(device, dtype, n, v, bias, high):
+    """Word 7 has a logit of high (1 to 2), the others 0: a loss of log(1 + (v - 1) e^-z).
+
+    The row's maximum is its word's logit, so the loss is log(s) with s = 1 + the others' sum: never
+    below 0.  s is a sum of v terms: off by 2^-24 of at most 2 for each of them, and each term by
+    2^-22 (|z| + 2) of itself, as in `exact`.  Where e^-z is below fp32's smallest number, s is 1,
+    the loss 0 and dz = 1 / s - 1 = 0."""
+    g = torch.Generator().manual_seed(n)
+    x, w = torch.zeros(n, 64, dtype=dtype, device=device), torch.zeros(64, v, dtype=dtype, device=device)
+    x[:, 0] = (1 + torch.rand(n, generator=g)).to(dtype).to(device)
+    w[0, 7] = high
+    t = torch.full((n,), 7, dtype=torch.int32, device=device)
+    b = torch.zeros(v, device=device) if bias else None
+    rows = dl.LinearCrossEntropyLoss("none").forward(x, w, t, b)
+    z = x[:, 0].double() * float(w[0, 7])
+    others = (v - 1) * torch.exp(-z)
+    want = torch.log1p(others)
+    # z itself is a product rounded to fp32
+    lim = (v + 2) * 2.0 ** -23 + others * (2.0 ** -22 * (z + 2) + 2.0 ** -24 * z)
+    assert bool((rows >= 0).all()), float(rows.min())
+    assert bool(((rows.double() - want).abs() <= lim).all()), float((rows.double() - want).abs().max())
+    loss, dx, dw, db = dl.LinearCrossEntropyLoss().value_and_grad(x, w, t, b)
+    assert float(loss) >= 0 and abs(float(loss) - float(want.mean())) <= float(lim.mean()) + 2.0 ** -24 * float(loss)
+    if high > 104:
+        assert float(loss) == 0.0 and not dx.any() and not dw.any() and (db is None or not db.any())
