@@ -160,7 +160,8 @@ int64_t block_of(int64_t rows, int64_t classes, int64_t room) {
 LinearCeResult linear_ce_op(const at::Tensor& x, const at::Tensor& w, const at::Tensor& target,
                             c10::optional<at::Tensor> bias, int64_t ignore_index, bool mean, bool want_grad,
                             c10::optional<at::Tensor> grad_scale, c10::optional<at::Tensor> dw_out, bool dw_accumulate,
-                            c10::optional<at::Tensor> db_out, bool db_accumulate, c10::optional<at::Tensor> correct) {
+                            c10::optional<at::Tensor> db_out, bool db_accumulate, c10::optional<at::Tensor> correct,
+                            c10::optional<at::Tensor> counted, c10::optional<at::Tensor> loss_sum) {
   check_cuda(x, "hidden");
   const at::Device dev = x.device();
   const auto dt = x.scalar_type();
@@ -182,6 +183,8 @@ LinearCeResult linear_ce_op(const at::Tensor& x, const at::Tensor& w, const at::
   };
   scalar(grad_scale, at::kFloat, "grad_scale");
   scalar(correct, at::kLong, "correct");
+  scalar(counted, at::kLong, "counted");
+  scalar(loss_sum, at::kFloat, "loss_sum");
   if (bias.has_value())
     TORCH_CHECK(bias->dim() == 1 && bias->size(0) == V && bias->device() == dev &&
                     (bias->scalar_type() == at::kFloat || bias->scalar_type() == at::kBFloat16),
@@ -382,6 +385,8 @@ LinearCeResult linear_ce_op(const at::Tensor& x, const at::Tensor& w, const at::
     f.grad_scale = gsp;
     f.loss = out.loss.data_ptr<float>();
     f.gscale = gscale;
+    f.loss_sum = loss_sum.has_value() ? loss_sum->data_ptr<float>() : nullptr;
+    f.counted = counted.has_value() ? reinterpret_cast<unsigned long long*>(counted->data_ptr<int64_t>()) : nullptr;
     f.correct = correct.has_value() ? reinterpret_cast<unsigned long long*>(correct->data_ptr<int64_t>()) : nullptr;
     f.partial = partial;
     f.done = done;

@@ -52,15 +52,17 @@ void register_ops(py::module& m) {
   m.def("linear_ce", [](const at::Tensor& x, const at::Tensor& w, const at::Tensor& target,
                         c10::optional<at::Tensor> bias, int64_t ignore_index, bool mean, bool want_grad,
                         c10::optional<at::Tensor> grad_scale, c10::optional<at::Tensor> dw_out, bool dw_accumulate,
-                        c10::optional<at::Tensor> db_out, bool db_accumulate, c10::optional<at::Tensor> correct) {
+                        c10::optional<at::Tensor> db_out, bool db_accumulate, c10::optional<at::Tensor> correct,
+                        c10::optional<at::Tensor> counted, c10::optional<at::Tensor> loss_sum) {
     auto r = linear_ce_op(x, w, target, bias, ignore_index, mean, want_grad, grad_scale, dw_out, dw_accumulate, db_out,
-                          db_accumulate, correct);
+                          db_accumulate, correct, counted, loss_sum);
     auto some = [](const at::Tensor& t) { return t.defined() ? c10::optional<at::Tensor>(t) : c10::nullopt; };
     return std::make_tuple(r.loss, r.rows, some(r.dx), some(r.dw), some(r.dbias));
   }, py::arg("hidden"), py::arg("weight"), py::arg("target"), py::arg("bias") = py::none(), py::arg("ignore_index") = -1,
      py::arg("mean") = true, py::arg("want_grad") = true, py::arg("grad_scale") = py::none(),
      py::arg("dw_out") = py::none(), py::arg("dw_accumulate") = false, py::arg("db_out") = py::none(),
-     py::arg("db_accumulate") = false, py::arg("correct") = py::none());
+     py::arg("db_accumulate") = false, py::arg("correct") = py::none(), py::arg("counted") = py::none(),
+     py::arg("loss_sum") = py::none());
   m.def("gemm_tc_ok", &gemm_tc_ok);
   m.def("gemm_tf32_ok", &gemm_tf32_ok);
   m.def("set_fp32_gemm_mode", &set_fp32_gemm_mode);

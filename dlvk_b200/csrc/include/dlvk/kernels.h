@@ -351,8 +351,9 @@ void ce_count(const CeRows& r, bool mean, const float* grad_scale, float* gscale
 // not count) and norm; x_clean, when given, becomes a copy of x whose
 // uncounted rows are 0.  The last of all `total_groups` groups of 32 rows (of
 // every block of rows; this one's are first_group onwards) adds up the
-// losses: *loss = sum (mean: / counted rows), *correct += rows whose class has
-// the largest logit, and, when set_gscale, *gscale as ce_count's.
+// losses: *loss = sum (mean: / counted rows), and, when set_gscale, *gscale as
+// ce_count's; where given, *loss_sum += the sum, *counted += the rows that
+// count, *correct += those whose class has the largest logit.
 // partial: 3 doubles per group.  `done` was set to 0 before the first block.
 struct CeFinish {
   const float2* stats;
@@ -363,7 +364,8 @@ struct CeFinish {
   bool mean, set_gscale;
   const float* grad_scale;
   float *loss, *gscale;
-  unsigned long long* correct;
+  float* loss_sum;
+  unsigned long long *counted, *correct;
   double* partial;
   unsigned* done;
   int first_group, total_groups;

@@ -209,6 +209,8 @@ __device__ __forceinline__ void total_sums(const CeFinish& f) {
   const double share = share_of(f.mean, v[1]);
   *f.loss = (float)(v[0] * share);
   if (f.set_gscale) *f.gscale = (float)(share * (f.grad_scale ? (double)*f.grad_scale : 1.0));
+  if (f.loss_sum) *f.loss_sum += (float)v[0];
+  if (f.counted) *f.counted += (unsigned long long)v[1];
   if (f.correct) *f.correct += (unsigned long long)v[2];
 }
 

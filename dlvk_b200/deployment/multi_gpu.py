@@ -132,21 +132,14 @@ class MultiGPUTrainer:
             for x, y in self._accumulated(train_loader):
                 self._step(x, y)(x, y)
                 nb += 1
-            loss_sum = correct = samples = rows = 0.0
-            for st in self._steps.values():
-                r = st.rows
-                l_, a_, n_ = st.epoch_metrics()
-                loss_sum += l_ * n_
-                correct += a_ * r
-                samples += n_
-                rows += r
+            totals = list(map(sum, zip((0,) * 5, *(st.epoch_totals() for st in self._steps.values()))))
             if self.model.dev.is_cuda:
                 torch.cuda.synchronize(self.model.dev.device)
             dt = time.perf_counter() - t0
-            tot = self._reduce([loss_sum, correct, samples, rows])
-            m = TrainingMetrics(loss=tot[0] / max(tot[2], 1), accuracy=tot[1] / max(tot[3], 1), epoch=epoch,
+            loss_sum, weight, correct, rows, samples = self._reduce(totals)
+            m = TrainingMetrics(loss=loss_sum / max(weight, 1), accuracy=correct / max(rows, 1), epoch=epoch,
                                 learning_rate=self.optimizer.get_learning_rate(), epoch_time_ms=dt * 1e3,
-                                samples_per_s=tot[2] / dt if dt > 0 else 0.0)
+                                samples_per_s=samples / dt if dt > 0 else 0.0)
             self.stats.total_batches += nb
             self.stats.sync_operations += nb * (len(self.dp.buckets) if self.dp else 0)
             self.stats.computation_time += dt
@@ -168,9 +161,8 @@ class MultiGPUTrainer:
         with torch.no_grad():
             for x, y in loader:
                 if getattr(self.loss_fn, "fuses_head", False):
-                    loss, hits, seen = self.model.head_loss(x, y, self.loss_fn)
-                    loss_sum, n = loss_sum + float(loss) * x.shape[0], n + x.shape[0]
-                    correct, rows = correct + hits, rows + seen
+                    loss, hits, seen = self.model.head_loss_totals(x, y, self.loss_fn)
+                    loss_sum, n, correct, rows = loss_sum + loss, n + seen, correct + hits, rows + seen
                     continue
                 out = self.model.forward_logits(x) if fused else self.model.forward(x)
                 yd = y.to(out.device)

@@ -113,11 +113,13 @@ class LinearCrossEntropyLoss(LossFunction):
             hidden, target = hidden.reshape(-1, hidden.shape[-1]), target.reshape(-1)
         return hidden, target
 
-    def forward(self, hidden, weight, target, bias=None, correct=None):
-        """The loss alone: a scalar, or with reduction "none" each row's (0 where it does not count)."""
+    def forward(self, hidden, weight, target, bias=None, correct=None, counted=None):
+        """The loss alone: a scalar, or with reduction "none" each row's (0 where it does not count).
+        `counted` and `correct` (int64 device scalars) are increased by the rows that count and by
+        those of them whose target has the largest logit."""
         x, t = self._rows(hidden, target)
         loss, rows, _, _, _ = K.linear_ce(x, _unwrap(weight), t, _unwrap(bias), self.ignore_index,
-                                          self.reduction != "sum", False, correct=correct)
+                                          self.reduction != "sum", False, correct=correct, counted=counted)
         return rows.reshape(_unwrap(target).shape) if self.reduction == "none" else loss
 
     def __call__(self, hidden, weight, target, bias=None):
@@ -133,9 +135,10 @@ class LinearCrossEntropyLoss(LossFunction):
                                           self.reduction == "mean", True, grad_scale)
         return loss, dx.reshape(_unwrap(hidden).shape), dw, db
 
-    def head_backward(self, head, hidden, target, grad_scale=None, correct=None):
+    def head_backward(self, head, hidden, target, grad_scale=None, correct=None, counted=None, loss_sum=None):
         """(loss, dhidden) for a Dense layer `head`, whose parameters receive
-        their gradients (and whose grad-ready hooks fire)."""
+        their gradients (and whose grad-ready hooks fire).  `counted`, `correct`
+        and `loss_sum` as in ops.core.linear_ce."""
         if self.reduction == "none":
             raise ValueError("training needs reduction mean or sum")
         x, t = self._rows(hidden, target)
@@ -143,7 +146,8 @@ class LinearCrossEntropyLoss(LossFunction):
         loss, _, dx, _, _ = K.linear_ce(
             x, W.value, t, b.master if b is not None else None, self.ignore_index, self.reduction == "mean", True,
             grad_scale, dw_out=W.grad, dw_accumulate=W.take_accumulate_flag(), db_out=b.grad if b is not None else None,
-            db_accumulate=b.take_accumulate_flag() if b is not None else False, correct=correct)
+            db_accumulate=b.take_accumulate_flag() if b is not None else False, correct=correct, counted=counted,
+            loss_sum=loss_sum)
         W.grad_ready()
         if b is not None:
             b.grad_ready()

@@ -330,13 +330,15 @@ class Sequential(Model):
             h = h.to(head.compute_dtype)
         return head, h, deferred
 
-    def head_loss_backward(self, x, y, loss_fn, grad_scale=None, correct=None):
+    def head_loss_backward(self, x, y, loss_fn, grad_scale=None, correct=None, counted=None, loss_sum=None):
         """Forward, loss and backward with a loss that takes the head
-        (LinearCrossEntropyLoss); returns the loss as a device scalar."""
+        (LinearCrossEntropyLoss); returns the loss as a device scalar.
+        `counted`, `correct` and `loss_sum`, where given, are increased as
+        ops.core.linear_ce says."""
         head, h, deferred = self._forward_hidden(x)
         self._last_out = None  # there are no logits for a later backward()
         y = y.to(h.device)
-        loss, dh = loss_fn.head_backward(head, h, y, grad_scale, correct)
+        loss, dh = loss_fn.head_backward(head, h, y, grad_scale, correct, counted, loss_sum)
         if h.requires_grad:
             if deferred:
                 dh = K.binary(dh, h.detach(), K.BIN_RELU_BWD)
@@ -345,14 +347,23 @@ class Sequential(Model):
         return loss
 
     def head_loss(self, x, y, loss_fn):
-        """(loss, correct rows, rows) of a batch without a gradient."""
+        """(loss, correct rows, rows) of a batch without a gradient; rows
+        whose target does not count are not among them."""
         if loss_fn.reduction == "none":
             raise ValueError("evaluation needs reduction mean or sum")
         head, h, _ = self._forward_hidden(x)
-        correct = torch.zeros(1, dtype=torch.int64, device=h.device)
+        seen = torch.zeros(2, dtype=torch.int64, device=h.device)
         loss = loss_fn.forward(h, head.weight.value, y.to(h.device), head.bias.master if head.bias is not None else None,
-                               correct=correct)
-        return loss, int(correct), y.numel()
+                               correct=seen[:1], counted=seen[1:])
+        correct, rows = seen.tolist()
+        return loss, correct, rows
+
+    def head_loss_totals(self, x, y, loss_fn):
+        """(sum of the losses, correct rows, rows) over the rows of a batch that
+        count, whichever reduction the loss has: what an evaluation over
+        batches of unequal padding adds up before it divides."""
+        loss, correct, rows = self.head_loss(x, y, loss_fn)
+        return float(loss) * (rows if loss_fn.reduction == "mean" else 1), correct, rows
 
     def backward(self, grad_output):
         """Backpropagate `grad_output` (gradient w.r.t. the last forward output)."""

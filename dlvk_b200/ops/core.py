@@ -281,7 +281,7 @@ def softmax_ce(logits: torch.Tensor, target: torch.Tensor, grad_scale: float = 1
 
 def linear_ce(hidden: torch.Tensor, weight: torch.Tensor, target: torch.Tensor, bias=None, ignore_index=None,
               mean: bool = True, want_grad: bool = True, grad_scale=None, dw_out=None, dw_accumulate: bool = False,
-              db_out=None, db_accumulate: bool = False, correct=None):
+              db_out=None, db_accumulate: bool = False, correct=None, counted=None, loss_sum=None):
     """Softmax cross entropy of hidden [N, E] @ weight [E, V] + bias without
     an [N, V] array of logits.  Returns (loss, rows, dhidden, dweight, dbias):
     the mean (or sum) over the rows that count and each row's own loss in
@@ -291,12 +291,13 @@ def linear_ce(hidden: torch.Tensor, weight: torch.Tensor, target: torch.Tensor, 
 
     weight may be the transpose of a [V, E] table; dweight has its layout and
     type, or goes to dw_out (fp32, `dw_accumulate` adds).  dbias is fp32.
-    `correct` (int64) is increased by the rows whose target has the largest
-    logit.  On the GPU: csrc/aten/linear_ce.cpp, bf16 and fp32."""
+    Where given, `counted` (int64) is increased by the rows that count,
+    `correct` (int64) by those whose target has the largest logit, `loss_sum`
+    (fp32) by the sum of their losses.  On the GPU: csrc/aten/linear_ce.cpp, bf16 and fp32."""
     ignore = -1 if ignore_index is None else int(ignore_index)
     if native(hidden):
         return N().linear_ce(hidden, weight, target, bias, ignore, mean, want_grad, grad_scale, dw_out, dw_accumulate,
-                             db_out, db_accumulate, correct)
+                             db_out, db_accumulate, correct, counted, loss_sum)
     hidden, weight = hidden.detach(), weight.detach()
     n, classes = hidden.shape[0], weight.shape[1]
     if hidden.dim() != 2 or weight.dim() != 2 or weight.shape[0] != hidden.shape[1] or classes < 1:
@@ -308,8 +309,8 @@ def linear_ce(hidden: torch.Tensor, weight: torch.Tensor, target: torch.Tensor, 
     if bias is not None and tuple(bias.shape) != (classes,):
         raise ValueError(f"linear_ce: bias must be [{classes}], got {tuple(bias.shape)}")
     lab = target.long()
-    counted = (lab >= 0) & (lab < classes) & (lab != ignore)
-    x, w, at = hidden.float()[counted], weight.float(), lab[counted]
+    keep = (lab >= 0) & (lab < classes) & (lab != ignore)
+    x, w, at = hidden.float()[keep], weight.float(), lab[keep]
     z = x @ w
     if bias is not None:
         z = z + bias.float()
@@ -318,18 +319,22 @@ def linear_ce(hidden: torch.Tensor, weight: torch.Tensor, target: torch.Tensor, 
     total = e.sum(-1, keepdim=True)
     zl = z.gather(1, at[:, None])[:, 0]
     rows = torch.zeros(n)
-    rows[counted] = top[:, 0] - zl + torch.log(total[:, 0])
-    share = (1.0 / max(int(counted.sum()), 1)) if mean else 1.0
+    rows[keep] = top[:, 0] - zl + torch.log(total[:, 0])
+    share = (1.0 / max(at.numel(), 1)) if mean else 1.0
     loss = rows.sum() * share
     if correct is not None:
         correct += (zl >= z.amax(-1)).sum() if zl.numel() else 0
+    if counted is not None:
+        counted += at.numel()
+    if loss_sum is not None:
+        loss_sum += rows.sum()
     if not want_grad:
         return loss, rows, None, None, None
     dz = e / total
     dz[torch.arange(at.numel()), at] -= 1.0
     dz *= share * (1.0 if grad_scale is None else float(grad_scale))
     dx = torch.zeros_like(hidden)
-    dx[counted] = (dz @ w.t()).to(hidden.dtype)
+    dx[keep] = (dz @ w.t()).to(hidden.dtype)
 
     def put(value, out, accumulate, like):
         if out is None:

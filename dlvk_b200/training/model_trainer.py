@@ -62,16 +62,8 @@ class ModelTrainer:
 
     def collect_metrics(self):
         """(mean loss, accuracy, samples) over every step since the last call."""
-        loss = acc_rows = 0.0
-        n = rows = 0
-        for st in self._steps.values():
-            r = st.rows
-            m_loss, m_acc, m_n = st.epoch_metrics()
-            loss += m_loss * m_n
-            acc_rows += m_acc * r
-            n += m_n
-            rows += r
-        return loss / max(n, 1), acc_rows / max(rows, 1), n
+        loss, weight, correct, rows, n = map(sum, zip((0,) * 5, *(st.epoch_totals() for st in self._steps.values())))
+        return loss / max(weight, 1), correct / max(rows, 1), n
 
     @staticmethod
     def split_data(x, y, validation_split: float):
@@ -155,10 +147,8 @@ class ModelTrainer:
         with torch.no_grad():
             for xb, yb in self.create_batches(x_test, y_test, batch_size):
                 if getattr(self.loss_function, "fuses_head", False):
-                    loss, hits, rows = self.model.head_loss(xb, yb, self.loss_function)
-                    tot_loss += float(loss) * xb.shape[0]
-                    correct += hits * xb.shape[0] / max(rows, 1)  # per sample: its rows' mean
-                    total += xb.shape[0]
+                    loss, hits, rows = self.model.head_loss_totals(xb, yb, self.loss_function)
+                    tot_loss, correct, total = tot_loss + loss, correct + hits, total + rows  # rows that count
                     continue
                 out = self.model.forward_logits(xb) if fused else self.model.forward(xb)
                 yb_d = yb.to(out.device)

@@ -29,7 +29,9 @@ class TrainStep:
     `regularizer` (a RegularizationManager) adds fused L1/L2 penalty
     gradients, `metrics=True` accumulates loss x batch and the number of
     correct argmax predictions into device counters (`epoch_metrics()` reads
-    and resets them) -- all inside the captured graph."""
+    and resets them) -- all inside the captured graph.  With a loss that takes
+    the head, whose rows need not all count, the counters hold the counted
+    rows' losses, their number and the correct ones among them."""
 
     def __init__(self, model, loss_fn, optimizer, dp=None, graph: bool = True, warmup_eager: int = 2,
                  scaler=None, regularizer=None, metrics: bool = False, overlap_update: Optional[bool] = None):
@@ -62,6 +64,8 @@ class TrainStep:
         dev = model.dev.device
         self.loss_sum = torch.zeros(1, dtype=torch.float32, device=dev) if metrics else None
         self.correct = torch.zeros(1, dtype=torch.int64, device=dev) if metrics else None
+        self._heads = bool(getattr(loss_fn, "fuses_head", False))
+        self.counted = torch.zeros(1, dtype=torch.int64, device=dev) if metrics and self._heads else None
         self.samples = 0
         self.rows = 0
         self.use_graph = bool(graph) and model.dev.is_cuda
@@ -81,11 +85,10 @@ class TrainStep:
         m.dev.advance_step()
         if self.dp is not None:
             self.dp.begin_step()
-        if getattr(self.loss_fn, "fuses_head", False):
+        if self._heads:
             loss = m.head_loss_backward(self.x, self.y, self.loss_fn,
-                                        self.scaler.scale if self.scaler is not None else None, self.correct)
-            if self.metrics:
-                self.loss_sum.add_(loss.reshape(1), alpha=float(self.x.shape[0]))
+                                        self.scaler.scale if self.scaler is not None else None, self.correct,
+                                        self.counted, self.loss_sum)
         else:
             fused = getattr(self.loss_fn, "fuses_softmax", False) and m.has_trailing_softmax()
             out = m.forward_logits(self.x) if fused else m.forward(self.x)
@@ -128,19 +131,30 @@ class TrainStep:
                 lab = y.reshape(rows, -1).argmax(-1) if y.is_floating_point() else y.reshape(rows).long()
                 self.correct += (pred == lab).sum()
 
-    def epoch_metrics(self, reset: bool = True):
-        """(mean loss per sample, accuracy per predicted row, samples) since
-        the last reset; one D2H read."""
+    def epoch_totals(self, reset: bool = True):
+        """(loss total, its weight, correct rows, rows, samples) since the last
+        reset: sums, for callers that add up several steps before they divide.
+        The weight is the samples, or with a loss that takes the head the rows
+        that counted.  One D2H read."""
         if not self.metrics:
             raise RuntimeError("TrainStep(metrics=True) is required")
-        vals = torch.stack([self.loss_sum.double().reshape(()), self.correct.double().reshape(())]).cpu()
-        out = (float(vals[0]) / max(self.samples, 1), float(vals[1]) / max(self.rows, 1), self.samples)
+        device = [self.loss_sum, self.correct] + ([self.counted] if self._heads else [])
+        loss, correct, *counted = torch.cat([t.double() for t in device]).tolist()
+        rows = int(counted[0]) if self._heads else self.rows
+        out = (loss, rows if self._heads else self.samples, correct, rows, self.samples)
         if reset:
-            self.loss_sum.zero_()
-            self.correct.zero_()
+            for t in device:
+                t.zero_()
             self.samples = 0
             self.rows = 0
         return out
+
+    def epoch_metrics(self, reset: bool = True):
+        """(mean loss per sample, accuracy per predicted row, samples) since
+        the last reset; with a loss that takes the head the mean loss and the
+        accuracy of the rows that counted.  One D2H read."""
+        loss, weight, correct, rows, samples = self.epoch_totals(reset)
+        return loss / max(weight, 1), correct / max(rows, 1), samples
 
     # ---------------------------------------------------------------- staging
     def stage(self, x: torch.Tensor, y: torch.Tensor) -> None:

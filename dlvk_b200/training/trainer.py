@@ -76,16 +76,8 @@ class Trainer:
         return m
 
     def _collect(self):
-        loss = acc_rows = 0.0
-        n = rows = 0
-        for st in self._steps.values():
-            r = st.rows
-            l_, a_, n_ = st.epoch_metrics()
-            loss += l_ * n_
-            acc_rows += a_ * r
-            n += n_
-            rows += r
-        return loss / max(n, 1), acc_rows / max(rows, 1), n
+        loss, weight, correct, rows, n = map(sum, zip((0,) * 5, *(st.epoch_totals() for st in self._steps.values())))
+        return loss / max(weight, 1), correct / max(rows, 1), n
 
     def fit(self, train_loader, val_loader=None, epochs: int = 1, verbose: bool = True) -> List[TrainingMetrics]:
         if verbose and not any(isinstance(c, ProgressCallback) for c in self.callbacks):
@@ -132,9 +124,8 @@ class Trainer:
         with torch.no_grad():
             for x, y in batches:
                 if getattr(self.loss_fn, "fuses_head", False):
-                    loss, hits, seen = self.model.head_loss(x, y, self.loss_fn)
-                    tot, n = tot + float(loss) * x.shape[0], n + x.shape[0]
-                    correct, rows = correct + hits, rows + seen
+                    loss, hits, seen = self.model.head_loss_totals(x, y, self.loss_fn)
+                    tot, n, correct, rows = tot + loss, n + seen, correct + hits, rows + seen
                     continue
                 out = self.model.forward_logits(x) if fused else self.model.forward(x)
                 yd = y.to(out.device)
