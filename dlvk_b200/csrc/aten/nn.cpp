@@ -449,7 +449,8 @@ at::Tensor embedding_grad_op(const at::Tensor& ids, const at::Tensor& dy, int64_
   const int64_t D = dy.size(-1);
   TORCH_CHECK(V >= 0, "dlvk.embedding_grad: num_embeddings ", V);
   TORCH_CHECK(D < (1LL << 31) - 4096, "dlvk.embedding_grad: rows of ", D, " elements");
-  TORCH_CHECK(n < (1LL << 31) - 1024 && V < (1LL << 31) - 1024, "dlvk.embedding_grad: more than 2^31 tokens or words");
+  TORCH_CHECK(n < EMBEDDING_GRAD_TOKENS && V < (1LL << 31) - 1024, "dlvk.embedding_grad: ", n, " tokens, ", V,
+              " words; at most ", EMBEDDING_GRAD_TOKENS - 1, " and ", (1LL << 31) - 1025);
   c10::cuda::CUDAGuard g(dy.device());
   at::AutoDispatchBelowADInplaceOrView below;
   at::Tensor dt;

@@ -454,7 +454,7 @@ void embedding_grad(DType dt, bool ids64, const void* ids, const void* dy, int64
                     int64_t V, int D, float scale, int64_t padding, bool accumulate, int* start, int* order, int* word,
                     float* part, cudaStream_t s) {
   if (V == 0 || D == 0) return;
-  DLVK_CHECK(n < (1LL << 31) - 1024 && V < (1LL << 31) - SORT_WORDS, "embedding_grad: more than 2^31 tokens or words");
+  DLVK_CHECK(n < EMBEDDING_GRAD_TOKENS && V < (1LL << 31) - SORT_WORDS, "embedding_grad: more than 2^31 tokens or words");
   // words of a block: all 148 SMs, at least 8 each, at most what its counts have room for
   const int R = (int)std::min<int64_t>(SORT_WORDS, std::max<int64_t>(8, (V + 147) / 148));
   const int blocks = (int)((V + R - 1) / R);
