@@ -18,6 +18,10 @@ namespace {
 int64_t round_up(int64_t n, int64_t a) { return (n + a - 1) / a * a; }
 int64_t ceil_div(int64_t n, int64_t a) { return (n + a - 1) / a; }
 
+// Rows of one launch: every pass covers at least 32 of them with one of the
+// 65535 blocks of a grid's second dimension.
+constexpr int64_t GRID_ROWS = 1LL << 20;
+
 // A matrix whose rows (one of its two strides is 1) can be read 16 bytes at
 // a time; otherwise a copy that can, in the same orientation.
 at::Tensor rows_of_16(const at::Tensor& t) {
@@ -108,7 +112,7 @@ void product(const Operand& A, const Operand& B, const Out& out, const float* sc
   if (A.type == at::kFloat && out.type == at::kFloat) {
     const float *pa = reinterpret_cast<const float*>(A.p), *pb = reinterpret_cast<const float*>(B.p);
     float* po = reinterpret_cast<float*>(out.p);
-    if (A.rows <= FEW_ROWS && A.cs == 1 && (B.cs == 1 || B.rs == 1) && !accumulate) {
+    if (A.rows <= FEW_ROWS && A.cols <= FEW_ROWS_K && A.cs == 1 && (B.cs == 1 || B.rs == 1) && !accumulate) {
       const bool turned = B.cs != 1;
       const int64_t n = few_rows_scratch_floats(A.rows, A.cols, B.cols, turned);
       const at::Tensor ws = n > 0 ? at::empty({n}, f32) : at::Tensor();
@@ -121,9 +125,14 @@ void product(const Operand& A, const Operand& B, const Out& out, const float* sc
       return;
     }
   }
-  const int64_t n = gemm_simt_workspace_floats(a);
-  const at::Tensor ws = n > 0 ? at::empty({n}, f32) : at::Tensor();
-  gemm_simt(dtype_of(A.type), odt, a, stream(), n > 0 ? ws.data_ptr<float>() : nullptr, n);
+  for (int64_t r = 0; r < A.rows; r += GRID_ROWS) {  // more rows than a launch has blocks for
+    a.M = std::min<int64_t>(GRID_ROWS, A.rows - r);
+    a.A = A.p + r * A.rs * (int64_t)c10::elementSize(A.type);
+    a.C = out.p + r * out.ld * (int64_t)c10::elementSize(out.type);
+    const int64_t n = gemm_simt_workspace_floats(a);
+    const at::Tensor ws = n > 0 ? at::empty({n}, f32) : at::Tensor();
+    gemm_simt(dtype_of(A.type), odt, a, stream(), n > 0 ? ws.data_ptr<float>() : nullptr, n);
+  }
 }
 
 // dst (+)= scale * A B.  On the tensor cores output rows that are no whole
@@ -146,16 +155,16 @@ void product_into(const Operand& A, const Operand& B, const Out& dst, const floa
               accumulate, stream());
 }
 
-// Rows of one block: `room` elements of [rows, classes], at least 2048 (every
-// block reads and writes the fp32 sums of dW once: 8 bytes per element of W
-// for 6 flops per row and element, 14% of the products' time at 2048), in
-// equal blocks of whole tiles.
-int64_t block_of(int64_t rows, int64_t classes, int64_t room) {
-  const int64_t most = std::max<int64_t>(2048, room / classes);
+}  // namespace
+
+// Rows of one block: `room` elements of [rows, classes] (rows of whole lines
+// of 64), at least 2048 (every block reads and writes the fp32 sums of dW once:
+// 8 bytes per element of W for 6 flops per row and element, 14% of the products'
+// time at 2048) and at most GRID_ROWS, in equal blocks of whole tiles.
+int64_t linear_ce_block_rows(int64_t rows, int64_t classes, int64_t room) {
+  const int64_t most = std::min(GRID_ROWS, std::max<int64_t>(2048, room / round_up(classes, 64)));
   return std::min(rows, round_up(ceil_div(rows, ceil_div(rows, most)), 256));
 }
-
-}  // namespace
 
 LinearCeResult linear_ce_op(const at::Tensor& x, const at::Tensor& w, const at::Tensor& target,
                             c10::optional<at::Tensor> bias, int64_t ignore_index, bool mean, bool want_grad,
@@ -299,7 +308,7 @@ LinearCeResult linear_ce_op(const at::Tensor& x, const at::Tensor& w, const at::
 
   // 256 MB of a block's exponentials, gradients or logits; the loss alone
   // keeps a 32nd of that on the tensor cores, the statistics
-  const int64_t rows = block_of(N, V, !fused ? (64LL << 20) : want_grad ? (128LL << 20) : (1LL << 30));
+  const int64_t rows = linear_ce_block_rows(N, V, !fused ? (64LL << 20) : want_grad ? (128LL << 20) : (1LL << 30));
   const int64_t blocks = ceil_div(N, rows);
   const auto stat_cols_of = [&](int64_t n) { return fused ? ce_tc_stat_cols(n, V, parts) : ce_memory_stat_cols(n, V); };
   // a last, smaller block may be cut into more statistics for each of fewer rows

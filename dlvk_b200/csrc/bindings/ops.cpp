@@ -63,6 +63,7 @@ void register_ops(py::module& m) {
      py::arg("dw_out") = py::none(), py::arg("dw_accumulate") = false, py::arg("db_out") = py::none(),
      py::arg("db_accumulate") = false, py::arg("correct") = py::none(), py::arg("counted") = py::none(),
      py::arg("loss_sum") = py::none());
+  m.def("linear_ce_block_rows", &linear_ce_block_rows, py::arg("rows"), py::arg("classes"), py::arg("room"));
   m.def("gemm_tc_ok", &gemm_tc_ok);
   m.def("gemm_tf32_ok", &gemm_tf32_ok);
   m.def("set_fp32_gemm_mode", &set_fp32_gemm_mode);

@@ -44,6 +44,7 @@ struct LinearCeResult {
   at::Tensor loss, rows, dx, dw, dbias;  // gradients undefined where not asked for
 };
 LinearCeResult linear_ce_op(const at::Tensor& x, const at::Tensor& w, const at::Tensor& target, c10::optional<at::Tensor> bias, int64_t ignore_index, bool mean, bool want_grad, c10::optional<at::Tensor> grad_scale, c10::optional<at::Tensor> dw_out, bool dw_accumulate, c10::optional<at::Tensor> db_out, bool db_accumulate, c10::optional<at::Tensor> correct, c10::optional<at::Tensor> counted, c10::optional<at::Tensor> loss_sum);
+int64_t linear_ce_block_rows(int64_t rows, int64_t classes, int64_t room);
 bool gemm_tc_ok(const at::Tensor& A, const at::Tensor& B);
 void optim_advance_op(const at::Tensor& hyper);
 void optim_update_op(int64_t kind, const at::Tensor& hyper, const at::Tensor& p, const at::Tensor& grad, c10::optional<at::Tensor> m, c10::optional<at::Tensor> v, c10::optional<at::Tensor> p_bf16, double extra_scale, int64_t max_ctas);

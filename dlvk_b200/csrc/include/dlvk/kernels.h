@@ -403,6 +403,7 @@ void copy_matrix(DType dst_dt, DType src_dt, const void* src, int64_t rs, int64_
 
 // ---- fp32 products with few rows (few_rows.cu) ---------------------------------
 constexpr int FEW_ROWS = 16;
+constexpr int64_t FEW_ROWS_K = 65535LL * 1024;  // longest K: a turned product has a block row for each 1024 of it
 // out [rows, cols] = A [rows, K] B (+ bias per column), rows <= FEW_ROWS; B is
 // [K, cols] with contiguous rows ldb apart, or (turned) its transpose is.
 // scratch: few_rows_scratch_floats() floats.

@@ -326,7 +326,8 @@ int64_t few_rows_scratch_floats(int64_t rows, int64_t K, int64_t cols, bool turn
 
 void few_rows_product(const float* A, int64_t lda, const float* B, int64_t ldb, bool turned, const float* bias,
                       float* out, int64_t ldo, int64_t rows, int64_t K, int64_t cols, float* scratch, cudaStream_t s) {
-  DLVK_CHECK(rows >= 1 && rows <= FEW_ROWS, "few_rows_product: rows");
+  static_assert(KT == 1024, "FEW_ROWS_K");
+  DLVK_CHECK(rows >= 1 && rows <= FEW_ROWS && K <= FEW_ROWS_K, "few_rows_product: size");
   DLVK_CHECK(scratch != nullptr || few_rows_scratch_floats(rows, K, cols, turned) == 0, "few_rows_product: scratch");
   const bool vec = al16(B) && ldb % 4 == 0 && (turned ? K : cols) % 4 == 0;
   const int n = (int)rows;

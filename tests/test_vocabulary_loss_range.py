@@ -68,3 +68,62 @@ def test_rows_whose_word_is_certain(device, dtype, n, v, bias, high):
     assert float(loss) >= 0 and abs(float(loss) - float(want.mean())) <= float(lim.mean()) + 2.0 ** -24 * float(loss)
     if high > 104:
         assert float(loss) == 0.0 and not dx.any() and not dw.any() and (db is None or not db.any())
+
+
+@pytest.mark.parametrize("room", [1 << 26, 1 << 27, 1 << 30])  # fp32 logits, exponentials, statistics alone
+@pytest.mark.parametrize("classes", [1, 2, 5, 15, 63, 64, 65, 127, 1000, 4096, 50257, 65537, 151936, 2 ** 30 - 1])
+def test_blocks_of_rows_fit_every_launch(classes, room):
+    """Passes over a block have a grid of rows / 32 or rows / 64 in its second dimension: at most 65535."""
+    f = dl._ext.C().linear_ce_block_rows
+    for rows in (1, 31, 255, 2048, 2049, 2 ** 20 - 1, 2 ** 20 + 1, 2 ** 21, 2 ** 22, 4470000, 2 ** 26, 2 ** 31 - 257):
+        n = f(rows, classes, room)
+        assert 1 <= n <= rows and (n == rows or n % 256 == 0)
+        assert -(-n // 32) <= 65535
+        line = -(-classes // 64) * 64
+        # equal blocks of whole tiles: at most a tile's rows above the room
+        assert n * line <= max(2048 * line, room) + 256 * line
+
+
+def in_parts(x, w, t, b, parts):
+    """What `check` compares, with the 64-bit values made of a part of the rows at a time."""
+    loss, dx, dw, db = dl.LinearCrossEntropyLoss("sum").value_and_grad(x, w, t, b)
+    rows = dl.LinearCrossEntropyLoss("none").forward(x, w, t, b)
+    n, total = x.shape[0], {}
+    for i in range(parts):
+        s = slice(i * n // parts, (i + 1) * n // parts)
+        want = exact(x[s], w, t[s], b, mean=False)
+        near(rows[s], want["rows"], "rows")
+        near(dx[s], want["dx"], "dx")
+        for k in ("loss", "dw", "db"):
+            value, lim = total.get(k, (0.0, 0.0))
+            # the whole sum has `parts` times the additions that a part's limit counts
+            total[k] = value + want[k][0], lim + parts * want[k][1]
+    near(loss, total["loss"], "loss")
+    near(dw, total["dw"], "dw")
+    if b is not None:
+        near(db, total["db"], "db")
+
+
+@pytest.mark.gpu
+def test_two_million_rows_of_64_words():
+    in_parts(*operands(2 ** 21, 16, 64, torch.bfloat16, "cuda"), 16)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_millions_of_rows_of_a_few_words(dtype):
+    """Logits by the SIMT product: 64 rows to a block."""
+    in_parts(*operands(4300000, 8, 5, dtype, "cuda", bias=True), 10)
+
+
+@pytest.mark.gpu
+def test_millions_of_words_of_a_few_numbers():
+    """dW of a tied table by the SIMT product: a row of it per word, 64 to a block."""
+    n, e, v = 20, 4, 4300000
+    x, w, t, _ = operands(n, e, v, torch.float32, "cuda", tied=True)
+    t[0] = v - 1
+    want = exact(x, w, t, None)
+    loss, dx, dw, _ = dl.LinearCrossEntropyLoss().value_and_grad(x, w, t)
+    near(loss, want["loss"], "loss")
+    near(dx, want["dx"], "dx")
+    near(dw, want["dw"], "dw")
