@@ -47,7 +47,8 @@ struct Operand {
   int64_t rows, cols, rs, cs;
   int64_t pitch = 0;
   at::ScalarType type;
-  Operand t() const { return {p, cols, rows, cs, rs, pitch, type}; }
+  int64_t done = 0;  // of its columns (or, on the right, rows) before p
+  Operand t() const { return {p, cols, rows, cs, rs, pitch, type, done}; }
 };
 // Rows [r0, r0 + n) of a row-major matrix with rows ld apart.
 Operand rows_operand(const at::Tensor& t, int64_t r0, int64_t n, int64_t cols, int64_t ld) {
@@ -101,6 +102,19 @@ void product(const Operand& A, const Operand& B, const Out& out, const float* sc
     a.ldr = before->ld;
     a.residual_f32 = true;
   }
+  if (a.parts && a.K > GEMM_PARTS_K) {  // pieces of K, each added to those before
+    const int64_t piece = round_up(ceil_div(a.K, ceil_div(a.K, GEMM_PARTS_K)), 64);
+    for (int64_t k = 0; k < A.cols; k += piece) {
+      Operand x = A, w = B;
+      x.p += 2 * k * A.cs;
+      w.p += 2 * k * B.rs;
+      x.cols = w.rows = std::min(piece, A.cols - k);
+      x.done = w.done = k;
+      product(x, w, out, scale, accumulate || k > 0, f32, k == 0 ? bias : nullptr);
+    }
+    return;
+  }
+  a.k_done = A.done;
   if (A.type == at::kBFloat16 && gemm_tc_supported(a)) {
     a.alpha_ptr = scale;
     const int64_t n = gemm_tc_workspace_floats(a, 0, odt);
@@ -303,7 +317,9 @@ LinearCeResult linear_ce_op(const at::Tensor& x, const at::Tensor& w, const at::
   // Where the logits are: in the accumulators (bf16, and the loss alone of
   // fp32 parts), else a block of them in memory as fp32.
   const bool tc_ok = (bf || parts) && E >= 16 && ce_tc_supported(c);
-  const bool fused = tc_ok && (bf || !want_grad);
+  // (fp32: while one accumulator may hold the whole width, which the epilogue
+  // that reduces the logits does not split)
+  const bool fused = tc_ok && (bf || (!want_grad && E <= GEMM_PARTS_ACC));
   const bool keep = fused && want_grad && !bias.has_value();  // exponentials kept, not made again
 
   // 256 MB of a block's exponentials, gradients or logits; the loss alone

@@ -101,10 +101,17 @@ struct GemmArgs {
   // their contiguous dimension, pitch_a / pitch_b (multiples of 64) elements
   // apart (split_parts): C = the fp32 product, as six bf16 ones.  The padding
   // of K is zero.  Tensor-core path; gemm_tc_workspace_floats() says what room
-  // its split-K takes, without which the sums are unsplit.
+  // its split-K takes, without which the sums are unsplit.  K is at most
+  // GEMM_PARTS_K; a longer product is a sum of such ones (beta = 1), whose
+  // pointers are k_done elements of K further on.
   bool parts = false;
-  int64_t pitch_a = 0, pitch_b = 0;
+  int64_t pitch_a = 0, pitch_b = 0, k_done = 0;
 };
+// The accumulators lose up to 2^-23 of themselves with every addition, always
+// towards zero (plain fp32 rounds, and errs to both sides), so that a product
+// in parts is as good as fp32 only while one accumulator sums few elements of K;
+// the rest is summed by the split-K reduction, of at most 32 splits.
+constexpr int64_t GEMM_PARTS_ACC = 1280, GEMM_PARTS_K = 32 * GEMM_PARTS_ACC;
 // SIMT GEMM.  With a workspace of gemm_simt_workspace_floats(a) floats, a
 // small 2-D GEMM with a plain epilogue splits K across blocks (fp32 partials,
 // then a finish kernel; deterministic).

@@ -1676,12 +1676,9 @@ void choose_tiling(const GemmArgs& a, int sms, int& BN, int& splits, bool& pair,
     for (int sp : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32}) {
       if (sp > 8 && !a.parts) break;
       if (sp > 1 && kbs * products / sp < 8) break;
-      // The accumulators lose a little with every addition (2^-24, always
-      // towards zero): at most 1280 elements of K for products that are to be
-      // as good as fp32, the rest is summed in the reduction (gradients of 768 x
-      // 512 x 10007 against 64 bits: 1.1e-6, plain fp32 1.8e-6; 0.9e-6 with 640,
-      // which costs 7% of the time).
-      if (a.parts && sp < 32 && (kbs + sp - 1) / sp > 20) continue;
+      // GEMM_PARTS_ACC elements of K to an accumulator at most (768 x 512 x
+      // 10007: 0.9e-6 off with half as many, which costs 7% of the time)
+      if (a.parts && (kbs + sp - 1) / sp > GEMM_PARTS_ACC / BK) continue;
       const int64_t units = tiles * sp;
       const int64_t waves = (units + slots - 1) / slots;
       const double unit_s = (double)tile_m * c.bn * BK * 2.0 * products * ((kbs + sp - 1) / sp) /
@@ -1855,6 +1852,7 @@ void gemm_tc_impl(DType out_dt, const GemmArgs& a, cudaStream_t s, uint32_t* err
   const Elem el = tf32 ? Elem::F32 : Elem::BF16;
   const int bke = tf32 ? BK / 2 : BK;
   if (a.M == 0 || a.N == 0) return;
+  DLVK_CHECK(!a.parts || a.K <= GEMM_PARTS_K, "gemm_tc: K of a product in parts");
   // The tensor-map encoder is a driver call and needs a current context on
   // this thread.  Threads that have only used the runtime through a "same
   // device" cudaSetDevice shortcut (e.g. PyTorch's autograd workers) may not
@@ -1918,7 +1916,7 @@ void gemm_tc_impl(DType out_dt, const GemmArgs& a, cudaStream_t s, uint32_t* err
   const uint64_t ab2 = a_bcast ? 1 : (uint64_t)a.batch2, ab = a_bcast ? 1 : (uint64_t)a.batch;
   if (a_k) {
     const uint64_t d = (uint64_t)a.sam * (uint64_t)a.M;
-    ta = make_tmap(a.A, a.parts ? 3 * a.pitch_a : a.K, a.M, ab2, ab, a.sam, pick((int64_t)ab2, a.batch2_stride_a, d),
+    ta = make_tmap(a.A, a.parts ? 3 * a.pitch_a - a.k_done : a.K, a.M, ab2, ab, a.sam, pick((int64_t)ab2, a.batch2_stride_a, d),
                    pick((int64_t)ab, a.batch_stride_a, d), BM, el);
   } else {
     const uint64_t d = (uint64_t)a.sak * (uint64_t)a.K;
@@ -1927,7 +1925,7 @@ void gemm_tc_impl(DType out_dt, const GemmArgs& a, cudaStream_t s, uint32_t* err
   }
   if (b_k) {
     const uint64_t d = (uint64_t)a.sbn * (uint64_t)a.N;
-    tb = make_tmap(a.B, a.parts ? 3 * a.pitch_b : a.K, a.N, a.batch2, a.batch, a.sbn, pick(a.batch2, a.batch2_stride_b, d),
+    tb = make_tmap(a.B, a.parts ? 3 * a.pitch_b - a.k_done : a.K, a.N, a.batch2, a.batch, a.sbn, pick(a.batch2, a.batch2_stride_b, d),
                         pick(a.batch, a.batch_stride_b, d), pair ? 128 : BN, el);
   } else {
     const uint64_t d = (uint64_t)a.sbk * (uint64_t)a.K;
