@@ -187,10 +187,10 @@ __device__ __forceinline__ double list_norm(const double* partial, int parts) {
   for (int i = threadIdx.x; i < parts; i += THREADS) acc += partial[i];
   return sqrt(block_sum_f64(acc));
 }
-// A norm that is not finite scales nothing: the caller sees it in the result.
+// A norm that is not finite as the caller gets it, in fp32, scales nothing.
 __device__ __forceinline__ float clip_coefficient(double norm, float max_norm) {
   const double c = (double)max_norm / (norm + 1e-6);
-  return (norm < INFINITY && c < 1.0) ? (float)c : 1.f;
+  return ((float)norm < INFINITY && c < 1.0) ? (float)c : 1.f;
 }
 
 __global__ void __launch_bounds__(THREADS) list_norm_kernel(const double* __restrict__ partial, int parts,

@@ -400,7 +400,7 @@ class GradientClipping:
         if grads and grads[0].is_cuda:
             return K.N().clip_global_norm(grads, float(max_norm), outs)
         norm = _cpu_norm(grads)
-        coef = min(1.0, float(max_norm) / (float(norm) + 1e-6)) if math.isfinite(norm) else 1.0
+        coef = min(1.0, float(max_norm) / (float(norm) + 1e-6)) if math.isfinite(norm.float()) else 1.0
         for g, o in zip(grads, grads if outs is None else outs):
             if g.shape != o.shape:
                 raise ValueError(f"clip_global_norm: a gradient is {tuple(g.shape)}, its output {tuple(o.shape)}")
