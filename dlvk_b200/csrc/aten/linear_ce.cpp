@@ -219,11 +219,21 @@ LinearCeResult linear_ce_op(const at::Tensor& x, const at::Tensor& w, const at::
                 "dlvk.linear_ce: the weight gradient must be fp32 (or, overwritten, of the weight's type) ", w.sizes(),
                 " with one unit stride on ", dev);
   if (dw_out.has_value()) {
-    TORCH_CHECK(V == 1 || E == 1 || dw_out->stride(1) + dw_out->stride(0) > (dw_out->stride(1) == 1 ? V : E),
+    const int64_t se = dw_out->stride(0), sv = dw_out->stride(1);
+    TORCH_CHECK((V == 1 || sv >= 1) && (E == 1 || se >= 1) && (V == 1 || E == 1 || sv + se > (sv == 1 ? V : E)),
                 "dlvk.linear_ce: the weight gradient repeats its elements, strides ", dw_out->strides());
-    at::assert_no_overlap(*dw_out, w);
-    at::assert_no_overlap(*dw_out, x);
   }
+  // blocks of rows write the gradients before the next ones read the operands
+  const auto apart = [&](const c10::optional<at::Tensor>& t) {
+    if (!t.has_value()) return;
+    at::assert_no_overlap(*t, w);
+    at::assert_no_overlap(*t, x);
+    at::assert_no_overlap(*t, target);
+    if (bias.has_value()) at::assert_no_overlap(*t, *bias);
+  };
+  apart(dw_out);
+  apart(db_out);
+  if (dw_out.has_value() && db_out.has_value()) at::assert_no_overlap(*dw_out, *db_out);
   if (db_out.has_value())
     TORCH_CHECK(bias.has_value() && db_out->scalar_type() == at::kFloat && db_out->is_contiguous() &&
                     db_out->numel() == V && db_out->device() == dev,

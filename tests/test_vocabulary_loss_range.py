@@ -10,6 +10,7 @@ import pytest
 import torch
 
 import dlvk_b200 as dl
+from dlvk_b200.ops import core as K
 from test_linear_cross_entropy import exact, near, operands
 
 DEVICES = [pytest.param("cpu"), pytest.param("cuda", marks=pytest.mark.gpu)]
@@ -127,3 +128,31 @@ def test_millions_of_words_of_a_few_numbers():
     near(loss, want["loss"], "loss")
     near(dx, want["dx"], "dx")
     near(dw, want["dw"], "dw")
+
+
+@pytest.mark.gpu
+def test_refusals_of_gradients_that_repeat_or_lie_on_operands():
+    x, w, t, b = operands(40, 1, 70, torch.float32, "cuda", bias=True)
+    with pytest.raises(RuntimeError, match="repeats"):  # one row, one element for all words
+        K.linear_ce(x, w, t, b, dw_out=torch.zeros(1, 1, device="cuda").expand(1, 70))
+    x, w, t, b = operands(40, 16, 1, torch.float32, "cuda", bias=True)
+    with pytest.raises(RuntimeError, match="repeats"):
+        K.linear_ce(x, w, t, b, dw_out=torch.zeros(1, 1, device="cuda").expand(16, 1))
+    out = torch.zeros(16, 3, device="cuda")[:, :1]  # rows apart: one column of a wider matrix
+    K.linear_ce(x, w, t, b, dw_out=out)
+    x, w, t, b = operands(40, 16, 70, torch.float32, "cuda", bias=True)
+    with pytest.raises(RuntimeError, match="memory"):
+        K.linear_ce(x, w, t, b, db_out=b)
+    with pytest.raises(RuntimeError, match="memory"):
+        K.linear_ce(x, w, t, b, db_out=w[0])
+    with pytest.raises(RuntimeError, match="memory"):
+        K.linear_ce(x, w, t, b, db_out=x.reshape(-1)[:70])
+    both = torch.zeros(16 * 70 + 70, device="cuda")
+    with pytest.raises(RuntimeError, match="memory"):
+        K.linear_ce(x, w, t, b, dw_out=both[:1120].view(16, 70), db_out=both[1100:1170])
+    with pytest.raises(RuntimeError, match="memory"):
+        K.linear_ce(x, w, t, both[1000:1070], dw_out=both[:1120].view(16, 70))
+    K.linear_ce(x, w, t, b, dw_out=both[:1120].view(16, 70), db_out=both[1120:])
+    want = exact(x, w, t, b)
+    near(both[:1120].view(16, 70), want["dw"], "dw")
+    near(both[1120:], want["db"], "db")
