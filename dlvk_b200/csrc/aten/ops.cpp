@@ -288,12 +288,10 @@ void gemm_tf32_op(const at::Tensor& A, const at::Tensor& B, at::Tensor& C, const
   GemmArgs lin = fill_args(sa.second, sb.first, C);
   lin.alpha = args.alpha;
   lin.beta = args.beta;
-  lin.ordered = args.ordered;
   run_tf32(lin, max_ctas, C);
   lin = fill_args(sa.first, sb.second, C);
   lin.alpha = args.alpha;
   lin.beta = 1.f;
-  lin.ordered = args.ordered;
   run_tf32(lin, max_ctas, C);
   GemmArgs last = args;
   const GemmArgs hh = fill_args(sa.first, sb.first, C);
@@ -345,7 +343,7 @@ at::Tensor gemm_op(const at::Tensor& A, const at::Tensor& B, c10::optional<at::T
                    int64_t force_path, int64_t max_ctas, c10::optional<at::Tensor> residual,
                    c10::optional<at::Tensor> relu_mask, c10::optional<at::Tensor> colsum_out,
                    double colsum_scale, bool colsum_accumulate, c10::optional<at::Tensor> relu_bits_out,
-                   c10::optional<at::Tensor> relu_bits, bool ordered) {
+                   c10::optional<at::Tensor> relu_bits) {
   check_cuda(A, "A");
   check_cuda(B, "B");
   TORCH_CHECK(A.scalar_type() == B.scalar_type(), "dlvk.gemm: A and B must have the same dtype");
@@ -369,7 +367,6 @@ at::Tensor gemm_op(const at::Tensor& A, const at::Tensor& B, c10::optional<at::T
   GemmArgs a = fill_args(A, B, C);
   a.alpha = (float)alpha;
   a.beta = (float)beta;
-  a.ordered = ordered;
   at::Tensor bc;
   if (bias.has_value()) {
     bc = bias->contiguous();

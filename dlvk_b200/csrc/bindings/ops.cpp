@@ -48,7 +48,7 @@ void register_ops(py::module& m) {
         py::arg("force_path") = 0, py::arg("max_ctas") = 0, py::arg("residual") = py::none(),
         py::arg("relu_mask") = py::none(), py::arg("colsum_out") = py::none(), py::arg("colsum_scale") = 1.0,
         py::arg("colsum_accumulate") = false, py::arg("relu_bits_out") = py::none(),
-        py::arg("relu_bits") = py::none(), py::arg("ordered") = false);
+        py::arg("relu_bits") = py::none());
   m.def("linear_ce", [](const at::Tensor& x, const at::Tensor& w, const at::Tensor& target,
                         c10::optional<at::Tensor> bias, int64_t ignore_index, bool mean, bool want_grad,
                         c10::optional<at::Tensor> grad_scale, c10::optional<at::Tensor> dw_out, bool dw_accumulate,
