@@ -449,8 +449,8 @@ at::Tensor embedding_grad_op(const at::Tensor& ids, const at::Tensor& dy, int64_
   const int64_t D = dy.size(-1);
   TORCH_CHECK(V >= 0, "dlvk.embedding_grad: num_embeddings ", V);
   TORCH_CHECK(D < (1LL << 31) - 4096, "dlvk.embedding_grad: rows of ", D, " elements");
-  TORCH_CHECK(n < EMBEDDING_GRAD_TOKENS && V < (1LL << 31) - 1024, "dlvk.embedding_grad: ", n, " tokens, ", V,
-              " words; at most ", EMBEDDING_GRAD_TOKENS - 1, " and ", (1LL << 31) - 1025);
+  TORCH_CHECK(n < EMBEDDING_GRAD_TOKENS && V < EMBEDDING_GRAD_WORDS, "dlvk.embedding_grad: ", n, " tokens, ", V,
+              " words; at most ", EMBEDDING_GRAD_TOKENS - 1, " and ", EMBEDDING_GRAD_WORDS - 1);
   c10::cuda::CUDAGuard g(dy.device());
   at::AutoDispatchBelowADInplaceOrView below;
   at::Tensor dt;
@@ -470,12 +470,13 @@ at::Tensor embedding_grad_op(const at::Tensor& ids, const at::Tensor& dy, int64_
   auto io = dy.options().dtype(at::kInt);
   const int64_t pf = embedding_grad_part_floats(n, (int)D);
   // one allocation: part first (16-byte aligned), then the three integer arrays
-  auto ws = at::empty({pf + V + 1 + 2 * n}, io);
+  const int64_t starts = embedding_grad_start_ints(V);
+  auto ws = at::empty({pf + starts + 2 * n}, io);
   int* base = ws.data_ptr<int>();
   int* start = base + pf;
   embedding_grad(to_dtype(dyc), idc.scalar_type() == at::kLong, idc.data_ptr(), dyc.data_ptr(),
                  dyc.dim() == 2 ? dyc.stride(0) : D, dt.data_ptr<float>(), n, V, (int)D, (float)scale, padding_idx,
-                 accumulate, start, start + V + 1, start + V + 1 + n, reinterpret_cast<float*>(base), stream());
+                 accumulate, start, start + starts, start + starts + n, reinterpret_cast<float*>(base), stream());
   return dt;
 }
 

@@ -428,11 +428,13 @@ void embedding_lookup(DType dt, bool ids64, const void* ids, const void* table, 
                       int64_t ld, float scale, cudaStream_t s);
 // dtable[v, :] (fp32 [V, D]) = (or, accumulate, +=) scale * sum of dy[i, :] over
 // ids[i] == v, in a fixed order; ids outside [0, V) and `padding` (-1: none)
-// have no gradient.  Scratch: start V + 1 ints, order and word n ints each,
+// have no gradient.  Scratch: start embedding_grad_start_ints(V) ints, order and word n ints each,
 // part embedding_grad_part_floats(n, D) floats.
-// Fewer tokens than this: the places of the last block's chunks, up to 256 of 64
-// places past the end, are ints.
-constexpr int64_t EMBEDDING_GRAD_TOKENS = (1LL << 31) - 32768;
+// Fewer tokens and words than these: the places of the last block's chunks, up to
+// 256 of 64 places past the end, are ints, and so are those of the words in the
+// sort, of which each of up to 2^21 blocks may have one without a word.
+constexpr int64_t EMBEDDING_GRAD_TOKENS = (1LL << 31) - 32768, EMBEDDING_GRAD_WORDS = (1LL << 31) - (1LL << 22);
+int64_t embedding_grad_start_ints(int64_t V);
 int64_t embedding_grad_part_floats(int64_t n, int D);
 void embedding_grad(DType dt, bool ids64, const void* ids, const void* dy, int64_t ld, float* dtable, int64_t n,
                     int64_t V, int D, float scale, int64_t padding, bool accumulate, int* start, int* order, int* word,

@@ -97,14 +97,29 @@ __device__ __forceinline__ void clear_span(float* p, int64_t floats) {
     *reinterpret_cast<float4*>(p + head + c) = make_float4(0.f, 0.f, 0.f, 0.f);
   if (head + body + lane < floats) p[head + body + lane] = 0.f;
 }
+// The order of the words in the sort: word v is the (v >> log)-th of block
+// v mod 2^log's `per` places.  Tokenizers number their words by frequency; blocks
+// of neighbouring words would leave the first one most of the tokens (65536
+// tokens x 1024 over 32000 words, word k as common as 1 / (k + 2.7): the sort 57 us,
+// dealt out 27).
+struct WordOrder {
+  int log, per;
+  __device__ __forceinline__ int at(int v) const { return (v & ((1 << log) - 1)) * per + (v >> log); }
+  __host__ __device__ __forceinline__ int places() const { return per << log; }
+};
+
 // A warp of `warps` takes every warps-th group of consecutive rows (about 4 KB,
 // at most 32) of [v0, v1) and clears the runs of rows without a token in it.
-__device__ __forceinline__ void clear_rows(const int* start, float* dtable, int v0, int v1, int D, int warp,
-                                           int warps) {
+__device__ __forceinline__ void clear_rows(const int* start, WordOrder words, float* dtable, int v0, int v1, int D,
+                                           int warp, int warps) {
   const int lane = threadIdx.x & 31, per = max(1, min(32, 1024 / D));
   for (int64_t v = v0 + (int64_t)warp * per; v < v1; v += (int64_t)warps * per) {
     const int rows = (int)min((int64_t)per, v1 - v);
-    const bool empty = lane < rows && start[v + lane] == start[v + lane + 1];
+    bool empty = false;
+    if (lane < rows) {
+      const int at = words.at((int)v + lane);
+      empty = start[at] == start[at + 1];
+    }
     unsigned left = __ballot_sync(0xffffffffu, empty);
     while (left) {
       const int first = __ffs(left) - 1, run = __ffs(~(left >> first)) - 1;  // run 32: ~0 has no bit, __ffs gives 0
@@ -116,8 +131,7 @@ __device__ __forceinline__ void clear_rows(const int* start, float* dtable, int 
 }
 
 // The word of token i < hi, -1 for none: past the end, padding, or an id that
-// no int holds (any other id outside [0, V) falls out of every block's range;
-// negative ones are kept negative).
+// no int holds (negative ones are kept negative).
 template <typename ID>
 __device__ __forceinline__ int word_at(const ID* ids, int i, int hi, int padding) {
   if (i >= hi) return -1;
@@ -128,25 +142,29 @@ __device__ __forceinline__ int word_at(const ID* ids, int i, int hi, int padding
 }
 
 // Stable sort of the tokens by word in one launch, without a word between
-// blocks.  Block b owns the words [b R, (b + 1) R) and reads all ids twice:
-// once to count its own words (per warp: warp w has the w-th part of the ids)
-// and the tokens of smaller words, which is where its part of the order
-// begins; once more to place its tokens.  A token's place is its word's
+// blocks.  Block b of B = 2^log owns the words b, b + B, b + 2 B, ... and reads all
+// ids twice: once to count its own words (per warp: warp w has the w-th part of
+// the ids) and the tokens of the blocks before it, which is where its part of
+// the order begins; once more to place its tokens.  Rotated right by log, an id has
+// its block in the upper bits and its place there in the lower ones, so that one
+// subtraction and comparison tell both.  A token's place is its word's
 // start + the counts of earlier warps + its rank among the warp's tokens so
 // far, so equal words stay in ascending position.  Every block reading all
-// ids costs 148 x 4 n bytes from L2 (8192 tokens: 5 MB), far less than the
+// ids costs 128 x 4 n bytes from L2 (8192 tokens: 4 MB), far less than the
 // passes over memory of a radix sort of so few keys.
-//   start[v], v in [0, V]: first place of word v; order[place]: the token.
+//   start[words.at(v)]: first place of word v, start[that + 1]: of what follows it;
+//   order[place]: the token.
 template <typename ID>
-__global__ void __launch_bounds__(SORT_THREADS) sort_tokens_kernel(const ID* __restrict__ ids, int n, int V, int R,
-                                                                   int padding, int* __restrict__ start,
+__global__ void __launch_bounds__(SORT_THREADS) sort_tokens_kernel(const ID* __restrict__ ids, int n, int V,
+                                                                   WordOrder words, int padding, int* __restrict__ start,
                                                                    int* __restrict__ order, int* __restrict__ word) {
   pdl_wait();
   extern __shared__ int cnt[];  // [SORT_WARPS][R], then [R]: a word's first place
   __shared__ int warp_part[SORT_WARPS];
   __shared__ int before_sm;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int v0 = blockIdx.x * R, v1 = min(V, v0 + R);
+  const int R = words.per, B = 1 << words.log, b = blockIdx.x;
+  const unsigned base0 = words.log > 0 ? (unsigned)b << (32 - words.log) : 0u;
   int* first = cnt + SORT_WARPS * R;
   const int per = (max(n, 1) + SORT_THREADS - 1) / SORT_THREADS * 32;  // ids of a warp, whole groups of 32
   const int used = (int)(((unsigned)n + per - 1) / per);               // warps that have any
@@ -156,17 +174,18 @@ __global__ void __launch_bounds__(SORT_THREADS) sort_tokens_kernel(const ID* __r
 
   const int lo = min((int64_t)n, (int64_t)warp * per), hi = min((int64_t)n, (int64_t)(warp + 1) * per);
   int* mine = cnt + warp * R;
-  const unsigned range = (unsigned)(v1 - v0);
+  const unsigned range = (unsigned)((V - b + B - 1) >> words.log);  // words of this block
   int before = 0;
-  unsigned key[8];  // id - v0 of the warp's last 256 ids: below `range` for this block's words
+  unsigned key[8];  // places of the warp's last 256 ids in this block: below `range` for its words
   for (int base = lo; base < hi; base += 256) {
     int id[8];
 #pragma unroll
     for (int k = 0; k < 8; ++k) id[k] = word_at(ids, base + k * 32 + lane, hi, padding);
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
-      before += (unsigned)id[k] < (unsigned)v0;  // -1 is never below
-      key[k] = (unsigned)id[k] - (unsigned)v0;
+      const unsigned turned = __funnelshift_r((unsigned)id[k], (unsigned)id[k], words.log);
+      before += turned < base0 && (unsigned)id[k] < (unsigned)V;
+      key[k] = turned - base0;
       if (key[k] < range) atomicAdd(&mine[key[k]], 1);
     }
   }
@@ -174,7 +193,7 @@ __global__ void __launch_bounds__(SORT_THREADS) sort_tokens_kernel(const ID* __r
   if (lane == 0 && before) atomicAdd(&before_sm, before);
   __syncthreads();
 
-  // Thread r scans word v0 + r's counts over the warps that have tokens, eight
+  // Thread r scans its word's counts over the warps that have tokens, eight
   // loads at a time (a warp to a word, with shuffles, took 16.6 us instead of
   // 6.4 for 200000 words, 6.0 instead of 5.2 for 2048 tokens over 32000), ...
   int total = 0;
@@ -210,9 +229,9 @@ __global__ void __launch_bounds__(SORT_THREADS) sort_tokens_kernel(const ID* __r
   }
   __syncthreads();
   const int at = before_sm + incl - total + (warp > 0 ? warp_part[warp - 1] : 0);
-  if (tid < R && v0 + tid < V) {
-    start[v0 + tid] = at;
-    if (v0 + tid == V - 1) start[V] = at + total;
+  if (tid < R) {  // places without a word have none of the tokens
+    start[b * R + tid] = at;
+    if (b == B - 1 && tid == R - 1) start[words.places()] = at + total;
   }
   if (tid < R) first[tid] = at;
   __syncthreads();
@@ -221,7 +240,10 @@ __global__ void __launch_bounds__(SORT_THREADS) sort_tokens_kernel(const ID* __r
   for (int base = lo; base < hi; base += 256) {
     if (!held) {
 #pragma unroll
-      for (int k = 0; k < 8; ++k) key[k] = (unsigned)word_at(ids, base + k * 32 + lane, hi, padding) - (unsigned)v0;
+      for (int k = 0; k < 8; ++k) {
+        const unsigned id = (unsigned)word_at(ids, base + k * 32 + lane, hi, padding);
+        key[k] = __funnelshift_r(id, id, words.log) - base0;
+      }
     }
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
@@ -231,7 +253,7 @@ __global__ void __launch_bounds__(SORT_THREADS) sort_tokens_kernel(const ID* __r
       if (hit) {
         const int place = first[key[k]] + mine[key[k]] + __popc(peers & ((1u << lane) - 1u));
         order[place] = base + k * 32 + lane;
-        word[place] = v0 + (int)key[k];
+        word[place] = (int)(key[k] << words.log) + b;
       }
       __syncwarp();
       if (hit && lane == __ffs(peers) - 1) mine[key[k]] += __popc(peers);
@@ -266,18 +288,18 @@ __device__ __forceinline__ void put_row(float* dst, const float* acc, float scal
 template <typename T, int VEC>
 __global__ void __launch_bounds__(RED_THREADS) sum_chunks_kernel(
     const T* __restrict__ dy, int64_t ld, const int* __restrict__ start, const int* __restrict__ order,
-    const int* __restrict__ word, float* __restrict__ dtable, float* __restrict__ part, int V, int D, int C, int TX,
-    int chunk_blocks, float scale, int accumulate, int clear_to) {
+    const int* __restrict__ word, float* __restrict__ dtable, float* __restrict__ part, WordOrder words, int D, int C,
+    int TX, int chunk_blocks, float scale, int accumulate, int clear_to) {
   pdl_wait();
   if ((int)blockIdx.x >= chunk_blocks) {
-    clear_rows(start, dtable, 0, clear_to, D,
+    clear_rows(start, words, dtable, 0, clear_to, D,
                (blockIdx.x - chunk_blocks) * (RED_THREADS / 32) + (threadIdx.x >> 5),
                (gridDim.x - chunk_blocks) * (RED_THREADS / 32));
     return;
   }
   const int tx = threadIdx.x % TX;
   const int chunk = blockIdx.x * (RED_THREADS / TX) + threadIdx.x / TX;
-  const int total = start[V];
+  const int total = start[words.places()];
   const int c0 = chunk * C, c1 = min(total, c0 + C);
   // the words beside the chunk (-1: none): one that goes on there is not finished here
   const int before = c0 > 0 && c0 < c1 ? word[c0 - 1] : -1, after = c0 < c1 && c1 < total ? word[c1] : -1;
@@ -320,22 +342,23 @@ __global__ void __launch_bounds__(RED_THREADS) sum_chunks_kernel(
 template <int VEC>
 __global__ void __launch_bounds__(RED_THREADS) join_kernel(const int* __restrict__ start, const int* __restrict__ word,
                                                            const float* __restrict__ part, float* __restrict__ dtable,
-                                                           int V, int D, int C, int TX, int chunks, float scale,
-                                                           int accumulate, int join_blocks, int clear_from) {
+                                                           WordOrder words, int V, int D, int C, int TX, int chunks,
+                                                           float scale, int accumulate, int join_blocks,
+                                                           int clear_from) {
   pdl_wait();
   if ((int)blockIdx.x >= join_blocks) {
-    clear_rows(start, dtable, clear_from, V, D,
+    clear_rows(start, words, dtable, clear_from, V, D,
                (blockIdx.x - join_blocks) * (RED_THREADS / 32) + (threadIdx.x >> 5),
                (gridDim.x - join_blocks) * (RED_THREADS / 32));
     return;
   }
   const int chunk = blockIdx.x * (RED_THREADS / TX) + threadIdx.x / TX;
-  const int total = start[V];
+  const int total = start[words.places()];
   const int64_t c1 = (int64_t)(chunk + 1) * C;
   if (chunk >= chunks || c1 >= total) return;
   const int w = word[c1 - 1];
-  const int end = start[w + 1];
-  if (end <= c1 || start[w] < c1 - C) return;
+  const int at = words.at(w), end = start[at + 1];
+  if (end <= c1 || start[at] < c1 - C) return;
   const int last = (end - 1) / C;  // the chunk that holds its last token
   for (int col = (threadIdx.x % TX) * VEC; col < D; col += TX * VEC) {
     float acc[VEC];
@@ -392,7 +415,7 @@ void lookup_t(const ID* ids, const T* table, T* out, int64_t n, int64_t V, int D
 
 template <typename T, int VEC>
 void sums(const T* dy, int64_t ld, const int* start, const int* order, const int* word, float* dtable, float* part,
-          int64_t n, int V, int D, float scale, bool accumulate, cudaStream_t s) {
+          int64_t n, WordOrder words, int V, int D, float scale, bool accumulate, cudaStream_t s) {
   const int C = chunk_of(n);
   const int chunks = (int)((n + C - 1) / C);
   const int tx = across(D, VEC), per = RED_THREADS / tx;
@@ -409,7 +432,7 @@ void sums(const T* dy, int64_t ld, const int* start, const int* order, const int
   const int zero_blocks = clear_blocks(z, D, RED_THREADS / 32);
   if (chunk_blocks + zero_blocks > 0) {
     launch_pdl(sum_chunks_kernel<T, VEC>, dim3(chunk_blocks + zero_blocks), dim3(RED_THREADS), 0, s, dy, ld, start,
-               order, word, dtable, part, V, D, C, tx, chunk_blocks, scale, accumulate ? 1 : 0, z);
+               order, word, dtable, part, words, D, C, tx, chunk_blocks, scale, accumulate ? 1 : 0, z);
     DLVK_POST_LAUNCH();
   }
   const int last_blocks = accumulate ? 0 : clear_blocks(V - z, D, RED_THREADS / 32);
@@ -417,8 +440,8 @@ void sums(const T* dy, int64_t ld, const int* start, const int* order, const int
     constexpr int JV = VEC > 1 ? 4 : 1;
     const int jx = across(D, JV), jper = RED_THREADS / jx;
     const int join_blocks = chunks > 1 ? (chunks + jper - 1) / jper : 0;
-    launch_pdl(join_kernel<JV>, dim3(join_blocks + last_blocks), dim3(RED_THREADS), 0, s, start, word, part, dtable, V,
-               D, C, jx, chunks, scale, accumulate ? 1 : 0, join_blocks, z);
+    launch_pdl(join_kernel<JV>, dim3(join_blocks + last_blocks), dim3(RED_THREADS), 0, s, start, word, part, dtable,
+               words, V, D, C, jx, chunks, scale, accumulate ? 1 : 0, join_blocks, z);
     DLVK_POST_LAUNCH();
   }
 }
@@ -445,6 +468,17 @@ void embedding_lookup(DType dt, bool ids64, const void* ids, const void* table, 
   }
 }
 
+// Blocks of the sort: a power of two near the number of SMs with at least 8 words
+// each, more where the counts of a block's words have no room.
+static WordOrder word_order(int64_t V) {
+  int log = 0;
+  while (log < 7 && V >> (log + 1) >= 8) ++log;
+  while ((V + (1LL << log) - 1) >> log > SORT_WORDS) ++log;
+  return {log, (int)((V + (1LL << log) - 1) >> log)};
+}
+
+int64_t embedding_grad_start_ints(int64_t V) { return word_order(V).places() + 1; }
+
 int64_t embedding_grad_part_floats(int64_t n, int D) {
   const int C = chunk_of(n);
   return (n + C - 1) / C * 2 * D;
@@ -454,12 +488,10 @@ void embedding_grad(DType dt, bool ids64, const void* ids, const void* dy, int64
                     int64_t V, int D, float scale, int64_t padding, bool accumulate, int* start, int* order, int* word,
                     float* part, cudaStream_t s) {
   if (V == 0 || D == 0) return;
-  DLVK_CHECK(n < EMBEDDING_GRAD_TOKENS && V < (1LL << 31) - SORT_WORDS, "embedding_grad: more than 2^31 tokens or words");
-  // words of a block: all 148 SMs, at least 8 each, at most what its counts have room for
-  const int R = (int)std::min<int64_t>(SORT_WORDS, std::max<int64_t>(8, (V + 147) / 148));
-  const int blocks = (int)((V + R - 1) / R);
-  const auto room = [](int words) { return (SORT_WARPS + 1) * words * (int)sizeof(int); };
-  const size_t smem = (size_t)room(R);
+  DLVK_CHECK(n < EMBEDDING_GRAD_TOKENS && V < EMBEDDING_GRAD_WORDS, "embedding_grad: more than 2^31 tokens or words");
+  const WordOrder words = word_order(V);
+  const auto room = [](int per) { return (SORT_WARPS + 1) * per * (int)sizeof(int); };
+  const size_t smem = (size_t)room(words.per);
   static bool attr_set[kMaxDevices] = {false};
   const int dev = current_device_slot();
   if (!attr_set[dev]) {
@@ -476,19 +508,19 @@ void embedding_grad(DType dt, bool ids64, const void* ids, const void* dy, int64
   const bool vec = D % step == 0 && ld % step == 0 && al16(dy) && al16(dtable) && al16(part);
   const auto sort = [&](const auto* p) {
     using ID = std::remove_cv_t<std::remove_reference_t<decltype(*p)>>;
-    launch_pdl(sort_tokens_kernel<ID>, dim3(blocks), dim3(SORT_THREADS), smem, s, p, (int)n, (int)V, R, pad, start,
-               order, word);
+    launch_pdl(sort_tokens_kernel<ID>, dim3(1u << words.log), dim3(SORT_THREADS), smem, s, p, (int)n, (int)V, words,
+               pad, start, order, word);
   };
   if (ids64) sort(reinterpret_cast<const int64_t*>(ids));
   else sort(reinterpret_cast<const int32_t*>(ids));
   DLVK_POST_LAUNCH();
   const float* gf = reinterpret_cast<const float*>(dy);
   const __nv_bfloat16* gb = reinterpret_cast<const __nv_bfloat16*>(dy);
-  if (f32 && vec) sums<float, 4>(gf, ld, start, order, word, dtable, part, n, (int)V, D, scale, accumulate, s);
-  else if (f32) sums<float, 1>(gf, ld, start, order, word, dtable, part, n, (int)V, D, scale, accumulate, s);
+  if (f32 && vec) sums<float, 4>(gf, ld, start, order, word, dtable, part, n, words, (int)V, D, scale, accumulate, s);
+  else if (f32) sums<float, 1>(gf, ld, start, order, word, dtable, part, n, words, (int)V, D, scale, accumulate, s);
   else if (vec)
-    sums<__nv_bfloat16, 8>(gb, ld, start, order, word, dtable, part, n, (int)V, D, scale, accumulate, s);
-  else sums<__nv_bfloat16, 1>(gb, ld, start, order, word, dtable, part, n, (int)V, D, scale, accumulate, s);
+    sums<__nv_bfloat16, 8>(gb, ld, start, order, word, dtable, part, n, words, (int)V, D, scale, accumulate, s);
+  else sums<__nv_bfloat16, 1>(gb, ld, start, order, word, dtable, part, n, words, (int)V, D, scale, accumulate, s);
 }
 
 }  // namespace dlvk
