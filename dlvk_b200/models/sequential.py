@@ -335,6 +335,8 @@ class Sequential(Model):
         (LinearCrossEntropyLoss); returns the loss as a device scalar.
         `counted`, `correct` and `loss_sum`, where given, are increased as
         ops.core.linear_ce says."""
+        if not self.is_training:  # the layers before the head would keep no graph, and only the head learn
+            raise RuntimeError("a training step needs the model in training mode: set_training(True)")
         head, h, deferred = self._forward_hidden(x)
         self._last_out = None  # there are no logits for a later backward()
         y = y.to(h.device)

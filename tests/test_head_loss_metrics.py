@@ -34,7 +34,7 @@ def _model(device, right):
     if right:
         head.master.copy_(table.master.t())
         m.store.sync_value()
-    return m, table.master.cpu(), head.master.cpu()
+    return m, table.master.cpu().clone(), head.master.cpu().clone()
 
 
 def _expected(x, y, table, head):
@@ -105,3 +105,20 @@ def test_a_step_whose_rows_do_not_count(device):
     assert 0.0 <= loss <= 2.0 ** -20 and acc == 1.0 and samples == 5 * N
     assert step.epoch_totals() == (0.0, 0, 0.0, 0, 0)
     step.close()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("loss", [dl.LinearCrossEntropyLoss, dl.CrossEntropyLoss])
+def test_a_training_step_in_evaluation_mode_is_refused(device, loss):
+    """As with CrossEntropyLoss, whose output has no graph then: not a step of the head alone."""
+    m, _, head = _model(device, False)
+    x, y = _data()
+    m.set_training(False)
+    with pytest.raises(RuntimeError):
+        m.train_step(x, y.clamp(min=0).to(m.dev.device), loss(), dl.SGD(0.1))
+    with pytest.raises(RuntimeError):
+        dl.TrainStep(m, loss(), dl.SGD(0.1), graph=False)(x, y.clamp(min=0))
+    assert torch.equal(m.m_layers[1].weight.master.cpu(), head)
+    m.set_training(True)
+    m.train_step(x, y.clamp(min=0).to(m.dev.device), loss(), dl.SGD(0.1))
+    assert not torch.equal(m.m_layers[1].weight.master.cpu(), head)
