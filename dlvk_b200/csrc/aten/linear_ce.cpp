@@ -332,8 +332,12 @@ LinearCeResult linear_ce_op(const at::Tensor& x, const at::Tensor& w, const at::
   const bool fused = tc_ok && (bf || (!want_grad && E <= GEMM_PARTS_ACC));
   const bool keep = fused && want_grad && !bias.has_value();  // exponentials kept, not made again
 
-  // 256 MB of a block's exponentials, gradients or logits; the loss alone
-  // keeps a 32nd of that on the tensor cores, the statistics
+  // Room for 256 MB of a block's exponentials (2 bytes), or logits that become
+  // gradients (4), of which linear_ce_block_rows() takes at least 2048 rows: with
+  // V words max(256 MB, 2048 V times that).  fp32 gradients in parts are 6 bytes
+  // a logit beside it, x and W in parts 6 bytes an element, and the split sums of
+  // a product up to 32 of its outputs.  The loss alone keeps the statistics, 8
+  // bytes for 128 logits, on the tensor cores.
   const int64_t rows = linear_ce_block_rows(N, V, !fused ? (64LL << 20) : want_grad ? (128LL << 20) : (1LL << 30));
   const int64_t blocks = ceil_div(N, rows);
   const auto stat_cols_of = [&](int64_t n) { return fused ? ce_tc_stat_cols(n, V, parts) : ce_memory_stat_cols(n, V); };

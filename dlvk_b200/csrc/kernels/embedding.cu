@@ -12,8 +12,12 @@
 // What bounds them: the lookup moves n D elements in and out; the gradient
 // reads dy once and writes V D fp32 once (8192 x 1024 bf16 tokens over 32000
 // words: 17 MB in, 131 MB out, 22.6 us at the measured copy rate), so the
-// sort has to be short.  Measured: that lookup 6.1 us, that gradient 36.7 (sort
-// 6.6, sums 21.8, joins 9.8, each starting up while the one before it ends).
+// sort has to be short.  Measured: that lookup 6.1 us, that gradient 35.3 (sort
+// 6.2, sums 21.0, joins 10.0, each starting up while the one before it ends).
+// The same bits on every run have a price where the sort is most of the work.
+// Against float atomics after a memset, cold caches, one call: 40.0 us (39.7
+// with atomics) at that size, 17 (11) for 512 tokens x 256 over 5000 words, 52 (30)
+// for 65536 x 64 over 100000, 517 (503) for 524288 x 1024 over 32000.
 #include <algorithm>
 #include <type_traits>
 

@@ -554,8 +554,9 @@ __device__ __forceinline__ void epi_store(const TcParams& p, const float* stg, i
 // they keep 11 bits down to 2e-9 of the largest and some down to 1e-12, where
 // bf16 would round every one of them as coarsely as the gradient itself.
 // A 256 x 256 tile of a CTA pair takes the epilogue 3.3 us (EPI 3), 5.0 (EPI 5)
-// or 6.5 (EPI 4 with column sums; a plain bf16 store 3.2), beside MMAs of 4.5 us
-// at K = 1024 (7.1 with every SM at it): 4096 x 1024 x 32000 takes 180, 210 and 217.
+// or 6.3 (EPI 4 with column sums; a plain bf16 store 3.4), beside MMAs of 4.5 us
+// at K = 1024 (7.0 with every SM at it): 4096 x 1024 x 32000 takes 180, 201 and 223
+// (201 and 210 in a block of several).
 constexpr float CE_EXP_SCALE = 32768.f;
 constexpr float LOG2E = 1.4426950408889634f;
 

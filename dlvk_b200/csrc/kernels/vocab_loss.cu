@@ -10,12 +10,12 @@
 // are taken a tile of 256 words at a time: the first product's epilogue keeps
 // a maximum and a sum per row and 128 words, ce_finish joins them.  For the
 // gradients a block of rows at a time leaves exp(z - local maximum) behind
-// (16 bits, at most 256 MB whatever the batch), ce_rescale turns those into
-// dz, and the two gradient products read dz: three products, one pass over
-// the block.  Making the logits a second time instead costs a fourth product
-// (8192 x 1024 x 32000: 434 us against 2 x 95 us for the pass); it is
-// what a bias gradient takes, whose fp32 sums 16-bit exponentials are too
-// coarse for.
+// (16 bits: 256 MB, or 4 KB a word where 2048 rows of a vocabulary above 65536
+// take more), ce_rescale turns those into dz, and the two gradient products
+// read dz: three products, one pass over the block.  Making the logits a second
+// time instead costs a fourth product (8192 x 1024 x 32000: 1633 us of kernels
+// against 1388); it is what a bias gradient takes, whose fp32 sums 16-bit
+// exponentials are too coarse for.
 #include <algorithm>
 
 #include <cuda_fp16.h>
@@ -34,8 +34,8 @@ __device__ __forceinline__ int row_label(const CeRows& r, int64_t i) {
   return (lab >= 0 && lab < r.classes && lab != r.ignore) ? (int)lab : -1;
 }
 
-// x = q0 + q1 + q2 to 2^-24 of x, bf16 each: what rounding leaves is exact in
-// fp32 and goes to the next part.  An infinity or NaN is in q0 alone, and a
+// x = q0 + q1 + q2 to 2^-24 of x, bf16 each (the split of Henry, Tang and
+// Heinecke, 2019): what rounding leaves is exact in fp32 and goes to the next part.  An infinity or NaN is in q0 alone, and a
 // finite x above bf16's range is held at its end.
 __device__ __forceinline__ void three_parts(float x, __nv_bfloat16* q) {
   q[0] = __float2bfloat16_rn(x);

@@ -19,8 +19,9 @@ uint32_t* g_err_words[kMaxDevices] = {nullptr};
 
 uint64_t launch_count() { return g_launches.load(std::memory_order_relaxed); }
 
-// Opt-in (DLVK_PDL=1): on the transformer training step it measured the same
-// as stream-serialised launches (14.34-14.46 vs 14.36-14.39 ms per step).
+// Outside a PdlScope opt-in (DLVK_PDL=1): on the transformer training step it
+// measured the same as stream-serialised launches (14.34-14.46 vs 14.36-14.39 ms
+// per step).
 namespace {
 thread_local int pdl_scopes = 0;
 }

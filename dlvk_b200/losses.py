@@ -90,7 +90,14 @@ class LinearCrossEntropyLoss(LossFunction):
     hidden [..., E], weight [E, V] (also the transpose of a [V, E] embedding
     table), bias [V] or None, target int32 / int64 [...].  Targets outside
     [0, V) and `ignore_index` do not count; the mean is over those that do
-    (CrossEntropyLoss divides by all rows), and 0 when there are none.
+    (CrossEntropyLoss divides by all rows), and 0 when there are none.  Under
+    data parallelism every rank's mean is over its own counted rows and the
+    ranks' gradients are averaged: with unequal padding that is not the mean
+    over all ranks' counted rows (reduction "sum" weighs them alike).
+
+    What it keeps is a block of rows at a time: in bf16 2 bytes a logit, at
+    most max(256 MB, 4096 bytes a word), in fp32 4 bytes and, with gradients,
+    6 more, at most max(640 MB, 20 KB a word).
 
     `Sequential.train_step`, `TrainStep` and the trainers take it in the place
     of CrossEntropyLoss for a model that ends in a Dense layer without

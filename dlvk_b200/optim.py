@@ -375,8 +375,9 @@ class GradientClipping:
     def global_norm(grads: Iterable[torch.Tensor]) -> torch.Tensor:
         """sqrt(sum of squares over all tensors) as an fp32 scalar on their
         device, without a host read (csrc/kernels/grad_norm.cu).  fp32 and
-        bf16 tensors of any strides may be mixed; a tensor given twice counts
-        twice, no tensors at all have norm 0."""
+        bf16 tensors may be mixed, of any strides of which at most four do not
+        continue one another; a tensor given twice counts twice, no tensors at
+        all have norm 0."""
         grads = _tensor_list(grads)
         if grads and grads[0].is_cuda:
             return K.N().global_norm(grads)
