@@ -16,6 +16,7 @@ using ::dlvk::aten::to_dtype;
 void register_ops(py::module& m);
 void register_runtime(py::module& m);
 void register_nn(py::module& m);
+void register_sequence(py::module& m);
 void register_comm(py::module& m);
 
 }  // namespace bind

@@ -6,5 +6,6 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   dlvk::bind::register_ops(m);
   dlvk::bind::register_runtime(m);
   dlvk::bind::register_nn(m);
+  dlvk::bind::register_sequence(m);
   dlvk::bind::register_comm(m);
 }

@@ -440,6 +440,87 @@ void embedding_grad(DType dt, bool ids64, const void* ids, const void* dy, int64
                     int64_t V, int D, float scale, int64_t padding, bool accumulate, int* start, int* order, int* word,
                     float* part, cudaStream_t s);
 
+// ---- operators over sequences with a state (short_conv.cu, state_scan.cu) ------
+// Elements [B, T, D]: channels contiguous, tokens and sequences any number of
+// elements apart.  p null: not there.
+struct SeqRef {
+  void* p = nullptr;
+  int64_t batch = 0, token = 0;
+};
+
+// Causal depthwise convolution over `taps` tokens (2 to 4), with or without SiLU:
+//   y[t] = act(bias + sum_j weight[:, j] x[t - taps + 1 + j])
+// x before the first token is `state` [B, taps - 1, D], or zeros.  lengths
+// (int32 [B], null: all T): positions past a sequence's length are neither read
+// nor counted, and y is 0 there.
+struct ShortConv {
+  DType dt = DType::F32;
+  int64_t B = 0, T = 0;
+  int D = 0, taps = 0;
+  bool silu = false;
+  SeqRef x, state;
+  const float* weight = nullptr;  // [D, taps]
+  const float* bias = nullptr;    // [D]
+  const int32_t* lengths = nullptr;
+};
+// out_state [B, taps - 1, D] (may be `state`): the last taps - 1 tokens that count.
+void short_conv_fwd(const ShortConv& a, SeqRef y, SeqRef out_state, cudaStream_t s);
+// dx, dweight [D, taps] and dbias [D] (either may be null), written or added to
+// (accumulate).  part: short_conv_part_floats() floats.
+int64_t short_conv_part_floats(const ShortConv& a);
+void short_conv_bwd(const ShortConv& a, SeqRef dy, SeqRef dx, float* dweight, float* dbias, bool accumulate, float* part,
+                    cudaStream_t s);
+
+// Selective state space scan, for each channel d of its group's b and c:
+//   s = softplus(dt + dt_bias)   h[t] = exp(-s exp(a_log)) h[t-1] + s u b[t]
+//   y = (sum_n c h + skip u) silu(z)          (no gate where z is not there)
+// h before the first token is `state`, or zeros.  lengths as above: a position
+// past a sequence's length changes no state and its y is 0.
+constexpr int STATE_SCAN_STATES = 64;  // most states of a channel
+constexpr int STATE_SCAN_SPAN = 16;    // tokens between two kept states
+struct StateScan {
+  DType type = DType::F32;
+  int64_t B = 0, T = 0;
+  int D = 0, N = 0, G = 1;
+  SeqRef u, dt, z;                  // [B, T, D]
+  SeqRef b, c;                      // [B, T, G, N], groups and states contiguous
+  const float* a_log = nullptr;     // [D, N]
+  const float* skip = nullptr;      // [D]
+  const float* dt_bias = nullptr;   // [D]
+  const float* state = nullptr;     // [B, D, N]
+  const int32_t* lengths = nullptr;
+};
+// out_state [B, D, N] (may be `state`): h after the last token that counts.
+// saved [B, ceil(T / STATE_SCAN_SPAN), D, N]: h before every span's first token, for the backward pass.
+void state_scan_fwd(const StateScan& a, SeqRef y, float* out_state, float* saved, cudaStream_t s);
+struct StateScanGrads {
+  SeqRef du, ddt, dz, db, dc;                                      // all written; dz where there is z
+  float *da_log = nullptr, *dskip = nullptr, *ddt_bias = nullptr;  // written or (accumulate) added to; null: not wanted
+  bool accumulate = false;
+};
+// scratch: state_scan_scratch_floats() floats.
+int64_t state_scan_scratch_floats(const StateScan& a);
+void state_scan_bwd(const StateScan& a, const float* saved, SeqRef dy, const StateScanGrads& g, float* scratch,
+                    cudaStream_t s);
+
+// ---- choice of the next word (sampling.cu) ---------------------------------------
+// A setting: one value, or one for each row where the pointer is given.
+template <typename T, typename One>
+struct RowSetting {
+  const T* rows = nullptr;
+  One one = 0;
+};
+struct Sampling {
+  DType dt = DType::F32;
+  const void* logits = nullptr;  // [rows, words], rows ld elements apart
+  int64_t rows = 0, words = 0, ld = 0;
+  const float* uniform = nullptr;  // [rows]
+  RowSetting<float, double> temperature, top_p, min_p;
+  RowSetting<int32_t, int64_t> top_k;
+};
+constexpr int64_t SAMPLING_WORDS = 1 << 18;  // most words: sums of that many weights of 2^44 fit 64 bits
+void sample_tokens(const Sampling& a, int32_t* tokens, cudaStream_t s);
+
 // ---- device error word -------------------------------------------------------
 uint32_t* device_error_word();     // per current device, zero-initialised
 uint32_t read_device_error(bool clear);
