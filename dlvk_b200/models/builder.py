@@ -53,6 +53,9 @@ def layer_from_config(d: dict) -> L.ModernLayer:
         cls = {"RNN": L.RNNLayer, "LSTM": L.LSTMLayer, "GRU": L.GRULayer}[t]
         return cls(d["input_size"], d["hidden_size"], g("return_sequences", True), g("reverse", False),
                    g("use_bias", True))
+    if t == "StateSpace":
+        return L.StateSpaceLayer(d["d_model"], g("d_state", 16), g("d_conv", 4), g("expand", 2), g("dt_rank", None),
+                                 g("groups", 1), g("residual", False))
     if t == "Bidirectional":
         return L.BidirectionalRNN(d["cell"], d["input_size"], d["hidden_size"], g("return_sequences", True))
     raise ValueError(f"unknown layer type '{t}' in architecture")

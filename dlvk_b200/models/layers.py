@@ -20,13 +20,14 @@ import io
 import math
 import struct
 from dataclasses import dataclass
-from typing import List, Optional
+from typing import List, NamedTuple, Optional
 
 import torch
 
 from ..ops import core as K
 from ..ops import functional as Fn
 from ..ops import nn as NN
+from ..ops import ssm as SSM
 from .params import Parameter, ParamStore
 from .. import runtime
 
@@ -901,6 +902,112 @@ def BiGRU(input_size: int, hidden_size: int, **kw):
 
 def BiRNN(input_size: int, hidden_size: int, **kw):
     return BidirectionalRNN(RNNLayer, input_size, hidden_size, **kw)
+
+
+class StateSpaceState(NamedTuple):
+    """What a state space layer keeps of the tokens so far: the convolution's
+    last tokens [sequences, taps - 1, width] and the scan's states
+    [sequences, width, states] (fp32)."""
+
+    conv: torch.Tensor
+    scan: torch.Tensor
+
+
+class StateSpaceLayer(ModernLayer):
+    """A causal layer whose work is linear in the tokens: x [B, T, d_model] is
+    projected to a signal and a gate of width expand * d_model each; the signal
+    passes a causal convolution over d_conv tokens with SiLU and a selective
+    state space scan of d_state states a channel, whose steps, inputs and
+    outputs (dt, b, c) are projections of the signal (dt through dt_rank
+    columns); the gate's SiLU and an output projection follow.  With
+    `residual=True` the output projection adds its input in its epilogue.
+
+    `prompt` and `step` run it on a sequence piece by piece with a state, for
+    text that is being written; they keep no gradient."""
+
+    type_name = "StateSpace"
+
+    def __init__(self, d_model: int, d_state: int = 16, d_conv: int = 4, expand: int = 2, dt_rank: Optional[int] = None,
+                 groups: int = 1, residual: bool = False, init_std: Optional[float] = None):
+        super().__init__()
+        self.d_model, self.d_state, self.d_conv, self.expand = int(d_model), int(d_state), int(d_conv), int(expand)
+        self.width, self.groups, self.residual = self.expand * self.d_model, int(groups), bool(residual)
+        self.dt_rank = int(dt_rank) if dt_rank is not None else -(-self.d_model // 16)
+        if not 2 <= self.d_conv <= 4 or not 1 <= self.d_state <= 64 or self.dt_rank < 1:
+            raise ValueError("a state space layer has 2 to 4 taps, 1 to 64 states and a dt_rank of 1 or more")
+        if self.groups < 1 or self.width % self.groups:
+            raise ValueError(f"{self.width} channels in {self.groups} groups")
+        n, w = self.d_state, self.width
+        std = lambda a, b: init_std if init_std is not None else math.sqrt(2.0 / (a + b))  # noqa: E731
+        uniform = lambda *size: torch.rand(*size, generator=_GEN)  # noqa: E731
+        cols = self.dt_rank + 2 * self.groups * n
+        self.w_in = self._param("w_in", _normal((self.d_model, 2 * w), std(self.d_model, 2 * w)))
+        self.conv_weight = self._param("conv_weight", (uniform(w, self.d_conv) * 2 - 1) / math.sqrt(self.d_conv))
+        self.conv_bias = self._param("conv_bias", torch.zeros(w), decay=False)
+        self.w_x = self._param("w_x", _normal((w, cols), std(w, cols)))
+        self.w_dt = self._param("w_dt", (uniform(self.dt_rank, w) * 2 - 1) / math.sqrt(self.dt_rank))
+        # steps of 0.001 to 0.1 to begin with, decays of 1 to d_state a unit of time
+        step = torch.exp(uniform(w) * math.log(100.0) + math.log(1e-3))
+        self.dt_bias = self._param("dt_bias", step + torch.log(-torch.expm1(-step)), decay=False)
+        self.a_log = self._param("a_log", torch.log(torch.arange(1, n + 1, dtype=torch.float32)).repeat(w, 1), decay=False)
+        self.skip = self._param("skip", torch.ones(w), decay=False)
+        self.w_out = self._param("w_out", _normal((w, self.d_model), std(w, self.d_model)))
+
+    def split(self, p):
+        """The columns of the signal's projection [B, T, :]: dt's, b, c (views)."""
+        low, b, c = p.split([self.dt_rank, self.groups * self.d_state, self.groups * self.d_state], -1)
+        if self.groups > 1:
+            b, c = (v.unflatten(-1, (self.groups, self.d_state)) for v in (b, c))
+        return low, b, c
+
+    def project(self, x2, B, T, state=None, lengths=None, out_state=None, want_state=False):
+        """x2 [B T, d_model] -> signal and gate, the convolved signal, dt's
+        columns, b, c, dt, the convolution's state (None unless wanted)."""
+        xz = K.gemm(x2, self.w_in.value).reshape(B, T, 2 * self.width)
+        v, last = SSM.short_conv_fwd(xz[..., :self.width], self.conv_weight.master, self.conv_bias.master, state=state,
+                                     lengths=lengths, want_state=want_state, out_state=out_state)
+        p = K.gemm(v.reshape(B * T, self.width), self.w_x.value).reshape(B, T, -1)
+        low, b, c = self.split(p)
+        dt = K.gemm(low.flatten(0, 1), self.w_dt.value).reshape(B, T, self.width)
+        return xz, v, low, b, c, dt, last
+
+    def _forward(self, x):
+        if x.dtype != self.compute_dtype:
+            x = x.to(self.compute_dtype)
+        return Fn.StateSpaceFn.apply(x.contiguous(), Fn._ANCHOR, self)
+
+    def init_state(self, batch: int) -> StateSpaceState:
+        """The state before the first token: zeros."""
+        dev = self.w_in.value.device
+        return StateSpaceState(torch.zeros(batch, self.d_conv - 1, self.width, dtype=self.compute_dtype, device=dev),
+                               torch.zeros(batch, self.width, self.d_state, device=dev))
+
+    @torch.no_grad()
+    def prompt(self, x, state: Optional[StateSpaceState] = None, lengths=None):
+        """(output, state after the last token that counts) of x [B, T, d_model]
+        from `state` (zeros); `lengths` (int32 [B]) as in ops.ssm."""
+        self._ensure_placed(x)
+        x = x.to(self.compute_dtype).contiguous()
+        B, T, _ = x.shape
+        x2 = x.reshape(B * T, self.d_model)
+        xz, v, _, b, c, dt, conv = self.project(x2, B, T, state.conv if state is not None else None, lengths,
+                                                want_state=True)
+        y, scan, _ = SSM.state_scan_fwd(v, dt, self.a_log.master, b, c, self.skip.master, xz[..., self.width:],
+                                        self.dt_bias.master, state.scan if state is not None else None, lengths,
+                                        want_state=True)
+        out = K.gemm(y.reshape(B * T, self.width), self.w_out.value, residual=x2 if self.residual else None)
+        return out.reshape(x.shape), StateSpaceState(conv, scan)
+
+    @torch.no_grad()
+    def step(self, x, state: StateSpaceState):
+        """The output of one token x [B, d_model]; `state` moves on in place."""
+        self._ensure_placed(x)
+        x = x.to(self.compute_dtype).contiguous()
+        B = x.shape[0]
+        xz, v, _, b, c, dt, _ = self.project(x, B, 1, state.conv, out_state=state.conv)
+        y, _, _ = SSM.state_scan_fwd(v, dt, self.a_log.master, b, c, self.skip.master, xz[..., self.width:],
+                                     self.dt_bias.master, state.scan, out_state=state.scan)
+        return K.gemm(y.reshape(B, self.width), self.w_out.value, residual=x if self.residual else None)
 
 
 # Reference adapter / legacy names (include/dlvk/layers/layer_adapters.h).

@@ -36,7 +36,7 @@ _CONFIG_KEYS = ("input_size", "output_size", "in_channels", "out_channels", "ker
                 "pool_size", "num_features", "rate", "num_embeddings", "embedding_dim", "normalized_shape",
                 "embed_dim", "num_heads", "d_model", "nhead", "dim_feedforward", "max_len", "eps", "momentum",
                 "num_groups", "num_channels", "residual", "hidden_size", "num_layers", "return_sequences",
-                "bidirectional", "cell", "reverse")
+                "bidirectional", "cell", "reverse", "d_state", "d_conv", "expand", "dt_rank", "groups")
 
 
 def layer_config(layer) -> dict:
@@ -183,6 +183,10 @@ class Sequential(Model):
     def add_bidirectional(self, cell: str, input_size: int, hidden_size: int, return_sequences: bool = True):
         return self.add(L.BidirectionalRNN(cell, input_size, hidden_size, return_sequences))
 
+    def add_state_space(self, d_model: int, d_state: int = 16, d_conv: int = 4, expand: int = 2, dt_rank=None,
+                        groups: int = 1, residual: bool = False, init_std=None):
+        return self.add(L.StateSpaceLayer(d_model, d_state, d_conv, expand, dt_rank, groups, residual, init_std))
+
     # ----------------------------------------------------------- build
     def build(self) -> "Sequential":
         if self.store is None:
@@ -300,6 +304,84 @@ class Sequential(Model):
             y = self._run(x, upto=n)
         self._last_out = y
         return y
+
+    # ----------------------------------------------------------- writing text
+    def generate(self, prompt, steps: int, uniform=None, lengths=None, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+        """`steps` words after each prompt, int32 [B, steps], for a model of an
+        embedding, state space layers (plain or in a Residual) and layers that
+        treat every token alike, ending in the logits of the words (and a
+        Softmax or none).
+
+        prompt: ids [B, T], `lengths` (int [B], 1 to T) where prompts are
+        padded.  The k-th word is ops.sampling.sample_tokens of the logits and
+        uniform[:, k] (fp32 [B, steps], by default torch.rand); the settings are
+        its too.  The prompt passes the layers once, every word once more."""
+        from ..ops.sampling import sample_tokens
+
+        self.build()
+        n = len(self.m_layers) - (1 if self.has_trailing_softmax() else 0)
+        layers = self.m_layers[:n]
+        tokenwise = (L.DenseLayer, L.LayerNormLayer, L.DropoutLayer, L.EmbeddingLayer)
+
+        def state_of(layer):
+            inner = layer.inner if isinstance(layer, L.ResidualLayer) else layer
+            if isinstance(inner, L.StateSpaceLayer):
+                return inner
+            alike = isinstance(inner, tokenwise) or (isinstance(inner, L.ActivationLayer) and
+                                                     inner.activation != L.ActivationType.Softmax)
+            if not alike:
+                raise ValueError(f"generate: a {inner.type_name} layer neither treats every token alike nor has a state")
+            return None
+
+        inner = [state_of(layer) for layer in layers]
+        if not layers or not isinstance(layers[0], L.EmbeddingLayer):
+            raise ValueError("generate: the model begins with an embedding of the words")
+        dev = self.dev.device
+        prompt = torch.as_tensor(prompt).to(dev)
+        if prompt.dim() != 2 or prompt.shape[1] < 1:
+            raise ValueError(f"generate: prompts are ids [sequences, 1 or more tokens], got {tuple(prompt.shape)}")
+        B, T = prompt.shape
+        steps = int(steps)
+        if uniform is None:
+            uniform = torch.rand(B, steps, device=dev)
+        uniform = uniform.to(dev)
+        if uniform.dtype != torch.float32 or tuple(uniform.shape) != (B, steps):
+            raise ValueError(f"generate: uniform numbers are fp32 [{B}, {steps}], got {uniform.dtype} {tuple(uniform.shape)}")
+        if lengths is not None:
+            lengths = torch.as_tensor(lengths)
+            if tuple(lengths.shape) != (B,) or bool((lengths < 1).any()) or bool((lengths > T).any()):
+                raise ValueError(f"generate: {B} lengths of 1 to {T} tokens")
+            lengths = lengths.to(dev, torch.int32)
+        training = self.is_training
+        self.set_training(False)
+        last_state = max((i for i, m in enumerate(inner) if m is not None), default=-1)
+        words = torch.empty(B, steps, dtype=torch.int32, device=dev)
+        try:
+            with torch.no_grad():
+                states, x = {}, prompt
+                for i, layer in enumerate(layers):
+                    if i == max(last_state + 1, 1):  # what follows needs the last token alone
+                        x = x[:, -1:] if lengths is None else torch.gather(
+                            x, 1, (lengths.long() - 1)[:, None, None].expand(-1, 1, x.shape[2]))
+                    if inner[i] is not None:
+                        y, states[i] = inner[i].prompt(x, lengths=lengths)
+                        x = K.binary(x.contiguous(), y, K.BIN_ADD) if isinstance(layer, L.ResidualLayer) else y
+                    else:
+                        x = layer._forward(x.contiguous())
+                for k in range(steps):
+                    words[:, k] = sample_tokens(x[:, -1], uniform[:, k].contiguous(), temperature, top_k, top_p, min_p)
+                    if k + 1 == steps:
+                        break
+                    x = words[:, k:k + 1].contiguous()
+                    for i, layer in enumerate(layers):
+                        if inner[i] is not None:
+                            y = inner[i].step(x[:, 0], states[i])[:, None]
+                            x = K.binary(x.contiguous(), y, K.BIN_ADD) if isinstance(layer, L.ResidualLayer) else y
+                        else:
+                            x = layer._forward(x)
+        finally:
+            self.set_training(training)
+        return words
 
     # ----------------------------------------------------------- losses that take the head
     def _head(self):

@@ -16,6 +16,7 @@ import torch
 
 from . import core as K
 from . import nn as NN
+from . import ssm as SSM
 from .core import ACT_NONE, ACT_RELU, ACT_GELU
 
 # DLVK_FUSE_COLSUM=0: bias gradients by a separate column-sum pass instead of
@@ -406,3 +407,66 @@ class TransformerBlockFn(torch.autograd.Function):
         for p in (f2.weight, f2.bias, f1.weight, f1.bias, ln2.gamma, ln2.beta, at.w_o, at.w_qkv, ln1.gamma, ln1.beta):
             p.grad_ready()
         return dx.reshape(B, S, -1), None, None
+
+
+class StateSpaceFn(torch.autograd.Function):
+    """One state space layer as a single autograd node:
+
+        xz = x Win;  v = silu(conv(xz[:, :W]));  p = v Wx = [low | b | c]
+        y = scan(v, low Wdt, b, c, gate xz[:, W:]);  out = y Wout (+ x)
+
+    Column slices are read and written in place: the gradients of xz and p are
+    each put together by the kernels that make their parts."""
+
+    @staticmethod
+    def forward(ctx, x, anchor, layer):
+        B, T, _ = x.shape
+        x2 = _flat2(x)
+        xz, v, low, b, c, dt = layer.project(x2, B, T)[:6]
+        y, _, saved = SSM.state_scan_fwd(v, dt, layer.a_log.master, b, c, layer.skip.master, xz[..., layer.width:],
+                                         layer.dt_bias.master, save=True)
+        out = K.gemm(_flat2(y), layer.w_out.value, residual=x2 if layer.residual else None)
+        ctx.layer, ctx.dims = layer, (B, T)
+        ctx.save_for_backward(x2, xz, v, low, b, c, dt, y, saved)
+        return out.reshape(x.shape)
+
+    @staticmethod
+    def backward(ctx, gy):
+        x2, xz, v, low, b, c, dt, y, saved = ctx.saved_tensors
+        m, (B, T) = ctx.layer, ctx.dims
+        g = _flat2(gy)
+        if g.dtype != x2.dtype:
+            g = g.to(x2.dtype)
+        g = g.contiguous()
+
+        def wgrad(p, a_t, grad):
+            K.gemm(a_t, grad, out=p.grad, beta=1.0 if p.take_accumulate_flag() else 0.0)
+
+        wgrad(m.w_out, _flat2(y).t(), g)
+        dy = K.gemm(g, m.w_out.value.t()).reshape(B, T, m.width)
+        dxz = torch.empty_like(xz)
+        dp = torch.empty(B, T, m.w_x.shape[1], dtype=x2.dtype, device=x2.device)
+        _, db, dc = m.split(dp)
+        acc = m.a_log.take_accumulate_flag()
+        m.skip.take_accumulate_flag()
+        m.dt_bias.take_accumulate_flag()
+        d = SSM.state_scan_bwd(v, dt, m.a_log.master, b, c, dy, saved, m.skip.master, xz[..., m.width:],
+                               m.dt_bias.master, db=db, dc=dc, dz=dxz[..., m.width:], da_log=m.a_log.grad,
+                               dskip=m.skip.grad, ddt_bias=m.dt_bias.grad, accumulate=acc)
+        ddt, dp2 = _flat2(d.ddt), _flat2(dp)
+        wgrad(m.w_dt, _flat2(low).t(), ddt)
+        K.gemm(ddt, m.w_dt.value.t(), out=dp2[:, :m.dt_rank])
+        wgrad(m.w_x, _flat2(v).t(), dp2)
+        dv = K.gemm(dp2, m.w_x.value.t(), residual=_flat2(d.du)).reshape(B, T, m.width)
+        acc = m.conv_weight.take_accumulate_flag()
+        m.conv_bias.take_accumulate_flag()
+        SSM.short_conv_bwd(xz[..., :m.width], m.conv_weight.master, m.conv_bias.master, dv, dx=dxz[..., :m.width],
+                           dweight=m.conv_weight.grad, dbias=m.conv_bias.grad, accumulate=acc)
+        dxz2 = _flat2(dxz)
+        wgrad(m.w_in, x2.t(), dxz2)
+        dx = None
+        if ctx.needs_input_grad[0]:
+            dx = K.gemm(dxz2, m.w_in.value.t(), residual=g if m.residual else None).reshape(B, T, -1)
+        for p in (m.w_out, m.skip, m.a_log, m.dt_bias, m.w_dt, m.w_x, m.conv_bias, m.conv_weight, m.w_in):
+            p.grad_ready()
+        return dx, None, None
