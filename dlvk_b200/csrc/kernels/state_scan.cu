@@ -14,7 +14,9 @@
 // span.  What is one value a token and channel (softplus, gates) is made by all
 // threads together before a span and after it; the scan between them gives each
 // thread four states of a channel, which stay in its registers, so a channel of
-// N states has N / 4 lanes and sums over states cross lanes by shuffles.
+// N states has N / 4 lanes, and sums over states and channels cross lanes by
+// shuffles.  The next span's elements are on their way to shared memory
+// meanwhile, each to a place that only the thread that asked for it reads.
 #include <algorithm>
 #include <type_traits>
 
@@ -24,8 +26,9 @@
 namespace dlvk {
 namespace {
 
-constexpr int THREADS = 128;
+constexpr int THREADS = 128, WARPS = THREADS / 32;
 constexpr int NS = 4;  // states of a thread
+constexpr int V = 4;   // elements of a thread's load
 constexpr int SPAN = STATE_SCAN_SPAN;
 constexpr float LOG2E = 1.4426950408889634f;
 
@@ -35,27 +38,121 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 __device__ __forceinline__ float sigmoid(float x) { return __fdividef(1.f, 1.f + __expf(-x)); }
-// steps are small, so log1p of a small number has to keep its relative precision
-__device__ __forceinline__ float softplus(float x) { return x > 20.f ? x : log1pf(expf(x)); }
+// softplus(x) = max(x, 0) + log(1 + e), e = exp(-|x|).  Steps are small, so log(1 + e) has to
+// keep its relative precision: 2 atanh(r), r = e / (2 + e) <= 1/3, by its series (to r^17: 2^-25);
+// the exponent's rounding is made good by its remainder.
+__device__ __forceinline__ float softplus(float x) {
+  const float m = -fabsf(x), t = m * LOG2E, rest = fmaf(m, LOG2E, -t) + m * 1.925963033500e-8f;
+  float e = ex2(t);
+  e = fmaf(e, rest * 0.6931472f, e);
+  const float r = __fdividef(e, 2.f + e), r2 = r * r;
+  float p = fmaf(r2, 1.f / 17, 1.f / 15);
+  p = fmaf(r2, p, 1.f / 13);
+  p = fmaf(r2, p, 1.f / 11);
+  p = fmaf(r2, p, 1.f / 9);
+  p = fmaf(r2, p, 1.f / 7);
+  p = fmaf(r2, p, 1.f / 5);
+  p = fmaf(r2, p, 1.f / 3);
+  return fmaxf(x, 0.f) + 2.f * fmaf(r * r2, p, r);
+}
 
-template <typename T, int V> struct Pack;
-template <> struct Pack<float, 4> { using type = float4; };
-template <> struct Pack<float, 1> { using type = float; };
-template <> struct Pack<__nv_bfloat16, 8> { using type = uint4; };
-template <> struct Pack<__nv_bfloat16, 1> { using type = __nv_bfloat16; };
-template <typename T, int V>
-struct Vec {
-  typename Pack<T, V>::type raw;
-  __device__ __forceinline__ void load(const T* p) { raw = *reinterpret_cast<const typename Pack<T, V>::type*>(p); }
-  __device__ __forceinline__ void store(T* p) const { *reinterpret_cast<typename Pack<T, V>::type*>(p) = raw; }
-  __device__ __forceinline__ void zero() {
-    T* e = reinterpret_cast<T*>(&raw);
-#pragma unroll
-    for (int i = 0; i < V; ++i) e[i] = from_f32<T>(0.f);
-  }
+// Two fp32 numbers in one instruction.
+using f2 = unsigned long long;
+__device__ __forceinline__ f2 pack(float a, float b) {
+  f2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float2 unpack(f2 a) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(a));
+  return r;
+}
+__device__ __forceinline__ f2 fma2(f2 a, f2 b, f2 c) {
+  f2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ f2 mul2(f2 a, f2 b) {
+  f2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ float both(f2 a) {
+  const float2 v = unpack(a);
+  return v.x + v.y;
+}
+__device__ __forceinline__ f2 ex2_2(f2 x) {
+  const float2 v = unpack(x);
+  return pack(ex2(v.x), ex2(v.y));
+}
+// The same, never taken from a register that an equal one has filled before: the
+// backward pass's decays of a span would fill 64.
+__device__ __forceinline__ f2 ex2_2_again(f2 x) {
+  float2 v = unpack(x);
+  asm volatile("ex2.approx.ftz.f32 %0, %0;" : "+f"(v.x));
+  asm volatile("ex2.approx.ftz.f32 %0, %0;" : "+f"(v.y));
+  return pack(v.x, v.y);
+}
+struct Quad {  // a thread's four states
+  f2 v[2];
+};
+__device__ __forceinline__ Quad load_quad(const float* p) {
+  const ulonglong2 u = *reinterpret_cast<const ulonglong2*>(p);
+  return {{u.x, u.y}};
+}
+
+// Four neighbouring elements of a row.
+template <typename T> struct Raw;
+template <> struct Raw<float> { using type = float4; };
+template <> struct Raw<__nv_bfloat16> { using type = uint2; };
+template <typename T>
+struct Four {
+  typename Raw<T>::type raw;
   __device__ __forceinline__ float get(int i) const { return to_f32(reinterpret_cast<const T*>(&raw)[i]); }
   __device__ __forceinline__ void set(int i, float v) { reinterpret_cast<T*>(&raw)[i] = from_f32<T>(v); }
+  // `count` of them
+  template <bool WIDE>
+  __device__ __forceinline__ void store(T* p, int count) const {
+    if constexpr (WIDE) {
+      *reinterpret_cast<typename Raw<T>::type*>(p) = raw;
+    } else {
+#pragma unroll
+      for (int i = 0; i < V; ++i)
+        if (i < count) p[i] = reinterpret_cast<const T*>(&raw)[i];
+    }
+  }
 };
+
+// BYTES from global to shared memory without a register, zeros instead where not `there`.
+template <int BYTES>
+__device__ __forceinline__ void copy_async(void* dst, const void* src, bool there) {
+  const uint32_t to = (uint32_t)__cvta_generic_to_shared(dst);
+  const int n = there ? BYTES : 0;
+  asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(to), "l"(src), "n"(BYTES), "r"(n) : "memory");
+}
+__device__ __forceinline__ void copies_issued() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+// All copies of this thread but those of the last group have come.
+__device__ __forceinline__ void wait_but_last() { asm volatile("cp.async.wait_group 1;" ::: "memory"); }
+
+// Four elements from p on, `count` of them (0: none) from memory, the others zeros.
+// WIDE: rows of whole aligned fours, one copy.  Else fp32 is copied element by
+// element, bf16 (2 bytes are too few for a copy) loaded.
+template <typename T, bool WIDE>
+__device__ __forceinline__ void fetch_four(Four<T>* dst, const T* p, const void* valid, int count) {
+  if constexpr (WIDE) {
+    copy_async<V * sizeof(T)>(dst, count > 0 ? (const void*)p : valid, count > 0);
+  } else if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+      copy_async<4>(reinterpret_cast<T*>(dst) + i, i < count ? (const void*)(p + i) : valid, i < count);
+  } else {
+    Four<T> f;
+#pragma unroll
+    for (int i = 0; i < V; ++i) f.set(i, i < count ? to_f32(p[i]) : 0.f);
+    *dst = f;
+  }
+}
 
 template <typename T>
 __device__ __forceinline__ T* at(const SeqRef& r, int64_t b, int64_t t, int64_t c) {
@@ -70,15 +167,16 @@ template <int L>
 struct Tile {
   static constexpr int CH = THREADS / L;
   int64_t b;
-  int group, c0, count;  // first channel, channels of the tile that exist
+  int group, k, c0, count;  // tile of the group; first channel, channels of the tile that exist
   __device__ __forceinline__ explicit Tile(const StateScan& a) {
     const int per = a.D / a.G, tiles = (per + CH - 1) / CH;
     const int64_t i = blockIdx.x;
-    const int k = (int)(i % ((int64_t)tiles * a.G));
+    const int j = (int)(i % ((int64_t)tiles * a.G));
     b = i / ((int64_t)tiles * a.G);
-    group = k / tiles;
-    c0 = group * per + k % tiles * CH;
-    count = min(CH, per - k % tiles * CH);
+    group = j / tiles;
+    k = j % tiles;
+    c0 = group * per + k * CH;
+    count = min(CH, per - k * CH);
   }
 };
 
@@ -106,198 +204,280 @@ __device__ __forceinline__ void deal(float* v, int lane, int& first, bool& mine)
   }
 }
 
-// b or c of a span to shared memory, rows of NS L states, zeros past N and past the tokens.
-template <typename T, int L>
-__device__ __forceinline__ void load_states(float (*dst)[NS * L], const SeqRef& r, int64_t b, int64_t t0, int64_t n,
-                                            int group, int N) {
-  for (int i = threadIdx.x; i < SPAN * NS * L; i += THREADS) {
-    const int t = i / (NS * L), k = i % (NS * L);
-    dst[t][k] = t0 + t < n && k < N ? to_f32(*at<T>(r, b, t0 + t, (int64_t)group * N + k)) : 0.f;
+// b and c of a span, b's rows of NS L states and then c's, zeros past N; a
+// thread has four neighbouring states at a time.
+template <typename T, int L, bool WIDE>
+struct SpanStates {
+  static constexpr int PER = (2 * SPAN * L + THREADS - 1) / THREADS;
+  using Stage = Four<T>[PER][THREADS];
+  __device__ __forceinline__ static void fetch(Stage& to, const StateScan& a, int64_t seq, int group, int64_t t0, int64_t n) {
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int e = threadIdx.x + i * THREADS, t = e / L % SPAN, k = e % L * NS;
+      const SeqRef& r = e < SPAN * L ? a.b : a.c;
+      if (e < 2 * SPAN * L)
+        fetch_four<T, WIDE>(&to[i][threadIdx.x], at<T>(r, seq, t0 + t, (int64_t)group * a.N + k), r.p,
+                            t0 + t < n ? a.N - k : 0);
+    }
   }
-}
+  __device__ __forceinline__ static void widen(const Stage& from, float* sb) {
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int e = threadIdx.x + i * THREADS;
+      if (e < 2 * SPAN * L) {
+        const Four<T> f = from[i][threadIdx.x];
+        *reinterpret_cast<float4*>(sb + e * NS) = make_float4(f.get(0), f.get(1), f.get(2), f.get(3));
+      }
+    }
+  }
+};
 
-__device__ __forceinline__ void load4(float (&h)[NS], const float* p, int n0, int N) {
+__device__ __forceinline__ Quad load_states(const float* p, int n0, int N) {
+  float h[NS];
 #pragma unroll
   for (int i = 0; i < NS; ++i) h[i] = n0 + i < N ? p[i] : 0.f;
+  return {{pack(h[0], h[1]), pack(h[2], h[3])}};
 }
-__device__ __forceinline__ void store4(const float (&h)[NS], float* p, int n0, int N) {
+__device__ __forceinline__ void store_states(const Quad& q, float* p, int n0, int N) {
+  const float2 a = unpack(q.v[0]), b = unpack(q.v[1]);
+  const float h[NS] = {a.x, a.y, b.x, b.y};
 #pragma unroll
   for (int i = 0; i < NS; ++i)
     if (n0 + i < N) p[i] = h[i];
 }
+// -exp(a_log) of a thread's states, 0 past N.
+__device__ __forceinline__ Quad load_rates(const StateScan& a, int d, int n0, float scale) {
+  float r[NS];
+#pragma unroll
+  for (int i = 0; i < NS; ++i) r[i] = n0 + i < a.N ? -expf(a.a_log[(int64_t)d * a.N + n0 + i]) * scale : 0.f;
+  return {{pack(r[0], r[1]), pack(r[2], r[3])}};
+}
+
+// A thread's elements of a span: four neighbouring channels from c on, tokens t, t + STEP, ...
+template <int CH>
+struct Mine {
+  static constexpr int PER = (SPAN * CH / V + THREADS - 1) / THREADS, STEP = THREADS * V / CH;
+  int c, t, left;  // left: channels from c on that exist
+  __device__ __forceinline__ explicit Mine(int count)
+      : c(threadIdx.x * V % CH), t(threadIdx.x * V / CH), left(count - (int)(threadIdx.x * V % CH)) {}
+};
 
 // ---------------------------------------------------------------- forward
-template <typename T, int L, int V>
+template <typename T, int L, bool WIDE>
+struct FwdShared {
+  static constexpr int CH = THREADS / L, PER = Mine<CH>::PER;
+  float2 sx[SPAN][CH];  // s, s u
+  float sy[SPAN][CH];   // sum_n c h
+  float sb[2 * SPAN * NS * L];
+  float bias[CH], skip[CH];
+  struct {
+    Four<T> u[PER][THREADS], dt[PER][THREADS], z[PER][THREADS];
+    typename SpanStates<T, L, WIDE>::Stage bc;
+  } stage[2];
+};
+
+template <typename T, int L, bool WIDE>
 __global__ void __launch_bounds__(THREADS) scan_fwd_kernel(StateScan a, SeqRef y, float* out_state, float* saved) {
   using Tl = Tile<L>;
-  constexpr int CH = Tl::CH, PER = (SPAN * CH / V + THREADS - 1) / THREADS;
-  __shared__ float2 sx[SPAN][CH];   // s, s u
-  __shared__ float sy[SPAN][CH];
-  __shared__ float sb[SPAN][NS * L], sc[SPAN][NS * L];
+  using States = SpanStates<T, L, WIDE>;
+  constexpr int CH = Tl::CH;
+  extern __shared__ __align__(16) char raw[];
+  auto& sh = *reinterpret_cast<FwdShared<T, L, WIDE>*>(raw);
   const Tl tile(a);
-  const int lane = threadIdx.x % L, ch = threadIdx.x / L, n0 = lane * NS;
+  const Mine<CH> my(tile.count);
+  const int lane = threadIdx.x % 32, n0 = threadIdx.x % L * NS, ch = threadIdx.x / L;
   const bool real = ch < tile.count;
-  const int64_t n = length_of(a, tile.b);
+  const int64_t n = length_of(a, tile.b), spans = (a.T + SPAN - 1) / SPAN;
   const int64_t row = (tile.b * a.D + tile.c0 + ch) * a.N + n0;  // of this thread's states
-  float h[NS], rate[NS];
-#pragma unroll
-  for (int i = 0; i < NS; ++i) h[i] = rate[i] = 0.f;
+  Quad h{}, rate{};
   if (real) {
-    if (a.state) load4(h, a.state + row, n0, a.N);
-    load4(rate, a.a_log + (int64_t)(tile.c0 + ch) * a.N + n0, n0, a.N);
-#pragma unroll
-    for (int i = 0; i < NS; ++i) rate[i] = n0 + i < a.N ? -expf(rate[i]) * LOG2E : 0.f;
+    if (a.state) h = load_states(a.state + row, n0, a.N);
+    rate = load_rates(a, tile.c0 + ch, n0, LOG2E);
   }
-  const int64_t spans = (a.T + SPAN - 1) / SPAN;
+  for (int j = threadIdx.x; j < CH; j += THREADS) {
+    sh.bias[j] = a.dt_bias && j < tile.count ? a.dt_bias[tile.c0 + j] : 0.f;
+    sh.skip[j] = a.skip && j < tile.count ? a.skip[tile.c0 + j] : 0.f;
+  }
+  const auto fetch = [&](int64_t k) {
+    auto& to = sh.stage[k % 2];
+    const int64_t t0 = k * SPAN;
+#pragma unroll
+    for (int i = 0; i < my.PER; ++i) {
+      const int t = my.t + i * my.STEP;
+      if (t >= SPAN) break;
+      const int count = t0 + t < n ? my.left : 0;
+      fetch_four<T, WIDE>(&to.u[i][threadIdx.x], at<T>(a.u, tile.b, t0 + t, tile.c0 + my.c), a.u.p, count);
+      fetch_four<T, WIDE>(&to.dt[i][threadIdx.x], at<T>(a.dt, tile.b, t0 + t, tile.c0 + my.c), a.dt.p, count);
+      if (a.z.p) fetch_four<T, WIDE>(&to.z[i][threadIdx.x], at<T>(a.z, tile.b, t0 + t, tile.c0 + my.c), a.z.p, count);
+    }
+    States::fetch(to.bc, a, tile.b, tile.group, t0, n);
+  };
+  if (spans > 0) fetch(0);
+  copies_issued();
+  __syncthreads();
   for (int64_t k = 0; k < spans; ++k) {
     const int64_t t0 = k * SPAN;
-    Vec<T, V> u[PER];
+    auto& now = sh.stage[k % 2];
+    if (k + 1 < spans) fetch(k + 1);
+    copies_issued();
+    wait_but_last();
 #pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      const int e = (threadIdx.x + i * THREADS) * V, t = e / CH, c = e % CH;
+    for (int i = 0; i < my.PER; ++i) {
+      const int t = my.t + i * my.STEP;
       if (t >= SPAN) break;
-      Vec<T, V> dt;
-      u[i].zero();
-      const bool here = t0 + t < n && c < tile.count;
-      if (here) {
-        u[i].load(at<T>(a.u, tile.b, t0 + t, tile.c0 + c));
-        dt.load(at<T>(a.dt, tile.b, t0 + t, tile.c0 + c));
-      }
+      const Four<T> u = now.u[i][threadIdx.x], dt = now.dt[i][threadIdx.x];
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        const float s = here ? softplus(dt.get(j) + (a.dt_bias ? a.dt_bias[tile.c0 + c + j] : 0.f)) : 0.f;
-        sx[t][c + j] = make_float2(s, s * u[i].get(j));
+        const float s = t0 + t < n && j < my.left ? softplus(dt.get(j) + sh.bias[my.c + j]) : 0.f;
+        sh.sx[t][my.c + j] = make_float2(s, s * u.get(j));
       }
     }
-    load_states<T, L>(sb, a.b, tile.b, t0, n, tile.group, a.N);
-    load_states<T, L>(sc, a.c, tile.b, t0, n, tile.group, a.N);
+    States::widen(now.bc, sh.sb);
     __syncthreads();
-    if (saved && real) store4(h, saved + ((tile.b * spans + k) * a.D + tile.c0 + ch) * a.N + n0, n0, a.N);
+    if (saved && real) store_states(h, saved + ((tile.b * spans + k) * a.D + tile.c0 + ch) * a.N + n0, n0, a.N);
 #pragma unroll
     for (int t = 0; t < SPAN; t += 4) {
       float v[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const float2 x = sx[t + j][ch];
-        const float4 bb = *reinterpret_cast<const float4*>(&sb[t + j][n0]);
-        const float4 cc = *reinterpret_cast<const float4*>(&sc[t + j][n0]);
-        h[0] = fmaf(ex2(x.x * rate[0]), h[0], x.y * bb.x);
-        h[1] = fmaf(ex2(x.x * rate[1]), h[1], x.y * bb.y);
-        h[2] = fmaf(ex2(x.x * rate[2]), h[2], x.y * bb.z);
-        h[3] = fmaf(ex2(x.x * rate[3]), h[3], x.y * bb.w);
-        v[j] = fmaf(cc.x, h[0], fmaf(cc.y, h[1], fmaf(cc.z, h[2], cc.w * h[3])));
+        const float2 x = sh.sx[t + j][ch];
+        const Quad qb = load_quad(&sh.sb[(t + j) * NS * L + n0]), qc = load_quad(&sh.sb[(SPAN + t + j) * NS * L + n0]);
+        const f2 s = pack(x.x, x.x), su = pack(x.y, x.y);
+        h.v[0] = fma2(ex2_2(mul2(s, rate.v[0])), h.v[0], mul2(su, qb.v[0]));
+        h.v[1] = fma2(ex2_2(mul2(s, rate.v[1])), h.v[1], mul2(su, qb.v[1]));
+        v[j] = both(fma2(qc.v[0], h.v[0], mul2(qc.v[1], h.v[1])));
       }
       int first = 0;
       bool mine = true;
-      deal<4, 1, L>(v, threadIdx.x & 31, first, mine);
+      deal<4, 1, L>(v, lane, first, mine);
       if (mine) {
 #pragma unroll
-        for (int j = 0; j < dealt(4, 1, L); ++j) sy[t + first + j][ch] = v[j];
+        for (int j = 0; j < dealt(4, 1, L); ++j) sh.sy[t + first + j][ch] = v[j];
       }
     }
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      const int e = (threadIdx.x + i * THREADS) * V, t = e / CH, c = e % CH;
-      if (t >= SPAN || t0 + t >= a.T || c >= tile.count) break;
-      Vec<T, V> z, out;
-      z.zero();
-      if (a.z.p && t0 + t < n) z.load(at<T>(a.z, tile.b, t0 + t, tile.c0 + c));
+    for (int i = 0; i < my.PER; ++i) {
+      const int t = my.t + i * my.STEP;
+      if (t >= SPAN || t0 + t >= a.T || my.left <= 0) break;
+      const Four<T> u = now.u[i][threadIdx.x], z = now.z[i][threadIdx.x];
+      Four<T> out;
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        float p = sy[t][c + j];
-        if (a.skip) p = fmaf(a.skip[tile.c0 + c + j], u[i].get(j), p);
+        float p = fmaf(sh.skip[my.c + j], u.get(j), sh.sy[t][my.c + j]);
         if (a.z.p) p *= z.get(j) * sigmoid(z.get(j));
         out.set(j, t0 + t < n ? p : 0.f);
       }
-      out.store(at<T>(y, tile.b, t0 + t, tile.c0 + c));
+      out.template store<WIDE>(at<T>(y, tile.b, t0 + t, tile.c0 + my.c), my.left);
     }
   }
-  if (out_state && real) store4(h, out_state + row, n0, a.N);
+  if (out_state && real) store_states(h, out_state + row, n0, a.N);
 }
 
 // ---------------------------------------------------------------- backward
-// part_bc [tiles of a group][B][T][G][2][N]; part_d [B][D][N + 2]: da, dskip, ddt_bias.
-template <typename T, int L, int V>
-__global__ void __launch_bounds__(THREADS) scan_bwd_kernel(StateScan a, const float* __restrict__ saved, SeqRef dy,
-                                                           StateScanGrads g, float* __restrict__ part_bc,
-                                                           float* __restrict__ part_d) {
+template <typename T, int L, bool WIDE>
+struct BwdShared {
+  static constexpr int CH = THREADS / L, PER = Mine<CH>::PER;
+  float2 sx[SPAN][CH];                // s, s u
+  float sq[SPAN][CH];                 // q
+  float sy[SPAN][CH];                 // sum_n c h
+  float sv[SPAN][CH], sd[SPAN][CH];   // sum_n g b, sum_n g a h' A
+  float sb[2 * SPAN * NS * L];
+  float red[WARPS][SPAN][2 * NS * L]; // db and dc of a warp's channels
+  float4 sums[2][THREADS];            // dskip and ddt_bias of a thread's elements
+  float bias[CH], skip[CH];
+  struct {
+    Four<T> u[PER][THREADS], dt[PER][THREADS], z[PER][THREADS], go[PER][THREADS];
+    typename SpanStates<T, L, WIDE>::Stage bc;
+    float4 h[THREADS];
+  } stage[2];
+};
+
+// part_bc [tiles of a group][B][T][G][2][NS L]; part_d [B][D][N + 2]: da, dskip, ddt_bias.
+template <typename T, int L, bool WIDE>
+__global__ void __launch_bounds__(THREADS, 4) scan_bwd_kernel(StateScan a, const float* __restrict__ saved, SeqRef dy,
+                                                              StateScanGrads g, float* __restrict__ part_bc,
+                                                              float* __restrict__ part_d) {
   using Tl = Tile<L>;
-  constexpr int CH = Tl::CH, PER = (SPAN * CH / V + THREADS - 1) / THREADS, WARPS = THREADS / 32;
-  __shared__ float2 sx[SPAN][CH];         // s, s u
-  __shared__ float sq[SPAN][CH];          // q
-  __shared__ float sy[SPAN][CH];          // sum_n c h
-  __shared__ float sv[SPAN][CH], sd[SPAN][CH];  // sum_n g b, sum_n g a h' A
-  __shared__ float sb[SPAN][NS * L], sc[SPAN][NS * L];
-  __shared__ float red[WARPS][SPAN][2 * NS * L];
+  using States = SpanStates<T, L, WIDE>;
+  constexpr int CH = Tl::CH, ROW = 2 * NS * L;
+  extern __shared__ __align__(16) char raw[];
+  auto& sh = *reinterpret_cast<BwdShared<T, L, WIDE>*>(raw);
   const Tl tile(a);
-  const int lane = threadIdx.x % L, ch = threadIdx.x / L, n0 = lane * NS, warp = threadIdx.x / 32;
+  const Mine<CH> my(tile.count);
+  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, n0 = threadIdx.x % L * NS, ch = threadIdx.x / L;
   const bool real = ch < tile.count;
   const int64_t n = length_of(a, tile.b), spans = (a.T + SPAN - 1) / SPAN;
-  const int per = a.D / a.G, tile_of_group = (tile.c0 - tile.group * per) / CH;
-  float rate[NS], ga[NS], da[NS], dskip[V], dbias[V];
-#pragma unroll
-  for (int i = 0; i < NS; ++i) rate[i] = ga[i] = da[i] = 0.f;
-#pragma unroll
-  for (int j = 0; j < V; ++j) dskip[j] = dbias[j] = 0.f;
-  if (real) {
-    load4(rate, a.a_log + (int64_t)(tile.c0 + ch) * a.N + n0, n0, a.N);
-#pragma unroll
-    for (int i = 0; i < NS; ++i) rate[i] = n0 + i < a.N ? -expf(rate[i]) : 0.f;
+  Quad rate{}, ga{}, da{};
+  if (real) rate = load_rates(a, tile.c0 + ch, n0, 1.f);
+  const f2 log2e = pack(LOG2E, LOG2E);
+  for (int j = threadIdx.x; j < CH; j += THREADS) {
+    sh.bias[j] = a.dt_bias && j < tile.count ? a.dt_bias[tile.c0 + j] : 0.f;
+    sh.skip[j] = a.skip && j < tile.count ? a.skip[tile.c0 + j] : 0.f;
   }
+  sh.sums[0][threadIdx.x] = sh.sums[1][threadIdx.x] = make_float4(0.f, 0.f, 0.f, 0.f);
+  const auto fetch = [&](int64_t k) {
+    auto& to = sh.stage[k % 2];
+    const int64_t t0 = k * SPAN;
+#pragma unroll
+    for (int i = 0; i < my.PER; ++i) {
+      const int t = my.t + i * my.STEP;
+      if (t >= SPAN) break;
+      const int count = t0 + t < n ? my.left : 0;
+      fetch_four<T, WIDE>(&to.u[i][threadIdx.x], at<T>(a.u, tile.b, t0 + t, tile.c0 + my.c), a.u.p, count);
+      fetch_four<T, WIDE>(&to.dt[i][threadIdx.x], at<T>(a.dt, tile.b, t0 + t, tile.c0 + my.c), a.dt.p, count);
+      if (a.z.p) fetch_four<T, WIDE>(&to.z[i][threadIdx.x], at<T>(a.z, tile.b, t0 + t, tile.c0 + my.c), a.z.p, count);
+      fetch_four<T, WIDE>(&to.go[i][threadIdx.x], at<T>(dy, tile.b, t0 + t, tile.c0 + my.c), dy.p, count);
+    }
+    States::fetch(to.bc, a, tile.b, tile.group, t0, n);
+    fetch_four<float, WIDE>(reinterpret_cast<Four<float>*>(&to.h[threadIdx.x]),
+                            saved + ((tile.b * spans + k) * a.D + tile.c0 + ch) * a.N + n0, saved, real ? a.N - n0 : 0);
+  };
+  if (spans > 0) fetch(spans - 1);
+  copies_issued();
+  __syncthreads();
   for (int64_t k = spans - 1; k >= 0; --k) {
     const int64_t t0 = k * SPAN;
-    Vec<T, V> u[PER], dt[PER], z[PER], go[PER];
+    auto& now = sh.stage[k % 2];
+    if (k > 0) fetch(k - 1);
+    copies_issued();
+    wait_but_last();
 #pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      const int e = (threadIdx.x + i * THREADS) * V, t = e / CH, c = e % CH;
-      u[i].zero();
-      dt[i].zero();
-      z[i].zero();
-      go[i].zero();
+    for (int i = 0; i < my.PER; ++i) {
+      const int t = my.t + i * my.STEP;
       if (t >= SPAN) break;
-      const bool here = t0 + t < n && c < tile.count;
-      if (here) {
-        u[i].load(at<T>(a.u, tile.b, t0 + t, tile.c0 + c));
-        dt[i].load(at<T>(a.dt, tile.b, t0 + t, tile.c0 + c));
-        if (a.z.p) z[i].load(at<T>(a.z, tile.b, t0 + t, tile.c0 + c));
-        go[i].load(at<T>(dy, tile.b, t0 + t, tile.c0 + c));
-      }
+      const Four<T> u = now.u[i][threadIdx.x], dt = now.dt[i][threadIdx.x], z = now.z[i][threadIdx.x],
+                    go = now.go[i][threadIdx.x];
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        const float s = here ? softplus(dt[i].get(j) + (a.dt_bias ? a.dt_bias[tile.c0 + c + j] : 0.f)) : 0.f;
-        sx[t][c + j] = make_float2(s, s * u[i].get(j));
-        sq[t][c + j] = go[i].get(j) * (a.z.p ? z[i].get(j) * sigmoid(z[i].get(j)) : 1.f);
+        const float s = t0 + t < n && j < my.left ? softplus(dt.get(j) + sh.bias[my.c + j]) : 0.f;
+        sh.sx[t][my.c + j] = make_float2(s, s * u.get(j));
+        sh.sq[t][my.c + j] = go.get(j) * (a.z.p ? z.get(j) * sigmoid(z.get(j)) : 1.f);
       }
     }
-    load_states<T, L>(sb, a.b, tile.b, t0, n, tile.group, a.N);
-    load_states<T, L>(sc, a.c, tile.b, t0, n, tile.group, a.N);
-    float h[SPAN + 1][NS];  // h[t]: before token t of the span
-#pragma unroll
-    for (int i = 0; i < NS; ++i) h[0][i] = 0.f;
-    if (real) load4(h[0], saved + ((tile.b * spans + k) * a.D + tile.c0 + ch) * a.N + n0, n0, a.N);
+    States::widen(now.bc, sh.sb);
+    Quad h[SPAN + 1];  // h[t]: before token t of the span
+    h[0] = load_quad(reinterpret_cast<const float*>(&now.h[threadIdx.x]));
     __syncthreads();
 #pragma unroll
     for (int t = 0; t < SPAN; t += 4) {
       float v[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const float2 x = sx[t + j][ch];
-        const float4 bb = *reinterpret_cast<const float4*>(&sb[t + j][n0]);
-        const float4 cc = *reinterpret_cast<const float4*>(&sc[t + j][n0]);
-        const float sl = x.x * LOG2E;
-        h[t + j + 1][0] = fmaf(ex2(sl * rate[0]), h[t + j][0], x.y * bb.x);
-        h[t + j + 1][1] = fmaf(ex2(sl * rate[1]), h[t + j][1], x.y * bb.y);
-        h[t + j + 1][2] = fmaf(ex2(sl * rate[2]), h[t + j][2], x.y * bb.z);
-        h[t + j + 1][3] = fmaf(ex2(sl * rate[3]), h[t + j][3], x.y * bb.w);
-        v[j] = cc.x * h[t + j + 1][0] + cc.y * h[t + j + 1][1] + cc.z * h[t + j + 1][2] + cc.w * h[t + j + 1][3];
+        const float2 x = sh.sx[t + j][ch];
+        const Quad qb = load_quad(&sh.sb[(t + j) * NS * L + n0]), qc = load_quad(&sh.sb[(SPAN + t + j) * NS * L + n0]);
+        const f2 s = mul2(pack(x.x, x.x), log2e), su = pack(x.y, x.y);
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+          h[t + j + 1].v[i] = fma2(ex2_2(mul2(s, rate.v[i])), h[t + j].v[i], mul2(su, qb.v[i]));
+        v[j] = both(fma2(qc.v[0], h[t + j + 1].v[0], mul2(qc.v[1], h[t + j + 1].v[1])));
       }
       int first = 0;
       bool mine = true;
-      deal<4, 1, L>(v, threadIdx.x & 31, first, mine);
+      deal<4, 1, L>(v, lane, first, mine);
       if (mine) {
 #pragma unroll
-        for (int j = 0; j < dealt(4, 1, L); ++j) sy[t + first + j][ch] = v[j];
+        for (int j = 0; j < dealt(4, 1, L); ++j) sh.sy[t + first + j][ch] = v[j];
       }
     }
 #pragma unroll
@@ -306,117 +486,111 @@ __global__ void __launch_bounds__(THREADS) scan_bwd_kernel(StateScan a, const fl
 #pragma unroll
       for (int j = 3; j >= 0; --j) {
         const int t = t4 + j;
-        const float2 x = sx[t][ch];
-        const float q = sq[t][ch], sl = x.x * LOG2E;
-        float w[8];  // db and dc of this channel
-        sums[2 * j] = sums[2 * j + 1] = 0.f;
+        const float2 x = sh.sx[t][ch];
+        const float q1 = sh.sq[t][ch];
+        const Quad qb = load_quad(&sh.sb[t * NS * L + n0]), qc = load_quad(&sh.sb[(SPAN + t) * NS * L + n0]);
+        const f2 q = pack(q1, q1), s = pack(x.x, x.x), su = pack(x.y, x.y), sl = mul2(s, log2e);
+        f2 into = 0, through_a = 0;  // two zeros
+        float w[8];                  // db and dc of this channel
 #pragma unroll
-        for (int i = 0; i < NS; ++i) {
-          const float gi = fmaf(q, sc[t][n0 + i], ga[i]);
-          w[i] = gi * x.y;
-          w[NS + i] = q * h[t + 1][i];
-          sums[2 * j] = fmaf(gi, sb[t][n0 + i], sums[2 * j]);
-          ga[i] = gi * ex2(sl * rate[i]);
-          const float through = ga[i] * h[t][i];
-          sums[2 * j + 1] = fmaf(through, rate[i], sums[2 * j + 1]);
-          da[i] = fmaf(through, x.x, da[i]);
+        for (int i = 0; i < 2; ++i) {
+          const f2 gi = fma2(q, qc.v[i], ga.v[i]);
+          const float2 wb = unpack(mul2(gi, su)), wc = unpack(mul2(q, h[t + 1].v[i]));
+          w[2 * i] = wb.x, w[2 * i + 1] = wb.y, w[NS + 2 * i] = wc.x, w[NS + 2 * i + 1] = wc.y;
+          into = fma2(gi, qb.v[i], into);
+          ga.v[i] = mul2(gi, ex2_2_again(mul2(sl, rate.v[i])));
+          const f2 through = mul2(ga.v[i], h[t].v[i]);
+          through_a = fma2(through, rate.v[i], through_a);
+          da.v[i] = fma2(through, s, da.v[i]);
         }
+        sums[2 * j] = both(into);
+        sums[2 * j + 1] = both(through_a);
         int first = 0;
         bool mine = true;
-        deal<8, L, 32>(w, threadIdx.x & 31, first, mine);
+        deal<8, L, 32>(w, lane, first, mine);
         if (mine) {
 #pragma unroll
           for (int i = 0; i < dealt(8, L, 32); ++i) {
             const int e = first + i;  // < NS: db of state n0 + e
-            red[warp][t][(e / NS) * NS * L + n0 + e % NS] = w[i];
+            sh.red[warp][t][(e / NS) * NS * L + n0 + e % NS] = w[i];
           }
         }
       }
       int first = 0;
       bool mine = true;
-      deal<8, 1, L>(sums, threadIdx.x & 31, first, mine);
+      deal<8, 1, L>(sums, lane, first, mine);
       if (mine) {
 #pragma unroll
         for (int i = 0; i < dealt(8, 1, L); ++i) {
           const int e = first + i;
-          (e % 2 ? sd : sv)[t4 + e / 2][ch] = sums[i];
+          (e % 2 ? sh.sd : sh.sv)[t4 + e / 2][ch] = sums[i];
         }
       }
     }
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      const int e = (threadIdx.x + i * THREADS) * V, t = e / CH, c = e % CH;
-      if (t >= SPAN || t0 + t >= a.T || c >= tile.count) break;
+    for (int i = 0; i < my.PER; ++i) {
+      const int t = my.t + i * my.STEP;
+      if (t >= SPAN || t0 + t >= a.T || my.left <= 0) break;
       const bool here = t0 + t < n;
-      Vec<T, V> du, ddt, dz;
+      const Four<T> u = now.u[i][threadIdx.x], dt = now.dt[i][threadIdx.x], z = now.z[i][threadIdx.x],
+                    go = now.go[i][threadIdx.x];
+      Four<T> du, ddt, dz;
+      float4 ds = sh.sums[0][threadIdx.x], db = sh.sums[1][threadIdx.x];
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        const int d = tile.c0 + c + j;
-        const float uj = u[i].get(j), zj = z[i].get(j), sk = a.skip ? a.skip[d] : 0.f, q = sq[t][c + j];
-        const float raw = dt[i].get(j) + (a.dt_bias ? a.dt_bias[d] : 0.f), v = sv[t][c + j];
-        du.set(j, here ? fmaf(v, sx[t][c + j].x, q * sk) : 0.f);
-        const float dr = here ? fmaf(v, uj, sd[t][c + j]) * sigmoid(raw) : 0.f;
+        const float uj = u.get(j), zj = z.get(j), q = sh.sq[t][my.c + j], v = sh.sv[t][my.c + j], skip = sh.skip[my.c + j];
+        du.set(j, here ? fmaf(v, sh.sx[t][my.c + j].x, q * skip) : 0.f);
+        const float dr = here ? fmaf(v, uj, sh.sd[t][my.c + j]) * sigmoid(dt.get(j) + sh.bias[my.c + j]) : 0.f;
         ddt.set(j, dr);
-        dbias[j] += dr;
-        dskip[j] = fmaf(q, uj, dskip[j]);
-        if (a.z.p) {
-          const float sz = sigmoid(zj);
-          dz.set(j, here ? go[i].get(j) * fmaf(sk, uj, sy[t][c + j]) * sz * fmaf(zj, 1.f - sz, 1.f) : 0.f);
-        }
+        (&ds.x)[j] = fmaf(q, uj, (&ds.x)[j]);
+        (&db.x)[j] += dr;
+        const float sz = sigmoid(zj);
+        dz.set(j, here ? go.get(j) * fmaf(skip, uj, sh.sy[t][my.c + j]) * sz * fmaf(zj, 1.f - sz, 1.f) : 0.f);
       }
-      du.store(at<T>(g.du, tile.b, t0 + t, tile.c0 + c));
-      ddt.store(at<T>(g.ddt, tile.b, t0 + t, tile.c0 + c));
-      if (a.z.p) dz.store(at<T>(g.dz, tile.b, t0 + t, tile.c0 + c));
+      sh.sums[0][threadIdx.x] = ds;
+      sh.sums[1][threadIdx.x] = db;
+      du.template store<WIDE>(at<T>(g.du, tile.b, t0 + t, tile.c0 + my.c), my.left);
+      ddt.template store<WIDE>(at<T>(g.ddt, tile.b, t0 + t, tile.c0 + my.c), my.left);
+      if (a.z.p) dz.template store<WIDE>(at<T>(g.dz, tile.b, t0 + t, tile.c0 + my.c), my.left);
     }
-    for (int i = threadIdx.x; i < SPAN * 2 * NS * L; i += THREADS) {
-      const int t = i / (2 * NS * L), e = i % (2 * NS * L), half = e / (NS * L), st = e % (NS * L);
-      if (t0 + t >= a.T || st >= a.N) continue;
-      float s = 0.f;
+    float* part = part_bc + (((tile.k * a.B + tile.b) * a.T + t0) * a.G + tile.group) * ROW;
+    for (int i = threadIdx.x * 4; i < SPAN * ROW; i += THREADS * 4) {
+      const int t = i / ROW, e = i % ROW;
+      if (t0 + t >= a.T) break;
+      float4 s = *reinterpret_cast<const float4*>(&sh.red[0][t][e]);
 #pragma unroll
-      for (int w = 0; w < WARPS; ++w) s += red[w][t][e];
-      part_bc[((((tile_of_group * a.B + tile.b) * a.T + t0 + t) * a.G + tile.group) * 2 + half) * a.N + st] = s;
+      for (int w = 1; w < WARPS; ++w) {
+        const float4 x = *reinterpret_cast<const float4*>(&sh.red[w][t][e]);
+        s.x += x.x, s.y += x.y, s.z += x.z, s.w += x.w;
+      }
+      *reinterpret_cast<float4*>(part + (int64_t)t * a.G * ROW + e) = s;
     }
-    __syncthreads();
+    // (the barrier after the next span's elements is between these reads and what comes to their places)
   }
-  if (real) {
-    float* out = part_d + (tile.b * a.D + tile.c0 + ch) * (a.N + 2);
-#pragma unroll
-    for (int i = 0; i < NS; ++i)
-      if (n0 + i < a.N) out[n0 + i] = da[i] * rate[i];
-  }
+  if (real) store_states({{mul2(da.v[0], rate.v[0]), mul2(da.v[1], rate.v[1])}},
+                         part_d + (tile.b * a.D + tile.c0 + ch) * (a.N + 2) + n0, n0, a.N);
   // dskip and ddt_bias: threads CH / V apart hold the same channels
-  constexpr int SAME = CH / V < THREADS ? CH / V : THREADS;
-  float* buf = &sv[0][0];
-  const int c = threadIdx.x * V % CH, rows = SPAN * CH / V < THREADS ? SPAN * CH / V : THREADS;
-#pragma unroll
-  for (int half = 0; half < 2; ++half) {
-    __syncthreads();
-    if (threadIdx.x < rows) {
-#pragma unroll
-      for (int j = 0; j < V; ++j) buf[threadIdx.x * V + j] = half ? dbias[j] : dskip[j];
-    }
-    __syncthreads();
-    if (threadIdx.x < SAME) {
-#pragma unroll
-      for (int j = 0; j < V; ++j) {
-        float s = 0.f;
-        for (int r = threadIdx.x; r < rows; r += SAME) s += buf[r * V + j];
-        if (c + j < tile.count) part_d[(tile.b * a.D + tile.c0 + c + j) * (a.N + 2) + a.N + half] = s;
-      }
-    }
+  constexpr int SAME = CH / V, ROWS = SPAN * SAME < THREADS ? SPAN * SAME : THREADS;
+  __syncthreads();
+  for (int i = threadIdx.x; i < 2 * CH; i += THREADS) {
+    const int half = i / CH, at_ch = i % CH;
+    float s = 0.f;
+    for (int r = at_ch / V; r < ROWS; r += SAME) s += (&sh.sums[half][r].x)[at_ch % V];
+    if (at_ch < tile.count) part_d[(tile.b * a.D + tile.c0 + at_ch) * (a.N + 2) + a.N + half] = s;
   }
 }
 
-// db and dc: the sums over a group's tiles, in their order.
+// db and dc: the sums over a group's tiles, in their order; rows of 2 `states`, of which N are real.
 template <typename T>
 __global__ void __launch_bounds__(256) join_bc_kernel(const float* __restrict__ part, int tiles, int64_t B, int64_t T_,
-                                                      int G, int N, SeqRef db, SeqRef dc) {
-  const int64_t row = (int64_t)G * 2 * N, total = B * T_ * row;
+                                                      int G, int N, int states, SeqRef db, SeqRef dc) {
+  const int64_t row = (int64_t)G * 2 * states, total = B * T_ * row;
   for (int64_t i = blockIdx.x * 256LL + threadIdx.x; i < total; i += 256LL * gridDim.x) {
+    const int e = (int)(i % row), group = e / (2 * states), half = e / states % 2, n = e % states;
+    if (n >= N) continue;
     float s = 0.f;
     for (int k = 0; k < tiles; ++k) s += part[k * total + i];
-    const int e = (int)(i % row), group = e / (2 * N), half = e / N % 2, n = e % N;
     const int64_t t = i / row % T_, b = i / row / T_;
     *at<T>(half ? dc : db, b, t, (int64_t)group * N + n) = from_f32<T>(s);
   }
@@ -435,8 +609,10 @@ __global__ void __launch_bounds__(256) join_d_kernel(const float* __restrict__ p
   if (out) *out = g.accumulate ? *out + s : s;
 }
 
-bool aligned(const SeqRef& r, int64_t bytes) {
-  return !r.p || (reinterpret_cast<uintptr_t>(r.p) % 16 == 0 && r.batch * bytes % 16 == 0 && r.token * bytes % 16 == 0);
+// Whether four neighbouring elements are one load.
+bool aligned(const SeqRef& r, DType type) {
+  const int64_t bytes = type == DType::BF16 ? 2 : 4;
+  return !r.p || (reinterpret_cast<uintptr_t>(r.p) % (V * bytes) == 0 && r.batch % V == 0 && r.token % V == 0);
 }
 int lanes_of(int N) { return N <= 8 ? 2 : N <= 16 ? 4 : N <= 32 ? 8 : 16; }
 int tiles_of(const StateScan& a) {  // of a group
@@ -452,16 +628,6 @@ void by_lanes(int N, F&& f) {
     default: f(std::integral_constant<int, 16>());
   }
 }
-template <typename F>
-void by_type(DType dt, bool wide, F&& f) {
-  if (dt == DType::BF16) {
-    if (wide) f(__nv_bfloat16(), std::integral_constant<int, 8>());
-    else f(__nv_bfloat16(), std::integral_constant<int, 1>());
-  } else {
-    if (wide) f(float(), std::integral_constant<int, 4>());
-    else f(float(), std::integral_constant<int, 1>());
-  }
-}
 unsigned grid_of(const StateScan& a) {
   const int64_t g = a.B * a.G * tiles_of(a);
   DLVK_CHECK(g < (1LL << 31), "state_scan: too many channels for one launch");
@@ -475,51 +641,73 @@ void check(const StateScan& a) {
 
 }  // namespace
 
+namespace {
+template <typename Kernel, typename... Args>
+void launch(Kernel kernel, size_t smem, const StateScan& a, cudaStream_t s, Args... args) {
+  if (smem > 48 * 1024)
+    DLVK_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  kernel<<<grid_of(a), THREADS, smem, s>>>(a, args...);
+  DLVK_POST_LAUNCH();
+}
+// f(element type, lanes of a channel, whether rows are of whole aligned fours)
+template <typename F>
+void by_kind(const StateScan& a, bool wide, F&& f) {
+  by_lanes(a.N, [&](auto lanes) {
+    if (a.type == DType::BF16) {
+      if (wide) f(__nv_bfloat16(), lanes, std::true_type());
+      else f(__nv_bfloat16(), lanes, std::false_type());
+    } else {
+      if (wide) f(float(), lanes, std::true_type());
+      else f(float(), lanes, std::false_type());
+    }
+  });
+}
+bool wide_operands(const StateScan& a) {
+  return a.D / a.G % V == 0 && a.N % V == 0 && aligned(a.u, a.type) && aligned(a.dt, a.type) && aligned(a.z, a.type) &&
+         aligned(a.b, a.type) && aligned(a.c, a.type);
+}
+int64_t part_bc_floats(const StateScan& a) { return (int64_t)tiles_of(a) * a.B * a.T * a.G * 2 * NS * lanes_of(a.N); }
+}  // namespace
+
 void state_scan_fwd(const StateScan& a, SeqRef y, float* out_state, float* saved, cudaStream_t s) {
   check(a);
   if (a.B == 0 || a.D == 0) return;
-  const int64_t bytes = a.type == DType::BF16 ? 2 : 4;
-  const bool wide = a.D / a.G % (16 / bytes) == 0 && aligned(a.u, bytes) && aligned(a.dt, bytes) &&
-                    aligned(a.z, bytes) && aligned(y, bytes);
-  by_type(a.type, wide, [&](auto type, auto vec) {
-    by_lanes(a.N, [&](auto lanes) {
-      scan_fwd_kernel<decltype(type), decltype(lanes)::value, decltype(vec)::value>
-          <<<grid_of(a), THREADS, 0, s>>>(a, y, out_state, saved);
-    });
+  by_kind(a, wide_operands(a) && aligned(y, a.type), [&](auto type, auto lanes, auto wide) {
+    using T = decltype(type);
+    constexpr int L = decltype(lanes)::value;
+    constexpr bool W = decltype(wide)::value;
+    launch(scan_fwd_kernel<T, L, W>, sizeof(FwdShared<T, L, W>), a, s, y, out_state, saved);
   });
-  DLVK_POST_LAUNCH();
 }
 
 int64_t state_scan_scratch_floats(const StateScan& a) {
   check(a);
-  return (int64_t)tiles_of(a) * a.B * a.T * a.G * 2 * a.N + a.B * a.D * (a.N + 2);
+  return part_bc_floats(a) + a.B * a.D * (a.N + 2);
 }
 
 void state_scan_bwd(const StateScan& a, const float* saved, SeqRef dy, const StateScanGrads& g, float* scratch,
                     cudaStream_t s) {
   check(a);
   if (a.D == 0) return;
-  const int64_t bytes = a.type == DType::BF16 ? 2 : 4;
   float* part_bc = scratch;
-  float* part_d = scratch + (int64_t)tiles_of(a) * a.B * a.T * a.G * 2 * a.N;
+  float* part_d = scratch + part_bc_floats(a);
   if (a.B > 0) {
-    const bool wide = a.D / a.G % (16 / bytes) == 0 && aligned(a.u, bytes) && aligned(a.dt, bytes) &&
-                      aligned(a.z, bytes) && aligned(dy, bytes) && aligned(g.du, bytes) && aligned(g.ddt, bytes) &&
-                      aligned(g.dz, bytes);
-    by_type(a.type, wide, [&](auto type, auto vec) {
-      by_lanes(a.N, [&](auto lanes) {
-        scan_bwd_kernel<decltype(type), decltype(lanes)::value, decltype(vec)::value>
-            <<<grid_of(a), THREADS, 0, s>>>(a, saved, dy, g, part_bc, part_d);
-      });
+    const bool w = wide_operands(a) && aligned(dy, a.type) && aligned(g.du, a.type) && aligned(g.ddt, a.type) &&
+                   aligned(g.dz, a.type);
+    by_kind(a, w, [&](auto type, auto lanes, auto wide) {
+      using T = decltype(type);
+      constexpr int L = decltype(lanes)::value;
+      constexpr bool W = decltype(wide)::value;
+      launch(scan_bwd_kernel<T, L, W>, sizeof(BwdShared<T, L, W>), a, s, saved, dy, g, part_bc, part_d);
     });
-    DLVK_POST_LAUNCH();
-    const int64_t total = a.B * a.T * a.G * 2 * a.N;
+    const int64_t total = part_bc_floats(a) / tiles_of(a);
     if (total > 0) {
       const unsigned blocks = (unsigned)std::min<int64_t>((total + 255) / 256, 148 * 16);
+      const int states = NS * lanes_of(a.N);
       if (a.type == DType::BF16)
-        join_bc_kernel<__nv_bfloat16><<<blocks, 256, 0, s>>>(part_bc, tiles_of(a), a.B, a.T, a.G, a.N, g.db, g.dc);
+        join_bc_kernel<__nv_bfloat16><<<blocks, 256, 0, s>>>(part_bc, tiles_of(a), a.B, a.T, a.G, a.N, states, g.db, g.dc);
       else
-        join_bc_kernel<float><<<blocks, 256, 0, s>>>(part_bc, tiles_of(a), a.B, a.T, a.G, a.N, g.db, g.dc);
+        join_bc_kernel<float><<<blocks, 256, 0, s>>>(part_bc, tiles_of(a), a.B, a.T, a.G, a.N, states, g.db, g.dc);
       DLVK_POST_LAUNCH();
     }
   }
