@@ -253,6 +253,22 @@ __device__ __forceinline__ Quad load_rates(const StateScan& a, int d, int n0, fl
   return {{pack(r[0], r[1]), pack(r[2], r[3])}};
 }
 
+// A thread's channel of the block and first state.  The lanes of one state group
+// are neighbours: eight lanes that read the same sixteen bytes of b or c take half
+// the shared memory's cycles of eight that read different ones (measured: 2.1 and 4.0).
+template <int L>
+struct Place {
+  static constexpr int CHANNELS = 32 / L;  // of a warp
+  int lane, ch, n0;
+  __device__ __forceinline__ Place()
+      : lane(threadIdx.x % 32), ch(threadIdx.x / 32 * CHANNELS + threadIdx.x % CHANNELS),
+        n0(threadIdx.x % 32 / CHANNELS * NS) {}
+};
+__device__ __forceinline__ float4 four(const float* p) { return *reinterpret_cast<const float4*>(p); }
+__device__ __forceinline__ void put_four(float* p, const float (&v)[V]) {
+  *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+}
+
 // A thread's elements of a span: four neighbouring channels from c on, tokens t, t + STEP, ...
 template <int CH>
 struct Mine {
@@ -266,8 +282,8 @@ struct Mine {
 template <typename T, int L, bool WIDE>
 struct FwdShared {
   static constexpr int CH = THREADS / L, PER = Mine<CH>::PER;
-  float2 sx[SPAN][CH];  // s, s u
-  float sy[SPAN][CH];   // sum_n c h
+  float ss[SPAN][CH], su[SPAN][CH];  // s, s u
+  float sy[SPAN][CH];                // sum_n c h
   float sb[2 * SPAN * NS * L];
   float bias[CH], skip[CH];
   struct {
@@ -285,7 +301,8 @@ __global__ void __launch_bounds__(THREADS) scan_fwd_kernel(StateScan a, SeqRef y
   auto& sh = *reinterpret_cast<FwdShared<T, L, WIDE>*>(raw);
   const Tl tile(a);
   const Mine<CH> my(tile.count);
-  const int lane = threadIdx.x % 32, n0 = threadIdx.x % L * NS, ch = threadIdx.x / L;
+  const Place<L> me;
+  const int lane = me.lane, n0 = me.n0, ch = me.ch;
   const bool real = ch < tile.count;
   const int64_t n = length_of(a, tile.b), spans = (a.T + SPAN - 1) / SPAN;
   const int64_t row = (tile.b * a.D + tile.c0 + ch) * a.N + n0;  // of this thread's states
@@ -326,11 +343,15 @@ __global__ void __launch_bounds__(THREADS) scan_fwd_kernel(StateScan a, SeqRef y
       const int t = my.t + i * my.STEP;
       if (t >= SPAN) break;
       const Four<T> u = now.u[i][threadIdx.x], dt = now.dt[i][threadIdx.x];
+      const float4 bias = four(&sh.bias[my.c]);
+      float s[V], su[V];
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        const float s = t0 + t < n && j < my.left ? softplus(dt.get(j) + sh.bias[my.c + j]) : 0.f;
-        sh.sx[t][my.c + j] = make_float2(s, s * u.get(j));
+        s[j] = t0 + t < n && j < my.left ? softplus(dt.get(j) + (&bias.x)[j]) : 0.f;
+        su[j] = s[j] * u.get(j);
       }
+      put_four(&sh.ss[t][my.c], s);
+      put_four(&sh.su[t][my.c], su);
     }
     States::widen(now.bc, sh.sb);
     __syncthreads();
@@ -340,19 +361,19 @@ __global__ void __launch_bounds__(THREADS) scan_fwd_kernel(StateScan a, SeqRef y
       float v[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const float2 x = sh.sx[t + j][ch];
+        const float s1 = sh.ss[t + j][ch], su1 = sh.su[t + j][ch];
         const Quad qb = load_quad(&sh.sb[(t + j) * NS * L + n0]), qc = load_quad(&sh.sb[(SPAN + t + j) * NS * L + n0]);
-        const f2 s = pack(x.x, x.x), su = pack(x.y, x.y);
+        const f2 s = pack(s1, s1), su = pack(su1, su1);
         h.v[0] = fma2(ex2_2(mul2(s, rate.v[0])), h.v[0], mul2(su, qb.v[0]));
         h.v[1] = fma2(ex2_2(mul2(s, rate.v[1])), h.v[1], mul2(su, qb.v[1]));
         v[j] = both(fma2(qc.v[0], h.v[0], mul2(qc.v[1], h.v[1])));
       }
       int first = 0;
       bool mine = true;
-      deal<4, 1, L>(v, lane, first, mine);
+      deal<4, me.CHANNELS, 32>(v, lane, first, mine);
       if (mine) {
 #pragma unroll
-        for (int j = 0; j < dealt(4, 1, L); ++j) sh.sy[t + first + j][ch] = v[j];
+        for (int j = 0; j < dealt(4, me.CHANNELS, 32); ++j) sh.sy[t + first + j][ch] = v[j];
       }
     }
     __syncthreads();
@@ -361,10 +382,11 @@ __global__ void __launch_bounds__(THREADS) scan_fwd_kernel(StateScan a, SeqRef y
       const int t = my.t + i * my.STEP;
       if (t >= SPAN || t0 + t >= a.T || my.left <= 0) break;
       const Four<T> u = now.u[i][threadIdx.x], z = now.z[i][threadIdx.x];
+      const float4 skip = four(&sh.skip[my.c]), sum = four(&sh.sy[t][my.c]);
       Four<T> out;
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        float p = fmaf(sh.skip[my.c + j], u.get(j), sh.sy[t][my.c + j]);
+        float p = fmaf((&skip.x)[j], u.get(j), (&sum.x)[j]);
         if (a.z.p) p *= z.get(j) * sigmoid(z.get(j));
         out.set(j, t0 + t < n ? p : 0.f);
       }
@@ -378,7 +400,7 @@ __global__ void __launch_bounds__(THREADS) scan_fwd_kernel(StateScan a, SeqRef y
 template <typename T, int L, bool WIDE>
 struct BwdShared {
   static constexpr int CH = THREADS / L, PER = Mine<CH>::PER;
-  float2 sx[SPAN][CH];                // s, s u
+  float ss[SPAN][CH], su[SPAN][CH];   // s, s u
   float sq[SPAN][CH];                 // q
   float sy[SPAN][CH];                 // sum_n c h
   float sv[SPAN][CH], sd[SPAN][CH];   // sum_n g b, sum_n g a h' A
@@ -405,12 +427,12 @@ __global__ void __launch_bounds__(THREADS, 4) scan_bwd_kernel(StateScan a, const
   auto& sh = *reinterpret_cast<BwdShared<T, L, WIDE>*>(raw);
   const Tl tile(a);
   const Mine<CH> my(tile.count);
-  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, n0 = threadIdx.x % L * NS, ch = threadIdx.x / L;
+  const Place<L> me;
+  const int lane = me.lane, warp = threadIdx.x / 32, n0 = me.n0, ch = me.ch;
   const bool real = ch < tile.count;
   const int64_t n = length_of(a, tile.b), spans = (a.T + SPAN - 1) / SPAN;
   Quad rate{}, ga{}, da{};
   if (real) rate = load_rates(a, tile.c0 + ch, n0, 1.f);
-  const f2 log2e = pack(LOG2E, LOG2E);
   for (int j = threadIdx.x; j < CH; j += THREADS) {
     sh.bias[j] = a.dt_bias && j < tile.count ? a.dt_bias[tile.c0 + j] : 0.f;
     sh.skip[j] = a.skip && j < tile.count ? a.skip[tile.c0 + j] : 0.f;
@@ -448,12 +470,17 @@ __global__ void __launch_bounds__(THREADS, 4) scan_bwd_kernel(StateScan a, const
       if (t >= SPAN) break;
       const Four<T> u = now.u[i][threadIdx.x], dt = now.dt[i][threadIdx.x], z = now.z[i][threadIdx.x],
                     go = now.go[i][threadIdx.x];
+      const float4 bias = four(&sh.bias[my.c]);
+      float s[V], su[V], q[V];
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        const float s = t0 + t < n && j < my.left ? softplus(dt.get(j) + sh.bias[my.c + j]) : 0.f;
-        sh.sx[t][my.c + j] = make_float2(s, s * u.get(j));
-        sh.sq[t][my.c + j] = go.get(j) * (a.z.p ? z.get(j) * sigmoid(z.get(j)) : 1.f);
+        s[j] = t0 + t < n && j < my.left ? softplus(dt.get(j) + (&bias.x)[j]) : 0.f;
+        su[j] = s[j] * u.get(j);
+        q[j] = go.get(j) * (a.z.p ? z.get(j) * sigmoid(z.get(j)) : 1.f);
       }
+      put_four(&sh.ss[t][my.c], s);
+      put_four(&sh.su[t][my.c], su);
+      put_four(&sh.sq[t][my.c], q);
     }
     States::widen(now.bc, sh.sb);
     Quad h[SPAN + 1];  // h[t]: before token t of the span
@@ -464,9 +491,9 @@ __global__ void __launch_bounds__(THREADS, 4) scan_bwd_kernel(StateScan a, const
       float v[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const float2 x = sh.sx[t + j][ch];
+        const float s1 = sh.ss[t + j][ch] * LOG2E, su1 = sh.su[t + j][ch];
         const Quad qb = load_quad(&sh.sb[(t + j) * NS * L + n0]), qc = load_quad(&sh.sb[(SPAN + t + j) * NS * L + n0]);
-        const f2 s = mul2(pack(x.x, x.x), log2e), su = pack(x.y, x.y);
+        const f2 s = pack(s1, s1), su = pack(su1, su1);
 #pragma unroll
         for (int i = 0; i < 2; ++i)
           h[t + j + 1].v[i] = fma2(ex2_2(mul2(s, rate.v[i])), h[t + j].v[i], mul2(su, qb.v[i]));
@@ -474,10 +501,10 @@ __global__ void __launch_bounds__(THREADS, 4) scan_bwd_kernel(StateScan a, const
       }
       int first = 0;
       bool mine = true;
-      deal<4, 1, L>(v, lane, first, mine);
+      deal<4, me.CHANNELS, 32>(v, lane, first, mine);
       if (mine) {
 #pragma unroll
-        for (int j = 0; j < dealt(4, 1, L); ++j) sh.sy[t + first + j][ch] = v[j];
+        for (int j = 0; j < dealt(4, me.CHANNELS, 32); ++j) sh.sy[t + first + j][ch] = v[j];
       }
     }
 #pragma unroll
@@ -486,10 +513,9 @@ __global__ void __launch_bounds__(THREADS, 4) scan_bwd_kernel(StateScan a, const
 #pragma unroll
       for (int j = 3; j >= 0; --j) {
         const int t = t4 + j;
-        const float2 x = sh.sx[t][ch];
-        const float q1 = sh.sq[t][ch];
+        const float s1 = sh.ss[t][ch], su1 = sh.su[t][ch], q1 = sh.sq[t][ch], sl1 = s1 * LOG2E;
         const Quad qb = load_quad(&sh.sb[t * NS * L + n0]), qc = load_quad(&sh.sb[(SPAN + t) * NS * L + n0]);
-        const f2 q = pack(q1, q1), s = pack(x.x, x.x), su = pack(x.y, x.y), sl = mul2(s, log2e);
+        const f2 q = pack(q1, q1), s = pack(s1, s1), su = pack(su1, su1), sl = pack(sl1, sl1);
         f2 into = 0, through_a = 0;  // two zeros
         float w[8];                  // db and dc of this channel
 #pragma unroll
@@ -507,10 +533,10 @@ __global__ void __launch_bounds__(THREADS, 4) scan_bwd_kernel(StateScan a, const
         sums[2 * j + 1] = both(through_a);
         int first = 0;
         bool mine = true;
-        deal<8, L, 32>(w, lane, first, mine);
+        deal<8, 1, me.CHANNELS>(w, lane, first, mine);
         if (mine) {
 #pragma unroll
-          for (int i = 0; i < dealt(8, L, 32); ++i) {
+          for (int i = 0; i < dealt(8, 1, me.CHANNELS); ++i) {
             const int e = first + i;  // < NS: db of state n0 + e
             sh.red[warp][t][(e / NS) * NS * L + n0 + e % NS] = w[i];
           }
@@ -518,10 +544,10 @@ __global__ void __launch_bounds__(THREADS, 4) scan_bwd_kernel(StateScan a, const
       }
       int first = 0;
       bool mine = true;
-      deal<8, 1, L>(sums, lane, first, mine);
+      deal<8, me.CHANNELS, 32>(sums, lane, first, mine);
       if (mine) {
 #pragma unroll
-        for (int i = 0; i < dealt(8, 1, L); ++i) {
+        for (int i = 0; i < dealt(8, me.CHANNELS, 32); ++i) {
           const int e = first + i;
           (e % 2 ? sh.sd : sh.sv)[t4 + e / 2][ch] = sums[i];
         }
@@ -537,16 +563,19 @@ __global__ void __launch_bounds__(THREADS, 4) scan_bwd_kernel(StateScan a, const
                     go = now.go[i][threadIdx.x];
       Four<T> du, ddt, dz;
       float4 ds = sh.sums[0][threadIdx.x], db = sh.sums[1][threadIdx.x];
+      const float4 q4 = four(&sh.sq[t][my.c]), v4 = four(&sh.sv[t][my.c]), d4 = four(&sh.sd[t][my.c]),
+                   y4 = four(&sh.sy[t][my.c]), s4 = four(&sh.ss[t][my.c]), skip4 = four(&sh.skip[my.c]),
+                   bias4 = four(&sh.bias[my.c]);
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        const float uj = u.get(j), zj = z.get(j), q = sh.sq[t][my.c + j], v = sh.sv[t][my.c + j], skip = sh.skip[my.c + j];
-        du.set(j, here ? fmaf(v, sh.sx[t][my.c + j].x, q * skip) : 0.f);
-        const float dr = here ? fmaf(v, uj, sh.sd[t][my.c + j]) * sigmoid(dt.get(j) + sh.bias[my.c + j]) : 0.f;
+        const float uj = u.get(j), zj = z.get(j), q = (&q4.x)[j], v = (&v4.x)[j], skip = (&skip4.x)[j];
+        du.set(j, here ? fmaf(v, (&s4.x)[j], q * skip) : 0.f);
+        const float dr = here ? fmaf(v, uj, (&d4.x)[j]) * sigmoid(dt.get(j) + (&bias4.x)[j]) : 0.f;
         ddt.set(j, dr);
         (&ds.x)[j] = fmaf(q, uj, (&ds.x)[j]);
         (&db.x)[j] += dr;
         const float sz = sigmoid(zj);
-        dz.set(j, here ? go.get(j) * fmaf(skip, uj, sh.sy[t][my.c + j]) * sz * fmaf(zj, 1.f - sz, 1.f) : 0.f);
+        dz.set(j, here ? go.get(j) * fmaf(skip, uj, (&y4.x)[j]) * sz * fmaf(zj, 1.f - sz, 1.f) : 0.f);
       }
       sh.sums[0][threadIdx.x] = ds;
       sh.sums[1][threadIdx.x] = db;
