@@ -222,7 +222,7 @@ std::vector<OptTensor> state_scan_fwd_op(const at::Tensor& u, const at::Tensor& 
   const Call& k = v.call;
   c10::cuda::CUDAGuard g(k.device);
   at::AutoDispatchBelowADInplaceOrView below;
-  at::Tensor y = at::empty({k.B, k.T, k.D}, u.options()), last, saved;
+  at::Tensor y = at::empty({k.B, k.T, k.D}, u.options()), last, saved, scratch;
   const auto f32 = at::TensorOptions().dtype(at::kFloat).device(k.device);
   if (want_state || out_state.has_value()) {
     last = written(k, out_state, "out_state", at::kFloat, {k.B, k.D, v.a.N});
@@ -231,8 +231,10 @@ std::vector<OptTensor> state_scan_fwd_op(const at::Tensor& u, const at::Tensor& 
     in_place_or_apart(k, last, v.state);
   }
   if (save) saved = at::empty({k.B, (k.T + STATE_SCAN_SPAN - 1) / STATE_SCAN_SPAN, k.D, v.a.N}, f32);
+  const int64_t floats = state_scan_fwd_scratch_floats(v.a);
+  if (floats > 0) scratch = at::empty({floats}, f32);
   state_scan_fwd(v.a, {y.data_ptr(), y.stride(0), y.stride(1)}, last.defined() ? last.data_ptr<float>() : nullptr,
-                 save ? saved.data_ptr<float>() : nullptr, stream());
+                 save ? saved.data_ptr<float>() : nullptr, floats > 0 ? scratch.data_ptr<float>() : nullptr, stream());
   return {y, last.defined() ? OptTensor(last) : c10::nullopt, save ? OptTensor(saved) : c10::nullopt};
 }
 
@@ -278,7 +280,7 @@ std::vector<OptTensor> state_scan_bwd_op(const at::Tensor& u, const at::Tensor& 
   in.push_back(dyk);
   in.push_back(saved);
   apart(k, {gu, gdt, gb, gc, gz, *da_log, dskip.value_or(at::Tensor()), ddt_bias.value_or(at::Tensor())}, in);
-  at::Tensor scratch = at::empty({std::max<int64_t>(1, state_scan_scratch_floats(v.a))}, f32);
+  at::Tensor scratch = at::empty({std::max<int64_t>(1, state_scan_bwd_scratch_floats(v.a))}, f32);
   state_scan_bwd(v.a, saved.data_ptr<float>(), go, r, scratch.data_ptr<float>(), stream());
   return {gu, gdt, da_log, gb, gc, dskip, gz.defined() ? OptTensor(gz) : c10::nullopt, ddt_bias};
 }

@@ -492,14 +492,16 @@ struct StateScan {
 };
 // out_state [B, D, N] (may be `state`): h after the last token that counts.
 // saved [B, ceil(T / STATE_SCAN_SPAN), D, N]: h before every span's first token, for the backward pass.
-void state_scan_fwd(const StateScan& a, SeqRef y, float* out_state, float* saved, cudaStream_t s);
+// scratch: state_scan_fwd_scratch_floats() floats.
+int64_t state_scan_fwd_scratch_floats(const StateScan& a);
+void state_scan_fwd(const StateScan& a, SeqRef y, float* out_state, float* saved, float* scratch, cudaStream_t s);
 struct StateScanGrads {
   SeqRef du, ddt, dz, db, dc;                                      // all written; dz where there is z
   float *da_log = nullptr, *dskip = nullptr, *ddt_bias = nullptr;  // written or (accumulate) added to; null: not wanted
   bool accumulate = false;
 };
-// scratch: state_scan_scratch_floats() floats.
-int64_t state_scan_scratch_floats(const StateScan& a);
+// scratch: state_scan_bwd_scratch_floats() floats.
+int64_t state_scan_bwd_scratch_floats(const StateScan& a);
 void state_scan_bwd(const StateScan& a, const float* saved, SeqRef dy, const StateScanGrads& g, float* scratch,
                     cudaStream_t s);
 

@@ -204,27 +204,27 @@ __device__ __forceinline__ void deal(float* v, int lane, int& first, bool& mine)
   }
 }
 
-// b and c of a span, b's rows of NS L states and then c's, zeros past N; a
-// thread has four neighbouring states at a time.
-template <typename T, int L, bool WIDE>
+// Rows of NS L states of a span, of b and behind them of c (or of one of them),
+// zeros past N; a thread has four neighbouring states at a time.
+template <typename T, int L, bool WIDE, int COUNT>
 struct SpanStates {
-  static constexpr int PER = (2 * SPAN * L + THREADS - 1) / THREADS;
+  static constexpr int PER = (COUNT * SPAN * L + THREADS - 1) / THREADS;
   using Stage = Four<T>[PER][THREADS];
-  __device__ __forceinline__ static void fetch(Stage& to, const StateScan& a, int64_t seq, int group, int64_t t0, int64_t n) {
+  __device__ __forceinline__ static void fetch(Stage& to, const SeqRef& first, const SeqRef& second, int64_t seq,
+                                               int group, int N, int64_t t0, int64_t n) {
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
       const int e = threadIdx.x + i * THREADS, t = e / L % SPAN, k = e % L * NS;
-      const SeqRef& r = e < SPAN * L ? a.b : a.c;
-      if (e < 2 * SPAN * L)
-        fetch_four<T, WIDE>(&to[i][threadIdx.x], at<T>(r, seq, t0 + t, (int64_t)group * a.N + k), r.p,
-                            t0 + t < n ? a.N - k : 0);
+      const SeqRef& r = COUNT == 1 || e < SPAN * L ? first : second;
+      if (e < COUNT * SPAN * L)
+        fetch_four<T, WIDE>(&to[i][threadIdx.x], at<T>(r, seq, t0 + t, (int64_t)group * N + k), r.p, t0 + t < n ? N - k : 0);
     }
   }
   __device__ __forceinline__ static void widen(const Stage& from, float* sb) {
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
       const int e = threadIdx.x + i * THREADS;
-      if (e < 2 * SPAN * L) {
+      if (e < COUNT * SPAN * L) {
         const Four<T> f = from[i][threadIdx.x];
         *reinterpret_cast<float4*>(sb + e * NS) = make_float4(f.get(0), f.get(1), f.get(2), f.get(3));
       }
@@ -278,6 +278,138 @@ struct Mine {
       : c(threadIdx.x * V % CH), t(threadIdx.x * V / CH), left(count - (int)(threadIdx.x * V % CH)) {}
 };
 
+// ---------------------------------------------------------------- pieces of the tokens
+// Few channels leave most of the GPU idle, so long sequences are cut into pieces
+// that run side by side: one pass takes each piece from a state of zeros to its
+// end, the ends are joined in order (a piece's decays are exp(A sum s)), and the
+// pass proper starts every piece from the state before it.  That makes the
+// exponentials twice; where the channels fill the GPU there is one piece.
+struct Pieces {
+  int count = 1;
+  int64_t spans = 0;        // of a piece
+  float* ends = nullptr;    // [B][count][D][N]: the state after a piece of its own; joined: before it
+  float* steps = nullptr;   // [B][count][D]: sum of s
+};
+
+template <typename T, int L, bool WIDE>
+struct EndsShared {
+  static constexpr int CH = THREADS / L, PER = Mine<CH>::PER;
+  float ss[SPAN][CH], sx[SPAN][CH];  // s; s u, or q
+  float sb[SPAN * NS * L];           // b, or c
+  float bias[CH];
+  float4 sums[THREADS];              // of a thread's steps
+  struct {
+    Four<T> dt[PER][THREADS], x[PER][THREADS], z[PER][THREADS];
+    typename SpanStates<T, L, WIDE, 1>::Stage bc;
+  } stage[2];
+};
+
+// The end of a piece.  Forward: h[t] = a[t] h[t-1] + s u b[t].  BACK (what
+// reaches the token before the piece): g[t] = c[t] q + a[t+1] g[t+1], times a[t].
+template <typename T, int L, bool WIDE, bool BACK>
+__global__ void __launch_bounds__(THREADS) scan_ends_kernel(StateScan a, SeqRef dy, Pieces pieces) {
+  using States = SpanStates<T, L, WIDE, 1>;
+  constexpr int CH = THREADS / L;
+  extern __shared__ __align__(16) char raw[];
+  auto& sh = *reinterpret_cast<EndsShared<T, L, WIDE>*>(raw);
+  const Tile<L> tile(a);
+  const Mine<CH> my(tile.count);
+  const Place<L> me;
+  const bool real = me.ch < tile.count;
+  const int64_t n = length_of(a, tile.b), spans = (a.T + SPAN - 1) / SPAN;
+  const int64_t from = blockIdx.y * pieces.spans, to = min(spans, from + pieces.spans);
+  Quad h{}, rate{};
+  if (real) rate = load_rates(a, tile.c0 + me.ch, me.n0, LOG2E);
+  for (int j = threadIdx.x; j < CH; j += THREADS) sh.bias[j] = a.dt_bias && j < tile.count ? a.dt_bias[tile.c0 + j] : 0.f;
+  float total[V] = {0.f, 0.f, 0.f, 0.f};
+  const auto fetch = [&](int64_t k) {
+    auto& st = sh.stage[k % 2];
+    const int64_t t0 = k * SPAN;
+#pragma unroll
+    for (int i = 0; i < my.PER; ++i) {
+      const int t = my.t + i * my.STEP;
+      if (t >= SPAN) break;
+      const int count = t0 + t < n ? my.left : 0;
+      const SeqRef& x = BACK ? dy : a.u;
+      fetch_four<T, WIDE>(&st.dt[i][threadIdx.x], at<T>(a.dt, tile.b, t0 + t, tile.c0 + my.c), a.dt.p, count);
+      fetch_four<T, WIDE>(&st.x[i][threadIdx.x], at<T>(x, tile.b, t0 + t, tile.c0 + my.c), x.p, count);
+      if (BACK && a.z.p)
+        fetch_four<T, WIDE>(&st.z[i][threadIdx.x], at<T>(a.z, tile.b, t0 + t, tile.c0 + my.c), a.z.p, count);
+    }
+    States::fetch(st.bc, BACK ? a.c : a.b, a.b, tile.b, tile.group, a.N, t0, n);
+  };
+  const int64_t count = to - from;
+  const auto span_of = [&](int64_t i) { return BACK ? to - 1 - i : from + i; };
+  if (count > 0) fetch(span_of(0));
+  copies_issued();
+  __syncthreads();
+  for (int64_t i = 0; i < count; ++i) {
+    const int64_t k = span_of(i), t0 = k * SPAN;
+    auto& now = sh.stage[k % 2];
+    if (i + 1 < count) fetch(span_of(i + 1));
+    copies_issued();
+    wait_but_last();
+#pragma unroll
+    for (int e = 0; e < my.PER; ++e) {
+      const int t = my.t + e * my.STEP;
+      if (t >= SPAN) break;
+      const Four<T> dt = now.dt[e][threadIdx.x], x = now.x[e][threadIdx.x], z = now.z[e][threadIdx.x];
+      const float4 bias = four(&sh.bias[my.c]);
+      float s[V], sx[V];
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        s[j] = t0 + t < n && j < my.left ? softplus(dt.get(j) + (&bias.x)[j]) : 0.f;
+        total[j] += s[j];
+        sx[j] = !BACK ? s[j] * x.get(j) : a.z.p ? x.get(j) * z.get(j) * sigmoid(z.get(j)) : x.get(j);
+      }
+      put_four(&sh.ss[t][my.c], s);
+      put_four(&sh.sx[t][my.c], sx);
+    }
+    States::widen(now.bc, sh.sb);
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < SPAN; ++j) {
+      const int t = BACK ? SPAN - 1 - j : j;
+      const float s1 = sh.ss[t][me.ch], x1 = sh.sx[t][me.ch];
+      const Quad q = load_quad(&sh.sb[t * NS * L + me.n0]);
+      const f2 s = pack(s1, s1), x = pack(x1, x1);
+#pragma unroll
+      for (int v = 0; v < 2; ++v) {
+        const f2 decay = ex2_2(mul2(s, rate.v[v]));
+        h.v[v] = BACK ? mul2(fma2(x, q.v[v], h.v[v]), decay) : fma2(decay, h.v[v], mul2(x, q.v[v]));
+      }
+    }
+    __syncthreads();
+  }
+  const int64_t piece = tile.b * pieces.count + blockIdx.y;
+  if (real) store_states(h, pieces.ends + (piece * a.D + tile.c0 + me.ch) * a.N + me.n0, me.n0, a.N);
+  put_four(&sh.sums[threadIdx.x].x, total);
+  __syncthreads();
+  constexpr int SAME = CH / V, ROWS = SPAN * SAME < THREADS ? SPAN * SAME : THREADS;
+  for (int j = threadIdx.x; j < tile.count; j += THREADS) {
+    float s = 0.f;
+    for (int r = j / V; r < ROWS; r += SAME) s += (&sh.sums[r].x)[j % V];
+    pieces.steps[piece * a.D + tile.c0 + j] = s;
+  }
+}
+
+// ends: from what a piece ends with to what the one before it (BACK: behind it) passes on to it.
+template <bool BACK>
+__global__ void __launch_bounds__(256) scan_join_kernel(StateScan a, Pieces pieces) {
+  const int64_t dn = (int64_t)a.D * a.N, i = blockIdx.x * 256LL + threadIdx.x;
+  if (i >= a.B * dn) return;
+  const int64_t b = i / dn, e = i % dn, d = e / a.N;
+  const float rate = -expf(a.a_log[e]);
+  float carry = !BACK && a.state ? a.state[i] : 0.f;
+  for (int j = 0; j < pieces.count; ++j) {
+    const int64_t piece = b * pieces.count + (BACK ? pieces.count - 1 - j : j);
+    float& end = pieces.ends[piece * dn + e];
+    const float own = end;
+    end = carry;
+    carry = fmaf(expf(rate * pieces.steps[piece * a.D + d]), carry, own);
+  }
+}
+
 // ---------------------------------------------------------------- forward
 template <typename T, int L, bool WIDE>
 struct FwdShared {
@@ -288,14 +420,15 @@ struct FwdShared {
   float bias[CH], skip[CH];
   struct {
     Four<T> u[PER][THREADS], dt[PER][THREADS], z[PER][THREADS];
-    typename SpanStates<T, L, WIDE>::Stage bc;
+    typename SpanStates<T, L, WIDE, 2>::Stage bc;
   } stage[2];
 };
 
 template <typename T, int L, bool WIDE>
-__global__ void __launch_bounds__(THREADS) scan_fwd_kernel(StateScan a, SeqRef y, float* out_state, float* saved) {
+__global__ void __launch_bounds__(THREADS) scan_fwd_kernel(StateScan a, SeqRef y, float* out_state, float* saved,
+                                                           Pieces pieces) {
   using Tl = Tile<L>;
-  using States = SpanStates<T, L, WIDE>;
+  using States = SpanStates<T, L, WIDE, 2>;
   constexpr int CH = Tl::CH;
   extern __shared__ __align__(16) char raw[];
   auto& sh = *reinterpret_cast<FwdShared<T, L, WIDE>*>(raw);
@@ -305,10 +438,14 @@ __global__ void __launch_bounds__(THREADS) scan_fwd_kernel(StateScan a, SeqRef y
   const int lane = me.lane, n0 = me.n0, ch = me.ch;
   const bool real = ch < tile.count;
   const int64_t n = length_of(a, tile.b), spans = (a.T + SPAN - 1) / SPAN;
+  const int64_t from = blockIdx.y * pieces.spans, to = min(spans, from + pieces.spans);
   const int64_t row = (tile.b * a.D + tile.c0 + ch) * a.N + n0;  // of this thread's states
   Quad h{}, rate{};
   if (real) {
-    if (a.state) h = load_states(a.state + row, n0, a.N);
+    if (pieces.ends)
+      h = load_states(pieces.ends + ((tile.b * pieces.count + blockIdx.y) * a.D + tile.c0 + ch) * a.N + n0, n0, a.N);
+    else if (a.state)
+      h = load_states(a.state + row, n0, a.N);
     rate = load_rates(a, tile.c0 + ch, n0, LOG2E);
   }
   for (int j = threadIdx.x; j < CH; j += THREADS) {
@@ -316,26 +453,26 @@ __global__ void __launch_bounds__(THREADS) scan_fwd_kernel(StateScan a, SeqRef y
     sh.skip[j] = a.skip && j < tile.count ? a.skip[tile.c0 + j] : 0.f;
   }
   const auto fetch = [&](int64_t k) {
-    auto& to = sh.stage[k % 2];
+    auto& st = sh.stage[k % 2];
     const int64_t t0 = k * SPAN;
 #pragma unroll
     for (int i = 0; i < my.PER; ++i) {
       const int t = my.t + i * my.STEP;
       if (t >= SPAN) break;
       const int count = t0 + t < n ? my.left : 0;
-      fetch_four<T, WIDE>(&to.u[i][threadIdx.x], at<T>(a.u, tile.b, t0 + t, tile.c0 + my.c), a.u.p, count);
-      fetch_four<T, WIDE>(&to.dt[i][threadIdx.x], at<T>(a.dt, tile.b, t0 + t, tile.c0 + my.c), a.dt.p, count);
-      if (a.z.p) fetch_four<T, WIDE>(&to.z[i][threadIdx.x], at<T>(a.z, tile.b, t0 + t, tile.c0 + my.c), a.z.p, count);
+      fetch_four<T, WIDE>(&st.u[i][threadIdx.x], at<T>(a.u, tile.b, t0 + t, tile.c0 + my.c), a.u.p, count);
+      fetch_four<T, WIDE>(&st.dt[i][threadIdx.x], at<T>(a.dt, tile.b, t0 + t, tile.c0 + my.c), a.dt.p, count);
+      if (a.z.p) fetch_four<T, WIDE>(&st.z[i][threadIdx.x], at<T>(a.z, tile.b, t0 + t, tile.c0 + my.c), a.z.p, count);
     }
-    States::fetch(to.bc, a, tile.b, tile.group, t0, n);
+    States::fetch(st.bc, a.b, a.c, tile.b, tile.group, a.N, t0, n);
   };
-  if (spans > 0) fetch(0);
+  if (from < to) fetch(from);
   copies_issued();
   __syncthreads();
-  for (int64_t k = 0; k < spans; ++k) {
+  for (int64_t k = from; k < to; ++k) {
     const int64_t t0 = k * SPAN;
     auto& now = sh.stage[k % 2];
-    if (k + 1 < spans) fetch(k + 1);
+    if (k + 1 < to) fetch(k + 1);
     copies_issued();
     wait_but_last();
 #pragma unroll
@@ -393,7 +530,68 @@ __global__ void __launch_bounds__(THREADS) scan_fwd_kernel(StateScan a, SeqRef y
       out.template store<WIDE>(at<T>(y, tile.b, t0 + t, tile.c0 + my.c), my.left);
     }
   }
-  if (out_state && real) store_states(h, out_state + row, n0, a.N);
+  if (out_state && real && blockIdx.y + 1 == pieces.count) store_states(h, out_state + row, n0, a.N);
+}
+
+// One token of each sequence: a thread has four states of a channel, neighbours'
+// states are neighbours, and nothing passes through shared memory.
+template <typename T, int L, bool WIDE>
+__global__ void __launch_bounds__(THREADS) scan_step_kernel(StateScan a, SeqRef y, float* out_state, float* saved) {
+  const int64_t i = blockIdx.x * (int64_t)THREADS + threadIdx.x, channel = i / L;
+  const bool real = channel < a.B * a.D;
+  const int64_t b = real ? channel / a.D : 0;
+  const int d = real ? (int)(channel % a.D) : 0, n0 = (int)(i % L) * NS, group = d / (a.D / a.G);
+  const bool here = length_of(a, b) > 0;
+  const int64_t row = (b * a.D + d) * a.N + n0;
+  const T *pb = at<T>(a.b, b, 0, (int64_t)group * a.N + n0), *pc = at<T>(a.c, b, 0, (int64_t)group * a.N + n0);
+  float h[NS], rate[NS], bb[NS], cc[NS];
+  const int count = real ? a.N - n0 : 0;
+  if (WIDE && count > 0) {
+    const float4 r4 = four(a.a_log + (int64_t)d * a.N + n0), h4 = a.state ? four(a.state + row) : make_float4(0.f, 0.f, 0.f, 0.f);
+    Four<T> fb, fc;
+    fb.raw = *reinterpret_cast<const typename Raw<T>::type*>(pb);
+    fc.raw = *reinterpret_cast<const typename Raw<T>::type*>(pc);
+#pragma unroll
+    for (int j = 0; j < NS; ++j) h[j] = (&h4.x)[j], rate[j] = (&r4.x)[j], bb[j] = fb.get(j), cc[j] = fc.get(j);
+  } else {
+#pragma unroll
+    for (int j = 0; j < NS; ++j) {
+      const bool in = j < count;
+      h[j] = in && a.state ? a.state[row + j] : 0.f;
+      rate[j] = in ? a.a_log[(int64_t)d * a.N + n0 + j] : 0.f;
+      bb[j] = in ? to_f32(pb[j]) : 0.f;
+      cc[j] = in ? to_f32(pc[j]) : 0.f;
+    }
+  }
+  if (saved) {
+#pragma unroll
+    for (int j = 0; j < NS; ++j)
+      if (j < count) saved[row + j] = h[j];
+  }
+  const float u = to_f32(*at<T>(a.u, b, 0, d)), raw = to_f32(*at<T>(a.dt, b, 0, d)) + (a.dt_bias ? a.dt_bias[d] : 0.f);
+  const float z = a.z.p ? to_f32(*at<T>(a.z, b, 0, d)) : 0.f, skip = a.skip ? a.skip[d] : 0.f;
+  const float s = softplus(raw), su = s * u;
+  float p = 0.f;
+#pragma unroll
+  for (int j = 0; j < NS; ++j) {
+    if (here && j < count) h[j] = fmaf(ex2(-s * expf(rate[j]) * LOG2E), h[j], su * bb[j]);
+    p = fmaf(j < count ? cc[j] : 0.f, h[j], p);
+  }
+  if (out_state) {
+    if (WIDE && count > 0) {
+      put_four(out_state + row, h);
+    } else {
+#pragma unroll
+      for (int j = 0; j < NS; ++j)
+        if (j < count) out_state[row + j] = h[j];
+    }
+  }
+#pragma unroll
+  for (int o = 1; o < L; o <<= 1) p += __shfl_xor_sync(0xffffffffu, p, o);
+  if (!real || n0) return;
+  p = fmaf(skip, u, p);
+  if (a.z.p) p *= z * sigmoid(z);
+  *at<T>(y, b, 0, d) = from_f32<T>(here ? p : 0.f);
 }
 
 // ---------------------------------------------------------------- backward
@@ -410,18 +608,18 @@ struct BwdShared {
   float bias[CH], skip[CH];
   struct {
     Four<T> u[PER][THREADS], dt[PER][THREADS], z[PER][THREADS], go[PER][THREADS];
-    typename SpanStates<T, L, WIDE>::Stage bc;
+    typename SpanStates<T, L, WIDE, 2>::Stage bc;
     float4 h[THREADS];
   } stage[2];
 };
 
-// part_bc [tiles of a group][B][T][G][2][NS L]; part_d [B][D][N + 2]: da, dskip, ddt_bias.
+// part_bc [tiles of a group][B][T][G][2][NS L]; part_d [B][pieces][D][N + 2]: da, dskip, ddt_bias.
 template <typename T, int L, bool WIDE>
 __global__ void __launch_bounds__(THREADS, 4) scan_bwd_kernel(StateScan a, const float* __restrict__ saved, SeqRef dy,
                                                               StateScanGrads g, float* __restrict__ part_bc,
-                                                              float* __restrict__ part_d) {
+                                                              float* __restrict__ part_d, Pieces pieces) {
   using Tl = Tile<L>;
-  using States = SpanStates<T, L, WIDE>;
+  using States = SpanStates<T, L, WIDE, 2>;
   constexpr int CH = Tl::CH, ROW = 2 * NS * L;
   extern __shared__ __align__(16) char raw[];
   auto& sh = *reinterpret_cast<BwdShared<T, L, WIDE>*>(raw);
@@ -432,36 +630,41 @@ __global__ void __launch_bounds__(THREADS, 4) scan_bwd_kernel(StateScan a, const
   const bool real = ch < tile.count;
   const int64_t n = length_of(a, tile.b), spans = (a.T + SPAN - 1) / SPAN;
   Quad rate{}, ga{}, da{};
-  if (real) rate = load_rates(a, tile.c0 + ch, n0, 1.f);
+  const int64_t from = blockIdx.y * pieces.spans, to = min(spans, from + pieces.spans);
+  const int64_t piece = tile.b * pieces.count + blockIdx.y;
+  if (real) {
+    rate = load_rates(a, tile.c0 + ch, n0, 1.f);
+    if (pieces.ends) ga = load_states(pieces.ends + (piece * a.D + tile.c0 + ch) * a.N + n0, n0, a.N);
+  }
   for (int j = threadIdx.x; j < CH; j += THREADS) {
     sh.bias[j] = a.dt_bias && j < tile.count ? a.dt_bias[tile.c0 + j] : 0.f;
     sh.skip[j] = a.skip && j < tile.count ? a.skip[tile.c0 + j] : 0.f;
   }
   sh.sums[0][threadIdx.x] = sh.sums[1][threadIdx.x] = make_float4(0.f, 0.f, 0.f, 0.f);
   const auto fetch = [&](int64_t k) {
-    auto& to = sh.stage[k % 2];
+    auto& st = sh.stage[k % 2];
     const int64_t t0 = k * SPAN;
 #pragma unroll
     for (int i = 0; i < my.PER; ++i) {
       const int t = my.t + i * my.STEP;
       if (t >= SPAN) break;
       const int count = t0 + t < n ? my.left : 0;
-      fetch_four<T, WIDE>(&to.u[i][threadIdx.x], at<T>(a.u, tile.b, t0 + t, tile.c0 + my.c), a.u.p, count);
-      fetch_four<T, WIDE>(&to.dt[i][threadIdx.x], at<T>(a.dt, tile.b, t0 + t, tile.c0 + my.c), a.dt.p, count);
-      if (a.z.p) fetch_four<T, WIDE>(&to.z[i][threadIdx.x], at<T>(a.z, tile.b, t0 + t, tile.c0 + my.c), a.z.p, count);
-      fetch_four<T, WIDE>(&to.go[i][threadIdx.x], at<T>(dy, tile.b, t0 + t, tile.c0 + my.c), dy.p, count);
+      fetch_four<T, WIDE>(&st.u[i][threadIdx.x], at<T>(a.u, tile.b, t0 + t, tile.c0 + my.c), a.u.p, count);
+      fetch_four<T, WIDE>(&st.dt[i][threadIdx.x], at<T>(a.dt, tile.b, t0 + t, tile.c0 + my.c), a.dt.p, count);
+      if (a.z.p) fetch_four<T, WIDE>(&st.z[i][threadIdx.x], at<T>(a.z, tile.b, t0 + t, tile.c0 + my.c), a.z.p, count);
+      fetch_four<T, WIDE>(&st.go[i][threadIdx.x], at<T>(dy, tile.b, t0 + t, tile.c0 + my.c), dy.p, count);
     }
-    States::fetch(to.bc, a, tile.b, tile.group, t0, n);
-    fetch_four<float, WIDE>(reinterpret_cast<Four<float>*>(&to.h[threadIdx.x]),
+    States::fetch(st.bc, a.b, a.c, tile.b, tile.group, a.N, t0, n);
+    fetch_four<float, WIDE>(reinterpret_cast<Four<float>*>(&st.h[threadIdx.x]),
                             saved + ((tile.b * spans + k) * a.D + tile.c0 + ch) * a.N + n0, saved, real ? a.N - n0 : 0);
   };
-  if (spans > 0) fetch(spans - 1);
+  if (from < to) fetch(to - 1);
   copies_issued();
   __syncthreads();
-  for (int64_t k = spans - 1; k >= 0; --k) {
+  for (int64_t k = to - 1; k >= from; --k) {
     const int64_t t0 = k * SPAN;
     auto& now = sh.stage[k % 2];
-    if (k > 0) fetch(k - 1);
+    if (k > from) fetch(k - 1);
     copies_issued();
     wait_but_last();
 #pragma unroll
@@ -598,7 +801,7 @@ __global__ void __launch_bounds__(THREADS, 4) scan_bwd_kernel(StateScan a, const
     // (the barrier after the next span's elements is between these reads and what comes to their places)
   }
   if (real) store_states({{mul2(da.v[0], rate.v[0]), mul2(da.v[1], rate.v[1])}},
-                         part_d + (tile.b * a.D + tile.c0 + ch) * (a.N + 2) + n0, n0, a.N);
+                         part_d + (piece * a.D + tile.c0 + ch) * (a.N + 2) + n0, n0, a.N);
   // dskip and ddt_bias: threads CH / V apart hold the same channels
   constexpr int SAME = CH / V, ROWS = SPAN * SAME < THREADS ? SPAN * SAME : THREADS;
   __syncthreads();
@@ -606,7 +809,7 @@ __global__ void __launch_bounds__(THREADS, 4) scan_bwd_kernel(StateScan a, const
     const int half = i / CH, at_ch = i % CH;
     float s = 0.f;
     for (int r = at_ch / V; r < ROWS; r += SAME) s += (&sh.sums[half][r].x)[at_ch % V];
-    if (at_ch < tile.count) part_d[(tile.b * a.D + tile.c0 + at_ch) * (a.N + 2) + a.N + half] = s;
+    if (at_ch < tile.count) part_d[(piece * a.D + tile.c0 + at_ch) * (a.N + 2) + a.N + half] = s;
   }
 }
 
@@ -624,7 +827,7 @@ __global__ void __launch_bounds__(256) join_bc_kernel(const float* __restrict__ 
     *at<T>(half ? dc : db, b, t, (int64_t)group * N + n) = from_f32<T>(s);
   }
 }
-// da_log, dskip and ddt_bias: the sums over the sequences.
+// da_log, dskip and ddt_bias: the sums over the sequences and their pieces.
 __global__ void __launch_bounds__(256) join_d_kernel(const float* __restrict__ part, int64_t B, int D, int N,
                                                      StateScanGrads g) {
   const int64_t total = (int64_t)D * (N + 2), i = blockIdx.x * 256LL + threadIdx.x;
@@ -672,10 +875,10 @@ void check(const StateScan& a) {
 
 namespace {
 template <typename Kernel, typename... Args>
-void launch(Kernel kernel, size_t smem, const StateScan& a, cudaStream_t s, Args... args) {
+void launch(Kernel kernel, size_t smem, const StateScan& a, int pieces, cudaStream_t s, Args... args) {
   if (smem > 48 * 1024)
     DLVK_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-  kernel<<<grid_of(a), THREADS, smem, s>>>(a, args...);
+  kernel<<<dim3(grid_of(a), pieces), THREADS, smem, s>>>(a, args...);
   DLVK_POST_LAUNCH();
 }
 // f(element type, lanes of a channel, whether rows are of whole aligned fours)
@@ -696,30 +899,71 @@ bool wide_operands(const StateScan& a) {
          aligned(a.b, a.type) && aligned(a.c, a.type);
 }
 int64_t part_bc_floats(const StateScan& a) { return (int64_t)tiles_of(a) * a.B * a.T * a.G * 2 * NS * lanes_of(a.N); }
+
+// Pieces as long as there are blocks for them at once (`fill` fit the GPU), of at
+// least 8 spans each; one piece where two would not both fit.
+Pieces pieces_of(const StateScan& a, int64_t fill) {
+  Pieces p;
+  const int64_t spans = (a.T + SPAN - 1) / SPAN, blocks = std::max<int64_t>(1, a.B * a.G * tiles_of(a));
+  const int64_t most = std::min(fill / blocks, spans / 8);
+  p.spans = most >= 2 ? (spans + most - 1) / most : std::max<int64_t>(spans, 1);
+  p.count = (int)((spans + p.spans - 1) / p.spans);
+  if (p.count < 1) p.count = 1;
+  return p;
+}
+constexpr int64_t FWD_FILL = 148 * 7, BWD_FILL = 148 * 4;
+int64_t pieces_floats(const StateScan& a, const Pieces& p) { return p.count > 1 ? a.B * p.count * a.D * (a.N + 1) : 0; }
+
+template <typename T, int L, bool W, bool BACK>
+void join_pieces(const StateScan& a, SeqRef dy, Pieces& p, float* scratch, cudaStream_t s) {
+  if (p.count == 1) return;
+  p.ends = scratch;
+  p.steps = scratch + a.B * p.count * a.D * a.N;
+  launch(scan_ends_kernel<T, L, W, BACK>, sizeof(EndsShared<T, L, W>), a, p.count, s, dy, p);
+  scan_join_kernel<BACK><<<(unsigned)((a.B * a.D * a.N + 255) / 256), 256, 0, s>>>(a, p);
+  DLVK_POST_LAUNCH();
+}
 }  // namespace
 
-void state_scan_fwd(const StateScan& a, SeqRef y, float* out_state, float* saved, cudaStream_t s) {
+int64_t state_scan_fwd_scratch_floats(const StateScan& a) {
+  check(a);
+  return pieces_floats(a, pieces_of(a, FWD_FILL));
+}
+
+void state_scan_fwd(const StateScan& a, SeqRef y, float* out_state, float* saved, float* scratch, cudaStream_t s) {
   check(a);
   if (a.B == 0 || a.D == 0) return;
   by_kind(a, wide_operands(a) && aligned(y, a.type), [&](auto type, auto lanes, auto wide) {
     using T = decltype(type);
     constexpr int L = decltype(lanes)::value;
     constexpr bool W = decltype(wide)::value;
-    launch(scan_fwd_kernel<T, L, W>, sizeof(FwdShared<T, L, W>), a, s, y, out_state, saved);
+    if (a.T == 1) {
+      const int64_t blocks = (a.B * a.D * L + THREADS - 1) / THREADS;
+      DLVK_CHECK(blocks < (1LL << 31), "state_scan: too many channels for one launch");
+      scan_step_kernel<T, L, W><<<(unsigned)blocks, THREADS, 0, s>>>(a, y, out_state, saved);
+      DLVK_POST_LAUNCH();
+      return;
+    }
+    Pieces p = pieces_of(a, FWD_FILL);
+    join_pieces<T, L, W, false>(a, {}, p, scratch, s);
+    launch(scan_fwd_kernel<T, L, W>, sizeof(FwdShared<T, L, W>), a, p.count, s, y, out_state, saved, p);
   });
 }
 
-int64_t state_scan_scratch_floats(const StateScan& a) {
+int64_t state_scan_bwd_scratch_floats(const StateScan& a) {
   check(a);
-  return part_bc_floats(a) + a.B * a.D * (a.N + 2);
+  const Pieces p = pieces_of(a, BWD_FILL);
+  return part_bc_floats(a) + a.B * p.count * a.D * (a.N + 2) + pieces_floats(a, p);
 }
 
 void state_scan_bwd(const StateScan& a, const float* saved, SeqRef dy, const StateScanGrads& g, float* scratch,
                     cudaStream_t s) {
   check(a);
   if (a.D == 0) return;
+  Pieces p = pieces_of(a, BWD_FILL);
   float* part_bc = scratch;
-  float* part_d = scratch + part_bc_floats(a);
+  float* part_d = part_bc + part_bc_floats(a);
+  float* ends = part_d + a.B * p.count * a.D * (a.N + 2);
   if (a.B > 0) {
     const bool w = wide_operands(a) && aligned(dy, a.type) && aligned(g.du, a.type) && aligned(g.ddt, a.type) &&
                    aligned(g.dz, a.type);
@@ -727,7 +971,8 @@ void state_scan_bwd(const StateScan& a, const float* saved, SeqRef dy, const Sta
       using T = decltype(type);
       constexpr int L = decltype(lanes)::value;
       constexpr bool W = decltype(wide)::value;
-      launch(scan_bwd_kernel<T, L, W>, sizeof(BwdShared<T, L, W>), a, s, saved, dy, g, part_bc, part_d);
+      join_pieces<T, L, W, true>(a, dy, p, ends, s);
+      launch(scan_bwd_kernel<T, L, W>, sizeof(BwdShared<T, L, W>), a, p.count, s, saved, dy, g, part_bc, part_d, p);
     });
     const int64_t total = part_bc_floats(a) / tiles_of(a);
     if (total > 0) {
@@ -740,7 +985,7 @@ void state_scan_bwd(const StateScan& a, const float* saved, SeqRef dy, const Sta
       DLVK_POST_LAUNCH();
     }
   }
-  join_d_kernel<<<(unsigned)(((int64_t)a.D * (a.N + 2) + 255) / 256), 256, 0, s>>>(part_d, a.B, a.D, a.N, g);
+  join_d_kernel<<<(unsigned)(((int64_t)a.D * (a.N + 2) + 255) / 256), 256, 0, s>>>(part_d, a.B * p.count, a.D, a.N, g);
   DLVK_POST_LAUNCH();
 }
 

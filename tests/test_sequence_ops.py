@@ -373,6 +373,17 @@ def test_scan(device, dtype, B, T, D, N, G):
 
 @pytest.mark.parametrize("device", DEVICES)
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("B,T,D,N", [(1, 257, 8, 16), (2, 300, 12, 3), (1, 530, 7, 20)])
+def test_scan_of_many_tokens(device, dtype, B, T, D, N):
+    """Long enough to be cut into pieces; states that last across them."""
+    p, dy, state, n = scan_inputs(B, T, D, N, 1, dtype, device, T, lengths=B > 1)
+    p["dt_bias"] -= 3.0
+    p["a_log"] -= 2.0
+    scan_check(p, dy, state, n)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("T,N", [(1, 16), (5, 4), (16, 16), (41, 16), (37, 64)])
 def test_scan_lengths_and_what_lies_behind_them(device, dtype, T, N):
     p, dy, state, n = scan_inputs(5, T, 24, N, 1, dtype, device, T, lengths=True)
