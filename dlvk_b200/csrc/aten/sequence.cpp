@@ -15,21 +15,34 @@ namespace {
 
 using OptTensor = c10::optional<at::Tensor>;
 
-// What the tensors of one call have in common.
+// What the tensors of one call have in common.  `one`: a token of each sequence,
+// whose tensors have no dimension of tokens.
 struct Call {
   const char* what;
   at::Device device;
   at::ScalarType type;
   int64_t B, T, D;
+  bool one = false;
 };
 
-Call call_of(const at::Tensor& x, const char* what, const char* name) {
+Call call_of(const at::Tensor& x, const char* what, const char* name, bool one) {
   TORCH_CHECK(x.is_cuda(), "dlvk.", what, ": ", name, " must be a CUDA tensor");
-  TORCH_CHECK(x.dim() == 3, "dlvk.", what, ": ", name, " is [sequences, tokens, channels], got ", x.sizes());
+  TORCH_CHECK(x.dim() == (one ? 2 : 3), "dlvk.", what, ": ", name, one ? " is [sequences, channels], got " :
+              " is [sequences, tokens, channels], got ", x.sizes());
   TORCH_CHECK(x.scalar_type() == at::kFloat || x.scalar_type() == at::kBFloat16, "dlvk.", what, ": ", name,
               " is fp32 or bf16, got ", x.scalar_type());
-  TORCH_CHECK(x.size(2) < (1LL << 31) - 4096, "dlvk.", what, ": ", x.size(2), " channels");
-  return {what, x.device(), x.scalar_type(), x.size(0), x.size(1), x.size(2)};
+  const int64_t D = x.size(one ? 1 : 2);
+  TORCH_CHECK(D < (1LL << 31) - 4096, "dlvk.", what, ": ", D, " channels");
+  return {what, x.device(), x.scalar_type(), x.size(0), one ? 1 : x.size(1), D, one};
+}
+
+// Sizes [B, T, rest...], without T for one token.
+using Sizes = c10::SmallVector<int64_t, 4>;
+Sizes sizes_of(const Call& c, std::initializer_list<int64_t> rest) {
+  Sizes s{c.B};
+  if (!c.one) s.push_back(c.T);
+  s.append(rest.begin(), rest.end());
+  return s;
 }
 
 void check(const Call& c, const at::Tensor& t, const char* name, at::ScalarType type, at::IntArrayRef sizes) {
@@ -39,16 +52,19 @@ void check(const Call& c, const at::Tensor& t, const char* name, at::ScalarType 
   TORCH_CHECK(t.sizes() == sizes, "dlvk.", c.what, ": ", name, " is ", t.sizes(), ", expected ", sizes);
 }
 
-// A tensor that is read, its last dimension contiguous (and the one before it
-// behind it, where there are four); a copy where it is not.  `keep` holds it.
-SeqRef read(const Call& c, const at::Tensor& t, const char* name, at::ScalarType type, at::IntArrayRef sizes,
-            at::Tensor& keep) {
-  check(c, t, name, type, sizes);
-  const int64_t d = t.dim();
-  const bool rows = t.size(d - 1) <= 1 || t.stride(d - 1) == 1;
-  const bool groups = d < 4 || t.size(2) <= 1 || t.stride(2) == t.size(3);
-  keep = rows && groups ? t : t.contiguous();
-  return {keep.data_ptr(), keep.stride(0), keep.stride(1)};
+// Whether what follows the tokens (channels, or groups of states) is one run.
+bool runs(const Call& c, const at::Tensor& t) {
+  const int64_t d = t.dim(), groups = c.one ? 1 : 2;
+  return t.numel() == 0 || ((t.size(d - 1) <= 1 || t.stride(d - 1) == 1) &&
+                            (d <= groups + 1 || t.size(groups) <= 1 || t.stride(groups) == t.size(groups + 1)));
+}
+SeqRef ref(const Call& c, const at::Tensor& t) { return {t.data_ptr(), t.stride(0), c.one ? 0 : t.stride(1)}; }
+
+// A tensor that is read; a copy where its rows are no runs.  `keep` holds it.
+SeqRef read(const Call& c, const at::Tensor& t, const char* name, std::initializer_list<int64_t> rest, at::Tensor& keep) {
+  check(c, t, name, c.type, sizes_of(c, rest));
+  keep = runs(c, t) ? t : t.contiguous();
+  return ref(c, keep);
 }
 
 const float* read_param(const Call& c, const OptTensor& t, const char* name, at::IntArrayRef sizes, at::Tensor& keep) {
@@ -73,11 +89,17 @@ at::Tensor written(const Call& c, const OptTensor& out, const char* name, at::Sc
   return *out;
 }
 SeqRef written_rows(const Call& c, const at::Tensor& t, const char* name) {
-  const int64_t d = t.dim();
-  TORCH_CHECK(t.numel() == 0 || ((t.size(d - 1) <= 1 || t.stride(d - 1) == 1) &&
-                                 (d < 4 || t.size(2) <= 1 || t.stride(2) == t.size(3))),
-              "dlvk.", c.what, ": ", name, " needs a contiguous last dimension");
-  return {t.data_ptr(), t.stride(0), t.stride(1)};
+  TORCH_CHECK(runs(c, t), "dlvk.", c.what, ": ", name, " needs a contiguous last dimension");
+  return ref(c, t);
+}
+// The convolution's state [B, taps - 1, D], whatever the call's tensors have.
+SeqRef conv_state(const Call& c, const at::Tensor& t, int64_t taps, const char* name, bool write, at::Tensor& keep) {
+  check(c, t, name, c.type, {c.B, taps - 1, c.D});
+  const bool rows = t.numel() == 0 || c.D <= 1 || t.stride(2) == 1;
+  TORCH_CHECK(rows || !write, "dlvk.", c.what, ": ", name, " needs a contiguous last dimension");
+  TORCH_CHECK(!write || !may_repeat(t), "dlvk.", c.what, ": ", name, " repeats its elements (an expanded tensor)");
+  keep = rows ? t : t.contiguous();
+  return {keep.data_ptr(), keep.stride(0), keep.stride(1)};
 }
 float* written_param(const Call& c, const OptTensor& t, const char* name, at::IntArrayRef sizes) {
   if (!t.has_value()) return nullptr;
@@ -109,8 +131,8 @@ struct Conv {
   at::Tensor x, weight, bias, state, lengths;
 };
 Conv conv_of(const char* what, const at::Tensor& x, const at::Tensor& weight, const OptTensor& bias,
-             const OptTensor& state, const OptTensor& lengths, bool silu) {
-  Conv v{call_of(x, what, "x"), {}, {}, {}, {}, {}, {}};
+             const OptTensor& state, const OptTensor& lengths, bool silu, bool one = false) {
+  Conv v{call_of(x, what, "x", one), {}, {}, {}, {}, {}, {}};
   const Call& c = v.call;
   TORCH_CHECK(weight.dim() == 2 && weight.size(1) >= 2 && weight.size(1) <= 4, "dlvk.", what,
               ": weight is [channels, 2 to 4 taps], got ", weight.sizes());
@@ -121,10 +143,10 @@ Conv conv_of(const char* what, const at::Tensor& x, const at::Tensor& weight, co
   v.a.D = (int)c.D;
   v.a.taps = (int)taps;
   v.a.silu = silu;
-  v.a.x = read(c, x, "x", c.type, {c.B, c.T, c.D}, v.x);
+  v.a.x = read(c, x, "x", {c.D}, v.x);
   v.a.weight = read_param(c, weight, "weight", {c.D, taps}, v.weight);
   v.a.bias = read_param(c, bias, "bias", {c.D}, v.bias);
-  if (state.has_value()) v.a.state = read(c, *state, "state", c.type, {c.B, taps - 1, c.D}, v.state);
+  if (state.has_value()) v.a.state = conv_state(c, *state, taps, "state", false, v.state);
   v.a.lengths = read_lengths(c, lengths, v.lengths);
   return v;
 }
@@ -133,35 +155,40 @@ struct Scan {
   Call call;
   StateScan a;
   at::Tensor u, dt, b, c, z, a_log, skip, dt_bias, state, lengths;
-  std::vector<int64_t> bc;  // sizes of b and c as given
+  Sizes bc;  // sizes of b and c as given
   std::vector<at::Tensor> inputs() const { return {u, dt, b, c, z, a_log, skip, dt_bias, lengths}; }
 };
 Scan scan_of(const char* what, const at::Tensor& u, const at::Tensor& dt, const at::Tensor& a_log, const at::Tensor& b,
              const at::Tensor& c, const OptTensor& skip, const OptTensor& z, const OptTensor& dt_bias,
-             const OptTensor& state, const OptTensor& lengths) {
-  Scan v{call_of(u, what, "u")};
+             const OptTensor& state, const OptTensor& lengths, bool one = false) {
+  Scan v{call_of(u, what, "u", one)};
   const Call& k = v.call;
   TORCH_CHECK(a_log.dim() == 2 && a_log.size(1) >= 1 && a_log.size(1) <= STATE_SCAN_STATES, "dlvk.", what,
               ": a_log is [channels, 1 to ", STATE_SCAN_STATES, " states], got ", a_log.sizes());
-  const int64_t N = a_log.size(1);
-  TORCH_CHECK(b.dim() == 3 || b.dim() == 4, "dlvk.", what,
-              ": b is [sequences, tokens, states] or [sequences, tokens, groups, states], got ", b.sizes());
-  v.bc = b.sizes().vec();
-  const int64_t G = b.dim() == 4 ? b.size(2) : 1;
+  const int64_t N = a_log.size(1), flat = one ? 2 : 3;  // dimensions of b without groups
+  TORCH_CHECK(b.dim() == flat || b.dim() == flat + 1, "dlvk.", what, ": b is [sequences, ", one ? "" : "tokens, ",
+              "states] or the same with groups before the states, got ", b.sizes());
+  const bool grouped = b.dim() > flat;
+  const int64_t G = grouped ? b.size(flat - 1) : 1;
   TORCH_CHECK(G >= 1 && k.D % G == 0, "dlvk.", what, ": ", k.D, " channels in ", G, " groups");
-  std::vector<int64_t> bc{k.B, k.T, N};
-  if (b.dim() == 4) bc.insert(bc.begin() + 2, G);
   v.a.type = to_dtype(u);
   v.a.B = k.B;
   v.a.T = k.T;
   v.a.D = (int)k.D;
   v.a.N = (int)N;
   v.a.G = (int)G;
-  v.a.u = read(k, u, "u", k.type, {k.B, k.T, k.D}, v.u);
-  v.a.dt = read(k, dt, "dt", k.type, {k.B, k.T, k.D}, v.dt);
-  v.a.b = read(k, b, "b", k.type, bc, v.b);
-  v.a.c = read(k, c, "c", k.type, bc, v.c);
-  if (z.has_value()) v.a.z = read(k, *z, "z", k.type, {k.B, k.T, k.D}, v.z);
+  v.a.u = read(k, u, "u", {k.D}, v.u);
+  v.a.dt = read(k, dt, "dt", {k.D}, v.dt);
+  if (grouped) {
+    v.bc = sizes_of(k, {G, N});
+    v.a.b = read(k, b, "b", {G, N}, v.b);
+    v.a.c = read(k, c, "c", {G, N}, v.c);
+  } else {
+    v.bc = sizes_of(k, {N});
+    v.a.b = read(k, b, "b", {N}, v.b);
+    v.a.c = read(k, c, "c", {N}, v.c);
+  }
+  if (z.has_value()) v.a.z = read(k, *z, "z", {k.D}, v.z);
   v.a.a_log = read_param(k, a_log, "a_log", {k.D, N}, v.a_log);
   v.a.skip = read_param(k, skip, "skip", {k.D}, v.skip);
   v.a.dt_bias = read_param(k, dt_bias, "dt_bias", {k.D}, v.dt_bias);
@@ -181,13 +208,29 @@ std::vector<OptTensor> short_conv_fwd_op(const at::Tensor& x, const at::Tensor& 
   at::Tensor y = at::empty({c.B, c.T, c.D}, x.options()), last;
   SeqRef to;
   if (want_state || out_state.has_value()) {
-    last = written(c, out_state, "out_state", c.type, {c.B, v.a.taps - 1, c.D});
-    to = written_rows(c, last, "out_state");
+    at::Tensor keep;
+    last = out_state.has_value() ? *out_state : at::empty({c.B, v.a.taps - 1, c.D}, x.options());
+    to = conv_state(c, last, v.a.taps, "out_state", true, keep);
     apart(c, {last}, {v.x, v.weight, v.bias, v.lengths});
     in_place_or_apart(c, last, v.state);
   }
   short_conv_fwd(v.a, {y.data_ptr(), y.stride(0), y.stride(1)}, to, stream());
   return {y, last.defined() ? OptTensor(last) : c10::nullopt};
+}
+
+at::Tensor short_conv_step_op(const at::Tensor& x, const at::Tensor& weight, OptTensor bias, const at::Tensor& state,
+                              bool silu, OptTensor out_state) {
+  Conv v = conv_of("short_conv_step", x, weight, bias, state, c10::nullopt, silu, true);
+  const Call& c = v.call;
+  c10::cuda::CUDAGuard g(c.device);
+  at::AutoDispatchBelowADInplaceOrView below;
+  at::Tensor y = at::empty({c.B, c.D}, x.options()), keep;
+  const at::Tensor& last = out_state.has_value() ? *out_state : state;
+  const SeqRef to = conv_state(c, last, v.a.taps, "out_state", true, keep);
+  apart(c, {last}, {v.x, v.weight, v.bias});
+  if (out_state.has_value()) in_place_or_apart(c, last, v.state);
+  short_conv_fwd(v.a, ref(c, y), to, stream());
+  return y;
 }
 
 std::vector<OptTensor> short_conv_bwd_op(const at::Tensor& x, const at::Tensor& weight, OptTensor bias,
@@ -201,7 +244,7 @@ std::vector<OptTensor> short_conv_bwd_op(const at::Tensor& x, const at::Tensor& 
   c10::cuda::CUDAGuard g(c.device);
   at::AutoDispatchBelowADInplaceOrView below;
   at::Tensor dyk;
-  const SeqRef go = read(c, dy, "dy", c.type, {c.B, c.T, c.D}, dyk);
+  const SeqRef go = read(c, dy, "dy", {c.D}, dyk);
   at::Tensor gx = written(c, dx, "dx", c.type, {c.B, c.T, c.D});
   const auto f32 = at::TensorOptions().dtype(at::kFloat).device(c.device);
   if (!dweight.has_value()) dweight = at::empty({c.D, v.a.taps}, f32);
@@ -238,6 +281,25 @@ std::vector<OptTensor> state_scan_fwd_op(const at::Tensor& u, const at::Tensor& 
   return {y, last.defined() ? OptTensor(last) : c10::nullopt, save ? OptTensor(saved) : c10::nullopt};
 }
 
+at::Tensor state_scan_step_op(const at::Tensor& u, const at::Tensor& dt, const at::Tensor& a_log, const at::Tensor& b,
+                              const at::Tensor& c, const at::Tensor& state, OptTensor skip, OptTensor z,
+                              OptTensor dt_bias, OptTensor out_state) {
+  Scan v = scan_of("state_scan_step", u, dt, a_log, b, c, skip, z, dt_bias, state, c10::nullopt, true);
+  const Call& k = v.call;
+  c10::cuda::CUDAGuard g(k.device);
+  at::AutoDispatchBelowADInplaceOrView below;
+  const at::Tensor& last = out_state.has_value() ? *out_state : state;
+  check(k, last, "out_state", at::kFloat, {k.B, k.D, v.a.N});
+  TORCH_CHECK(last.is_contiguous(), "dlvk.state_scan_step: ", out_state.has_value() ? "out_state" : "state",
+              " must be contiguous");
+  for (const at::Tensor& t : {v.u, v.dt, v.b, v.c, v.z, v.a_log, v.skip, v.dt_bias})
+    TORCH_CHECK(!share(last, t), "dlvk.state_scan_step: the state shares memory with an operand");
+  if (out_state.has_value()) in_place_or_apart(k, last, v.state);
+  at::Tensor y = at::empty({k.B, k.D}, u.options());
+  state_scan_fwd(v.a, ref(k, y), last.data_ptr<float>(), nullptr, nullptr, stream());
+  return y;
+}
+
 std::vector<OptTensor> state_scan_bwd_op(const at::Tensor& u, const at::Tensor& dt, const at::Tensor& a_log,
                                          const at::Tensor& b, const at::Tensor& c, OptTensor skip, OptTensor z,
                                          OptTensor dt_bias, const at::Tensor& dy, const at::Tensor& saved,
@@ -257,7 +319,7 @@ std::vector<OptTensor> state_scan_bwd_op(const at::Tensor& u, const at::Tensor& 
   c10::cuda::CUDAGuard g(k.device);
   at::AutoDispatchBelowADInplaceOrView below;
   at::Tensor dyk;
-  const SeqRef go = read(k, dy, "dy", k.type, {k.B, k.T, k.D}, dyk);
+  const SeqRef go = read(k, dy, "dy", {k.D}, dyk);
   const std::vector<int64_t> rows{k.B, k.T, k.D};
   at::Tensor gu = written(k, du, "du", k.type, rows), gdt = written(k, ddt, "ddt", k.type, rows);
   at::Tensor gb = written(k, db, "db", k.type, v.bc), gc = written(k, dc, "dc", k.type, v.bc), gz;

@@ -11,6 +11,11 @@ void register_sequence(py::module& m) {
   m.def("short_conv_fwd", &short_conv_fwd_op, py::arg("x"), py::arg("weight"), py::arg("bias") = py::none(),
         py::arg("state") = py::none(), py::arg("lengths") = py::none(), py::arg("silu") = true,
         py::arg("want_state") = false, py::arg("out_state") = py::none());
+  m.def("short_conv_step", &short_conv_step_op, py::arg("x"), py::arg("weight"), py::arg("bias"), py::arg("state"),
+        py::arg("silu") = true, py::arg("out_state") = py::none());
+  m.def("state_scan_step", &state_scan_step_op, py::arg("u"), py::arg("dt"), py::arg("a_log"), py::arg("b"),
+        py::arg("c"), py::arg("state"), py::arg("skip") = py::none(), py::arg("z") = py::none(),
+        py::arg("dt_bias") = py::none(), py::arg("out_state") = py::none());
   m.def("short_conv_bwd", &short_conv_bwd_op, py::arg("x"), py::arg("weight"), py::arg("bias"), py::arg("dy"),
         py::arg("state") = py::none(), py::arg("lengths") = py::none(), py::arg("silu") = true,
         py::arg("dx") = py::none(), py::arg("dweight") = py::none(), py::arg("dbias") = py::none(),

@@ -78,6 +78,8 @@ at::Tensor embedding_lookup_op(const at::Tensor& ids, const at::Tensor& table, d
 at::Tensor embedding_grad_op(const at::Tensor& ids, const at::Tensor& dy, int64_t num_embeddings, double scale, int64_t padding_idx, c10::optional<at::Tensor> out, bool accumulate);
 void embedding_bwd_op(const at::Tensor& ids, const at::Tensor& dy, const at::Tensor& dtable);
 std::vector<c10::optional<at::Tensor>> short_conv_fwd_op(const at::Tensor& x, const at::Tensor& weight, c10::optional<at::Tensor> bias, c10::optional<at::Tensor> state, c10::optional<at::Tensor> lengths, bool silu, bool want_state, c10::optional<at::Tensor> out_state);
+at::Tensor short_conv_step_op(const at::Tensor& x, const at::Tensor& weight, c10::optional<at::Tensor> bias, const at::Tensor& state, bool silu, c10::optional<at::Tensor> out_state);
+at::Tensor state_scan_step_op(const at::Tensor& u, const at::Tensor& dt, const at::Tensor& a_log, const at::Tensor& b, const at::Tensor& c, const at::Tensor& state, c10::optional<at::Tensor> skip, c10::optional<at::Tensor> z, c10::optional<at::Tensor> dt_bias, c10::optional<at::Tensor> out_state);
 std::vector<c10::optional<at::Tensor>> short_conv_bwd_op(const at::Tensor& x, const at::Tensor& weight, c10::optional<at::Tensor> bias, const at::Tensor& dy, c10::optional<at::Tensor> state, c10::optional<at::Tensor> lengths, bool silu, c10::optional<at::Tensor> dx, c10::optional<at::Tensor> dweight, c10::optional<at::Tensor> dbias, bool accumulate);
 std::vector<c10::optional<at::Tensor>> state_scan_fwd_op(const at::Tensor& u, const at::Tensor& dt, const at::Tensor& a_log, const at::Tensor& b, const at::Tensor& c, c10::optional<at::Tensor> skip, c10::optional<at::Tensor> z, c10::optional<at::Tensor> dt_bias, c10::optional<at::Tensor> state, c10::optional<at::Tensor> lengths, bool want_state, bool save, c10::optional<at::Tensor> out_state);
 std::vector<c10::optional<at::Tensor>> state_scan_bwd_op(const at::Tensor& u, const at::Tensor& dt, const at::Tensor& a_log, const at::Tensor& b, const at::Tensor& c, c10::optional<at::Tensor> skip, c10::optional<at::Tensor> z, c10::optional<at::Tensor> dt_bias, const at::Tensor& dy, const at::Tensor& saved, c10::optional<at::Tensor> lengths, c10::optional<at::Tensor> du, c10::optional<at::Tensor> ddt, c10::optional<at::Tensor> db, c10::optional<at::Tensor> dc, c10::optional<at::Tensor> dz, c10::optional<at::Tensor> da_log, c10::optional<at::Tensor> dskip, c10::optional<at::Tensor> ddt_bias, bool accumulate);

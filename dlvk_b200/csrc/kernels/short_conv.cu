@@ -22,14 +22,13 @@
 namespace dlvk {
 namespace {
 
-constexpr int RUN = 16;    // tokens of a thread: 3 of 19 reads come twice (K = 4)
 constexpr int RUNS = 8;    // runs of a block, a warp each
-constexpr int AHEAD = 8;   // tokens whose loads are in flight
 
 template <typename T, int V> struct Pack;  // V elements as loaded
 template <> struct Pack<float, 4> { using type = float4; };
 template <> struct Pack<float, 1> { using type = float; };
 template <> struct Pack<__nv_bfloat16, 8> { using type = uint4; };
+template <> struct Pack<__nv_bfloat16, 4> { using type = uint2; };
 template <> struct Pack<__nv_bfloat16, 1> { using type = __nv_bfloat16; };
 
 template <typename T, int V>
@@ -37,11 +36,6 @@ struct Vec {
   typename Pack<T, V>::type raw;
   __device__ __forceinline__ void load(const T* p) { raw = *reinterpret_cast<const typename Pack<T, V>::type*>(p); }
   __device__ __forceinline__ void store(T* p) const { *reinterpret_cast<typename Pack<T, V>::type*>(p) = raw; }
-  __device__ __forceinline__ void zero() {
-    T* e = reinterpret_cast<T*>(&raw);
-#pragma unroll
-    for (int i = 0; i < V; ++i) e[i] = from_f32<T>(0.f);
-  }
   __device__ __forceinline__ float get(int i) const { return to_f32(reinterpret_cast<const T*>(&raw)[i]); }
   __device__ __forceinline__ void set(int i, float v) { reinterpret_cast<T*>(&raw)[i] = from_f32<T>(v); }
 };
@@ -55,28 +49,41 @@ __device__ __forceinline__ T* at(const SeqRef& r, int64_t b, int64_t t, int c) {
 
 template <int V, int K>
 __device__ __forceinline__ void load_taps(const ShortConv& a, int c, float (&w)[V][K], float (&bias)[V]) {
+  float flat[V * K];
+  if constexpr (V > 1) {  // whole aligned fours
+#pragma unroll
+    for (int i = 0; i < V * K; i += 4)
+      *reinterpret_cast<float4*>(&flat[i]) = *reinterpret_cast<const float4*>(a.weight + (int64_t)c * K + i);
+  } else {
+#pragma unroll
+    for (int i = 0; i < K; ++i) flat[i] = a.weight[(int64_t)c * K + i];
+  }
 #pragma unroll
   for (int i = 0; i < V; ++i) {
 #pragma unroll
-    for (int j = 0; j < K; ++j) w[i][j] = a.weight[(int64_t)(c + i) * K + j];
+    for (int j = 0; j < K; ++j) w[i][j] = flat[i * K + j];
     bias[i] = a.bias ? a.bias[c + i] : 0.f;
   }
 }
 
-// The place of a thread: sequence, first token and first channel of its run.
-struct Place {
-  int64_t b, t;
+// The work's division: `run` tokens of a sequence and 32 V channels a warp.
+struct Grid {
+  int64_t runs, run, rows;  // runs of a sequence; rows of blocks
+  int blocks;               // blocks of a row
+};
+struct Place {  // of a thread: sequence, tokens [t, end), first channel
+  int64_t b, t, end;
   int c;
   bool ok;
 };
 template <int V>
-__device__ __forceinline__ Place place(const ShortConv& a, int64_t runs, int64_t row) {
-  const int blocks = (a.D + 32 * V - 1) / (32 * V);
-  const int64_t q = row * RUNS + threadIdx.y;
+__device__ __forceinline__ Place place(const ShortConv& a, const Grid& g) {
+  const int64_t q = (int64_t)(blockIdx.x / g.blocks) * RUNS + threadIdx.y;
   Place p;
-  p.b = q / runs;
-  p.t = (q % runs) * RUN;
-  p.c = ((int)(blockIdx.x % blocks) * 32 + threadIdx.x) * V;
+  p.b = q / g.runs;
+  p.t = q % g.runs * g.run;
+  p.end = min(p.t + g.run, a.T);
+  p.c = ((int)(blockIdx.x % g.blocks) * 32 + threadIdx.x) * V;
   p.ok = p.b < a.B && p.c < a.D;
   return p;
 }
@@ -87,46 +94,59 @@ __device__ __forceinline__ int64_t length_of(const ShortConv& a, int64_t b) {
 
 // Token t of a sequence of n that counts, or of the tokens before it, or zeros.
 template <typename T, int V, int K>
-__device__ __forceinline__ Vec<T, V> token(const ShortConv& a, const Place& p, int64_t t, int64_t n) {
-  Vec<T, V> v;
-  if (t >= 0 && t < n) v.load(at<T>(a.x, p.b, t, p.c));
-  else if (t < 0 && a.state.p) v.load(at<T>(a.state, p.b, t + K - 1, p.c));
-  else v.zero();
-  return v;
+__device__ __forceinline__ void token(const ShortConv& a, const Place& p, int64_t t, int64_t n, float (&x)[V]) {
+  const T* from = t >= 0 ? (t < n ? at<T>(a.x, p.b, t, p.c) : nullptr)
+                         : (a.state.p ? at<T>(a.state, p.b, t + K - 1, p.c) : nullptr);
+#pragma unroll
+  for (int i = 0; i < V; ++i) x[i] = 0.f;
+  if (from) {
+    Vec<T, V> v;
+    v.load(from);
+#pragma unroll
+    for (int i = 0; i < V; ++i) x[i] = v.get(i);
+  }
+}
+
+// COUNT tokens of r from t on, all asked for before any is used.  Past the
+// sequence's last one that is read again: a branch around a load would make the
+// next one wait for it.
+template <typename T, int V, int COUNT>
+__device__ __forceinline__ void load_tokens(const SeqRef& r, const Place& p, int64_t t, int64_t n, Vec<T, V> (&v)[COUNT]) {
+#pragma unroll
+  for (int k = 0; k < COUNT; ++k) v[k].load(at<T>(r, p.b, max(min(t + k, n - 1), (int64_t)0), p.c));
 }
 
 template <typename T, int V, int K>
-__global__ void __launch_bounds__(32 * RUNS) conv_fwd_kernel(ShortConv a, SeqRef y, SeqRef out_state, int64_t runs) {
-  const int blocks = (a.D + 32 * V - 1) / (32 * V);
-  const Place p = place<V>(a, runs, blockIdx.x / blocks);
+__global__ void __launch_bounds__(32 * RUNS) conv_fwd_kernel(ShortConv a, SeqRef y, SeqRef out_state, Grid grid) {
+  constexpr int AHEAD = 8;
+  const Place p = place<V>(a, grid);
   if (!p.ok) return;
   const int64_t n = length_of(a, p.b);
+  Vec<T, V> v[AHEAD];
+  if (p.t < p.end) load_tokens<T, V, AHEAD>(a.x, p, p.t, n, v);
   float w[V][K], bias[V], last[K - 1][V];
   load_taps<V, K>(a, p.c, w, bias);
 #pragma unroll
-  for (int j = 0; j < K - 1; ++j) {
-    const Vec<T, V> v = token<T, V, K>(a, p, p.t - (K - 1) + j, n);
-#pragma unroll
-    for (int i = 0; i < V; ++i) last[j][i] = v.get(i);
-  }
+  for (int j = 0; j < K - 1; ++j) token<T, V, K>(a, p, p.t - (K - 1) + j, n, last[j]);
   if (out_state.p && p.t == 0) {
     // read before any of it is written: out_state may be the state
-    Vec<T, V> keep[K - 1];
+    float keep[K - 1][V];
 #pragma unroll
-    for (int j = 0; j < K - 1; ++j) keep[j] = token<T, V, K>(a, p, n - (K - 1) + j, n);
+    for (int j = 0; j < K - 1; ++j) token<T, V, K>(a, p, n - (K - 1) + j, n, keep[j]);
 #pragma unroll
-    for (int j = 0; j < K - 1; ++j) keep[j].store(at<T>(out_state, p.b, j, p.c));
-  }
-  for (int64_t t0 = p.t; t0 < min(p.t + RUN, a.T); t0 += AHEAD) {
-    Vec<T, V> v[AHEAD];
+    for (int j = 0; j < K - 1; ++j) {
+      Vec<T, V> o;
 #pragma unroll
-    for (int k = 0; k < AHEAD; ++k) {
-      v[k].zero();
-      if (t0 + k < n) v[k].load(at<T>(a.x, p.b, t0 + k, p.c));
+      for (int i = 0; i < V; ++i) o.set(i, keep[j][i]);
+      o.store(at<T>(out_state, p.b, j, p.c));
     }
+  }
+  for (int64_t t0 = p.t; t0 < p.end; t0 += AHEAD) {
+    if (t0 > p.t) load_tokens<T, V, AHEAD>(a.x, p, t0, n, v);
 #pragma unroll
     for (int k = 0; k < AHEAD; ++k) {
-      if (t0 + k >= a.T) break;
+      if (t0 + k >= p.end) break;
+      const bool here = t0 + k < n;
       Vec<T, V> out;
 #pragma unroll
       for (int i = 0; i < V; ++i) {
@@ -138,7 +158,7 @@ __global__ void __launch_bounds__(32 * RUNS) conv_fwd_kernel(ShortConv a, SeqRef
         for (int j = 0; j < K - 2; ++j) last[j][i] = last[j + 1][i];
         last[K - 2][i] = x;
         if (a.silu) s *= sigmoid(s);
-        out.set(i, t0 + k < n ? s : 0.f);
+        out.set(i, here ? s : 0.f);
       }
       out.store(at<T>(y, p.b, t0 + k, p.c));
     }
@@ -148,10 +168,9 @@ __global__ void __launch_bounds__(32 * RUNS) conv_fwd_kernel(ShortConv a, SeqRef
 // part [block rows][K + 1][D]: the sums of a block's runs, bias last.
 template <typename T, int V, int K>
 __global__ void __launch_bounds__(32 * RUNS) conv_bwd_kernel(ShortConv a, SeqRef dy, SeqRef dx, float* __restrict__ part,
-                                                             int64_t runs) {
-  const int blocks = (a.D + 32 * V - 1) / (32 * V);
-  const int64_t row = blockIdx.x / blocks;
-  const Place p = place<V>(a, runs, row);
+                                                             Grid grid) {
+  constexpr int AHEAD = 4;
+  const Place p = place<V>(a, grid);
   float dw[V][K + 1];
 #pragma unroll
   for (int i = 0; i < V; ++i)
@@ -159,52 +178,55 @@ __global__ void __launch_bounds__(32 * RUNS) conv_bwd_kernel(ShortConv a, SeqRef
     for (int j = 0; j <= K; ++j) dw[i][j] = 0.f;
   if (p.ok) {
     const int64_t n = length_of(a, p.b);
-    float w[V][K], bias[V], x[K][V], g[K][V];  // the last K tokens of each, the current one at K - 1
+    float w[V][K], bias[V], x[K - 1 + AHEAD][V], g[K - 1 + AHEAD][V];  // the last K - 1 tokens first
     load_taps<V, K>(a, p.c, w, bias);
 #pragma unroll
     for (int j = 0; j < K - 1; ++j) {
-      const Vec<T, V> v = token<T, V, K>(a, p, p.t - (K - 1) + j, n);
+      token<T, V, K>(a, p, p.t - (K - 1) + j, n, x[j]);
 #pragma unroll
-      for (int i = 0; i < V; ++i) x[j + 1][i] = v.get(i), g[j + 1][i] = 0.f;
+      for (int i = 0; i < V; ++i) g[j][i] = 0.f;
     }
-    const int64_t end = min(p.t + RUN, a.T);
-    for (int64_t t = p.t; t < end + K - 1; ++t) {
-      Vec<T, V> vx, vg;
-      vx.zero();
-      vg.zero();
-      if (t < n) {
-        vx.load(at<T>(a.x, p.b, t, p.c));
-        vg.load(at<T>(dy, p.b, t, p.c));
-      }
-      Vec<T, V> out;
+    // the K - 1 tokens behind the run for their g alone
+    for (int64_t t0 = p.t; t0 < p.end + K - 1; t0 += AHEAD) {
+      Vec<T, V> vx[AHEAD], vg[AHEAD];
+      load_tokens<T, V, AHEAD>(a.x, p, t0, n, vx);
+      load_tokens<T, V, AHEAD>(dy, p, t0, n, vg);
 #pragma unroll
-      for (int i = 0; i < V; ++i) {
+      for (int k = 0; k < AHEAD; ++k) {
+        const int64_t t = t0 + k;
+        Vec<T, V> out;
 #pragma unroll
-        for (int j = 0; j < K - 1; ++j) x[j][i] = x[j + 1][i], g[j][i] = g[j + 1][i];
-        x[K - 1][i] = vx.get(i);
-        float gi = vg.get(i);
-        if (a.silu) {
-          float s = bias[i];
+        for (int i = 0; i < V; ++i) {
+          x[K - 1 + k][i] = t < n ? vx[k].get(i) : 0.f;
+          float gi = vg[k].get(i);
+          if (a.silu) {
+            float s = bias[i];
 #pragma unroll
-          for (int j = 0; j < K; ++j) s = fmaf(w[i][j], x[j][i], s);
-          const float q = sigmoid(s);
-          gi *= t < n ? q * fmaf(s, 1.f - q, 1.f) : 0.f;
+            for (int j = 0; j < K; ++j) s = fmaf(w[i][j], x[k + j][i], s);
+            const float q = sigmoid(s);
+            gi *= q * fmaf(s, 1.f - q, 1.f);
+          }
+          gi = t < n ? gi : 0.f;
+          g[K - 1 + k][i] = gi;
+          const float own = t < p.end ? gi : 0.f;
+#pragma unroll
+          for (int j = 0; j < K; ++j) dw[i][j] = fmaf(own, x[k + j][i], dw[i][j]);
+          dw[i][K] += own;
+          float d = 0.f;  // dx[t - K + 1] = sum_j w[j] g[t - j]
+#pragma unroll
+          for (int j = 0; j < K; ++j) d = fmaf(w[i][j], g[K - 1 + k - j][i], d);
+          out.set(i, d);
         }
-        g[K - 1][i] = gi;
-        if (t < end) {
-#pragma unroll
-          for (int j = 0; j < K; ++j) dw[i][j] = fmaf(gi, x[j][i], dw[i][j]);
-          dw[i][K] += gi;
-        }
-        float d = 0.f;  // dx[t - K + 1] = sum_j w[j] g[t - j]
-#pragma unroll
-        for (int j = 0; j < K; ++j) d = fmaf(w[i][j], g[K - 1 - j][i], d);
-        out.set(i, d);
+        if (t - (K - 1) >= p.t && t - (K - 1) < p.end) out.store(at<T>(dx, p.b, t - (K - 1), p.c));
       }
-      if (t - (K - 1) >= p.t) out.store(at<T>(dx, p.b, t - (K - 1), p.c));
+#pragma unroll
+      for (int j = 0; j < K - 1; ++j)
+#pragma unroll
+        for (int i = 0; i < V; ++i) x[j][i] = x[AHEAD + j][i], g[j][i] = g[AHEAD + j][i];
     }
   }
   __shared__ float sums[RUNS][32 * V + 1];
+  const int64_t row = blockIdx.x / grid.blocks;
 #pragma unroll
   for (int j = 0; j <= K; ++j) {
     __syncthreads();
@@ -215,7 +237,7 @@ __global__ void __launch_bounds__(32 * RUNS) conv_bwd_kernel(ShortConv a, SeqRef
       float s = 0.f;
 #pragma unroll
       for (int r = 0; r < RUNS; ++r) s += sums[r][c];
-      const int d = (int)(blockIdx.x % blocks) * 32 * V + c;
+      const int d = (int)(blockIdx.x % grid.blocks) * 32 * V + c;
       if (d < a.D) part[(row * (K + 1) + j) * a.D + d] = s;
     }
   }
@@ -241,13 +263,30 @@ __global__ void __launch_bounds__(256) conv_join_kernel(const float* __restrict_
   if (out) *out = accumulate ? *out + s : s;
 }
 
-bool aligned(const SeqRef& r, int64_t bytes) {
-  return !r.p || (reinterpret_cast<uintptr_t>(r.p) % 16 == 0 && r.batch * bytes % 16 == 0 && r.token * bytes % 16 == 0);
+// Whether `v` neighbouring elements are one load.
+bool aligned(const SeqRef& r, int v, int64_t bytes) {
+  return !r.p || (reinterpret_cast<uintptr_t>(r.p) % (v * bytes) == 0 && r.batch % v == 0 && r.token % v == 0);
+}
+bool aligned(const ShortConv& a, int v) {
+  const int64_t bytes = a.dt == DType::BF16 ? 2 : 4;
+  return a.D % v == 0 && reinterpret_cast<uintptr_t>(a.weight) % 16 == 0 && aligned(a.x, v, bytes) &&
+         aligned(a.state, v, bytes);
 }
 
-int64_t run_rows(const ShortConv& a) {  // rows of blocks
-  return (a.B * ((a.T + RUN - 1) / RUN) + RUNS - 1) / RUNS;
+// Runs as long as some ten warps are left for every SM (a run reads K - 1 tokens
+// again, and the taps), at most `most` tokens.
+Grid grid_of(const ShortConv& a, int v, int64_t most) {
+  Grid g;
+  g.blocks = (a.D + 32 * v - 1) / (32 * v);
+  g.run = most;
+  while (g.run > 8 && a.B * ((a.T + g.run - 1) / g.run) * g.blocks < 148 * 10) g.run /= 2;
+  g.runs = std::max<int64_t>(1, (a.T + g.run - 1) / g.run);
+  g.rows = (a.B * g.runs + RUNS - 1) / RUNS;
+  DLVK_CHECK(g.rows * g.blocks < (1LL << 31), "short_conv: too many elements for one launch");
+  return g;
 }
+constexpr int64_t FWD_RUN = 32, BWD_RUN = 64;
+constexpr int BWD_VEC = 4;  // the backward pass keeps K + 3 tokens of two tensors in registers
 
 template <typename F>
 void by_taps(int taps, F&& f) {
@@ -259,61 +298,63 @@ void by_taps(int taps, F&& f) {
   }
 }
 
-// f(element type, channels of a thread): 16 bytes, or one element where the rows do not allow it.
-template <typename F>
-void by_type(DType dt, bool wide, F&& f) {
-  if (dt == DType::BF16) {
-    if (wide) f(__nv_bfloat16(), std::integral_constant<int, 8>());
-    else f(__nv_bfloat16(), std::integral_constant<int, 1>());
-  } else {
-    DLVK_CHECK(dt == DType::F32, "short_conv: fp32 or bf16");
-    if (wide) f(float(), std::integral_constant<int, 4>());
-    else f(float(), std::integral_constant<int, 1>());
-  }
-}
-
-unsigned grid_of(const ShortConv& a, int v) {
-  const int64_t g = run_rows(a) * ((a.D + 32 * v - 1) / (32 * v));
-  DLVK_CHECK(g < (1LL << 31), "short_conv: too many elements for one launch");
-  return (unsigned)g;
-}
-
 }  // namespace
 
 void short_conv_fwd(const ShortConv& a, SeqRef y, SeqRef out_state, cudaStream_t s) {
-  if (a.B == 0 || a.D == 0) return;
-  // a state without tokens is copied by the same kernel: one run
-  const int64_t bytes = a.dt == DType::BF16 ? 2 : 4, runs = std::max<int64_t>(1, (a.T + RUN - 1) / RUN);
-  if (a.T == 0 && !out_state.p) return;
-  const bool wide = a.D % (16 / bytes) == 0 && aligned(a.x, bytes) && aligned(a.state, bytes) && aligned(y, bytes) &&
-                    aligned(out_state, bytes);
-  ShortConv k = a;
-  if (a.T == 0) k.x = a.state;  // never read
-  by_type(a.dt, wide, [&](auto type, auto vec) {
-    by_taps(a.taps, [&](auto taps) {
-      const int64_t rows = (a.B * runs + RUNS - 1) / RUNS, g = rows * ((a.D + 32 * vec - 1) / (32 * vec));
-      DLVK_CHECK(g < (1LL << 31), "short_conv: too many elements for one launch");
-      conv_fwd_kernel<decltype(type), decltype(vec)::value, decltype(taps)::value>
-          <<<(unsigned)g, dim3(32, RUNS), 0, s>>>(k, y, out_state, runs);
-    });
+  DLVK_CHECK(a.dt == DType::BF16 || a.dt == DType::F32, "short_conv: fp32 or bf16");
+  // without tokens there is a state to copy, or nothing to do
+  if (a.B == 0 || a.D == 0 || (a.T == 0 && !out_state.p)) return;
+  const int64_t bytes = a.dt == DType::BF16 ? 2 : 4;
+  const int v = 16 / (int)bytes;
+  const bool wide = aligned(a, v) && aligned(y, v, bytes) && aligned(out_state, v, bytes);
+  const Grid g = grid_of(a, wide ? v : 1, FWD_RUN);
+  const unsigned n = (unsigned)(g.rows * g.blocks);
+  const dim3 block(32, RUNS);
+  by_taps(a.taps, [&](auto taps) {
+    constexpr int K = decltype(taps)::value;
+    if (a.dt == DType::BF16) {
+      if (wide) conv_fwd_kernel<__nv_bfloat16, 8, K><<<n, block, 0, s>>>(a, y, out_state, g);
+      else conv_fwd_kernel<__nv_bfloat16, 1, K><<<n, block, 0, s>>>(a, y, out_state, g);
+    } else {
+      if (wide) conv_fwd_kernel<float, 4, K><<<n, block, 0, s>>>(a, y, out_state, g);
+      else conv_fwd_kernel<float, 1, K><<<n, block, 0, s>>>(a, y, out_state, g);
+    }
   });
   DLVK_POST_LAUNCH();
 }
 
-int64_t short_conv_part_floats(const ShortConv& a) { return run_rows(a) * (a.taps + 1) * a.D; }
+namespace {
+bool wide_bwd(const ShortConv& a, const SeqRef& dy, const SeqRef& dx) {
+  const int64_t bytes = a.dt == DType::BF16 ? 2 : 4;
+  return aligned(a, BWD_VEC) && aligned(dy, BWD_VEC, bytes) && aligned(dx, BWD_VEC, bytes);
+}
+}  // namespace
+
+// The larger of the two ways to divide the channels.
+int64_t short_conv_part_floats(const ShortConv& a) {
+  return std::max(grid_of(a, BWD_VEC, BWD_RUN).rows, grid_of(a, 1, BWD_RUN).rows) * (a.taps + 1) * a.D;
+}
 
 void short_conv_bwd(const ShortConv& a, SeqRef dy, SeqRef dx, float* dweight, float* dbias, bool accumulate, float* part,
                     cudaStream_t s) {
+  DLVK_CHECK(a.dt == DType::BF16 || a.dt == DType::F32, "short_conv: fp32 or bf16");
   if (a.D == 0) return;
-  const int64_t bytes = a.dt == DType::BF16 ? 2 : 4, rows = run_rows(a);
-  if (rows > 0) {
-    const bool wide = a.D % (16 / bytes) == 0 && aligned(a.x, bytes) && aligned(a.state, bytes) && aligned(dy, bytes) &&
-                      aligned(dx, bytes);
-    by_type(a.dt, wide, [&](auto type, auto vec) {
-      by_taps(a.taps, [&](auto taps) {
-        conv_bwd_kernel<decltype(type), decltype(vec)::value, decltype(taps)::value>
-            <<<grid_of(a, vec), dim3(32, RUNS), 0, s>>>(a, dy, dx, part, (a.T + RUN - 1) / RUN);
-      });
+  int64_t rows = 0;
+  if (a.B > 0 && a.T > 0) {
+    const bool wide = wide_bwd(a, dy, dx);
+    const Grid g = grid_of(a, wide ? BWD_VEC : 1, BWD_RUN);
+    rows = g.rows;
+    const unsigned n = (unsigned)(g.rows * g.blocks);
+    const dim3 block(32, RUNS);
+    by_taps(a.taps, [&](auto taps) {
+      constexpr int K = decltype(taps)::value;
+      if (a.dt == DType::BF16) {
+        if (wide) conv_bwd_kernel<__nv_bfloat16, BWD_VEC, K><<<n, block, 0, s>>>(a, dy, dx, part, g);
+        else conv_bwd_kernel<__nv_bfloat16, 1, K><<<n, block, 0, s>>>(a, dy, dx, part, g);
+      } else {
+        if (wide) conv_bwd_kernel<float, BWD_VEC, K><<<n, block, 0, s>>>(a, dy, dx, part, g);
+        else conv_bwd_kernel<float, 1, K><<<n, block, 0, s>>>(a, dy, dx, part, g);
+      }
     });
     DLVK_POST_LAUNCH();
   }

@@ -111,6 +111,12 @@ struct Four {
   typename Raw<T>::type raw;
   __device__ __forceinline__ float get(int i) const { return to_f32(reinterpret_cast<const T*>(&raw)[i]); }
   __device__ __forceinline__ void set(int i, float v) { reinterpret_cast<T*>(&raw)[i] = from_f32<T>(v); }
+  __device__ __forceinline__ static Four zeros() {
+    Four f;
+#pragma unroll
+    for (int i = 0; i < V; ++i) f.set(i, 0.f);
+    return f;
+  }
   // `count` of them
   template <bool WIDE>
   __device__ __forceinline__ void store(T* p, int count) const {
@@ -317,7 +323,8 @@ __global__ void __launch_bounds__(THREADS) scan_ends_kernel(StateScan a, SeqRef 
   const Place<L> me;
   const bool real = me.ch < tile.count;
   const int64_t n = length_of(a, tile.b), spans = (a.T + SPAN - 1) / SPAN;
-  const int64_t from = blockIdx.y * pieces.spans, to = min(spans, from + pieces.spans);
+  const int64_t from = blockIdx.y * pieces.spans;
+  const int64_t to = min(min(spans, from + pieces.spans), (n + SPAN - 1) / SPAN);  // spans with a token that counts
   Quad h{}, rate{};
   if (real) rate = load_rates(a, tile.c0 + me.ch, me.n0, LOG2E);
   for (int j = threadIdx.x; j < CH; j += THREADS) sh.bias[j] = a.dt_bias && j < tile.count ? a.dt_bias[tile.c0 + j] : 0.f;
@@ -438,7 +445,8 @@ __global__ void __launch_bounds__(THREADS) scan_fwd_kernel(StateScan a, SeqRef y
   const int lane = me.lane, n0 = me.n0, ch = me.ch;
   const bool real = ch < tile.count;
   const int64_t n = length_of(a, tile.b), spans = (a.T + SPAN - 1) / SPAN;
-  const int64_t from = blockIdx.y * pieces.spans, to = min(spans, from + pieces.spans);
+  const int64_t from = blockIdx.y * pieces.spans, end = min(spans, from + pieces.spans);
+  const int64_t to = max(from, min(end, (n + SPAN - 1) / SPAN));  // spans with a token that counts
   const int64_t row = (tile.b * a.D + tile.c0 + ch) * a.N + n0;  // of this thread's states
   Quad h{}, rate{};
   if (real) {
@@ -528,6 +536,15 @@ __global__ void __launch_bounds__(THREADS) scan_fwd_kernel(StateScan a, SeqRef y
         out.set(j, t0 + t < n ? p : 0.f);
       }
       out.template store<WIDE>(at<T>(y, tile.b, t0 + t, tile.c0 + my.c), my.left);
+    }
+  }
+  for (int64_t k = to; k < end; ++k) {  // behind the sequence
+    if (saved && real) store_states(h, saved + ((tile.b * spans + k) * a.D + tile.c0 + ch) * a.N + n0, n0, a.N);
+#pragma unroll
+    for (int i = 0; i < my.PER; ++i) {
+      const int t = my.t + i * my.STEP;
+      if (t < SPAN && k * SPAN + t < a.T && my.left > 0)
+        Four<T>::zeros().template store<WIDE>(at<T>(y, tile.b, k * SPAN + t, tile.c0 + my.c), my.left);
     }
   }
   if (out_state && real && blockIdx.y + 1 == pieces.count) store_states(h, out_state + row, n0, a.N);
@@ -630,7 +647,8 @@ __global__ void __launch_bounds__(THREADS, 4) scan_bwd_kernel(StateScan a, const
   const bool real = ch < tile.count;
   const int64_t n = length_of(a, tile.b), spans = (a.T + SPAN - 1) / SPAN;
   Quad rate{}, ga{}, da{};
-  const int64_t from = blockIdx.y * pieces.spans, to = min(spans, from + pieces.spans);
+  const int64_t from = blockIdx.y * pieces.spans, end = min(spans, from + pieces.spans);
+  const int64_t to = max(from, min(end, (n + SPAN - 1) / SPAN));  // spans with a token that counts
   const int64_t piece = tile.b * pieces.count + blockIdx.y;
   if (real) {
     rate = load_rates(a, tile.c0 + ch, n0, 1.f);
@@ -658,6 +676,22 @@ __global__ void __launch_bounds__(THREADS, 4) scan_bwd_kernel(StateScan a, const
     fetch_four<float, WIDE>(reinterpret_cast<Four<float>*>(&st.h[threadIdx.x]),
                             saved + ((tile.b * spans + k) * a.D + tile.c0 + ch) * a.N + n0, saved, real ? a.N - n0 : 0);
   };
+  for (int64_t k = to; k < end; ++k) {  // behind the sequence
+    const int64_t t0 = k * SPAN;
+#pragma unroll
+    for (int i = 0; i < my.PER; ++i) {
+      const int t = my.t + i * my.STEP;
+      if (t < SPAN && t0 + t < a.T && my.left > 0) {
+        Four<T>::zeros().template store<WIDE>(at<T>(g.du, tile.b, t0 + t, tile.c0 + my.c), my.left);
+        Four<T>::zeros().template store<WIDE>(at<T>(g.ddt, tile.b, t0 + t, tile.c0 + my.c), my.left);
+        if (a.z.p) Four<T>::zeros().template store<WIDE>(at<T>(g.dz, tile.b, t0 + t, tile.c0 + my.c), my.left);
+      }
+    }
+    float* part = part_bc + (((tile.k * a.B + tile.b) * a.T + t0) * a.G + tile.group) * ROW;
+    for (int i = threadIdx.x * 4; i < SPAN * ROW; i += THREADS * 4)
+      if (t0 + i / ROW < a.T)
+        *reinterpret_cast<float4*>(part + (int64_t)(i / ROW) * a.G * ROW + i % ROW) = make_float4(0.f, 0.f, 0.f, 0.f);
+  }
   if (from < to) fetch(to - 1);
   copies_issued();
   __syncthreads();

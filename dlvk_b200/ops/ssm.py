@@ -129,8 +129,10 @@ def short_conv_bwd(x, weight, bias, dy, state=None, lengths=None, silu: bool = T
 
 
 def short_conv_step(x, weight, bias, state, silu: bool = True, out_state=None):
-    """One token x [sequences, channels] of each sequence: (y), and `state`
+    """y of one token x [sequences, channels] of each sequence; `state`
     moves on by it in place, or into `out_state` where that is given."""
+    if native(x):
+        return N().short_conv_step(x, weight, bias, state, silu, out_state)
     y, _ = short_conv_fwd(x.unsqueeze(1), weight, bias, state=state, silu=silu,
                           out_state=state if out_state is None else out_state)
     return y.squeeze(1)
@@ -290,6 +292,8 @@ def state_scan_step(u, dt, a_log, b, c, state, skip=None, z=None, dt_bias=None, 
     """One token of each sequence: u, dt, z [sequences, channels], b, c
     [sequences, states] or [sequences, groups, states].  Returns y; `state`
     moves on in place, or into `out_state` where that is given."""
+    if native(u):
+        return N().state_scan_step(u, dt, a_log, b, c, state, skip, z, dt_bias, out_state)
     y, _, _ = state_scan_fwd(u.unsqueeze(1), dt.unsqueeze(1), a_log, b.unsqueeze(1), c.unsqueeze(1), skip,
                              z.unsqueeze(1) if z is not None else None, dt_bias, state,
                              out_state=state if out_state is None else out_state)
