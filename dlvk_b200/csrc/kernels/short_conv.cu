@@ -16,8 +16,7 @@
 #include <algorithm>
 #include <type_traits>
 
-#include "dlvk/common.h"
-#include "dlvk/kernels.h"
+#include "dlvk/seq.h"
 
 namespace dlvk {
 namespace {
@@ -39,13 +38,6 @@ struct Vec {
   __device__ __forceinline__ float get(int i) const { return to_f32(reinterpret_cast<const T*>(&raw)[i]); }
   __device__ __forceinline__ void set(int i, float v) { reinterpret_cast<T*>(&raw)[i] = from_f32<T>(v); }
 };
-
-__device__ __forceinline__ float sigmoid(float x) { return __fdividef(1.f, 1.f + __expf(-x)); }
-
-template <typename T>
-__device__ __forceinline__ T* at(const SeqRef& r, int64_t b, int64_t t, int c) {
-  return static_cast<T*>(r.p) + b * r.batch + t * r.token + c;
-}
 
 template <int V, int K>
 __device__ __forceinline__ void load_taps(const ShortConv& a, int c, float (&w)[V][K], float (&bias)[V]) {
@@ -92,38 +84,51 @@ __device__ __forceinline__ int64_t length_of(const ShortConv& a, int64_t b) {
   return a.lengths ? min(max((int64_t)a.lengths[b], (int64_t)0), a.T) : a.T;
 }
 
-// Token t of a sequence of n that counts, or of the tokens before it, or zeros.
+// Token t of a sequence of n that counts, or of the tokens before it, or zeros:
+// always one load, of the taps where there is no such token (a branch around a
+// load would make the next one wait for it).
 template <typename T, int V, int K>
 __device__ __forceinline__ void token(const ShortConv& a, const Place& p, int64_t t, int64_t n, float (&x)[V]) {
-  const T* from = t >= 0 ? (t < n ? at<T>(a.x, p.b, t, p.c) : nullptr)
-                         : (a.state.p ? at<T>(a.state, p.b, t + K - 1, p.c) : nullptr);
+  const bool here = t >= 0 ? t < n : a.state.p != nullptr;
+  Vec<T, V> v;
+  v.load(!here ? reinterpret_cast<const T*>(a.weight) : t >= 0 ? at<T>(a.x, p.b, t, p.c) : at<T>(a.state, p.b, t + K - 1, p.c));
 #pragma unroll
-  for (int i = 0; i < V; ++i) x[i] = 0.f;
-  if (from) {
-    Vec<T, V> v;
-    v.load(from);
-#pragma unroll
-    for (int i = 0; i < V; ++i) x[i] = v.get(i);
-  }
+  for (int i = 0; i < V; ++i) x[i] = here ? v.get(i) : 0.f;
 }
 
-// COUNT tokens of r from t on, all asked for before any is used.  Past the
-// sequence's last one that is read again: a branch around a load would make the
-// next one wait for it.
+// Tokens t to t + COUNT of r, zeros past the sequence's n: copied to a place in
+// shared memory that this thread alone reads; single elements are loaded.
 template <typename T, int V, int COUNT>
-__device__ __forceinline__ void load_tokens(const SeqRef& r, const Place& p, int64_t t, int64_t n, Vec<T, V> (&v)[COUNT]) {
+struct Ahead {
+  Vec<T, V> v[COUNT][32 * RUNS];
+  __device__ __forceinline__ void fetch(const SeqRef& r, const Place& p, int64_t t, int64_t n) {
+    const int me = threadIdx.y * 32 + threadIdx.x;
 #pragma unroll
-  for (int k = 0; k < COUNT; ++k) v[k].load(at<T>(r, p.b, max(min(t + k, n - 1), (int64_t)0), p.c));
-}
+    for (int k = 0; k < COUNT; ++k) {
+      const bool here = t + k < n;
+      if constexpr (V * sizeof(T) >= 4) copy_async<V * sizeof(T)>(&v[k][me], here ? at<T>(r, p.b, t + k, p.c) : r.p, here);
+      else v[k][me].raw = here ? *at<T>(r, p.b, t + k, p.c) : from_f32<T>(0.f);
+    }
+  }
+  __device__ __forceinline__ const Vec<T, V>& operator[](int k) const { return v[k][threadIdx.y * 32 + threadIdx.x]; }
+};
+
+template <typename T, int V>
+struct FwdShared {
+  static constexpr int AHEAD = 8;
+  Ahead<T, V, AHEAD> x[2];
+};
 
 template <typename T, int V, int K>
-__global__ void __launch_bounds__(32 * RUNS) conv_fwd_kernel(ShortConv a, SeqRef y, SeqRef out_state, Grid grid) {
-  constexpr int AHEAD = 8;
+__global__ void __launch_bounds__(32 * RUNS, 2) conv_fwd_kernel(ShortConv a, SeqRef y, SeqRef out_state, Grid grid) {
+  constexpr int AHEAD = FwdShared<T, V>::AHEAD;
+  extern __shared__ __align__(16) char raw[];
+  auto& sh = *reinterpret_cast<FwdShared<T, V>*>(raw);
   const Place p = place<V>(a, grid);
   if (!p.ok) return;
-  const int64_t n = length_of(a, p.b);
-  Vec<T, V> v[AHEAD];
-  if (p.t < p.end) load_tokens<T, V, AHEAD>(a.x, p, p.t, n, v);
+  const int64_t n = length_of(a, p.b), stop = min(p.end, n);  // tokens of the run that count
+  if (p.t < stop) sh.x[0].fetch(a.x, p, p.t, stop);
+  copies_issued();
   float w[V][K], bias[V], last[K - 1][V];
   load_taps<V, K>(a, p.c, w, bias);
 #pragma unroll
@@ -141,16 +146,20 @@ __global__ void __launch_bounds__(32 * RUNS) conv_fwd_kernel(ShortConv a, SeqRef
       o.store(at<T>(out_state, p.b, j, p.c));
     }
   }
-  for (int64_t t0 = p.t; t0 < p.end; t0 += AHEAD) {
-    if (t0 > p.t) load_tokens<T, V, AHEAD>(a.x, p, t0, n, v);
+  int now = 0;
+  for (int64_t t0 = p.t; t0 < p.end; t0 += AHEAD, now ^= 1) {
+    if (t0 + AHEAD < stop) sh.x[now ^ 1].fetch(a.x, p, t0 + AHEAD, stop);
+    copies_issued();
+    wait_copies<1>();
 #pragma unroll
     for (int k = 0; k < AHEAD; ++k) {
       if (t0 + k >= p.end) break;
       const bool here = t0 + k < n;
+      const Vec<T, V> v = sh.x[now][k];
       Vec<T, V> out;
 #pragma unroll
       for (int i = 0; i < V; ++i) {
-        const float x = v[k].get(i);
+        const float x = v.get(i);
         float s = fmaf(w[i][K - 1], x, bias[i]);
 #pragma unroll
         for (int j = 0; j < K - 1; ++j) s = fmaf(w[i][j], last[j][i], s);
@@ -165,11 +174,20 @@ __global__ void __launch_bounds__(32 * RUNS) conv_fwd_kernel(ShortConv a, SeqRef
   }
 }
 
+template <typename T, int V>
+struct BwdShared {
+  static constexpr int AHEAD = 4, STAGES = 3;
+  Ahead<T, V, AHEAD> x[STAGES], g[STAGES];
+  float sums[RUNS][32 * V + 1];
+};
+
 // part [block rows][K + 1][D]: the sums of a block's runs, bias last.
 template <typename T, int V, int K>
-__global__ void __launch_bounds__(32 * RUNS) conv_bwd_kernel(ShortConv a, SeqRef dy, SeqRef dx, float* __restrict__ part,
-                                                             Grid grid) {
-  constexpr int AHEAD = 4;
+__global__ void __launch_bounds__(32 * RUNS, 2) conv_bwd_kernel(ShortConv a, SeqRef dy, SeqRef dx, float* __restrict__ part,
+                                                                Grid grid) {
+  constexpr int AHEAD = BwdShared<T, V>::AHEAD, STAGES = BwdShared<T, V>::STAGES;
+  extern __shared__ __align__(16) char raw[];
+  auto& sh = *reinterpret_cast<BwdShared<T, V>*>(raw);
   const Place p = place<V>(a, grid);
   float dw[V][K + 1];
 #pragma unroll
@@ -178,6 +196,16 @@ __global__ void __launch_bounds__(32 * RUNS) conv_bwd_kernel(ShortConv a, SeqRef
     for (int j = 0; j <= K; ++j) dw[i][j] = 0.f;
   if (p.ok) {
     const int64_t n = length_of(a, p.b);
+    const int64_t past = p.end + K - 1, stop = min(past, n);  // the tokens behind the run for their g alone
+    const auto fetch = [&](int64_t t, int stage) {
+      if (t < stop) {
+        sh.x[stage].fetch(a.x, p, t, stop);
+        sh.g[stage].fetch(dy, p, t, stop);
+      }
+      copies_issued();
+    };
+#pragma unroll
+    for (int i = 0; i < STAGES - 1; ++i) fetch(p.t + i * AHEAD, i);
     float w[V][K], bias[V], x[K - 1 + AHEAD][V], g[K - 1 + AHEAD][V];  // the last K - 1 tokens first
     load_taps<V, K>(a, p.c, w, bias);
 #pragma unroll
@@ -186,27 +214,27 @@ __global__ void __launch_bounds__(32 * RUNS) conv_bwd_kernel(ShortConv a, SeqRef
 #pragma unroll
       for (int i = 0; i < V; ++i) g[j][i] = 0.f;
     }
-    // the K - 1 tokens behind the run for their g alone
-    for (int64_t t0 = p.t; t0 < p.end + K - 1; t0 += AHEAD) {
-      Vec<T, V> vx[AHEAD], vg[AHEAD];
-      load_tokens<T, V, AHEAD>(a.x, p, t0, n, vx);
-      load_tokens<T, V, AHEAD>(dy, p, t0, n, vg);
+    int now = 0;
+    for (int64_t t0 = p.t; t0 < past; t0 += AHEAD) {
+      fetch(t0 + (STAGES - 1) * AHEAD, now == 0 ? STAGES - 1 : now - 1);
+      wait_copies<STAGES - 1>();
 #pragma unroll
       for (int k = 0; k < AHEAD; ++k) {
         const int64_t t = t0 + k;
+        const Vec<T, V> vx = sh.x[now][k], vg = sh.g[now][k];
+        const bool here = t < stop;
         Vec<T, V> out;
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-          x[K - 1 + k][i] = t < n ? vx[k].get(i) : 0.f;
-          float gi = vg[k].get(i);
+          x[K - 1 + k][i] = here ? vx.get(i) : 0.f;
+          float gi = here ? vg.get(i) : 0.f;
           if (a.silu) {
             float s = bias[i];
 #pragma unroll
             for (int j = 0; j < K; ++j) s = fmaf(w[i][j], x[k + j][i], s);
             const float q = sigmoid(s);
-            gi *= q * fmaf(s, 1.f - q, 1.f);
+            gi = here ? gi * (q * fmaf(s, 1.f - q, 1.f)) : 0.f;
           }
-          gi = t < n ? gi : 0.f;
           g[K - 1 + k][i] = gi;
           const float own = t < p.end ? gi : 0.f;
 #pragma unroll
@@ -217,26 +245,26 @@ __global__ void __launch_bounds__(32 * RUNS) conv_bwd_kernel(ShortConv a, SeqRef
           for (int j = 0; j < K; ++j) d = fmaf(w[i][j], g[K - 1 + k - j][i], d);
           out.set(i, d);
         }
-        if (t - (K - 1) >= p.t && t - (K - 1) < p.end) out.store(at<T>(dx, p.b, t - (K - 1), p.c));
+        if (t - (K - 1) >= p.t && t < past) out.store(at<T>(dx, p.b, t - (K - 1), p.c));
       }
 #pragma unroll
       for (int j = 0; j < K - 1; ++j)
 #pragma unroll
         for (int i = 0; i < V; ++i) x[j][i] = x[AHEAD + j][i], g[j][i] = g[AHEAD + j][i];
+      now = now + 1 == STAGES ? 0 : now + 1;
     }
   }
-  __shared__ float sums[RUNS][32 * V + 1];
   const int64_t row = blockIdx.x / grid.blocks;
 #pragma unroll
   for (int j = 0; j <= K; ++j) {
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < V; ++i) sums[threadIdx.y][threadIdx.x * V + i] = dw[i][j];
+    for (int i = 0; i < V; ++i) sh.sums[threadIdx.y][threadIdx.x * V + i] = dw[i][j];
     __syncthreads();
     for (int c = threadIdx.y * 32 + threadIdx.x; c < 32 * V; c += 32 * RUNS) {
       float s = 0.f;
 #pragma unroll
-      for (int r = 0; r < RUNS; ++r) s += sums[r][c];
+      for (int r = 0; r < RUNS; ++r) s += sh.sums[r][c];
       const int d = (int)(blockIdx.x % grid.blocks) * 32 * V + c;
       if (d < a.D) part[(row * (K + 1) + j) * a.D + d] = s;
     }
@@ -273,19 +301,25 @@ bool aligned(const ShortConv& a, int v) {
          aligned(a.state, v, bytes);
 }
 
-// Runs as long as some ten warps are left for every SM (a run reads K - 1 tokens
-// again, and the taps), at most `most` tokens.
-Grid grid_of(const ShortConv& a, int v, int64_t most) {
+// As many runs as there are warps on the GPU at once (two blocks an SM), each of
+// at least eight tokens: a run reads K - 1 tokens again, and the taps.
+Grid grid_of(const ShortConv& a, int v) {
   Grid g;
   g.blocks = (a.D + 32 * v - 1) / (32 * v);
-  g.run = most;
-  while (g.run > 8 && a.B * ((a.T + g.run - 1) / g.run) * g.blocks < 148 * 10) g.run /= 2;
+  const int64_t fit = std::max<int64_t>(1, 148 * 2 * RUNS / std::max<int64_t>(1, a.B * g.blocks));
+  g.run = std::max<int64_t>(8, (a.T + fit - 1) / fit);
   g.runs = std::max<int64_t>(1, (a.T + g.run - 1) / g.run);
   g.rows = (a.B * g.runs + RUNS - 1) / RUNS;
   DLVK_CHECK(g.rows * g.blocks < (1LL << 31), "short_conv: too many elements for one launch");
   return g;
 }
-constexpr int64_t FWD_RUN = 32, BWD_RUN = 64;
+template <typename Kernel, typename... Args>
+void launch(Kernel kernel, size_t smem, const Grid& g, cudaStream_t s, Args... args) {
+  if (smem > 48 * 1024)
+    DLVK_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  kernel<<<(unsigned)(g.rows * g.blocks), dim3(32, RUNS), smem, s>>>(args..., g);
+  DLVK_POST_LAUNCH();
+}
 constexpr int BWD_VEC = 4;  // the backward pass keeps K + 3 tokens of two tensors in registers
 
 template <typename F>
@@ -307,20 +341,18 @@ void short_conv_fwd(const ShortConv& a, SeqRef y, SeqRef out_state, cudaStream_t
   const int64_t bytes = a.dt == DType::BF16 ? 2 : 4;
   const int v = 16 / (int)bytes;
   const bool wide = aligned(a, v) && aligned(y, v, bytes) && aligned(out_state, v, bytes);
-  const Grid g = grid_of(a, wide ? v : 1, FWD_RUN);
-  const unsigned n = (unsigned)(g.rows * g.blocks);
-  const dim3 block(32, RUNS);
+  const Grid g = grid_of(a, wide ? v : 1);
   by_taps(a.taps, [&](auto taps) {
     constexpr int K = decltype(taps)::value;
+    using bf16 = __nv_bfloat16;
     if (a.dt == DType::BF16) {
-      if (wide) conv_fwd_kernel<__nv_bfloat16, 8, K><<<n, block, 0, s>>>(a, y, out_state, g);
-      else conv_fwd_kernel<__nv_bfloat16, 1, K><<<n, block, 0, s>>>(a, y, out_state, g);
+      if (wide) launch(conv_fwd_kernel<bf16, 8, K>, sizeof(FwdShared<bf16, 8>), g, s, a, y, out_state);
+      else launch(conv_fwd_kernel<bf16, 1, K>, sizeof(FwdShared<bf16, 1>), g, s, a, y, out_state);
     } else {
-      if (wide) conv_fwd_kernel<float, 4, K><<<n, block, 0, s>>>(a, y, out_state, g);
-      else conv_fwd_kernel<float, 1, K><<<n, block, 0, s>>>(a, y, out_state, g);
+      if (wide) launch(conv_fwd_kernel<float, 4, K>, sizeof(FwdShared<float, 4>), g, s, a, y, out_state);
+      else launch(conv_fwd_kernel<float, 1, K>, sizeof(FwdShared<float, 1>), g, s, a, y, out_state);
     }
   });
-  DLVK_POST_LAUNCH();
 }
 
 namespace {
@@ -332,7 +364,7 @@ bool wide_bwd(const ShortConv& a, const SeqRef& dy, const SeqRef& dx) {
 
 // The larger of the two ways to divide the channels.
 int64_t short_conv_part_floats(const ShortConv& a) {
-  return std::max(grid_of(a, BWD_VEC, BWD_RUN).rows, grid_of(a, 1, BWD_RUN).rows) * (a.taps + 1) * a.D;
+  return std::max(grid_of(a, BWD_VEC).rows, grid_of(a, 1).rows) * (a.taps + 1) * a.D;
 }
 
 void short_conv_bwd(const ShortConv& a, SeqRef dy, SeqRef dx, float* dweight, float* dbias, bool accumulate, float* part,
@@ -342,21 +374,19 @@ void short_conv_bwd(const ShortConv& a, SeqRef dy, SeqRef dx, float* dweight, fl
   int64_t rows = 0;
   if (a.B > 0 && a.T > 0) {
     const bool wide = wide_bwd(a, dy, dx);
-    const Grid g = grid_of(a, wide ? BWD_VEC : 1, BWD_RUN);
+    const Grid g = grid_of(a, wide ? BWD_VEC : 1);
     rows = g.rows;
-    const unsigned n = (unsigned)(g.rows * g.blocks);
-    const dim3 block(32, RUNS);
     by_taps(a.taps, [&](auto taps) {
-      constexpr int K = decltype(taps)::value;
+      constexpr int K = decltype(taps)::value, W = BWD_VEC;
+      using bf16 = __nv_bfloat16;
       if (a.dt == DType::BF16) {
-        if (wide) conv_bwd_kernel<__nv_bfloat16, BWD_VEC, K><<<n, block, 0, s>>>(a, dy, dx, part, g);
-        else conv_bwd_kernel<__nv_bfloat16, 1, K><<<n, block, 0, s>>>(a, dy, dx, part, g);
+        if (wide) launch(conv_bwd_kernel<bf16, W, K>, sizeof(BwdShared<bf16, W>), g, s, a, dy, dx, part);
+        else launch(conv_bwd_kernel<bf16, 1, K>, sizeof(BwdShared<bf16, 1>), g, s, a, dy, dx, part);
       } else {
-        if (wide) conv_bwd_kernel<float, BWD_VEC, K><<<n, block, 0, s>>>(a, dy, dx, part, g);
-        else conv_bwd_kernel<float, 1, K><<<n, block, 0, s>>>(a, dy, dx, part, g);
+        if (wide) launch(conv_bwd_kernel<float, W, K>, sizeof(BwdShared<float, W>), g, s, a, dy, dx, part);
+        else launch(conv_bwd_kernel<float, 1, K>, sizeof(BwdShared<float, 1>), g, s, a, dy, dx, part);
       }
     });
-    DLVK_POST_LAUNCH();
   }
   conv_join_kernel<<<(unsigned)(((int64_t)(a.taps + 1) * a.D + 31) / 32), dim3(32, 8), 0, s>>>(
       part, rows, a.D, a.taps, dweight, dbias, accumulate);

@@ -20,8 +20,7 @@
 #include <algorithm>
 #include <type_traits>
 
-#include "dlvk/common.h"
-#include "dlvk/kernels.h"
+#include "dlvk/seq.h"
 
 namespace dlvk {
 namespace {
@@ -32,12 +31,6 @@ constexpr int V = 4;   // elements of a thread's load
 constexpr int SPAN = STATE_SCAN_SPAN;
 constexpr float LOG2E = 1.4426950408889634f;
 
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-__device__ __forceinline__ float sigmoid(float x) { return __fdividef(1.f, 1.f + __expf(-x)); }
 // softplus(x) = max(x, 0) + log(1 + e), e = exp(-|x|).  Steps are small, so log(1 + e) has to
 // keep its relative precision: 2 atanh(r), r = e / (2 + e) <= 1/3, by its series (to r^17: 2^-25);
 // the exponent's rounding is made good by its remainder.
@@ -130,17 +123,6 @@ struct Four {
   }
 };
 
-// BYTES from global to shared memory without a register, zeros instead where not `there`.
-template <int BYTES>
-__device__ __forceinline__ void copy_async(void* dst, const void* src, bool there) {
-  const uint32_t to = (uint32_t)__cvta_generic_to_shared(dst);
-  const int n = there ? BYTES : 0;
-  asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(to), "l"(src), "n"(BYTES), "r"(n) : "memory");
-}
-__device__ __forceinline__ void copies_issued() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-// All copies of this thread but those of the last group have come.
-__device__ __forceinline__ void wait_but_last() { asm volatile("cp.async.wait_group 1;" ::: "memory"); }
-
 // Four elements from p on, `count` of them (0: none) from memory, the others zeros.
 // WIDE: rows of whole aligned fours, one copy.  Else fp32 is copied element by
 // element, bf16 (2 bytes are too few for a copy) loaded.
@@ -160,10 +142,6 @@ __device__ __forceinline__ void fetch_four(Four<T>* dst, const T* p, const void*
   }
 }
 
-template <typename T>
-__device__ __forceinline__ T* at(const SeqRef& r, int64_t b, int64_t t, int64_t c) {
-  return static_cast<T*>(r.p) + b * r.batch + t * r.token + c;
-}
 __device__ __forceinline__ int64_t length_of(const StateScan& a, int64_t b) {
   return a.lengths ? min(max((int64_t)a.lengths[b], (int64_t)0), a.T) : a.T;
 }
@@ -355,7 +333,7 @@ __global__ void __launch_bounds__(THREADS) scan_ends_kernel(StateScan a, SeqRef 
     auto& now = sh.stage[k % 2];
     if (i + 1 < count) fetch(span_of(i + 1));
     copies_issued();
-    wait_but_last();
+    wait_copies<1>();
 #pragma unroll
     for (int e = 0; e < my.PER; ++e) {
       const int t = my.t + e * my.STEP;
@@ -482,7 +460,7 @@ __global__ void __launch_bounds__(THREADS) scan_fwd_kernel(StateScan a, SeqRef y
     auto& now = sh.stage[k % 2];
     if (k + 1 < to) fetch(k + 1);
     copies_issued();
-    wait_but_last();
+    wait_copies<1>();
 #pragma unroll
     for (int i = 0; i < my.PER; ++i) {
       const int t = my.t + i * my.STEP;
@@ -700,7 +678,7 @@ __global__ void __launch_bounds__(THREADS, 4) scan_bwd_kernel(StateScan a, const
     auto& now = sh.stage[k % 2];
     if (k > from) fetch(k - 1);
     copies_issued();
-    wait_but_last();
+    wait_copies<1>();
 #pragma unroll
     for (int i = 0; i < my.PER; ++i) {
       const int t = my.t + i * my.STEP;
