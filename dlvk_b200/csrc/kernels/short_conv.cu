@@ -30,31 +30,46 @@ template <> struct Pack<__nv_bfloat16, 8> { using type = uint4; };
 template <> struct Pack<__nv_bfloat16, 4> { using type = uint2; };
 template <> struct Pack<__nv_bfloat16, 1> { using type = __nv_bfloat16; };
 
+// V neighbouring channels of a token, in pairs (a single one is half a pair).
 template <typename T, int V>
 struct Vec {
+  static constexpr int PAIRS = (V + 1) / 2;
   typename Pack<T, V>::type raw;
   __device__ __forceinline__ void load(const T* p) { raw = *reinterpret_cast<const typename Pack<T, V>::type*>(p); }
   __device__ __forceinline__ void store(T* p) const { *reinterpret_cast<typename Pack<T, V>::type*>(p) = raw; }
-  __device__ __forceinline__ float get(int i) const { return to_f32(reinterpret_cast<const T*>(&raw)[i]); }
-  __device__ __forceinline__ void set(int i, float v) { reinterpret_cast<T*>(&raw)[i] = from_f32<T>(v); }
+  __device__ __forceinline__ f2 get(int i) const {
+    const T* e = reinterpret_cast<const T*>(&raw);
+    if constexpr (V == 1) return pack(to_f32(e[0]), 0.f);
+    else return pack(to_f32(e[2 * i]), to_f32(e[2 * i + 1]));
+  }
+  __device__ __forceinline__ void set(int i, f2 v) {
+    const float2 f = unpack(v);
+    T* e = reinterpret_cast<T*>(&raw);
+    if constexpr (V == 1) e[0] = from_f32<T>(f.x);
+    else if constexpr (sizeof(T) == 2) reinterpret_cast<__nv_bfloat162*>(&raw)[i] = __floats2bfloat162_rn(f.x, f.y);
+    else e[2 * i] = f.x, e[2 * i + 1] = f.y;
+  }
 };
 
 template <int V, int K>
-__device__ __forceinline__ void load_taps(const ShortConv& a, int c, float (&w)[V][K], float (&bias)[V]) {
-  float flat[V * K];
+__device__ __forceinline__ void load_taps(const ShortConv& a, int c, f2 (&w)[(V + 1) / 2][K], f2 (&bias)[(V + 1) / 2]) {
+  float flat[2 * K * ((V + 1) / 2)], b[V + V % 2];
   if constexpr (V > 1) {  // whole aligned fours
 #pragma unroll
     for (int i = 0; i < V * K; i += 4)
       *reinterpret_cast<float4*>(&flat[i]) = *reinterpret_cast<const float4*>(a.weight + (int64_t)c * K + i);
   } else {
 #pragma unroll
-    for (int i = 0; i < K; ++i) flat[i] = a.weight[(int64_t)c * K + i];
+    for (int i = 0; i < K; ++i) flat[i] = a.weight[(int64_t)c * K + i], flat[K + i] = 0.f;
+    b[1] = 0.f;
   }
 #pragma unroll
-  for (int i = 0; i < V; ++i) {
+  for (int i = 0; i < V; ++i) b[i] = a.bias ? a.bias[c + i] : 0.f;
 #pragma unroll
-    for (int j = 0; j < K; ++j) w[i][j] = flat[i * K + j];
-    bias[i] = a.bias ? a.bias[c + i] : 0.f;
+  for (int i = 0; i < (V + 1) / 2; ++i) {
+#pragma unroll
+    for (int j = 0; j < K; ++j) w[i][j] = pack(flat[2 * i * K + j], flat[(2 * i + 1) * K + j]);
+    bias[i] = pack(b[2 * i], b[2 * i + 1]);
   }
 }
 
@@ -88,12 +103,12 @@ __device__ __forceinline__ int64_t length_of(const ShortConv& a, int64_t b) {
 // always one load, of the taps where there is no such token (a branch around a
 // load would make the next one wait for it).
 template <typename T, int V, int K>
-__device__ __forceinline__ void token(const ShortConv& a, const Place& p, int64_t t, int64_t n, float (&x)[V]) {
+__device__ __forceinline__ void token(const ShortConv& a, const Place& p, int64_t t, int64_t n, f2 (&x)[(V + 1) / 2]) {
   const bool here = t >= 0 ? t < n : a.state.p != nullptr;
   Vec<T, V> v;
   v.load(!here ? reinterpret_cast<const T*>(a.weight) : t >= 0 ? at<T>(a.x, p.b, t, p.c) : at<T>(a.state, p.b, t + K - 1, p.c));
 #pragma unroll
-  for (int i = 0; i < V; ++i) x[i] = here ? v.get(i) : 0.f;
+  for (int i = 0; i < (V + 1) / 2; ++i) x[i] = here ? v.get(i) : 0;
 }
 
 // Tokens t to t + COUNT of r, zeros past the sequence's n: copied to a place in
@@ -129,47 +144,50 @@ __global__ void __launch_bounds__(32 * RUNS, 2) conv_fwd_kernel(ShortConv a, Seq
   const int64_t n = length_of(a, p.b), stop = min(p.end, n);  // tokens of the run that count
   if (p.t < stop) sh.x[0].fetch(a.x, p, p.t, stop);
   copies_issued();
-  float w[V][K], bias[V], last[K - 1][V];
+  constexpr int P = Vec<T, V>::PAIRS;
+  f2 w[P][K], bias[P], last[K - 1][P];
   load_taps<V, K>(a, p.c, w, bias);
 #pragma unroll
   for (int j = 0; j < K - 1; ++j) token<T, V, K>(a, p, p.t - (K - 1) + j, n, last[j]);
   if (out_state.p && p.t == 0) {
     // read before any of it is written: out_state may be the state
-    float keep[K - 1][V];
+    f2 keep[K - 1][P];
 #pragma unroll
     for (int j = 0; j < K - 1; ++j) token<T, V, K>(a, p, n - (K - 1) + j, n, keep[j]);
 #pragma unroll
     for (int j = 0; j < K - 1; ++j) {
       Vec<T, V> o;
 #pragma unroll
-      for (int i = 0; i < V; ++i) o.set(i, keep[j][i]);
+      for (int i = 0; i < P; ++i) o.set(i, keep[j][i]);
       o.store(at<T>(out_state, p.b, j, p.c));
     }
   }
   int now = 0;
+  T* to = at<T>(y, p.b, p.t, p.c);
   for (int64_t t0 = p.t; t0 < p.end; t0 += AHEAD, now ^= 1) {
     if (t0 + AHEAD < stop) sh.x[now ^ 1].fetch(a.x, p, t0 + AHEAD, stop);
     copies_issued();
     wait_copies<1>();
+    const int count = (int)min((int64_t)AHEAD, p.end - t0), real = (int)max((int64_t)0, min((int64_t)AHEAD, n - t0));
 #pragma unroll
     for (int k = 0; k < AHEAD; ++k) {
-      if (t0 + k >= p.end) break;
-      const bool here = t0 + k < n;
+      if (k >= count) break;
       const Vec<T, V> v = sh.x[now][k];
       Vec<T, V> out;
 #pragma unroll
-      for (int i = 0; i < V; ++i) {
-        const float x = v.get(i);
-        float s = fmaf(w[i][K - 1], x, bias[i]);
+      for (int i = 0; i < P; ++i) {
+        const f2 x = v.get(i);
+        f2 s = fma2(w[i][K - 1], x, bias[i]);
 #pragma unroll
-        for (int j = 0; j < K - 1; ++j) s = fmaf(w[i][j], last[j][i], s);
+        for (int j = 0; j < K - 1; ++j) s = fma2(w[i][j], last[j][i], s);
 #pragma unroll
         for (int j = 0; j < K - 2; ++j) last[j][i] = last[j + 1][i];
         last[K - 2][i] = x;
-        if (a.silu) s *= sigmoid(s);
-        out.set(i, here ? s : 0.f);
+        if (a.silu) s = mul2(s, sigmoid_2(s));
+        out.set(i, k < real ? s : 0);
       }
-      out.store(at<T>(y, p.b, t0 + k, p.c));
+      out.store(to);
+      to += y.token;
     }
   }
 }
@@ -188,12 +206,13 @@ __global__ void __launch_bounds__(32 * RUNS, 2) conv_bwd_kernel(ShortConv a, Seq
   constexpr int AHEAD = BwdShared<T, V>::AHEAD, STAGES = BwdShared<T, V>::STAGES;
   extern __shared__ __align__(16) char raw[];
   auto& sh = *reinterpret_cast<BwdShared<T, V>*>(raw);
+  constexpr int P = Vec<T, V>::PAIRS;
   const Place p = place<V>(a, grid);
-  float dw[V][K + 1];
+  f2 dw[P][K + 1];
 #pragma unroll
-  for (int i = 0; i < V; ++i)
+  for (int i = 0; i < P; ++i)
 #pragma unroll
-    for (int j = 0; j <= K; ++j) dw[i][j] = 0.f;
+    for (int j = 0; j <= K; ++j) dw[i][j] = 0;
   if (p.ok) {
     const int64_t n = length_of(a, p.b);
     const int64_t past = p.end + K - 1, stop = min(past, n);  // the tokens behind the run for their g alone
@@ -206,51 +225,61 @@ __global__ void __launch_bounds__(32 * RUNS, 2) conv_bwd_kernel(ShortConv a, Seq
     };
 #pragma unroll
     for (int i = 0; i < STAGES - 1; ++i) fetch(p.t + i * AHEAD, i);
-    float w[V][K], bias[V], x[K - 1 + AHEAD][V], g[K - 1 + AHEAD][V];  // the last K - 1 tokens first
+    f2 w[P][K], bias[P], x[K - 1 + AHEAD][P], g[K - 1 + AHEAD][P];  // the last K - 1 tokens first
     load_taps<V, K>(a, p.c, w, bias);
 #pragma unroll
     for (int j = 0; j < K - 1; ++j) {
       token<T, V, K>(a, p, p.t - (K - 1) + j, n, x[j]);
 #pragma unroll
-      for (int i = 0; i < V; ++i) g[j][i] = 0.f;
+      for (int i = 0; i < P; ++i) g[j][i] = 0;
     }
+    const f2 one = pack(1.f, 1.f), minus = pack(-1.f, -1.f);
     int now = 0;
-    for (int64_t t0 = p.t; t0 < past; t0 += AHEAD) {
-      fetch(t0 + (STAGES - 1) * AHEAD, now == 0 ? STAGES - 1 : now - 1);
-      wait_copies<STAGES - 1>();
+    T* to = at<T>(dx, p.b, p.t - (K - 1), p.c);
+    // AHEAD tokens from t0 on; EDGE: not all of them are the run's own, count, and lie behind its first K - 1
+    const auto walk = [&](int64_t t0, auto edge) {
+      constexpr bool EDGE = decltype(edge)::value;
 #pragma unroll
       for (int k = 0; k < AHEAD; ++k) {
         const int64_t t = t0 + k;
         const Vec<T, V> vx = sh.x[now][k], vg = sh.g[now][k];
-        const bool here = t < stop;
+        const bool here = !EDGE || t < stop;
         Vec<T, V> out;
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-          x[K - 1 + k][i] = here ? vx.get(i) : 0.f;
-          float gi = here ? vg.get(i) : 0.f;
+        for (int i = 0; i < P; ++i) {
+          x[K - 1 + k][i] = here ? vx.get(i) : 0;
+          f2 gi = vg.get(i);
           if (a.silu) {
-            float s = bias[i];
+            f2 s = bias[i];
 #pragma unroll
-            for (int j = 0; j < K; ++j) s = fmaf(w[i][j], x[k + j][i], s);
-            const float q = sigmoid(s);
-            gi = here ? gi * (q * fmaf(s, 1.f - q, 1.f)) : 0.f;
+            for (int j = 0; j < K; ++j) s = fma2(w[i][j], x[k + j][i], s);
+            const f2 q = sigmoid_2(s);
+            gi = mul2(gi, mul2(q, fma2(s, fma2(q, minus, one), one)));
           }
+          gi = here ? gi : 0;
           g[K - 1 + k][i] = gi;
-          const float own = t < p.end ? gi : 0.f;
+          const f2 own = !EDGE || t < p.end ? gi : 0;
 #pragma unroll
-          for (int j = 0; j < K; ++j) dw[i][j] = fmaf(own, x[k + j][i], dw[i][j]);
-          dw[i][K] += own;
-          float d = 0.f;  // dx[t - K + 1] = sum_j w[j] g[t - j]
+          for (int j = 0; j < K; ++j) dw[i][j] = fma2(own, x[k + j][i], dw[i][j]);
+          dw[i][K] = add2(dw[i][K], own);
+          f2 d = mul2(w[i][0], g[K - 1 + k][i]);  // dx[t - K + 1] = sum_j w[j] g[t - j]
 #pragma unroll
-          for (int j = 0; j < K; ++j) d = fmaf(w[i][j], g[K - 1 + k - j][i], d);
+          for (int j = 1; j < K; ++j) d = fma2(w[i][j], g[K - 1 + k - j][i], d);
           out.set(i, d);
         }
-        if (t - (K - 1) >= p.t && t < past) out.store(at<T>(dx, p.b, t - (K - 1), p.c));
+        if (!EDGE || (t - (K - 1) >= p.t && t < past)) out.store(to);
+        to += dx.token;
       }
+    };
+    for (int64_t t0 = p.t; t0 < past; t0 += AHEAD) {
+      fetch(t0 + (STAGES - 1) * AHEAD, now == 0 ? STAGES - 1 : now - 1);
+      wait_copies<STAGES - 1>();
+      if (t0 > p.t && t0 + AHEAD <= min(stop, p.end)) walk(t0, std::false_type());
+      else walk(t0, std::true_type());
 #pragma unroll
       for (int j = 0; j < K - 1; ++j)
 #pragma unroll
-        for (int i = 0; i < V; ++i) x[j][i] = x[AHEAD + j][i], g[j][i] = g[AHEAD + j][i];
+        for (int i = 0; i < P; ++i) x[j][i] = x[AHEAD + j][i], g[j][i] = g[AHEAD + j][i];
       now = now + 1 == STAGES ? 0 : now + 1;
     }
   }
@@ -259,7 +288,10 @@ __global__ void __launch_bounds__(32 * RUNS, 2) conv_bwd_kernel(ShortConv a, Seq
   for (int j = 0; j <= K; ++j) {
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < V; ++i) sh.sums[threadIdx.y][threadIdx.x * V + i] = dw[i][j];
+    for (int i = 0; i < V; ++i) {
+      const float2 d = unpack(dw[i / 2][j]);
+      sh.sums[threadIdx.y][threadIdx.x * V + i] = i % 2 ? d.y : d.x;
+    }
     __syncthreads();
     for (int c = threadIdx.y * 32 + threadIdx.x; c < 32 * V; c += 32 * RUNS) {
       float s = 0.f;

@@ -29,7 +29,6 @@ constexpr int THREADS = 128, WARPS = THREADS / 32;
 constexpr int NS = 4;  // states of a thread
 constexpr int V = 4;   // elements of a thread's load
 constexpr int SPAN = STATE_SCAN_SPAN;
-constexpr float LOG2E = 1.4426950408889634f;
 
 // softplus(x) = max(x, 0) + log(1 + e), e = exp(-|x|).  Steps are small, so log(1 + e) has to
 // keep its relative precision: 2 atanh(r), r = e / (2 + e) <= 1/3, by its series (to r^17: 2^-25);
@@ -38,7 +37,7 @@ __device__ __forceinline__ float softplus(float x) {
   const float m = -fabsf(x), t = m * LOG2E, rest = fmaf(m, LOG2E, -t) + m * 1.925963033500e-8f;
   float e = ex2(t);
   e = fmaf(e, rest * 0.6931472f, e);
-  const float r = __fdividef(e, 2.f + e), r2 = r * r;
+  const float r = e * rcp(2.f + e), r2 = r * r;
   float p = fmaf(r2, 1.f / 17, 1.f / 15);
   p = fmaf(r2, p, 1.f / 13);
   p = fmaf(r2, p, 1.f / 11);
@@ -49,37 +48,11 @@ __device__ __forceinline__ float softplus(float x) {
   return fmaxf(x, 0.f) + 2.f * fmaf(r * r2, p, r);
 }
 
-// Two fp32 numbers in one instruction.
-using f2 = unsigned long long;
-__device__ __forceinline__ f2 pack(float a, float b) {
-  f2 r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-  return r;
-}
-__device__ __forceinline__ float2 unpack(f2 a) {
-  float2 r;
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(a));
-  return r;
-}
-__device__ __forceinline__ f2 fma2(f2 a, f2 b, f2 c) {
-  f2 r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
-}
-__device__ __forceinline__ f2 mul2(f2 a, f2 b) {
-  f2 r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
 __device__ __forceinline__ float both(f2 a) {
   const float2 v = unpack(a);
   return v.x + v.y;
 }
-__device__ __forceinline__ f2 ex2_2(f2 x) {
-  const float2 v = unpack(x);
-  return pack(ex2(v.x), ex2(v.y));
-}
-// The same, never taken from a register that an equal one has filled before: the
+// ex2_2, never taken from a register that an equal one has filled before: the
 // backward pass's decays of a span would fill 64.
 __device__ __forceinline__ f2 ex2_2_again(f2 x) {
   float2 v = unpack(x);
@@ -913,12 +886,12 @@ bool wide_operands(const StateScan& a) {
 int64_t part_bc_floats(const StateScan& a) { return (int64_t)tiles_of(a) * a.B * a.T * a.G * 2 * NS * lanes_of(a.N); }
 
 // Pieces as long as there are blocks for them at once (`fill` fit the GPU), of at
-// least 8 spans each; one piece where two would not both fit.
+// least 8 spans each; one piece where fewer than three fit.
 Pieces pieces_of(const StateScan& a, int64_t fill) {
   Pieces p;
   const int64_t spans = (a.T + SPAN - 1) / SPAN, blocks = std::max<int64_t>(1, a.B * a.G * tiles_of(a));
   const int64_t most = std::min(fill / blocks, spans / 8);
-  p.spans = most >= 2 ? (spans + most - 1) / most : std::max<int64_t>(spans, 1);
+  p.spans = most >= 3 ? (spans + most - 1) / most : std::max<int64_t>(spans, 1);
   p.count = (int)((spans + p.spans - 1) / p.spans);
   if (p.count < 1) p.count = 1;
   return p;
