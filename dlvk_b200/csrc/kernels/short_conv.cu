@@ -26,7 +26,6 @@ constexpr int RUNS = 8;    // runs of a block, a warp each
 template <typename T, int V> struct Pack;  // V elements as loaded
 template <> struct Pack<float, 4> { using type = float4; };
 template <> struct Pack<float, 1> { using type = float; };
-template <> struct Pack<__nv_bfloat16, 8> { using type = uint4; };
 template <> struct Pack<__nv_bfloat16, 4> { using type = uint2; };
 template <> struct Pack<__nv_bfloat16, 1> { using type = __nv_bfloat16; };
 
@@ -135,7 +134,7 @@ struct FwdShared {
 };
 
 template <typename T, int V, int K>
-__global__ void __launch_bounds__(32 * RUNS, 2) conv_fwd_kernel(ShortConv a, SeqRef y, SeqRef out_state, Grid grid) {
+__global__ void __launch_bounds__(32 * RUNS, 3) conv_fwd_kernel(ShortConv a, SeqRef y, SeqRef out_state, Grid grid) {
   constexpr int AHEAD = FwdShared<T, V>::AHEAD;
   extern __shared__ __align__(16) char raw[];
   auto& sh = *reinterpret_cast<FwdShared<T, V>*>(raw);
@@ -333,12 +332,12 @@ bool aligned(const ShortConv& a, int v) {
          aligned(a.state, v, bytes);
 }
 
-// As many runs as there are warps on the GPU at once (two blocks an SM), each of
-// at least eight tokens: a run reads K - 1 tokens again, and the taps.
-Grid grid_of(const ShortConv& a, int v) {
+// As many runs as there are warps on the GPU at once, each of at least eight
+// tokens: a run reads K - 1 tokens again, and the taps.
+Grid grid_of(const ShortConv& a, int v, int blocks_an_sm) {
   Grid g;
   g.blocks = (a.D + 32 * v - 1) / (32 * v);
-  const int64_t fit = std::max<int64_t>(1, 148 * 2 * RUNS / std::max<int64_t>(1, a.B * g.blocks));
+  const int64_t fit = std::max<int64_t>(1, 148 * blocks_an_sm * RUNS / std::max<int64_t>(1, a.B * g.blocks));
   g.run = std::max<int64_t>(8, (a.T + fit - 1) / fit);
   g.runs = std::max<int64_t>(1, (a.T + g.run - 1) / g.run);
   g.rows = (a.B * g.runs + RUNS - 1) / RUNS;
@@ -352,7 +351,8 @@ void launch(Kernel kernel, size_t smem, const Grid& g, cudaStream_t s, Args... a
   kernel<<<(unsigned)(g.rows * g.blocks), dim3(32, RUNS), smem, s>>>(args..., g);
   DLVK_POST_LAUNCH();
 }
-constexpr int BWD_VEC = 4;  // the backward pass keeps K + 3 tokens of two tensors in registers
+constexpr int FWD_BLOCKS = 3, BWD_BLOCKS = 2;  // an SM holds; of bf16 too a thread has only four channels, and more registers
+constexpr int VEC = 4;
 
 template <typename F>
 void by_taps(int taps, F&& f) {
@@ -371,17 +371,16 @@ void short_conv_fwd(const ShortConv& a, SeqRef y, SeqRef out_state, cudaStream_t
   // without tokens there is a state to copy, or nothing to do
   if (a.B == 0 || a.D == 0 || (a.T == 0 && !out_state.p)) return;
   const int64_t bytes = a.dt == DType::BF16 ? 2 : 4;
-  const int v = 16 / (int)bytes;
-  const bool wide = aligned(a, v) && aligned(y, v, bytes) && aligned(out_state, v, bytes);
-  const Grid g = grid_of(a, wide ? v : 1);
+  const bool wide = aligned(a, VEC) && aligned(y, VEC, bytes) && aligned(out_state, VEC, bytes);
+  const Grid g = grid_of(a, wide ? VEC : 1, FWD_BLOCKS);
   by_taps(a.taps, [&](auto taps) {
     constexpr int K = decltype(taps)::value;
     using bf16 = __nv_bfloat16;
     if (a.dt == DType::BF16) {
-      if (wide) launch(conv_fwd_kernel<bf16, 8, K>, sizeof(FwdShared<bf16, 8>), g, s, a, y, out_state);
+      if (wide) launch(conv_fwd_kernel<bf16, VEC, K>, sizeof(FwdShared<bf16, VEC>), g, s, a, y, out_state);
       else launch(conv_fwd_kernel<bf16, 1, K>, sizeof(FwdShared<bf16, 1>), g, s, a, y, out_state);
     } else {
-      if (wide) launch(conv_fwd_kernel<float, 4, K>, sizeof(FwdShared<float, 4>), g, s, a, y, out_state);
+      if (wide) launch(conv_fwd_kernel<float, VEC, K>, sizeof(FwdShared<float, VEC>), g, s, a, y, out_state);
       else launch(conv_fwd_kernel<float, 1, K>, sizeof(FwdShared<float, 1>), g, s, a, y, out_state);
     }
   });
@@ -390,13 +389,13 @@ void short_conv_fwd(const ShortConv& a, SeqRef y, SeqRef out_state, cudaStream_t
 namespace {
 bool wide_bwd(const ShortConv& a, const SeqRef& dy, const SeqRef& dx) {
   const int64_t bytes = a.dt == DType::BF16 ? 2 : 4;
-  return aligned(a, BWD_VEC) && aligned(dy, BWD_VEC, bytes) && aligned(dx, BWD_VEC, bytes);
+  return aligned(a, VEC) && aligned(dy, VEC, bytes) && aligned(dx, VEC, bytes);
 }
 }  // namespace
 
 // The larger of the two ways to divide the channels.
 int64_t short_conv_part_floats(const ShortConv& a) {
-  return std::max(grid_of(a, BWD_VEC).rows, grid_of(a, 1).rows) * (a.taps + 1) * a.D;
+  return std::max(grid_of(a, VEC, BWD_BLOCKS).rows, grid_of(a, 1, BWD_BLOCKS).rows) * (a.taps + 1) * a.D;
 }
 
 void short_conv_bwd(const ShortConv& a, SeqRef dy, SeqRef dx, float* dweight, float* dbias, bool accumulate, float* part,
@@ -406,16 +405,16 @@ void short_conv_bwd(const ShortConv& a, SeqRef dy, SeqRef dx, float* dweight, fl
   int64_t rows = 0;
   if (a.B > 0 && a.T > 0) {
     const bool wide = wide_bwd(a, dy, dx);
-    const Grid g = grid_of(a, wide ? BWD_VEC : 1);
+    const Grid g = grid_of(a, wide ? VEC : 1, BWD_BLOCKS);
     rows = g.rows;
     by_taps(a.taps, [&](auto taps) {
-      constexpr int K = decltype(taps)::value, W = BWD_VEC;
+      constexpr int K = decltype(taps)::value;
       using bf16 = __nv_bfloat16;
       if (a.dt == DType::BF16) {
-        if (wide) launch(conv_bwd_kernel<bf16, W, K>, sizeof(BwdShared<bf16, W>), g, s, a, dy, dx, part);
+        if (wide) launch(conv_bwd_kernel<bf16, VEC, K>, sizeof(BwdShared<bf16, VEC>), g, s, a, dy, dx, part);
         else launch(conv_bwd_kernel<bf16, 1, K>, sizeof(BwdShared<bf16, 1>), g, s, a, dy, dx, part);
       } else {
-        if (wide) launch(conv_bwd_kernel<float, W, K>, sizeof(BwdShared<float, W>), g, s, a, dy, dx, part);
+        if (wide) launch(conv_bwd_kernel<float, VEC, K>, sizeof(BwdShared<float, VEC>), g, s, a, dy, dx, part);
         else launch(conv_bwd_kernel<float, 1, K>, sizeof(BwdShared<float, 1>), g, s, a, dy, dx, part);
       }
     });
