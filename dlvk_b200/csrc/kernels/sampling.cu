@@ -14,12 +14,15 @@
 //
 // A row is read once, into the shared memory of a cluster of up to eight blocks
 // that pass sums to each other.  Where the cut lies among the first thousand or
-// so, it is found in a list: the n-th largest of the threads' largest elements is
-// a bound that at least n elements reach, those that do are sorted by one block.
-// Otherwise histograms narrow the range down to as few elements.
+// so, one block finds it and the word in a list: what the n-th largest of
+// the threads' largest elements reaches, at least n elements do, and those that
+// do are the list.  Otherwise histograms of the elements' numbers narrow the
+// range down to as few: a bin's weights lie between those of its ends, which
+// brackets the cut, so that sums are made in registers and not in the bins.
 #include <cooperative_groups.h>
 
 #include <algorithm>
+#include <cstddef>
 
 #include "dlvk/common.h"
 #include "dlvk/kernels.h"
@@ -31,9 +34,12 @@ namespace {
 
 constexpr int THREADS = 512, WARPS = THREADS / 32;
 constexpr int MOST_BLOCKS = 8;     // of a cluster
-constexpr int LIST = 2048;         // elements that one block sorts
-constexpr int NUCLEUS = 512;       // elements of a list for top_p alone
-constexpr int BINS = 2048;
+constexpr int LIST = 3 * THREADS;  // elements that one block cuts by itself
+constexpr int ASK = 1152;          // most elements that a list is made for: it may have some more
+constexpr int SHORT = 128;         // elements of a list that all see all
+constexpr int NUCLEUS = 96, NUCLEUS_MORE = 900;  // elements of a list for top_p alone, first and second try
+constexpr int BINS = 2048;         // that a range of elements is cut into
+constexpr int PARTS = 1024;        // where they hold exact weights
 constexpr double ONE = 17592186044416.0;  // 2^44
 using u64 = unsigned long long;
 
@@ -47,25 +53,47 @@ __device__ __forceinline__ float value_of(uint32_t key) {
   return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key);
 }
 
+struct Settings {
+  int64_t top_k;
+  double top_p;
+  u64 least;      // smallest weight that min_p lets stand
+  double uniform;
+  bool cut_k, cut_p;
+};
+// What the functions below work on lies in shared memory, the row's keys behind
+// it: arguments of functions that are not inlined would pass through local memory,
+// which the row's loads push out of the first cache.
 struct Shared {
-  double powers[128];                   // 2^(i / 128)
-  u64 best[MOST_BLOCKS];                // of each block: its largest element
-  u64 sums[MOST_BLOCKS];                // and its sum of weights
-  unsigned listed[MOST_BLOCKS];         // and its elements in the list
+  Settings set;
+  float top;                               // the largest logit
+  double scale;                            // 128 / (ln 2 temperature)
+  int blocks, rank, first, n;              // the cluster; this block's words: first.., n of them
+  double powers[128];                      // 2^(i / 128)
+  u64 best[MOST_BLOCKS];                   // of each block: its largest element,
+  u64 sums[MOST_BLOCKS];                   // a sum of weights,
+  u64 lowest[MOST_BLOCKS], highest[MOST_BLOCKS];  // its elements' ends in a range
   uint32_t maxima[MOST_BLOCKS * THREADS];  // block 0: every thread's largest key
-  u64 scan[WARPS];
-  unsigned count[33];
-  unsigned members;
-  u64 lowest, highest;
-  u64 found[3];
+  u64 scan[WARPS], scan2[2 * WARPS];
+  unsigned count[8];
+  unsigned members;                        // block 0: elements of the list
+  u64 told[6];                             // by block 0, by Told
   union {
-    u64 list[LIST];
     struct {
-      u64 mass[BINS];
-      unsigned amount[BINS];
+      u64 list[LIST], weights[LIST];
+    };
+    struct {
+      alignas(16) unsigned amount[BINS];  // read by fours
+      unsigned mass[3][PARTS];
     } bins;
   };
 };
+static_assert(offsetof(Shared, bins.amount) % 16 == 0 && sizeof(Shared) % 16 == 0, "");
+
+enum Told { BOUND, IN_LIST, FIRST_BIN, LAST_BIN, IN_BINS, CUT };
+
+extern __shared__ __align__(16) char raw_shared[];
+__device__ __forceinline__ Shared& shared() { return *reinterpret_cast<Shared*>(raw_shared); }
+__device__ __forceinline__ uint32_t* row_keys() { return reinterpret_cast<uint32_t*>(raw_shared + sizeof(Shared)); }
 
 // exp(d), d <= 0, in steps of 2^-44, with the table of 2^(i/128) and the
 // exponential's series to the fourth power (P. T. P. Tang, "Table-driven
@@ -95,11 +123,16 @@ __device__ __forceinline__ u64 warp_add(u64 v) {
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
 }
-// Sum over the block, and the sum of the threads before this one.
-__device__ u64 block_scan(u64 v, u64& before, Shared& sh) {
+
+// The sum of the threads before this one, and that of the block.
+struct Scan {
+  u64 before, total;
+};
+__device__ __forceinline__ Scan block_scan(u64 v) {
+  Shared& sh = shared();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   u64 s = v;
-#pragma unroll
+#pragma unroll 1
   for (int o = 1; o < 32; o <<= 1) {
     const u64 t = __shfl_up_sync(0xffffffffu, s, o);
     if (lane >= o) s += t;
@@ -107,264 +140,418 @@ __device__ u64 block_scan(u64 v, u64& before, Shared& sh) {
   __syncthreads();
   if (lane == 31) sh.scan[warp] = s;
   __syncthreads();
-  u64 base = 0, total = 0;
-#pragma unroll
-  for (int w = 0; w < WARPS; ++w) {
-    if (w < warp) base += sh.scan[w];
-    total += sh.scan[w];
+  u64 w = lane < WARPS ? sh.scan[lane] : 0;
+#pragma unroll 1
+  for (int o = 1; o < WARPS; o <<= 1) {
+    const u64 t = __shfl_up_sync(0xffffffffu, w, o);
+    if (lane >= o) w += t;
   }
-  before = base + s - v;
-  return total;
+  const u64 base = __shfl_sync(0xffffffffu, w, warp ? warp - 1 : 0);
+  return {(warp ? base : 0) + s - v, __shfl_sync(0xffffffffu, w, WARPS - 1)};
 }
 
-// The n-th largest of `count` keys (all, where there are no more), up to its last 12 bits.
-__device__ uint32_t nth_largest(const uint32_t* keys, int count, int n, Shared& sh) {
+// A weight into a bin, in three numbers of 15 bits each: additions of 64 bits to
+// shared memory are loops, and equal logits meet in them.  2^17 weights fit.
+__device__ __forceinline__ void add_mass(unsigned (*mass)[PARTS], int bin, u64 w) {
+  atomicAdd(&mass[0][bin], (unsigned)w & 0x7fffu);
+  atomicAdd(&mass[1][bin], (unsigned)(w >> 15) & 0x7fffu);
+  atomicAdd(&mass[2][bin], (unsigned)(w >> 30));
+}
+__device__ __forceinline__ u64 mass_of(const unsigned (*mass)[PARTS], int bin) {
+  return mass[0][bin] + ((u64)mass[1][bin] << 15) + ((u64)mass[2][bin] << 30);
+}
+
+// A bound that at least n of the first `count` maxima reach, and few more: the
+// smallest of those whose distances from `top`, in 64 bins an octave, lie in the
+// n-th largest's bin or above.  0 where fewer than n are no zeros.
+__device__ __forceinline__ uint32_t bound_of(int count, int n) {
+  Shared& sh = shared();
+  const float top = sh.top;
+  const uint32_t* keys = sh.maxima;
+  const auto bin_of = [&](uint32_t k) {
+    const int b = (int)(__float_as_uint(top - value_of(k)) >> 17) - ((127 - 12) << 6);
+    return max(0, min(b, BINS - 1));  // (the largest of infinities: infinity - infinity is not a number, and far)
+  };
   uint32_t mine[MOST_BLOCKS];
 #pragma unroll
   for (int i = 0; i < MOST_BLOCKS; ++i) mine[i] = i * THREADS + threadIdx.x < count ? keys[i * THREADS + threadIdx.x] : 0;
-  if (threadIdx.x < 33) sh.count[threadIdx.x] = 0;
+  for (int i = threadIdx.x; i < BINS; i += THREADS) sh.bins.amount[i] = 0;
+  if (threadIdx.x == 0) sh.count[0] = BINS, sh.count[1] = 0xffffffffu;
   __syncthreads();
-  uint32_t bound = 0;
-  for (int bit = 31; bit >= 12; --bit) {
-    const uint32_t trial = bound | 1u << bit;
-    unsigned c = 0;
 #pragma unroll
-    for (int i = 0; i < MOST_BLOCKS; ++i) c += mine[i] >= trial;
-    c = __reduce_add_sync(0xffffffffu, c);
-    if ((threadIdx.x & 31) == 0 && c) atomicAdd(&sh.count[bit], c);
-    __syncthreads();
-    if (sh.count[bit] >= (unsigned)n) bound = trial;
-  }
-  return bound;
-}
-
-// Descending order of sh.list[0, n); n <= LIST.
-__device__ void sort_list(int n, Shared& sh) {
-  int size = 32;
-  while (size < n) size <<= 1;
-  for (int i = n + threadIdx.x; i < size; i += THREADS) sh.list[i] = 0;
+  for (int i = 0; i < MOST_BLOCKS; ++i)
+    if (mine[i]) atomicAdd(&sh.bins.amount[bin_of(mine[i])], 1u);
   __syncthreads();
-  for (int k = 2; k <= size; k <<= 1)
-    for (int j = k >> 1; j > 0; j >>= 1) {
-      for (int i = threadIdx.x; i < size / 2; i += THREADS) {
-        const int a = (i / j) * 2 * j + i % j, b = a + j;
-        const u64 x = sh.list[a], y = sh.list[b];
-        if ((x < y) == ((a & k) == 0)) sh.list[a] = y, sh.list[b] = x;
-      }
-      __syncthreads();
-    }
+  constexpr int PER = BINS / THREADS;
+  const uint4 a = *reinterpret_cast<const uint4*>(&sh.bins.amount[threadIdx.x * PER]);
+  static_assert(PER == 4, "");
+  const u64 upto = block_scan(a.x + a.y + a.z + a.w).before;
+  int first = BINS;
+#pragma unroll
+  for (int k = PER - 1; k >= 0; --k) {
+    u64 sum = upto;
+#pragma unroll
+    for (int j = 0; j <= k; ++j) sum += (&a.x)[j];
+    if (sum >= (u64)n) first = threadIdx.x * PER + k;
+  }
+  const unsigned lowest = __reduce_min_sync(0xffffffffu, first);
+  if ((threadIdx.x & 31) == 0) atomicMin(&sh.count[0], lowest);
+  __syncthreads();
+  const int bin = sh.count[0];
+  uint32_t bound = 0xffffffffu;
+#pragma unroll
+  for (int i = 0; i < MOST_BLOCKS; ++i)
+    if (mine[i] && bin_of(mine[i]) <= bin) bound = min(bound, mine[i]);
+  bound = __reduce_min_sync(0xffffffffu, bound);
+  if ((threadIdx.x & 31) == 0) atomicMin(&sh.count[1], bound);
+  __syncthreads();
+  return bin < BINS ? sh.count[1] : 0;
 }
 
-// One row's elements, dealt out to the blocks of a cluster in runs of `run` words.
+// The last element, in descending order, with less than `want` before it, of
+// `count` in sh.list, all above lo and none above hi.  What comes before is
+// counted, or weighed by sh.weights (BY_WORD: of the elements' lower halves alone,
+// whose descending order is the words' ascending one).  The range is cut into 1024
+// parts until the one that holds it has no other element: two or three rounds of
+// some 1500 cycles, where a bisection takes 50 of a thousand.
+enum Order { COUNTED, WEIGHED, BY_WORD };
+__device__ __forceinline__ u64 last_below(int count, u64 lo, u64 hi, u64 want, Order order) {
+  Shared& sh = shared();
+  constexpr int PER = LIST / THREADS;
+  static_assert(PARTS == 2 * THREADS && 4 * PARTS * sizeof(unsigned) <= sizeof(sh.maxima), "");
+  unsigned(*mass)[PARTS] = reinterpret_cast<unsigned(*)[PARTS]>(sh.maxima);  // no longer needed
+  unsigned* amount = mass[3];
+  u64 e[PER], w[PER], acc = 0;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const int at = i * THREADS + threadIdx.x;
+    e[i] = at < count ? sh.list[at] : 0;
+    if (order == BY_WORD) e[i] &= 0xffffffffull;
+    w[i] = at >= count || order == COUNTED ? 0 : sh.weights[at];
+    if (at >= count) e[i] = 0;
+  }
+#pragma unroll 1
+  while (true) {
+    const int shift = max(0, 64 - __clzll(hi - lo - 1) - 10);
+#pragma unroll
+    for (int i = threadIdx.x; i < 4 * PARTS; i += THREADS) mass[0][i] = 0;
+    if (threadIdx.x == 0) sh.scan2[0] = 0;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+      if (e[i] > lo && e[i] <= hi) {
+        const int part = (int)((hi - e[i]) >> shift);
+        atomicAdd(&amount[part], 1u);
+        if (order != COUNTED) add_mass(mass, part, w[i]);
+      }
+    __syncthreads();
+    const int mine = 2 * threadIdx.x;
+    const u64 first = order == COUNTED ? amount[mine] : mass_of(mass, mine),
+              second = order == COUNTED ? amount[mine + 1] : mass_of(mass, mine + 1);
+    const u64 before = acc + block_scan(first + second).before;
+    const bool in0 = amount[mine] && before < want, in1 = amount[mine + 1] && before + first < want;
+    if (in0 || in1) atomicMax(&sh.scan2[0], (u64)(in1 ? mine + 1 : mine) + 1);
+    __syncthreads();
+    const int part = (int)sh.scan2[0] - 1;
+    if (part >> 1 == threadIdx.x) sh.scan2[1] = part & 1 ? before + first : before;
+    __syncthreads();
+    if (part < 0) return hi;  // not reached: the first element has nothing before it
+    acc = sh.scan2[1];
+    hi -= (u64)part << shift;
+    if (shift < 64) lo = max(lo, hi - min(hi, (u64)1 << shift));
+    if (amount[part] == 1 || shift == 0) {
+#pragma unroll
+      for (int i = 0; i < PER; ++i)
+        if (e[i] > lo && e[i] <= hi) sh.scan2[2] = e[i];
+      __syncthreads();
+      return sh.scan2[2];
+    }
+    __syncthreads();
+  }
+}
+
+// The whole number that a sum is below where it is below top_p total.
+__device__ __forceinline__ u64 wanted(double top_p, u64 total) {
+  const double w = top_p > 0 ? ceil(top_p * (double)total) : 1.0;
+  return w >= 1.0 ? (u64)w : 1;
+}
+// Running sums above uniform total are above this.
+__device__ __forceinline__ u64 passed(double uniform, u64 total) {
+  const u64 want = uniform > 0 ? (u64)(fmin(uniform, 1.0) * (double)total) : 0;
+  return want < total ? want : total - 1;
+}
+
+// The word, from a list of `count` elements that begins the descending order and
+// holds the cut.  total: the weights of all words (top_p alone).  A row runs this
+// once, so most of its time is the fetching of its instructions: loops are short
+// and not unrolled (a sort in unrolled steps: 122000 cycles for 40 elements where
+// these loops take some thousands).
+//
+// Short lists: four threads an element add up what is larger.
+__device__ __forceinline__ void word_of_short_list(int count, u64 total, int32_t* token) {
+  Shared& sh = shared();
+  const Settings& set = sh.set;
+  u64* weights = sh.weights;
+  __syncthreads();
+  if (threadIdx.x < count) weights[threadIdx.x] = Weights{sh.top, sh.scale, sh.powers}((uint32_t)(sh.list[threadIdx.x] >> 32));
+  __syncthreads();
+  const int me = threadIdx.x / 4, part = threadIdx.x % 4;
+  const u64 e = me < count ? sh.list[me] : 0, w = me < count ? weights[me] : 0;
+  const auto add_parts = [](u64 v) {
+    v += __shfl_xor_sync(0xffffffffu, v, 1);
+    return v + __shfl_xor_sync(0xffffffffu, v, 2);
+  };
+  u64 before = 0, rank = 0;
+#pragma unroll 1
+  for (int j = part; j < count; j += 4)
+    if (sh.list[j] > e) before += weights[j], ++rank;
+  before = add_parts(before);
+  rank = add_parts(rank);
+  if (set.cut_k && me < count && rank + 1 == (u64)set.top_k) sh.scan2[0] = before + w;  // of the first top_k
+  __syncthreads();
+  if (set.cut_k) total = sh.scan2[0];
+  const bool keep = me < count && (!set.cut_k || rank < (u64)set.top_k) && (!set.cut_p || before < wanted(set.top_p, total)) &&
+                    w >= set.least;
+  if (part == 0 && me < count && !keep) weights[me] = 0;
+  __syncthreads();
+  u64 upto = 0, all = 0;
+#pragma unroll 1
+  for (int j = part; j < count; j += 4) {
+    all += weights[j];
+    if ((uint32_t)sh.list[j] > (uint32_t)e) upto += weights[j];  // words with smaller numbers
+  }
+  upto = add_parts(upto);
+  all = add_parts(all);
+  const u64 want = passed(set.uniform, all);
+  if (keep && part == 0 && upto <= want && want < upto + w) *token = (int32_t)~(uint32_t)e;
+}
+__device__ __forceinline__ void word_of_list(int count, u64 total, u64 lo, u64 hi, int words, int32_t* token) {
+  Shared& sh = shared();
+  const Settings& set = sh.set;
+  u64 cut = 0;
+#pragma unroll 1
+  for (int stage = set.cut_k ? COUNTED : WEIGHED; stage <= BY_WORD; ++stage) {
+    u64 want = (u64)set.top_k, from = lo, to = hi;
+    if (stage != COUNTED) {
+      const Weights weight{sh.top, sh.scale, sh.powers};
+      u64 mine = 0;
+#pragma unroll 1
+      for (int i = threadIdx.x; i < count; i += THREADS) {
+        const u64 e = sh.list[i], w = e >= cut ? weight((uint32_t)(e >> 32)) : 0;
+        mine += sh.weights[i] = stage == BY_WORD && w < set.least ? 0 : w;
+      }
+      const u64 sum = block_scan(mine).total;
+      if (stage == WEIGHED) {
+        if (!set.cut_p) continue;
+        want = wanted(set.top_p, set.cut_k ? sum : total);
+      } else {  // the last word, in ascending order, with no more than this before it
+        want = passed(set.uniform, sum) + 1;
+        from = ~(uint32_t)words, to = ~0u;
+      }
+    }
+    cut = last_below(count, from, to, want, (Order)stage);
+  }
+  if (threadIdx.x == 0) *token = (int32_t)~(uint32_t)cut;
+}
+
+// One row's elements, dealt out to the blocks of a cluster in runs of words.
 struct Row {
-  cg::cluster_group cluster;
-  int blocks, rank, first, n;  // this block's words: first.., n of them
-  const uint32_t* keys;
-  Weights weight;
   Shared& sh;
+  uint32_t* keys;
+  int blocks, rank, first, n;
+  Weights weight;
+  __device__ __forceinline__ Row()
+      : sh(shared()), keys(row_keys()), blocks(sh.blocks), rank(sh.rank), first(sh.first), n(sh.n),
+        weight{sh.top, sh.scale, sh.powers} {}
+  __device__ __forceinline__ static cg::cluster_group cluster() { return cg::this_cluster(); }
   __device__ __forceinline__ u64 element(int i) const { return (u64)keys[i] << 32 | ~(uint32_t)(first + i); }
 
-  // Everything for the whole cluster to see; ends with a barrier of all.
-  __device__ u64 total_weight(u64 cut, u64 least) {
-    u64 s = 0, before;
-    for (int i = threadIdx.x; i < n; i += THREADS)
-      if (element(i) >= cut) {
-        const u64 w = weight(keys[i]);
-        if (w >= least) s += w;
-      }
-    s = block_scan(s, before, sh);
-    if (threadIdx.x < blocks) *cluster.map_shared_rank(&sh.sums[rank], threadIdx.x) = s;
-    cluster.sync();
-    s = 0;
+  // A number of each block to all; ends with a barrier of all.
+  __device__ __forceinline__ u64 add_up(u64 mine) {
+    if (threadIdx.x < blocks) *cluster().map_shared_rank(&sh.sums[rank], threadIdx.x) = mine;
+    cluster().sync();
+    u64 s = 0;
     for (int b = 0; b < blocks; ++b) s += sh.sums[b];
     return s;
   }
-
-  // Lists the elements that `member` picks, at most LIST of a block; their number,
-  // smallest and largest in sh.members, sh.lowest, sh.highest.
-  template <typename F>
-  __device__ void gather(F&& member) {
-    __syncthreads();
-    if (threadIdx.x == 0) sh.members = 0, sh.lowest = ~0ull, sh.highest = 0;
-    __syncthreads();
-    const int lane = threadIdx.x & 31;
-    u64 lo = ~0ull, hi = 0;
-    for (int i0 = threadIdx.x & ~31; i0 < n; i0 += THREADS) {
-      const int i = i0 + lane;
-      const bool in = i < n && member(i);
-      const unsigned who = __ballot_sync(0xffffffffu, in);
-      if (!who) continue;
-      unsigned base = 0;
-      if (lane == 0) base = atomicAdd(&sh.members, __popc(who));
-      base = __shfl_sync(0xffffffffu, base, 0);
-      if (in) {
-        const u64 e = element(i);
-        const unsigned at = base + __popc(who & ((1u << lane) - 1));
-        if (at < LIST) sh.list[at] = e;
-        lo = e < lo ? e : lo;
-        hi = e > hi ? e : hi;
-      }
-    }
-    if (hi) {
-      atomicMin(&sh.lowest, lo);
-      atomicMax(&sh.highest, hi);
-    }
-    __syncthreads();
+  // The weights of the elements from `cut` on, of the whole row.
+  __device__ __forceinline__ u64 total_weight(u64 cut) {
+    u64 s = 0;
+#pragma unroll 4
+    for (int i = threadIdx.x; i < n; i += THREADS)
+      if (element(i) >= cut) s += weight(keys[i]);
+    return add_up(block_scan(s).total);
+  }
+  // Block 0's number to all, to be read behind the next barrier of the cluster.
+  // A kind of number has a place of its own: a thread may read it as late as
+  // before the barrier after that, when block 0 is at its next number already.
+  __device__ __forceinline__ void tell(int place, u64 v) {
+    if (rank == 0 && threadIdx.x < blocks) cluster().map_shared_rank(sh.told, threadIdx.x)[place] = v;
+  }
+  // Elements to block 0's list (its length counts those that found no room).
+  __device__ __forceinline__ void list(u64 e) {
+    Shared* to = cluster().map_shared_rank(&sh, 0);
+    const unsigned at = atomicAdd(&to->members, 1u);
+    if (at < LIST) to->list[at] = e;
   }
 
-  // Block 0: the lists of all blocks one after the other; their length, or -1 where there is no room.
-  __device__ int join_lists() {
-    int total = 0;
-    for (int b = 0; b < blocks; ++b) total += sh.listed[b];
-    if (total > LIST) return -1;
-    int at = sh.listed[0];
-    for (int b = 1; b < blocks; ++b) {
-      const u64* from = cluster.map_shared_rank(sh.list, b);
-      for (int i = threadIdx.x; i < (int)sh.listed[b]; i += THREADS) sh.list[at + i] = from[i];
-      at += sh.listed[b];
-    }
-    return total;
-  }
-
-  // Block 0, list sorted, `acc` the amount before its first element: the last
-  // element with less than `want` before it, and in sh.found[1] whether the
-  // list's amounts reach `want`.  by_count: amounts are 1, else weights; only the
-  // first `most` elements are looked at.
-  __device__ u64 cut_of_list(int total, int most, u64 acc, u64 want, bool by_count) {
-    const int per = (min(total, most) + THREADS - 1) / THREADS;
-    const int lo = min(min(total, most), (int)threadIdx.x * per), hi = min(min(total, most), lo + per);
-    u64 mine = 0, before;
-    for (int i = lo; i < hi; ++i) mine += by_count ? 1 : weight((uint32_t)(sh.list[i] >> 32));
-    const u64 sum = block_scan(mine, before, sh);
-    if (threadIdx.x == 0) sh.found[0] = 0;
-    __syncthreads();
-    u64 upto = acc + before;
-    int last = -1;
-    for (int i = lo; i < hi && upto < want; ++i) {
-      last = i;
-      upto += by_count ? 1 : weight((uint32_t)(sh.list[i] >> 32));
-    }
-    if (last >= 0) atomicMax(&sh.found[0], (u64)last + 1);
-    if (threadIdx.x == 0) sh.found[1] = acc + sum >= want;
-    __syncthreads();
-    return sh.found[0] ? sh.list[sh.found[0] - 1] : ~0ull;
-  }
-
-  // The sum of the weights of the first `most` elements of the list.
-  __device__ u64 weight_of_list(int most) {
-    u64 s = 0, before;
-    for (int i = threadIdx.x; i < most; i += THREADS) s += weight((uint32_t)(sh.list[i] >> 32));
-    return block_scan(s, before, sh);
-  }
-
-  // sh.found[..] of block 0 to all; ends with a barrier of all.
-  __device__ void tell(u64 a, u64 b, u64 c) {
-    if (rank == 0 && threadIdx.x < blocks) {
-      u64* to = cluster.map_shared_rank(sh.found, threadIdx.x);
-      to[0] = a, to[1] = b, to[2] = c;
-    }
-    cluster.sync();
-  }
-
-  // The cut where less than `want` comes before its element, wherever it lies:
-  // the range of elements is narrowed down by histograms, first over the logit's
-  // distance from the largest, then over the elements as numbers.
-  __device__ u64 search(u64 want, bool by_count, float per_unit) {
-    u64 acc = 0, lowest = 0, highest = ~0ull;
-    int shift = -1;  // -1: by distance
+  // The last element with less than `want` before it (by_count: elements, else
+  // weights), wherever it lies.  Histograms narrow the range of elements down,
+  // first over the logit's distance from the largest, then over the elements as
+  // numbers, until the elements that may be it fit a list.  The first two rounds
+  // bracket it by the weights of the bins' ends; where that leaves too many (very
+  // small weights, many equal ones) they hold their exact weights, and each round
+  // leaves one of 2^10 parts of the numbers.
+  __device__ __forceinline__ u64 search(u64 want, bool by_count, float per_unit) {
+    u64 acc = 0, lowest = 0, highest = ~0ull;  // acc: amount above `highest`
+    int shift = -1;                            // -1: by distance
+    bool exact = by_count;
     const auto bin_of = [&](int i) {
       if (shift >= 0) return (int)((highest - element(i)) >> shift);
       const float x = value_of(keys[i]), q = (weight.top - x) * per_unit;
       return x == weight.top ? 0 : q < BINS - 1 ? (int)q : BINS - 1;
     };
-    while (true) {
-      cluster.sync();  // the lists and bins of before have been read
-      for (int i = threadIdx.x; i < BINS; i += THREADS) sh.bins.mass[i] = 0, sh.bins.amount[i] = 0;
+    for (int round = 0; round < 10; ++round) {  // 2, and 10 of 64 bits in each of at most 7 more
+      exact = by_count || round >= 2;
+      cluster().sync();  // the list and bins of before have been read
+      for (int i = threadIdx.x; i < BINS; i += THREADS) sh.bins.amount[i] = 0;
+      if (exact) for (int i = threadIdx.x; i < 3 * PARTS; i += THREADS) sh.bins.mass[0][i] = 0;
       __syncthreads();
       for (int i = threadIdx.x; i < n; i += THREADS) {
         const u64 e = element(i);
         if (e < lowest || e > highest) continue;
         const int b = bin_of(i);
-        atomicAdd(&sh.bins.amount[b], 1u);
-        if (!by_count) {
-          const u64 w = weight(keys[i]);
-          if (w) atomicAdd(&sh.bins.mass[b], w);
-        }
+        // words that weigh nothing are no cut of weights
+        if (shift >= 0 || by_count || b < BINS - 1) atomicAdd(&sh.bins.amount[b], 1u);
+        if (exact && !by_count) add_mass(sh.bins.mass, b, weight(keys[i]));
       }
-      cluster.sync();
+      cluster().sync();
       if (rank == 0) {
         constexpr int PER = BINS / THREADS;
-        u64 mass[PER], mine = 0, before;
+        u64 low[PER], high[PER], lows = 0, highs = 0, low_before, high_before;
         unsigned amount[PER];
+        static_assert(PER == 4, "");
+        uint4 a[MOST_BLOCKS];
+#pragma unroll
+        for (int b = 0; b < MOST_BLOCKS; ++b)  // all blocks' loads at once
+          a[b] = b < blocks ? *reinterpret_cast<const uint4*>(&cluster().map_shared_rank(sh.bins.amount, b)[threadIdx.x * PER])
+                            : make_uint4(0, 0, 0, 0);
 #pragma unroll
         for (int k = 0; k < PER; ++k) {
-          mass[k] = 0, amount[k] = 0;
           const int i = threadIdx.x * PER + k;
-          for (int b = 0; b < blocks; ++b) {
-            amount[k] += cluster.map_shared_rank(sh.bins.amount, b)[i];
-            if (!by_count) mass[k] += cluster.map_shared_rank(sh.bins.mass, b)[i];
+          amount[k] = 0;
+#pragma unroll
+          for (int b = 0; b < MOST_BLOCKS; ++b) amount[k] += (&a[b].x)[k];
+          low[k] = high[k] = amount[k];
+          if (!by_count && exact) {
+            low[k] = 0;
+            if (i < PARTS)
+              for (int b = 0; b < blocks; ++b) low[k] += mass_of(cluster().map_shared_rank(sh.bins.mass, b), i);
+            high[k] = low[k];
+          } else if (!by_count && amount[k]) {
+            // the weights of a bin's ends, a step (of 2^-44) or 2^-12 of a bin's width to the safe side
+            u64 most, least;
+            if (shift >= 0) {
+              const u64 top = highest - ((u64)i << shift), bottom = top - (((u64)1 << shift) - 1);
+              most = weight((uint32_t)(top >> 32)) + 1;
+              least = weight((uint32_t)((bottom > top ? 0 : bottom) >> 32));
+            } else {
+              const double unit = weight.scale * 0.0054152123481245727 / (double)per_unit;  // a bin's width, in e-folds
+              const bool known = unit >= 0;  // not where the temperature is infinite
+              most = known ? (u64)(ONE * exp(-(i - 1.0 / 4096) * unit)) + 1 : (u64)ONE;
+              least = known ? (u64)(ONE * exp(-(i + 1 + 1.0 / 4096) * unit)) : 0;
+            }
+            low[k] = amount[k] * (least ? least - 1 : 0);
+            high[k] = amount[k] * min(most, (u64)ONE);
           }
-          if (by_count) mass[k] = amount[k];
-          mine += mass[k];
+          lows += low[k], highs += high[k];
         }
-        block_scan(mine, before, sh);
-        if (threadIdx.x == 0) sh.lowest = 0;
+        low_before = block_scan(lows).before;
+        high_before = block_scan(highs).before;
+        if (threadIdx.x == 0) sh.scan2[0] = ~0ull, sh.scan2[1] = 0, sh.scan2[2] = 0, sh.count[0] = 0, sh.members = 0;
         __syncthreads();
-        u64 upto = acc + before;
-        int last = -1;
-        u64 at = 0;
+        low_before += acc, high_before += acc;
 #pragma unroll
         for (int k = 0; k < PER; ++k) {
-          if (amount[k] && upto < want) last = threadIdx.x * PER + k, at = upto;
-          upto += mass[k];
+          const u64 i = threadIdx.x * PER + k;
+          if (amount[k]) {
+            atomicMax(&sh.scan2[2], i);                                          // the last bin of all
+            if (high_before + high[k] >= want) atomicMin(&sh.scan2[0], i);      // the first that the cut may lie in
+            if (low_before < want) atomicMax(&sh.scan2[1], i);                   // the last
+          }
+          low_before += low[k], high_before += high[k];
         }
-        if (last >= 0) atomicMax(&sh.lowest, (u64)last + 1);
         __syncthreads();
-        if (last >= 0 && sh.lowest == (u64)last + 1) sh.highest = at;
+        unsigned in = 0;
+#pragma unroll
+        for (int k = 0; k < PER; ++k) {
+          const u64 i = threadIdx.x * PER + k;
+          if (i >= min(sh.scan2[0], sh.scan2[2]) && i <= sh.scan2[1]) in += amount[k];
+        }
+        in = __reduce_add_sync(0xffffffffu, in);
+        if ((threadIdx.x & 31) == 0 && in) atomicAdd(&sh.count[0], in);
         __syncthreads();
       }
-      tell(sh.lowest - 1, sh.highest, 0);
-      const int pick = (int)sh.found[0];
-      acc = sh.found[1];
-      __syncthreads();
+      tell(FIRST_BIN, min(sh.scan2[0], sh.scan2[2]));
+      tell(LAST_BIN, sh.scan2[1]);
+      tell(IN_BINS, sh.count[0]);
+      cluster().sync();
+      const int from = (int)sh.told[FIRST_BIN], to = (int)sh.told[LAST_BIN];
+      const bool fits = sh.told[IN_BINS] <= LIST;
       const u64 lo = lowest, hi = highest;
-      gather([&](int i) {
+      u64 above = 0, least = ~0ull, most = 0;
+      for (int i = threadIdx.x; i < n; i += THREADS) {
         const u64 e = element(i);
-        return e >= lo && e <= hi && bin_of(i) == pick;
-      });
+        if (e < lo || e > hi) continue;
+        const int b = bin_of(i);
+        if (b < from) above += by_count ? 1 : weight(keys[i]);
+        if (b < from || b > to) continue;
+        least = min(least, e), most = max(most, e);
+        if (fits) list(e);
+      }
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) {
+        least = min(least, __shfl_xor_sync(0xffffffffu, least, o));
+        most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
+      }
+      if ((threadIdx.x & 31) == 0) sh.scan2[threadIdx.x >> 5] = least;
+      __syncthreads();
+      for (int w = 0; w < WARPS; ++w) least = min(least, sh.scan2[w]);
+      __syncthreads();
+      if ((threadIdx.x & 31) == 0) sh.scan2[threadIdx.x >> 5] = most;
+      __syncthreads();
+      for (int w = 0; w < WARPS; ++w) most = max(most, sh.scan2[w]);
       if (threadIdx.x < blocks) {
-        Shared* to = cluster.map_shared_rank(&sh, threadIdx.x);
-        to->listed[rank] = sh.members;
-        to->best[rank] = sh.lowest;
-        to->sums[rank] = sh.highest;
+        Shared* there = cluster().map_shared_rank(&sh, threadIdx.x);
+        there->lowest[rank] = least, there->highest[rank] = most;
       }
-      cluster.sync();
-      unsigned total = 0;
+      acc += add_up(block_scan(above).total);
       lowest = ~0ull, highest = 0;
-      for (int b = 0; b < blocks; ++b) {
-        total += sh.listed[b];
-        lowest = min(lowest, sh.best[b]);
-        highest = max(highest, sh.sums[b]);
-      }
-      if (total <= LIST) {
+      for (int b = 0; b < blocks; ++b) lowest = min(lowest, sh.lowest[b]), highest = max(highest, sh.highest[b]);
+      if (fits) {
         u64 cut = 0;
         if (rank == 0) {
-          sort_list(join_lists(), sh);
-          cut = cut_of_list((int)total, (int)total, acc, want, by_count);
+          const int count = (int)sh.members;
+          if (!by_count)
+            for (int i = threadIdx.x; i < count; i += THREADS) sh.weights[i] = weight((uint32_t)(sh.list[i] >> 32));
+          cut = last_below(count, lowest - 1, highest, want - acc, by_count ? COUNTED : WEIGHED);
         }
-        tell(cut, 0, 0);
-        return sh.found[0];
+        tell(CUT, cut);
+        cluster().sync();
+        return sh.told[CUT];
       }
-      shift = max(0, 64 - __clzll(highest - lowest) - 11);
+      if (lowest > highest) break;
+      shift = max(0, 64 - __clzll(highest - lowest) - (by_count || round == 0 ? 11 : 10));  // into BINS, or PARTS
     }
+    return lowest;  // not reached
   }
 };
 
 template <typename T, int VEC>
-__global__ void __launch_bounds__(THREADS) sample_kernel(Sampling a, int run, int32_t* __restrict__ tokens) {
-  extern __shared__ __align__(16) char raw[];
-  Shared& sh = *reinterpret_cast<Shared*>(raw);
-  uint32_t* keys = reinterpret_cast<uint32_t*>(raw + sizeof(Shared));
+__global__ void __launch_bounds__(THREADS, 2) sample_kernel(Sampling a, int run, int32_t* __restrict__ tokens) {
+  Shared& sh = shared();
+  uint32_t* keys = row_keys();
   cg::cluster_group cluster = cg::this_cluster();
   const int blocks = (int)cluster.num_blocks(), rank = (int)cluster.block_rank(), words = (int)a.words;
   const int64_t row = blockIdx.x / blocks;
@@ -378,29 +565,25 @@ __global__ void __launch_bounds__(THREADS) sample_kernel(Sampling a, int run, in
   cg::cluster_group::arrival_token begun = cluster.barrier_arrive();
   if (threadIdx.x < 128) sh.powers[threadIdx.x] = exp2(threadIdx.x / 128.0);
 
-  // the row, the largest element
+  // the row, the largest element; every thread's words in ascending order
   uint32_t high = 0;
   int where = 0;
-  if constexpr (VEC > 1) {
+  const auto note = [&](int i, uint32_t k) {
+    keys[i] = k;
+    if (k > high) high = k, where = i;
+  };
+  const int whole = n / VEC * VEC;
 #pragma unroll 4
-    for (int i = threadIdx.x * VEC; i < n; i += THREADS * VEC) {
+  for (int i = threadIdx.x * VEC; i < whole; i += THREADS * VEC) {
+    if constexpr (VEC > 1) {
       const uint4 u = *reinterpret_cast<const uint4*>(p + i);
-      const T* e = reinterpret_cast<const T*>(&u);
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) {
-        const uint32_t k = key_of(to_f32(e[j]));
-        keys[i + j] = k;
-        if (k > high) high = k, where = i + j;
-      }
-    }
-  } else {
-#pragma unroll 4
-    for (int i = threadIdx.x; i < n; i += THREADS) {
-      const uint32_t k = key_of(to_f32(p[i]));
-      keys[i] = k;
-      if (k > high) high = k, where = i;
+      for (int j = 0; j < VEC; ++j) note(i + j, key_of(to_f32(reinterpret_cast<const T*>(&u)[j])));
+    } else {
+      note(i, key_of(to_f32(p[i])));
     }
   }
+  if (whole + (int)threadIdx.x < n) note(whole + threadIdx.x, key_of(to_f32(p[whole + threadIdx.x])));
   u64 best = high ? (u64)high << 32 | ~(uint32_t)(first + where) : 0;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, o));
@@ -420,70 +603,89 @@ __global__ void __launch_bounds__(THREADS) sample_kernel(Sampling a, int run, in
     if (rank == 0 && threadIdx.x == 0) tokens[row] = top > -INFINITY ? (int32_t)~(uint32_t)best : -1;
     return;
   }
-  Row r{cluster, blocks, rank, first, n, keys, {top, 184.66496523378731 / temperature, sh.powers}, sh};  // 128 / ln 2
-
-  const bool cut_k = top_k > 0 && top_k < words, cut_p = top_p < 1;
-  const auto wanted = [&](u64 total) {  // the whole number that a running sum below top_p total is below
-    const double w = top_p > 0 ? ceil(top_p * (double)total) : 1.0;
-    return w >= 1.0 ? (u64)w : 1;
-  };
+  if (threadIdx.x == 0) {
+    sh.set = {top_k, top_p, min_p > 0 ? (u64)ceil(fmin(min_p, 1.0) * ONE) : 0, (double)a.uniform[row],
+              top_k > 0 && top_k < words, top_p < 1};
+    sh.top = top, sh.scale = 184.66496523378731 / temperature;  // 128 / ln 2
+    sh.blocks = blocks, sh.rank = rank, sh.first = first, sh.n = n;
+  }
+  __syncthreads();
+  const Settings& set = sh.set;
+  Row r;
   u64 cut = 0;
-  if (cut_k || cut_p) {
-    const int64_t ask = cut_k ? top_k : NUCLEUS;
+  if (set.cut_k || set.cut_p) {
     u64 total = 0;
-    if (!cut_k) total = r.total_weight(0, 0);
-    bool done = false;
-    if (ask <= (int64_t)blocks * THREADS) {
+    if (!set.cut_k) total = r.total_weight(0);
+    // no word weighs more than one, most weigh far less: the nucleus is likely to have some sixteen
+    // times as many words as its weight
+    const u64 likely = set.cut_k ? 0 : 16 * (wanted(top_p, total) >> 44);
+    for (int64_t ask = set.cut_k ? top_k : likely > NUCLEUS ? NUCLEUS_MORE : NUCLEUS;
+         ask <= ASK && likely <= (u64)NUCLEUS_MORE; ask = NUCLEUS_MORE) {
       uint32_t bound = 0;
-      if (rank == 0) bound = nth_largest(sh.maxima, blocks * THREADS, (int)ask, sh);
-      r.tell(bound, 0, 0);
-      bound = (uint32_t)sh.found[0];
-      r.gather([&](int i) { return keys[i] >= bound; });
-      if (threadIdx.x == 0) cluster.map_shared_rank(&sh, 0)->listed[rank] = sh.members;
+      if (rank == 0) bound = bound_of(blocks * THREADS, (int)ask);
+      if (threadIdx.x == 0) sh.members = 0;
+      r.tell(BOUND, bound);
       cluster.sync();
-      u64 mine = 0, ok = 0;
-      if (rank == 0) {
-        const int count = r.join_lists();
-        if (count >= 0) {
-          sort_list(count, sh);
-          const int most = cut_k ? min(count, (int)top_k) : count;  // at least top_k elements reach the bound
-          ok = 1;
-          if (cut_k) {
-            mine = sh.list[most - 1];
-            if (cut_p) total = r.weight_of_list(most);
-          }
-          if (cut_p) {
-            mine = r.cut_of_list(count, most, 0, wanted(total), false);
-            ok = sh.found[1];
+      bound = (uint32_t)sh.told[BOUND];
+      // (a bound of 0, where fewer threads than asked for have words, lists every word)
+      if (high >= bound && (bound || words <= LIST)) {
+#pragma unroll 2
+        for (int i = threadIdx.x * VEC; i < whole; i += THREADS * VEC) {
+          if constexpr (VEC >= 4) {
+#pragma unroll
+            for (int j = i; j < i + VEC; j += 4) {
+              const uint4 k = *reinterpret_cast<const uint4*>(keys + j);
+              if (max(max(k.x, k.y), max(k.z, k.w)) >= bound)
+#pragma unroll 1
+                for (int l = j; l < j + 4; ++l)
+                  if (keys[l] >= bound) r.list(r.element(l));
+            }
+          } else if (keys[i] >= bound) {
+            r.list(r.element(i));
           }
         }
-        __syncthreads();
+        if (whole + (int)threadIdx.x < n && keys[whole + threadIdx.x] >= bound) r.list(r.element(whole + threadIdx.x));
       }
-      r.tell(mine, ok, 0);
-      cut = sh.found[0];
-      done = sh.found[1];
+      cluster.sync();
+      u64 ok = 0;
+      if (rank == 0 && sh.members <= LIST && (bound || words <= LIST)) {
+        ok = 1;
+        if (!set.cut_k) {  // does the cut lie in the list?
+          u64 sum = 0;
+#pragma unroll 1
+          for (int i = threadIdx.x; i < (int)sh.members; i += THREADS) sum += r.weight((uint32_t)(sh.list[i] >> 32));
+          ok = block_scan(sum).total >= wanted(top_p, total);
+        }
+      }
+      r.tell(IN_LIST, ok);
+      cluster.sync();
+      if (sh.told[IN_LIST]) {
+        if (rank) return;  // block 0 finds the word; waiting for it would take issue slots from others
+        const int count = (int)sh.members;
+        if (count <= SHORT) word_of_short_list(count, total, tokens + row);
+        else word_of_list(count, total, ((u64)bound << 32) - (bound ? 1 : 0), best, words, tokens + row);
+        return;
+      }
+      if (set.cut_k || ask == NUCLEUS_MORE) break;
     }
-    if (!done) {
-      const float per_unit = (float)(BINS / (32.0 * temperature));
-      cut = 0;
-      if (cut_k) cut = r.search((u64)top_k, true, per_unit);
-      if (cut_p) {
-        if (cut_k) total = r.total_weight(cut, 0);
-        cut = max(cut, r.search(wanted(total), false, per_unit));
-      }
+    const float per_unit = (float)(BINS / (32.0 * temperature));
+#pragma unroll 1
+    for (int pass = set.cut_k ? 0 : 1; pass < (set.cut_p ? 2 : 1); ++pass) {
+      if (pass == 1 && set.cut_k) total = r.total_weight(cut);
+      cut = max(cut, r.search(pass ? wanted(set.top_p, total) : (u64)set.top_k, !pass, per_unit));
     }
   }
 
   // sums of what is left, by warps that each own neighbouring words
-  const u64 least = min_p > 0 ? (u64)ceil(fmin(min_p, 1.0) * ONE) : 0;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, per = ((n + WARPS - 1) / WARPS + 31) / 32 * 32;
   const int lo = min(n, warp * per), hi = min(n, lo + per);
   const auto kept = [&](int i) -> u64 {
     if (i >= hi || r.element(i) < cut) return 0;
     const u64 w = r.weight(keys[i]);
-    return w >= least ? w : 0;
+    return w >= set.least ? w : 0;
   };
   u64 mine = 0;
+#pragma unroll 4
   for (int i = lo + lane; i < hi; i += 32) mine += kept(i);
   mine = warp_add(mine);
   __syncthreads();
@@ -501,9 +703,7 @@ __global__ void __launch_bounds__(THREADS) sample_kernel(Sampling a, int run, in
     if (b < rank) before += sh.sums[b];
     total += sh.sums[b];
   }
-  const double u = (double)a.uniform[row];
-  u64 want = u > 0 ? (u64)(fmin(u, 1.0) * (double)total) : 0;  // a running sum above u total is above its whole part
-  want = want < total ? want : total - 1;
+  const u64 want = passed(set.uniform, total);
   if (want < before || want >= before + mine) return;
   for (int i0 = lo; i0 < hi; i0 += 32) {
     u64 s = kept(i0 + lane);
@@ -525,11 +725,11 @@ template <typename T, int VEC>
 void launch(const Sampling& a, int32_t* tokens, int blocks, int run, cudaStream_t s) {
   const size_t smem = sizeof(Shared) + (size_t)run * 4;
   const auto kernel = sample_kernel<T, VEC>;
-  static std::atomic<size_t> allowed[kMaxDevices];
-  std::atomic<size_t>& here = allowed[current_device_slot()];
-  if (here.load() < smem) {
+  static std::atomic<bool> allowed[kMaxDevices];
+  std::atomic<bool>& here = allowed[current_device_slot()];
+  if (!here.load()) {
     DLVK_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024));
-    here.store(227 * 1024);
+    here.store(true);
   }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(a.rows * blocks));
@@ -559,7 +759,7 @@ void sample_tokens(const Sampling& a, int32_t* tokens, cudaStream_t s) {
   while (blocks < MOST_BLOCKS && (run_of(blocks) > 16384 || (a.rows * blocks < 148 && run_of(blocks) > 2048))) blocks *= 2;
   const int run = run_of(blocks);
   const int64_t bytes = a.dt == DType::BF16 ? 2 : 4;
-  const bool wide = reinterpret_cast<uintptr_t>(a.logits) % 16 == 0 && a.ld * bytes % 16 == 0 && a.words * bytes % 16 == 0;
+  const bool wide = reinterpret_cast<uintptr_t>(a.logits) % 16 == 0 && (a.ld * bytes % 16 == 0 || a.rows == 1);
   if (a.dt == DType::BF16) {
     if (wide) launch<__nv_bfloat16, 8>(a, tokens, blocks, run, s);
     else launch<__nv_bfloat16, 1>(a, tokens, blocks, run, s);
