@@ -102,13 +102,16 @@ struct Weights {
   float top;
   double scale;  // 128 / (ln 2 temperature)
   const double* powers;
+  // No branches: the loops over words have several of these under way.
   __device__ __forceinline__ u64 operator()(uint32_t key) const {
     const float x = value_of(key);
-    if (x == top) return (u64)ONE;
-    if (top == INFINITY) return 0;
-    const double y = ((double)x - (double)top) * scale;  // -infinity where x is
-    if (!(y > -5800.0)) return 0;                        // below 2^-45
-    const double magic = 6755399441055744.0;             // 1.5 2^52: adding it rounds to whole numbers
+    const u64 w = at(((double)x - (double)top) * scale);
+    return x == top ? (u64)ONE : w;
+  }
+  // exp(y ln 2 / 128); nothing below 2^-45, nor where y is no number
+  __device__ __forceinline__ u64 at(double y) const {
+    y = fmax(y, -5888.0);
+    const double magic = 6755399441055744.0;  // 1.5 2^52: adding it rounds to whole numbers
     const double z = y + magic;
     const int k = __double2loint(z);
     const double r = (y - (z - magic)) * 0.0054152123481245727;  // ln 2 / 128
@@ -236,7 +239,7 @@ __device__ __forceinline__ u64 last_below(int count, u64 lo, u64 hi, u64 want, O
     const int shift = max(0, 64 - __clzll(hi - lo - 1) - 10);
 #pragma unroll
     for (int i = threadIdx.x; i < 4 * PARTS; i += THREADS) mass[0][i] = 0;
-    if (threadIdx.x == 0) sh.scan2[0] = 0;
+    if (threadIdx.x == 0) sh.count[0] = 0;
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < PER; ++i)
@@ -251,9 +254,10 @@ __device__ __forceinline__ u64 last_below(int count, u64 lo, u64 hi, u64 want, O
               second = order == COUNTED ? amount[mine + 1] : mass_of(mass, mine + 1);
     const u64 before = acc + block_scan(first + second).before;
     const bool in0 = amount[mine] && before < want, in1 = amount[mine + 1] && before + first < want;
-    if (in0 || in1) atomicMax(&sh.scan2[0], (u64)(in1 ? mine + 1 : mine) + 1);
+    const unsigned last = __reduce_max_sync(0xffffffffu, in1 ? mine + 2 : in0 ? mine + 1 : 0);
+    if ((threadIdx.x & 31) == 0 && last) atomicMax(&sh.count[0], last);
     __syncthreads();
-    const int part = (int)sh.scan2[0] - 1;
+    const int part = (int)sh.count[0] - 1;
     if (part >> 1 == threadIdx.x) sh.scan2[1] = part & 1 ? before + first : before;
     __syncthreads();
     if (part < 0) return hi;  // not reached: the first element has nothing before it
@@ -418,6 +422,7 @@ struct Row {
       for (int i = threadIdx.x; i < BINS; i += THREADS) sh.bins.amount[i] = 0;
       if (exact) for (int i = threadIdx.x; i < 3 * PARTS; i += THREADS) sh.bins.mass[0][i] = 0;
       __syncthreads();
+#pragma unroll 4
       for (int i = threadIdx.x; i < n; i += THREADS) {
         const u64 e = element(i);
         if (e < lowest || e > highest) continue;
@@ -457,10 +462,9 @@ struct Row {
               most = weight((uint32_t)(top >> 32)) + 1;
               least = weight((uint32_t)((bottom > top ? 0 : bottom) >> 32));
             } else {
-              const double unit = weight.scale * 0.0054152123481245727 / (double)per_unit;  // a bin's width, in e-folds
-              const bool known = unit >= 0;  // not where the temperature is infinite
-              most = known ? (u64)(ONE * exp(-(i - 1.0 / 4096) * unit)) + 1 : (u64)ONE;
-              least = known ? (u64)(ONE * exp(-(i + 1 + 1.0 / 4096) * unit)) : 0;
+              const double unit = weight.scale / (double)per_unit;  // a bin's width; no number where the temperature is infinite
+              most = unit >= 0 ? weight.at(fmin(0.0, -(i - 1.0 / 4096) * unit)) + 1 : (u64)ONE;
+              least = unit >= 0 ? weight.at(-(i + 1 + 1.0 / 4096) * unit) : 0;
             }
             low[k] = amount[k] * (least ? least - 1 : 0);
             high[k] = amount[k] * min(most, (u64)ONE);
@@ -469,44 +473,49 @@ struct Row {
         }
         low_before = block_scan(lows).before;
         high_before = block_scan(highs).before;
-        if (threadIdx.x == 0) sh.scan2[0] = ~0ull, sh.scan2[1] = 0, sh.scan2[2] = 0, sh.count[0] = 0, sh.members = 0;
+        if (threadIdx.x == 0) sh.count[0] = BINS, sh.count[1] = 0, sh.count[2] = 0, sh.count[3] = 0, sh.members = 0;
         __syncthreads();
         low_before += acc, high_before += acc;
+        // the first bin that the cut may lie in, the last that it may, the last of all
+        unsigned from = BINS, to = 0, last = 0, in = 0;
 #pragma unroll
         for (int k = 0; k < PER; ++k) {
-          const u64 i = threadIdx.x * PER + k;
+          const unsigned i = threadIdx.x * PER + k;
           if (amount[k]) {
-            atomicMax(&sh.scan2[2], i);                                          // the last bin of all
-            if (high_before + high[k] >= want) atomicMin(&sh.scan2[0], i);      // the first that the cut may lie in
-            if (low_before < want) atomicMax(&sh.scan2[1], i);                   // the last
+            last = i;
+            if (from == BINS && high_before + high[k] >= want) from = i;
+            if (low_before < want) to = i;
           }
           low_before += low[k], high_before += high[k];
         }
+        from = __reduce_min_sync(0xffffffffu, from);
+        to = __reduce_max_sync(0xffffffffu, to);
+        last = __reduce_max_sync(0xffffffffu, last);
+        if ((threadIdx.x & 31) == 0) atomicMin(&sh.count[0], from), atomicMax(&sh.count[1], to), atomicMax(&sh.count[2], last);
         __syncthreads();
-        unsigned in = 0;
+        from = min(sh.count[0], sh.count[2]), to = sh.count[1];
 #pragma unroll
-        for (int k = 0; k < PER; ++k) {
-          const u64 i = threadIdx.x * PER + k;
-          if (i >= min(sh.scan2[0], sh.scan2[2]) && i <= sh.scan2[1]) in += amount[k];
-        }
+        for (int k = 0; k < PER; ++k) in += threadIdx.x * PER + k >= from && threadIdx.x * PER + k <= to ? amount[k] : 0;
         in = __reduce_add_sync(0xffffffffu, in);
-        if ((threadIdx.x & 31) == 0 && in) atomicAdd(&sh.count[0], in);
+        if ((threadIdx.x & 31) == 0 && in) atomicAdd(&sh.count[3], in);
         __syncthreads();
       }
-      tell(FIRST_BIN, min(sh.scan2[0], sh.scan2[2]));
-      tell(LAST_BIN, sh.scan2[1]);
-      tell(IN_BINS, sh.count[0]);
+      tell(FIRST_BIN, min(sh.count[0], sh.count[2]));
+      tell(LAST_BIN, sh.count[1]);
+      tell(IN_BINS, sh.count[3]);
       cluster().sync();
       const int from = (int)sh.told[FIRST_BIN], to = (int)sh.told[LAST_BIN];
       const bool fits = sh.told[IN_BINS] <= LIST;
       const u64 lo = lowest, hi = highest;
       u64 above = 0, least = ~0ull, most = 0;
+#pragma unroll 2
       for (int i = threadIdx.x; i < n; i += THREADS) {
         const u64 e = element(i);
-        if (e < lo || e > hi) continue;
         const int b = bin_of(i);
-        if (b < from) above += by_count ? 1 : weight(keys[i]);
-        if (b < from || b > to) continue;
+        const bool range = e >= lo && e <= hi;
+        const u64 w = by_count ? 1 : weight(keys[i]);
+        above += range && b < from ? w : 0;
+        if (!range || b < from || b > to) continue;
         least = min(least, e), most = max(most, e);
         if (fits) list(e);
       }
@@ -515,13 +524,10 @@ struct Row {
         least = min(least, __shfl_xor_sync(0xffffffffu, least, o));
         most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
       }
-      if ((threadIdx.x & 31) == 0) sh.scan2[threadIdx.x >> 5] = least;
+      if ((threadIdx.x & 31) == 0) sh.scan2[threadIdx.x >> 5] = least, sh.scan2[WARPS + (threadIdx.x >> 5)] = most;
       __syncthreads();
-      for (int w = 0; w < WARPS; ++w) least = min(least, sh.scan2[w]);
-      __syncthreads();
-      if ((threadIdx.x & 31) == 0) sh.scan2[threadIdx.x >> 5] = most;
-      __syncthreads();
-      for (int w = 0; w < WARPS; ++w) most = max(most, sh.scan2[w]);
+#pragma unroll 4
+      for (int w = 0; w < WARPS; ++w) least = min(least, sh.scan2[w]), most = max(most, sh.scan2[WARPS + w]);
       if (threadIdx.x < blocks) {
         Shared* there = cluster().map_shared_rank(&sh, threadIdx.x);
         there->lowest[rank] = least, there->highest[rank] = most;
