@@ -28,25 +28,30 @@ namespace {
 constexpr int THREADS = 128, WARPS = THREADS / 32;
 constexpr int NS = 4;  // states of a thread
 constexpr int V = 4;   // elements of a thread's load
+constexpr int PAD = 8;  // behind rows of sums, which a warp writes for several tokens at once: other banks
 constexpr int SPAN = STATE_SCAN_SPAN;
 
 // softplus(x) = max(x, 0) + log(1 + e), e = exp(-|x|).  Steps are small, so log(1 + e) has to
 // keep its relative precision: 2 atanh(r), r = e / (2 + e) <= 1/3, by its series (to r^17: 2^-25);
 // the exponent's rounding is made good by its remainder.
-__device__ __forceinline__ float softplus(float x) {
-  const float m = -fabsf(x), t = m * LOG2E, rest = fmaf(m, LOG2E, -t) + m * 1.925963033500e-8f;
-  float e = ex2(t);
-  e = fmaf(e, rest * 0.6931472f, e);
-  const float r = e * rcp(2.f + e), r2 = r * r;
-  float p = fmaf(r2, 1.f / 17, 1.f / 15);
-  p = fmaf(r2, p, 1.f / 13);
-  p = fmaf(r2, p, 1.f / 11);
-  p = fmaf(r2, p, 1.f / 9);
-  p = fmaf(r2, p, 1.f / 7);
-  p = fmaf(r2, p, 1.f / 5);
-  p = fmaf(r2, p, 1.f / 3);
-  return fmaxf(x, 0.f) + 2.f * fmaf(r * r2, p, r);
+__device__ __forceinline__ f2 two(float x) { return pack(x, x); }
+__device__ __forceinline__ f2 softplus_2(float x0, float x1) {
+  const f2 m = pack(-fabsf(x0), -fabsf(x1)), t = mul2(m, two(-LOG2E));
+  const f2 rest = fma2(m, two(1.925963033500e-8f), fma2(m, two(LOG2E), t));
+  const float2 tv = unpack(t);
+  f2 e = pack(ex2(-tv.x), ex2(-tv.y));
+  e = fma2(mul2(e, rest), two(0.6931472f), e);
+  const f2 r = mul2(e, rcp_2(add2(e, two(2.f)))), r2 = mul2(r, r);
+  f2 p = fma2(r2, two(2.f / 17), two(2.f / 15));
+  p = fma2(r2, p, two(2.f / 13));
+  p = fma2(r2, p, two(2.f / 11));
+  p = fma2(r2, p, two(2.f / 9));
+  p = fma2(r2, p, two(2.f / 7));
+  p = fma2(r2, p, two(2.f / 5));
+  p = fma2(r2, p, two(2.f / 3));
+  return add2(pack(fmaxf(x0, 0.f), fmaxf(x1, 0.f)), fma2(mul2(r, r2), p, add2(r, r)));
 }
+__device__ __forceinline__ float softplus(float x) { return unpack(softplus_2(x, x)).x; }
 
 __device__ __forceinline__ float both(f2 a) {
   const float2 v = unpack(a);
@@ -119,10 +124,9 @@ __device__ __forceinline__ int64_t length_of(const StateScan& a, int64_t b) {
   return a.lengths ? min(max((int64_t)a.lengths[b], (int64_t)0), a.T) : a.T;
 }
 
-// The channels of a block: CH = THREADS / L of one group of one sequence.
-template <int L>
+// The channels of a block, CH of one group of one sequence.
+template <int CH>
 struct Tile {
-  static constexpr int CH = THREADS / L;
   int64_t b;
   int group, k, c0, count;  // tile of the group; first channel, channels of the tile that exist
   __device__ __forceinline__ explicit Tile(const StateScan& a) {
@@ -147,9 +151,16 @@ __device__ __forceinline__ void deal(float* v, int lane, int& first, bool& mine)
     const bool up = lane & FROM;
     if constexpr (M > 1) {
 #pragma unroll
-      for (int i = 0; i < M / 2; ++i) {
-        const float send = up ? v[i] : v[i + M / 2], keep = up ? v[i + M / 2] : v[i];
-        v[i] = keep + __shfl_xor_sync(0xffffffffu, send, FROM);
+      for (int i = 0; i < M / 2; i += 2) {
+        if constexpr (M > 2) {
+          const f2 low = pack(v[i], v[i + 1]), high = pack(v[i + M / 2], v[i + M / 2 + 1]);
+          const float2 send = unpack(up ? low : high), got = unpack(add2(up ? high : low, pack(
+              __shfl_xor_sync(0xffffffffu, send.x, FROM), __shfl_xor_sync(0xffffffffu, send.y, FROM))));
+          v[i] = got.x, v[i + 1] = got.y;
+        } else {
+          const float send = up ? v[0] : v[1], keep = up ? v[1] : v[0];
+          v[0] = keep + __shfl_xor_sync(0xffffffffu, send, FROM);
+        }
       }
       first += up ? M / 2 : 0;
       deal<M / 2, FROM * 2, TO>(v, lane, first, mine);
@@ -189,18 +200,29 @@ struct SpanStates {
   }
 };
 
+// WIDE: four aligned states, or none (past N).
+template <bool WIDE>
 __device__ __forceinline__ Quad load_states(const float* p, int n0, int N) {
-  float h[NS];
+  if constexpr (WIDE) {
+    return n0 < N ? load_quad(p) : Quad{};
+  } else {
+    float h[NS];
 #pragma unroll
-  for (int i = 0; i < NS; ++i) h[i] = n0 + i < N ? p[i] : 0.f;
-  return {{pack(h[0], h[1]), pack(h[2], h[3])}};
+    for (int i = 0; i < NS; ++i) h[i] = n0 + i < N ? p[i] : 0.f;
+    return {{pack(h[0], h[1]), pack(h[2], h[3])}};
+  }
 }
+template <bool WIDE>
 __device__ __forceinline__ void store_states(const Quad& q, float* p, int n0, int N) {
-  const float2 a = unpack(q.v[0]), b = unpack(q.v[1]);
-  const float h[NS] = {a.x, a.y, b.x, b.y};
+  if constexpr (WIDE) {
+    if (n0 < N) *reinterpret_cast<ulonglong2*>(p) = make_ulonglong2(q.v[0], q.v[1]);
+  } else {
+    const float2 a = unpack(q.v[0]), b = unpack(q.v[1]);
+    const float h[NS] = {a.x, a.y, b.x, b.y};
 #pragma unroll
-  for (int i = 0; i < NS; ++i)
-    if (n0 + i < N) p[i] = h[i];
+    for (int i = 0; i < NS; ++i)
+      if (n0 + i < N) p[i] = h[i];
+  }
 }
 // -exp(a_log) of a thread's states, 0 past N.
 __device__ __forceinline__ Quad load_rates(const StateScan& a, int d, int n0, float scale) {
@@ -215,13 +237,23 @@ __device__ __forceinline__ Quad load_rates(const StateScan& a, int d, int n0, fl
 // the shared memory's cycles of eight that read different ones (measured: 2.1 and 4.0).
 template <int L>
 struct Place {
-  static constexpr int CHANNELS = 32 / L;  // of a warp
+  static constexpr int LANES = 32 / L;  // of a state group
   int lane, ch, n0;
   __device__ __forceinline__ Place()
-      : lane(threadIdx.x % 32), ch(threadIdx.x / 32 * CHANNELS + threadIdx.x % CHANNELS),
-        n0(threadIdx.x % 32 / CHANNELS * NS) {}
+      : lane(threadIdx.x % 32), ch(threadIdx.x / 32 * LANES + threadIdx.x % LANES),
+        n0(threadIdx.x % 32 / LANES * NS) {}
 };
 __device__ __forceinline__ float4 four(const float* p) { return *reinterpret_cast<const float4*>(p); }
+// The steps of four elements, 0 where they do not count.
+template <typename T>
+__device__ __forceinline__ void steps_of(float (&s)[V], const Four<T>& dt, const float4& bias, bool here, int left) {
+#pragma unroll
+  for (int j = 0; j < V; j += 2) {
+    const float2 v = unpack(softplus_2(dt.get(j) + (&bias.x)[j], dt.get(j + 1) + (&bias.x)[j + 1]));
+    s[j] = here && j < left ? v.x : 0.f;
+    s[j + 1] = here && j + 1 < left ? v.y : 0.f;
+  }
+}
 __device__ __forceinline__ void put_four(float* p, const float (&v)[V]) {
   *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
 }
@@ -269,13 +301,13 @@ __global__ void __launch_bounds__(THREADS) scan_ends_kernel(StateScan a, SeqRef 
   constexpr int CH = THREADS / L;
   extern __shared__ __align__(16) char raw[];
   auto& sh = *reinterpret_cast<EndsShared<T, L, WIDE>*>(raw);
-  const Tile<L> tile(a);
+  const Tile<CH> tile(a);
   const Mine<CH> my(tile.count);
   const Place<L> me;
-  const bool real = me.ch < tile.count;
   const int64_t n = length_of(a, tile.b), spans = (a.T + SPAN - 1) / SPAN;
   const int64_t from = blockIdx.y * pieces.spans;
   const int64_t to = min(min(spans, from + pieces.spans), (n + SPAN - 1) / SPAN);  // spans with a token that counts
+  const bool real = me.ch < tile.count;
   Quad h{}, rate{};
   if (real) rate = load_rates(a, tile.c0 + me.ch, me.n0, LOG2E);
   for (int j = threadIdx.x; j < CH; j += THREADS) sh.bias[j] = a.dt_bias && j < tile.count ? a.dt_bias[tile.c0 + j] : 0.f;
@@ -314,9 +346,9 @@ __global__ void __launch_bounds__(THREADS) scan_ends_kernel(StateScan a, SeqRef 
       const Four<T> dt = now.dt[e][threadIdx.x], x = now.x[e][threadIdx.x], z = now.z[e][threadIdx.x];
       const float4 bias = four(&sh.bias[my.c]);
       float s[V], sx[V];
+      steps_of(s, dt, bias, t0 + t < n, my.left);
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        s[j] = t0 + t < n && j < my.left ? softplus(dt.get(j) + (&bias.x)[j]) : 0.f;
         total[j] += s[j];
         sx[j] = !BACK ? s[j] * x.get(j) : a.z.p ? x.get(j) * z.get(j) * sigmoid(z.get(j)) : x.get(j);
       }
@@ -328,9 +360,8 @@ __global__ void __launch_bounds__(THREADS) scan_ends_kernel(StateScan a, SeqRef 
 #pragma unroll
     for (int j = 0; j < SPAN; ++j) {
       const int t = BACK ? SPAN - 1 - j : j;
-      const float s1 = sh.ss[t][me.ch], x1 = sh.sx[t][me.ch];
       const Quad q = load_quad(&sh.sb[t * NS * L + me.n0]);
-      const f2 s = pack(s1, s1), x = pack(x1, x1);
+      const f2 s = two(sh.ss[t][me.ch]), x = two(sh.sx[t][me.ch]);
 #pragma unroll
       for (int v = 0; v < 2; ++v) {
         const f2 decay = ex2_2(mul2(s, rate.v[v]));
@@ -340,7 +371,7 @@ __global__ void __launch_bounds__(THREADS) scan_ends_kernel(StateScan a, SeqRef 
     __syncthreads();
   }
   const int64_t piece = tile.b * pieces.count + blockIdx.y;
-  if (real) store_states(h, pieces.ends + (piece * a.D + tile.c0 + me.ch) * a.N + me.n0, me.n0, a.N);
+  if (real) store_states<WIDE>(h, pieces.ends + (piece * a.D + tile.c0 + me.ch) * a.N + me.n0, me.n0, a.N);
   put_four(&sh.sums[threadIdx.x].x, total);
   __syncthreads();
   constexpr int SAME = CH / V, ROWS = SPAN * SAME < THREADS ? SPAN * SAME : THREADS;
@@ -373,7 +404,7 @@ template <typename T, int L, bool WIDE>
 struct FwdShared {
   static constexpr int CH = THREADS / L, PER = Mine<CH>::PER;
   float ss[SPAN][CH], su[SPAN][CH];  // s, s u
-  float sy[SPAN][CH];                // sum_n c h
+  float sy[SPAN][CH + PAD];          // sum_n c h
   float sb[2 * SPAN * NS * L];
   float bias[CH], skip[CH];
   struct {
@@ -385,26 +416,26 @@ struct FwdShared {
 template <typename T, int L, bool WIDE>
 __global__ void __launch_bounds__(THREADS) scan_fwd_kernel(StateScan a, SeqRef y, float* out_state, float* saved,
                                                            Pieces pieces) {
-  using Tl = Tile<L>;
   using States = SpanStates<T, L, WIDE, 2>;
-  constexpr int CH = Tl::CH;
+  constexpr int CH = THREADS / L;
   extern __shared__ __align__(16) char raw[];
   auto& sh = *reinterpret_cast<FwdShared<T, L, WIDE>*>(raw);
-  const Tl tile(a);
+  const Tile<CH> tile(a);
   const Mine<CH> my(tile.count);
   const Place<L> me;
   const int lane = me.lane, n0 = me.n0, ch = me.ch;
-  const bool real = ch < tile.count;
   const int64_t n = length_of(a, tile.b), spans = (a.T + SPAN - 1) / SPAN;
   const int64_t from = blockIdx.y * pieces.spans, end = min(spans, from + pieces.spans);
   const int64_t to = max(from, min(end, (n + SPAN - 1) / SPAN));  // spans with a token that counts
-  const int64_t row = (tile.b * a.D + tile.c0 + ch) * a.N + n0;  // of this thread's states
+  const bool real = ch < tile.count;
+  const int64_t states = (int64_t)(tile.c0 + ch) * a.N + n0;  // of this thread, in a [D][N]
+  const int64_t dn = (int64_t)a.D * a.N;
   Quad h{}, rate{};
   if (real) {
     if (pieces.ends)
-      h = load_states(pieces.ends + ((tile.b * pieces.count + blockIdx.y) * a.D + tile.c0 + ch) * a.N + n0, n0, a.N);
+      h = load_states<WIDE>(pieces.ends + (tile.b * pieces.count + blockIdx.y) * dn + states, n0, a.N);
     else if (a.state)
-      h = load_states(a.state + row, n0, a.N);
+      h = load_states<WIDE>(a.state + tile.b * dn + states, n0, a.N);
     rate = load_rates(a, tile.c0 + ch, n0, LOG2E);
   }
   for (int j = threadIdx.x; j < CH; j += THREADS) {
@@ -441,35 +472,32 @@ __global__ void __launch_bounds__(THREADS) scan_fwd_kernel(StateScan a, SeqRef y
       const Four<T> u = now.u[i][threadIdx.x], dt = now.dt[i][threadIdx.x];
       const float4 bias = four(&sh.bias[my.c]);
       float s[V], su[V];
+      steps_of(s, dt, bias, t0 + t < n, my.left);
 #pragma unroll
-      for (int j = 0; j < V; ++j) {
-        s[j] = t0 + t < n && j < my.left ? softplus(dt.get(j) + (&bias.x)[j]) : 0.f;
-        su[j] = s[j] * u.get(j);
-      }
+      for (int j = 0; j < V; ++j) su[j] = s[j] * u.get(j);
       put_four(&sh.ss[t][my.c], s);
       put_four(&sh.su[t][my.c], su);
     }
     States::widen(now.bc, sh.sb);
     __syncthreads();
-    if (saved && real) store_states(h, saved + ((tile.b * spans + k) * a.D + tile.c0 + ch) * a.N + n0, n0, a.N);
+    if (saved && real) store_states<WIDE>(h, saved + (tile.b * spans + k) * dn + states, n0, a.N);
 #pragma unroll
     for (int t = 0; t < SPAN; t += 4) {
       float v[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const float s1 = sh.ss[t + j][ch], su1 = sh.su[t + j][ch];
+        const f2 s = two(sh.ss[t + j][ch]), su = two(sh.su[t + j][ch]);
         const Quad qb = load_quad(&sh.sb[(t + j) * NS * L + n0]), qc = load_quad(&sh.sb[(SPAN + t + j) * NS * L + n0]);
-        const f2 s = pack(s1, s1), su = pack(su1, su1);
         h.v[0] = fma2(ex2_2(mul2(s, rate.v[0])), h.v[0], mul2(su, qb.v[0]));
         h.v[1] = fma2(ex2_2(mul2(s, rate.v[1])), h.v[1], mul2(su, qb.v[1]));
         v[j] = both(fma2(qc.v[0], h.v[0], mul2(qc.v[1], h.v[1])));
       }
       int first = 0;
       bool mine = true;
-      deal<4, me.CHANNELS, 32>(v, lane, first, mine);
+      deal<4, me.LANES, 32>(v, lane, first, mine);
       if (mine) {
 #pragma unroll
-        for (int j = 0; j < dealt(4, me.CHANNELS, 32); ++j) sh.sy[t + first + j][ch] = v[j];
+        for (int j = 0; j < dealt(4, me.LANES, 32); ++j) sh.sy[t + first + j][ch] = v[j];
       }
     }
     __syncthreads();
@@ -490,7 +518,7 @@ __global__ void __launch_bounds__(THREADS) scan_fwd_kernel(StateScan a, SeqRef y
     }
   }
   for (int64_t k = to; k < end; ++k) {  // behind the sequence
-    if (saved && real) store_states(h, saved + ((tile.b * spans + k) * a.D + tile.c0 + ch) * a.N + n0, n0, a.N);
+    if (saved && real) store_states<WIDE>(h, saved + (tile.b * spans + k) * dn + states, n0, a.N);
 #pragma unroll
     for (int i = 0; i < my.PER; ++i) {
       const int t = my.t + i * my.STEP;
@@ -498,7 +526,7 @@ __global__ void __launch_bounds__(THREADS) scan_fwd_kernel(StateScan a, SeqRef y
         Four<T>::zeros().template store<WIDE>(at<T>(y, tile.b, k * SPAN + t, tile.c0 + my.c), my.left);
     }
   }
-  if (out_state && real && blockIdx.y + 1 == pieces.count) store_states(h, out_state + row, n0, a.N);
+  if (out_state && real && blockIdx.y + 1 == pieces.count) store_states<WIDE>(h, out_state + tile.b * dn + states, n0, a.N);
 }
 
 // One token of each sequence: a thread has four states of a channel, neighbours'
@@ -568,8 +596,8 @@ struct BwdShared {
   static constexpr int CH = THREADS / L, PER = Mine<CH>::PER;
   float ss[SPAN][CH], su[SPAN][CH];   // s, s u
   float sq[SPAN][CH];                 // q
-  float sy[SPAN][CH];                 // sum_n c h
-  float sv[SPAN][CH], sd[SPAN][CH];   // sum_n g b, sum_n g a h' A
+  float sy[SPAN][CH + PAD];           // sum_n c h
+  float sv[SPAN][CH + PAD], sd[SPAN][CH + PAD];  // sum_n g b, sum_n g a h' A
   float sb[2 * SPAN * NS * L];
   float red[WARPS][SPAN][2 * NS * L]; // db and dc of a warp's channels
   float4 sums[2][THREADS];            // dskip and ddt_bias of a thread's elements
@@ -586,12 +614,11 @@ template <typename T, int L, bool WIDE>
 __global__ void __launch_bounds__(THREADS, 4) scan_bwd_kernel(StateScan a, const float* __restrict__ saved, SeqRef dy,
                                                               StateScanGrads g, float* __restrict__ part_bc,
                                                               float* __restrict__ part_d, Pieces pieces) {
-  using Tl = Tile<L>;
   using States = SpanStates<T, L, WIDE, 2>;
-  constexpr int CH = Tl::CH, ROW = 2 * NS * L;
+  constexpr int CH = THREADS / L, ROW = 2 * NS * L;
   extern __shared__ __align__(16) char raw[];
   auto& sh = *reinterpret_cast<BwdShared<T, L, WIDE>*>(raw);
-  const Tl tile(a);
+  const Tile<CH> tile(a);
   const Mine<CH> my(tile.count);
   const Place<L> me;
   const int lane = me.lane, warp = threadIdx.x / 32, n0 = me.n0, ch = me.ch;
@@ -603,7 +630,7 @@ __global__ void __launch_bounds__(THREADS, 4) scan_bwd_kernel(StateScan a, const
   const int64_t piece = tile.b * pieces.count + blockIdx.y;
   if (real) {
     rate = load_rates(a, tile.c0 + ch, n0, 1.f);
-    if (pieces.ends) ga = load_states(pieces.ends + (piece * a.D + tile.c0 + ch) * a.N + n0, n0, a.N);
+    if (pieces.ends) ga = load_states<WIDE>(pieces.ends + (piece * a.D + tile.c0 + ch) * a.N + n0, n0, a.N);
   }
   for (int j = threadIdx.x; j < CH; j += THREADS) {
     sh.bias[j] = a.dt_bias && j < tile.count ? a.dt_bias[tile.c0 + j] : 0.f;
@@ -660,9 +687,9 @@ __global__ void __launch_bounds__(THREADS, 4) scan_bwd_kernel(StateScan a, const
                     go = now.go[i][threadIdx.x];
       const float4 bias = four(&sh.bias[my.c]);
       float s[V], su[V], q[V];
+      steps_of(s, dt, bias, t0 + t < n, my.left);
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        s[j] = t0 + t < n && j < my.left ? softplus(dt.get(j) + (&bias.x)[j]) : 0.f;
         su[j] = s[j] * u.get(j);
         q[j] = go.get(j) * (a.z.p ? z.get(j) * sigmoid(z.get(j)) : 1.f);
       }
@@ -689,10 +716,10 @@ __global__ void __launch_bounds__(THREADS, 4) scan_bwd_kernel(StateScan a, const
       }
       int first = 0;
       bool mine = true;
-      deal<4, me.CHANNELS, 32>(v, lane, first, mine);
+      deal<4, me.LANES, 32>(v, lane, first, mine);
       if (mine) {
 #pragma unroll
-        for (int j = 0; j < dealt(4, me.CHANNELS, 32); ++j) sh.sy[t + first + j][ch] = v[j];
+        for (int j = 0; j < dealt(4, me.LANES, 32); ++j) sh.sy[t + first + j][ch] = v[j];
       }
     }
 #pragma unroll
@@ -721,10 +748,10 @@ __global__ void __launch_bounds__(THREADS, 4) scan_bwd_kernel(StateScan a, const
         sums[2 * j + 1] = both(through_a);
         int first = 0;
         bool mine = true;
-        deal<8, 1, me.CHANNELS>(w, lane, first, mine);
+        deal<8, 1, me.LANES>(w, lane, first, mine);
         if (mine) {
 #pragma unroll
-          for (int i = 0; i < dealt(8, 1, me.CHANNELS); ++i) {
+          for (int i = 0; i < dealt(8, 1, me.LANES); ++i) {
             const int e = first + i;  // < NS: db of state n0 + e
             sh.red[warp][t][(e / NS) * NS * L + n0 + e % NS] = w[i];
           }
@@ -732,10 +759,10 @@ __global__ void __launch_bounds__(THREADS, 4) scan_bwd_kernel(StateScan a, const
       }
       int first = 0;
       bool mine = true;
-      deal<8, me.CHANNELS, 32>(sums, lane, first, mine);
+      deal<8, me.LANES, 32>(sums, lane, first, mine);
       if (mine) {
 #pragma unroll
-        for (int i = 0; i < dealt(8, me.CHANNELS, 32); ++i) {
+        for (int i = 0; i < dealt(8, me.LANES, 32); ++i) {
           const int e = first + i;
           (e % 2 ? sh.sd : sh.sv)[t4 + e / 2][ch] = sums[i];
         }
@@ -785,7 +812,7 @@ __global__ void __launch_bounds__(THREADS, 4) scan_bwd_kernel(StateScan a, const
     }
     // (the barrier after the next span's elements is between these reads and what comes to their places)
   }
-  if (real) store_states({{mul2(da.v[0], rate.v[0]), mul2(da.v[1], rate.v[1])}},
+  if (real) store_states<false>({{mul2(da.v[0], rate.v[0]), mul2(da.v[1], rate.v[1])}},
                          part_d + (piece * a.D + tile.c0 + ch) * (a.N + 2) + n0, n0, a.N);
   // dskip and ddt_bias: threads CH / V apart hold the same channels
   constexpr int SAME = CH / V, ROWS = SPAN * SAME < THREADS ? SPAN * SAME : THREADS;
@@ -881,23 +908,28 @@ void by_kind(const StateScan& a, bool wide, F&& f) {
 }
 bool wide_operands(const StateScan& a) {
   return a.D / a.G % V == 0 && a.N % V == 0 && aligned(a.u, a.type) && aligned(a.dt, a.type) && aligned(a.z, a.type) &&
-         aligned(a.b, a.type) && aligned(a.c, a.type);
+         aligned(a.b, a.type) && aligned(a.c, a.type) && reinterpret_cast<uintptr_t>(a.state) % 16 == 0 &&
+         reinterpret_cast<uintptr_t>(a.a_log) % 16 == 0;
 }
+bool aligned16(const float* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 int64_t part_bc_floats(const StateScan& a) { return (int64_t)tiles_of(a) * a.B * a.T * a.G * 2 * NS * lanes_of(a.N); }
 
-// Pieces as long as there are blocks for them at once (`fill` fit the GPU), of at
-// least 8 spans each; one piece where fewer than three fit.
-Pieces pieces_of(const StateScan& a, int64_t fill) {
+// Pieces as long as the GPU has room for their blocks at once, of at least 8 spans
+// each; one piece where fewer than three fit.
+constexpr int FWD_BLOCKS = 7, BWD_BLOCKS = 4;  // that an SM has room for
+Pieces pieces_of(const StateScan& a, int blocks_an_sm) {
   Pieces p;
   const int64_t spans = (a.T + SPAN - 1) / SPAN, blocks = std::max<int64_t>(1, a.B * a.G * tiles_of(a));
-  const int64_t most = std::min(fill / blocks, spans / 8);
+  const int64_t most = std::min<int64_t>(148 * blocks_an_sm / blocks, spans / 8);
   p.spans = most >= 3 ? (spans + most - 1) / most : std::max<int64_t>(spans, 1);
   p.count = (int)((spans + p.spans - 1) / p.spans);
   if (p.count < 1) p.count = 1;
   return p;
 }
-constexpr int64_t FWD_FILL = 148 * 7, BWD_FILL = 148 * 4;
 int64_t pieces_floats(const StateScan& a, const Pieces& p) { return p.count > 1 ? a.B * p.count * a.D * (a.N + 1) : 0; }
+int64_t part_d_floats(const StateScan& a, const Pieces& p) {  // whole fours: the ends lie behind them
+  return (a.B * p.count * a.D * (a.N + 2) + 3) / 4 * 4;
+}
 
 template <typename T, int L, bool W, bool BACK>
 void join_pieces(const StateScan& a, SeqRef dy, Pieces& p, float* scratch, cudaStream_t s) {
@@ -912,13 +944,13 @@ void join_pieces(const StateScan& a, SeqRef dy, Pieces& p, float* scratch, cudaS
 
 int64_t state_scan_fwd_scratch_floats(const StateScan& a) {
   check(a);
-  return pieces_floats(a, pieces_of(a, FWD_FILL));
+  return pieces_floats(a, pieces_of(a, FWD_BLOCKS));
 }
 
 void state_scan_fwd(const StateScan& a, SeqRef y, float* out_state, float* saved, float* scratch, cudaStream_t s) {
   check(a);
   if (a.B == 0 || a.D == 0) return;
-  by_kind(a, wide_operands(a) && aligned(y, a.type), [&](auto type, auto lanes, auto wide) {
+  by_kind(a, wide_operands(a) && aligned(y, a.type) && aligned16(out_state), [&](auto type, auto lanes, auto wide) {
     using T = decltype(type);
     constexpr int L = decltype(lanes)::value;
     constexpr bool W = decltype(wide)::value;
@@ -929,7 +961,7 @@ void state_scan_fwd(const StateScan& a, SeqRef y, float* out_state, float* saved
       DLVK_POST_LAUNCH();
       return;
     }
-    Pieces p = pieces_of(a, FWD_FILL);
+    Pieces p = pieces_of(a, FWD_BLOCKS);
     join_pieces<T, L, W, false>(a, {}, p, scratch, s);
     launch(scan_fwd_kernel<T, L, W>, sizeof(FwdShared<T, L, W>), a, p.count, s, y, out_state, saved, p);
   });
@@ -937,21 +969,21 @@ void state_scan_fwd(const StateScan& a, SeqRef y, float* out_state, float* saved
 
 int64_t state_scan_bwd_scratch_floats(const StateScan& a) {
   check(a);
-  const Pieces p = pieces_of(a, BWD_FILL);
-  return part_bc_floats(a) + a.B * p.count * a.D * (a.N + 2) + pieces_floats(a, p);
+  const Pieces p = pieces_of(a, BWD_BLOCKS);
+  return part_bc_floats(a) + part_d_floats(a, p) + pieces_floats(a, p);
 }
 
 void state_scan_bwd(const StateScan& a, const float* saved, SeqRef dy, const StateScanGrads& g, float* scratch,
                     cudaStream_t s) {
   check(a);
   if (a.D == 0) return;
-  Pieces p = pieces_of(a, BWD_FILL);
+  Pieces p = pieces_of(a, BWD_BLOCKS);
   float* part_bc = scratch;
   float* part_d = part_bc + part_bc_floats(a);
-  float* ends = part_d + a.B * p.count * a.D * (a.N + 2);
+  float* ends = part_d + part_d_floats(a, p);
   if (a.B > 0) {
     const bool w = wide_operands(a) && aligned(dy, a.type) && aligned(g.du, a.type) && aligned(g.ddt, a.type) &&
-                   aligned(g.dz, a.type);
+                   aligned(g.dz, a.type) && aligned16(saved);
     by_kind(a, w, [&](auto type, auto lanes, auto wide) {
       using T = decltype(type);
       constexpr int L = decltype(lanes)::value;
