@@ -413,7 +413,9 @@ struct Row {
     bool exact = by_count;
     const auto bin_of = [&](int i) {
       if (shift >= 0) return (int)((highest - element(i)) >> shift);
-      const float x = value_of(keys[i]), q = (weight.top - x) * per_unit;
+      const float x = value_of(keys[i]), d = weight.top - x;
+      // (halves where the difference of two numbers is none of fp32)
+      const float q = d < INFINITY ? d * per_unit : (0.5f * weight.top - 0.5f * x) * per_unit * 2.f;
       return x == weight.top ? 0 : q < BINS - 1 ? (int)q : BINS - 1;
     };
     for (int round = 0; round < 10; ++round) {  // 2, and 10 of 64 bits in each of at most 7 more

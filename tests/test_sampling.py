@@ -258,3 +258,51 @@ def test_shares_follow_the_weights():
     got = torch.bincount(sampling.sample_tokens(z.expand(n, 50), u).long(), minlength=50).double()
     share = torch.softmax(z[0].double(), 0) * n
     assert bool(((got - share).abs() <= 1.01 + n * 2.0 ** -24).all())
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("temperature,spread", [(1e38, 1e38), (1e30, 1e30), (3e-30, 1e-30), (1e-300, 1.0), (1e300, 1.0),
+                                                (math.inf, 1.0), (5e-324, 3.0)])
+def test_temperatures_and_logits_at_the_ends_of_their_ranges(device, dtype, temperature, spread):
+    """Differences of logits that overflow fp32 or vanish against the temperature."""
+    z = rows_of(2, 6001, torch.float32, 9, 1.0).mul_(spread).clamp_(-3.2e38, 3.2e38).to(dtype)
+    for s in (dict(top_p=0.9), dict(top_p=0.5, top_k=4000), dict(top_k=2500, min_p=0.01), dict(top_p=0.3)):
+        check(z, dict(PLAIN, **s, temperature=temperature), device, 3, draws=2)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("words", [1100, 1600, 40000])
+def test_cuts_in_runs_of_equal_logits(device, words):
+    """One number, and two with ties across the cut: weights of 1 and 1/2 (to a
+    part of 2^-53) add up without a border within 2^-26 of these shares."""
+    z = torch.zeros(3, words)
+    z[1, ::2] = math.log(0.5)
+    z[2, words // 3:] = math.log(0.5)
+    for s in (dict(top_p=0.30001), dict(top_p=0.99999), dict(top_p=1 - 2.0 ** -50), dict(top_k=words // 2 + 7),
+              dict(top_k=1152), dict(top_k=1153), dict(top_k=1536), dict(top_k=1537), dict(top_k=words - 1),
+              dict(top_k=words - 3, top_p=0.70003), dict(min_p=0.6, top_p=0.8003)):
+        check(z, dict(PLAIN, **s), device, 5, draws=2)
+
+
+@pytest.mark.gpu
+def test_weights_of_a_few_steps():
+    """200000 words that weigh two steps of 2^-44 each behind one of 2^44: shares
+    that end among them, against the CPU's same whole numbers."""
+    z = torch.full((2, 200001), -30.0)
+    z[0, 7], z[1, 200000] = 0.0, 0.0
+    for p in (1 - 1e-8, 1 - 2e-8, 1 - 1e-9, 1 - 1e-12, 0.5):
+        for u in (0.0, 0.999, 1 - 2.0 ** -24):
+            u = torch.full((2,), u)
+            want = sampling.sample_tokens(z, u, top_p=p)
+            assert torch.equal(sampling.sample_tokens(z.cuda(), u.cuda(), top_p=p).cpu(), want)
+
+
+@pytest.mark.gpu
+def test_rows_past_31_bits():
+    z = torch.empty(70000, 32000, dtype=torch.bfloat16, device="cuda")
+    z.normal_(generator=torch.Generator("cuda").manual_seed(1))
+    u = torch.rand(70000, device="cuda")
+    got = sampling.sample_tokens(z, u, top_k=50, top_p=0.9)
+    for part in (slice(0, 300), slice(67100, 67120), slice(69700, 70000)):
+        assert torch.equal(got[part], sampling.sample_tokens(z[part].clone(), u[part], top_k=50, top_p=0.9))

@@ -614,3 +614,89 @@ def test_many_tokens_channels_and_sequences(dtype):
         assert float((last - s).abs().max()) <= 2 * 400 * 2.0 ** -20 * size
         off = (y.float() - parts.float()).abs()
         assert bool((off <= (2 * HALF[dtype]) * y.float().abs() + 2 * 400 * 2.0 ** -20 * float(y.float().abs().max())).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_states_in_place_in_pieces(dtype):
+    """A call that is cut along its tokens and moves its state on in place."""
+    p, dy, state, n = scan_inputs(2, 700, 12, 16, 1, dtype, "cuda", 31)
+    n = torch.tensor([700, 389], dtype=torch.int32, device="cuda")
+    y, last, _ = run_scan(p, state=state, lengths=n, want_state=True)
+    s = state.clone()
+    y2, same, _ = run_scan(p, state=s, lengths=n, out_state=s)
+    assert same.data_ptr() == s.data_ptr() and torch.equal(y2, y) and torch.equal(s, last)
+    w = torch.randn(12, 4, device="cuda")
+    cs = torch.randn(2, 3, 12, device="cuda").to(dtype)
+    y, last = ssm.short_conv_fwd(p["u"], w, state=cs, lengths=n, want_state=True)
+    y2, same = ssm.short_conv_fwd(p["u"], w, state=cs, lengths=n, out_state=cs)
+    assert same.data_ptr() == cs.data_ptr() and torch.equal(y2, y) and torch.equal(cs, last)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_scan_gradients_in_pieces_with_lengths(device, dtype):
+    p, dy, state, _ = scan_inputs(3, 420, 8, 16, 1, dtype, device, 33)
+    p["dt_bias"] -= 2.0
+    scan_check(p, dy, state, torch.tensor([420, 0, 131], dtype=torch.int32, device=device))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_strides_past_31_bits(dtype):
+    """Tokens 2^20 elements apart, in one buffer of 2^32 or so: the same bits as
+    from and to dense tensors."""
+    T, D, N, apart = 2100, 32, 16, 1 << 20
+    buffer = torch.empty(T * apart, dtype=dtype, device="cuda")
+    p, dy, _, _ = scan_inputs(1, T, D, N, 1, dtype, "cuda", 35)
+    at = [64]
+
+    def spread(t):
+        v = buffer.as_strided((1, T, t.shape[-1]), (T * apart, apart, 1), at[0])
+        at[0] += 64
+        return v.copy_(t) if t is not None else v
+
+    q = {k: spread(v) if k in ("u", "dt", "z", "b", "c") else v for k, v in p.items()}
+    far = spread(dy)
+    y, last, saved = run_scan(p, want_state=True, save=True)
+    y2, last2, saved2 = run_scan(q, want_state=True, save=True)
+    assert torch.equal(y, y2) and torch.equal(last, last2) and torch.equal(saved, saved2)
+    want = run_scan_bwd(p, dy, saved)
+    given = {k: spread(getattr(want, k)) for k in ("du", "ddt", "db", "dc", "dz")}
+    for v in given.values():
+        v.fill_(7.0)
+    got = run_scan_bwd(q, far, saved, **given)
+    assert all(torch.equal(a, b) for a, b in zip(got, want) if a is not None)
+    w, bias = torch.randn(D, 4, device="cuda"), torch.randn(D, device="cuda")
+    assert torch.equal(ssm.short_conv_fwd(q["u"], w, bias)[0], ssm.short_conv_fwd(p["u"], w, bias)[0])
+    given["du"].fill_(7.0)
+    want = ssm.short_conv_bwd(p["u"], w, bias, dy)
+    assert all(torch.equal(a, b) for a, b in zip(ssm.short_conv_bwd(q["u"], w, bias, far, dx=given["du"]), want))
+
+
+@pytest.mark.gpu
+def test_elements_past_31_bits():
+    """70000 sequences of 16 tokens of 2048 channels: the last ones as by themselves."""
+    B, T, D, N = 70000, 16, 2048, 16
+    g = torch.Generator("cuda").manual_seed(3)
+    r = lambda *s: torch.empty(*s, dtype=torch.bfloat16, device="cuda").normal_(generator=g)  # noqa: E731
+    u, dt, dy, b, c = r(B, T, D), r(B, T, D), r(B, T, D), r(B, T, N), r(B, T, N)
+    a_log, skip = torch.rand(D, N, device="cuda"), torch.rand(D, device="cuda")
+    some = lambda v: v[-300:].clone()  # noqa: E731
+    y, last, saved = ssm.state_scan_fwd(u, dt, a_log, b, c, skip, want_state=True, save=True)
+    few = (some(u), some(dt), a_log, some(b), some(c))
+    want = ssm.state_scan_fwd(*few, skip, want_state=True, save=True)
+    assert all(torch.equal(some(x), w) for x, w in zip((y, last, saved), want))
+    d = ssm.state_scan_bwd(u, dt, a_log, b, c, dy, saved, skip)
+    want = ssm.state_scan_bwd(*few, some(dy), want[2], skip)
+    assert all(torch.equal(some(getattr(d, k)), getattr(want, k)) for k in ("du", "ddt", "db", "dc"))
+    del d, saved
+    moved = some(last)
+    one = ssm.state_scan_step(u[:, 0], dt[:, 0], a_log, b[:, 0], c[:, 0], last, skip)
+    want = ssm.state_scan_step(few[0][:, 0], few[1][:, 0], a_log, few[3][:, 0], few[4][:, 0], moved, skip)
+    assert torch.equal(some(one), want) and torch.equal(some(last), moved)
+    w = torch.randn(D, 4, device="cuda")
+    y, last = ssm.short_conv_fwd(u, w, want_state=True)
+    want = ssm.short_conv_fwd(few[0], w, want_state=True)
+    assert torch.equal(some(y), want[0]) and torch.equal(some(last), want[1])
+    assert torch.equal(some(ssm.short_conv_bwd(u, w, None, dy)[0]), ssm.short_conv_bwd(few[0], w, None, some(dy))[0])
