@@ -73,9 +73,10 @@ struct Shared {
   u64 sums[MOST_BLOCKS];                   // a sum of weights,
   u64 lowest[MOST_BLOCKS], highest[MOST_BLOCKS];  // its elements' ends in a range
   uint32_t maxima[MOST_BLOCKS * THREADS];  // block 0: every thread's largest key
-  u64 scan[WARPS], scan2[2 * WARPS];
+  u64 scan[2][WARPS], scan2[2 * WARPS];
   unsigned count[8];
   unsigned members;                        // block 0: elements of the list
+  unsigned owned;                          // elements of this block's own list
   u64 told[6];                             // by block 0, by Told
   union {
     struct {
@@ -127,30 +128,57 @@ __device__ __forceinline__ u64 warp_add(u64 v) {
   return v;
 }
 
-// The sum of the threads before this one, and that of the block.
+// The sums of the threads before this one, and those of the block.
+template <int M>
+struct Scans {
+  u64 before[M], total[M];
+};
+template <int M>
+__device__ __forceinline__ Scans<M> block_scans(const u64 (&v)[M]) {
+  Shared& sh = shared();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  u64 s[M], w[M];
+#pragma unroll
+  for (int m = 0; m < M; ++m) s[m] = v[m];
+#pragma unroll 1
+  for (int o = 1; o < 32; o <<= 1) {
+#pragma unroll
+    for (int m = 0; m < M; ++m) {
+      const u64 t = __shfl_up_sync(0xffffffffu, s[m], o);
+      if (lane >= o) s[m] += t;
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int m = 0; m < M; ++m)
+    if (lane == 31) sh.scan[m][warp] = s[m];
+  __syncthreads();
+#pragma unroll
+  for (int m = 0; m < M; ++m) w[m] = lane < WARPS ? sh.scan[m][lane] : 0;
+#pragma unroll 1
+  for (int o = 1; o < WARPS; o <<= 1) {
+#pragma unroll
+    for (int m = 0; m < M; ++m) {
+      const u64 t = __shfl_up_sync(0xffffffffu, w[m], o);
+      if (lane >= o) w[m] += t;
+    }
+  }
+  Scans<M> r;
+#pragma unroll
+  for (int m = 0; m < M; ++m) {
+    const u64 base = __shfl_sync(0xffffffffu, w[m], warp ? warp - 1 : 0);
+    r.before[m] = (warp ? base : 0) + s[m] - v[m];
+    r.total[m] = __shfl_sync(0xffffffffu, w[m], WARPS - 1);
+  }
+  return r;
+}
 struct Scan {
   u64 before, total;
 };
 __device__ __forceinline__ Scan block_scan(u64 v) {
-  Shared& sh = shared();
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  u64 s = v;
-#pragma unroll 1
-  for (int o = 1; o < 32; o <<= 1) {
-    const u64 t = __shfl_up_sync(0xffffffffu, s, o);
-    if (lane >= o) s += t;
-  }
-  __syncthreads();
-  if (lane == 31) sh.scan[warp] = s;
-  __syncthreads();
-  u64 w = lane < WARPS ? sh.scan[lane] : 0;
-#pragma unroll 1
-  for (int o = 1; o < WARPS; o <<= 1) {
-    const u64 t = __shfl_up_sync(0xffffffffu, w, o);
-    if (lane >= o) w += t;
-  }
-  const u64 base = __shfl_sync(0xffffffffu, w, warp ? warp - 1 : 0);
-  return {(warp ? base : 0) + s - v, __shfl_sync(0xffffffffu, w, WARPS - 1)};
+  const u64 one[1] = {v};
+  const Scans<1> s = block_scans(one);
+  return {s.before[0], s.total[0]};
 }
 
 // A weight into a bin, in three numbers of 15 bits each: additions of 64 bits to
@@ -406,17 +434,46 @@ struct Row {
   // numbers, until the elements that may be it fit a list.  The first two rounds
   // bracket it by the weights of the bins' ends; where that leaves too many (very
   // small weights, many equal ones) they hold their exact weights, and each round
-  // leaves one of 2^10 parts of the numbers.
+  // leaves one of 2^10 parts of the numbers.  What the first round leaves of a
+  // block's elements makes a list of its own, where it has room, so that later
+  // rounds do not go through the whole row again.
   __device__ __forceinline__ u64 search(u64 want, bool by_count, float per_unit) {
     u64 acc = 0, lowest = 0, highest = ~0ull;  // acc: amount above `highest`
     int shift = -1;                            // -1: by distance
     bool exact = by_count;
-    const auto bin_of = [&](int i) {
-      if (shift >= 0) return (int)((highest - element(i)) >> shift);
-      const float x = value_of(keys[i]), d = weight.top - x;
-      // (halves where the difference of two numbers is none of fp32)
-      const float q = d < INFINITY ? d * per_unit : (0.5f * weight.top - 0.5f * x) * per_unit * 2.f;
-      return x == weight.top ? 0 : q < BINS - 1 ? (int)q : BINS - 1;
+    u64* own = reinterpret_cast<u64*>(sh.maxima);  // no longer needed
+    constexpr unsigned ROOM = sizeof(sh.maxima) / sizeof(u64);
+    bool listed = false;  // own has all elements of the range
+    // by distance: halves, as a difference of two numbers may be none of fp32; all that is far, or not a number, in the last
+    const float half_top = 0.5f * weight.top;
+    const auto distance_bin = [&](uint32_t key) {
+      const float x = value_of(key), q = fmaf(x, -0.5f, half_top) * (2.f * per_unit);
+      return x == weight.top ? 0 : (int)fminf(q, BINS - 1);
+    };
+    const auto bin_of = [&](u64 e) { return shift >= 0 ? (int)((highest - e) >> shift) : distance_bin((uint32_t)(e >> 32)); };
+    // The smallest number, up to the largest logit's, in a bin (by distance) before `bin`, which is none of the
+    // first: the bins fall as the numbers rise, and 32 lanes look at once.
+    const auto edge = [&](int bin) {
+      u64 lo = key_of(-INFINITY) - 1, hi = key_of(weight.top);
+#pragma unroll 1
+      while (hi - lo > 1) {
+        const u64 step = (hi - lo + 31) / 32, k = min(hi, lo + ((threadIdx.x & 31) + 1) * step);
+        const int first = __ffs(__ballot_sync(0xffffffffu, distance_bin((uint32_t)k) < bin)) - 1;
+        hi = min(hi, lo + (first + 1) * step);
+        lo += first * step;
+      }
+      return hi;
+    };
+    // f of every element that may lie in the range.  (Two loops: a choice of where from would be a branch around each load.)
+    const auto each = [&](auto&& f) {
+      if (listed) {
+        const int m = (int)sh.owned;
+#pragma unroll 1
+        for (int i = threadIdx.x; i < m; i += THREADS) f(own[i]);
+      } else {
+#pragma unroll 4
+        for (int i = threadIdx.x; i < n; i += THREADS) f(element(i));
+      }
     };
     for (int round = 0; round < 10; ++round) {  // 2, and 10 of 64 bits in each of at most 7 more
       exact = by_count || round >= 2;
@@ -424,19 +481,17 @@ struct Row {
       for (int i = threadIdx.x; i < BINS; i += THREADS) sh.bins.amount[i] = 0;
       if (exact) for (int i = threadIdx.x; i < 3 * PARTS; i += THREADS) sh.bins.mass[0][i] = 0;
       __syncthreads();
-#pragma unroll 4
-      for (int i = threadIdx.x; i < n; i += THREADS) {
-        const u64 e = element(i);
-        if (e < lowest || e > highest) continue;
-        const int b = bin_of(i);
+      each([&](u64 e) {
+        if (e < lowest || e > highest) return;
+        const int b = bin_of(e);
         // words that weigh nothing are no cut of weights
         if (shift >= 0 || by_count || b < BINS - 1) atomicAdd(&sh.bins.amount[b], 1u);
-        if (exact && !by_count) add_mass(sh.bins.mass, b, weight(keys[i]));
-      }
+        if (exact && !by_count) add_mass(sh.bins.mass, b, weight((uint32_t)(e >> 32)));
+      });
       cluster().sync();
       if (rank == 0) {
         constexpr int PER = BINS / THREADS;
-        u64 low[PER], high[PER], lows = 0, highs = 0, low_before, high_before;
+        u64 low[PER], high[PER];
         unsigned amount[PER];
         static_assert(PER == 4, "");
         uint4 a[MOST_BLOCKS];
@@ -446,35 +501,49 @@ struct Row {
                             : make_uint4(0, 0, 0, 0);
 #pragma unroll
         for (int k = 0; k < PER; ++k) {
-          const int i = threadIdx.x * PER + k;
           amount[k] = 0;
 #pragma unroll
           for (int b = 0; b < MOST_BLOCKS; ++b) amount[k] += (&a[b].x)[k];
           low[k] = high[k] = amount[k];
-          if (!by_count && exact) {
+        }
+        if (!by_count && exact) {
+#pragma unroll
+          for (int k = 0; k < PER; ++k) {
+            const int i = threadIdx.x * PER + k;
             low[k] = 0;
             if (i < PARTS)
               for (int b = 0; b < blocks; ++b) low[k] += mass_of(cluster().map_shared_rank(sh.bins.mass, b), i);
             high[k] = low[k];
-          } else if (!by_count && amount[k]) {
-            // the weights of a bin's ends, a step (of 2^-44) or 2^-12 of a bin's width to the safe side
-            u64 most, least;
-            if (shift >= 0) {
-              const u64 top = highest - ((u64)i << shift), bottom = top - (((u64)1 << shift) - 1);
-              most = weight((uint32_t)(top >> 32)) + 1;
-              least = weight((uint32_t)((bottom > top ? 0 : bottom) >> 32));
-            } else {
-              const double unit = weight.scale / (double)per_unit;  // a bin's width; no number where the temperature is infinite
-              most = unit >= 0 ? weight.at(fmin(0.0, -(i - 1.0 / 4096) * unit)) + 1 : (u64)ONE;
-              least = unit >= 0 ? weight.at(-(i + 1 + 1.0 / 4096) * unit) : 0;
-            }
-            low[k] = amount[k] * (least ? least - 1 : 0);
-            high[k] = amount[k] * min(most, (u64)ONE);
           }
-          lows += low[k], highs += high[k];
+        } else if (!by_count) {
+          // the weights of a bin's ends, a step (of 2^-44) or 2^-12 of a bin's width to the safe side; those of empty
+          // bins too, as a branch would keep them from being under way together
+          u64 most[PER], least[PER];
+          if (shift >= 0) {
+#pragma unroll
+            for (int k = 0; k < PER; ++k) {
+              const u64 top = highest - ((u64)(threadIdx.x * PER + k) << shift), bottom = top - (((u64)1 << shift) - 1);
+              most[k] = weight((uint32_t)(top >> 32)) + 1;
+              least[k] = weight((uint32_t)((bottom > top ? 0 : bottom) >> 32));
+            }
+          } else {
+            const double unit = weight.scale / (double)per_unit;  // a bin's width; no number where the temperature is infinite
+#pragma unroll
+            for (int k = 0; k < PER; ++k) {
+              const double i = threadIdx.x * PER + k;
+              most[k] = unit >= 0 ? weight.at(fmin(0.0, -(i - 1.0 / 4096) * unit)) + 1 : (u64)ONE;
+              least[k] = unit >= 0 ? weight.at(-(i + 1 + 1.0 / 4096) * unit) : 0;
+            }
+          }
+#pragma unroll
+          for (int k = 0; k < PER; ++k) {
+            low[k] = amount[k] * (least[k] ? least[k] - 1 : 0);
+            high[k] = amount[k] * min(most[k], (u64)ONE);
+          }
         }
-        low_before = block_scan(lows).before;
-        high_before = block_scan(highs).before;
+        const u64 sums[2] = {low[0] + low[1] + low[2] + low[3], high[0] + high[1] + high[2] + high[3]};
+        const Scans<2> scans = block_scans(sums);
+        u64 low_before = scans.before[0], high_before = scans.before[1];
         if (threadIdx.x == 0) sh.count[0] = BINS, sh.count[1] = 0, sh.count[2] = 0, sh.count[3] = 0, sh.members = 0;
         __syncthreads();
         low_before += acc, high_before += acc;
@@ -508,19 +577,39 @@ struct Row {
       cluster().sync();
       const int from = (int)sh.told[FIRST_BIN], to = (int)sh.told[LAST_BIN];
       const bool fits = sh.told[IN_BINS] <= LIST;
-      const u64 lo = lowest, hi = highest;
-      u64 above = 0, least = ~0ull, most = 0;
-#pragma unroll 2
-      for (int i = threadIdx.x; i < n; i += THREADS) {
-        const u64 e = element(i);
-        const int b = bin_of(i);
-        const bool range = e >= lo && e <= hi;
-        const u64 w = by_count ? 1 : weight(keys[i]);
-        above += range && b < from ? w : 0;
-        if (!range || b < from || b > to) continue;
-        least = min(least, e), most = max(most, e);
-        if (fits) list(e);
+      // the bins' ends
+      u64 hi, lo;
+      if (shift >= 0) {
+        hi = highest - ((u64)from << shift);
+        lo = max(lowest, highest - min(highest, ((u64)(to + 1) << shift) - 1));
+      } else {
+        hi = from ? (edge(from) << 32) - 1 : ~0ull;
+        lo = edge(to + 1) << 32;
       }
+      u64 sums[2] = {0, 0};  // above the range, and how many lie in it
+      each([&](u64 e) {
+        const u64 w = by_count ? 1 : weight((uint32_t)(e >> 32));
+        sums[0] += e > hi && e <= highest ? w : 0;
+        sums[1] += e >= lo && e <= hi;
+      });
+      const Scans<2> scans = block_scans(sums);
+      const bool keep = !listed && scans.total[1] <= ROOM;
+      if (keep || fits) {
+        u64* put = own + scans.before[1];
+        each([&](u64 e) {  // (apart: its branches would keep the weights from each other)
+          if (e < lo || e > hi) return;
+          if (keep) *put++ = e;
+          if (fits) list(e);
+        });
+      }
+      if (keep) sh.owned = (unsigned)scans.total[1];
+      listed = listed || keep;
+      __syncthreads();
+      // the ends of what is left
+      u64 least = ~0ull, most = 0;
+      each([&](u64 e) {
+        if (e >= lo && e <= hi) least = min(least, e), most = max(most, e);
+      });
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) {
         least = min(least, __shfl_xor_sync(0xffffffffu, least, o));
@@ -534,7 +623,7 @@ struct Row {
         Shared* there = cluster().map_shared_rank(&sh, threadIdx.x);
         there->lowest[rank] = least, there->highest[rank] = most;
       }
-      acc += add_up(block_scan(above).total);
+      acc += add_up(scans.total[0]);
       lowest = ~0ull, highest = 0;
       for (int b = 0; b < blocks; ++b) lowest = min(lowest, sh.lowest[b]), highest = max(highest, sh.highest[b]);
       if (fits) {
@@ -595,12 +684,12 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(Sampling a, int run,
   u64 best = high ? (u64)high << 32 | ~(uint32_t)(first + where) : 0;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, o));
-  if ((threadIdx.x & 31) == 0) sh.scan[threadIdx.x >> 5] = best;
+  if ((threadIdx.x & 31) == 0) sh.scan[0][threadIdx.x >> 5] = best;
   cluster.barrier_wait(std::move(begun));
   cluster.map_shared_rank(sh.maxima, 0)[rank * THREADS + threadIdx.x] = high;
   __syncthreads();
   if (threadIdx.x < blocks) {
-    for (int w = 0; w < WARPS; ++w) best = max(best, sh.scan[w]);
+    for (int w = 0; w < WARPS; ++w) best = max(best, sh.scan[0][w]);
     *cluster.map_shared_rank(&sh.best[rank], threadIdx.x) = best;
   }
   cluster.sync();
@@ -676,7 +765,7 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(Sampling a, int run,
       }
       if (set.cut_k || ask == NUCLEUS_MORE) break;
     }
-    const float per_unit = (float)(BINS / (32.0 * temperature));
+    const float per_unit = (float)fmin(BINS / (32.0 * temperature), 1.7e38);
 #pragma unroll 1
     for (int pass = set.cut_k ? 0 : 1; pass < (set.cut_p ? 2 : 1); ++pass) {
       if (pass == 1 && set.cut_k) total = r.total_weight(cut);
@@ -697,12 +786,12 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(Sampling a, int run,
   for (int i = lo + lane; i < hi; i += 32) mine += kept(i);
   mine = warp_add(mine);
   __syncthreads();
-  if (lane == 0) sh.scan[warp] = mine;
+  if (lane == 0) sh.scan[0][warp] = mine;
   __syncthreads();
   u64 before = 0, all = 0;
   for (int w = 0; w < WARPS; ++w) {
-    if (w < warp) before += sh.scan[w];
-    all += sh.scan[w];
+    if (w < warp) before += sh.scan[0][w];
+    all += sh.scan[0][w];
   }
   if (threadIdx.x < blocks) *cluster.map_shared_rank(&sh.sums[rank], threadIdx.x) = all;
   cluster.sync();

@@ -306,3 +306,12 @@ def test_rows_past_31_bits():
     got = sampling.sample_tokens(z, u, top_k=50, top_p=0.9)
     for part in (slice(0, 300), slice(67100, 67120), slice(69700, 70000)):
         assert torch.equal(got[part], sampling.sample_tokens(z[part].clone(), u[part], top_k=50, top_p=0.9))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_logits_that_are_no_normal_numbers(device):
+    """Logits of some steps of 2^-149 and temperatures as small, where 1 / temperature is no number of fp32."""
+    z = torch.randint(0, 200, (2, 6001), generator=torch.Generator().manual_seed(4)).float() * 2.0 ** -149
+    for t in (2.0 ** -125, 2.0 ** -140, 2.0 ** -149, 1e-30):
+        for s in (dict(top_p=0.9), dict(top_k=2500), dict(top_p=0.4, top_k=3999)):
+            check(z, dict(PLAIN, **s, temperature=t), device, 4, draws=2)
