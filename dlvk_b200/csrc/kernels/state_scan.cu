@@ -390,12 +390,24 @@ __global__ void __launch_bounds__(256) scan_join_kernel(StateScan a, Pieces piec
   const int64_t b = i / dn, e = i % dn, d = e / a.N;
   const float rate = -expf(a.a_log[e]);
   float carry = !BACK && a.state ? a.state[i] : 0.f;
-  for (int j = 0; j < pieces.count; ++j) {
-    const int64_t piece = b * pieces.count + (BACK ? pieces.count - 1 - j : j);
-    float& end = pieces.ends[piece * dn + e];
-    const float own = end;
-    end = carry;
-    carry = fmaf(expf(rate * pieces.steps[piece * a.D + d]), carry, own);
+  // eight pieces' loads ahead of the stores, which might be to the same place for all that the compiler knows
+  constexpr int AHEAD = 8;
+  for (int j0 = 0; j0 < pieces.count; j0 += AHEAD) {
+    float own[AHEAD], steps[AHEAD];
+    int64_t piece[AHEAD];
+#pragma unroll
+    for (int j = 0; j < AHEAD; ++j) {
+      const int k = min(j0 + j, pieces.count - 1);
+      piece[j] = b * pieces.count + (BACK ? pieces.count - 1 - k : k);
+      own[j] = pieces.ends[piece[j] * dn + e];
+      steps[j] = pieces.steps[piece[j] * a.D + d];
+    }
+#pragma unroll
+    for (int j = 0; j < AHEAD; ++j) {
+      if (j0 + j >= pieces.count) break;
+      pieces.ends[piece[j] * dn + e] = carry;
+      carry = fmaf(expf(rate * steps[j]), carry, own[j]);
+    }
   }
 }
 
