@@ -634,6 +634,7 @@ struct BwdShared {
   float sb[2 * SPAN * NS * L];
   float red[WARPS][SPAN][2 * NS * L]; // db and dc of a warp's channels
   float4 sums[2][THREADS];            // dskip and ddt_bias of a thread's elements
+  float4 da[THREADS];                 // da_log of its states
   float bias[CH], skip[CH];
   struct {
     Four<T> u[PER][THREADS], dt[PER][THREADS], z[PER][THREADS], go[PER][THREADS];
@@ -657,7 +658,7 @@ __global__ void __launch_bounds__(THREADS, 4) scan_bwd_kernel(StateScan a, const
   const int lane = me.lane, warp = threadIdx.x / 32, n0 = me.n0, ch = me.ch;
   const bool real = ch < tile.count;
   const int64_t n = length_of(a, tile.b), spans = (a.T + SPAN - 1) / SPAN;
-  Quad rate{}, ga{}, da{};
+  Quad rate{}, ga{};
   const int64_t from = blockIdx.y * pieces.spans, end = min(spans, from + pieces.spans);
   const int64_t to = max(from, min(end, (n + SPAN - 1) / SPAN));  // spans with a token that counts
   const int64_t piece = tile.b * pieces.count + blockIdx.y;
@@ -669,7 +670,7 @@ __global__ void __launch_bounds__(THREADS, 4) scan_bwd_kernel(StateScan a, const
     sh.bias[j] = a.dt_bias && j < tile.count ? a.dt_bias[tile.c0 + j] : 0.f;
     sh.skip[j] = a.skip && j < tile.count ? a.skip[tile.c0 + j] : 0.f;
   }
-  sh.sums[0][threadIdx.x] = sh.sums[1][threadIdx.x] = make_float4(0.f, 0.f, 0.f, 0.f);
+  sh.da[threadIdx.x] = sh.sums[0][threadIdx.x] = sh.sums[1][threadIdx.x] = make_float4(0.f, 0.f, 0.f, 0.f);
   const auto fetch = [&](int64_t k) {
     auto& st = sh.stage[k % 2];
     const int64_t t0 = k * SPAN;
@@ -755,6 +756,7 @@ __global__ void __launch_bounds__(THREADS, 4) scan_bwd_kernel(StateScan a, const
         for (int j = 0; j < dealt(4, me.LANES, 32); ++j) sh.sy[t + first + j][ch] = v[j];
       }
     }
+    Quad da{};
 #pragma unroll
     for (int t4 = SPAN - 4; t4 >= 0; t4 -= 4) {
       float sums[8];  // of four tokens: sum_n g b, sum_n g a h' A
@@ -801,6 +803,10 @@ __global__ void __launch_bounds__(THREADS, 4) scan_bwd_kernel(StateScan a, const
         }
       }
     }
+    {  // (span by span, so that the sum over all tokens rounds once a span)
+      const Quad before = load_quad(&sh.da[threadIdx.x].x);
+      store_states<true>({{add2(before.v[0], da.v[0]), add2(before.v[1], da.v[1])}}, &sh.da[threadIdx.x].x, 0, 1);
+    }
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < my.PER; ++i) {
@@ -845,6 +851,7 @@ __global__ void __launch_bounds__(THREADS, 4) scan_bwd_kernel(StateScan a, const
     }
     // (the barrier after the next span's elements is between these reads and what comes to their places)
   }
+  const Quad da = load_quad(&sh.da[threadIdx.x].x);
   if (real) store_states<false>({{mul2(da.v[0], rate.v[0]), mul2(da.v[1], rate.v[1])}},
                          part_d + (piece * a.D + tile.c0 + ch) * (a.N + 2) + n0, n0, a.N);
   // dskip and ddt_bias: threads CH / V apart hold the same channels
@@ -872,13 +879,15 @@ __global__ void __launch_bounds__(256) join_bc_kernel(const float* __restrict__ 
     *at<T>(half ? dc : db, b, t, (int64_t)group * N + n) = from_f32<T>(s);
   }
 }
-// da_log, dskip and ddt_bias: the sums over the sequences and their pieces.
+// da_log, dskip and ddt_bias: the sums over the sequences and their pieces, in 64 bits (there are few).
 __global__ void __launch_bounds__(256) join_d_kernel(const float* __restrict__ part, int64_t B, int D, int N,
                                                      StateScanGrads g) {
   const int64_t total = (int64_t)D * (N + 2), i = blockIdx.x * 256LL + threadIdx.x;
   if (i >= total) return;
-  float s = 0.f;
-  for (int64_t b = 0; b < B; ++b) s += part[b * total + i];
+  double sum = 0.0;
+#pragma unroll 4
+  for (int64_t b = 0; b < B; ++b) sum += part[b * total + i];
+  const float s = (float)sum;
   const int64_t d = i / (N + 2);
   const int k = (int)(i % (N + 2));
   float* out = k < N ? (g.da_log ? g.da_log + d * N + k : nullptr)
