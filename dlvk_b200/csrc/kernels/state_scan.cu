@@ -17,6 +17,14 @@
 // N states has N / 4 lanes, and sums over states and channels cross lanes by
 // shuffles.  The next span's elements are on their way to shared memory
 // meanwhile, each to a place that only the thread that asked for it reads.
+//
+// What bounds it is the exponentials, one a token, channel and state (the special
+// function units make 16 a clock and SM: 60 us for the 268 M of 16 x 512 tokens x
+// 2048 channels x 16 states), and the issue slots and shared memory around them;
+// the bytes are less (41 us of forward and backward together).  A thread has four
+// states because fewer share a channel's step and input among too many lanes, and
+// more leave too few warps: two channels a thread, whose loads of b and c are
+// shared, and blocks of 64 threads were both slower.
 #include <algorithm>
 #include <type_traits>
 
@@ -293,6 +301,9 @@ struct EndsShared {
   } stage[2];
 };
 
+// One sequence of 16384 tokens x 2048 channels, 16 pieces: 170-179 us, joining them 7,
+// the pass proper 241-256, where one piece a sequence took 4871 in all.
+//
 // The end of a piece.  Forward: h[t] = a[t] h[t-1] + s u b[t].  BACK (what
 // reaches the token before the piece): g[t] = c[t] q + a[t+1] g[t+1], times a[t].
 template <typename T, int L, bool WIDE, bool BACK>
@@ -425,6 +436,10 @@ struct FwdShared {
   } stage[2];
 };
 
+// 16 x 512 x 2048, 16 states, bf16 with gates: 133 us, 45% of the special function units' rate.
+// Issue slots 62%, shared memory 70%, special functions 60% busy on average; warps compete for all
+// three until the blocks that an SM began with end one by one.  62 registers: seven blocks an SM.
+// (Steps as pairs of equals in shared memory, which spares moves: 10% slower.)
 template <typename T, int L, bool WIDE>
 __global__ void __launch_bounds__(THREADS) scan_fwd_kernel(StateScan a, SeqRef y, float* out_state, float* saved,
                                                            Pieces pieces) {
@@ -545,7 +560,9 @@ __global__ void __launch_bounds__(THREADS) scan_fwd_kernel(StateScan a, SeqRef y
 // which share the channel's rates; what it reads is asked for before anything is
 // computed.  Steps and gates, one value a channel and sequence, are dealt out to the
 // channel's lanes: lane by lane they were most of the instructions, which bound this
-// kernel before the memory did.
+// kernel before the memory did.  130 sequences x 1600 channels of 64 states (106 MB of
+// states read and written): 27 us, 60% of the copy rate; 64 x 2048 of 16: 6.5 us, a
+// launch and one round to the memory.
 template <typename T, int L, bool WIDE, int R>
 __global__ void __launch_bounds__(THREADS) scan_step_kernel(StateScan a, SeqRef y, float* out_state, float* saved) {
   constexpr int CH = THREADS / L, OWN = dealt(R, 1, L);
@@ -643,6 +660,14 @@ struct BwdShared {
   } stage[2];
 };
 
+// A span's states are made again from the one saved before it and stay in registers
+// (68 of 128) while the tokens go back.  16 x 512 x 2048, 16 states, bf16 with gates:
+// 386 us and 19 joining the sums, 120 instructions a warp and token: the exponentials
+// twice, sums of db and dc over channels (7 shuffles, each of which halves the values
+// that a lane still adds up), of du and ds over states.  Issue slots 62%, shared memory
+// 67% busy; 16 warps an SM.  Sums over channels as tf32 products of ones and the values
+// took longer (some 9 cycles a product of 16 x 8 x 4) and needed two for fp32.
+//
 // part_bc [tiles of a group][B][T][G][2][NS L]; part_d [B][pieces][D][N + 2]: da, dskip, ddt_bias.
 template <typename T, int L, bool WIDE>
 __global__ void __launch_bounds__(THREADS, 4) scan_bwd_kernel(StateScan a, const float* __restrict__ saved, SeqRef dy,
@@ -956,14 +981,19 @@ bool wide_operands(const StateScan& a) {
 bool aligned16(const float* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 int64_t part_bc_floats(const StateScan& a) { return (int64_t)tiles_of(a) * a.B * a.T * a.G * 2 * NS * lanes_of(a.N); }
 
-// Pieces as long as the GPU has room for their blocks at once, of at least 8 spans
-// each; one piece where fewer than three fit.
+// Pieces as long as the GPU has room for their blocks at once, of at least four spans each
+// (1 x 4096 x 64 channels of 16 states, forward and backward: 30 and 48 us; of eight 33 and 57,
+// of two 32 and 54; one piece 334 and 795).  The pass for the ends costs two thirds of the pass
+// proper, so few pieces are worse than one: forward, 3 x 1024 x 2048, five take 99 us and one 106,
+// but of 4 x 1024 four take 122; backward, three of the former take 210 and one 277, two of the
+// latter 300.
 constexpr int FWD_BLOCKS = 7, BWD_BLOCKS = 4;  // that an SM has room for
-Pieces pieces_of(const StateScan& a, int blocks_an_sm) {
+constexpr int FWD_PIECES = 5, BWD_PIECES = 3, PIECE_SPANS = 4;
+Pieces pieces_of(const StateScan& a, int blocks_an_sm, int least) {
   Pieces p;
   const int64_t spans = (a.T + SPAN - 1) / SPAN, blocks = std::max<int64_t>(1, a.B * a.G * tiles_of(a));
-  const int64_t most = std::min<int64_t>(148 * blocks_an_sm / blocks, spans / 8);
-  p.spans = most >= 3 ? (spans + most - 1) / most : std::max<int64_t>(spans, 1);
+  const int64_t most = std::min<int64_t>(148 * blocks_an_sm / blocks, spans / PIECE_SPANS);
+  p.spans = most >= least ? (spans + most - 1) / most : std::max<int64_t>(spans, 1);
   p.count = (int)((spans + p.spans - 1) / p.spans);
   if (p.count < 1) p.count = 1;
   return p;
@@ -990,7 +1020,7 @@ constexpr int64_t STEP_BLOCKS = 148 * 4;
 
 int64_t state_scan_fwd_scratch_floats(const StateScan& a) {
   check(a);
-  return pieces_floats(a, pieces_of(a, FWD_BLOCKS));
+  return pieces_floats(a, pieces_of(a, FWD_BLOCKS, FWD_PIECES));
 }
 
 void state_scan_fwd(const StateScan& a, SeqRef y, float* out_state, float* saved, float* scratch, cudaStream_t s) {
@@ -1011,7 +1041,7 @@ void state_scan_fwd(const StateScan& a, SeqRef y, float* out_state, float* saved
       DLVK_POST_LAUNCH();
       return;
     }
-    Pieces p = pieces_of(a, FWD_BLOCKS);
+    Pieces p = pieces_of(a, FWD_BLOCKS, FWD_PIECES);
     join_pieces<T, L, W, false>(a, {}, p, scratch, s);
     launch(scan_fwd_kernel<T, L, W>, sizeof(FwdShared<T, L, W>), a, p.count, s, y, out_state, saved, p);
   });
@@ -1019,7 +1049,7 @@ void state_scan_fwd(const StateScan& a, SeqRef y, float* out_state, float* saved
 
 int64_t state_scan_bwd_scratch_floats(const StateScan& a) {
   check(a);
-  const Pieces p = pieces_of(a, BWD_BLOCKS);
+  const Pieces p = pieces_of(a, BWD_BLOCKS, BWD_PIECES);
   return part_bc_floats(a) + part_d_floats(a, p) + pieces_floats(a, p);
 }
 
@@ -1027,7 +1057,7 @@ void state_scan_bwd(const StateScan& a, const float* saved, SeqRef dy, const Sta
                     cudaStream_t s) {
   check(a);
   if (a.D == 0) return;
-  Pieces p = pieces_of(a, BWD_BLOCKS);
+  Pieces p = pieces_of(a, BWD_BLOCKS, BWD_PIECES);
   float* part_bc = scratch;
   float* part_d = part_bc + part_bc_floats(a);
   float* ends = part_d + part_d_floats(a, p);
