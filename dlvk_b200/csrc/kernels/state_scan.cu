@@ -41,10 +41,11 @@ constexpr int SPAN = STATE_SCAN_SPAN;
 
 // softplus(x) = max(x, 0) + log(1 + e), e = exp(-|x|).  Steps are small, so log(1 + e) has to
 // keep its relative precision: 2 atanh(r), r = e / (2 + e) <= 1/3, by its series (to r^17: 2^-25);
-// the exponent's rounding is made good by its remainder.
+// the exponent's rounding is made good by its remainder.  Below -200 e is 0 (an infinity would leave
+// no remainder); NaN passes through the first term.
 __device__ __forceinline__ f2 two(float x) { return pack(x, x); }
 __device__ __forceinline__ f2 softplus_2(float x0, float x1) {
-  const f2 m = pack(-fabsf(x0), -fabsf(x1)), t = mul2(m, two(-LOG2E));
+  const f2 m = pack(fmaxf(-fabsf(x0), -200.f), fmaxf(-fabsf(x1), -200.f)), t = mul2(m, two(-LOG2E));
   const f2 rest = fma2(m, two(1.925963033500e-8f), fma2(m, two(LOG2E), t));
   const float2 tv = unpack(t);
   f2 e = pack(ex2(-tv.x), ex2(-tv.y));
@@ -57,7 +58,7 @@ __device__ __forceinline__ f2 softplus_2(float x0, float x1) {
   p = fma2(r2, p, two(2.f / 7));
   p = fma2(r2, p, two(2.f / 5));
   p = fma2(r2, p, two(2.f / 3));
-  return add2(pack(fmaxf(x0, 0.f), fmaxf(x1, 0.f)), fma2(mul2(r, r2), p, add2(r, r)));
+  return add2(pack(x0 < 0.f ? 0.f : x0, x1 < 0.f ? 0.f : x1), fma2(mul2(r, r2), p, add2(r, r)));
 }
 __device__ __forceinline__ float softplus(float x) { return unpack(softplus_2(x, x)).x; }
 

@@ -700,3 +700,32 @@ def test_elements_past_31_bits():
     want = ssm.short_conv_fwd(few[0], w, want_state=True)
     assert torch.equal(some(y), want[0]) and torch.equal(some(last), want[1])
     assert torch.equal(some(ssm.short_conv_bwd(u, w, None, dy)[0]), ssm.short_conv_bwd(few[0], w, None, some(dy))[0])
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("T,N", [(1, 16), (21, 5), (300, 16)])
+def test_scan_steps_masked_by_infinities(device, dtype, T, N):
+    """A step of softplus(-infinity), of the type's lowest value or of -300 is 0:
+    the token changes no state.  NaN stays NaN."""
+    p, dy, state, _ = scan_inputs(2, T, 12, N, 1, dtype, device, 41)
+    gone = torch.rand(2, T, 12, generator=gen(5)).to(device) < 0.4
+
+    def masked(value):
+        q = dict(p, dt=torch.where(gone, torch.full_like(p["dt"], value), p["dt"]))
+        y, last, saved = run_scan(q, state=state, want_state=True, save=True)
+        return [y, last, *run_scan_bwd(q, dy, saved)]
+
+    want = masked(-300.0)
+    assert all(bool(torch.isfinite(v).all()) for v in want)
+    for value in (-float("inf"), torch.finfo(dtype).min):
+        assert all(torch.equal(a, b) for a, b in zip(masked(value), want))
+    if T == 1:
+        one = lambda v: v[:, 0]  # noqa: E731
+        moved = state.clone()
+        y = ssm.state_scan_step(one(p["u"]), torch.full_like(one(p["dt"]), -float("inf")), p["a_log"], one(p["b"]),
+                                one(p["c"]), moved, p["skip"], one(p["z"]), p["dt_bias"])
+        assert torch.equal(moved, state) and bool(torch.isfinite(y).all())
+    p["dt"][0, 0, 3] = float("nan")
+    y = run_scan(p)[0]
+    assert bool(torch.isnan(y[0, :, 3]).all()) and bool(torch.isfinite(y[1]).all())
