@@ -22,11 +22,11 @@
 //
 // One read of the logits is the floor (20 us for 256 x 128000 fp32, less than a launch
 // for what a server usually asks).  Small calls are a chain of barriers: 64 x 32000 bf16
-// with top_k 50 and top_p takes 16.4 us, some 23000 cycles: 5000 reading, 4000 the bound,
-// 5000 the list, 5000 the word, the rest the cluster's six barriers.  Large ones are bound
+// with top_k 50 and top_p takes 16.4 us, some 21000 cycles: 5000 reading, 4000 the bound,
+// 5000 the list, 5000 the word, the rest the cluster's five barriers.  Large ones are bound
 // by the weights, 64-bit arithmetic of some 50 issue slots a warp and word and pass: 256 x
-// 128000 take 58 us for the largest word alone, 122 with top_k 40, 167 from all words
-// (one pass), 739 with a nucleus of thousands of words (four), of mixed settings 231-238.
+// 128000 take 58 us for the largest word alone, 118 with top_k 40, 165 from all words
+// (one pass), 740-750 with a nucleus of thousands of words (four), of mixed settings 231-241.
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -764,9 +764,12 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(Sampling a, int run,
         }
       }
       r.tell(IN_LIST, ok);
-      cluster.sync();
-      if (sh.told[IN_LIST]) {
-        if (rank) return;  // block 0 finds the word; waiting for it would take issue slots from others
+      // Block 0 finds the word: it need not wait for the others, which wait for its number to leave (staying
+      // until it is done would take issue slots from other rows).
+      if (ok) (void)cluster.barrier_arrive();
+      else cluster.sync();
+      if (ok || sh.told[IN_LIST]) {
+        if (rank) return;
         const int count = (int)sh.members;
         if (count <= SHORT) word_of_short_list(count, total, tokens + row);
         else word_of_list(count, total, ((u64)bound << 32) - (bound ? 1 : 0), best, words, tokens + row);
