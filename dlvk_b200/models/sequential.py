@@ -352,6 +352,12 @@ class Sequential(Model):
             if tuple(lengths.shape) != (B,) or bool((lengths < 1).any()) or bool((lengths > T).any()):
                 raise ValueError(f"generate: {B} lengths of 1 to {T} tokens")
             lengths = lengths.to(dev, torch.int32)
+
+        def last_token(x):
+            if lengths is None:
+                return x[:, -1:]
+            return torch.gather(x, 1, (lengths.long() - 1)[:, None, None].expand(-1, 1, x.shape[2]))
+
         training = self.is_training
         self.set_training(False)
         last_state = max((i for i, m in enumerate(inner) if m is not None), default=-1)
@@ -359,15 +365,17 @@ class Sequential(Model):
         try:
             with torch.no_grad():
                 states, x = {}, prompt
+                alone = max(last_state + 1, 1)  # what follows from here on, layers or the choice, needs the last token alone
                 for i, layer in enumerate(layers):
-                    if i == max(last_state + 1, 1):  # what follows needs the last token alone
-                        x = x[:, -1:] if lengths is None else torch.gather(
-                            x, 1, (lengths.long() - 1)[:, None, None].expand(-1, 1, x.shape[2]))
+                    if i == alone:
+                        x = last_token(x)
                     if inner[i] is not None:
                         y, states[i] = inner[i].prompt(x, lengths=lengths)
                         x = K.binary(x.contiguous(), y, K.BIN_ADD) if isinstance(layer, L.ResidualLayer) else y
                     else:
                         x = layer._forward(x.contiguous())
+                if alone == n:
+                    x = last_token(x)
                 for k in range(steps):
                     words[:, k] = sample_tokens(x[:, -1], uniform[:, k].contiguous(), temperature, top_k, top_p, min_p)
                     if k + 1 == steps:

@@ -1,0 +1,52 @@
+"""StateSpaceLayer and Sequential.generate in the cases at their borders: models
+that end in the layer itself."""
+import pytest
+import torch
+
+import dlvk_b200 as dl
+from dlvk_b200.models.sequential import Sequential
+
+DEVICES = [pytest.param("cpu"), pytest.param("cuda", marks=pytest.mark.gpu)]
+WORDS = 40
+
+
+def ending_in(what, device):
+    """A model whose last layer, before a Softmax or none, is `what`."""
+    m = Sequential(device, "fp32", seed=5)
+    m.add_embedding(WORDS, WORDS)
+    if what == "state space":
+        m.add_state_space(WORDS, residual=True)
+    elif what == "state space, softmax":
+        m.add_state_space(WORDS, residual=True).add_softmax()
+    elif what == "residual":
+        m.add_dense(WORDS, WORDS).add(dl.ResidualLayer(dl.StateSpaceLayer(WORDS, d_state=5)))
+    elif what == "two, dense":
+        m.add_state_space(WORDS, residual=True).add_state_space(WORDS, residual=True).add_dense(WORDS, WORDS)
+    elif what == "embedding, softmax":
+        m.add_softmax()
+    return m.build()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("what", ["state space", "state space, softmax", "residual", "two, dense", "embedding",
+                                  "embedding, softmax"])
+def test_generate_takes_the_last_token_that_counts(device, what):
+    """Every word of a padded batch is the likeliest after its sequence's own
+    tokens, by the whole model's logits of them.  The two ways make the same fp32
+    sums of at most 80 terms in other orders (3 2^-17 each on the GPU's split
+    products), three layers deep: a word may be another one of the likeliest
+    within 2^-8 of the largest logit."""
+    m = ending_in(what, device)
+    g = torch.Generator().manual_seed(3)
+    n = [7, 2, 1, 5]
+    prompt = torch.randint(0, WORDS, (4, 7), generator=g, dtype=torch.int32)
+    for i, k in enumerate(n):
+        prompt[i, k:] = (prompt[i, k - 1] + 1) % WORDS  # not the last word that counts
+    got = m.generate(prompt, 4, lengths=n, temperature=0.0)
+    m.set_training(False)
+    for i, k in enumerate(n):
+        seq = prompt[i, :k].tolist()
+        for word in got[i].tolist():
+            z = m.forward_logits(torch.tensor([seq], dtype=torch.int32)).detach()[0, -1].float().cpu()
+            assert float(z.max() - z[word]) <= 2.0 ** -8 * float(z.abs().max()), (i, seq, word, int(z.argmax()))
+            seq.append(word)
