@@ -966,7 +966,7 @@ class StateSpaceLayer(ModernLayer):
         xz = K.gemm(x2, self.w_in.value).reshape(B, T, 2 * self.width)
         v, last = SSM.short_conv_fwd(xz[..., :self.width], self.conv_weight.master, self.conv_bias.master, state=state,
                                      lengths=lengths, want_state=want_state, out_state=out_state)
-        p = K.gemm(v.reshape(B * T, self.width), self.w_x.value).reshape(B, T, -1)
+        p = K.gemm(v.reshape(B * T, self.width), self.w_x.value).reshape(B, T, self.w_x.shape[1])
         low, b, c = self.split(p)
         dt = K.gemm(low.flatten(0, 1), self.w_dt.value).reshape(B, T, self.width)
         return xz, v, low, b, c, dt, last

@@ -466,7 +466,7 @@ class StateSpaceFn(torch.autograd.Function):
         wgrad(m.w_in, x2.t(), dxz2)
         dx = None
         if ctx.needs_input_grad[0]:
-            dx = K.gemm(dxz2, m.w_in.value.t(), residual=g if m.residual else None).reshape(B, T, -1)
+            dx = K.gemm(dxz2, m.w_in.value.t(), residual=g if m.residual else None).reshape(B, T, m.d_model)
         for p in (m.w_out, m.skip, m.a_log, m.dt_bias, m.w_dt, m.w_x, m.conv_bias, m.conv_weight, m.w_in):
             p.grad_ready()
         return dx, None, None

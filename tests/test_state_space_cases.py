@@ -50,3 +50,24 @@ def test_generate_takes_the_last_token_that_counts(device, what):
             z = m.forward_logits(torch.tensor([seq], dtype=torch.int32)).detach()[0, -1].float().cpu()
             assert float(z.max() - z[word]) <= 2.0 ** -8 * float(z.abs().max()), (i, seq, word, int(z.argmax()))
             seq.append(word)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("B,T", [(0, 5), (2, 0), (0, 0)])
+@pytest.mark.parametrize("groups", [1, 2])
+def test_layer_of_no_sequences_or_tokens(device, B, T, groups):
+    dl.manual_seed(3)
+    layer = dl.StateSpaceLayer(16, groups=groups, residual=True)
+    layer.to(device, torch.float32)
+    x = torch.zeros(B, T, 16, device=device)
+    y = layer.forward(x)
+    assert y.shape == (B, T, 16)
+    assert layer.backward(torch.zeros_like(y)).shape == (B, T, 16)
+    assert all(not p.grad.any() for p in layer.parameters())
+    start = layer.init_state(B)
+    start.conv.normal_()
+    start.scan.normal_()
+    y, state = layer.prompt(x, start)
+    assert y.shape == (B, T, 16) and torch.equal(state.conv, start.conv) and torch.equal(state.scan, start.scan)
+    if B == 0:
+        assert layer.step(x.new_zeros(0, 16), state).shape == (0, 16)
