@@ -26,6 +26,7 @@
 // more leave too few warps: two channels a thread, whose loads of b and c are
 // shared, and blocks of 64 threads were both slower.
 #include <algorithm>
+#include <cfloat>
 #include <type_traits>
 
 #include "dlvk/seq.h"
@@ -233,11 +234,17 @@ __device__ __forceinline__ void store_states(const Quad& q, float* p, int n0, in
       if (n0 + i < N) p[i] = h[i];
   }
 }
-// -exp(a_log) of a thread's states, 0 past N.
+// -exp(a_log), no further than fp32's lowest value: an infinity times a step of 0, which
+// tokens that do not count have, is not a number.  Steps past 2^-120 see no difference.
+__device__ __forceinline__ float rate_of(float a_log, float scale) {
+  const float r = expf(a_log) * scale;
+  return r > FLT_MAX ? -FLT_MAX : -r;
+}
+// Those of a thread's states, 0 past N.
 __device__ __forceinline__ Quad load_rates(const StateScan& a, int d, int n0, float scale) {
   float r[NS];
 #pragma unroll
-  for (int i = 0; i < NS; ++i) r[i] = n0 + i < a.N ? -expf(a.a_log[(int64_t)d * a.N + n0 + i]) * scale : 0.f;
+  for (int i = 0; i < NS; ++i) r[i] = n0 + i < a.N ? rate_of(a.a_log[(int64_t)d * a.N + n0 + i], scale) : 0.f;
   return {{pack(r[0], r[1]), pack(r[2], r[3])}};
 }
 
@@ -400,7 +407,7 @@ __global__ void __launch_bounds__(256) scan_join_kernel(StateScan a, Pieces piec
   const int64_t dn = (int64_t)a.D * a.N, i = blockIdx.x * 256LL + threadIdx.x;
   if (i >= a.B * dn) return;
   const int64_t b = i / dn, e = i % dn, d = e / a.N;
-  const float rate = -expf(a.a_log[e]);
+  const float rate = rate_of(a.a_log[e], 1.f);
   float carry = !BACK && a.state ? a.state[i] : 0.f;
   // eight pieces' loads ahead of the stores, which might be to the same place for all that the compiler knows
   constexpr int AHEAD = 8;
@@ -850,7 +857,9 @@ __global__ void __launch_bounds__(THREADS, 4) scan_bwd_kernel(StateScan a, const
       for (int j = 0; j < V; ++j) {
         const float uj = u.get(j), zj = z.get(j), q = (&q4.x)[j], v = (&v4.x)[j], skip = (&skip4.x)[j];
         du.set(j, here ? fmaf(v, (&s4.x)[j], q * skip) : 0.f);
-        const float dr = here ? fmaf(v, uj, (&d4.x)[j]) * sigmoid(dt.get(j) + (&bias4.x)[j]) : 0.f;
+        // a step of 0 has no slope, however large the rates are (an infinite sum times it is not a number)
+        const float slope = sigmoid(dt.get(j) + (&bias4.x)[j]);
+        const float dr = here && slope != 0.f ? fmaf(v, uj, (&d4.x)[j]) * slope : 0.f;
         ddt.set(j, dr);
         (&ds.x)[j] = fmaf(q, uj, (&ds.x)[j]);
         (&db.x)[j] += dr;

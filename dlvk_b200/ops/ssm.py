@@ -176,7 +176,8 @@ def _scan_parts(u, dt, a_log, b, c, skip, z, dt_bias, lengths):
     step = _where(counted, torch.clamp(raw, min=0) + torch.log1p(torch.exp(-raw.abs())))
     wide = lambda v: _where(counted, v.contiguous().reshape(B, T, groups * n).float()).reshape(B, T, groups, 1, n)  # noqa: E731
     uf = _where(counted, u.contiguous().float())
-    return counted, groups, raw, step, uf, wide(b), wide(c), -torch.exp(a_log)
+    # (no further than fp32's lowest value: an infinity times a step of 0 is not a number)
+    return counted, groups, raw, step, uf, wide(b), wide(c), -torch.exp(a_log).clamp(max=torch.finfo(torch.float32).max)
 
 
 def _scan_states(step, u, a, b, groups, state, T):
@@ -274,7 +275,8 @@ def state_scan_bwd(u, dt, a_log, b, c, dy, saved, skip=None, z=None, dt_bias=Non
         through = carry * hs[t]
         through_a[:, t] = (through * rate).sum(-1).reshape(B, D)
         ga += (through * split(step[:, t])).sum(0)
-    draw = _where(counted, (through_a + into * uf) * torch.sigmoid(raw))
+    slope = torch.sigmoid(raw)  # 0 for a step of 0, however large the rates are
+    draw = _where(counted, torch.where(slope == 0, slope, (through_a + into * uf) * slope))
     gu = into * step + (q * skip if skip is not None else 0.0)
     gz = None
     if z is not None:
