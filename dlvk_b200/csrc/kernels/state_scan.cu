@@ -1066,12 +1066,11 @@ int64_t state_scan_bwd_scratch_floats(const StateScan& a) {
 void state_scan_bwd(const StateScan& a, const float* saved, SeqRef dy, const StateScanGrads& g, float* scratch,
                     cudaStream_t s) {
   check(a);
-  if (a.D == 0) return;
   Pieces p = pieces_of(a, BWD_BLOCKS, BWD_PIECES);
   float* part_bc = scratch;
   float* part_d = part_bc + part_bc_floats(a);
   float* ends = part_d + part_d_floats(a, p);
-  if (a.B > 0) {
+  if (a.B > 0 && a.D > 0) {
     const bool w = wide_operands(a) && aligned(dy, a.type) && aligned(g.du, a.type) && aligned(g.ddt, a.type) &&
                    aligned(g.dz, a.type) && aligned16(saved);
     by_kind(a, w, [&](auto type, auto lanes, auto wide) {
@@ -1081,17 +1080,17 @@ void state_scan_bwd(const StateScan& a, const float* saved, SeqRef dy, const Sta
       join_pieces<T, L, W, true>(a, dy, p, ends, s);
       launch(scan_bwd_kernel<T, L, W>, sizeof(BwdShared<T, L, W>), a, p.count, s, saved, dy, g, part_bc, part_d, p);
     });
-    const int64_t total = part_bc_floats(a) / tiles_of(a);
-    if (total > 0) {
-      const unsigned blocks = (unsigned)std::min<int64_t>((total + 255) / 256, 148 * 16);
-      const int states = NS * lanes_of(a.N);
-      if (a.type == DType::BF16)
-        join_bc_kernel<__nv_bfloat16><<<blocks, 256, 0, s>>>(part_bc, tiles_of(a), a.B, a.T, a.G, a.N, states, g.db, g.dc);
-      else
-        join_bc_kernel<float><<<blocks, 256, 0, s>>>(part_bc, tiles_of(a), a.B, a.T, a.G, a.N, states, g.db, g.dc);
-      DLVK_POST_LAUNCH();
-    }
   }
+  const int states = NS * lanes_of(a.N);
+  if (const int64_t total = a.B * a.T * a.G * 2 * states) {  // without channels too: sums of no tiles
+    const unsigned blocks = (unsigned)std::min<int64_t>((total + 255) / 256, 148 * 16);
+    if (a.type == DType::BF16)
+      join_bc_kernel<__nv_bfloat16><<<blocks, 256, 0, s>>>(part_bc, tiles_of(a), a.B, a.T, a.G, a.N, states, g.db, g.dc);
+    else
+      join_bc_kernel<float><<<blocks, 256, 0, s>>>(part_bc, tiles_of(a), a.B, a.T, a.G, a.N, states, g.db, g.dc);
+    DLVK_POST_LAUNCH();
+  }
+  if (a.D == 0) return;
   join_d_kernel<<<(unsigned)(((int64_t)a.D * (a.N + 2) + 255) / 256), 256, 0, s>>>(part_d, a.B * p.count, a.D, a.N, g);
   DLVK_POST_LAUNCH();
 }

@@ -41,3 +41,16 @@ def test_scan_of_rates_past_fp32(device, dtype, T, N, G):
     nan["a_log"][5] = math.nan
     y = run_scan(nan, state=state)[0]
     assert bool(torch.isnan(y[..., 5]).all()) and bool(torch.isfinite(y[..., 6:]).all())
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("G", [1, 3])
+def test_scan_of_no_channels(device, dtype, G):
+    """No channel reads b and c: their gradients are zeros, whatever was there."""
+    p, dy, state, _ = scan_inputs(2, 19, 0, 5, G, dtype, device)
+    y, last, saved = run_scan(p, state=state, want_state=True, save=True)
+    assert y.shape == (2, 19, 0) and last.shape == (2, 0, 5)
+    given = {k: torch.full_like(p["b"], 7.0) for k in ("db", "dc")}
+    grads = run_scan_bwd(p, dy, saved, **given)
+    assert not given["db"].any() and not given["dc"].any() and grads.da_log.shape == (0, 5)
