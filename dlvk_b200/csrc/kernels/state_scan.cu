@@ -131,7 +131,7 @@ __device__ __forceinline__ void fetch_four(Four<T>* dst, const T* p, const void*
 }
 
 __device__ __forceinline__ int64_t length_of(const StateScan& a, int64_t b) {
-  return a.lengths ? min(max((int64_t)a.lengths[b], (int64_t)0), a.T) : a.T;
+  return a.lengths ? min(max((int64_t)a.lengths[b] - a.first, (int64_t)0), a.T) : a.T;
 }
 
 // The channels of a block, CH of one group of one sequence.
@@ -296,6 +296,13 @@ struct Pieces {
   float* steps = nullptr;   // [B][count][D]: sum of s
 };
 
+// Of a backward pass that goes through the tokens part by part, [B][D][N] (may be the
+// same memory): what the part behind passes on (null: zeros), and to the one before.
+struct Carry {
+  const float* in = nullptr;
+  float* out = nullptr;
+};
+
 template <typename T, int L, bool WIDE>
 struct EndsShared {
   static constexpr int CH = THREADS / L, PER = Mine<CH>::PER;
@@ -403,12 +410,12 @@ __global__ void __launch_bounds__(THREADS) scan_ends_kernel(StateScan a, SeqRef 
 
 // ends: from what a piece ends with to what the one before it (BACK: behind it) passes on to it.
 template <bool BACK>
-__global__ void __launch_bounds__(256) scan_join_kernel(StateScan a, Pieces pieces) {
+__global__ void __launch_bounds__(256) scan_join_kernel(StateScan a, Pieces pieces, Carry pass) {
   const int64_t dn = (int64_t)a.D * a.N, i = blockIdx.x * 256LL + threadIdx.x;
   if (i >= a.B * dn) return;
   const int64_t b = i / dn, e = i % dn, d = e / a.N;
   const float rate = rate_of(a.a_log[e], 1.f);
-  float carry = !BACK && a.state ? a.state[i] : 0.f;
+  float carry = BACK ? (pass.in ? pass.in[i] : 0.f) : a.state ? a.state[i] : 0.f;
   // eight pieces' loads ahead of the stores, which might be to the same place for all that the compiler knows
   constexpr int AHEAD = 8;
   for (int j0 = 0; j0 < pieces.count; j0 += AHEAD) {
@@ -428,6 +435,7 @@ __global__ void __launch_bounds__(256) scan_join_kernel(StateScan a, Pieces piec
       carry = fmaf(expf(rate * steps[j]), carry, own[j]);
     }
   }
+  if (BACK && pass.out) pass.out[i] = carry;
 }
 
 // ---------------------------------------------------------------- forward
@@ -676,11 +684,12 @@ struct BwdShared {
 // 67% busy; 16 warps an SM.  Sums over channels as tf32 products of ones and the values
 // took longer (some 9 cycles a product of 16 x 8 x 4) and needed two for fp32.
 //
+// saved: `kept` spans a sequence.
 // part_bc [tiles of a group][B][T][G][2][NS L]; part_d [B][pieces][D][N + 2]: da, dskip, ddt_bias.
 template <typename T, int L, bool WIDE>
-__global__ void __launch_bounds__(THREADS, 4) scan_bwd_kernel(StateScan a, const float* __restrict__ saved, SeqRef dy,
-                                                              StateScanGrads g, float* __restrict__ part_bc,
-                                                              float* __restrict__ part_d, Pieces pieces) {
+__global__ void __launch_bounds__(THREADS, 4) scan_bwd_kernel(StateScan a, const float* __restrict__ saved, int64_t kept,
+                                                              SeqRef dy, StateScanGrads g, float* __restrict__ part_bc,
+                                                              float* __restrict__ part_d, Pieces pieces, Carry pass) {
   using States = SpanStates<T, L, WIDE, 2>;
   constexpr int CH = THREADS / L, ROW = 2 * NS * L;
   extern __shared__ __align__(16) char raw[];
@@ -697,7 +706,8 @@ __global__ void __launch_bounds__(THREADS, 4) scan_bwd_kernel(StateScan a, const
   const int64_t piece = tile.b * pieces.count + blockIdx.y;
   if (real) {
     rate = load_rates(a, tile.c0 + ch, n0, 1.f);
-    if (pieces.ends) ga = load_states<WIDE>(pieces.ends + (piece * a.D + tile.c0 + ch) * a.N + n0, n0, a.N);
+    const float* in = pieces.ends ? pieces.ends : pass.in;  // (of one piece: passed on as it is)
+    if (in) ga = load_states<WIDE>(in + (piece * a.D + tile.c0 + ch) * a.N + n0, n0, a.N);
   }
   for (int j = threadIdx.x; j < CH; j += THREADS) {
     sh.bias[j] = a.dt_bias && j < tile.count ? a.dt_bias[tile.c0 + j] : 0.f;
@@ -719,7 +729,7 @@ __global__ void __launch_bounds__(THREADS, 4) scan_bwd_kernel(StateScan a, const
     }
     States::fetch(st.bc, a.b, a.c, tile.b, tile.group, a.N, t0, n);
     fetch_four<float, WIDE>(reinterpret_cast<Four<float>*>(&st.h[threadIdx.x]),
-                            saved + ((tile.b * spans + k) * a.D + tile.c0 + ch) * a.N + n0, saved, real ? a.N - n0 : 0);
+                            saved + ((tile.b * kept + k) * a.D + tile.c0 + ch) * a.N + n0, saved, real ? a.N - n0 : 0);
   };
   for (int64_t k = to; k < end; ++k) {  // behind the sequence
     const int64_t t0 = k * SPAN;
@@ -886,6 +896,7 @@ __global__ void __launch_bounds__(THREADS, 4) scan_bwd_kernel(StateScan a, const
     }
     // (the barrier after the next span's elements is between these reads and what comes to their places)
   }
+  if (real && pass.out && !pieces.ends) store_states<WIDE>(ga, pass.out + (piece * a.D + tile.c0 + ch) * a.N + n0, n0, a.N);
   const Quad da = load_quad(&sh.da[threadIdx.x].x);
   if (real) store_states<false>({{mul2(da.v[0], rate.v[0]), mul2(da.v[1], rate.v[1])}},
                          part_d + (piece * a.D + tile.c0 + ch) * (a.N + 2) + n0, n0, a.N);
@@ -1009,19 +1020,74 @@ Pieces pieces_of(const StateScan& a, int blocks_an_sm, int least) {
   return p;
 }
 int64_t pieces_floats(const StateScan& a, const Pieces& p) { return p.count > 1 ? a.B * p.count * a.D * (a.N + 1) : 0; }
-int64_t part_d_floats(const StateScan& a, const Pieces& p) {  // whole fours: the ends lie behind them
-  return (a.B * p.count * a.D * (a.N + 2) + 3) / 4 * 4;
-}
+int64_t part_d_floats(const StateScan& a, const Pieces& p) { return a.B * p.count * a.D * (a.N + 2); }
 
 template <typename T, int L, bool W, bool BACK>
-void join_pieces(const StateScan& a, SeqRef dy, Pieces& p, float* scratch, cudaStream_t s) {
+void join_pieces(const StateScan& a, SeqRef dy, Pieces& p, Carry pass, float* scratch, cudaStream_t s) {
   if (p.count == 1) return;
   p.ends = scratch;
   p.steps = scratch + a.B * p.count * a.D * a.N;
   launch(scan_ends_kernel<T, L, W, BACK>, sizeof(EndsShared<T, L, W>), a, p.count, s, dy, p);
-  scan_join_kernel<BACK><<<(unsigned)((a.B * a.D * a.N + 255) / 256), 256, 0, s>>>(a, p);
+  scan_join_kernel<BACK><<<(unsigned)((a.B * a.D * a.N + 255) / 256), 256, 0, s>>>(a, p, pass);
   DLVK_POST_LAUNCH();
 }
+
+// The sums by tile (part_bc) have a row of 8 L floats a tile and token: at 64 states 32 times
+// bf16 operands, 17 GB for 65536 tokens x 4096 channels.  So a backward pass goes in parts whose
+// sums fit the room of the states that the forward pass kept, or 1 GB.  Of bf16 and 64 states
+// 64 x 512 x 2048 takes 7068 us whole and 7206 in parts of whole sequences (7252 of some spans of all
+// of them; 256 x 128 x 2048 7206, 7228 and 8030).  Parts of fewer blocks than PART_BLOCKS leave SMs
+// without work at their ends: below it they are some spans of all sequences, from the last on
+// (32 x 4096 x 512 7230 whole, 7282 so, 9546 in whole sequences).
+struct Parts {
+  int64_t sequences, spans;  // of a part
+  bool along = false;        // the tokens: what crosses a border is carried
+};
+constexpr int64_t PART_FLOATS = 256LL << 20, PART_BLOCKS = 148 * 8;
+Parts parts_of(const StateScan& a) {
+  const int64_t spans = (a.T + SPAN - 1) / SPAN, tiles = a.G * tiles_of(a), span = (int64_t)SPAN * 2 * NS * lanes_of(a.N);
+  const int64_t room = std::max(PART_FLOATS, a.B * spans * a.D * a.N);
+  Parts p{std::max<int64_t>(a.B, 1), std::max<int64_t>(spans, 1)};
+  if (a.B * tiles * spans * span <= room) return p;
+  const auto equal = [](int64_t all, int64_t most) {
+    const int64_t n = (all + most - 1) / most;
+    return (all + n - 1) / n;
+  };
+  const int64_t whole = room / (spans * span);  // blocks whose sums of all tokens fit
+  if (whole >= std::max(PART_BLOCKS, tiles)) {
+    p.sequences = equal(a.B, whole / tiles);
+  } else {
+    p.spans = equal(spans, std::max<int64_t>(1, room / (a.B * tiles * span)));
+    p.along = p.spans < spans;
+  }
+  return p;
+}
+SeqRef from(SeqRef r, DType type, int64_t b, int64_t t) {
+  if (r.p) r.p = static_cast<char*>(r.p) + (b * r.batch + t * r.token) * (type == DType::BF16 ? 2 : 4);
+  return r;
+}
+// f(the part's operands, its first sequence and span), the last tokens first.
+template <typename F>
+void each_part(const StateScan& a, const Parts& p, F&& f) {
+  const int64_t spans = std::max<int64_t>(1, (a.T + SPAN - 1) / SPAN);
+  for (int64_t b = 0; b < a.B; b += p.sequences)
+    for (int64_t k = (spans - 1) / p.spans * p.spans; k >= 0; k -= p.spans) {
+      StateScan v = a;
+      const int64_t t = k * SPAN;
+      v.B = std::min(p.sequences, a.B - b);
+      v.T = std::min(p.spans * SPAN, a.T - t);
+      v.first = a.first + t;
+      for (SeqRef* r : {&v.u, &v.dt, &v.z, &v.b, &v.c}) *r = from(*r, a.type, b, t);
+      if (v.lengths) v.lengths += b;
+      f(v, b, k);
+    }
+}
+// Scratch of a backward pass, in floats: sums by tile of one part, rows of sums for the
+// parameters of all parts, what is carried, ends of one part's pieces.
+struct BwdScratch {
+  int64_t bc = 0, d = 0, carry = 0, ends = 0;
+  int64_t all() const { return bc + d + carry + ends; }
+};
 }  // namespace
 
 // Four sequences a thread where that still makes this many blocks: 64 x 1536 channels of 16
@@ -1052,46 +1118,79 @@ void state_scan_fwd(const StateScan& a, SeqRef y, float* out_state, float* saved
       return;
     }
     Pieces p = pieces_of(a, FWD_BLOCKS, FWD_PIECES);
-    join_pieces<T, L, W, false>(a, {}, p, scratch, s);
+    join_pieces<T, L, W, false>(a, {}, p, {}, scratch, s);
     launch(scan_fwd_kernel<T, L, W>, sizeof(FwdShared<T, L, W>), a, p.count, s, y, out_state, saved, p);
   });
 }
 
+namespace {
+BwdScratch bwd_scratch(const StateScan& a, const Parts& parts) {
+  const auto fours = [](int64_t n) { return (n + 3) / 4 * 4; };
+  BwdScratch r;
+  each_part(a, parts, [&](const StateScan& v, int64_t, int64_t) {
+    const Pieces p = pieces_of(v, BWD_BLOCKS, BWD_PIECES);
+    r.bc = std::max(r.bc, part_bc_floats(v));
+    r.d += part_d_floats(v, p);
+    r.ends = std::max(r.ends, pieces_floats(v, p));
+  });
+  r.d = fours(r.d);
+  if (parts.along) r.carry = fours(a.B * a.D * a.N);
+  return r;
+}
+void join_bc(const StateScan& a, const float* part_bc, const StateScanGrads& g, cudaStream_t s) {
+  const int states = NS * lanes_of(a.N);
+  const int64_t total = a.B * a.T * a.G * 2 * states;
+  if (total == 0) return;
+  const unsigned blocks = (unsigned)std::min<int64_t>((total + 255) / 256, 148 * 16);
+  if (a.type == DType::BF16)
+    join_bc_kernel<__nv_bfloat16><<<blocks, 256, 0, s>>>(part_bc, tiles_of(a), a.B, a.T, a.G, a.N, states, g.db, g.dc);
+  else
+    join_bc_kernel<float><<<blocks, 256, 0, s>>>(part_bc, tiles_of(a), a.B, a.T, a.G, a.N, states, g.db, g.dc);
+  DLVK_POST_LAUNCH();
+}
+}  // namespace
+
 int64_t state_scan_bwd_scratch_floats(const StateScan& a) {
   check(a);
-  const Pieces p = pieces_of(a, BWD_BLOCKS, BWD_PIECES);
-  return part_bc_floats(a) + part_d_floats(a, p) + pieces_floats(a, p);
+  return bwd_scratch(a, parts_of(a)).all();
 }
 
 void state_scan_bwd(const StateScan& a, const float* saved, SeqRef dy, const StateScanGrads& g, float* scratch,
                     cudaStream_t s) {
   check(a);
-  Pieces p = pieces_of(a, BWD_BLOCKS, BWD_PIECES);
+  if (a.D == 0) return join_bc(a, nullptr, g, s);  // sums of no tiles
+  const Parts parts = parts_of(a);
+  const BwdScratch room = bwd_scratch(a, parts);
   float* part_bc = scratch;
-  float* part_d = part_bc + part_bc_floats(a);
-  float* ends = part_d + part_d_floats(a, p);
-  if (a.B > 0 && a.D > 0) {
-    const bool w = wide_operands(a) && aligned(dy, a.type) && aligned(g.du, a.type) && aligned(g.ddt, a.type) &&
-                   aligned(g.dz, a.type) && aligned16(saved);
-    by_kind(a, w, [&](auto type, auto lanes, auto wide) {
+  float* part_d = part_bc + room.bc;
+  float* carry = part_d + room.d;
+  float* ends = carry + room.carry;
+  const int64_t spans = (a.T + SPAN - 1) / SPAN;
+  int64_t rows = 0;
+  each_part(a, parts, [&](const StateScan& v, int64_t b, int64_t k) {
+    Pieces p = pieces_of(v, BWD_BLOCKS, BWD_PIECES);
+    Carry pass;
+    if (parts.along && k + parts.spans < spans) pass.in = carry;
+    if (parts.along && k > 0) pass.out = carry;
+    const auto of = [&](const SeqRef& r) { return from(r, a.type, b, k * SPAN); };
+    StateScanGrads h = g;
+    for (SeqRef* r : {&h.du, &h.ddt, &h.dz, &h.db, &h.dc}) *r = of(*r);
+    const SeqRef go = of(dy);
+    const float* kept = saved + (b * spans + k) * a.D * a.N;
+    const bool w = wide_operands(v) && aligned(go, a.type) && aligned(h.du, a.type) && aligned(h.ddt, a.type) &&
+                   aligned(h.dz, a.type) && aligned16(kept);
+    by_kind(v, w, [&](auto type, auto lanes, auto wide) {
       using T = decltype(type);
       constexpr int L = decltype(lanes)::value;
       constexpr bool W = decltype(wide)::value;
-      join_pieces<T, L, W, true>(a, dy, p, ends, s);
-      launch(scan_bwd_kernel<T, L, W>, sizeof(BwdShared<T, L, W>), a, p.count, s, saved, dy, g, part_bc, part_d, p);
+      join_pieces<T, L, W, true>(v, go, p, pass, ends, s);
+      launch(scan_bwd_kernel<T, L, W>, sizeof(BwdShared<T, L, W>), v, p.count, s, kept, spans, go, h, part_bc,
+             part_d + rows * a.D * (a.N + 2), p, pass);
     });
-  }
-  const int states = NS * lanes_of(a.N);
-  if (const int64_t total = a.B * a.T * a.G * 2 * states) {  // without channels too: sums of no tiles
-    const unsigned blocks = (unsigned)std::min<int64_t>((total + 255) / 256, 148 * 16);
-    if (a.type == DType::BF16)
-      join_bc_kernel<__nv_bfloat16><<<blocks, 256, 0, s>>>(part_bc, tiles_of(a), a.B, a.T, a.G, a.N, states, g.db, g.dc);
-    else
-      join_bc_kernel<float><<<blocks, 256, 0, s>>>(part_bc, tiles_of(a), a.B, a.T, a.G, a.N, states, g.db, g.dc);
-    DLVK_POST_LAUNCH();
-  }
-  if (a.D == 0) return;
-  join_d_kernel<<<(unsigned)(((int64_t)a.D * (a.N + 2) + 255) / 256), 256, 0, s>>>(part_d, a.B * p.count, a.D, a.N, g);
+    join_bc(v, part_bc, h, s);
+    rows += v.B * p.count;
+  });
+  join_d_kernel<<<(unsigned)(((int64_t)a.D * (a.N + 2) + 255) / 256), 256, 0, s>>>(part_d, rows, a.D, a.N, g);
   DLVK_POST_LAUNCH();
 }
 

@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from dlvk_b200.ops import ssm
-from test_sequence_ops import DEVICES, DTYPES, limits, near, run_scan, run_scan_bwd, scan_check, scan_inputs, scan_ref
+from test_sequence_ops import DEVICES, DTYPES, HALF, limits, near, run_scan, run_scan_bwd, scan_check, scan_inputs, scan_ref
 
 
 @pytest.mark.parametrize("device", DEVICES)
@@ -54,3 +54,139 @@ def test_scan_of_no_channels(device, dtype, G):
     given = {k: torch.full_like(p["b"], 7.0) for k in ("db", "dc")}
     grads = run_scan_bwd(p, dy, saved, **given)
     assert not given["db"].any() and not given["dc"].any() and grads.da_log.shape == (0, 5)
+
+
+def scan_ref_wide(p, dy, n, absolute=False):
+    """The gradients of test_sequence_ops.scan_ref, from a state of zeros, for many
+    sequences and tokens at once: in 64 bits where the tensors are.  With `absolute`
+    the magnitudes of all products, and how far rounded decays and running sums
+    move them: a decay of argument x is off by 2^-22 + 2^-21 x of itself, as in
+    test_sequence_ops, a running sum by 2^-23 a token (its product and its sum)."""
+    m = (lambda v: v.abs()) if absolute else (lambda v: v)
+    p = {k: v.double() for k, v in p.items()}
+    B, T, D = p["u"].shape
+    N = p["a_log"].shape[1]
+    b, c = (v[:, :, None] if v.dim() == 3 else v for v in (p["b"], p["c"]))
+    G = b.shape[2]
+    ends = n if n is not None else torch.full((B,), T, device=dy.device)
+    on = (torch.arange(T, device=dy.device)[None, :] < ends[:, None])[..., None].double()
+    raw = p["dt"] + p["dt_bias"]
+    s = torch.logaddexp(raw, torch.zeros_like(raw)) * on
+    A = -torch.exp(p["a_log"])
+    sz = torch.sigmoid(p["z"])
+    dy = m(dy.double()) * on
+    q = dy * m(p["z"]) * sz
+    wide = lambda v: m(v).repeat_interleave(D // G, 1)  # [B, G, N] -> [B, D, N]  # noqa: E731
+    group = lambda v: v.reshape(B, G, D // G, N).sum(2)  # noqa: E731
+    su = m(s * p["u"])
+    hs = torch.zeros(T + 1, B, D, N, dtype=torch.float64, device=dy.device)
+    off = torch.zeros_like(hs) if absolute else None
+    step, lost = 2.0 ** -23, lambda x: 2.0 ** -22 - 2.0 ** -21 * x
+    for t in range(T):
+        x = s[:, t, :, None] * A
+        hs[t + 1] = torch.exp(x) * hs[t] + su[:, t, :, None] * wide(b[:, t])
+        if absolute:
+            off[t + 1] = torch.exp(x) * (off[t] + hs[t] * lost(x)) + step * hs[t + 1]
+    got = {k: torch.zeros_like(v) for k, v in p.items()}
+    gb, gc = got["b"].view(b.shape), got["c"].view(c.shape)
+    pre, v, through_a = (torch.zeros_like(s) for _ in range(3))
+    carry = torch.zeros_like(hs[0])
+    err = {k: torch.zeros_like(v) for k, v in p.items()}
+    eb, ec = err["b"].view(b.shape), err["c"].view(c.shape)
+    epre, ev, ethrough_a, ecarry = (torch.zeros_like(w) for w in (s, s, s, carry))
+    for t in range(T - 1, -1, -1):
+        wb, wc, qt, sut, st = wide(b[:, t]), wide(c[:, t]), q[:, t, :, None], su[:, t, :, None], s[:, t, :, None]
+        g, x = wc * qt + carry, st * A
+        a = torch.exp(x)
+        gc[:, t], gb[:, t] = group(hs[t + 1] * qt), group(g * sut)
+        pre[:, t], v[:, t] = (hs[t + 1] * wc).sum(-1), (g * wb).sum(-1)
+        carry = g * a
+        through = carry * hs[t]
+        through_a[:, t] = (through * m(A)).sum(-1)
+        got["a_log"] += (through * st).sum(0) * m(A)
+        if absolute:
+            eg = ecarry + step * g
+            ec[:, t], eb[:, t] = group(off[t + 1] * qt), group(eg * sut)
+            epre[:, t], ev[:, t] = (off[t + 1] * wc).sum(-1), (eg * wb).sum(-1)
+            ecarry = a * (eg + g * lost(x))
+            e = ecarry * hs[t] + carry * off[t]
+            ethrough_a[:, t] = (e * m(A)).sum(-1)
+            err["a_log"] += (e * st).sum(0) * m(A)
+
+    def close(out, pre, v, through_a, extra):
+        u, skip = m(p["u"]), m(p["skip"]) * extra
+        out["u"] = (v * s + q * skip) * on
+        out["dt"] = (through_a + v * u) * torch.sigmoid(raw) * on
+        out["z"] = dy * (pre + skip * u) * sz * (1 + m(p["z"]) * (1 - sz))
+        out["skip"], out["dt_bias"] = (q * u).sum((0, 1)) * extra, out["dt"].sum((0, 1))
+        return out
+
+    got = close(got, pre, v, through_a, 1.0)
+    return got, close(err, epre, ev, ethrough_a, 0.0) if absolute else None
+
+
+@pytest.mark.parametrize("G", [1, 3])
+def test_wide_reference(G):
+    p, dy, _, n = scan_inputs(3, 14, 12, 5, G, torch.float32, "cpu", 4, lengths=True)
+    for a in (False, True):
+        want, (got, err) = scan_ref(p, dy, None, n, absolute=a)[2], scan_ref_wide(p, dy, n, absolute=a)
+        for k in got:
+            assert bool(((got[k] - want[k]).abs() <= 1e-12 * (1 + want[k].abs())).all()), k
+            assert not a or bool((err[k] <= 2.0 ** -12 * got[k]).all())
+
+
+def wide_check(p, dy, n, saved):
+    """Gradients against scan_ref_wide: what rounded decays and running sums move, 24
+    other roundings and sigmoids of 2^-17, the terms of the longest sum (states of a
+    row; channels for b and c; tokens for the parameters, whose sums over sequences
+    are in 64 bits), and the rounding to the type."""
+    grads = run_scan_bwd(p, dy, saved, lengths=n)
+    want, _ = scan_ref_wide(p, dy, n)
+    mag, err = scan_ref_wide(p, dy, n, absolute=True)
+    B, T, D = dy.shape
+    N = p["a_log"].shape[1]
+    terms = {"b": N + D, "c": N + D, "a_log": N + T, "skip": N + T, "dt_bias": N + T}
+    for k in want:
+        got = getattr(grads, "d" + k)
+        off = (got.double() - want[k]).abs()
+        lim = err[k] + (2.0 ** -17 + (24 + terms.get(k, N)) * 2.0 ** -24) * mag[k]
+        lim += HALF[got.dtype] * (want[k].abs() + lim) + 1e-30
+        assert bool((off <= lim).all()), f"{k}: off by {float((off / lim).max()):.3g} of the limit"
+        del off, lim
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_scan_gradients_by_the_wide_reference(device, dtype):
+    p, dy, _, n = scan_inputs(5, 70, 40, 33, 2, dtype, device, 3, lengths=True)
+    wide_check(p, dy, n, run_scan(p, lengths=n, save=True)[2])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("B,T,D,N,G", [
+    (4, 8300, 520, 33, 1),    # some spans of all sequences at a time, one piece
+    (4, 8300, 522, 36, 2),    # the same, groups and rows that are no whole fours
+    (1, 10700, 1576, 64, 1),  # the same, in pieces
+    (4000, 9, 264, 64, 1),    # some sequences at a time
+    (170, 400, 1023, 20, 1),  # the same, fewer states
+])
+def test_scan_gradients_in_parts(dtype, B, T, D, N, G):
+    """Sums by tile past the room that a backward pass takes: it goes part by part,
+    with the gradients of the formula, and with no more memory than its outputs,
+    the kept states or 1 GB, and a quarter of that for the parameters' sums."""
+    p, dy, _, _ = scan_inputs(B, T, D, N, G, dtype, "cuda", B + T)
+    p["dt_bias"] -= 1.0
+    n = torch.randint(0, T + 1, (B,), generator=torch.Generator().manual_seed(7)).to(torch.int32).cuda()
+    n[0] = T
+    saved = run_scan(p, lengths=n, save=True)[2]
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    grads = run_scan_bwd(p, dy, saved, lengths=n)
+    torch.cuda.synchronize()
+    taken = torch.cuda.max_memory_allocated() - before
+    outputs = sum(v.numel() * v.element_size() for v in grads)
+    del grads
+    assert taken <= outputs + 1.25 * max(1 << 30, saved.numel() * 4)
+    wide_check(p, dy, n, saved)
