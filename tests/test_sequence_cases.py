@@ -190,3 +190,98 @@ def test_scan_gradients_in_parts(dtype, B, T, D, N, G):
     del grads
     assert taken <= outputs + 1.25 * max(1 << 30, saved.numel() * 4)
     wide_check(p, dy, n, saved)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("B", [601, 602, 603, 604])
+@pytest.mark.parametrize("D,N,G", [(256, 3, 1), (250, 3, 2), (256, 8, 1), (256, 4, 2), (128, 12, 1), (128, 16, 1), (129, 16, 3), (65, 20, 1), (64, 32, 2),
+                                   (40, 33, 1), (33, 64, 1), (40, 64, 5)])
+def test_single_tokens_of_many_sequences(device, dtype, B, D, N, G):
+    """Batches that give a thread four sequences, with one to four in the last
+    thread: every lane's share of a channel's states."""
+    p, _, state, _ = scan_inputs(B, 1, D, N, G, dtype, device, B + D + N)
+    gate = B % 2 == 0
+    one = {k: v[:, 0] if k in ("u", "dt", "z", "b", "c") else v for k, v in p.items()}
+    if not gate:
+        one["z"] = one["dt_bias"] = one["skip"] = None
+    q = {k: v.cpu().double() if v is not None else None for k, v in one.items()}
+    raw = q["dt"] + (q["dt_bias"] if gate else 0.0)
+    s = torch.logaddexp(raw, torch.zeros_like(raw))[..., None]
+    A = -torch.exp(q["a_log"])
+    wide = lambda v: (v if G == 1 else v.repeat_interleave(D // G, 1)).reshape(B, -1, N)  # noqa: E731
+    own, b, c, u = torch.exp(s * A) * state.cpu().double(), wide(q["b"]), wide(q["c"]), q["u"][..., None]
+    values = []
+    for m in (lambda v: v, lambda v: v.abs()):
+        h = m(own) + m(s * u * b)
+        y = (m(h) * m(c)).sum(-1) + (m(q["skip"] * q["u"]) if gate else 0.0)
+        values.append((y * m(q["z"]) * torch.sigmoid(q["z"]) if gate else y, h))
+    (y, h), (my, mh) = values
+    rel = limits(p, float((s * -A).max()))[0]
+    args = [one[k] for k in ("u", "dt", "a_log", "b", "c")]
+    rest = dict(skip=one["skip"], z=one["z"], dt_bias=one["dt_bias"])
+    other = torch.full_like(state, 7.0)
+    near(ssm.state_scan_step(*args, state, **rest, out_state=other), y, my, rel, "y")
+    near(other, h, mh, rel, "state")
+    moved = state.clone()
+    near(ssm.state_scan_step(*args, moved, **rest), y, my, rel, "y in place")
+    assert torch.equal(moved, other)
+    # as a piece of one token of a padded batch: sequences of no tokens keep their states
+    n = (torch.arange(B, device=device) % 5 != 2).to(torch.int32)
+    p = dict(p, skip=rest["skip"], z=p["z"] if gate else None, dt_bias=rest["dt_bias"])
+    gy, gh, saved = run_scan(p, state=state, lengths=n, want_state=True, save=True)
+    on = n.cpu().bool()
+    near(gy[:, 0].cpu()[on], y[on], my[on], rel, "padded y")
+    near(gh.cpu()[on], h[on], mh[on], rel, "padded state")
+    assert not gy.cpu()[~on].any() and torch.equal(gh.cpu()[~on], state.cpu()[~on]) and torch.equal(saved[:, 0], state)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("B,T,D,N,G", [(1, 530, 12, 33, 1), (1, 545, 16, 64, 1), (2, 400, 24, 64, 3), (1, 450, 9, 36, 3),
+                                       (3, 420, 20, 20, 2), (1, 700, 130, 8, 1), (2, 610, 66, 5, 2)])
+def test_scan_in_pieces_with_many_states_and_groups(device, dtype, B, T, D, N, G):
+    """Outputs, states and gradients of calls that are cut along the tokens,
+    within what rounded decays move (far less than the sizes of the values)."""
+    p, dy, state, _ = scan_inputs(B, T, D, N, G, dtype, device, T + N)
+    p["dt_bias"] -= 1.0
+    for n in (None, torch.tensor([T, 0, T // 3][:B], dtype=torch.int32, device=device)):
+        y, last, saved = run_scan(p, lengths=n, want_state=True, save=True)
+        wide_check(p, dy, n, saved)
+        forward_check(p, None, n, y, last)
+        s = state.clone()
+        y, last, _ = run_scan(p, state=s, lengths=n, out_state=s)
+        forward_check(p, state, n, y, s)
+        if n is not None:
+            gone = torch.arange(T, device=device)[None, :] >= n[:, None]
+            assert not y[gone].any()
+
+
+def forward_check(p, state, n, y, last):
+    """y and the last state against the formula in 64 bits, as wide_check."""
+    B, T, D = y.shape
+    N = p["a_log"].shape[1]
+    q = {k: v.double() for k, v in p.items()}
+    b, c = (v if v.dim() == 4 else v[:, :, None] for v in (q["b"], q["c"]))
+    wide = lambda v: v.repeat_interleave(D // v.shape[1], 1)  # noqa: E731
+    raw = q["dt"] + q["dt_bias"]
+    s, A = torch.logaddexp(raw, torch.zeros_like(raw)), -torch.exp(q["a_log"])
+    h = state.double() if state is not None else torch.zeros(B, D, N, dtype=torch.float64, device=y.device)
+    mh, eh = h.abs(), torch.zeros_like(h)
+    gate = q["z"] * torch.sigmoid(q["z"])
+    rest = 2.0 ** -17 + (24 + N) * 2.0 ** -24
+    ends = n if n is not None else torch.full((B,), T, device=y.device)
+    for t in range(T):
+        on = (t < ends)[:, None]
+        x = s[:, t, :, None] * A
+        own, u, sb = torch.exp(x), q["u"][:, t], (s[:, t] * q["u"][:, t])[..., None] * wide(b[:, t])
+        to = own * h + sb, own * mh + sb.abs(), own * (eh + mh * (2.0 ** -22 - 2.0 ** -21 * x))
+        h, mh = (torch.where(on[..., None], a, v) for a, v in zip(to, (h, mh)))
+        eh = torch.where(on[..., None], to[2] + 2.0 ** -23 * mh, eh)
+        wc = wide(c[:, t])
+        want = ((h * wc).sum(-1) + q["skip"] * u) * gate[:, t] * on
+        mag = ((mh * wc.abs()).sum(-1) + (q["skip"] * u).abs()) * gate[:, t].abs() * on
+        lim = (eh * wc.abs()).sum(-1) * gate[:, t].abs() + rest * mag
+        lim += HALF[y.dtype] * (want.abs() + lim) + 1e-30
+        assert bool(((y[:, t].double() - want).abs() <= lim).all()), t
+    assert bool(((last.double() - h).abs() <= eh + rest * mh + 1e-30).all())
