@@ -974,7 +974,7 @@ class StateSpaceLayer(ModernLayer):
     def _forward(self, x):
         if x.dtype != self.compute_dtype:
             x = x.to(self.compute_dtype)
-        return Fn.StateSpaceFn.apply(x.contiguous(), Fn._ANCHOR, self)
+        return Fn.StateSpaceFn.apply(x.contiguous(), Fn._ANCHOR, self, torch.is_grad_enabled())
 
     def init_state(self, batch: int) -> StateSpaceState:
         """The state before the first token: zeros."""

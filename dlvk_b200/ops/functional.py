@@ -416,18 +416,21 @@ class StateSpaceFn(torch.autograd.Function):
         y = scan(v, low Wdt, b, c, gate xz[:, W:]);  out = y Wout (+ x)
 
     Column slices are read and written in place: the gradients of xz and p are
-    each put together by the kernels that make their parts."""
+    each put together by the kernels that make their parts.  `keep`: a backward
+    pass may follow, which needs the scan's states between spans (of 16 states
+    and bf16 twice a signal's bytes)."""
 
     @staticmethod
-    def forward(ctx, x, anchor, layer):
+    def forward(ctx, x, anchor, layer, keep):
         B, T, _ = x.shape
         x2 = _flat2(x)
         xz, v, low, b, c, dt = layer.project(x2, B, T)[:6]
         y, _, saved = SSM.state_scan_fwd(v, dt, layer.a_log.master, b, c, layer.skip.master, xz[..., layer.width:],
-                                         layer.dt_bias.master, save=True)
+                                         layer.dt_bias.master, save=keep)
         out = K.gemm(_flat2(y), layer.w_out.value, residual=x2 if layer.residual else None)
         ctx.layer, ctx.dims = layer, (B, T)
-        ctx.save_for_backward(x2, xz, v, low, b, c, dt, y, saved)
+        if keep:
+            ctx.save_for_backward(x2, xz, v, low, b, c, dt, y, saved)
         return out.reshape(x.shape)
 
     @staticmethod
@@ -469,4 +472,4 @@ class StateSpaceFn(torch.autograd.Function):
             dx = K.gemm(dxz2, m.w_in.value.t(), residual=g if m.residual else None).reshape(B, T, m.d_model)
         for p in (m.w_out, m.skip, m.a_log, m.dt_bias, m.w_dt, m.w_x, m.conv_bias, m.conv_weight, m.w_in):
             p.grad_ready()
-        return dx, None, None
+        return dx, None, None, None

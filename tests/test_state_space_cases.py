@@ -71,3 +71,36 @@ def test_layer_of_no_sequences_or_tokens(device, B, T, groups):
     assert y.shape == (B, T, 16) and torch.equal(state.conv, start.conv) and torch.equal(state.scan, start.scan)
     if B == 0:
         assert layer.step(x.new_zeros(0, 16), state).shape == (0, 16)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_states_are_kept_for_a_backward_pass_alone(device, monkeypatch):
+    """Where no gradient is wanted the scan keeps no states between spans; outputs
+    are the same bits."""
+    from dlvk_b200.ops import ssm
+
+    kept = []
+    scan = ssm.state_scan_fwd
+
+    def seen(*args, save=False, **kw):
+        got = scan(*args, save=save, **kw)
+        kept.append(got[2] is not None)
+        return got
+
+    monkeypatch.setattr(ssm, "state_scan_fwd", seen)
+    m = Sequential(device, "fp32", seed=2)
+    m.add_embedding(WORDS, 16).add_state_space(16, residual=True).add_dense(16, WORDS).build()
+    x = torch.randint(0, WORDS, (2, 37), generator=torch.Generator().manual_seed(1), dtype=torch.int32).to(device)
+    trained = m.forward(x)
+    m.set_training(False)
+    assert torch.equal(m.forward(x), trained)
+    assert kept == [True, False]
+    with torch.no_grad():
+        layer = dl.StateSpaceLayer(16)
+        layer.to(device, torch.float32)
+        layer.track = False
+        layer.forward(torch.zeros(2, 5, 16, device=device))
+    assert kept == [True, False, False]
+    layer.track = True
+    layer.forward(torch.zeros(2, 5, 16, device=device))
+    assert layer.backward(torch.ones(2, 5, 16, device=device)).shape == (2, 5, 16) and kept[-1]
