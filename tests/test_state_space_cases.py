@@ -5,6 +5,7 @@ import torch
 
 import dlvk_b200 as dl
 from dlvk_b200.models.sequential import Sequential
+from test_state_space_layer import layer_ref
 
 DEVICES = [pytest.param("cpu"), pytest.param("cuda", marks=pytest.mark.gpu)]
 WORDS = 40
@@ -104,3 +105,27 @@ def test_states_are_kept_for_a_backward_pass_alone(device, monkeypatch):
     layer.track = True
     layer.forward(torch.zeros(2, 5, 16, device=device))
     assert layer.backward(torch.ones(2, 5, 16, device=device)).shape == (2, 5, 16) and kept[-1]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("d_model,groups,kw", [(100, 1, {}), (100, 4, {}), (33, 1, dict(d_state=5, d_conv=3)),
+                                               (72, 3, dict(dt_rank=9, d_state=33))])
+def test_bf16_layer_of_odd_columns(d_model, groups, kw):
+    """Columns of dt, b and c that begin at no multiple of four elements.  As in
+    test_state_space_layer: eight roundings of 2^-8 in a row to the output, 24 with
+    the way back, of values whose sums grow errors no more than themselves."""
+    dl.manual_seed(3)
+    layer = dl.StateSpaceLayer(d_model, groups=groups, residual=True, **kw)
+    layer.to("cuda", torch.bfloat16)
+    g = torch.Generator().manual_seed(6)
+    x, dy = (torch.randn(2, 70, d_model, generator=g).bfloat16() for _ in range(2))
+    y = layer.forward(x.cuda())
+    dx = layer.backward(dy.cuda())
+    xr = x.double().requires_grad_(True)
+    ref, p = layer_ref(layer, xr)
+    names = list(p)
+    grads = torch.autograd.grad(ref, [xr] + [p[k] for k in names], dy.double())
+    off = lambda a, b: float((a.detach().cpu().double() - b).norm() / b.norm())  # noqa: E731
+    assert off(y, ref) <= 8 * 2.0 ** -8 and off(dx, grads[0]) <= 24 * 2.0 ** -8
+    for k, r in zip(names, grads[1:]):
+        assert off(getattr(layer, k).grad, r) <= 24 * 2.0 ** -8, k
