@@ -489,7 +489,6 @@ struct StateScan {
   const float* dt_bias = nullptr;   // [D]
   const float* state = nullptr;     // [B, D, N]
   const int32_t* lengths = nullptr;
-  int64_t first = 0;                // tokens before these, which lengths count too
 };
 // out_state [B, D, N] (may be `state`): h after the last token that counts.
 // saved [B, ceil(T / STATE_SCAN_SPAN), D, N]: h before every span's first token, for the backward pass.

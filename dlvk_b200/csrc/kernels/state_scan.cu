@@ -130,8 +130,9 @@ __device__ __forceinline__ void fetch_four(Four<T>* dst, const T* p, const void*
   }
 }
 
-__device__ __forceinline__ int64_t length_of(const StateScan& a, int64_t b) {
-  return a.lengths ? min(max((int64_t)a.lengths[b] - a.first, (int64_t)0), a.T) : a.T;
+// first: tokens before these, which lengths count too
+__device__ __forceinline__ int64_t length_of(const StateScan& a, int64_t b, int64_t first = 0) {
+  return a.lengths ? min(max((int64_t)a.lengths[b] - first, (int64_t)0), a.T) : a.T;
 }
 
 // The channels of a block, CH of one group of one sequence.
@@ -296,11 +297,12 @@ struct Pieces {
   float* steps = nullptr;   // [B][count][D]: sum of s
 };
 
-// Of a backward pass that goes through the tokens part by part, [B][D][N] (may be the
-// same memory): what the part behind passes on (null: zeros), and to the one before.
-struct Carry {
-  const float* in = nullptr;
-  float* out = nullptr;
+// A part of the tokens of a backward pass that goes through them part by part, from the last on.
+struct Part {
+  int64_t first = 0;          // tokens before it, which lengths count too
+  int64_t kept = 0;           // spans of a sequence, of all its tokens, whose states are kept
+  const float* in = nullptr;  // [B][D][N]: what the part behind passes on; null: zeros
+  float* out = nullptr;       // what this one passes on (may be `in`); null: not wanted
 };
 
 template <typename T, int L, bool WIDE>
@@ -322,7 +324,7 @@ struct EndsShared {
 // The end of a piece.  Forward: h[t] = a[t] h[t-1] + s u b[t].  BACK (what
 // reaches the token before the piece): g[t] = c[t] q + a[t+1] g[t+1], times a[t].
 template <typename T, int L, bool WIDE, bool BACK>
-__global__ void __launch_bounds__(THREADS) scan_ends_kernel(StateScan a, SeqRef dy, Pieces pieces) {
+__global__ void __launch_bounds__(THREADS) scan_ends_kernel(StateScan a, SeqRef dy, Pieces pieces, int64_t first) {
   using States = SpanStates<T, L, WIDE, 1>;
   constexpr int CH = THREADS / L;
   extern __shared__ __align__(16) char raw[];
@@ -330,7 +332,7 @@ __global__ void __launch_bounds__(THREADS) scan_ends_kernel(StateScan a, SeqRef 
   const Tile<CH> tile(a);
   const Mine<CH> my(tile.count);
   const Place<L> me;
-  const int64_t n = length_of(a, tile.b), spans = (a.T + SPAN - 1) / SPAN;
+  const int64_t n = length_of(a, tile.b, BACK ? first : 0), spans = (a.T + SPAN - 1) / SPAN;
   const int64_t from = blockIdx.y * pieces.spans;
   const int64_t to = min(min(spans, from + pieces.spans), (n + SPAN - 1) / SPAN);  // spans with a token that counts
   const bool real = me.ch < tile.count;
@@ -410,12 +412,12 @@ __global__ void __launch_bounds__(THREADS) scan_ends_kernel(StateScan a, SeqRef 
 
 // ends: from what a piece ends with to what the one before it (BACK: behind it) passes on to it.
 template <bool BACK>
-__global__ void __launch_bounds__(256) scan_join_kernel(StateScan a, Pieces pieces, Carry pass) {
+__global__ void __launch_bounds__(256) scan_join_kernel(StateScan a, Pieces pieces, Part part) {
   const int64_t dn = (int64_t)a.D * a.N, i = blockIdx.x * 256LL + threadIdx.x;
   if (i >= a.B * dn) return;
   const int64_t b = i / dn, e = i % dn, d = e / a.N;
   const float rate = rate_of(a.a_log[e], 1.f);
-  float carry = BACK ? (pass.in ? pass.in[i] : 0.f) : a.state ? a.state[i] : 0.f;
+  float carry = BACK ? (part.in ? part.in[i] : 0.f) : a.state ? a.state[i] : 0.f;
   // eight pieces' loads ahead of the stores, which might be to the same place for all that the compiler knows
   constexpr int AHEAD = 8;
   for (int j0 = 0; j0 < pieces.count; j0 += AHEAD) {
@@ -435,7 +437,7 @@ __global__ void __launch_bounds__(256) scan_join_kernel(StateScan a, Pieces piec
       carry = fmaf(expf(rate * steps[j]), carry, own[j]);
     }
   }
-  if (BACK && pass.out) pass.out[i] = carry;
+  if (BACK && part.out) part.out[i] = carry;
 }
 
 // ---------------------------------------------------------------- forward
@@ -684,12 +686,13 @@ struct BwdShared {
 // 67% busy; 16 warps an SM.  Sums over channels as tf32 products of ones and the values
 // took longer (some 9 cycles a product of 16 x 8 x 4) and needed two for fp32.
 //
-// saved: `kept` spans a sequence.
+// ALONG: a part of the tokens (pieces.ends has what reaches its last one).  An instance of its own: the
+// registers of the others stay as they are, 358 us and not 380 at 16 x 512 x 2048 with 8 states.
 // part_bc [tiles of a group][B][T][G][2][NS L]; part_d [B][pieces][D][N + 2]: da, dskip, ddt_bias.
-template <typename T, int L, bool WIDE>
-__global__ void __launch_bounds__(THREADS, 4) scan_bwd_kernel(StateScan a, const float* __restrict__ saved, int64_t kept,
-                                                              SeqRef dy, StateScanGrads g, float* __restrict__ part_bc,
-                                                              float* __restrict__ part_d, Pieces pieces, Carry pass) {
+template <typename T, int L, bool WIDE, bool ALONG>
+__global__ void __launch_bounds__(THREADS, 4) scan_bwd_kernel(StateScan a, const float* __restrict__ saved, SeqRef dy,
+                                                              StateScanGrads g, float* __restrict__ part_bc,
+                                                              float* __restrict__ part_d, Pieces pieces, Part part) {
   using States = SpanStates<T, L, WIDE, 2>;
   constexpr int CH = THREADS / L, ROW = 2 * NS * L;
   extern __shared__ __align__(16) char raw[];
@@ -699,15 +702,14 @@ __global__ void __launch_bounds__(THREADS, 4) scan_bwd_kernel(StateScan a, const
   const Place<L> me;
   const int lane = me.lane, warp = threadIdx.x / 32, n0 = me.n0, ch = me.ch;
   const bool real = ch < tile.count;
-  const int64_t n = length_of(a, tile.b), spans = (a.T + SPAN - 1) / SPAN;
+  const int64_t n = length_of(a, tile.b, ALONG ? part.first : 0), spans = (a.T + SPAN - 1) / SPAN;
   Quad rate{}, ga{};
   const int64_t from = blockIdx.y * pieces.spans, end = min(spans, from + pieces.spans);
   const int64_t to = max(from, min(end, (n + SPAN - 1) / SPAN));  // spans with a token that counts
   const int64_t piece = tile.b * pieces.count + blockIdx.y;
   if (real) {
     rate = load_rates(a, tile.c0 + ch, n0, 1.f);
-    const float* in = pieces.ends ? pieces.ends : pass.in;  // (of one piece: passed on as it is)
-    if (in) ga = load_states<WIDE>(in + (piece * a.D + tile.c0 + ch) * a.N + n0, n0, a.N);
+    if (pieces.ends) ga = load_states<WIDE>(pieces.ends + (piece * a.D + tile.c0 + ch) * a.N + n0, n0, a.N);
   }
   for (int j = threadIdx.x; j < CH; j += THREADS) {
     sh.bias[j] = a.dt_bias && j < tile.count ? a.dt_bias[tile.c0 + j] : 0.f;
@@ -729,7 +731,7 @@ __global__ void __launch_bounds__(THREADS, 4) scan_bwd_kernel(StateScan a, const
     }
     States::fetch(st.bc, a.b, a.c, tile.b, tile.group, a.N, t0, n);
     fetch_four<float, WIDE>(reinterpret_cast<Four<float>*>(&st.h[threadIdx.x]),
-                            saved + ((tile.b * kept + k) * a.D + tile.c0 + ch) * a.N + n0, saved, real ? a.N - n0 : 0);
+                            saved + ((tile.b * (ALONG ? part.kept : spans) + k) * a.D + tile.c0 + ch) * a.N + n0, saved, real ? a.N - n0 : 0);
   };
   for (int64_t k = to; k < end; ++k) {  // behind the sequence
     const int64_t t0 = k * SPAN;
@@ -896,7 +898,7 @@ __global__ void __launch_bounds__(THREADS, 4) scan_bwd_kernel(StateScan a, const
     }
     // (the barrier after the next span's elements is between these reads and what comes to their places)
   }
-  if (real && pass.out && !pieces.ends) store_states<WIDE>(ga, pass.out + (piece * a.D + tile.c0 + ch) * a.N + n0, n0, a.N);
+  if (ALONG && real && part.out) store_states<WIDE>(ga, part.out + (piece * a.D + tile.c0 + ch) * a.N + n0, n0, a.N);
   const Quad da = load_quad(&sh.da[threadIdx.x].x);
   if (real) store_states<false>({{mul2(da.v[0], rate.v[0]), mul2(da.v[1], rate.v[1])}},
                          part_d + (piece * a.D + tile.c0 + ch) * (a.N + 2) + n0, n0, a.N);
@@ -1023,22 +1025,22 @@ int64_t pieces_floats(const StateScan& a, const Pieces& p) { return p.count > 1 
 int64_t part_d_floats(const StateScan& a, const Pieces& p) { return a.B * p.count * a.D * (a.N + 2); }
 
 template <typename T, int L, bool W, bool BACK>
-void join_pieces(const StateScan& a, SeqRef dy, Pieces& p, Carry pass, float* scratch, cudaStream_t s) {
-  if (p.count == 1) return;
+void join_pieces(const StateScan& a, SeqRef dy, Pieces& p, const Part& part, float* scratch, cudaStream_t s) {
+  if (p.count == 1) return;  // (what is carried is its end)
   p.ends = scratch;
   p.steps = scratch + a.B * p.count * a.D * a.N;
-  launch(scan_ends_kernel<T, L, W, BACK>, sizeof(EndsShared<T, L, W>), a, p.count, s, dy, p);
-  scan_join_kernel<BACK><<<(unsigned)((a.B * a.D * a.N + 255) / 256), 256, 0, s>>>(a, p, pass);
+  launch(scan_ends_kernel<T, L, W, BACK>, sizeof(EndsShared<T, L, W>), a, p.count, s, dy, p, part.first);
+  scan_join_kernel<BACK><<<(unsigned)((a.B * a.D * a.N + 255) / 256), 256, 0, s>>>(a, p, part);
   DLVK_POST_LAUNCH();
 }
 
 // The sums by tile (part_bc) have a row of 8 L floats a tile and token: at 64 states 32 times
 // bf16 operands, 17 GB for 65536 tokens x 4096 channels.  So a backward pass goes in parts whose
 // sums fit the room of the states that the forward pass kept, or 1 GB.  Of bf16 and 64 states
-// 64 x 512 x 2048 takes 7068 us whole and 7206 in parts of whole sequences (7252 of some spans of all
+// 64 x 512 x 2048 takes 7073 us whole and 7178 in parts of whole sequences (7252 of some spans of all
 // of them; 256 x 128 x 2048 7206, 7228 and 8030).  Parts of fewer blocks than PART_BLOCKS leave SMs
 // without work at their ends: below it they are some spans of all sequences, from the last on
-// (32 x 4096 x 512 7230 whole, 7282 so, 9546 in whole sequences).
+// (32 x 4096 x 512 7240 whole, 7300 so, 9546 in whole sequences).
 struct Parts {
   int64_t sequences, spans;  // of a part
   bool along = false;        // the tokens: what crosses a border is carried
@@ -1076,7 +1078,6 @@ void each_part(const StateScan& a, const Parts& p, F&& f) {
       const int64_t t = k * SPAN;
       v.B = std::min(p.sequences, a.B - b);
       v.T = std::min(p.spans * SPAN, a.T - t);
-      v.first = a.first + t;
       for (SeqRef* r : {&v.u, &v.dt, &v.z, &v.b, &v.c}) *r = from(*r, a.type, b, t);
       if (v.lengths) v.lengths += b;
       f(v, b, k);
@@ -1169,9 +1170,9 @@ void state_scan_bwd(const StateScan& a, const float* saved, SeqRef dy, const Sta
   int64_t rows = 0;
   each_part(a, parts, [&](const StateScan& v, int64_t b, int64_t k) {
     Pieces p = pieces_of(v, BWD_BLOCKS, BWD_PIECES);
-    Carry pass;
-    if (parts.along && k + parts.spans < spans) pass.in = carry;
-    if (parts.along && k > 0) pass.out = carry;
+    Part part{k * SPAN, spans};
+    if (parts.along && k + parts.spans < spans) part.in = p.ends = carry;
+    if (parts.along && k > 0) part.out = carry;
     const auto of = [&](const SeqRef& r) { return from(r, a.type, b, k * SPAN); };
     StateScanGrads h = g;
     for (SeqRef* r : {&h.du, &h.ddt, &h.dz, &h.db, &h.dc}) *r = of(*r);
@@ -1183,9 +1184,10 @@ void state_scan_bwd(const StateScan& a, const float* saved, SeqRef dy, const Sta
       using T = decltype(type);
       constexpr int L = decltype(lanes)::value;
       constexpr bool W = decltype(wide)::value;
-      join_pieces<T, L, W, true>(v, go, p, pass, ends, s);
-      launch(scan_bwd_kernel<T, L, W>, sizeof(BwdShared<T, L, W>), v, p.count, s, kept, spans, go, h, part_bc,
-             part_d + rows * a.D * (a.N + 2), p, pass);
+      join_pieces<T, L, W, true>(v, go, p, part, ends, s);
+      if (p.count > 1) part.out = nullptr;  // joining the pieces has passed it on
+      launch(parts.along ? scan_bwd_kernel<T, L, W, true> : scan_bwd_kernel<T, L, W, false>, sizeof(BwdShared<T, L, W>), v,
+             p.count, s, kept, go, h, part_bc, part_d + rows * a.D * (a.N + 2), p, part);
     });
     join_bc(v, part_bc, h, s);
     rows += v.B * p.count;
