@@ -1010,7 +1010,10 @@ int64_t part_bc_floats(const StateScan& a) { return (int64_t)tiles_of(a) * a.B *
 // proper, so few pieces are worse than one: forward, 3 x 1024 x 2048, five take 99 us and one 106,
 // but of 4 x 1024 four take 122; backward, three of the former take 210 and one 277, two of the
 // latter 300.
-constexpr int FWD_BLOCKS = 7, BWD_BLOCKS = 4;  // that an SM has room for
+// These times, and the blocks that an SM is taken to have room for, are those of 9 to 16 states.  By
+// shared memory fp32 has room for 5 (forward) at 8 states or fewer and past 32, for 2 or 3 (backward)
+// there and at 17 to 32, bf16 for 3 (backward) there: pieces of such calls may take two rounds.
+constexpr int FWD_BLOCKS = 7, BWD_BLOCKS = 4;
 constexpr int FWD_PIECES = 5, BWD_PIECES = 3, PIECE_SPANS = 4;
 Pieces pieces_of(const StateScan& a, int blocks_an_sm, int least) {
   Pieces p;
